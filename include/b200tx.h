@@ -405,6 +405,116 @@ int b200tx_residual_layer_norm_peer_rs(const float* residual_in, const void* con
  * in b200tx_device_error. */
 int b200tx_peer_wait(const uint32_t* flags, int count, int self, uint32_t epoch, cudaStream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Decoding: what a model needs to go on token by token from a prompt.  The
+ * reference runs whole sequences only; these have no counterpart in it.
+ *   norm and rotation of queries and keys, fused with the append to
+ *   a paged 8-bit key/value cache, attention over that cache, and
+ *   linear layers with 4-bit weights for a few rows.
+ * ------------------------------------------------------------------------ */
+
+/* Rotation tables: cos and sin F32 [positions, rotary / 2]; the first `rotary`
+ * dims of a head are turned, pairs (i, i + rotary / 2), or (2i, 2i + 1) when
+ * interleaved.  rotary: a multiple of 8 (16 for head_dim 256) up to head_dim.
+ * A position outside the table gives NaN heads. */
+typedef struct b200tx_rope {
+  const float* cos;
+  const float* sin;
+  int64_t positions;
+  int64_t rotary;
+  int interleaved;
+} b200tx_rope;
+
+/*
+ * RMS norm of each query and key head (x / sqrt(mean(x^2) + eps) * weight; a NULL
+ * weight: none) and the rotation (rope NULL: none), over the packed projection
+ * [batch, tokens, (heads + 2 kv_heads) * head_dim]: query, key, value heads.
+ * Value heads are copied; out may be qkv (in place).  dtype F32 or BF16 for both; pointers
+ * 16-byte aligned, strides in elements, multiples of 8; head_dim 8..256, a power
+ * of two.  positions: int32 (or int64 with positions_64), element
+ * [b * position_batch_stride + t], or NULL = t.
+ */
+int b200tx_qk_norm_rope(const void* qkv, void* out, int dtype, int64_t batch, int64_t tokens, int64_t heads,
+                        int64_t kv_heads, int64_t head_dim, int64_t in_batch_stride, int64_t in_token_stride,
+                        int64_t out_batch_stride, int64_t out_token_stride, const float* q_weight,
+                        const float* k_weight, float eps, const b200tx_rope* rope, const void* positions,
+                        int positions_64, int64_t position_batch_stride, cudaStream_t stream);
+
+/* A paged key/value cache in 8 bits.  Tokens lie in blocks of 64; page
+ * page_table[slot][block] holds a full block of a sequence as codes (value =
+ * (code - 128) * scale, one scale per kv head for keys and one for values); the
+ * open block is BF16 in tail[slot][block & 1].  lengths[slot] = tokens held
+ * before the call at hand; head_dim 32, 64, 128 or 256.  The kernels check
+ * slots, pages and lengths: what is out of range is not stored, and what is read
+ * from there is NaN. */
+#define B200TX_KV8_BLOCK 64
+
+typedef struct b200tx_kv8_cache {
+  void* codes;               /* uint8 [pages, 2, kv_heads, 64, head_dim] (keys, values), 16-byte aligned */
+  float* scales;             /* [pages, 2, kv_heads] */
+  void* tail;                /* BF16 [slots, 2, 2, kv_heads, 64, head_dim], 16-byte aligned */
+  const int32_t* page_table; /* [slots, max_blocks] */
+  const int32_t* lengths;    /* [slots] */
+  int64_t pages;
+  int64_t slots;
+  int64_t max_blocks;
+  int64_t kv_heads;
+  int64_t head_dim;
+} b200tx_kv8_cache;
+
+/*
+ * Appends `tokens` new tokens (counts[b] of them where counts is given) of each
+ * of `batch` sequences (slot slot_ids[b], or b): keys normed and rotated at
+ * their position lengths[slot] + t as b200tx_qk_norm_rope does, keys and values
+ * rounded to BF16 and stored; blocks that fill are quantised.  q_out BF16
+ * [batch, tokens, heads, head_dim]: the queries, normed and rotated.  qkv
+ * [batch, tokens, (heads + 2 kv_heads) * head_dim] in dtype, strides in
+ * elements.  lengths is not changed: the caller advances it when every layer
+ * has run, by any number up to `tokens` when that is at most 64 (tokens past it
+ * are then forgotten), else by all of them.
+ */
+int b200tx_kv8_append(const b200tx_kv8_cache* cache, const void* qkv, int dtype, void* q_out, int64_t batch,
+                      int64_t tokens, int64_t heads, int64_t batch_stride, int64_t token_stride,
+                      const int32_t* slot_ids, const int32_t* counts, const float* q_weight, const float* k_weight,
+                      float eps, const b200tx_rope* rope, cudaStream_t stream);
+
+/* The first `most` tokens of each sequence as BF16 values, k_out and v_out
+ * [batch, most, kv_heads, head_dim]; zero past lengths[slot] + counts[b]
+ * (tokens where counts is NULL). */
+int b200tx_kv8_gather(const b200tx_kv8_cache* cache, void* k_out, void* v_out, int64_t batch, int64_t most,
+                      int64_t tokens, const int32_t* slot_ids, const int32_t* counts, cudaStream_t stream);
+
+/* Bytes of workspace that b200tx_kv8_attention needs on the current device. */
+int b200tx_kv8_workspace_bytes(int64_t head_dim, int64_t* bytes_out);
+
+/*
+ * Attention of the `tokens` tokens appended last (query t at position
+ * lengths[slot] + t sees the keys up to there) over the cache: softmax(scale q k) v per
+ * head, heads / kv_heads query heads to a kv head.  q BF16 [batch, tokens, heads,
+ * head_dim] (heads dense, strides in elements), out BF16 dense.  Rows past
+ * counts[b] are zero.  workspace: 16-byte aligned, zeroed once before its first
+ * use, for one stream at a time; the kernel leaves its counters zero.
+ */
+int b200tx_kv8_attention(const b200tx_kv8_cache* cache, const void* q, void* out, int64_t batch, int64_t tokens,
+                         int64_t heads, int64_t q_batch_stride, int64_t q_token_stride, const int32_t* slot_ids,
+                         const int32_t* counts, float scale, void* workspace, int64_t workspace_bytes,
+                         cudaStream_t stream);
+
+/*
+ * out[M, N] = epilogue(x[M, K] . W^T + bias), W[n, k] = scales[k / group, n] *
+ * (code[n, k] - 8) with 4-bit codes, for a few rows (the weights are read once
+ * for each 32).  x BF16, rows x_stride elements apart (a multiple of 8); scales
+ * BF16 [Kp / group, N], Kp = K rounded up to 128; bias F32 or NULL; out F32 or
+ * BF16; group 32, 64 or 128; K a multiple of 8; epilogue B200TX_EPI_*.
+ * packed [N, Kp / 2] uint8, 16-byte aligned, codes past K any, x counts as 0 there: the
+ * 128 codes of a run are 16 little-endian 32-bit words of 8 consecutive weights, nibble i of a
+ * word (from the lowest) holding weight {0,2,4,6,1,3,5,7}[i]; word 4 a + b is
+ * stored at 4 b + a.
+ */
+int b200tx_linear_w4(const void* x, int64_t x_stride, const void* packed, const void* scales, const float* bias,
+                     void* out, int out_dtype, int64_t M, int64_t N, int64_t K, int64_t group, int epilogue,
+                     cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -26,7 +26,11 @@
 #include "gemm_kernels.cuh"
 #include "gemm_rownorm_kernels.cuh"
 #include "gemm_warp_kernels.cuh"
+#include "kv8_attention_kernels.cuh"
+#include "kv8_cache_kernels.cuh"
+#include "linear_w4_kernels.cuh"
 #include "norm_kernels.cuh"
+#include "rope_kernels.cuh"
 #include "seq_forward_kernels.cuh"
 #include "sm100_common.cuh"
 
@@ -78,6 +82,7 @@ struct DeviceState {
   bool attn_attr[2 * kAttnVariants] = {};  // unmasked builds by variant, then the masked builds
   bool rownorm_attr[4] = {};               // GEMM + residual LayerNorm builds by (in, out) dtype
   int rownorm_clusters[4][5] = {};         // their co-resident clusters by CTA pairs per cluster
+  bool kv8_attr[4] = {};                   // 8-bit cache attention builds by head_dim
   bool seq_forward_attr = false;           // whole-forward kernel's shared-memory size set
   uint8_t* seq_noalloc_images = nullptr;   // device address of g_seq_noalloc_images on this device
 };
@@ -1461,3 +1466,5 @@ int b200tx_attention(const void* qkv, void* out, int64_t batch, int64_t seq, int
 }
 
 }  // extern "C"
+
+#include "decode_api.cuh"

@@ -1,0 +1,414 @@
+// decode_api.cuh -- argument checks and launches of the decoding operators:
+// norm and rotation of queries and keys, the 8-bit key/value cache, and 4-bit
+// linear layers.  Part of b200tx.cu's translation unit.
+#pragma once
+
+namespace {
+
+// Head groups of one warp when a token's heads are dealt to `splits` warps:
+// with few tokens each warp takes one round of loads, so that a step is as
+// short as it can be; with enough tokens to fill the SMs a warp takes the whole
+// token and loads its angles once.
+void split_heads(int64_t tokens, int groups, int sm_count, int* splits, int* span) {
+  const int64_t wanted = static_cast<int64_t>(sm_count) * b200tx::kRopeWarps * 4;
+  const int rounds = (groups + b200tx::kRopeUnroll - 1) / b200tx::kRopeUnroll;
+  int64_t s = (wanted + tokens - 1) / tokens;
+  if (s > rounds) s = rounds;
+  if (s < 1) s = 1;
+  const int per = static_cast<int>((rounds + s - 1) / s);
+  *span = per * b200tx::kRopeUnroll;
+  *splits = (rounds + per - 1) / per;
+}
+
+int rope_table(const char* what, const b200tx_rope* rope, int64_t head_dim, b200tx::RopeTable* out) {
+  *out = b200tx::RopeTable{};
+  if (rope == nullptr) return B200TX_OK;
+  if (rope->cos == nullptr || rope->sin == nullptr || rope->positions <= 0 || rope->positions > 0x7fffffffLL)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "%s: bad rotation table", what);
+  const int64_t step = head_dim == 256 ? 16 : 8;
+  if (rope->rotary <= 0 || rope->rotary > head_dim || rope->rotary % step != 0)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "%s: rotary %lld is not a multiple of %lld up to head_dim %lld", what,
+                (long long)rope->rotary, (long long)step, (long long)head_dim);
+  out->cos = rope->cos;
+  out->sin = rope->sin;
+  out->positions = static_cast<int>(rope->positions);
+  out->rotary = static_cast<int>(rope->rotary);
+  out->interleaved = rope->interleaved != 0;
+  return B200TX_OK;
+}
+
+int heads_shape(const char* what, int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads) {
+  if (batch <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || batch > (1 << 20) || tokens > (1 << 26) ||
+      heads > (1 << 14) || kv_heads > heads)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "%s: bad shape batch %lld tokens %lld heads %lld kv_heads %lld", what,
+                (long long)batch, (long long)tokens, (long long)heads, (long long)kv_heads);
+  return B200TX_OK;
+}
+
+int kv8_view(const char* what, const b200tx_kv8_cache* c, b200tx::Kv8Cache* out) {
+  if (c == nullptr || c->codes == nullptr || c->scales == nullptr || c->tail == nullptr || c->page_table == nullptr ||
+      c->lengths == nullptr)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "%s: null cache pointer", what);
+  if (c->head_dim != 32 && c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+    return fail(B200TX_ERR_UNSUPPORTED, "%s: head_dim %lld (32, 64, 128 and 256 are built)", what,
+                (long long)c->head_dim);
+  if (c->pages <= 0 || c->pages > 0x7fffffffLL || c->slots <= 0 || c->slots > (1 << 20) || c->max_blocks <= 0 ||
+      c->max_blocks > 0x7fffffffLL / b200tx::kKv8Block || c->kv_heads <= 0 || c->kv_heads > (1 << 14))
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "%s: bad cache shape", what);
+  if (!aligned16(c->codes) || !aligned16(c->tail))
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "%s: the cache's codes and tail must be 16-byte aligned", what);
+  out->codes = static_cast<uint8_t*>(c->codes);
+  out->scales = c->scales;
+  out->tail = static_cast<__nv_bfloat16*>(c->tail);
+  out->page_table = c->page_table;
+  out->lengths = c->lengths;
+  out->pages = c->pages;
+  out->slots = static_cast<int>(c->slots);
+  out->max_blocks = static_cast<int>(c->max_blocks);
+  out->kv_heads = static_cast<int>(c->kv_heads);
+  return B200TX_OK;
+}
+
+template <int D, typename T>
+cudaError_t launch_rope(b200tx::RopeArgs& a, int sm_count, cudaStream_t stream) {
+  const int heads = a.heads + (a.copy_values ? 2 : 1) * a.kv_heads;
+  constexpr int HEADS = b200tx::HeadLanes<D>::HEADS;
+  split_heads(a.total_tokens, (heads + HEADS - 1) / HEADS, sm_count, &a.splits, &a.span);
+  const int64_t units = a.total_tokens * a.splits;
+  return launch(b200tx::qk_norm_rope_kernel<D, T>,
+                dim3(static_cast<unsigned>((units + b200tx::kRopeWarps - 1) / b200tx::kRopeWarps)),
+                dim3(b200tx::kRopeWarps * 32), 0, stream, a);
+}
+
+template <typename T>
+cudaError_t launch_rope_dim(int64_t head_dim, b200tx::RopeArgs& a, int sm_count, cudaStream_t stream) {
+  switch (head_dim) {
+    case 8: return launch_rope<8, T>(a, sm_count, stream);
+    case 16: return launch_rope<16, T>(a, sm_count, stream);
+    case 32: return launch_rope<32, T>(a, sm_count, stream);
+    case 64: return launch_rope<64, T>(a, sm_count, stream);
+    case 128: return launch_rope<128, T>(a, sm_count, stream);
+    default: return launch_rope<256, T>(a, sm_count, stream);
+  }
+}
+
+template <int D, typename T>
+cudaError_t launch_kv8_append(b200tx::Kv8AppendArgs& a, int sm_count, cudaStream_t stream) {
+  constexpr int HEADS = b200tx::HeadLanes<D>::HEADS;
+  const int64_t tokens = static_cast<int64_t>(a.batch) * a.tokens;
+  split_heads(tokens, (a.heads + HEADS - 1) / HEADS, sm_count, &a.splits, &a.span);
+  const int64_t q_ctas = (tokens * a.splits + b200tx::kKv8AppendWarps - 1) / b200tx::kKv8AppendWarps;
+  return launch(b200tx::kv8_append_kernel<D, T>, dim3(static_cast<unsigned>(a.kv_ctas + q_ctas)),
+                dim3(b200tx::kKv8AppendWarps * 32), 0, stream, a);
+}
+
+template <typename T>
+cudaError_t launch_kv8_append_dim(int64_t head_dim, b200tx::Kv8AppendArgs& a, int sm_count, cudaStream_t stream) {
+  switch (head_dim) {
+    case 32: return launch_kv8_append<32, T>(a, sm_count, stream);
+    case 64: return launch_kv8_append<64, T>(a, sm_count, stream);
+    case 128: return launch_kv8_append<128, T>(a, sm_count, stream);
+    default: return launch_kv8_append<256, T>(a, sm_count, stream);
+  }
+}
+
+template <int D>
+cudaError_t launch_kv8_gather(const b200tx::Kv8GatherArgs& a, cudaStream_t stream) {
+  const int64_t threads = static_cast<int64_t>(a.batch) * a.most * a.cache.kv_heads * (D / 8);
+  return launch(b200tx::kv8_gather_kernel<D>, dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, stream, a);
+}
+
+// The workspace of the attention: arrival counters, then the parts of tiles
+// that lie in two or more CTAs.
+constexpr int64_t kKv8ArrivalBytes = 8192;
+
+template <int D>
+int kv8_attention_grid(int sm_count) {
+  using S = b200tx::Kv8Shape<D>;
+  // a tile's parts have their (max, sum) rows in shared memory when they are joined
+  const int most = S::MAIN / (b200tx::kKv8Rows * 8);
+  const int grid = sm_count * S::CTAS;
+  return grid < most ? grid : most;
+}
+
+template <int D>
+int64_t kv8_workspace(int sm_count) {
+  return kKv8ArrivalBytes + static_cast<int64_t>(kv8_attention_grid<D>(sm_count)) * 2 * b200tx::Kv8Shape<D>::PART_FLOATS * 4;
+}
+
+template <int D>
+cudaError_t launch_kv8_attention(const b200tx::Kv8AttnArgs& a, DeviceState* dev, int index, cudaStream_t stream) {
+  constexpr int smem = b200tx::Kv8Shape<D>::MAIN;
+  if (!dev->kv8_attr[index]) {
+    cudaError_t err = cudaFuncSetAttribute(b200tx::kv8_attention_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (err != cudaSuccess) return err;
+    dev->kv8_attr[index] = true;
+  }
+  return launch(b200tx::kv8_attention_kernel<D>, dim3(static_cast<unsigned>(kv8_attention_grid<D>(dev->sm_count))),
+                dim3(b200tx::kKv8Warps * 32), smem, stream, a);
+}
+
+template <int TN, int GROUP>
+cudaError_t launch_w4(b200tx::W4Args& a, int out_dtype, int sm_count, cudaStream_t stream) {
+  // Warps of a CTA along K: the fewest (they are joined at the end) that leave
+  // two CTAs for each SM.
+  const int tiles = (a.outer + 15) / 16;
+  a.split = 1;
+  while (a.split < b200tx::kW4Warps && a.split < a.runs &&
+         (tiles * a.split + b200tx::kW4Warps - 1) / b200tx::kW4Warps < 2 * sm_count)
+    a.split *= 2;
+  const int per = b200tx::kW4Warps / a.split;
+  const dim3 grid(static_cast<unsigned>((tiles + per - 1) / per), static_cast<unsigned>((a.rows + TN * 8 - 1) / (TN * 8)));
+  if (out_dtype == B200TX_F32)
+    return launch(b200tx::linear_w4_kernel<TN, GROUP, float>, grid, dim3(b200tx::kW4Warps * 32), 0, stream, a);
+  return launch(b200tx::linear_w4_kernel<TN, GROUP, __nv_bfloat16>, grid, dim3(b200tx::kW4Warps * 32), 0, stream, a);
+}
+
+template <int TN>
+cudaError_t launch_w4_group(int64_t group, b200tx::W4Args& a, int out_dtype, int sm_count, cudaStream_t stream) {
+  switch (group) {
+    case 32: return launch_w4<TN, 32>(a, out_dtype, sm_count, stream);
+    case 64: return launch_w4<TN, 64>(a, out_dtype, sm_count, stream);
+    default: return launch_w4<TN, 128>(a, out_dtype, sm_count, stream);
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int b200tx_qk_norm_rope(const void* qkv, void* out, int dtype, int64_t batch, int64_t tokens, int64_t heads,
+                        int64_t kv_heads, int64_t head_dim, int64_t in_batch_stride, int64_t in_token_stride,
+                        int64_t out_batch_stride, int64_t out_token_stride, const float* q_weight,
+                        const float* k_weight, float eps, const b200tx_rope* rope, const void* positions,
+                        int positions_64, int64_t position_batch_stride, cudaStream_t stream) {
+  if (qkv == nullptr || out == nullptr)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "qk_norm_rope: null tensor pointer");
+  int rc = heads_shape("qk_norm_rope", batch, tokens, heads, kv_heads);
+  if (rc != B200TX_OK) return rc;
+  if (head_dim < 8 || head_dim > 256 || (head_dim & (head_dim - 1)) != 0)
+    return fail(B200TX_ERR_UNSUPPORTED, "qk_norm_rope: head_dim %lld (8, 16, 32, 64, 128 and 256 are built)",
+                (long long)head_dim);
+  if (dtype != B200TX_F32 && dtype != B200TX_BF16)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "qk_norm_rope: dtype %d", dtype);
+  if (!aligned16(qkv) || !aligned16(out) || (in_batch_stride | in_token_stride | out_batch_stride | out_token_stride) % 8 != 0)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "qk_norm_rope: pointers must be 16-byte aligned, strides multiples of 8");
+  if ((q_weight != nullptr && !aligned16(q_weight)) || (k_weight != nullptr && !aligned16(k_weight)))
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "qk_norm_rope: the norm weights must be 16-byte aligned");
+  b200tx::RopeArgs a{};
+  rc = rope_table("qk_norm_rope", rope, head_dim, &a.norm.rope);
+  if (rc != B200TX_OK) return rc;
+  DeviceState* dev = nullptr;
+  rc = current_device(&dev);
+  if (rc != B200TX_OK) return rc;
+  a.in = qkv;
+  a.out = out;
+  a.in_batch_stride = in_batch_stride;
+  a.in_token_stride = in_token_stride;
+  a.out_batch_stride = out_batch_stride;
+  a.out_token_stride = out_token_stride;
+  a.positions = positions;
+  a.positions_64 = positions_64;
+  a.position_batch_stride = position_batch_stride;
+  a.tokens = static_cast<int>(tokens);
+  a.heads = static_cast<int>(heads);
+  a.kv_heads = static_cast<int>(kv_heads);
+  a.copy_values = out != qkv;
+  a.total_tokens = batch * tokens;
+  a.norm.q_weight = q_weight;
+  a.norm.k_weight = k_weight;
+  a.norm.eps = eps;
+  if (a.total_tokens > 0x7fffffffLL / 64)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "qk_norm_rope: too many tokens");
+  cudaError_t err = dtype == B200TX_F32 ? launch_rope_dim<float>(head_dim, a, dev->sm_count, stream)
+                                        : launch_rope_dim<__nv_bfloat16>(head_dim, a, dev->sm_count, stream);
+  return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "qk_norm_rope");
+}
+
+int b200tx_kv8_append(const b200tx_kv8_cache* cache, const void* qkv, int dtype, void* q_out, int64_t batch,
+                      int64_t tokens, int64_t heads, int64_t batch_stride, int64_t token_stride,
+                      const int32_t* slot_ids, const int32_t* counts, const float* q_weight, const float* k_weight,
+                      float eps, const b200tx_rope* rope, cudaStream_t stream) {
+  b200tx::Kv8AppendArgs a{};
+  int rc = kv8_view("kv8_append", cache, &a.cache);
+  if (rc != B200TX_OK) return rc;
+  if (qkv == nullptr || q_out == nullptr) return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_append: null tensor pointer");
+  rc = heads_shape("kv8_append", batch, tokens, heads, cache->kv_heads);
+  if (rc != B200TX_OK) return rc;
+  if (dtype != B200TX_F32 && dtype != B200TX_BF16)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_append: dtype %d", dtype);
+  if (!aligned16(qkv) || !aligned16(q_out) || (batch_stride | token_stride) % 8 != 0)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_append: pointers must be 16-byte aligned, strides multiples of 8");
+  if ((q_weight != nullptr && !aligned16(q_weight)) || (k_weight != nullptr && !aligned16(k_weight)))
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_append: the norm weights must be 16-byte aligned");
+  if (slot_ids == nullptr && batch > cache->slots)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_append: batch %lld in a cache of %lld slots", (long long)batch,
+                (long long)cache->slots);
+  rc = rope_table("kv8_append", rope, cache->head_dim, &a.norm.rope);
+  if (rc != B200TX_OK) return rc;
+  DeviceState* dev = nullptr;
+  rc = current_device(&dev);
+  if (rc != B200TX_OK) return rc;
+  a.qkv = qkv;
+  a.q_out = static_cast<__nv_bfloat16*>(q_out);
+  a.batch_stride = batch_stride;
+  a.token_stride = token_stride;
+  a.slot_ids = slot_ids;
+  a.counts = counts;
+  a.batch = static_cast<int>(batch);
+  a.tokens = static_cast<int>(tokens);
+  a.heads = static_cast<int>(heads);
+  a.block_span = static_cast<int>((tokens + b200tx::kKv8Block - 2) / b200tx::kKv8Block + 1);
+  a.kv_ctas = batch * cache->kv_heads * a.block_span;
+  a.norm.q_weight = q_weight;
+  a.norm.k_weight = k_weight;
+  a.norm.eps = eps;
+  if (batch * tokens > 0x7fffffffLL / 64 || a.kv_ctas > 0x3fffffffLL)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_append: too many tokens");
+  cudaError_t err = dtype == B200TX_F32 ? launch_kv8_append_dim<float>(cache->head_dim, a, dev->sm_count, stream)
+                                        : launch_kv8_append_dim<__nv_bfloat16>(cache->head_dim, a, dev->sm_count, stream);
+  return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "kv8_append");
+}
+
+int b200tx_kv8_gather(const b200tx_kv8_cache* cache, void* k_out, void* v_out, int64_t batch, int64_t most,
+                      int64_t tokens, const int32_t* slot_ids, const int32_t* counts, cudaStream_t stream) {
+  b200tx::Kv8GatherArgs a{};
+  int rc = kv8_view("kv8_gather", cache, &a.cache);
+  if (rc != B200TX_OK) return rc;
+  if (k_out == nullptr || v_out == nullptr || !aligned16(k_out) || !aligned16(v_out))
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_gather: outputs must be 16-byte aligned");
+  if (batch <= 0 || batch > (1 << 20) || most <= 0 || most > 0x7fffffffLL || tokens < 0 || tokens > (1 << 26))
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_gather: bad shape batch %lld tokens %lld", (long long)batch,
+                (long long)most);
+  if (slot_ids == nullptr && batch > cache->slots)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_gather: batch %lld in a cache of %lld slots", (long long)batch,
+                (long long)cache->slots);
+  if (static_cast<double>(batch) * most * cache->kv_heads * (cache->head_dim / 8) > 256.0 * 0x7fffffff)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_gather: too many values");
+  DeviceState* dev = nullptr;
+  rc = current_device(&dev);
+  if (rc != B200TX_OK) return rc;
+  a.slot_ids = slot_ids;
+  a.counts = counts;
+  a.tokens = static_cast<int>(tokens);
+  a.batch = static_cast<int>(batch);
+  a.most = static_cast<int>(most);
+  a.k = static_cast<__nv_bfloat16*>(k_out);
+  a.v = static_cast<__nv_bfloat16*>(v_out);
+  cudaError_t err;
+  switch (cache->head_dim) {
+    case 32: err = launch_kv8_gather<32>(a, stream); break;
+    case 64: err = launch_kv8_gather<64>(a, stream); break;
+    case 128: err = launch_kv8_gather<128>(a, stream); break;
+    default: err = launch_kv8_gather<256>(a, stream); break;
+  }
+  return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "kv8_gather");
+}
+
+int b200tx_kv8_workspace_bytes(int64_t head_dim, int64_t* bytes_out) {
+  if (bytes_out == nullptr) return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_workspace_bytes: null result");
+  DeviceState* dev = nullptr;
+  int rc = current_device(&dev);
+  if (rc != B200TX_OK) return rc;
+  switch (head_dim) {
+    case 32: *bytes_out = kv8_workspace<32>(dev->sm_count); return B200TX_OK;
+    case 64: *bytes_out = kv8_workspace<64>(dev->sm_count); return B200TX_OK;
+    case 128: *bytes_out = kv8_workspace<128>(dev->sm_count); return B200TX_OK;
+    case 256: *bytes_out = kv8_workspace<256>(dev->sm_count); return B200TX_OK;
+    default: return fail(B200TX_ERR_UNSUPPORTED, "kv8_workspace_bytes: head_dim %lld", (long long)head_dim);
+  }
+}
+
+int b200tx_kv8_attention(const b200tx_kv8_cache* cache, const void* q, void* out, int64_t batch, int64_t tokens,
+                         int64_t heads, int64_t q_batch_stride, int64_t q_token_stride, const int32_t* slot_ids,
+                         const int32_t* counts, float scale, void* workspace, int64_t workspace_bytes,
+                         cudaStream_t stream) {
+  b200tx::Kv8AttnArgs a{};
+  int rc = kv8_view("kv8_attention", cache, &a.cache);
+  if (rc != B200TX_OK) return rc;
+  if (q == nullptr || out == nullptr || workspace == nullptr)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_attention: null tensor pointer");
+  rc = heads_shape("kv8_attention", batch, tokens, heads, cache->kv_heads);
+  if (rc != B200TX_OK) return rc;
+  if (heads % cache->kv_heads != 0)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_attention: %lld heads do not share %lld kv heads evenly",
+                (long long)heads, (long long)cache->kv_heads);
+  if (tokens * heads > (1 << 26)) return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_attention: too many query rows");
+  if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || (q_batch_stride | q_token_stride) % 8 != 0)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_attention: pointers must be 16-byte aligned, strides multiples of 8");
+  if (!(scale > 0.f) || scale > 1e30f) return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_attention: scale must be positive");
+  if (slot_ids == nullptr && batch > cache->slots)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_attention: batch %lld in a cache of %lld slots", (long long)batch,
+                (long long)cache->slots);
+  DeviceState* dev = nullptr;
+  rc = current_device(&dev);
+  if (rc != B200TX_OK) return rc;
+  int64_t need = 0;
+  rc = b200tx_kv8_workspace_bytes(cache->head_dim, &need);
+  if (rc != B200TX_OK) return rc;
+  if (workspace_bytes < need)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_attention: workspace of %lld bytes, %lld needed",
+                (long long)workspace_bytes, (long long)need);
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.q_batch_stride = q_batch_stride;
+  a.q_token_stride = q_token_stride;
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.slot_ids = slot_ids;
+  a.counts = counts;
+  a.batch = static_cast<int>(batch);
+  a.tokens = static_cast<int>(tokens);
+  a.heads = static_cast<int>(heads);
+  a.group = static_cast<int>(heads / cache->kv_heads);
+  a.row_tiles = static_cast<int>((tokens * a.group + b200tx::kKv8Rows - 1) / b200tx::kKv8Rows);
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.arrivals = static_cast<unsigned int*>(workspace);
+  a.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kKv8ArrivalBytes);
+  cudaError_t err;
+  switch (cache->head_dim) {
+    case 32: err = launch_kv8_attention<32>(a, dev, 0, stream); break;
+    case 64: err = launch_kv8_attention<64>(a, dev, 1, stream); break;
+    case 128: err = launch_kv8_attention<128>(a, dev, 2, stream); break;
+    default: err = launch_kv8_attention<256>(a, dev, 3, stream); break;
+  }
+  return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "kv8_attention");
+}
+
+int b200tx_linear_w4(const void* x, int64_t x_stride, const void* packed, const void* scales, const float* bias,
+                     void* out, int out_dtype, int64_t M, int64_t N, int64_t K, int64_t group, int epilogue,
+                     cudaStream_t stream) {
+  if (x == nullptr || packed == nullptr || scales == nullptr || out == nullptr)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "linear_w4: null tensor pointer");
+  if (M <= 0 || N <= 0 || K <= 0 || M > (1 << 20) || N > (1 << 24) || K > (1 << 24) || K % 8 != 0)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "linear_w4: bad shape M %lld N %lld K %lld (K a multiple of 8)",
+                (long long)M, (long long)N, (long long)K);
+  if (group != 32 && group != 64 && group != 128)
+    return fail(B200TX_ERR_UNSUPPORTED, "linear_w4: group %lld (32, 64 and 128 are built)", (long long)group);
+  if (out_dtype != B200TX_F32 && out_dtype != B200TX_BF16)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "linear_w4: out_dtype %d", out_dtype);
+  if (epilogue != B200TX_EPI_BIAS && epilogue != B200TX_EPI_BIAS_GELU)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "linear_w4: epilogue %d", epilogue);
+  if (!aligned16(x) || !aligned16(packed) || x_stride % 8 != 0)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "linear_w4: x and packed must be 16-byte aligned, x_stride a multiple of 8");
+  DeviceState* dev = nullptr;
+  int rc = current_device(&dev);
+  if (rc != B200TX_OK) return rc;
+  b200tx::W4Args a{};
+  a.x = static_cast<const __nv_bfloat16*>(x);
+  a.packed = static_cast<const uint8_t*>(packed);
+  a.scales = static_cast<const __nv_bfloat16*>(scales);
+  a.bias = bias;
+  a.out = out;
+  a.x_stride = x_stride;
+  a.rows = static_cast<int>(M);
+  a.outer = static_cast<int>(N);
+  a.inner = static_cast<int>(K);
+  a.runs = static_cast<int>((K + b200tx::kW4Run - 1) / b200tx::kW4Run);
+  a.gelu = epilogue == B200TX_EPI_BIAS_GELU;
+  // rows of x by eights: 1, 2 or 4 MMA columns; past 32 the weights are read again
+  cudaError_t err = M <= 8    ? launch_w4_group<1>(group, a, out_dtype, dev->sm_count, stream)
+                    : M <= 16 ? launch_w4_group<2>(group, a, out_dtype, dev->sm_count, stream)
+                              : launch_w4_group<4>(group, a, out_dtype, dev->sm_count, stream);
+  return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "linear_w4");
+}
+
+}  // extern "C"

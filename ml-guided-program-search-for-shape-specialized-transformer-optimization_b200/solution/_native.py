@@ -296,6 +296,95 @@ def _declare(lib: ctypes.CDLL) -> None:
         ctypes.c_int,  # variant
         _c_void_p,  # stream
     ]
+    lib.b200tx_qk_norm_rope.restype = ctypes.c_int
+    lib.b200tx_qk_norm_rope.argtypes = [
+        _c_void_p,  # qkv
+        _c_void_p,  # out
+        ctypes.c_int,  # dtype
+        _c_int64,  # batch
+        _c_int64,  # tokens
+        _c_int64,  # heads
+        _c_int64,  # kv_heads
+        _c_int64,  # head_dim
+        _c_int64,  # in_batch_stride
+        _c_int64,  # in_token_stride
+        _c_int64,  # out_batch_stride
+        _c_int64,  # out_token_stride
+        _c_void_p,  # q_weight
+        _c_void_p,  # k_weight
+        ctypes.c_float,  # eps
+        _c_void_p,  # rope (b200tx_rope* or NULL)
+        _c_void_p,  # positions
+        ctypes.c_int,  # positions_64
+        _c_int64,  # position_batch_stride
+        _c_void_p,  # stream
+    ]
+    lib.b200tx_kv8_append.restype = ctypes.c_int
+    lib.b200tx_kv8_append.argtypes = [
+        _c_void_p,  # cache (b200tx_kv8_cache*)
+        _c_void_p,  # qkv
+        ctypes.c_int,  # dtype
+        _c_void_p,  # q_out
+        _c_int64,  # batch
+        _c_int64,  # tokens
+        _c_int64,  # heads
+        _c_int64,  # batch_stride
+        _c_int64,  # token_stride
+        _c_void_p,  # slot_ids
+        _c_void_p,  # counts
+        _c_void_p,  # q_weight
+        _c_void_p,  # k_weight
+        ctypes.c_float,  # eps
+        _c_void_p,  # rope
+        _c_void_p,  # stream
+    ]
+    lib.b200tx_kv8_gather.restype = ctypes.c_int
+    lib.b200tx_kv8_gather.argtypes = [
+        _c_void_p,  # cache
+        _c_void_p,  # k_out
+        _c_void_p,  # v_out
+        _c_int64,  # batch
+        _c_int64,  # most
+        _c_int64,  # tokens
+        _c_void_p,  # slot_ids
+        _c_void_p,  # counts
+        _c_void_p,  # stream
+    ]
+    lib.b200tx_kv8_workspace_bytes.restype = ctypes.c_int
+    lib.b200tx_kv8_workspace_bytes.argtypes = [_c_int64, ctypes.POINTER(_c_int64)]
+    lib.b200tx_kv8_attention.restype = ctypes.c_int
+    lib.b200tx_kv8_attention.argtypes = [
+        _c_void_p,  # cache
+        _c_void_p,  # q
+        _c_void_p,  # out
+        _c_int64,  # batch
+        _c_int64,  # tokens
+        _c_int64,  # heads
+        _c_int64,  # q_batch_stride
+        _c_int64,  # q_token_stride
+        _c_void_p,  # slot_ids
+        _c_void_p,  # counts
+        ctypes.c_float,  # scale
+        _c_void_p,  # workspace
+        _c_int64,  # workspace_bytes
+        _c_void_p,  # stream
+    ]
+    lib.b200tx_linear_w4.restype = ctypes.c_int
+    lib.b200tx_linear_w4.argtypes = [
+        _c_void_p,  # x
+        _c_int64,  # x_stride
+        _c_void_p,  # packed
+        _c_void_p,  # scales
+        _c_void_p,  # bias
+        _c_void_p,  # out
+        ctypes.c_int,  # out_dtype
+        _c_int64,  # M
+        _c_int64,  # N
+        _c_int64,  # K
+        _c_int64,  # group
+        ctypes.c_int,  # epilogue
+        _c_void_p,  # stream
+    ]
 
 
 def library_path() -> Path:
@@ -316,6 +405,8 @@ def load() -> ctypes.CDLL:
     """Load libb200tx once; raise RuntimeError with the reason on failure."""
 
     global _lib, _load_error
+    if _lib is not None:  # set once and never cleared
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -886,7 +977,171 @@ def peer_wait(flags: int, count: int, self_index: int, epoch: int, device: torch
            "b200tx_peer_wait")
 
 
+class Rope(ctypes.Structure):
+    """b200tx_rope: rotation tables."""
+
+    _fields_ = [
+        ("cos", ctypes.c_void_p),
+        ("sin", ctypes.c_void_p),
+        ("positions", ctypes.c_int64),
+        ("rotary", ctypes.c_int64),
+        ("interleaved", ctypes.c_int),
+    ]
+
+
+class Kv8CacheView(ctypes.Structure):
+    """b200tx_kv8_cache: device pointers of one layer of an 8-bit cache."""
+
+    _fields_ = [
+        ("codes", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("tail", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("pages", ctypes.c_int64),
+        ("slots", ctypes.c_int64),
+        ("max_blocks", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+    ]
+
+
+KV8_BLOCK = 64  # B200TX_KV8_BLOCK
+
+
+def _pointer(tensor: torch.Tensor | None) -> int | None:
+    return None if tensor is None else tensor.data_ptr()
+
+
+def qk_norm_rope(
+    qkv: torch.Tensor,
+    out: torch.Tensor,
+    heads: int,
+    kv_heads: int,
+    head_dim: int,
+    q_weight: torch.Tensor | None,
+    k_weight: torch.Tensor | None,
+    eps: float,
+    rope: object | None,
+    positions: torch.Tensor | None,
+) -> None:
+    """Launch b200tx_qk_norm_rope over qkv [B, T, W]; `rope` is a ctypes
+    reference to a Rope, `positions` [B, T] or [T]."""
+
+    batch, tokens, _ = qkv.shape
+    status = load().b200tx_qk_norm_rope(
+        qkv.data_ptr(), out.data_ptr(), dtype_code(qkv.dtype), batch, tokens, heads, kv_heads, head_dim,
+        qkv.stride(0), qkv.stride(1), out.stride(0), out.stride(1), _pointer(q_weight), _pointer(k_weight), eps, rope,
+        _pointer(positions), int(positions is not None and positions.dtype == torch.int64),
+        positions.stride(0) if positions is not None and positions.ndim == 2 else 0, _stream(qkv.device),
+    )
+    if status:
+        _check(status, "b200tx_qk_norm_rope")
+
+
+def kv8_append(
+    cache: object,
+    qkv: torch.Tensor,
+    q_out: torch.Tensor,
+    heads: int,
+    slot_ids: torch.Tensor | None,
+    counts: torch.Tensor | None,
+    q_weight: torch.Tensor | None,
+    k_weight: torch.Tensor | None,
+    eps: float,
+    rope: object | None,
+) -> None:
+    """Launch b200tx_kv8_append; `cache` is a ctypes reference to a Kv8CacheView."""
+
+    batch, tokens, _ = qkv.shape
+    status = load().b200tx_kv8_append(
+        cache, qkv.data_ptr(), dtype_code(qkv.dtype), q_out.data_ptr(), batch, tokens, heads, qkv.stride(0),
+        qkv.stride(1), _pointer(slot_ids), _pointer(counts), _pointer(q_weight), _pointer(k_weight), eps, rope,
+        _stream(qkv.device),
+    )
+    if status:
+        _check(status, "b200tx_kv8_append")
+
+
+def kv8_gather(
+    cache: object,
+    k_out: torch.Tensor,
+    v_out: torch.Tensor,
+    tokens: int,
+    slot_ids: torch.Tensor | None,
+    counts: torch.Tensor | None,
+) -> None:
+    """Launch b200tx_kv8_gather into k_out and v_out [B, most, Hkv, D]."""
+
+    status = load().b200tx_kv8_gather(
+        cache, k_out.data_ptr(), v_out.data_ptr(), k_out.shape[0], k_out.shape[1], tokens, _pointer(slot_ids),
+        _pointer(counts), _stream(k_out.device),
+    )
+    if status:
+        _check(status, "b200tx_kv8_gather")
+
+
+def kv8_workspace_bytes(head_dim: int) -> int:
+    """The attention's workspace on the current device."""
+
+    size = ctypes.c_int64(0)
+    _check(load().b200tx_kv8_workspace_bytes(head_dim, ctypes.byref(size)), "b200tx_kv8_workspace_bytes")
+    return int(size.value)
+
+
+def kv8_attention(
+    cache: object,
+    q: torch.Tensor,
+    out: torch.Tensor,
+    slot_ids: torch.Tensor | None,
+    counts: torch.Tensor | None,
+    scale: float,
+    workspace: torch.Tensor,
+    stream: int,
+) -> None:
+    """Launch b200tx_kv8_attention for q [B, T, H, D] on `stream`, the stream
+    that `workspace` (uint8) belongs to."""
+
+    batch, tokens, heads, _ = q.shape
+    status = load().b200tx_kv8_attention(
+        cache, q.data_ptr(), out.data_ptr(), batch, tokens, heads, q.stride(0), q.stride(1), _pointer(slot_ids),
+        _pointer(counts), scale, workspace.data_ptr(), workspace.numel(), stream,
+    )
+    if status:
+        _check(status, "b200tx_kv8_attention")
+
+
+def linear_w4(
+    x: torch.Tensor,
+    packed: torch.Tensor,
+    scales: torch.Tensor,
+    bias: torch.Tensor | None,
+    out: torch.Tensor,
+    rows: int,
+    inner: int,
+    group: int,
+    epilogue: int,
+) -> None:
+    """Launch b200tx_linear_w4 for `rows` dense rows of x."""
+
+    status = load().b200tx_linear_w4(
+        x.data_ptr(), inner, packed.data_ptr(), scales.data_ptr(), _pointer(bias), out.data_ptr(),
+        dtype_code(out.dtype), rows, packed.shape[0], inner, group, epilogue, _stream(x.device),
+    )
+    if status:
+        _check(status, "b200tx_linear_w4")
+
+
 __all__ = [
+    "KV8_BLOCK",
+    "Kv8CacheView",
+    "Rope",
+    "kv8_append",
+    "kv8_attention",
+    "kv8_gather",
+    "kv8_workspace_bytes",
+    "linear_w4",
+    "qk_norm_rope",
     "IPC_HANDLE_BYTES",
     "peer_alloc",
     "peer_close",

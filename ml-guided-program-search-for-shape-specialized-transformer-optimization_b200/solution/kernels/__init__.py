@@ -30,6 +30,26 @@ from .boundary import (
     sm100_linear_residual_norm,
     sm100_mlp_residual_norm,
 )
+from .kv_cache import (
+    KV8_BLOCK,
+    SM100_KV8_APPEND_BACKEND,
+    SM100_KV8_ATTENTION_BACKEND,
+    SM100_KV8_GATHER_BACKEND,
+    Kv8Cache,
+    can_use_sm100_kv8_append,
+    can_use_sm100_kv8_attention,
+    sm100_kv8_append,
+    sm100_kv8_attention,
+    sm100_kv8_gather,
+)
+from .linear_w4 import (
+    SM100_LINEAR_W4_BACKEND,
+    SM100_LINEAR_W4_GELU_BACKEND,
+    W4Weight,
+    can_use_sm100_linear_w4,
+    pack_w4,
+    sm100_linear_w4,
+)
 from .norm import (
     MASK_DROP_UPDATE,
     MASK_ZERO_NORMED,
@@ -48,9 +68,35 @@ from .projection import (
     sm100_linear,
     sm100_linear_available,
 )
+from .rotary import (
+    SM100_QK_NORM_ROPE_BACKEND,
+    RotaryTable,
+    can_use_sm100_qk_norm_rope,
+    sm100_qk_norm_rope,
+)
 from . import ops  # noqa: E402 - registers the torch.ops.b200tx.* operators
 
 __all__ = [
+    "KV8_BLOCK",
+    "Kv8Cache",
+    "RotaryTable",
+    "SM100_KV8_APPEND_BACKEND",
+    "SM100_KV8_ATTENTION_BACKEND",
+    "SM100_KV8_GATHER_BACKEND",
+    "SM100_LINEAR_W4_BACKEND",
+    "SM100_LINEAR_W4_GELU_BACKEND",
+    "SM100_QK_NORM_ROPE_BACKEND",
+    "W4Weight",
+    "can_use_sm100_kv8_append",
+    "can_use_sm100_kv8_attention",
+    "can_use_sm100_linear_w4",
+    "can_use_sm100_qk_norm_rope",
+    "pack_w4",
+    "sm100_kv8_append",
+    "sm100_kv8_attention",
+    "sm100_kv8_gather",
+    "sm100_linear_w4",
+    "sm100_qk_norm_rope",
     "MASK_DROP_UPDATE",
     "MASK_ZERO_NORMED",
     "MASK_ZERO_RESIDUAL",
