@@ -9,6 +9,7 @@
 
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -82,7 +83,7 @@ struct DeviceState {
   bool attn_attr[2 * kAttnVariants] = {};  // unmasked builds by variant, then the masked builds
   bool rownorm_attr[4] = {};               // GEMM + residual LayerNorm builds by (in, out) dtype
   int rownorm_clusters[4][5] = {};         // their co-resident clusters by CTA pairs per cluster
-  bool kv8_attr[4] = {};                   // 8-bit cache attention builds by head_dim
+  bool kv8_attr[9] = {};                   // 8-bit cache attention builds by head_dim and row groups
   bool seq_forward_attr = false;           // whole-forward kernel's shared-memory size set
   uint8_t* seq_noalloc_images = nullptr;   // device address of g_seq_noalloc_images on this device
 };

@@ -122,30 +122,44 @@ cudaError_t launch_kv8_gather(const b200tx::Kv8GatherArgs& a, cudaStream_t strea
 // that lie in two or more CTAs.
 constexpr int64_t kKv8ArrivalBytes = 8192;
 
-template <int D>
+template <int D, int NR>
 int kv8_attention_grid(int sm_count) {
-  using S = b200tx::Kv8Shape<D>;
-  // a tile's parts have their (max, sum) rows in shared memory when they are joined
-  const int most = S::MAIN / (b200tx::kKv8Rows * 8);
-  const int grid = sm_count * S::CTAS;
-  return grid < most ? grid : most;
+  return sm_count * b200tx::Kv8Shape<D, NR>::CTAS;
+}
+
+template <int D, int NR>
+int64_t kv8_part_bytes(int sm_count) {
+  return static_cast<int64_t>(kv8_attention_grid<D, NR>(sm_count)) * 2 * b200tx::Kv8Shape<D, NR>::PART_FLOATS * 4;
+}
+
+// Row groups of 8 in a tile, for which a code is expanded once: up to 4 where the
+// outputs of 32 rows fit in the registers (head_dim 32 and 64), 2 for 128, 1 for 256.
+int kv8_row_groups(int64_t head_dim, int64_t rows) {
+  if (rows <= 8 || head_dim == 256) return 1;
+  if (rows <= 16 || head_dim == 128) return 2;
+  return 4;
 }
 
 template <int D>
 int64_t kv8_workspace(int sm_count) {
-  return kKv8ArrivalBytes + static_cast<int64_t>(kv8_attention_grid<D>(sm_count)) * 2 * b200tx::Kv8Shape<D>::PART_FLOATS * 4;
+  int64_t most = kv8_part_bytes<D, 1>(sm_count);
+  if constexpr (D <= 128) most = std::max(most, kv8_part_bytes<D, 2>(sm_count));
+  if constexpr (D <= 64) most = std::max(most, kv8_part_bytes<D, 4>(sm_count));
+  return kKv8ArrivalBytes + most;
 }
 
-template <int D>
-cudaError_t launch_kv8_attention(const b200tx::Kv8AttnArgs& a, DeviceState* dev, int index, cudaStream_t stream) {
-  constexpr int smem = b200tx::Kv8Shape<D>::MAIN;
+template <int D, int NR>
+cudaError_t launch_kv8_attention(b200tx::Kv8AttnArgs& a, DeviceState* dev, int index, cudaStream_t stream) {
+  using S = b200tx::Kv8Shape<D, NR>;
+  a.row_tiles = (a.tokens * a.group + S::ROWS - 1) / S::ROWS;
   if (!dev->kv8_attr[index]) {
-    cudaError_t err = cudaFuncSetAttribute(b200tx::kv8_attention_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t err =
+        cudaFuncSetAttribute(b200tx::kv8_attention_kernel<D, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::MAIN);
     if (err != cudaSuccess) return err;
     dev->kv8_attr[index] = true;
   }
-  return launch(b200tx::kv8_attention_kernel<D>, dim3(static_cast<unsigned>(kv8_attention_grid<D>(dev->sm_count))),
-                dim3(b200tx::kKv8Warps * 32), smem, stream, a);
+  return launch(b200tx::kv8_attention_kernel<D, NR>, dim3(static_cast<unsigned>(kv8_attention_grid<D, NR>(dev->sm_count))),
+                dim3(b200tx::kKv8Warps * 32), S::MAIN, stream, a);
 }
 
 template <int TN, int GROUP>
@@ -359,16 +373,26 @@ int b200tx_kv8_attention(const b200tx_kv8_cache* cache, const void* q, void* out
   a.tokens = static_cast<int>(tokens);
   a.heads = static_cast<int>(heads);
   a.group = static_cast<int>(heads / cache->kv_heads);
-  a.row_tiles = static_cast<int>((tokens * a.group + b200tx::kKv8Rows - 1) / b200tx::kKv8Rows);
   a.scale_log2 = scale * 1.4426950408889634f;
   a.arrivals = static_cast<unsigned int*>(workspace);
   a.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kKv8ArrivalBytes);
   cudaError_t err;
-  switch (cache->head_dim) {
-    case 32: err = launch_kv8_attention<32>(a, dev, 0, stream); break;
-    case 64: err = launch_kv8_attention<64>(a, dev, 1, stream); break;
-    case 128: err = launch_kv8_attention<128>(a, dev, 2, stream); break;
-    default: err = launch_kv8_attention<256>(a, dev, 3, stream); break;
+  const int groups = kv8_row_groups(cache->head_dim, tokens * a.group);
+  // all steps of the longest sequences that the page table can hold, and the tiles' own cost
+  const double units = static_cast<double>(batch) * cache->kv_heads * ((tokens * a.group + 8 * groups - 1) / (8 * groups)) *
+                       (2.0 * cache->max_blocks + 4 + b200tx::kKv8TileCost);
+  if (units >= 4294967296.0)
+    return fail(B200TX_ERR_UNSUPPORTED, "kv8_attention: batch x heads x rows x blocks of this call pass 2^32 steps");
+  switch (cache->head_dim + groups) {
+    case 33: err = launch_kv8_attention<32, 1>(a, dev, 0, stream); break;
+    case 34: err = launch_kv8_attention<32, 2>(a, dev, 1, stream); break;
+    case 36: err = launch_kv8_attention<32, 4>(a, dev, 2, stream); break;
+    case 65: err = launch_kv8_attention<64, 1>(a, dev, 3, stream); break;
+    case 66: err = launch_kv8_attention<64, 2>(a, dev, 4, stream); break;
+    case 68: err = launch_kv8_attention<64, 4>(a, dev, 5, stream); break;
+    case 129: err = launch_kv8_attention<128, 1>(a, dev, 6, stream); break;
+    case 130: err = launch_kv8_attention<128, 2>(a, dev, 7, stream); break;
+    default: err = launch_kv8_attention<256, 1>(a, dev, 8, stream); break;
   }
   return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "kv8_attention");
 }

@@ -10,27 +10,36 @@
 // equal share of them whatever the lengths are.
 //
 // Split.  The rows of a (sequence, kv head) are its tokens x the query heads of
-// the group, in tiles of 16, one m16 MMA tile.  A tile's keys are cut into
-// steps of 32 codes (16 tokens in the open block: as many bytes).  All steps
-// of all tiles form one line, cut into equal ranges, one per CTA: a CTA ends
-// within a tile's keys, or does several tiles, and no length of any sequence
-// leaves SMs idle.  A tile that lies in several CTAs is joined by the one
-// that finishes last, in the order of the ranges, so results do not depend on
-// the order of arrival.
+// the group, in tiles of 8 NR.  A tile's keys are cut into steps of 32 or 64 codes
+// (half as many tokens in the open block: as many bytes).  All steps of all tiles, and a
+// fixed cost for each tile, form one line, cut into equal ranges, one per CTA: a
+// CTA ends within a tile's keys, or does several tiles, and no length of any
+// sequence leaves SMs idle.  A tile that lies in several CTAs is joined by the
+// one that finishes last, in the order of the ranges, so results do not
+// depend on the order of arrival.
 //
 // Within a CTA the steps of a tile go round the four warps.  Each lane copies
 // exactly the bytes that it will use itself (cp.async into its own place of a
 // ring in shared memory): a queue with neither barriers nor bank conflicts,
 // deep enough to cover the HBM latency.
 //
-// Numbers.  Codes become fp16 by one permute and one subtraction (exact), the
-// queries are scaled by a power of two per row into fp16 (exact but for what
-// is 2^-24 of the row's largest value), products accumulate in fp32, the
-// block scale multiplies the sum.  Probabilities are rounded to fp16 (2^-11,
-// finer than the bf16 output's 2^-8).  In the open block keys and
+// Products.  Keys and values are the A operand (16 tokens, or 16 dims), queries
+// and probabilities the B operand (8 rows), so that 8 rows cost one MMA and a
+// code is expanded once for all rows of a tile.  The dims' order within a product
+// is free: a lane's bytes are consecutive in memory, and the queries are laid out to match.
+//
+// Numbers.  A code byte under a zero byte is the fp16 number code 2^-24, a
+// subnormal, which the tensor cores take as exactly as any other: expanding two
+// codes is one instruction.  The offset of 128 comes out of the sums, as the
+// accumulators start at -128 2^-24 times the row's sum of queries (or
+// probabilities; both are MMAs with a constant, and the latter also gives the softmax's
+// denominator).  The queries are scaled by a power of two per row into fp16
+// (exact but for what is 2^-24 of the row's largest value), products accumulate
+// in fp32, the block's scale multiplies the sum.  Probabilities are rounded to
+// fp16 (2^-11, finer than the bf16 output's 2^-8).  In the open block keys and
 // queries are bf16 and each probability is the sum of two bf16 numbers.  The
 // running maximum moves only when a score exceeds it by more than 2^8, which
-// leaves room in fp16 and saves most rescalings.
+// leaves room in fp16 and saves most rescalings and most reductions.
 #pragma once
 
 #include "attention_mma_kernels.cuh"
@@ -39,28 +48,36 @@
 namespace b200tx {
 
 constexpr int kKv8Warps = 4;
-constexpr int kKv8Step = 32;      // tokens per step in full blocks
-constexpr int kKv8TailStep = 16;  // tokens per step in the open block
-constexpr int kKv8Rows = 16;      // rows per tile
+constexpr int kKv8TileCost = 6;   // what beginning and joining a tile costs, in steps
 constexpr float kKv8Headroom = 8.f;  // log2 of how far a score may pass the running maximum
+constexpr float kKv8Unit = 16777216.f;  // 2^24: a code's fp16 number is code / 2^24
+constexpr uint32_t kKv8OffsetF16 = 0x80808080u;   // two fp16 -2^-17 = -128 / 2^24
+constexpr uint32_t kKv8OffsetBf16 = 0xb700b700u;  // two bf16 -2^-17
+constexpr float kKv8SumUnit = -131072.f;          // -2^17
 
-template <int D>
+template <int D, int NR>
 struct Kv8Shape {
-  static constexpr int STAGES = D >= 128 ? 3 : D == 64 ? 4 : 6;
-  static constexpr int CTAS = D == 256 ? 1 : D == 128 ? 2 : D == 64 ? 3 : 4;  // per SM
+  static constexpr int TOK = D <= 64 ? 64 : 32;       // tokens per step in full blocks
+  static constexpr int TAIL = TOK / 2;                // and in the open block
+  static constexpr int T16 = TOK / 16;
+  static constexpr int STAGES = D == 32 ? 4 : D == 64 ? 2 : 3;
+  static constexpr int CTAS = D == 256 ? 1 : D == 128 || NR == 4 ? 2 : 3;  // per SM
+  static constexpr int ROWS = 8 * NR;                 // rows per tile
   static constexpr int KB = D / 4 < 16 ? D / 4 : 16;  // bytes per key copy
   static constexpr int KC = D / 4 / KB;               // key copies per row and lane
   static constexpr int VB = D / 8 < 16 ? D / 8 : 16;  // bytes per value copy
   static constexpr int VC = D / 8 / VB;
-  static constexpr int HALF = kKv8Step * D;           // bytes of a step's keys (or values)
+  static constexpr int HALF = TOK * D;                // bytes of a step's keys (or values)
   static constexpr int STAGE = 2 * HALF + 16;         // and the two scales
   static constexpr int KSTEPS = D / 16;               // k16 steps of q . k
-  static constexpr int NT = D / 8;                    // n8 tiles of the output
+  static constexpr int MT = D / 16;                   // m16 tiles of the output
+  static constexpr int FRAGS = MT * NR;               // fragments (4 floats a lane) of the output
+  static constexpr int SHARE = FRAGS >= kKv8Warps ? FRAGS / kKv8Warps : 1;  // of one warp, when joining
   static constexpr int RING = kKv8Warps * STAGES * STAGE;
-  static constexpr int JOIN = kKv8Warps * kKv8Rows * D * 4;  // the warps' outputs, over the ring
+  static constexpr int JOIN = kKv8Warps * ROWS * D * 4;  // the warps' outputs, over the ring
   static constexpr int MAIN = RING > JOIN ? RING : JOIN;
-  // a CTA's part of a tile: outputs as fragments, then (max, sum) of 16 rows
-  static constexpr int PART_FLOATS = kKv8Rows * D + 2 * kKv8Rows;
+  // a CTA's part of a tile: outputs as fragments, then (max, sum) of the rows
+  static constexpr int PART_FLOATS = ROWS * D + 2 * ROWS;
 };
 
 struct Kv8AttnArgs {
@@ -77,8 +94,18 @@ struct Kv8AttnArgs {
 };
 
 template <int BYTES>
-__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool take) {
-  const int n = take ? BYTES : 0;  // what is not taken reads as zero
+__device__ __forceinline__ void cp_async(uint32_t dst, const void* src) {
+  if constexpr (BYTES == 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  } else {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+  }
+}
+
+// What is not taken is written as zero, and not read.
+template <int BYTES>
+__device__ __forceinline__ void cp_async_or_zero(uint32_t dst, const void* src, bool take) {
+  const int n = take ? BYTES : 0;
   if constexpr (BYTES == 16) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
   } else {
@@ -106,14 +133,27 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Two codes (bytes SEL of the words) as fp16 numbers code - 128: the byte under
-// 0x64 is 1024 + code.
-template <int SEL>
-__device__ __forceinline__ uint32_t codes_f16x2(uint32_t w) {
-  const uint32_t biased = __byte_perm(w, 0x64646464u, SEL);
-  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&biased), __half2half2(__ushort_as_half(0x6480)));
-  return *reinterpret_cast<const uint32_t*>(&v);
+// The same with the accumulator read from elsewhere: d = a b + (c0, c1, c0, c1).
+__device__ __forceinline__ void mma_m16n8k16_f16_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                                      float c0, float c1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %10, %11};\n"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
+
+// An 8 x 8 matrix of 16-bit values, row lane / 4 and columns 2 (lane % 4) + {0, 1}
+// in each lane, transposed.
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// Codes 0 and 2 (1 and 3) of a word as fp16 numbers code 2^-24.
+__device__ __forceinline__ uint32_t codes_even(uint32_t w) { return w & 0x00ff00ffu; }
+__device__ __forceinline__ uint32_t codes_odd(uint32_t w) { return __byte_perm(w, 0u, 0x4341); }
 
 template <int BYTES>
 __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[BYTES / 4]) {
@@ -134,6 +174,7 @@ struct Kv8Sequence {
   bool bad;  // no such slot, or longer than its page table: outputs are NaN
 };
 
+template <int TOK>
 __device__ __forceinline__ Kv8Sequence kv8_sequence(const Kv8AttnArgs& a, int b) {
   Kv8Sequence s;
   s.slot = a.slot_ids == nullptr ? b : a.slot_ids[b];
@@ -145,33 +186,43 @@ __device__ __forceinline__ Kv8Sequence kv8_sequence(const Kv8AttnArgs& a, int b)
   const int open = s.total % kKv8Block;
   s.steps = s.bad || s.count == 0
                 ? 0
-                : s.total / kKv8Block * (kKv8Block / kKv8Step) + (open + kKv8TailStep - 1) / kKv8TailStep;
+                : s.total / kKv8Block * (kKv8Block / TOK) + (open + TOK / 2 - 1) / (TOK / 2);
   return s;
 }
 
-template <int D>
-__global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D>::CTAS) kv8_attention_kernel(Kv8AttnArgs a) {
-  using S = Kv8Shape<D>;
+// The line of all units cut into ranges: the first `more` have each + 1.
+struct Kv8Ranges {
+  unsigned each, more;
+  __device__ __forceinline__ unsigned begin(unsigned cta) const { return cta * each + min(cta, more); }
+  __device__ __forceinline__ unsigned of(unsigned unit) const {
+    const unsigned big = more * (each + 1);
+    return unit < big ? unit / (each + 1) : more + (unit - big) / each;
+  }
+};
+
+template <int D, int NR>
+__global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_attention_kernel(Kv8AttnArgs a) {
+  using S = Kv8Shape<D, NR>;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int64_t scan[kKv8Warps];
-  __shared__ int64_t found_offset;
+  __shared__ unsigned scan[kKv8Warps];
+  __shared__ unsigned found_offset;
   __shared__ int found_b;
-  __shared__ float2 warp_ml[kKv8Warps][kKv8Rows];
-  __shared__ float row_sum[kKv8Rows];
-  __shared__ float row_part[8][kKv8Rows];
+  __shared__ float2 warp_ml[kKv8Warps][S::ROWS];
   __shared__ int is_last;
 
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t4 = lane % 4;
-  const int tiles = a.cache.kv_heads * a.row_tiles;  // of a sequence
+  const unsigned tiles = a.cache.kv_heads * a.row_tiles;  // of a sequence
+  const float minus_inf = __int_as_float(0xff800000), nan = __int_as_float(0x7fffffff);
   griddep_wait();
   griddep_launch_dependents();
 
   // ---- where this CTA's range begins
+  auto cost_of = [&](int steps) { return steps == 0 ? 0u : static_cast<unsigned>(steps + kKv8TileCost); };
   const int chunk = (a.batch + kKv8Warps * 32 - 1) / (kKv8Warps * 32);
-  int64_t mine = 0;
+  unsigned mine = 0;
   for (int b = tid * chunk; b < min(a.batch, (tid + 1) * chunk); ++b) {
-    const Kv8Sequence s = kv8_sequence(a, b);
-    mine += s.steps;
+    const Kv8Sequence s = kv8_sequence<S::TOK>(a, b);
+    mine += cost_of(s.steps);
     if (s.steps == 0 && b % gridDim.x == blockIdx.x) {
       // nothing to attend to: zeros (NaN if the sequence is not one)
       const uint32_t fill = s.bad ? 0x7fff7fffu : 0u;
@@ -179,31 +230,35 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D>::CTAS) kv8_attenti
       for (int64_t i = 0; i < static_cast<int64_t>(a.tokens) * a.heads * D / 8; ++i) o[i] = make_uint4(fill, fill, fill, fill);
     }
   }
-  int64_t before = mine;  // inclusive sum over the warp, then exclusive over the CTA
+  // inclusive sums over the warp, then exclusive over the CTA
+  unsigned before = mine;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
-    const int64_t n = __shfl_up_sync(0xffffffffu, before, d);
+    const unsigned n = __shfl_up_sync(0xffffffffu, before, d);
     if (lane >= d) before += n;
   }
   if (lane == 31) scan[warp] = before;
   __syncthreads();
   before -= mine;
-  int64_t all = 0;
+  unsigned all = 0;
 #pragma unroll
   for (int w = 0; w < kKv8Warps; ++w) {
     if (w < warp) before += scan[w];
     all += scan[w];
   }
-  const int64_t total = all * tiles;
-  // at least one step a warp, so that short contexts are not cut into crumbs
-  const int64_t ctas = min(static_cast<int64_t>(gridDim.x), (total + kKv8Warps - 1) / kKv8Warps);
+  const unsigned total = all * tiles;  // the host has checked that it fits
+  // at least a step for each warp, so that short contexts are not cut into crumbs
+  const unsigned ctas = min((total + kKv8Warps - 1) / kKv8Warps, gridDim.x);
   if (blockIdx.x >= ctas) return;
-  const int64_t lo = total * blockIdx.x / ctas, hi = total * (blockIdx.x + 1) / ctas;
+  Kv8Ranges ranges;
+  ranges.each = total / ctas;
+  ranges.more = total - ranges.each * ctas;
+  const unsigned lo = ranges.begin(blockIdx.x), hi = ranges.begin(blockIdx.x + 1);
   if (lo >= before * tiles && lo < (before + mine) * tiles) {
-    int64_t offset = before * tiles;
+    unsigned offset = before * tiles;
     int b = tid * chunk;
     for (;; ++b) {
-      const int64_t n = static_cast<int64_t>(kv8_sequence(a, b).steps) * tiles;
+      const unsigned n = cost_of(kv8_sequence<S::TOK>(a, b).steps) * tiles;
       if (lo < offset + n) break;
       offset += n;
     }
@@ -213,294 +268,399 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D>::CTAS) kv8_attenti
   __syncthreads();
 
   int b = found_b;
-  int64_t offset = found_offset;  // of sequence b in the line
-  Kv8Sequence seq = kv8_sequence(a, b);
+  unsigned offset = found_offset;  // of sequence b in the line
+  Kv8Sequence seq = kv8_sequence<S::TOK>(a, b);
   uint8_t* const ring = smem + warp * S::STAGES * S::STAGE;
-  int64_t cur = lo;
+  unsigned cur = lo;
+  bool first_piece = true;
   while (cur < hi) {
-    while (cur >= offset + static_cast<int64_t>(seq.steps) * tiles) {
-      offset += static_cast<int64_t>(seq.steps) * tiles;
-      seq = kv8_sequence(a, ++b);
+    while (cur >= offset + cost_of(seq.steps) * tiles) {
+      offset += cost_of(seq.steps) * tiles;
+      seq = kv8_sequence<S::TOK>(a, ++b);
     }
-    const int tile = static_cast<int>((cur - offset) / seq.steps);
-    const int64_t tile_begin = offset + static_cast<int64_t>(tile) * seq.steps;
-    const int step0 = static_cast<int>(cur - tile_begin);
-    const int step1 = static_cast<int>(min(static_cast<int64_t>(seq.steps), hi - tile_begin));
+    const unsigned cost = cost_of(seq.steps);
+    const int tile = static_cast<int>((cur - offset) / cost);
+    const unsigned tile_begin = offset + tile * cost;
+    // a tile's units are its fixed cost, then its steps
+    const int from_unit = static_cast<int>(cur - tile_begin);
+    const int to_unit = static_cast<int>(min(cost, hi - tile_begin));
+    const int step0 = max(0, from_unit - kKv8TileCost);
+    const int step1 = max(0, to_unit - kKv8TileCost);
+    cur = tile_begin + to_unit;
+    const int which = first_piece ? 0 : 1;
+    if (step1 <= step0) continue;  // the range ends within the fixed cost: nothing to do here
+    first_piece = false;
+
     const int head = tile % a.cache.kv_heads;
-    const int row0 = tile / a.cache.kv_heads * kKv8Rows;
-    const int rows = min(kKv8Rows, a.tokens * a.group - row0);
+    const int row0 = tile / a.cache.kv_heads * S::ROWS;
     const int full = seq.total / kKv8Block;
     const int open = seq.total - full * kKv8Block;
     const int start = seq.total - seq.count;
     const int mine_steps = max(0, (step1 - step0 - warp + kKv8Warps - 1) / kKv8Warps);
     bool poisoned = false;
 
+    // ---- queries: lane (g, t) has dims of row g of each row group, as B fragments.
+    // Their loads go out first, to wait together with the page numbers'.
+    uint2 q_bits[NR][S::KSTEPS];
+    int my_limit[NR];
+    int least = 0x7fffffff;
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const int row = row0 + r * 8 + g;
+      const int token = a.tokens == 1 ? row >= a.group : row / a.group;
+      const bool real = row < a.tokens * a.group && token < seq.count;
+      my_limit[r] = real ? start + token : -1;
+      if (real) least = min(least, my_limit[r]);
+      const __nv_bfloat16* src = a.q + static_cast<int64_t>(b) * a.q_batch_stride + token * a.q_token_stride +
+                                 (head * a.group + row - token * a.group) * D + t4 * S::KB;
+#pragma unroll
+      for (int k = 0; k < S::KSTEPS; ++k) {
+        q_bits[r][k] = make_uint2(0u, 0u);
+        if (real) q_bits[r][k] = *reinterpret_cast<const uint2*>(src + k / (S::KB / 4) * 64 + 4 * (k % (S::KB / 4)));
+      }
+    }
+
     // ---- this warp's copies.  Step k of the warp is step step0 + warp + 4 k.
+    const int coded_steps = full * (kKv8Block / S::TOK);
     int pages = 0;  // lane i: the page of step (k & ~31) + i of the warp
     auto issue = [&](int k) {
       if (k < mine_steps) {
         if ((k & 31) == 0) {
           const int step = step0 + warp + kKv8Warps * (k + lane);
-          pages = step < 2 * full && k + lane < mine_steps ? kv8_page(a.cache, seq.slot, step / 2) : 0;
+          pages = step < coded_steps && k + lane < mine_steps ? kv8_page(a.cache, seq.slot, step / (kKv8Block / S::TOK)) : 0;
         }
         const int step = step0 + warp + kKv8Warps * k;
-        const int page = __shfl_sync(0xffffffffu, pages, k & 31);
-        const uint32_t stage = smem_u32(ring + (k % S::STAGES) * S::STAGE);
-        if (step < 2 * full) {
-          const bool good = page >= 0;
-          poisoned = poisoned || !good;
-          const int64_t at = static_cast<int64_t>(good ? page : 0) * 2 * a.cache.kv_heads + head;
-          const uint8_t* kp = a.cache.codes + at * kKv8Block * D + (step & 1) * S::HALF;
-          const uint8_t* vp = kp + static_cast<int64_t>(a.cache.kv_heads) * kKv8Block * D;
+        int page = __shfl_sync(0xffffffffu, pages, k & 31);
+        uint8_t* const stage_at = ring + (k % S::STAGES) * S::STAGE;
+        const uint32_t k_stage = smem_u32(stage_at) + lane * S::KB;
+        const uint32_t v_stage = smem_u32(stage_at) + S::HALF + lane * S::VB;
+        if (step < coded_steps) {
+          poisoned = poisoned || page < 0;
+          page = max(page, 0);  // page 0 is always there
+          const int64_t at = static_cast<int64_t>(page) * 2 * a.cache.kv_heads + head;
+          const uint8_t* block = a.cache.codes + at * kKv8Block * D + step % (kKv8Block / S::TOK) * S::HALF;
+          const uint8_t* kp = block + g * D + t4 * S::KB;
+          const uint8_t* vp = block + static_cast<int64_t>(a.cache.kv_heads) * kKv8Block * D + 2 * t4 * D + g * S::VB;
 #pragma unroll
-          for (int n = 0; n < 4; ++n) {
+          for (int x = 0; x < 2 * S::T16 * S::KC; ++x)
+            cp_async<S::KB>(k_stage + x * 32 * S::KB, kp + x / S::KC * 8 * D + x % S::KC * 64);
 #pragma unroll
-            for (int c = 0; c < S::KC; ++c)
-              cp_async<S::KB>(stage + ((n * S::KC + c) * 32 + lane) * S::KB, kp + (n * 8 + g) * D + c * 64 + t4 * S::KB, good);
+          for (int x = 0; x < 4 * S::T16 * S::VC; ++x) {  // tokens 16 (i / 4) + {2t, 2t+1, 2t+8, 2t+9}
+            const int i = x / S::VC;
+            cp_async<S::VB>(v_stage + x * 32 * S::VB,
+                            vp + ((i / 4) * 16 + (i & 1) + ((i >> 1) & 1) * 8) * D + x % S::VC * 128);
           }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {  // tokens (i / 4) * 16 + {2t, 2t+1, 2t+8, 2t+9}
-            const int token = (i / 4) * 16 + 2 * t4 + (i & 1) + ((i >> 1) & 1) * 8;
-#pragma unroll
-            for (int c = 0; c < S::VC; ++c)
-              cp_async<S::VB>(stage + S::HALF + ((i * S::VC + c) * 32 + lane) * S::VB, vp + token * D + c * 128 + g * S::VB, good);
-          }
-          if (lane < 2) cp_async<4>(stage + 2 * S::HALF + 4 * lane, a.cache.scales + at + lane * a.cache.kv_heads, good);
+          if (lane < 2) cp_async<4>(smem_u32(stage_at) + 2 * S::HALF + 4 * lane, a.cache.scales + at + lane * a.cache.kv_heads);
         } else {
-          const int first = (step - 2 * full) * kKv8TailStep;
-          const __nv_bfloat16* kp = kv8_tail(a.cache, seq.slot, full & 1, 0, head, D);
-          const __nv_bfloat16* vp = kv8_tail(a.cache, seq.slot, full & 1, 1, head, D);
+          const int first = (step - coded_steps) * S::TAIL;
+          const __nv_bfloat16* kp = kv8_tail(a.cache, seq.slot, full & 1, 0, head, D) + (first + g) * D + t4 * S::KB;
+          const __nv_bfloat16* vp = kv8_tail(a.cache, seq.slot, full & 1, 1, head, D) + (first + 2 * t4) * D + g * S::VB;
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            const int token = first + n * 8 + g;
-#pragma unroll
-            for (int c = 0; c < S::KC; ++c) {
-#pragma unroll
-              for (int h = 0; h < 2; ++h)
-                cp_async<S::KB>(stage + (((n * S::KC + c) * 2 + h) * 32 + lane) * S::KB,
-                                kp + token * D + c * 64 + t4 * S::KB + h * (S::KB / 2), token < open);
-            }
+          for (int x = 0; x < 2 * S::T16 * S::KC; ++x) {
+            const int n = x / (2 * S::KC), c = x / 2 % S::KC, h = x % 2;
+            cp_async_or_zero<S::KB>(k_stage + x * 32 * S::KB, kp + n * 8 * D + c * 64 + h * (S::KB / 2), first + g + n * 8 < open);
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int token = first + 2 * t4 + (i & 1) + (i >> 1) * 8;
-#pragma unroll
-            for (int c = 0; c < S::VC; ++c) {
-#pragma unroll
-              for (int h = 0; h < 2; ++h)
-                cp_async<S::VB>(stage + S::HALF + (((i * S::VC + c) * 2 + h) * 32 + lane) * S::VB,
-                                vp + token * D + c * 128 + g * S::VB + h * (S::VB / 2), token < open);
-            }
+          for (int x = 0; x < 4 * S::T16 * S::VC; ++x) {
+            const int i = x / (2 * S::VC), c = x / 2 % S::VC, h = x % 2;
+            const int token = (i / 4) * 16 + (i & 1) + ((i >> 1) & 1) * 8;
+            cp_async_or_zero<S::VB>(v_stage + x * 32 * S::VB, vp + token * D + c * 128 + h * (S::VB / 2),
+                                    first + 2 * t4 + token < open);
           }
         }
       }
       cp_async_commit();
     };
-#pragma unroll
+#pragma unroll 1  // straight-line code that runs once costs its fetch
     for (int k = 0; k < S::STAGES - 1; ++k) issue(k);
 
-    // ---- queries: rows g and g + 8 of the tile, scaled by a power of two into fp16
-    uint32_t qf[S::KSTEPS][4];
-    float row_scale[2];  // turns a sum of products into a log2 score
-    int limit[2];        // the row's own position: the last key that it sees
-    int least = 0x7fffffff;
+    uint32_t qf[NR][S::KSTEPS][2];
+    // of rows 2 t and 2 t + 1 of each group, the columns of the accumulators:
+    float row_scale[NR][2];  // turns a sum of products into a log2 score
+    float q_start[NR][2];    // where the sum starts, -128 2^-24 times the sum of the queries
+    int limit[NR][2];        // the row's own position: the last key that it sees
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = row0 + g + 8 * r;
-      const int token = row / a.group;
-      const bool real = row < a.tokens * a.group && token < seq.count;
-      limit[r] = real ? start + token : -1;
-      if (real) least = min(least, limit[r]);
-      const __nv_bfloat16* src = a.q + static_cast<int64_t>(b) * a.q_batch_stride + token * a.q_token_stride +
-                                 (head * a.group + row % a.group) * D;
-      float x[S::KSTEPS][4];
-      float peak = 0.f;
-      bool finite = true;
+    for (int r = 0; r < NR; ++r) {
+      const uint2(&x)[S::KSTEPS] = q_bits[r];
+      uint32_t peak_bits = 0;
 #pragma unroll
-      for (int c = 0; c < S::KC; ++c) {
-#pragma unroll
-        for (int i = 0; i < S::KB / 4; ++i) {
-          uint2 w = make_uint2(0u, 0u);
-          if (real) w = *reinterpret_cast<const uint2*>(src + c * 64 + t4 * S::KB + 4 * i);
-          float* y = x[c * (S::KB / 4) + i];
-          y[0] = __uint_as_float(w.x << 16); y[1] = __uint_as_float(w.x & 0xffff0000u);
-          y[2] = __uint_as_float(w.y << 16); y[3] = __uint_as_float(w.y & 0xffff0000u);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            peak = fmaxf(peak, fabsf(y[e]));
-            finite = finite && fabsf(y[e]) < __int_as_float(0x7f800000);
-          }
-        }
-      }
-      peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
-      peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
-      const unsigned ok = __ballot_sync(0xffffffffu, finite);
-      finite = ((ok >> (lane & ~3)) & 15u) == 15u;
+      for (int k = 0; k < S::KSTEPS; ++k)
+        peak_bits = max(peak_bits, max(max((x[k].x << 16) & 0x7fff0000u, x[k].x & 0x7fff0000u),
+                                       max((x[k].y << 16) & 0x7fff0000u, x[k].y & 0x7fff0000u)));
+      peak_bits = max(peak_bits, __shfl_xor_sync(0xffffffffu, peak_bits, 1));
+      peak_bits = max(peak_bits, __shfl_xor_sync(0xffffffffu, peak_bits, 2));
+      const bool finite = peak_bits < 0x7f800000u;
       // 2^e <= peak < 2^(e+1), clamped so that 2^e and 2^-e are normal numbers
-      const int e = min(126, max(-100, static_cast<int>(__float_as_uint(peak) >> 23) - 127));
+      const int e = min(126, max(-100, static_cast<int>(peak_bits >> 23) - 127));
       const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
       const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-      row_scale[r] = finite ? up * a.scale_log2 : __int_as_float(0x7fffffff);
+      float start_sum[4];
 #pragma unroll
       for (int k = 0; k < S::KSTEPS; ++k) {
-        qf[k][r] = finite ? pack_f16x2(x[k][0] * down, x[k][1] * down) : 0u;
-        qf[k][2 + r] = finite ? pack_f16x2(x[k][2] * down, x[k][3] * down) : 0u;
+        const float y0 = __uint_as_float(x[k].x << 16), y1 = __uint_as_float(x[k].x & 0xffff0000u);
+        const float y2 = __uint_as_float(x[k].y << 16), y3 = __uint_as_float(x[k].y & 0xffff0000u);
+        qf[r][k][0] = finite ? pack_f16x2(y0 * down, y2 * down) : 0u;
+        qf[r][k][1] = finite ? pack_f16x2(y1 * down, y3 * down) : 0u;
+        const uint32_t offset[4] = {kKv8OffsetF16, kKv8OffsetF16, kKv8OffsetF16, kKv8OffsetF16};
+        if (k == 0) {
+          mma_m16n8k16_f16_from(start_sum, offset, qf[r][k][0], qf[r][k][1], 0.f, 0.f);
+        } else {
+          mma_m16n8k16_f16(start_sum, offset, qf[r][k][0], qf[r][k][1]);
+        }
+      }
+      const float my_scale = finite ? up * a.scale_log2 : nan;
+#pragma unroll
+      for (int e2 = 0; e2 < 2; ++e2) {
+        const int from = (2 * t4 + e2) * 4;
+        row_scale[r][e2] = __shfl_sync(0xffffffffu, my_scale, from);
+        limit[r][e2] = __shfl_sync(0xffffffffu, my_limit[r], from);
+        q_start[r][e2] = start_sum[e2];
       }
     }
     least = __reduce_min_sync(0xffffffffu, least);
 
-    float o[S::NT][4];
+    float o[NR][S::MT][4];
+    float m[NR][2], l[NR][2];
 #pragma unroll
-    for (int j = 0; j < S::NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    const float minus_inf = __int_as_float(0xff800000);
-    float m[2] = {minus_inf, minus_inf}, l[2] = {0.f, 0.f};
+    for (int r = 0; r < NR; ++r) {
+#pragma unroll
+      for (int j = 0; j < S::MT; ++j) o[r][j][0] = o[r][j][1] = o[r][j][2] = o[r][j][3] = 0.f;
+      m[r][0] = m[r][1] = minus_inf;
+      l[r][0] = l[r][1] = 0.f;
+    }
 
-    // Scores (log2) in place to probabilities; `factor` turns sums into scores.
-    auto softmax = [&](auto& s, const float (&factor)[2], int first_token, bool masked) {
-      constexpr int N = sizeof(s) / sizeof(s[0]);
-      float top[2] = {minus_inf, minus_inf};
+    // Sums s (tokens 16 i + g and + 8, rows 2 t and 2 t + 1) to probabilities 2^(s factor - m).
+    auto softmax = [&](auto& s, float (&factor)[NR][2], int first_token, bool masked) {
+      constexpr int TILES = sizeof(s) / sizeof(s[0]);
+      float top[NR][2];
+      bool above = false;
 #pragma unroll
-      for (int n = 0; n < N; ++n) {
+      for (int r = 0; r < NR; ++r) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[n][e] *= factor[e >> 1];
-          if (masked && first_token + n * 8 + 2 * t4 + (e & 1) > limit[e >> 1]) s[n][e] = minus_inf;
-          top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
+        for (int e = 0; e < 2; ++e) {
+          float t = minus_inf;
+          // never 0, so that a masked -inf stays -inf (a block of zeros has scale 0)
+          factor[r][e] = factor[r][e] == 0.f ? 1e-30f : factor[r][e];
+          if (masked) {
+            if (first_token > limit[r][e]) factor[r][e] = 1e-30f;  // sees none: a NaN scale is not its own
+#pragma unroll
+            for (int i = 0; i < TILES; ++i) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                if (first_token + i * 16 + h * 8 + g > limit[r][e]) s[i][r][2 * h + e] = minus_inf;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < TILES; ++i) t = max3(t, s[i][r][e], s[i][r][2 + e]);
+          top[r][e] = t * factor[r][e];
+          above = above || top[r][e] > m[r][e] + kKv8Headroom;
         }
       }
+      if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-      }
-      if (__any_sync(0xffffffffu, top[0] > m[0] + kKv8Headroom || top[1] > m[1] + kKv8Headroom)) {
+        for (int r = 0; r < NR; ++r) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float next = fmaxf(m[r], top[r]);
-          const float by = m[r] == minus_inf ? 0.f : fast_exp2(m[r] - next);
-          m[r] = next;
-          l[r] *= by;
+          for (int e = 0; e < 2; ++e) {
+            float next = fmaxf(top[r][e], __shfl_xor_sync(0xffffffffu, top[r][e], 4));
+            next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, 8));
+            next = max3(next, __shfl_xor_sync(0xffffffffu, next, 16), m[r][e]);
+            const float by = m[r][e] == minus_inf ? 0.f : fast_exp2(m[r][e] - next);
+            m[r][e] = next;
+            l[r][e] *= by;
 #pragma unroll
-          for (int j = 0; j < S::NT; ++j) {
-            o[j][2 * r] *= by;
-            o[j][2 * r + 1] *= by;
+            for (int j = 0; j < S::MT; ++j) {
+              o[r][j][e] *= by;
+              o[r][j][2 + e] *= by;
+            }
           }
         }
       }
-      const float from[2] = {m[0] == minus_inf ? 0.f : m[0], m[1] == minus_inf ? 0.f : m[1]};
 #pragma unroll
-      for (int n = 0; n < N; ++n) {
+      for (int r = 0; r < NR; ++r) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[n][e] = fast_exp2(s[n][e] - from[e >> 1]);
-          l[e >> 1] += s[n][e];
+        for (int e = 0; e < 2; ++e) {
+          const float from = m[r][e] == minus_inf ? 0.f : m[r][e];
+#pragma unroll
+          for (int i = 0; i < TILES; ++i) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              s[i][r][2 * h + e] = fast_exp2(fmaf(s[i][r][2 * h + e], factor[r][e], -from));
+          }
         }
       }
     };
 
+#pragma unroll 1
     for (int k = 0; k < mine_steps; ++k) {
       cp_async_wait<S::STAGES - 2>();
       __syncwarp();
       issue(k + S::STAGES - 1);
       const int step = step0 + warp + kKv8Warps * k;
       uint8_t* stage = ring + (k % S::STAGES) * S::STAGE;
-      if (step < 2 * full) {
-        const int first_token = step * kKv8Step;
+      if (step < coded_steps) {
+        const int first_token = step * S::TOK;
         const float2 scales = *reinterpret_cast<const float2*>(stage + 2 * S::HALF);
-        float s[4][4];
+        float s[S::T16][NR][4];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+        for (int c = 0; c < S::KC; ++c) {
+          uint32_t w[2 * S::T16][S::KB / 4];
 #pragma unroll
-          for (int c = 0; c < S::KC; ++c) {
-            uint32_t w[S::KB / 4];
-            lds_words<S::KB>(stage + ((n * S::KC + c) * 32 + lane) * S::KB, w);
+          for (int n = 0; n < 2 * S::T16; ++n) lds_words<S::KB>(stage + ((n * S::KC + c) * 32 + lane) * S::KB, w[n]);
 #pragma unroll
-            for (int i = 0; i < S::KB / 4; ++i)
-              mma_m16n8k16_f16(s[n], qf[c * (S::KB / 4) + i], codes_f16x2<0x4140>(w[i]), codes_f16x2<0x4342>(w[i]));
+          for (int i = 0; i < S::KB / 4; ++i) {
+            const int ks = c * (S::KB / 4) + i;
+#pragma unroll
+            for (int t = 0; t < S::T16; ++t) {
+              const uint32_t kf[4] = {codes_even(w[2 * t][i]), codes_even(w[2 * t + 1][i]), codes_odd(w[2 * t][i]),
+                                      codes_odd(w[2 * t + 1][i])};
+#pragma unroll
+              for (int r = 0; r < NR; ++r) {
+                if (ks == 0) {
+                  mma_m16n8k16_f16_from(s[t][r], kf, qf[r][0][0], qf[r][0][1], q_start[r][0], q_start[r][1]);
+                } else {
+                  mma_m16n8k16_f16(s[t][r], kf, qf[r][ks][0], qf[r][ks][1]);
+                }
+              }
+            }
           }
         }
-        const bool masked = first_token + kKv8Step - 1 > least;
-        const float factor[2] = {row_scale[0] * scales.x, row_scale[1] * scales.x};
-        softmax(s, factor, first_token, masked);
-        // a row that sees none of these keys takes nothing of them, whatever the scale
-        const float vs[2] = {masked && first_token > limit[0] ? 0.f : scales.y, masked && first_token > limit[1] ? 0.f : scales.y};
-        uint32_t p[2][4];
+        const bool masked = first_token + S::TOK - 1 > least;
+        float factor[NR][2];
+        const float k_unit = scales.x * kKv8Unit, v_unit = scales.y * kKv8Unit;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          p[h][0] = pack_f16x2(s[2 * h][0], s[2 * h][1]);
-          p[h][1] = pack_f16x2(s[2 * h][2], s[2 * h][3]);
-          p[h][2] = pack_f16x2(s[2 * h + 1][0], s[2 * h + 1][1]);
-          p[h][3] = pack_f16x2(s[2 * h + 1][2], s[2 * h + 1][3]);
+        for (int r = 0; r < NR; ++r) {
+          factor[r][0] = row_scale[r][0] * k_unit;
+          factor[r][1] = row_scale[r][1] * k_unit;
+        }
+        softmax(s, factor, first_token, masked);
+        uint32_t p[S::T16][NR][2];
+        float v_start[NR][2], v_scale[NR][2];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          float sum[4];
+          const uint32_t offset[4] = {kKv8OffsetF16, kKv8OffsetF16, kKv8OffsetF16, kKv8OffsetF16};
+#pragma unroll
+          for (int t = 0; t < S::T16; ++t) {
+            p[t][r][0] = transpose_8x8(pack_f16x2(s[t][r][0], s[t][r][1]));
+            p[t][r][1] = transpose_8x8(pack_f16x2(s[t][r][2], s[t][r][3]));
+            if (t == 0) {
+              mma_m16n8k16_f16_from(sum, offset, p[0][r][0], p[0][r][1], 0.f, 0.f);
+            } else {
+              mma_m16n8k16_f16(sum, offset, p[t][r][0], p[t][r][1]);
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            l[r][e] += sum[e];
+            v_start[r][e] = sum[e];
+            // a row that sees none of these keys takes nothing of them, whatever the scale
+            v_scale[r][e] = masked && first_token > limit[r][e] ? 0.f : v_unit;
+          }
         }
 #pragma unroll
         for (int c = 0; c < S::VC; ++c) {
-          uint32_t w[8][S::VB / 4];
+          uint32_t w[4 * S::T16][S::VB / 4];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) lds_words<S::VB>(stage + S::HALF + ((i * S::VC + c) * 32 + lane) * S::VB, w[i]);
+          for (int i = 0; i < 4 * S::T16; ++i)
+            lds_words<S::VB>(stage + S::HALF + ((i * S::VC + c) * 32 + lane) * S::VB, w[i]);
 #pragma unroll
           for (int i = 0; i < S::VB / 4; ++i) {
-            float acc[4][4] = {};
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              // bytes of two tokens side by side: the b fragments' pairs along k
-              const uint32_t ab0 = __byte_perm(w[4 * h][i], w[4 * h + 1][i], 0x5140);
-              const uint32_t ab1 = __byte_perm(w[4 * h][i], w[4 * h + 1][i], 0x7362);
-              const uint32_t cd0 = __byte_perm(w[4 * h + 2][i], w[4 * h + 3][i], 0x5140);
-              const uint32_t cd1 = __byte_perm(w[4 * h + 2][i], w[4 * h + 3][i], 0x7362);
-              mma_m16n8k16_f16(acc[0], p[h], codes_f16x2<0x4140>(ab0), codes_f16x2<0x4140>(cd0));
-              mma_m16n8k16_f16(acc[1], p[h], codes_f16x2<0x4342>(ab0), codes_f16x2<0x4342>(cd0));
-              mma_m16n8k16_f16(acc[2], p[h], codes_f16x2<0x4140>(ab1), codes_f16x2<0x4140>(cd1));
-              mma_m16n8k16_f16(acc[3], p[h], codes_f16x2<0x4342>(ab1), codes_f16x2<0x4342>(cd1));
-            }
+            for (int h = 0; h < 2; ++h) {  // dims 4 i + 2 h and + 1 of the lane's bytes
+              float acc[NR][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float(&dst)[4] = o[c * S::VB + 4 * i + e];
-              dst[0] = fmaf(vs[0], acc[e][0], dst[0]);
-              dst[1] = fmaf(vs[0], acc[e][1], dst[1]);
-              dst[2] = fmaf(vs[1], acc[e][2], dst[2]);
-              dst[3] = fmaf(vs[1], acc[e][3], dst[3]);
+              for (int t = 0; t < S::T16; ++t) {
+                // two tokens' bytes of two dims each, then the tokens' pairs per dim
+                const uint32_t ab = __byte_perm(w[4 * t][i], w[4 * t + 1][i], h ? 0x7632 : 0x5410);
+                const uint32_t cd = __byte_perm(w[4 * t + 2][i], w[4 * t + 3][i], h ? 0x7632 : 0x5410);
+                const uint32_t vf[4] = {codes_even(ab), codes_odd(ab), codes_even(cd), codes_odd(cd)};
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                  if (t == 0) {
+                    mma_m16n8k16_f16_from(acc[r], vf, p[0][r][0], p[0][r][1], v_start[r][0], v_start[r][1]);
+                  } else {
+                    mma_m16n8k16_f16(acc[r], vf, p[t][r][0], p[t][r][1]);
+                  }
+                }
+              }
+#pragma unroll
+              for (int r = 0; r < NR; ++r) {
+                float(&dst)[4] = o[r][c * (S::VB / 2) + 2 * i + h];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) dst[e] = fmaf(v_scale[r][e & 1], acc[r][e], dst[e]);
+              }
             }
           }
         }
       } else {
-        const int in_tail = (step - 2 * full) * kKv8TailStep;
-        const int first_token = full * kKv8Block + in_tail;
-        float s[2][4];
+        constexpr int TT = S::T16 / 2;  // 16-token groups
+        const int first_token = full * kKv8Block + (step - coded_steps) * S::TAIL;
+        float s[TT][NR][4];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+        for (int c = 0; c < 2 * S::KC; ++c) {
+          uint32_t w[2 * TT][S::KB / 4];
 #pragma unroll
-          for (int c = 0; c < 2 * S::KC; ++c) {
-            uint32_t w[S::KB / 4];
-            lds_words<S::KB>(stage + ((n * 2 * S::KC + c) * 32 + lane) * S::KB, w);
+          for (int n = 0; n < 2 * TT; ++n) lds_words<S::KB>(stage + ((n * 2 * S::KC + c) * 32 + lane) * S::KB, w[n]);
 #pragma unroll
-            for (int i = 0; i < S::KB / 8; ++i) {
-              const int ks = c * (S::KB / 8) + i;
-              uint32_t qb[4];  // fp16 -> bf16, exact: they came from bf16
+          for (int i = 0; i < S::KB / 8; ++i) {
+            const int ks = c * (S::KB / 8) + i;
+            uint32_t qb[NR][2];  // fp16 -> bf16, exact: they came from bf16
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&qf[ks][e]));
-                qb[e] = pack_bf16x2(v.x, v.y);
+            for (int r = 0; r < NR; ++r) {
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&qf[r][ks][e]));
+                qb[r][e] = pack_bf16x2(v.x, v.y);
               }
-              mma_m16n8k16_bf16(s[n], qb, w[2 * i], w[2 * i + 1]);
+            }
+#pragma unroll
+            for (int t = 0; t < TT; ++t) {
+              const uint32_t(&wa)[S::KB / 4] = w[2 * t];
+              const uint32_t(&wb)[S::KB / 4] = w[2 * t + 1];
+              const uint32_t kf[4] = {__byte_perm(wa[2 * i], wa[2 * i + 1], 0x5410), __byte_perm(wb[2 * i], wb[2 * i + 1], 0x5410),
+                                      __byte_perm(wa[2 * i], wa[2 * i + 1], 0x7632), __byte_perm(wb[2 * i], wb[2 * i + 1], 0x7632)};
+#pragma unroll
+              for (int r = 0; r < NR; ++r) {
+                if (ks == 0) s[t][r][0] = s[t][r][1] = s[t][r][2] = s[t][r][3] = 0.f;
+                mma_m16n8k16_bf16(s[t][r], kf, qb[r][0], qb[r][1]);
+              }
             }
           }
         }
-        softmax(s, row_scale, first_token, true);
-        uint32_t hi[4], low[4];
+        float factor[NR][2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = s[e >> 1][2 * (e & 1)], y = s[e >> 1][2 * (e & 1) + 1];
-          hi[e] = pack_bf16x2(x, y);
-          low[e] = pack_bf16x2(x - __uint_as_float(hi[e] << 16), y - __uint_as_float(hi[e] & 0xffff0000u));
+        for (int r = 0; r < NR; ++r) {
+          factor[r][0] = row_scale[r][0];
+          factor[r][1] = row_scale[r][1];
+        }
+        softmax(s, factor, first_token, true);
+        uint32_t high[TT][NR][2], low[TT][NR][2];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          const uint32_t offset[4] = {kKv8OffsetBf16, kKv8OffsetBf16, kKv8OffsetBf16, kKv8OffsetBf16};
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int t = 0; t < TT; ++t) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float x = s[t][r][2 * h], y = s[t][r][2 * h + 1];
+              const uint32_t hi2 = pack_bf16x2(x, y);
+              const uint32_t lo2 = pack_bf16x2(x - __uint_as_float(hi2 << 16), y - __uint_as_float(hi2 & 0xffff0000u));
+              high[t][r][h] = transpose_8x8(hi2);
+              low[t][r][h] = transpose_8x8(lo2);
+            }
+            mma_m16n8k16_bf16(sum, offset, high[t][r][0], high[t][r][1]);
+            mma_m16n8k16_bf16(sum, offset, low[t][r][0], low[t][r][1]);
+          }
+          l[r][0] += sum[0];
+          l[r][1] += sum[1];
         }
         // Values that are not finite, and rows that must not see them: 0 x inf
         // would be NaN, so such a step goes value by value.
         bool odd = false;
-        if (seq.count > 1) {
+        if (seq.count > 1 && first_token + S::TAIL - 1 > least) {
 #pragma unroll
-          for (int i = 0; i < 8 * S::VC; ++i) {
+          for (int i = 0; i < 4 * S::T16 * S::VC; ++i) {
             uint32_t w[S::VB / 4];
             lds_words<S::VB>(stage + S::HALF + (i * 32 + lane) * S::VB, w);
 #pragma unroll
@@ -514,46 +674,52 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D>::CTAS) kv8_attenti
           for (int c = 0; c < S::VC; ++c) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              uint32_t w[4][S::VB / 4];
+              uint32_t w[4 * TT][S::VB / 4];
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
+              for (int i = 0; i < 4 * TT; ++i)
                 lds_words<S::VB>(stage + S::HALF + (((i * S::VC + c) * 2 + h) * 32 + lane) * S::VB, w[i]);
 #pragma unroll
               for (int i = 0; i < S::VB / 4; ++i) {
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  float(&dst)[4] = o[c * S::VB + h * (S::VB / 2) + 2 * i + e];
-                  const uint32_t b0 = __byte_perm(w[0][i], w[1][i], e ? 0x7632 : 0x5410);
-                  const uint32_t b1 = __byte_perm(w[2][i], w[3][i], e ? 0x7632 : 0x5410);
-                  mma_m16n8k16_bf16(dst, hi, b0, b1);
-                  mma_m16n8k16_bf16(dst, low, b0, b1);
+                for (int t = 0; t < TT; ++t) {
+                  const uint32_t vf[4] = {
+                      __byte_perm(w[4 * t][i], w[4 * t + 1][i], 0x5410), __byte_perm(w[4 * t][i], w[4 * t + 1][i], 0x7632),
+                      __byte_perm(w[4 * t + 2][i], w[4 * t + 3][i], 0x5410), __byte_perm(w[4 * t + 2][i], w[4 * t + 3][i], 0x7632)};
+#pragma unroll
+                  for (int r = 0; r < NR; ++r) {
+                    float(&dst)[4] = o[r][c * (S::VB / 2) + h * (S::VB / 4) + i];
+                    mma_m16n8k16_bf16(dst, vf, high[t][r][0], high[t][r][1]);
+                    mma_m16n8k16_bf16(dst, vf, low[t][r][0], low[t][r][1]);
+                  }
                 }
               }
             }
           }
         } else {
-          // probabilities over the step's keys, which are used up: [16 rows][16 tokens]
-          __syncwarp();
+          // 16 tokens of a row group's probabilities at a time, over the step's keys, which are used up
           float* pr = reinterpret_cast<float*>(stage);
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
+          for (int rt = 0; rt < NR * TT; ++rt) {
+            const int r = rt / TT, t = rt % TT;
+            __syncwarp();
 #pragma unroll
-            for (int e = 0; e < 4; ++e) pr[(g + 8 * (e >> 1)) * 16 + n * 8 + 2 * t4 + (e & 1)] = s[n][e];
-          }
-          __syncwarp();
-          for (int token = 0; token < kKv8TailStep; ++token) {
-            // token = 2t' + (i & 1) + (i >> 1) * 8 lies with lanes t' in copy i
-            const int from_t = (token % 8) / 2, i = (token & 1) + (token / 8) * 2;
-            const int where = first_token + token;
+            for (int e = 0; e < 4; ++e) pr[(2 * t4 + (e & 1)) * 16 + g + 8 * (e >> 1)] = s[t][r][e];
+            __syncwarp();
+#pragma unroll 1
+            for (int token = 0; token < 16; ++token) {
+              // token = 2 t' + (i & 1) + (i >> 1) * 8 lies with lanes t' in copy 4 t + i
+              const int from_t = (token % 8) / 2, i = 4 * t + (token & 1) + (token / 8) * 2;
+              const int where = first_token + 16 * t + token;
 #pragma unroll
-            for (int j = 0; j < S::NT; ++j) {
-              const int c = j / S::VB, h = (j % S::VB) / (S::VB / 2), at = j % (S::VB / 2);
+              for (int j = 0; j < S::MT; ++j) {
+                const int c = j / (S::VB / 2), h = j % (S::VB / 2) / (S::VB / 4), at = j % (S::VB / 4);
+                const uint32_t two = *reinterpret_cast<const uint32_t*>(
+                    stage + S::HALF + (((i * S::VC + c) * 2 + h) * 32 + g * 4 + from_t) * S::VB + 4 * at);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int from = (2 * t4 + (e & 1)) * 4 + from_t;
-                const uint8_t* p = stage + S::HALF + (((i * S::VC + c) * 2 + h) * 32 + from) * S::VB + 2 * at;
-                const float v = __uint_as_float(static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p)) << 16);
-                if (where <= limit[e >> 1]) o[j][e] = fmaf(pr[(g + 8 * (e >> 1)) * 16 + token], v, o[j][e]);
+                for (int e = 0; e < 4; ++e) {
+                  const float v = __uint_as_float(e < 2 ? two << 16 : two & 0xffff0000u);
+                  if (where <= limit[r][e & 1]) o[r][j][e] = fmaf(pr[(2 * t4 + (e & 1)) * 16 + token], v, o[r][j][e]);
+                }
               }
             }
           }
@@ -563,153 +729,174 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D>::CTAS) kv8_attenti
     }
     cp_async_wait<0>();
 
-    // ---- join the warps: fragments [warp][n tile][lane], a quarter of the n tiles each
+    // ---- join the warps: fragments [warp][r, j][lane], a share of them for each warp
+    if (g == 0) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      if (poisoned) l[r] = __int_as_float(0x7fffffff);
-      if (t4 == 0) warp_ml[warp][g + 8 * r] = make_float2(m[r], l[r]);
+      for (int r = 0; r < NR; ++r) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          warp_ml[warp][r * 8 + 2 * t4 + e] = make_float2(m[r][e], poisoned ? nan : l[r][e] * kKv8SumUnit);
+      }
     }
     __syncthreads();  // everyone is done with the ring
     float4* const join = reinterpret_cast<float4*>(smem);
 #pragma unroll
-    for (int j = 0; j < S::NT; ++j) join[(warp * S::NT + j) * 32 + lane] = make_float4(o[j][0], o[j][1], o[j][2], o[j][3]);
-    __syncthreads();
-    float weight[kKv8Warps][2], top[2], sum[2];
+    for (int r = 0; r < NR; ++r) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      float2 ml[kKv8Warps];
-      top[r] = minus_inf;
-      sum[r] = 0.f;
-#pragma unroll
-      for (int w = 0; w < kKv8Warps; ++w) {
-        ml[w] = warp_ml[w][g + 8 * r];
-        top[r] = fmaxf(top[r], ml[w].x);
-      }
-#pragma unroll
-      for (int w = 0; w < kKv8Warps; ++w) {
-        weight[w][r] = ml[w].x == minus_inf ? 0.f : fast_exp2(ml[w].x - top[r]);
-        sum[r] += ml[w].x == minus_inf && ml[w].y == 0.f ? 0.f : weight[w][r] * ml[w].y;
-      }
+      for (int j = 0; j < S::MT; ++j)
+        join[(warp * S::FRAGS + r * S::MT + j) * 32 + lane] = make_float4(o[r][j][0], o[r][j][1], o[r][j][2], o[r][j][3]);
     }
-    constexpr int QUARTER = S::NT / kKv8Warps;
-    float4 acc[QUARTER];
+    __syncthreads();
+    const int frag0 = warp * S::SHARE;
+    const bool has_share = frag0 < S::FRAGS;
+    // the maximum and the sum of one row over n (max, sum) pairs, the pairs' weights
+    auto weigh = [&](const float2 (&ml)[kKv8Warps], float (&weight)[kKv8Warps]) {
+      float top = minus_inf, sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < QUARTER; ++i) {
-      const int j = warp * QUARTER + i;
-      acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int w = 0; w < kKv8Warps; ++w) top = fmaxf(top, ml[w].x);
+      const float from = top == minus_inf ? 0.f : top;
 #pragma unroll
       for (int w = 0; w < kKv8Warps; ++w) {
-        const float4 v = join[(w * S::NT + j) * 32 + lane];
-        acc[i].x = fmaf(weight[w][0], v.x, acc[i].x);
-        acc[i].y = fmaf(weight[w][0], v.y, acc[i].y);
-        acc[i].z = fmaf(weight[w][1], v.z, acc[i].z);
-        acc[i].w = fmaf(weight[w][1], v.w, acc[i].w);
+        weight[w] = fast_exp2(ml[w].x - from);
+        sum = fmaf(weight[w], ml[w].y, sum);
+      }
+      return make_float2(top, sum);
+    };
+    float4 acc[S::SHARE];
+    float2 ml_out[S::SHARE][2];
+#pragma unroll
+    for (int i = 0; i < S::SHARE; ++i) {
+      const int r = (frag0 + i) / S::MT;
+      float weight[2][kKv8Warps];
+      acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (!has_share) continue;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float2 ml[kKv8Warps];
+#pragma unroll
+        for (int w = 0; w < kKv8Warps; ++w) ml[w] = warp_ml[w][r * 8 + 2 * t4 + e];
+        ml_out[i][e] = weigh(ml, weight[e]);
+      }
+#pragma unroll
+      for (int w = 0; w < kKv8Warps; ++w) {
+        const float4 v = join[(w * S::FRAGS + frag0 + i) * 32 + lane];
+        acc[i].x = fmaf(weight[0][w], v.x, acc[i].x);
+        acc[i].y = fmaf(weight[1][w], v.y, acc[i].y);
+        acc[i].z = fmaf(weight[0][w], v.z, acc[i].z);
+        acc[i].w = fmaf(weight[1][w], v.w, acc[i].w);
       }
     }
 
     // ---- a tile in several CTAs: leave the part, the last to arrive joins them
     bool write = step0 == 0 && step1 == seq.steps;
     if (!write) {
-      const int64_t c0 = ((tile_begin + 1) * ctas - 1) / total;
-      const int64_t c1 = ((tile_begin + seq.steps) * ctas - 1) / total;
+      const unsigned c0 = ranges.of(tile_begin + kKv8TileCost);
+      const unsigned c1 = ranges.of(tile_begin + cost - 1);
       const int n_parts = static_cast<int>(c1 - c0) + 1;
-      float* part = a.parts + (static_cast<int64_t>(blockIdx.x) * 2 + (cur == lo ? 0 : 1)) * S::PART_FLOATS;
+      float* part = a.parts + (static_cast<int64_t>(blockIdx.x) * 2 + which) * S::PART_FLOATS;
+      if (has_share) {
 #pragma unroll
-      for (int i = 0; i < QUARTER; ++i)
-        __stcg(reinterpret_cast<float4*>(part) + (warp * QUARTER + i) * 32 + lane, acc[i]);
-      if (warp == 0 && t4 == 0) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-          __stcg(reinterpret_cast<float2*>(part + kKv8Rows * D) + g + 8 * r, make_float2(top[r], sum[r]));
+        for (int i = 0; i < S::SHARE; ++i) {
+          __stcg(reinterpret_cast<float4*>(part) + (frag0 + i) * 32 + lane, acc[i]);
+          if ((frag0 + i) % S::MT == 0 && g == 0) {
+            const int row = (frag0 + i) / S::MT * 8 + 2 * t4;
+            __stcg(reinterpret_cast<float4*>(part + S::ROWS * D + 2 * row),
+                   make_float4(ml_out[i][0].x, ml_out[i][0].y, ml_out[i][1].x, ml_out[i][1].y));
+          }
+        }
       }
-      __threadfence();
       __syncthreads();
       if (tid == 0) {
-        const unsigned int had = atomicAdd(a.arrivals + c0, 1u);
+        // releases the CTA's part (ordered before by the barrier), acquires the others'
+        unsigned int had;
+        asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(had) : "l"(a.arrivals + c0) : "memory");
         is_last = had + 1 == static_cast<unsigned int>(n_parts);
         if (is_last) a.arrivals[c0] = 0;  // ready for the next launch
       }
       __syncthreads();
       write = is_last;
-      if (write) {
-        __threadfence();
-        const int64_t first_lo = total * c0 / ctas;
-        auto part_of = [&](int i) {
-          const int which = i == 0 && first_lo != tile_begin ? 1 : 0;
-          return a.parts + ((c0 + i) * 2 + which) * S::PART_FLOATS;
-        };
-        // every row's maximum and sum over the parts; the parts' weights go to shared memory
-        float2* const ml = reinterpret_cast<float2*>(smem);
-        const int row = tid % kKv8Rows, lane8 = tid / kKv8Rows;
-        float best = minus_inf;
-        for (int i = lane8; i < n_parts; i += 8) {
-          const float2 v = __ldcg(reinterpret_cast<const float2*>(part_of(i) + kKv8Rows * D) + row);
-          ml[i * kKv8Rows + row] = v;
-          best = fmaxf(best, v.x);
+      if (write && has_share) {
+        // The parts in the order of the ranges, kAhead at a time with all loads
+        // in flight: the latency of L2 is what this costs.
+        constexpr int kAhead = S::SHARE == 1 ? 16 : S::SHARE == 2 ? 8 : 4;
+        // in the tile's first CTA it is the second part if the range begins before the tile
+        const float* first_part = a.parts + (static_cast<int64_t>(c0) * 2 + (ranges.begin(c0) < tile_begin ? 1 : 0)) * S::PART_FLOATS;
+        const float* next_part = a.parts + static_cast<int64_t>(c0) * 2 * S::PART_FLOATS;
+        float top[S::SHARE][2];
+#pragma unroll
+        for (int i = 0; i < S::SHARE; ++i) {
+          acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+          ml_out[i][0].y = ml_out[i][1].y = 0.f;
+          top[i][0] = top[i][1] = minus_inf;
         }
-        row_part[lane8][row] = best;
-        __syncthreads();
+#pragma unroll 1
+        for (int n0 = 0; n0 < n_parts; n0 += kAhead) {
+          float4 v[kAhead][S::SHARE], ml[kAhead][S::SHARE];  // ml: (max, sum) of rows 2 t and 2 t + 1
 #pragma unroll
-        for (int i = 0; i < 8; ++i) best = fmaxf(best, row_part[i][row]);
-        __syncthreads();
-        float part_sum = 0.f;
-        for (int i = lane8; i < n_parts; i += 8) {
-          const float2 v = ml[i * kKv8Rows + row];
-          const float w = v.x == minus_inf ? 0.f : fast_exp2(v.x - best);
-          part_sum += v.x == minus_inf && v.y == 0.f ? 0.f : w * v.y;
-          ml[i * kKv8Rows + row].x = w;
-        }
-        row_part[lane8][row] = part_sum;
-        __syncthreads();
-        if (tid < kKv8Rows) {
-          float s = 0.f;
+          for (int n = 0; n < kAhead; ++n) {
+            const float* part_n = n0 + n == 0 ? first_part : next_part + static_cast<int64_t>(n0 + n) * 2 * S::PART_FLOATS;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) s += row_part[i][tid];
-          row_sum[tid] = s;
-        }
-        __syncthreads();
-        sum[0] = row_sum[g];
-        sum[1] = row_sum[g + 8];
+            for (int i = 0; i < S::SHARE; ++i) {
+              v[n][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+              ml[n][i] = make_float4(minus_inf, 0.f, minus_inf, 0.f);
+              if (n0 + n < n_parts) {
+                v[n][i] = __ldcg(reinterpret_cast<const float4*>(part_n) + (frag0 + i) * 32 + lane);
+                ml[n][i] = __ldcg(reinterpret_cast<const float4*>(part_n + S::ROWS * D) + (frag0 + i) / S::MT * 4 + t4);
+              }
+            }
+          }
 #pragma unroll
-        for (int i = 0; i < QUARTER; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int i = 0; i < n_parts; ++i) {
-          const float w0 = ml[i * kKv8Rows + g].x, w1 = ml[i * kKv8Rows + g + 8].x;
-          const float4* src = reinterpret_cast<const float4*>(part_of(i)) + warp * QUARTER * 32 + lane;
+          for (int i = 0; i < S::SHARE; ++i) {
+            float next[2] = {top[i][0], top[i][1]}, from[2];
 #pragma unroll
-          for (int j = 0; j < QUARTER; ++j) {
-            const float4 v = __ldcg(src + j * 32);
-            acc[j].x = fmaf(w0, v.x, acc[j].x);
-            acc[j].y = fmaf(w0, v.y, acc[j].y);
-            acc[j].z = fmaf(w1, v.z, acc[j].z);
-            acc[j].w = fmaf(w1, v.w, acc[j].w);
+            for (int n = 0; n < kAhead; ++n) {
+              next[0] = fmaxf(next[0], ml[n][i].x);
+              next[1] = fmaxf(next[1], ml[n][i].z);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              from[e] = next[e] == minus_inf ? 0.f : next[e];
+              const float by = fast_exp2(top[i][e] - from[e]);
+              top[i][e] = next[e];
+              ml_out[i][e].y *= by;
+              (e ? acc[i].y : acc[i].x) *= by;
+              (e ? acc[i].w : acc[i].z) *= by;
+            }
+#pragma unroll
+            for (int n = 0; n < kAhead; ++n) {
+              const float w0 = fast_exp2(ml[n][i].x - from[0]), w1 = fast_exp2(ml[n][i].z - from[1]);
+              ml_out[i][0].y = fmaf(w0, ml[n][i].y, ml_out[i][0].y);
+              ml_out[i][1].y = fmaf(w1, ml[n][i].w, ml_out[i][1].y);
+              acc[i].x = fmaf(w0, v[n][i].x, acc[i].x);
+              acc[i].y = fmaf(w1, v[n][i].y, acc[i].y);
+              acc[i].z = fmaf(w0, v[n][i].z, acc[i].z);
+              acc[i].w = fmaf(w1, v[n][i].w, acc[i].w);
+            }
           }
         }
       }
     }
-    if (write) {
+    if (write && has_share) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = g + 8 * r;
-        if (row >= rows) continue;
-        const int token = (row0 + row) / a.group;
-        const bool real = token < seq.count && sum[r] != 0.f;  // padding rows are zero
-        const float by = real ? 1.f / sum[r] : 0.f;
-        __nv_bfloat16* dst = a.out + ((static_cast<int64_t>(b) * a.tokens + token) * a.heads + head * a.group +
-                                      (row0 + row) % a.group) * D;
+      for (int i = 0; i < S::SHARE; ++i) {
+        const int r = (frag0 + i) / S::MT, j = (frag0 + i) % S::MT;
+        // fragment j has bytes 2 j' and 2 j' + 1 of copy c of lane g
+        const int d = j / (S::VB / 2) * 128 + g * S::VB + j % (S::VB / 2) * 2;
 #pragma unroll
-        for (int i = 0; i < QUARTER; ++i) {
-          const int j = warp * QUARTER + i;  // dims c * 128 + n * VB + j % VB of columns n = 2t, 2t + 1
-          const int d = j / S::VB * 128 + j % S::VB;
-          dst[d + (2 * t4) * S::VB] = __float2bfloat16_rn(real ? (r ? acc[i].z : acc[i].x) * by : 0.f);
-          dst[d + (2 * t4 + 1) * S::VB] = __float2bfloat16_rn(real ? (r ? acc[i].w : acc[i].y) * by : 0.f);
+        for (int e = 0; e < 2; ++e) {
+          const int row = row0 + r * 8 + 2 * t4 + e;
+          if (row >= a.tokens * a.group) continue;
+          const int token = row / a.group;
+          const float sum = ml_out[i][e].y;
+          const bool real = token < seq.count && sum != 0.f;  // padding rows are zero
+          const float by = real ? 1.f / sum : 0.f;
+          const uint32_t two = real ? pack_bf16x2((e ? acc[i].y : acc[i].x) * by, (e ? acc[i].w : acc[i].z) * by) : 0u;
+          *reinterpret_cast<uint32_t*>(a.out + ((static_cast<int64_t>(b) * a.tokens + token) * a.heads + head * a.group +
+                                                row % a.group) * D + d) = two;
         }
       }
     }
     __syncthreads();  // the ring and the shared rows are free again
-    cur = tile_begin + step1;
   }
 }
 
