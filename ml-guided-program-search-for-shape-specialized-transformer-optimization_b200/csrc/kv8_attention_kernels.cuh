@@ -18,10 +18,13 @@
 // one that finishes last, in the order of the ranges, so results do not
 // depend on the order of arrival.
 //
-// Within a CTA the steps of a tile go round the four warps.  Each lane copies
-// exactly the bytes that it will use itself (cp.async into its own place of a
-// ring in shared memory): a queue with neither barriers nor bank conflicts,
-// deep enough to cover the HBM latency.
+// Within a CTA the steps of a tile go round the four warps.  Each warp has a ring
+// of steps in shared memory of its own, filled by cp.async: no barrier between
+// warps, deep enough to cover the HBM latency.  A copy of 8 lanes is one
+// 128-byte line; with the lanes in the fragments' order instead (rows 2 t for
+// values) the same loads took 67 us where these take 52 (16 sequences x 8192
+// tokens, 8 heads of 128).  Within a line the 16-byte chunks are permuted by
+// the row, so that the fragments are read without bank conflicts.
 //
 // Products.  Keys and values are the A operand (16 tokens, or 16 dims), queries
 // and probabilities the B operand (8 rows), so that 8 rows cost one MMA and a
@@ -102,15 +105,10 @@ __device__ __forceinline__ void cp_async(uint32_t dst, const void* src) {
   }
 }
 
-// What is not taken is written as zero, and not read.
-template <int BYTES>
+// 16 bytes; what is not taken is written as zero, and not read.
 __device__ __forceinline__ void cp_async_or_zero(uint32_t dst, const void* src, bool take) {
-  const int n = take ? BYTES : 0;
-  if constexpr (BYTES == 16) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-  } else {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
-  }
+  const int n = take ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -166,6 +164,27 @@ __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[BYTES 
   } else {
     w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
+}
+
+// Where byte `at` of a step's keys or values lies in its half of a stage: chunk
+// bits (4..6) exchanged by row bits.  All are linear over exclusive or, so a
+// lane's part and a constant part are permuted apart.
+template <int D>
+__host__ __device__ constexpr uint32_t kv8_k_place(uint32_t at) {  // rows of D codes, read 8 rows x 4 chunks
+  return D >= 128 ? at ^ (((at / D) & 1u) << 6) : at;
+}
+template <int D>
+__host__ __device__ constexpr uint32_t kv8_v_place(uint32_t at) {  // read rows {0, 2, 4, 6} x 2 chunks
+  return D >= 128 ? at ^ (((at / (2 * D)) & 3u) << 5) : D == 64 ? at ^ (((at >> 7) & 3u) << 5) : at ^ (((at >> 7) & 1u) << 5);
+}
+template <int D>
+__host__ __device__ constexpr uint32_t kv8_tail_k_place(uint32_t at) {  // rows of D bf16, read every other chunk
+  return D >= 64 ? at ^ (((at / (2 * D)) & 1u) << 4) : at;
+}
+template <int D>
+__host__ __device__ constexpr uint32_t kv8_tail_v_place(uint32_t at) {
+  const uint32_t pair = at / (4 * D);
+  return D >= 64 ? at ^ (((pair & 1u) << 4) | ((pair & 2u) << 5)) : at;
 }
 
 // What one sequence asks for: its tokens in all, and the steps over them.
@@ -331,41 +350,31 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
         }
         const int step = step0 + warp + kKv8Warps * k;
         int page = __shfl_sync(0xffffffffu, pages, k & 31);
-        uint8_t* const stage_at = ring + (k % S::STAGES) * S::STAGE;
-        const uint32_t k_stage = smem_u32(stage_at) + lane * S::KB;
-        const uint32_t v_stage = smem_u32(stage_at) + S::HALF + lane * S::VB;
+        const uint32_t stage = smem_u32(ring + (k % S::STAGES) * S::STAGE);
+        constexpr int COPIES = S::HALF / 512;  // of 16 bytes a lane
         if (step < coded_steps) {
           poisoned = poisoned || page < 0;
           page = max(page, 0);  // page 0 is always there
           const int64_t at = static_cast<int64_t>(page) * 2 * a.cache.kv_heads + head;
-          const uint8_t* block = a.cache.codes + at * kKv8Block * D + step % (kKv8Block / S::TOK) * S::HALF;
-          const uint8_t* kp = block + g * D + t4 * S::KB;
-          const uint8_t* vp = block + static_cast<int64_t>(a.cache.kv_heads) * kKv8Block * D + 2 * t4 * D + g * S::VB;
+          const uint8_t* kp = a.cache.codes + at * kKv8Block * D + step % (kKv8Block / S::TOK) * S::HALF + lane * 16;
+          const uint8_t* vp = kp + static_cast<int64_t>(a.cache.kv_heads) * kKv8Block * D;
 #pragma unroll
-          for (int x = 0; x < 2 * S::T16 * S::KC; ++x)
-            cp_async<S::KB>(k_stage + x * 32 * S::KB, kp + x / S::KC * 8 * D + x % S::KC * 64);
+          for (int x = 0; x < COPIES; ++x) cp_async<16>(stage + kv8_k_place<D>(lane * 16) + x * 512, kp + x * 512);
 #pragma unroll
-          for (int x = 0; x < 4 * S::T16 * S::VC; ++x) {  // tokens 16 (i / 4) + {2t, 2t+1, 2t+8, 2t+9}
-            const int i = x / S::VC;
-            cp_async<S::VB>(v_stage + x * 32 * S::VB,
-                            vp + ((i / 4) * 16 + (i & 1) + ((i >> 1) & 1) * 8) * D + x % S::VC * 128);
-          }
-          if (lane < 2) cp_async<4>(smem_u32(stage_at) + 2 * S::HALF + 4 * lane, a.cache.scales + at + lane * a.cache.kv_heads);
+          for (int x = 0; x < COPIES; ++x)
+            cp_async<16>(stage + S::HALF + (kv8_v_place<D>(lane * 16) ^ (kv8_v_place<D>(x * 512) & 511u)) + x * 512, vp + x * 512);
+          if (lane < 2) cp_async<4>(stage + 2 * S::HALF + 4 * lane, a.cache.scales + at + lane * a.cache.kv_heads);
         } else {
           const int first = (step - coded_steps) * S::TAIL;
-          const __nv_bfloat16* kp = kv8_tail(a.cache, seq.slot, full & 1, 0, head, D) + (first + g) * D + t4 * S::KB;
-          const __nv_bfloat16* vp = kv8_tail(a.cache, seq.slot, full & 1, 1, head, D) + (first + 2 * t4) * D + g * S::VB;
+          const __nv_bfloat16* kp = kv8_tail(a.cache, seq.slot, full & 1, 0, head, D) + first * D + lane * 8;
+          const __nv_bfloat16* vp = kv8_tail(a.cache, seq.slot, full & 1, 1, head, D) + first * D + lane * 8;
 #pragma unroll
-          for (int x = 0; x < 2 * S::T16 * S::KC; ++x) {
-            const int n = x / (2 * S::KC), c = x / 2 % S::KC, h = x % 2;
-            cp_async_or_zero<S::KB>(k_stage + x * 32 * S::KB, kp + n * 8 * D + c * 64 + h * (S::KB / 2), first + g + n * 8 < open);
-          }
-#pragma unroll
-          for (int x = 0; x < 4 * S::T16 * S::VC; ++x) {
-            const int i = x / (2 * S::VC), c = x / 2 % S::VC, h = x % 2;
-            const int token = (i / 4) * 16 + (i & 1) + ((i >> 1) & 1) * 8;
-            cp_async_or_zero<S::VB>(v_stage + x * 32 * S::VB, vp + token * D + c * 128 + h * (S::VB / 2),
-                                    first + 2 * t4 + token < open);
+          for (int x = 0; x < COPIES; ++x) {
+            const bool take = first + (x * 256 + lane * 8) / D < open;
+            cp_async_or_zero(stage + (kv8_tail_k_place<D>(lane * 16) ^ (kv8_tail_k_place<D>(x * 512) & 511u)) + x * 512,
+                             kp + x * 256, take);
+            cp_async_or_zero(stage + S::HALF + (kv8_tail_v_place<D>(lane * 16) ^ (kv8_tail_v_place<D>(x * 512) & 511u)) + x * 512,
+                             vp + x * 256, take);
           }
         }
       }
@@ -490,6 +499,10 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
       }
     };
 
+    // a lane's place in a step: the parts of its fragments that do not depend on the step
+    const uint32_t k_at = kv8_k_place<D>(g * D + t4 * S::KB), v_at = kv8_v_place<D>(2 * t4 * D + g * S::VB);
+    const uint32_t tail_k_at = kv8_tail_k_place<D>(g * 2 * D + t4 * 2 * S::KB);
+    const uint32_t tail_v_at = kv8_tail_v_place<D>(2 * t4 * 2 * D + g * 2 * S::VB);
 #pragma unroll 1
     for (int k = 0; k < mine_steps; ++k) {
       cp_async_wait<S::STAGES - 2>();
@@ -505,7 +518,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
         for (int c = 0; c < S::KC; ++c) {
           uint32_t w[2 * S::T16][S::KB / 4];
 #pragma unroll
-          for (int n = 0; n < 2 * S::T16; ++n) lds_words<S::KB>(stage + ((n * S::KC + c) * 32 + lane) * S::KB, w[n]);
+          for (int n = 0; n < 2 * S::T16; ++n) lds_words<S::KB>(stage + (k_at ^ (c * 64)) + n * 8 * D, w[n]);
 #pragma unroll
           for (int i = 0; i < S::KB / 4; ++i) {
             const int ks = c * (S::KB / 4) + i;
@@ -561,8 +574,10 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
         for (int c = 0; c < S::VC; ++c) {
           uint32_t w[4 * S::T16][S::VB / 4];
 #pragma unroll
-          for (int i = 0; i < 4 * S::T16; ++i)
-            lds_words<S::VB>(stage + S::HALF + ((i * S::VC + c) * 32 + lane) * S::VB, w[i]);
+          for (int i = 0; i < 4 * S::T16; ++i) {  // tokens 16 (i / 4) + {2t, 2t + 1, 2t + 8, 2t + 9}
+            const uint32_t at = D <= 64 ? v_at ^ ((i & 1) * D) : v_at + (i & 1) * D;
+            lds_words<S::VB>(stage + S::HALF + at + ((i / 4) * 16 + (i >> 1 & 1) * 8) * D + c * 128, w[i]);
+          }
 #pragma unroll
           for (int i = 0; i < S::VB / 4; ++i) {
 #pragma unroll
@@ -600,7 +615,8 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
         for (int c = 0; c < 2 * S::KC; ++c) {
           uint32_t w[2 * TT][S::KB / 4];
 #pragma unroll
-          for (int n = 0; n < 2 * TT; ++n) lds_words<S::KB>(stage + ((n * 2 * S::KC + c) * 32 + lane) * S::KB, w[n]);
+          for (int n = 0; n < 2 * TT; ++n)
+            lds_words<S::KB>(stage + (tail_k_at ^ (c % 2 * S::KB)) + c / 2 * 128 + n * 16 * D, w[n]);
 #pragma unroll
           for (int i = 0; i < S::KB / 8; ++i) {
             const int ks = c * (S::KB / 8) + i;
@@ -660,11 +676,11 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
         bool odd = false;
         if (seq.count > 1 && first_token + S::TAIL - 1 > least) {
 #pragma unroll
-          for (int i = 0; i < 4 * S::T16 * S::VC; ++i) {
-            uint32_t w[S::VB / 4];
-            lds_words<S::VB>(stage + S::HALF + (i * 32 + lane) * S::VB, w);
+          for (int i = 0; i < S::HALF / 512; ++i) {
+            uint32_t w[4];
+            lds_words<16>(stage + S::HALF + i * 512 + lane * 16, w);
 #pragma unroll
-            for (int e = 0; e < S::VB / 4; ++e)
+            for (int e = 0; e < 4; ++e)
               odd = odd || (w[e] & 0x7f80u) == 0x7f80u || (w[e] & 0x7f800000u) == 0x7f800000u;
           }
           odd = __any_sync(0xffffffffu, odd);
@@ -677,7 +693,8 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
               uint32_t w[4 * TT][S::VB / 4];
 #pragma unroll
               for (int i = 0; i < 4 * TT; ++i)
-                lds_words<S::VB>(stage + S::HALF + (((i * S::VC + c) * 2 + h) * 32 + lane) * S::VB, w[i]);
+                lds_words<S::VB>(stage + S::HALF + (tail_v_at ^ (h * S::VB)) + c * 256 +
+                                     ((i / 4) * 16 + (i & 1) + (i >> 1 & 1) * 8) * 2 * D, w[i]);
 #pragma unroll
               for (int i = 0; i < S::VB / 4; ++i) {
 #pragma unroll
@@ -707,14 +724,12 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
             __syncwarp();
 #pragma unroll 1
             for (int token = 0; token < 16; ++token) {
-              // token = 2 t' + (i & 1) + (i >> 1) * 8 lies with lanes t' in copy 4 t + i
-              const int from_t = (token % 8) / 2, i = 4 * t + (token & 1) + (token / 8) * 2;
               const int where = first_token + 16 * t + token;
 #pragma unroll
               for (int j = 0; j < S::MT; ++j) {
                 const int c = j / (S::VB / 2), h = j % (S::VB / 2) / (S::VB / 4), at = j % (S::VB / 4);
                 const uint32_t two = *reinterpret_cast<const uint32_t*>(
-                    stage + S::HALF + (((i * S::VC + c) * 2 + h) * 32 + g * 4 + from_t) * S::VB + 4 * at);
+                    stage + S::HALF + kv8_tail_v_place<D>((16 * t + token) * 2 * D + (c * 128 + g * S::VB) * 2 + h * S::VB + 4 * at));
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                   const float v = __uint_as_float(e < 2 ? two << 16 : two & 0xffff0000u);
