@@ -162,29 +162,46 @@ cudaError_t launch_kv8_attention(b200tx::Kv8AttnArgs& a, DeviceState* dev, int i
                 dim3(b200tx::kKv8Warps * 32), S::MAIN, stream, a);
 }
 
-template <int TN, int GROUP>
-cudaError_t launch_w4(b200tx::W4Args& a, int out_dtype, int sm_count, cudaStream_t stream) {
-  // Warps of a CTA along K: the fewest (they are joined at the end) that leave
-  // two CTAs for each SM.
-  const int tiles = (a.outer + 15) / 16;
-  a.split = 1;
-  while (a.split < b200tx::kW4Warps && a.split < a.runs &&
-         (tiles * a.split + b200tx::kW4Warps - 1) / b200tx::kW4Warps < 2 * sm_count)
-    a.split *= 2;
-  const int per = b200tx::kW4Warps / a.split;
+template <int TN, int RT, int GROUP>
+cudaError_t launch_w4(b200tx::W4Args& a, DeviceState* dev, int index, cudaStream_t stream) {
+  constexpr int kMost = 112 * 1024;  // two CTAs for each SM
+  if (!dev->w4_attr[index]) {
+    cudaError_t err =
+        cudaFuncSetAttribute(b200tx::linear_w4_kernel<TN, RT, GROUP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+    if (err != cudaSuccess) return err;
+    dev->w4_attr[index] = true;
+  }
+  // Slices of K: the fewest (they are joined at the end) that give every SM a CTA.
+  const int tiles = (a.outer + 16 * RT - 1) / (16 * RT), all_stages = (a.runs + 1) / 2;
+  a.slices = 1;
+  while (a.slices < b200tx::kW4Warps && a.slices < all_stages &&
+         (tiles * a.slices + b200tx::kW4Warps - 1) / b200tx::kW4Warps < dev->sm_count &&
+         2 * b200tx::w4_stage_bytes<TN, RT>(2 * a.slices) <= kMost)
+    a.slices *= 2;
+  const int stage = b200tx::w4_stage_bytes<TN, RT>(a.slices);
+  a.stages = 4 * stage <= kMost ? 4 : 3 * stage <= kMost ? 3 : 2;
+  const int join = b200tx::kW4Warps * RT * TN * 512;
+  const int per = b200tx::kW4Warps / a.slices;
   const dim3 grid(static_cast<unsigned>((tiles + per - 1) / per), static_cast<unsigned>((a.rows + TN * 8 - 1) / (TN * 8)));
-  if (out_dtype == B200TX_F32)
-    return launch(b200tx::linear_w4_kernel<TN, GROUP, float>, grid, dim3(b200tx::kW4Warps * 32), 0, stream, a);
-  return launch(b200tx::linear_w4_kernel<TN, GROUP, __nv_bfloat16>, grid, dim3(b200tx::kW4Warps * 32), 0, stream, a);
+  return launch(b200tx::linear_w4_kernel<TN, RT, GROUP>, grid, dim3(b200tx::kW4Warps * 32),
+                static_cast<size_t>(std::max(a.stages * stage, join)), stream, a);
 }
 
-template <int TN>
-cudaError_t launch_w4_group(int64_t group, b200tx::W4Args& a, int out_dtype, int sm_count, cudaStream_t stream) {
+template <int TN, int RT>
+cudaError_t launch_w4_group(int64_t group, b200tx::W4Args& a, DeviceState* dev, int index, cudaStream_t stream) {
   switch (group) {
-    case 32: return launch_w4<TN, 32>(a, out_dtype, sm_count, stream);
-    case 64: return launch_w4<TN, 64>(a, out_dtype, sm_count, stream);
-    default: return launch_w4<TN, 128>(a, out_dtype, sm_count, stream);
+    case 32: return launch_w4<TN, RT, 32>(a, dev, index, stream);
+    case 64: return launch_w4<TN, RT, 64>(a, dev, index + 1, stream);
+    default: return launch_w4<TN, RT, 128>(a, dev, index + 2, stream);
   }
+}
+
+// Column tiles of a warp: two where enough are left for every SM to have 8 warps
+// (x is read from shared memory once for both), else one.
+template <int TN>
+cudaError_t launch_w4_tiles(int64_t group, b200tx::W4Args& a, DeviceState* dev, int index, cudaStream_t stream) {
+  if (a.outer >= 32 * b200tx::kW4Warps * dev->sm_count / 2) return launch_w4_group<TN, 2>(group, a, dev, index, stream);
+  return launch_w4_group<TN, 1>(group, a, dev, index + 3, stream);
 }
 
 }  // namespace
@@ -428,10 +445,11 @@ int b200tx_linear_w4(const void* x, int64_t x_stride, const void* packed, const 
   a.inner = static_cast<int>(K);
   a.runs = static_cast<int>((K + b200tx::kW4Run - 1) / b200tx::kW4Run);
   a.gelu = epilogue == B200TX_EPI_BIAS_GELU;
+  a.out_f32 = out_dtype == B200TX_F32;
   // rows of x by eights: 1, 2 or 4 MMA columns; past 32 the weights are read again
-  cudaError_t err = M <= 8    ? launch_w4_group<1>(group, a, out_dtype, dev->sm_count, stream)
-                    : M <= 16 ? launch_w4_group<2>(group, a, out_dtype, dev->sm_count, stream)
-                              : launch_w4_group<4>(group, a, out_dtype, dev->sm_count, stream);
+  cudaError_t err = M <= 8    ? launch_w4_tiles<1>(group, a, dev, 0, stream)
+                    : M <= 16 ? launch_w4_tiles<2>(group, a, dev, 6, stream)
+                              : launch_w4_tiles<4>(group, a, dev, 12, stream);
   return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "linear_w4");
 }
 

@@ -3,28 +3,33 @@
 //   W[n, k] = scale[k / group, n] * (code[n, k] - 8),   code in 0..15
 //
 // What bounds it: with up to 32 rows the weights' bytes over HBM, N K / 2 (and
-// 2 N K / group of scales).
+// 2 N K / group of scales); next to it the instructions that turn codes into
+// numbers, 11 for a word of 8.
 //
 // Layout.  A word is 8 consecutive weights of a row, ordered so that one mask
 // takes two neighbours (nibble i holds weight {0,2,4,6,1,3,5,7}[i]): the
 // nibbles under bf16's 128.0 are 128 + code, and subtracting 136 is exact.  A run of
 // 128 weights is 16 words, word (a, b) of the 4 x 4 stored at (b, a): lane t of
-// a quad loads 16 bytes and has words of four consecutive 32-weight pieces,
+// a quad reads 16 bytes and has words of four consecutive 32-weight pieces,
 // so that whatever the group is, a product of the tensor core stays within one.
 //
 // The weights are the A operand (m16: output columns), x the B operand (n8: rows
-// of x), so 8 rows of x cost one MMA.  Weights go from HBM to registers to the
-// tensor core without shared memory; x comes from L1.  The sum of a group is
-// multiplied by its scale and added in fp32.  A CTA is 8 warps: column tiles x
-// splits of K (runs dealt in turn), joined in shared memory in a fixed order.
+// of x), so 8 rows of x cost one MMA.  A CTA is 8 warps: 8 / KS tiles of 16 RT
+// columns x KS slices of K.  A slice goes through K 256 weights at a time, weights
+// and x by cp.async into a ring (8 lanes copy one 128-byte line, chunks permuted by
+// the row so that the fragments are read without bank conflicts); its warps
+// share x.  The sum of a group is multiplied by its scale and added in fp32; the
+// slices are joined in shared memory in a fixed order.
 #pragma once
 
 #include "attention_mma_kernels.cuh"
+#include "kv8_attention_kernels.cuh"
 
 namespace b200tx {
 
 constexpr int kW4Warps = 8;
-constexpr int kW4Run = 128;  // weights of a row that lie together
+constexpr int kW4Run = 128;    // weights of a row that lie together
+constexpr int kW4Stage = 256;  // weights of a row in a stage
 
 struct W4Args {
   const __nv_bfloat16* x;        // [M, K]
@@ -34,8 +39,9 @@ struct W4Args {
   void* out;                     // [M, N]
   int64_t x_stride;
   int rows, outer, inner, runs;
-  int gelu;
-  int split;                     // warps along K, a power of two up to 8
+  int gelu, out_f32;
+  int slices;                    // warps along K, a power of two up to 8
+  int stages;                    // of the ring
 };
 
 __device__ __forceinline__ uint32_t nibbles_bf16x2(uint32_t w) {
@@ -45,121 +51,186 @@ __device__ __forceinline__ uint32_t nibbles_bf16x2(uint32_t w) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// TN: n8 tiles of x rows; AHEAD: runs whose loads are in flight together.
-template <int TN, int GROUP, typename OutT>
-__global__ void __launch_bounds__(kW4Warps * 32) linear_w4_kernel(W4Args a) {
-  constexpr int AHEAD = TN == 4 ? 2 : 4;
+// Bytes of a ring stage: 8 warps' weights, then the slices' x.
+template <int TN, int RT>
+constexpr int w4_stage_bytes(int slices) {
+  return kW4Warps * RT * 16 * (kW4Stage / 2) + slices * TN * 8 * kW4Stage * 2;
+}
+
+// TN: n8 tiles of x rows; RT: m16 tiles of columns of a warp.
+template <int TN, int RT, int GROUP>
+__global__ void __launch_bounds__(kW4Warps * 32, 2) linear_w4_kernel(W4Args a) {
   constexpr int GROUPS = kW4Run / GROUP;  // groups per run
   constexpr int WORDS = 4 / GROUPS;       // words per group and lane
-  __shared__ float4 join[kW4Warps][TN][32];
+  constexpr int W_BYTES = RT * 16 * (kW4Stage / 2);  // of a warp's stage
+  constexpr int X_BYTES = TN * 8 * kW4Stage * 2;     // of a slice's stage
+  extern __shared__ __align__(128) uint8_t w4_smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t4 = lane % 4;
-  const int part = warp % a.split, tile = warp / a.split;
-  const int n0 = (blockIdx.x * (kW4Warps / a.split) + tile) * 16;
+  const int per = kW4Warps / a.slices;  // warps of a slice
+  const int slice = warp / per, tile = warp % per;
+  const int n0 = (blockIdx.x * per + tile) * (16 * RT);
   const int m0 = blockIdx.y * (TN * 8);
-  // columns past the end read the last one and are not written
-  const int col[2] = {min(n0 + g, a.outer - 1), min(n0 + g + 8, a.outer - 1)};
-  const int64_t pitch = static_cast<int64_t>(a.runs) * (kW4Run / 2);
-  const uint8_t* w_row[2] = {a.packed + col[0] * pitch + t4 * 16, a.packed + col[1] * pitch + t4 * 16};
+  const int stage_bytes = kW4Warps * W_BYTES + a.slices * X_BYTES;
+  const int all_stages = (a.runs + 1) / 2, each = (all_stages + a.slices - 1) / a.slices;
+  const int begin = min(all_stages, slice * each), count = min(all_stages, begin + each) - begin;
   griddep_wait();
   griddep_launch_dependents();
 
-  const __nv_bfloat16* x_row[TN];
-  bool x_in[TN];
+  // ---- copies: 4 rows x 128 bytes of weights at a time, and this thread's share of the slice's x
+  const int64_t pitch = static_cast<int64_t>(a.runs) * (kW4Run / 2);
+  const int first_row = min(n0, a.outer - 1);  // columns past the end read the last one and are not written
+  const uint8_t* const w_src = a.packed + first_row * pitch + lane % 8 * 16;
+  unsigned w_off[RT * 4];
 #pragma unroll
-  for (int i = 0; i < TN; ++i) {
-    const int m = m0 + i * 8 + g;
-    x_in[i] = m < a.rows;
-    x_row[i] = a.x + (x_in[i] ? m : 0) * a.x_stride + t4 * 8;
-  }
-
-  float sum[TN][4];
+  for (int i = 0; i < RT * 4; ++i)
+    w_off[i] = static_cast<unsigned>(min(n0 + i * 4 + lane / 8, a.outer - 1) - first_row) * static_cast<unsigned>(pitch);
+  const uint32_t ring = smem_u32(w4_smem);
+  const uint32_t w_put = ring + warp * W_BYTES + kv8_k_place<128>(lane * 16);
+  auto issue = [&](int s) {
+    if (s < count) {
+      const int at = begin + s;
+      const uint32_t stage = (s % a.stages) * stage_bytes;
+      const bool take = at * 2 + (lane % 8) / 4 < a.runs;
 #pragma unroll
-  for (int i = 0; i < TN; ++i) sum[i][0] = sum[i][1] = sum[i][2] = sum[i][3] = 0.f;
-
-  for (int r0 = part; r0 < a.runs; r0 += a.split * AHEAD) {
-    uint4 w[AHEAD][2];
-    __nv_bfloat16 s[AHEAD][GROUPS][2];
-#pragma unroll
-    for (int p = 0; p < AHEAD; ++p) {
-      const int r = r0 + p * a.split;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        w[p][h] = make_uint4(0u, 0u, 0u, 0u);
-        if (r < a.runs) w[p][h] = __ldg(reinterpret_cast<const uint4*>(w_row[h] + static_cast<int64_t>(r) * (kW4Run / 2)));
-#pragma unroll
-        for (int q = 0; q < GROUPS; ++q) {
-          s[p][q][h] = __ushort_as_bfloat16(0);
-          if (r < a.runs) s[p][q][h] = a.scales[static_cast<int64_t>(r * GROUPS + q) * a.outer + col[h]];
-        }
+      for (int i = 0; i < RT * 4; ++i)
+        cp_async_or_zero(w_put + stage + i * 512, w_src + w_off[i] + static_cast<int64_t>(at) * 128, take);
+      // x: 32 chunks of 16 bytes a row, a warp copies whole rows
+      for (int row = tile; row < TN * 8; row += per) {
+        const int m = m0 + row, k = at * kW4Stage + lane * 8;
+        const bool in = m < a.rows && k < a.inner;
+        cp_async_or_zero(ring + stage + kW4Warps * W_BYTES + slice * X_BYTES + row * 512 + ((lane * 16) ^ ((row & 1) << 6)),
+                         a.x + (in ? m * a.x_stride + k : 0), in);
       }
     }
+    cp_async_commit();
+  };
+  for (int s = 0; s < a.stages - 1; ++s) issue(s);
+
+  // ---- scales: lane = a column of the tile, RT GROUPS registers for a stage's 2 GROUPS groups
+  constexpr int SCALES = RT * GROUPS;
+  const int s_col = min(n0 + lane % (16 * RT), a.outer - 1);
+  const int all_groups = a.runs * GROUPS;
+  auto load_scales = [&](int s, uint16_t (&to)[SCALES]) {
 #pragma unroll
-    for (int p = 0; p < AHEAD; ++p) {
-      const int r = r0 + p * a.split;
-      if (r >= a.runs) break;
-      const uint32_t wa[4] = {w[p][0].x, w[p][0].y, w[p][0].z, w[p][0].w};
-      const uint32_t wb[4] = {w[p][1].x, w[p][1].y, w[p][1].z, w[p][1].w};
+    for (int i = 0; i < SCALES; ++i) {
+      const int q = (begin + s) * 2 * GROUPS + (RT == 2 ? i : 2 * i + lane / 16);
+      to[i] = 0;
+      if (s < count && q < all_groups)
+        to[i] = __ldg(reinterpret_cast<const uint16_t*>(a.scales) + static_cast<int64_t>(q) * a.outer + s_col);
+    }
+  };
+  uint16_t scales[SCALES], next_scales[SCALES];
+  load_scales(0, scales);
+
+  float sum[RT][TN][4] = {};
+  const uint32_t w_get = warp * W_BYTES + kv8_k_place<128>(g * 128 + t4 * 16);
+  const uint32_t x_get = kW4Warps * W_BYTES + slice * X_BYTES + g * 512;
+  const uint32_t x_low = (t4 * 16) ^ ((g & 1) << 6);
+#pragma unroll 1
+  for (int s = 0; s < count; ++s) {
+    if (a.stages == 2) cp_async_wait<0>();
+    else if (a.stages == 3) cp_async_wait<1>();
+    else cp_async_wait<2>();
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + slice), "r"(per * 32) : "memory");
+    issue(s + a.stages - 1);
+    load_scales(s + 1, next_scales);
+    const uint8_t* const stage = w4_smem + (s % a.stages) * stage_bytes;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      uint32_t w[RT][2][4];
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        lds_words<16>(stage + (w_get ^ (r * 64)) + i * 2048, w[i][0]);
+        lds_words<16>(stage + (w_get ^ (r * 64)) + i * 2048 + 1024, w[i][1]);
+      }
 #pragma unroll
       for (int q = 0; q < GROUPS; ++q) {
-        float acc[TN][4] = {};
+        float acc[RT][TN][4];
 #pragma unroll
         for (int c = q * WORDS; c < (q + 1) * WORDS; ++c) {
-          const uint32_t a0[4] = {nibbles_bf16x2(wa[c]), nibbles_bf16x2(wb[c]), nibbles_bf16x2(wa[c] >> 4),
-                                  nibbles_bf16x2(wb[c] >> 4)};
-          const uint32_t a1[4] = {nibbles_bf16x2(wa[c] >> 8), nibbles_bf16x2(wb[c] >> 8), nibbles_bf16x2(wa[c] >> 12),
-                                  nibbles_bf16x2(wb[c] >> 12)};
-          const int k = r * kW4Run + c * 32;
+          uint32_t xf[TN][4];
 #pragma unroll
-          for (int i = 0; i < TN; ++i) {
-            uint4 x = make_uint4(0u, 0u, 0u, 0u);
-            if (x_in[i] && k + t4 * 8 < a.inner) x = *reinterpret_cast<const uint4*>(x_row[i] + k);
-            mma_m16n8k16_bf16(acc[i], a0, x.x, x.y);
-            mma_m16n8k16_bf16(acc[i], a1, x.z, x.w);
+          for (int j = 0; j < TN; ++j)
+            lds_words<16>(stage + x_get + (x_low ^ ((c & 1) << 6)) + (c >> 1) * 128 + r * 256 + j * 4096, xf[j]);
+#pragma unroll
+          for (int i = 0; i < RT; ++i) {
+            const uint32_t wa = w[i][0][c], wb = w[i][1][c];
+            const uint32_t a0[4] = {nibbles_bf16x2(wa), nibbles_bf16x2(wb), nibbles_bf16x2(wa >> 4), nibbles_bf16x2(wb >> 4)};
+            const uint32_t a1[4] = {nibbles_bf16x2(wa >> 8), nibbles_bf16x2(wb >> 8), nibbles_bf16x2(wa >> 12),
+                                    nibbles_bf16x2(wb >> 12)};
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+              if (c == q * WORDS) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.f;
+              mma_m16n8k16_bf16(acc[i][j], a0, xf[j][0], xf[j][1]);
+              mma_m16n8k16_bf16(acc[i][j], a1, xf[j][2], xf[j][3]);
+            }
           }
         }
-        const float s0 = __bfloat162float(s[p][q][0]), s1 = __bfloat162float(s[p][q][1]);
+        const int group = r * GROUPS + q;
 #pragma unroll
-        for (int i = 0; i < TN; ++i) {
-          sum[i][0] = fmaf(s0, acc[i][0], sum[i][0]);
-          sum[i][1] = fmaf(s0, acc[i][1], sum[i][1]);
-          sum[i][2] = fmaf(s1, acc[i][2], sum[i][2]);
-          sum[i][3] = fmaf(s1, acc[i][3], sum[i][3]);
+        for (int i = 0; i < RT; ++i) {
+          const uint32_t held = scales[RT == 2 ? group : group / 2];
+          const int from = RT == 2 ? i * 16 : group % 2 * 16;
+          const float s0 = __uint_as_float(__shfl_sync(0xffffffffu, held, from + g) << 16);
+          const float s1 = __uint_as_float(__shfl_sync(0xffffffffu, held, from + g + 8) << 16);
+#pragma unroll
+          for (int j = 0; j < TN; ++j) {
+            sum[i][j][0] = fmaf(s0, acc[i][j][0], sum[i][j][0]);
+            sum[i][j][1] = fmaf(s0, acc[i][j][1], sum[i][j][1]);
+            sum[i][j][2] = fmaf(s1, acc[i][j][2], sum[i][j][2]);
+            sum[i][j][3] = fmaf(s1, acc[i][j][3], sum[i][j][3]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < SCALES; ++i) scales[i] = next_scales[i];
+  }
+
+  if (a.slices > 1) {
+    cp_async_wait<0>();
+    __syncthreads();
+    float4* const join = reinterpret_cast<float4*>(w4_smem);  // [warp][RT * TN][32]
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+        join[(warp * RT * TN + i * TN + j) * 32 + lane] = make_float4(sum[i][j][0], sum[i][j][1], sum[i][j][2], sum[i][j][3]);
+    }
+    __syncthreads();
+    if (slice != 0) return;
+    for (int w = 1; w < a.slices; ++w) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const float4 v = join[((w * per + tile) * RT * TN + i * TN + j) * 32 + lane];
+          sum[i][j][0] += v.x; sum[i][j][1] += v.y; sum[i][j][2] += v.z; sum[i][j][3] += v.w;
         }
       }
     }
   }
-
-  if (a.split > 1) {
 #pragma unroll
-    for (int i = 0; i < TN; ++i) join[warp][i][lane] = make_float4(sum[i][0], sum[i][1], sum[i][2], sum[i][3]);
-    __syncthreads();
-    if (part != 0) return;
-    for (int w = 1; w < a.split; ++w) {
+  for (int i = 0; i < RT; ++i) {
 #pragma unroll
-      for (int i = 0; i < TN; ++i) {
-        const float4 v = join[warp + w][i][lane];
-        sum[i][0] += v.x; sum[i][1] += v.y; sum[i][2] += v.z; sum[i][3] += v.w;
-      }
-    }
-  }
+    for (int h = 0; h < 2; ++h) {
+      const int n = n0 + i * 16 + g + 8 * h;
+      if (n >= a.outer) continue;
+      const float bias = a.bias == nullptr ? 0.f : a.bias[n];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int n = n0 + g + 8 * h;
-    if (n >= a.outer) continue;
-    const float bias = a.bias == nullptr ? 0.f : a.bias[n];
+      for (int j = 0; j < TN; ++j) {
 #pragma unroll
-    for (int i = 0; i < TN; ++i) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int m = m0 + i * 8 + 2 * t4 + e;
-        if (m >= a.rows) continue;
-        float y = sum[i][2 * h + e] + bias;
-        if (a.gelu) y = 0.5f * y * (1.f + erff(y * 0.70710678118654752f));
-        OutT* dst = static_cast<OutT*>(a.out) + static_cast<int64_t>(m) * a.outer + n;
-        if constexpr (sizeof(OutT) == 4) {
-          *dst = y;
-        } else {
-          *dst = __float2bfloat16_rn(y);
+        for (int e = 0; e < 2; ++e) {
+          const int m = m0 + j * 8 + 2 * t4 + e;
+          if (m >= a.rows) continue;
+          float y = sum[i][j][2 * h + e] + bias;
+          if (a.gelu) y = 0.5f * y * (1.f + erff(y * 0.70710678118654752f));
+          const int64_t at = static_cast<int64_t>(m) * a.outer + n;
+          if (a.out_f32) {
+            static_cast<float*>(a.out)[at] = y;
+          } else {
+            static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y);
+          }
         }
       }
     }
