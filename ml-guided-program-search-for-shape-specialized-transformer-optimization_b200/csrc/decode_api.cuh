@@ -171,11 +171,13 @@ cudaError_t launch_w4(b200tx::W4Args& a, DeviceState* dev, int index, cudaStream
     if (err != cudaSuccess) return err;
     dev->w4_attr[index] = true;
   }
-  // Slices of K: the fewest (they are joined at the end) that give every SM a CTA.
+  // Slices of K: the fewest (they are joined at the end) that give most SMs a second
+  // CTA (1 x 8192 -> 8192: 128 CTAs 20.3 us, 256 CTAs 15.9; 8 x 8192 -> 28672:
+  // 224 CTAs 38.6 us, 448 CTAs 41.9).
   const int tiles = (a.outer + 16 * RT - 1) / (16 * RT), all_stages = (a.runs + 1) / 2;
   a.slices = 1;
   while (a.slices < b200tx::kW4Warps && a.slices < all_stages &&
-         (tiles * a.slices + b200tx::kW4Warps - 1) / b200tx::kW4Warps < dev->sm_count &&
+         (tiles * a.slices + b200tx::kW4Warps - 1) / b200tx::kW4Warps < dev->sm_count * 5 / 4 &&
          2 * b200tx::w4_stage_bytes<TN, RT>(2 * a.slices) <= kMost)
     a.slices *= 2;
   const int stage = b200tx::w4_stage_bytes<TN, RT>(a.slices);
@@ -196,11 +198,14 @@ cudaError_t launch_w4_group(int64_t group, b200tx::W4Args& a, DeviceState* dev, 
   }
 }
 
-// Column tiles of a warp: two where enough are left for every SM to have 8 warps
-// (x is read from shared memory once for both), else one.
+// Column tiles of a warp: two, sharing the x fragments, where the columns are many
+// (8 x 4096 -> 14336: one 13.8 us, two 12.9; 1 x 8192 -> 8192: one 15.9, two 18.9) and the
+// accumulators fit (32 x 4096 -> 14336: one 24.9 us, two 43.1).
 template <int TN>
 cudaError_t launch_w4_tiles(int64_t group, b200tx::W4Args& a, DeviceState* dev, int index, cudaStream_t stream) {
-  if (a.outer >= 32 * b200tx::kW4Warps * dev->sm_count / 2) return launch_w4_group<TN, 2>(group, a, dev, index, stream);
+  if constexpr (TN <= 2) {
+    if (a.outer >= 80 * dev->sm_count) return launch_w4_group<TN, 2>(group, a, dev, index, stream);
+  }
   return launch_w4_group<TN, 1>(group, a, dev, index + 3, stream);
 }
 

@@ -44,8 +44,12 @@ struct W4Args {
   int stages;                    // of the ring
 };
 
+// The lowest nibbles of both halves as bf16 numbers code - 8.  The mask and the
+// exponent are one three-input operation: these and the shifts run at half
+// rate and are what the kernel issues most.
 __device__ __forceinline__ uint32_t nibbles_bf16x2(uint32_t w) {
-  const uint32_t biased = (w & 0x000f000fu) | 0x43004300u;
+  uint32_t biased;
+  asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xEA;" : "=r"(biased) : "r"(w), "r"(0x43004300u));  // (w & mask) | 128.0
   const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&biased),
                                    __bfloat162bfloat162(__ushort_as_bfloat16(0x4308)));  // 136
   return *reinterpret_cast<const uint32_t*>(&v);

@@ -15,6 +15,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libb200tx.so"
+BINDING_PATH = Path(__file__).resolve().parent / "_lib" / "_decode_binding.so"
 ABI_VERSION = 2
 
 F32 = 0

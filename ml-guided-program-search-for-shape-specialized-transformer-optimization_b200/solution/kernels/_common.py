@@ -4,11 +4,17 @@ from __future__ import annotations
 
 import torch
 
-from .. import _native
+from .. import _binding, _native
 
 
 def library_ready() -> bool:
     return _native.library_available()
+
+
+def binding():  # noqa: ANN201 - the extension module
+    """The compiled calls of the decoding operators; RuntimeError where it or the library is missing."""
+
+    return _binding.load()
 
 
 _SM100_BY_DEVICE: dict[int, bool] = {}

@@ -17,8 +17,8 @@ import ctypes
 import torch
 
 from .. import _native
-from ._common import is_sm100_cuda, launch, library_ready, require
-from .rotary import RotaryTable, check_norm_weights, check_rope, packed_ok
+from ._common import binding, is_sm100_cuda, library_ready, require
+from .rotary import RotaryTable
 
 SM100_KV8_APPEND_BACKEND = "sm100_kv8_append"
 SM100_KV8_GATHER_BACKEND = "sm100_kv8_gather"
@@ -91,7 +91,8 @@ class Kv8Cache:
             )
             for i in range(layers)
         ]
-        self._references = [ctypes.byref(view) for view in self._views]
+        # what the binding takes for a layer: the struct's address and the device
+        self._handles = [(ctypes.addressof(view), codes.get_device()) for view in self._views]
         # The attention's workspace (arrival counters that every launch leaves
         # zero, and the parts of split tiles), one for each stream it runs on.
         self._workspaces: dict[int, torch.Tensor] = {}
@@ -125,9 +126,15 @@ class Kv8Cache:
 
         return 2 * self.layers * self.kv_heads * (self.head_dim + 4 / KV8_BLOCK)
 
-    def reference(self, layer: int) -> object:
+    def handle(self, layer: int) -> tuple[int, int]:
         require(0 <= layer < self.layers, f"layer {layer} of a cache of {self.layers}")
-        return self._references[layer]
+        return self._handles[layer]
+
+    def reference(self, layer: int) -> object:
+        """The layer's b200tx_kv8_cache, as ctypes passes it."""
+
+        require(0 <= layer < self.layers, f"layer {layer} of a cache of {self.layers}")
+        return ctypes.byref(self._views[layer])
 
     def workspace(self, stream: int) -> torch.Tensor:
         found = self._workspaces.get(stream)
@@ -147,36 +154,11 @@ class Kv8Cache:
             self.lengths.index_add_(0, slots, torch.full_like(slots, tokens, dtype=torch.int32))
 
 
-def _ready(tensor: torch.Tensor, cache: Kv8Cache) -> bool:
-    return (
-        library_ready() and not torch.is_grad_enabled() and is_sm100_cuda(tensor) and tensor.device == cache.device
-    )
-
-
-def _check_selection(
-    cache: Kv8Cache, batch: int, slots: torch.Tensor | None, counts: torch.Tensor | None
-) -> None:
-    for name, value in (("slots", slots), ("counts", counts)):
-        if value is not None:
-            require(
-                value.dtype == torch.int32 and tuple(value.shape) == (batch,) and value.is_contiguous()
-                and value.device == cache.device,
-                f"{name} must be a contiguous int32 [B] tensor on the cache's device",
-            )
-    if slots is None:
-        require(batch <= cache.slots, f"a batch of {batch} in a cache of {cache.slots} slots")
-
-
 def can_use_sm100_kv8_append(cache: Kv8Cache, qkv: torch.Tensor, num_heads: int) -> bool:
     """Whether the kernel can append this packed projection (never raises)."""
 
     try:
-        return (
-            _ready(qkv, cache)
-            and packed_ok(qkv)
-            and num_heads >= cache.kv_heads
-            and qkv.shape[2] == (num_heads + 2 * cache.kv_heads) * cache.head_dim
-        )
+        return library_ready() and is_sm100_cuda(qkv) and binding().kv8_append_ok(cache.handle(0), qkv, num_heads)
     except Exception:  # noqa: BLE001 - predicate contract: never raise
         return False
 
@@ -204,23 +186,9 @@ def sm100_kv8_append(
     T).  ``lengths`` stays as it is until ``cache.advance``: by all the tokens,
     or, for ``T <= 64``, by any number of them (the rest is forgotten)."""
 
-    if not can_use_sm100_kv8_append(cache, qkv, num_heads):
-        raise RuntimeError("sm100 kv8 append is ineligible for the requested inputs")
-    batch, tokens, _ = qkv.shape
-    check_norm_weights(q_weight, k_weight, cache.head_dim, qkv.device)
-    check_rope(rope, cache.head_dim, qkv.device)
-    _check_selection(cache, batch, slots, counts)
-    shape = (batch, tokens, num_heads, cache.head_dim)
-    result = torch.empty(shape, dtype=torch.bfloat16, device=qkv.device) if out is None else out
-    if out is not None:
-        require(
-            tuple(out.shape) == shape and out.dtype == torch.bfloat16 and out.is_contiguous()
-            and out.device == qkv.device and out.data_ptr() % 16 == 0,
-            "out must be a contiguous, 16-byte aligned bf16 [B, T, H, D] tensor",
-        )
-    launch(
-        _native.kv8_append, cache.reference(layer), qkv, result, num_heads, slots, counts, q_weight, k_weight,
-        float(eps), None if rope is None else rope.reference,
+    result = binding().kv8_append(
+        cache.handle(layer), qkv, num_heads, q_weight, k_weight, eps, None if rope is None else rope.handle, slots,
+        counts, out,
     )
     return result, SM100_KV8_APPEND_BACKEND
 
@@ -239,15 +207,8 @@ def sm100_kv8_gather(
     tensors, zero past each sequence's end.  ``tokens`` (or ``counts``) more than
     ``lengths`` are read: those appended since the last ``advance``."""
 
-    if not _ready(cache.codes, cache):
-        raise RuntimeError("sm100 kv8 gather is ineligible for the requested inputs")
     rows = batch if batch is not None else cache.slots if slots is None else slots.shape[0]
-    require(max_tokens > 0 and rows > 0 and tokens >= 0, "max_tokens and the batch must be positive")
-    _check_selection(cache, rows, slots, counts)
-    shape = (rows, max_tokens, cache.kv_heads, cache.head_dim)
-    k = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
-    v = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
-    launch(_native.kv8_gather, cache.reference(layer), k, v, int(tokens), slots, counts)
+    k, v = binding().kv8_gather(cache.handle(layer), cache.codes, rows, max_tokens, tokens, slots, counts)
     return k, v, SM100_KV8_GATHER_BACKEND
 
 
@@ -255,19 +216,7 @@ def can_use_sm100_kv8_attention(cache: Kv8Cache, q: torch.Tensor) -> bool:
     """Whether the kernel can attend with these queries (never raises)."""
 
     try:
-        return (
-            _ready(q, cache)
-            and q.dtype == torch.bfloat16
-            and q.ndim == 4
-            and q.numel() > 0
-            and q.shape[3] == cache.head_dim
-            and q.shape[2] % cache.kv_heads == 0
-            and q.stride(3) == 1
-            and q.stride(2) == cache.head_dim
-            and q.stride(1) % 8 == 0
-            and q.stride(0) % 8 == 0
-            and q.data_ptr() % 16 == 0
-        )
+        return library_ready() and is_sm100_cuda(q) and binding().kv8_attention_ok(cache.handle(0), q)
     except Exception:  # noqa: BLE001 - predicate contract: never raise
         return False
 
@@ -287,23 +236,8 @@ def sm100_kv8_attention(
     Returns the context, bf16 ``[B, T, H * D]``; rows past ``counts[b]`` are zero.
     ``H / Hkv`` query heads share a kv head; ``scale`` defaults to ``D ** -0.5``."""
 
-    if not can_use_sm100_kv8_attention(cache, q):
-        raise RuntimeError("sm100 kv8 attention is ineligible for the requested inputs")
-    batch, tokens, heads, dim = q.shape
-    _check_selection(cache, batch, slots, counts)
-    factor = dim**-0.5 if scale is None else float(scale)
-    require(0.0 < factor <= 1e30, "scale must be positive and finite")
-    shape = (batch, tokens, heads * dim)
-    result = torch.empty(shape, dtype=torch.bfloat16, device=q.device) if out is None else out
-    if out is not None:
-        require(
-            tuple(out.shape) == shape and out.dtype == torch.bfloat16 and out.is_contiguous()
-            and out.device == q.device and out.data_ptr() % 16 == 0,
-            "out must be a contiguous, 16-byte aligned bf16 [B, T, H * D] tensor",
-        )
-    stream = _native._stream(q.device)
-    launch(
-        _native.kv8_attention, cache.reference(layer), q, result, slots, counts, factor, cache.workspace(stream), stream
+    result = binding().kv8_attention(
+        cache.handle(layer), q, scale, slots, counts, out, cache._workspaces, cache.workspace
     )
     return result, SM100_KV8_ATTENTION_BACKEND
 

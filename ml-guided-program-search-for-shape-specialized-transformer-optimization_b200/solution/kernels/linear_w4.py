@@ -10,8 +10,7 @@ from __future__ import annotations
 
 import torch
 
-from .. import _native
-from ._common import is_sm100_cuda, launch, library_ready, require
+from ._common import binding, is_sm100_cuda, library_ready, require
 
 SM100_LINEAR_W4_BACKEND = "sm100_linear_w4"
 SM100_LINEAR_W4_GELU_BACKEND = "sm100_linear_w4_gelu"
@@ -88,15 +87,10 @@ def can_use_sm100_linear_w4(value: torch.Tensor, weight: W4Weight, bias: torch.T
     """Whether the kernel can run on these operands (never raises)."""
 
     try:
-        if not library_ready() or torch.is_grad_enabled() or not is_sm100_cuda(value):
-            return False
-        if value.dtype != torch.bfloat16 or value.ndim < 1 or value.shape[-1] != weight.in_features:
-            return False
-        if not value.is_contiguous() or value.numel() == 0 or value.data_ptr() % 16 or weight.device != value.device:
-            return False
-        return bias is None or (
-            bias.dtype == torch.float32 and bias.shape == (weight.out_features,) and bias.is_contiguous()
-            and bias.device == value.device
+        return (
+            library_ready()
+            and is_sm100_cuda(value)
+            and binding().linear_w4_ok(value, weight.packed, bias, weight.in_features)
         )
     except Exception:  # noqa: BLE001 - predicate contract: never raise
         return False
@@ -115,19 +109,10 @@ def sm100_linear_w4(
     fp32 accumulation, fp32 bias and erf GELU before the cast.  Made for up to 32
     rows; more are taken 32 at a time, each time reading the weight again."""
 
-    if not can_use_sm100_linear_w4(value, weight, bias):
-        raise RuntimeError("sm100 4-bit linear is ineligible for the requested operands")
     require(out_dtype in _OUT, "out_dtype must be float32 or bfloat16")
-    shape = (*value.shape[:-1], weight.out_features)
-    result = torch.empty(shape, dtype=out_dtype, device=value.device) if out is None else out
-    if out is not None:
-        require(
-            tuple(out.shape) == shape and out.dtype == out_dtype and out.is_contiguous() and out.device == value.device,
-            "out has the wrong shape, dtype, device or layout",
-        )
-    launch(
-        _native.linear_w4, value, weight.packed, weight.scales, bias, result, value.numel() // weight.in_features,
-        weight.in_features, weight.group, _native.EPI_BIAS_GELU if gelu else _native.EPI_BIAS,
+    result = binding().linear_w4(
+        value, weight.packed, weight.scales, bias, weight.in_features, weight.group, gelu,
+        out_dtype == torch.float32, out,
     )
     return result, SM100_LINEAR_W4_GELU_BACKEND if gelu else SM100_LINEAR_W4_BACKEND
 

@@ -16,12 +16,10 @@ import ctypes
 import torch
 
 from .. import _native
-from ._common import is_sm100_cuda, launch, library_ready, require
+from ._common import binding, is_sm100_cuda, library_ready, require
 
 SM100_QK_NORM_ROPE_BACKEND = "sm100_qk_norm_rope"
 ROPE_HEAD_DIMS = (8, 16, 32, 64, 128, 256)
-
-_IO = (torch.float32, torch.bfloat16)
 
 
 class RotaryTable:
@@ -45,7 +43,8 @@ class RotaryTable:
         self.rotary = 2 * cos.shape[1]
         self.device = cos.device
         self._struct = _native.Rope(cos.data_ptr(), sin.data_ptr(), cos.shape[0], self.rotary, int(self.interleaved))
-        self.reference = ctypes.byref(self._struct)
+        # what the binding takes: the struct's address, the turned dims and the device
+        self.handle = (ctypes.addressof(self._struct), self.rotary, cos.get_device())
 
     @classmethod
     def create(
@@ -58,52 +57,15 @@ class RotaryTable:
         return cls(angle.cos().float().to(device), angle.sin().float().to(device), interleaved=interleaved)
 
 
-def check_norm_weights(
-    q_weight: torch.Tensor | None, k_weight: torch.Tensor | None, head_dim: int, device: torch.device
-) -> None:
-    for weight in (q_weight, k_weight):
-        if weight is not None:
-            require(
-                weight.dtype == torch.float32 and weight.shape == (head_dim,) and weight.is_contiguous()
-                and weight.device == device and weight.data_ptr() % 16 == 0,
-                "the norm weights must be contiguous, 16-byte aligned float32 [head_dim] tensors on the input's device",
-            )
-
-
-def check_rope(rope: RotaryTable | None, head_dim: int, device: torch.device) -> None:
-    if rope is not None:
-        require(rope.device == device, "the rotation table must be on the input's device")
-        require(
-            rope.rotary <= head_dim and rope.rotary % (16 if head_dim == 256 else 8) == 0,
-            f"rotary {rope.rotary} must be a multiple of {16 if head_dim == 256 else 8} up to head_dim {head_dim}",
-        )
-
-
-def packed_ok(qkv: torch.Tensor) -> bool:
-    """Layout the kernels read: dense heads, any 16-byte aligned token and batch strides."""
-
-    return (
-        qkv.ndim == 3
-        and qkv.dtype in _IO
-        and qkv.stride(2) == 1
-        and qkv.stride(0) % 8 == 0
-        and qkv.stride(1) % 8 == 0
-        and qkv.data_ptr() % 16 == 0
-        and qkv.numel() > 0
-    )
-
-
 def can_use_sm100_qk_norm_rope(qkv: torch.Tensor, num_heads: int, num_kv_heads: int | None = None) -> bool:
     """Whether the kernel can read this packed projection (never raises)."""
 
     try:
-        if not library_ready() or torch.is_grad_enabled() or not is_sm100_cuda(qkv) or not packed_ok(qkv):
-            return False
-        kv_heads = num_heads if num_kv_heads is None else num_kv_heads
-        total = num_heads + 2 * kv_heads
-        if num_heads <= 0 or kv_heads <= 0 or kv_heads > num_heads or qkv.shape[2] % total:
-            return False
-        return qkv.shape[2] // total in ROPE_HEAD_DIMS
+        return (
+            library_ready()
+            and is_sm100_cuda(qkv)
+            and binding().qk_norm_rope_ok(qkv, num_heads, num_heads if num_kv_heads is None else num_kv_heads)
+        )
     except Exception:  # noqa: BLE001 - predicate contract: never raise
         return False
 
@@ -126,29 +88,9 @@ def sm100_qk_norm_rope(
     heads as they are.  fp32 inside, one rounding to ``qkv``'s dtype.  ``out=qkv``
     works in place and leaves the value heads alone."""
 
-    if not can_use_sm100_qk_norm_rope(qkv, num_heads, num_kv_heads):
-        raise RuntimeError("sm100 qk norm + rotation is ineligible for the requested inputs")
-    kv_heads = num_heads if num_kv_heads is None else num_kv_heads
-    head_dim = qkv.shape[2] // (num_heads + 2 * kv_heads)
-    check_norm_weights(q_weight, k_weight, head_dim, qkv.device)
-    check_rope(rope, head_dim, qkv.device)
-    if positions is not None:
-        require(
-            positions.dtype in (torch.int32, torch.int64) and positions.device == qkv.device
-            and tuple(positions.shape) in ((qkv.shape[0], qkv.shape[1]), (qkv.shape[1],))
-            and positions.stride(-1) == 1,
-            "positions must be an int32 or int64 [B, T] or [T] tensor on the input's device",
-        )
-    result = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device) if out is None else out
-    if out is not None:
-        require(
-            out.shape == qkv.shape and out.dtype == qkv.dtype and out.device == qkv.device and packed_ok(out)
-            and (out.data_ptr() != qkv.data_ptr() or out.stride() == qkv.stride()),
-            "out must have qkv's shape, dtype and device, 16-byte aligned heads, and qkv's strides when it is qkv",
-        )
-    launch(
-        _native.qk_norm_rope, qkv, result, num_heads, kv_heads, head_dim, q_weight, k_weight, float(eps),
-        None if rope is None else rope.reference, positions,
+    result = binding().qk_norm_rope(
+        qkv, num_heads, num_heads if num_kv_heads is None else num_kv_heads, q_weight, k_weight, eps,
+        None if rope is None else rope.handle, positions, out,
     )
     return result, SM100_QK_NORM_ROPE_BACKEND
 
@@ -158,8 +100,5 @@ __all__ = [
     "RotaryTable",
     "SM100_QK_NORM_ROPE_BACKEND",
     "can_use_sm100_qk_norm_rope",
-    "check_norm_weights",
-    "check_rope",
-    "packed_ok",
     "sm100_qk_norm_rope",
 ]
