@@ -5,19 +5,12 @@
 
 namespace {
 
-// Head groups of one warp when a token's heads are dealt to `splits` warps:
-// with few tokens each warp takes one round of loads, so that a step is as
-// short as it can be; with enough tokens to fill the SMs a warp takes the whole
-// token and loads its angles once.
-void split_heads(int64_t tokens, int groups, int sm_count, int* splits, int* span) {
-  const int64_t wanted = static_cast<int64_t>(sm_count) * b200tx::kRopeWarps * 4;
-  const int rounds = (groups + b200tx::kRopeUnroll - 1) / b200tx::kRopeUnroll;
-  int64_t s = (wanted + tokens - 1) / tokens;
-  if (s > rounds) s = rounds;
-  if (s < 1) s = 1;
-  const int per = static_cast<int>((rounds + s - 1) / s);
-  *span = per * b200tx::kRopeUnroll;
-  *splits = (rounds + per - 1) / per;
+// Values a lane: eight of bf16, four of fp32 (16 bytes; 25 x 420 tokens of 6 heads of 64
+// in fp32: four 8.0 us, eight 13.7), four of bf16 where the pairs' halves do not lie
+// eight apart, eight of fp32 for head_dim 256 (a head is at most one warp).
+bool eight_values(const b200tx::RopeTable& rope, int dtype, int64_t head_dim) {
+  if (head_dim == 256) return true;
+  return dtype == B200TX_BF16 && (rope.cos == nullptr || rope.interleaved || rope.rotary % 16 == 0);
 }
 
 int rope_table(const char* what, const b200tx_rope* rope, int64_t head_dim, b200tx::RopeTable* out) {
@@ -25,6 +18,8 @@ int rope_table(const char* what, const b200tx_rope* rope, int64_t head_dim, b200
   if (rope == nullptr) return B200TX_OK;
   if (rope->cos == nullptr || rope->sin == nullptr || rope->positions <= 0 || rope->positions > 0x7fffffffLL)
     return fail(B200TX_ERR_INVALID_ARGUMENT, "%s: bad rotation table", what);
+  if (!aligned16(rope->cos) || !aligned16(rope->sin))
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "%s: the rotation tables must be 16-byte aligned", what);
   const int64_t step = head_dim == 256 ? 16 : 8;
   if (rope->rotary <= 0 || rope->rotary > head_dim || rope->rotary % step != 0)
     return fail(B200TX_ERR_INVALID_ARGUMENT, "%s: rotary %lld is not a multiple of %lld up to head_dim %lld", what,
@@ -69,46 +64,60 @@ int kv8_view(const char* what, const b200tx_kv8_cache* c, b200tx::Kv8Cache* out)
   return B200TX_OK;
 }
 
-template <int D, typename T>
-cudaError_t launch_rope(b200tx::RopeArgs& a, int sm_count, cudaStream_t stream) {
-  const int heads = a.heads + (a.copy_values ? 2 : 1) * a.kv_heads;
-  constexpr int HEADS = b200tx::HeadLanes<D>::HEADS;
-  split_heads(a.total_tokens, (heads + HEADS - 1) / HEADS, sm_count, &a.splits, &a.span);
-  const int64_t units = a.total_tokens * a.splits;
-  return launch(b200tx::qk_norm_rope_kernel<D, T>,
-                dim3(static_cast<unsigned>((units + b200tx::kRopeWarps - 1) / b200tx::kRopeWarps)),
-                dim3(b200tx::kRopeWarps * 32), 0, stream, a);
+template <int D, int E, typename T>
+cudaError_t launch_rope(b200tx::RopeArgs& a, cudaStream_t stream) {
+  const int64_t rounds =
+      b200tx::rope_rounds<D, E>(a.heads) + (a.copy_values ? 2 : 1) * b200tx::rope_rounds<D, E>(a.kv_heads);
+  const int64_t ctas = (a.total_tokens * rounds + b200tx::kRopeWarps - 1) / b200tx::kRopeWarps;
+  return launch(b200tx::qk_norm_rope_kernel<D, E, T>, dim3(static_cast<unsigned>(ctas)), dim3(b200tx::kRopeWarps * 32), 0,
+                stream, a);
 }
 
-template <typename T>
-cudaError_t launch_rope_dim(int64_t head_dim, b200tx::RopeArgs& a, int sm_count, cudaStream_t stream) {
+cudaError_t launch_rope_dim(int64_t head_dim, int dtype, b200tx::RopeArgs& a, cudaStream_t stream) {
+  using bf16 = __nv_bfloat16;
+  if (eight_values(a.norm.rope, dtype, head_dim)) {
+    switch (head_dim) {
+      case 8: return launch_rope<8, 8, bf16>(a, stream);
+      case 16: return launch_rope<16, 8, bf16>(a, stream);
+      case 32: return launch_rope<32, 8, bf16>(a, stream);
+      case 64: return launch_rope<64, 8, bf16>(a, stream);
+      case 128: return launch_rope<128, 8, bf16>(a, stream);
+      default: return dtype == B200TX_F32 ? launch_rope<256, 8, float>(a, stream) : launch_rope<256, 8, bf16>(a, stream);
+    }
+  }
+  const bool f32 = dtype == B200TX_F32;
   switch (head_dim) {
-    case 8: return launch_rope<8, T>(a, sm_count, stream);
-    case 16: return launch_rope<16, T>(a, sm_count, stream);
-    case 32: return launch_rope<32, T>(a, sm_count, stream);
-    case 64: return launch_rope<64, T>(a, sm_count, stream);
-    case 128: return launch_rope<128, T>(a, sm_count, stream);
-    default: return launch_rope<256, T>(a, sm_count, stream);
+    case 8: return f32 ? launch_rope<8, 4, float>(a, stream) : launch_rope<8, 4, bf16>(a, stream);
+    case 16: return f32 ? launch_rope<16, 4, float>(a, stream) : launch_rope<16, 4, bf16>(a, stream);
+    case 32: return f32 ? launch_rope<32, 4, float>(a, stream) : launch_rope<32, 4, bf16>(a, stream);
+    case 64: return f32 ? launch_rope<64, 4, float>(a, stream) : launch_rope<64, 4, bf16>(a, stream);
+    default: return f32 ? launch_rope<128, 4, float>(a, stream) : launch_rope<128, 4, bf16>(a, stream);
   }
 }
 
-template <int D, typename T>
-cudaError_t launch_kv8_append(b200tx::Kv8AppendArgs& a, int sm_count, cudaStream_t stream) {
-  constexpr int HEADS = b200tx::HeadLanes<D>::HEADS;
-  const int64_t tokens = static_cast<int64_t>(a.batch) * a.tokens;
-  split_heads(tokens, (a.heads + HEADS - 1) / HEADS, sm_count, &a.splits, &a.span);
-  const int64_t q_ctas = (tokens * a.splits + b200tx::kKv8AppendWarps - 1) / b200tx::kKv8AppendWarps;
-  return launch(b200tx::kv8_append_kernel<D, T>, dim3(static_cast<unsigned>(a.kv_ctas + q_ctas)),
+template <int D, int E, typename T>
+cudaError_t launch_kv8_append(b200tx::Kv8AppendArgs& a, cudaStream_t stream) {
+  const int64_t units = static_cast<int64_t>(a.batch) * a.tokens * b200tx::rope_rounds<D, E>(a.heads);
+  const int64_t q_ctas = (units + b200tx::kKv8AppendWarps - 1) / b200tx::kKv8AppendWarps;
+  return launch(b200tx::kv8_append_kernel<D, E, T>, dim3(static_cast<unsigned>(a.kv_ctas + q_ctas)),
                 dim3(b200tx::kKv8AppendWarps * 32), 0, stream, a);
 }
 
-template <typename T>
-cudaError_t launch_kv8_append_dim(int64_t head_dim, b200tx::Kv8AppendArgs& a, int sm_count, cudaStream_t stream) {
+cudaError_t launch_kv8_append_dim(int64_t head_dim, int dtype, b200tx::Kv8AppendArgs& a, cudaStream_t stream) {
+  using bf16 = __nv_bfloat16;
+  if (eight_values(a.norm.rope, dtype, head_dim)) {
+    switch (head_dim) {
+      case 32: return launch_kv8_append<32, 8, bf16>(a, stream);
+      case 64: return launch_kv8_append<64, 8, bf16>(a, stream);
+      case 128: return launch_kv8_append<128, 8, bf16>(a, stream);
+      default: return dtype == B200TX_F32 ? launch_kv8_append<256, 8, float>(a, stream) : launch_kv8_append<256, 8, bf16>(a, stream);
+    }
+  }
+  const bool f32 = dtype == B200TX_F32;
   switch (head_dim) {
-    case 32: return launch_kv8_append<32, T>(a, sm_count, stream);
-    case 64: return launch_kv8_append<64, T>(a, sm_count, stream);
-    case 128: return launch_kv8_append<128, T>(a, sm_count, stream);
-    default: return launch_kv8_append<256, T>(a, sm_count, stream);
+    case 32: return f32 ? launch_kv8_append<32, 4, float>(a, stream) : launch_kv8_append<32, 4, bf16>(a, stream);
+    case 64: return f32 ? launch_kv8_append<64, 4, float>(a, stream) : launch_kv8_append<64, 4, bf16>(a, stream);
+    default: return f32 ? launch_kv8_append<128, 4, float>(a, stream) : launch_kv8_append<128, 4, bf16>(a, stream);
   }
 }
 
@@ -254,10 +263,9 @@ int b200tx_qk_norm_rope(const void* qkv, void* out, int dtype, int64_t batch, in
   a.norm.q_weight = q_weight;
   a.norm.k_weight = k_weight;
   a.norm.eps = eps;
-  if (a.total_tokens > 0x7fffffffLL / 64)
+  if (static_cast<double>(a.total_tokens) * (heads + 2 * kv_heads) > 2147483647.0)
     return fail(B200TX_ERR_INVALID_ARGUMENT, "qk_norm_rope: too many tokens");
-  cudaError_t err = dtype == B200TX_F32 ? launch_rope_dim<float>(head_dim, a, dev->sm_count, stream)
-                                        : launch_rope_dim<__nv_bfloat16>(head_dim, a, dev->sm_count, stream);
+  cudaError_t err = launch_rope_dim(head_dim, dtype, a, stream);
   return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "qk_norm_rope");
 }
 
@@ -299,10 +307,9 @@ int b200tx_kv8_append(const b200tx_kv8_cache* cache, const void* qkv, int dtype,
   a.norm.q_weight = q_weight;
   a.norm.k_weight = k_weight;
   a.norm.eps = eps;
-  if (batch * tokens > 0x7fffffffLL / 64 || a.kv_ctas > 0x3fffffffLL)
+  if (static_cast<double>(batch) * tokens * heads > 1073741823.0 || a.kv_ctas > 0x3fffffffLL)
     return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_append: too many tokens");
-  cudaError_t err = dtype == B200TX_F32 ? launch_kv8_append_dim<float>(cache->head_dim, a, dev->sm_count, stream)
-                                        : launch_kv8_append_dim<__nv_bfloat16>(cache->head_dim, a, dev->sm_count, stream);
+  cudaError_t err = launch_kv8_append_dim(cache->head_dim, dtype, a, stream);
   return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "kv8_append");
 }
 

@@ -282,10 +282,9 @@ PyObject* kv8_gather(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int32_t* slots = per_sequence(args[5], batch, *codes, kSlots);
     const int32_t* counts = per_sequence(args[6], batch, *codes, kCounts);
     require(slots != nullptr || batch <= c.view->slots, kBatch);
-    // keys and values are two halves of one allocation
-    const at::Tensor both = at::empty({2, batch, most, c.view->kv_heads, c.view->head_dim},
-                                      at::TensorOptions().dtype(at::kBFloat16).device(codes->device()));
-    at::Tensor k = both.select(0, 0), v = both.select(0, 1);
+    const auto kind = at::TensorOptions().dtype(at::kBFloat16).device(codes->device());
+    const int64_t shape[4] = {batch, most, c.view->kv_heads, c.view->head_dim};
+    at::Tensor k = at::empty(shape, kind), v = at::empty(shape, kind);
     launched(entry.kv8_gather(c.view, k.data_ptr(), v.data_ptr(), batch, most, tokens, slots, counts, stream_of(*codes)),
              "b200tx_kv8_gather");
     PyObject* pk = THPVariable_Wrap(k);

@@ -62,7 +62,6 @@ struct Kv8AppendArgs {
   int batch, tokens, heads;
   int block_span;                      // blocks a sequence's new tokens can touch
   int64_t kv_ctas;                     // batch * kv_heads * block_span
-  int splits, span;                    // query part: warps per token, head groups per warp
   QkNormArgs norm;
 };
 
@@ -70,61 +69,68 @@ constexpr int kKv8AppendWarps = 8;
 
 // One block of one kv head: its new tokens normed, rotated and stored, and the
 // block quantised if it is full now.
-template <int D, typename T>
+template <int D, int E, typename T>
 __device__ __forceinline__ void kv8_append_block(const Kv8AppendArgs& a, int b, int slot, int head, int block, int start,
                                                  int count, uint32_t (*peak)[kKv8AppendWarps]) {
-  constexpr int E = HeadLanes<D>::E;
-  constexpr int L = HeadLanes<D>::L;
-  constexpr int HEADS = HeadLanes<D>::HEADS;                 // tokens per warp and pass
-  constexpr int PASS = kKv8AppendWarps * HEADS;              // tokens per pass
+  using Lanes = HeadLanes<D, E>;
+  constexpr int L = Lanes::L;
+  constexpr int TOKENS = Lanes::HEADS;                      // per warp and pass
+  constexpr int PASS = kKv8AppendWarps * TOKENS;            // tokens per pass
   constexpr int PASSES = (kKv8Block + PASS - 1) / PASS;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, in_head = lane % L;
   const int first = block * kKv8Block;
   const int end = start + count;
   const bool full = first + kKv8Block <= end;
   const bool keep = !full || a.tokens <= kKv8Block;
-  const T* src = static_cast<const T*>(a.qkv) + b * a.batch_stride;
-  __nv_bfloat16* const tail_k = kv8_tail(a.cache, slot, block & 1, 0, head, D);
-  __nv_bfloat16* const tail_v = kv8_tail(a.cache, slot, block & 1, 1, head, D);
-  float kw[E] = {};
-  if (a.norm.k_weight != nullptr) load_values<E>(a.norm.k_weight + in_head * E, kw);
+  const T* src = static_cast<const T*>(a.qkv) + b * a.batch_stride + (a.heads + head) * D + in_head * E;
+  __nv_bfloat16* const tail_k = kv8_tail(a.cache, slot, block & 1, 0, head, D) + in_head * E;
+  __nv_bfloat16* const tail_v = kv8_tail(a.cache, slot, block & 1, 1, head, D) + in_head * E;
+  const int partner = partner_lane<D, E>(a.norm.rope, lane);
 
   uint32_t k_bits[PASSES][E / 2], v_bits[PASSES][E / 2];  // bf16 pairs
+  // every pass's loads go out before the first is used
+  Raw<T, E> k_raw[PASSES], v_raw[PASSES];
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
-    const int in_block = p * PASS + warp * HEADS + lane / L;
+    const int in_block = p * PASS + warp * TOKENS + lane / L;
+    const int token = first + in_block;
+    k_raw[p].zero();
+    v_raw[p].zero();
+    if (in_block < kKv8Block && token >= start && token < end) {
+      k_raw[p].load(src + (token - start) * a.token_stride);
+      v_raw[p].load(src + (token - start) * a.token_stride + a.cache.kv_heads * D);
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) {
+    const int in_block = p * PASS + warp * TOKENS + lane / L;
     const int token = first + in_block;
     const bool fresh = in_block < kKv8Block && token >= start && token < end;
-    const bool held = in_block < kKv8Block && token < start && full;
-    float k[E] = {}, v[E] = {};
-    if (fresh) {
-      const T* row = src + (token - start) * a.token_stride + in_head * E;
-      load_values<E>(row + (a.heads + head) * D, k);
-      load_values<E>(row + (a.heads + a.cache.kv_heads + head) * D, v);
-    } else if (held) {
-      load_values<E>(tail_k + in_block * D + in_head * E, k);
-      load_values<E>(tail_v + in_block * D + in_head * E, v);
-    }
+    Raw<__nv_bfloat16, E> k, v;
+    k.zero();
+    v.zero();
     if (__any_sync(0xffffffffu, fresh)) {
-      LaneAngles<D> angles;
+      LaneAngles<D, E> angles;
       angles.load(a.norm.rope, fresh ? token : 0, in_head);
-      float y[E];
-#pragma unroll
-      for (int i = 0; i < E; ++i) y[i] = k[i];
-      norm_rotate<D>(y, kw, a.norm.k_weight != nullptr, a.norm.eps, angles, a.norm.rope, lane);
-      if (fresh) {
-#pragma unroll
-        for (int i = 0; i < E; ++i) k[i] = y[i];
-        if (keep) {
-          store_values<E>(tail_k + in_block * D + in_head * E, k);
-          store_values<E>(tail_v + in_block * D + in_head * E, v);
-        }
-      }
+      LaneFactors<D, E> f;
+      f.set(a.norm.k_weight, angles, a.norm.rope, lane);
+      float y[E], x[E];
+      norm_rotate<D, E, T>(k_raw[p], y, f, a.norm.k_weight != nullptr, a.norm.eps, angles.turned, a.norm.rope, partner);
+      v_raw[p].values(x);
+      k.set(y);
+      v.set(x);
+    }
+    if (fresh && keep) {
+      k.store(tail_k + in_block * D);
+      v.store(tail_v + in_block * D);
+    } else if (!fresh && full && in_block < kKv8Block && token < start) {
+      k.load(tail_k + in_block * D);
+      v.load(tail_v + in_block * D);
     }
 #pragma unroll
     for (int i = 0; i < E / 2; ++i) {
-      k_bits[p][i] = pack_bf16x2(k[2 * i], k[2 * i + 1]);
-      v_bits[p][i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+      k_bits[p][i] = k.w[i];
+      v_bits[p][i] = v.w[i];
     }
   }
   if (!full) return;
@@ -171,7 +177,7 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendArgs& a, int b, 
   };
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
-    const int in_block = p * PASS + warp * HEADS + lane / L;
+    const int in_block = p * PASS + warp * TOKENS + lane / L;
     if (in_block >= kKv8Block) continue;
 #pragma unroll
     for (int i = 0; i < E / 4; ++i) {
@@ -189,20 +195,15 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendArgs& a, int b, 
 }
 
 // CTAs below kv_ctas each take one block of one kv head; the rest norm and
-// rotate the queries, a warp for a token's head groups as in
-// qk_norm_rope_kernel.
-template <int D, typename T>
+// rotate the queries, a warp for a round of a token's heads as in qk_norm_rope_kernel.
+template <int D, int E, typename T>
 __global__ void __launch_bounds__(kKv8AppendWarps * 32) kv8_append_kernel(Kv8AppendArgs a) {
-  constexpr int E = HeadLanes<D>::E;
-  constexpr int L = HeadLanes<D>::L;
-  constexpr int HEADS = HeadLanes<D>::HEADS;
   __shared__ uint32_t peak[2][kKv8AppendWarps];
   griddep_wait();
   griddep_launch_dependents();
-  const bool is_kv = blockIdx.x < a.kv_ctas;
-  const int lane = threadIdx.x % 32, in_head = lane % L;
+  const int lane = threadIdx.x % 32;
 
-  if (is_kv) {
+  if (blockIdx.x < a.kv_ctas) {
     const int64_t item = blockIdx.x / a.cache.kv_heads;
     const int head = static_cast<int>(blockIdx.x - item * a.cache.kv_heads);
     const int b = static_cast<int>(item / a.block_span);
@@ -221,47 +222,26 @@ __global__ void __launch_bounds__(kKv8AppendWarps * 32) kv8_append_kernel(Kv8App
     const bool shared_slot = at == 0 ? last > first && ((last - first) & 1) == 0
                                      : block == last && (at & 1) == 0;
     if (at != 0 && shared_slot) return;
-    kv8_append_block<D, T>(a, b, slot, head, block, start, count, peak);
-    if (at == 0 && shared_slot) {
+    for (int now = block;; now = last) {
+      kv8_append_block<D, E, T>(a, b, slot, head, now, start, count, peak);
+      if (!shared_slot || now == last) return;
       __syncthreads();
-      kv8_append_block<D, T>(a, b, slot, head, last, start, count, peak);
     }
-    return;
   }
 
-  const int64_t unit = (static_cast<int64_t>(blockIdx.x) - a.kv_ctas) * kKv8AppendWarps + threadIdx.x / 32;
-  const int64_t token = unit / a.splits;
-  if (token >= static_cast<int64_t>(a.batch) * a.tokens) return;
-  const int split = static_cast<int>(unit - token * a.splits);
-  const int b = static_cast<int>(token / a.tokens);
-  const int t = static_cast<int>(token - static_cast<int64_t>(b) * a.tokens);
+  constexpr int PER = kRopeUnroll * HeadLanes<D, E>::HEADS;
+  const unsigned rounds = rope_rounds<D, E>(a.heads);
+  const unsigned unit = (blockIdx.x - static_cast<unsigned>(a.kv_ctas)) * kKv8AppendWarps + threadIdx.x / 32;
+  const unsigned token = unit / rounds;
+  if (token >= static_cast<unsigned>(a.batch) * a.tokens) return;
+  const int first = static_cast<int>(unit - token * rounds) * PER;
+  const unsigned b = token / a.tokens, t = token - b * a.tokens;
   const int slot = a.slot_ids == nullptr ? b : a.slot_ids[b];
   // a slot that is none has no position: its queries become NaN where there is a rotation
   const int64_t position = slot < 0 || slot >= a.cache.slots ? -1 : static_cast<int64_t>(max(0, a.cache.lengths[slot])) + t;
-  LaneAngles<D> angles;
-  angles.load(a.norm.rope, position, in_head);
-  float qw[E] = {};
-  if (a.norm.q_weight != nullptr) load_values<E>(a.norm.q_weight + in_head * E, qw);
-  const T* src = static_cast<const T*>(a.qkv) + b * a.batch_stride + t * a.token_stride;
-  __nv_bfloat16* dst = a.q_out + token * a.heads * D;
-  const int first = split * a.span * HEADS;
-  const int last = min(a.heads, first + a.span * HEADS);
-  for (int h0 = first; h0 < last; h0 += kRopeUnroll * HEADS) {
-    float x[kRopeUnroll][E];
-#pragma unroll
-    for (int u = 0; u < kRopeUnroll; ++u) {
-      const int h = h0 + u * HEADS + lane / L;
-#pragma unroll
-      for (int i = 0; i < E; ++i) x[u][i] = 0.f;
-      if (h < last) load_values<E>(src + h * D + in_head * E, x[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < kRopeUnroll; ++u) {
-      const int h = h0 + u * HEADS + lane / L;
-      norm_rotate<D>(x[u], qw, a.norm.q_weight != nullptr, a.norm.eps, angles, a.norm.rope, lane);
-      if (h < last) store_values<E>(dst + h * D + in_head * E, x[u]);
-    }
-  }
+  norm_rotate_round<D, E, T, __nv_bfloat16>(static_cast<const T*>(a.qkv) + b * a.batch_stride + t * a.token_stride,
+                                            a.q_out + static_cast<int64_t>(token) * a.heads * D, first,
+                                            min(first + PER, a.heads), a.norm.q_weight, position, a.norm, lane);
 }
 
 struct Kv8GatherArgs {

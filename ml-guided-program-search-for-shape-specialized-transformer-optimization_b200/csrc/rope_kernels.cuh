@@ -8,11 +8,15 @@
 // copied.  Everything is computed in fp32 and rounded once.
 //
 // The work is elementwise, so HBM bounds it: each value is read and written
-// once.  A head lies across L = D / E lanes with E = max(4, D/32) consecutive
-// values each (one 8- or 16-byte access), so that the sum of squares and the
-// pair's other half are shuffles and never leave the registers.  A lane holds
-// the same dims of every head, so a warp loads its token's angles once and
-// walks over the token's heads, four at a time to keep loads in flight.
+// once.  A head lies across L = D / E lanes with E = 8 (or 4) consecutive values
+// each, one 16-byte access of bf16, so that the sum of squares and the pair's
+// other half are shuffles and never leave the registers.  The factor of the norm
+// is common to a head, so the pair's other half is exchanged as it was read (two
+// bf16 a shuffle) and
+//   y = r (x (w c) + x' (w' s))
+// with w c and w' s computed once for the four groups of heads that a warp takes
+// of a token (a lane holds the same dims of every head); their loads go out
+// together.
 #pragma once
 
 #include "sm100_common.cuh"
@@ -20,7 +24,7 @@
 namespace b200tx {
 
 constexpr int kRopeWarps = 8;   // warps per CTA
-constexpr int kRopeUnroll = 4;  // head groups in flight per warp
+constexpr int kRopeUnroll = 4;  // head groups of a warp
 
 struct RopeTable {
   const float* cos;  // [positions, rotary/2]; null = no rotation
@@ -35,67 +39,78 @@ struct QkNormArgs {
   RopeTable rope;
 };
 
-template <int D>
+template <int D, int E>
 struct HeadLanes {
-  static constexpr int E = D / 32 > 4 ? D / 32 : 4;  // values per lane
-  static constexpr int L = D / E;                    // lanes per head
-  static constexpr int HEADS = 32 / L;               // heads per warp
+  static constexpr int L = D / E;      // lanes per head
+  static constexpr int HEADS = 32 / L;  // heads per warp
 };
 
-// E consecutive values as fp32.
-template <int E>
-__device__ __forceinline__ void load_values(const float* p, float (&x)[E]) {
+// E consecutive values as they lie in memory: one access of up to 16 bytes, two of fp32.
+template <typename T, int E>
+struct Raw {
+  static constexpr int WORDS = E * static_cast<int>(sizeof(T)) / 4;
+  uint32_t w[WORDS];
+
+  __device__ __forceinline__ void zero() {
 #pragma unroll
-  for (int i = 0; i < E; i += 4) {
-    const float4 v = *reinterpret_cast<const float4*>(p + i);
-    x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+    for (int i = 0; i < WORDS; ++i) w[i] = 0u;
   }
-}
-
-template <int E>
-__device__ __forceinline__ void load_values(const __nv_bfloat16* p, float (&x)[E]) {
-  uint32_t w[E / 2];
-  if constexpr (E == 4) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    w[0] = v.x; w[1] = v.y;
-  } else {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-  }
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (WORDS == 2) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      w[0] = v.x; w[1] = v.y;
+    } else {
 #pragma unroll
-  for (int i = 0; i < E / 2; ++i) {
-    x[2 * i] = __uint_as_float(w[i] << 16);
-    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      for (int i = 0; i < WORDS; i += 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + i);
+        w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w;
+      }
+    }
   }
-}
-
-template <int E>
-__device__ __forceinline__ void store_values(float* p, const float (&x)[E]) {
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (WORDS == 2) {
+      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    } else {
 #pragma unroll
-  for (int i = 0; i < E; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
-}
-
-template <int E>
-__device__ __forceinline__ void store_values(__nv_bfloat16* p, const float (&x)[E]) {
-  if constexpr (E == 4) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
-  } else {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]),
-                                              pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+      for (int i = 0; i < WORDS; i += 4)
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(p) + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+    }
   }
-}
+  __device__ __forceinline__ void values(float (&x)[E]) const {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) x[i] = __uint_as_float(w[i]);
+    }
+  }
+  __device__ __forceinline__ void set(const float (&x)[E]) {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) w[i] = __float_as_uint(x[i]);
+    }
+  }
+};
 
-// The angles of a lane's dims at one position.  c multiplies the value, s its
-// partner: dims past `rotary` get (1, 0); the first of a pair carries -sin.
-// A position outside the table gives NaN, which marks the head.
-template <int D>
+// The angles of a lane's dims at one position: c multiplies the value, s the
+// pair's other half (-sin for the first of a pair).  A position outside the table
+// gives NaN, which marks the head.
+template <int D, int E>
 struct LaneAngles {
-  static constexpr int E = HeadLanes<D>::E;
   float c[E], s[E];
+  bool turned;  // the lane's dims are among the first `rotary`
 
   __device__ __forceinline__ void load(const RopeTable& r, int64_t position, int lane_in_head) {
     const int d0 = lane_in_head * E;
-    if (r.cos == nullptr || d0 >= r.rotary) {
+    turned = r.cos != nullptr && d0 < r.rotary;
+    if (!turned) {
 #pragma unroll
       for (int i = 0; i < E; ++i) { c[i] = 1.f; s[i] = 0.f; }
       return;
@@ -120,50 +135,121 @@ struct LaneAngles {
       const bool first = d0 < half;
       const int at = first ? d0 : d0 - half;
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        c[i] = __ldg(cr + at + i);
-        const float sv = __ldg(sr + at + i);
-        s[i] = first ? -sv : sv;
+      for (int i = 0; i < E; i += 4) {
+        const float4 cv = *reinterpret_cast<const float4*>(cr + at + i);
+        const float4 sv = *reinterpret_cast<const float4*>(sr + at + i);
+        c[i] = cv.x; c[i + 1] = cv.y; c[i + 2] = cv.z; c[i + 3] = cv.w;
+        s[i] = sv.x; s[i + 1] = sv.y; s[i + 2] = sv.z; s[i + 3] = sv.w;
       }
+#pragma unroll
+      for (int i = 0; i < E; ++i) s[i] = first ? -s[i] : s[i];
     }
   }
 };
 
-// One head's values in a lane: the norm if this lane's head has one, then the
-// rotation.  All lanes of the warp take part in the shuffles.
-template <int D>
-__device__ __forceinline__ void norm_rotate(float (&x)[HeadLanes<D>::E], const float (&w)[HeadLanes<D>::E], bool normed,
-                                            float eps, const LaneAngles<D>& angles, const RopeTable& rope, int lane) {
-  constexpr int E = HeadLanes<D>::E;
-  constexpr int L = HeadLanes<D>::L;
-  float sum = 0.f;
+// The lane that has the pair's other half (itself where there is none).
+template <int D, int E>
+__device__ __forceinline__ int partner_lane(const RopeTable& r, int lane) {
+  const int apart = r.rotary / (2 * E);
+  const int l = lane % HeadLanes<D, E>::L;
+  return l < apart ? lane + apart : l < 2 * apart ? lane - apart : lane;
+}
+
+// w c and w' s of a lane's dims, for one kind of head at one position.
+template <int D, int E>
+struct LaneFactors {
+  float own[E], other[E];
+
+  __device__ __forceinline__ void set(const float* weight, const LaneAngles<D, E>& a, const RopeTable& r, int lane) {
+    const int d0 = lane % HeadLanes<D, E>::L * E;
+    const int p0 = r.interleaved ? d0 : partner_lane<D, E>(r, lane) % HeadLanes<D, E>::L * E;
 #pragma unroll
-  for (int i = 0; i < E; ++i) sum = fmaf(x[i], x[i], sum);
-#pragma unroll
-  for (int o = L / 2; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (normed) {
-    const float r = rsqrtf(sum * (1.f / D) + eps);
-#pragma unroll
-    for (int i = 0; i < E; ++i) x[i] = x[i] * r * w[i];
+    for (int i = 0; i < E; i += 4) {
+      float4 w = make_float4(1.f, 1.f, 1.f, 1.f), p = w;
+      if (weight != nullptr) {
+        w = __ldg(reinterpret_cast<const float4*>(weight + d0 + i));
+        p = __ldg(reinterpret_cast<const float4*>(weight + p0 + i));
+        if (r.interleaved) p = make_float4(p.y, p.x, p.w, p.z);
+      }
+      own[i] = a.c[i] * w.x; own[i + 1] = a.c[i + 1] * w.y; own[i + 2] = a.c[i + 2] * w.z; own[i + 3] = a.c[i + 3] * w.w;
+      other[i] = a.s[i] * p.x; other[i + 1] = a.s[i + 1] * p.y; other[i + 2] = a.s[i + 2] * p.z; other[i + 3] = a.s[i + 3] * p.w;
+    }
   }
-  if (rope.cos == nullptr) return;
-  if (rope.interleaved) {
+};
+
+// One head's values in a lane, normed and turned.  All lanes of the warp take part.
+template <int D, int E, typename T>
+__device__ __forceinline__ void norm_rotate(const Raw<T, E>& raw, float (&y)[E], const LaneFactors<D, E>& f, bool normed,
+                                            float eps, bool turned, const RopeTable& rope, int partner) {
+  float x[E];
+  raw.values(x);
+  float r = 1.f;
+  if (normed) {
+    uint64_t two = f32x2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < E; i += 2) {
-      const float a = x[i], b = x[i + 1];
-      x[i] = fmaf(a, angles.c[i], b * angles.s[i]);
-      x[i + 1] = fmaf(b, angles.c[i + 1], a * angles.s[i + 1]);
+      const uint64_t v = f32x2(x[i], x[i + 1]);
+      two = fma_f32x2(v, v, two);
     }
-  } else {
-    const int apart = rope.rotary / (2 * E);  // lanes between the halves of a pair
-    const int l = lane % L;
-    const int from = l < apart ? lane + apart : l < 2 * apart ? lane - apart : lane;
+    float sum = unpack_f32x2(two).x + unpack_f32x2(two).y;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const float other = __shfl_sync(0xffffffffu, x[i], from);
-      x[i] = fmaf(x[i], angles.c[i], other * angles.s[i]);
-    }
+    for (int o = HeadLanes<D, E>::L / 2; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    r = rsqrtf(sum * (1.f / D) + eps);
   }
+  float z[E];
+  if (rope.cos != nullptr && !rope.interleaved) {
+    Raw<T, E> other;
+#pragma unroll
+    for (int i = 0; i < Raw<T, E>::WORDS; ++i) other.w[i] = __shfl_sync(0xffffffffu, raw.w[i], partner);
+    other.values(z);
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) z[i] = x[i ^ 1];
+  }
+  const uint64_t rr = f32x2(r, r);
+#pragma unroll
+  for (int i = 0; i < E; i += 2) {
+    uint64_t v = mul_f32x2(f32x2(x[i], x[i + 1]), f32x2(f.own[i], f.own[i + 1]));
+    if (turned) v = fma_f32x2(f32x2(z[i], z[i + 1]), f32x2(f.other[i], f.other[i + 1]), v);
+    const float2 out = unpack_f32x2(mul_f32x2(v, rr));
+    y[i] = out.x;
+    y[i + 1] = out.y;
+  }
+}
+
+// Heads [first, last) of one kind at one token, up to kRopeUnroll x HEADS of them.
+template <int D, int E, typename T, typename OutT>
+__device__ __forceinline__ void norm_rotate_round(const T* src, OutT* dst, int first, int last, const float* weight,
+                                                  int64_t position, const QkNormArgs& norm, int lane) {
+  constexpr int HEADS = HeadLanes<D, E>::HEADS;
+  constexpr int L = HeadLanes<D, E>::L;
+  const int at = lane / L * D + lane % L * E;
+  Raw<T, E> x[kRopeUnroll];
+#pragma unroll
+  for (int u = 0; u < kRopeUnroll; ++u) {
+    x[u].zero();
+    if (first + u * HEADS + lane / L < last) x[u].load(src + (first + u * HEADS) * D + at);
+  }
+  LaneAngles<D, E> angles;
+  angles.load(norm.rope, position, lane % L);
+  LaneFactors<D, E> f;
+  f.set(weight, angles, norm.rope, lane);
+  const int partner = partner_lane<D, E>(norm.rope, lane);
+#pragma unroll
+  for (int u = 0; u < kRopeUnroll; ++u) {
+    if (first + u * HEADS >= last) break;
+    float y[E];
+    norm_rotate<D, E, T>(x[u], y, f, weight != nullptr, norm.eps, angles.turned, norm.rope, partner);
+    Raw<OutT, E> out;
+    out.set(y);
+    if (first + u * HEADS + lane / L < last) out.store(dst + (first + u * HEADS) * D + at);
+  }
+}
+
+// Rounds of a kind of head: what one warp does at once.
+template <int D, int E>
+__host__ __device__ constexpr int rope_rounds(int heads) {
+  return (heads + kRopeUnroll * HeadLanes<D, E>::HEADS - 1) / (kRopeUnroll * HeadLanes<D, E>::HEADS);
 }
 
 struct RopeArgs {
@@ -177,74 +263,48 @@ struct RopeArgs {
   int tokens, heads, kv_heads;
   int copy_values;        // 0: the values are left as they are (in place)
   int64_t total_tokens;   // batch * tokens
-  int splits, span;       // warps per token, head groups per warp
   QkNormArgs norm;
 };
 
-template <int D, typename T>
+// A warp for each round of each token: queries, keys, values.
+template <int D, int E, typename T>
 __global__ void __launch_bounds__(kRopeWarps * 32) qk_norm_rope_kernel(RopeArgs a) {
-  constexpr int E = HeadLanes<D>::E;
-  constexpr int L = HeadLanes<D>::L;
-  constexpr int HEADS = HeadLanes<D>::HEADS;
+  constexpr int PER = kRopeUnroll * HeadLanes<D, E>::HEADS;
   griddep_wait();
   griddep_launch_dependents();
   const int lane = threadIdx.x % 32;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * kRopeWarps + threadIdx.x / 32;
-  const int64_t token = unit / a.splits;
+  const int q_rounds = rope_rounds<D, E>(a.heads), k_rounds = rope_rounds<D, E>(a.kv_heads);
+  const unsigned rounds = q_rounds + k_rounds + (a.copy_values ? k_rounds : 0);
+  const unsigned unit = blockIdx.x * kRopeWarps + threadIdx.x / 32;
+  const unsigned token = unit / rounds;
   if (token >= a.total_tokens) return;
-  const int split = static_cast<int>(unit - token * a.splits);
-  const int64_t b = token / a.tokens;
-  const int64_t t = token - b * a.tokens;
-  const int in_head = lane % L;
-
-  int64_t position = t;
-  if (a.positions != nullptr) {
-    const int64_t at = b * a.position_batch_stride + t;
-    position = a.positions_64 ? static_cast<const int64_t*>(a.positions)[at] : static_cast<const int32_t*>(a.positions)[at];
-  }
-  LaneAngles<D> angles;
-  angles.load(a.norm.rope, position, in_head);
-  float qw[E] = {}, kw[E] = {};
-  if (a.norm.q_weight != nullptr) load_values<E>(a.norm.q_weight + in_head * E, qw);
-  if (a.norm.k_weight != nullptr) load_values<E>(a.norm.k_weight + in_head * E, kw);
-
+  int round = static_cast<int>(unit - token * rounds);
+  const unsigned b = token / a.tokens, t = token - b * a.tokens;
   const T* src = static_cast<const T*>(a.in) + b * a.in_batch_stride + t * a.in_token_stride;
   T* dst = static_cast<T*>(a.out) + b * a.out_batch_stride + t * a.out_token_stride;
-  const int turned = a.heads + a.kv_heads;
-  const int all = a.copy_values ? turned + a.kv_heads : turned;
-  const int first = split * a.span * HEADS;
-  const int last = min(all, first + a.span * HEADS);
-  for (int h0 = first; h0 < last; h0 += kRopeUnroll * HEADS) {
-    float x[kRopeUnroll][E];
-#pragma unroll
-    for (int u = 0; u < kRopeUnroll; ++u) {
-      const int h = h0 + u * HEADS + lane / L;
-      if (h < last) {
-        load_values<E>(src + h * D + in_head * E, x[u]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < E; ++i) x[u][i] = 0.f;
-      }
+
+  if (round < q_rounds + k_rounds) {
+    int64_t position = t;
+    if (a.positions != nullptr) {
+      const int64_t at = b * a.position_batch_stride + t;
+      position = a.positions_64 ? static_cast<const int64_t*>(a.positions)[at] : static_cast<const int32_t*>(a.positions)[at];
     }
-#pragma unroll
-    for (int u = 0; u < kRopeUnroll; ++u) {
-      const int h = h0 + u * HEADS + lane / L;
-      const bool is_q = h < a.heads;
-      float y[E], w[E];
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        y[i] = x[u][i];
-        w[i] = is_q ? qw[i] : kw[i];
-      }
-      const bool normed = is_q ? a.norm.q_weight != nullptr : a.norm.k_weight != nullptr;
-      norm_rotate<D>(y, w, normed, a.norm.eps, angles, a.norm.rope, lane);
-      if (h < turned) {
-#pragma unroll
-        for (int i = 0; i < E; ++i) x[u][i] = y[i];
-      }
-      if (h < last) store_values<E>(dst + h * D + in_head * E, x[u]);
-    }
+    const bool is_q = round < q_rounds;
+    const int first = is_q ? round * PER : a.heads + (round - q_rounds) * PER;
+    const int last = min(first + PER, is_q ? a.heads : a.heads + a.kv_heads);
+    norm_rotate_round<D, E, T, T>(src, dst, first, last, is_q ? a.norm.q_weight : a.norm.k_weight, position, a.norm, lane);
+    return;
   }
+  constexpr int L = HeadLanes<D, E>::L;
+  const int first = a.heads + a.kv_heads + (round - q_rounds - k_rounds) * PER + lane / L;
+  const int last = a.heads + 2 * a.kv_heads;
+  Raw<T, E> x[kRopeUnroll];
+#pragma unroll
+  for (int u = 0; u < kRopeUnroll; ++u)
+    if (first + u * HeadLanes<D, E>::HEADS < last) x[u].load(src + (first + u * HeadLanes<D, E>::HEADS) * D + lane % L * E);
+#pragma unroll
+  for (int u = 0; u < kRopeUnroll; ++u)
+    if (first + u * HeadLanes<D, E>::HEADS < last) x[u].store(dst + (first + u * HeadLanes<D, E>::HEADS) * D + lane % L * E);
 }
 
 }  // namespace b200tx
