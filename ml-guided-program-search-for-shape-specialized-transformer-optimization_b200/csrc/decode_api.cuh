@@ -5,6 +5,9 @@
 
 namespace {
 
+constexpr int64_t kRopeManyTokens = 4096;
+constexpr int kRopeChunks = 4;
+
 // Values a lane: eight of bf16, four of fp32 (16 bytes; 25 x 420 tokens of 6 heads of 64
 // in fp32: four 8.0 us, eight 13.7), four of bf16 where the pairs' halves do not lie
 // eight apart, eight of fp32 for head_dim 256 (a head is at most one warp).
@@ -64,11 +67,17 @@ int kv8_view(const char* what, const b200tx_kv8_cache* c, b200tx::Kv8Cache* out)
   return B200TX_OK;
 }
 
+// Chunks of heads for a warp: one, for the shortest step, or where there are
+// tokens enough to fill the SMs several, so that angles and factors are made
+// fewer times.
+int rope_chunks(int64_t tokens) { return tokens >= kRopeManyTokens ? kRopeChunks : 1; }
+
 template <int D, int E, typename T>
 cudaError_t launch_rope(b200tx::RopeArgs& a, cudaStream_t stream) {
-  const int64_t rounds =
-      b200tx::rope_rounds<D, E>(a.heads) + (a.copy_values ? 2 : 1) * b200tx::rope_rounds<D, E>(a.kv_heads);
-  const int64_t ctas = (a.total_tokens * rounds + b200tx::kRopeWarps - 1) / b200tx::kRopeWarps;
+  a.chunks = rope_chunks(a.total_tokens);
+  const int64_t rounds = b200tx::rope_rounds<D, E>(a.heads, a.chunks) +
+                         (a.copy_values ? 2 : 1) * b200tx::rope_rounds<D, E>(a.kv_heads, a.chunks);
+  const int64_t ctas = (a.total_tokens + b200tx::kRopeWarps - 1) / b200tx::kRopeWarps * rounds;
   return launch(b200tx::qk_norm_rope_kernel<D, E, T>, dim3(static_cast<unsigned>(ctas)), dim3(b200tx::kRopeWarps * 32), 0,
                 stream, a);
 }
@@ -97,7 +106,8 @@ cudaError_t launch_rope_dim(int64_t head_dim, int dtype, b200tx::RopeArgs& a, cu
 
 template <int D, int E, typename T>
 cudaError_t launch_kv8_append(b200tx::Kv8AppendArgs& a, cudaStream_t stream) {
-  const int64_t units = static_cast<int64_t>(a.batch) * a.tokens * b200tx::rope_rounds<D, E>(a.heads);
+  a.chunks = rope_chunks(static_cast<int64_t>(a.batch) * a.tokens);
+  const int64_t units = static_cast<int64_t>(a.batch) * a.tokens * b200tx::rope_rounds<D, E>(a.heads, a.chunks);
   const int64_t q_ctas = (units + b200tx::kKv8AppendWarps - 1) / b200tx::kKv8AppendWarps;
   return launch(b200tx::kv8_append_kernel<D, E, T>, dim3(static_cast<unsigned>(a.kv_ctas + q_ctas)),
                 dim3(b200tx::kKv8AppendWarps * 32), 0, stream, a);
@@ -122,9 +132,11 @@ cudaError_t launch_kv8_append_dim(int64_t head_dim, int dtype, b200tx::Kv8Append
 }
 
 template <int D>
-cudaError_t launch_kv8_gather(const b200tx::Kv8GatherArgs& a, cudaStream_t stream) {
-  const int64_t threads = static_cast<int64_t>(a.batch) * a.most * a.cache.kv_heads * (D / 8);
-  return launch(b200tx::kv8_gather_kernel<D>, dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, stream, a);
+cudaError_t launch_kv8_gather(b200tx::Kv8GatherArgs& a, cudaStream_t stream) {
+  const int64_t threads = static_cast<int64_t>(a.most) * a.cache.kv_heads * (D / 8);
+  a.ctas = static_cast<int>((threads + 255) / 256);
+  return launch(b200tx::kv8_gather_kernel<D>, dim3(static_cast<unsigned>(a.ctas) * static_cast<unsigned>(a.batch)),
+                dim3(256), 0, stream, a);
 }
 
 // The workspace of the attention: arrival counters, then the parts of tiles
@@ -326,7 +338,7 @@ int b200tx_kv8_gather(const b200tx_kv8_cache* cache, void* k_out, void* v_out, i
   if (slot_ids == nullptr && batch > cache->slots)
     return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_gather: batch %lld in a cache of %lld slots", (long long)batch,
                 (long long)cache->slots);
-  if (static_cast<double>(batch) * most * cache->kv_heads * (cache->head_dim / 8) > 256.0 * 0x7fffffff)
+  if (static_cast<double>(batch) * most * cache->kv_heads * (cache->head_dim / 8) > 2147483647.0)
     return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_gather: too many values");
   DeviceState* dev = nullptr;
   rc = current_device(&dev);

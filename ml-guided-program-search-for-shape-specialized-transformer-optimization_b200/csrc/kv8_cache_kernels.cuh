@@ -4,7 +4,7 @@
 // A sequence's tokens lie in blocks of 64.  A block that is full is held as
 // 8-bit codes with one fp32 scale per kv head, for keys and for values:
 //     scale = max |x| / 127 over the block's 64 x D values of the head
-//     code  = rint(x / scale) + 128,       x ~ (code - 128) * scale
+//     code  = rint(x (1 / scale)) + 128,       x ~ (code - 128) * scale
 // The block that is still open is held in bf16 in the sequence's tail.  Its
 // scale is only known when its last token arrives; with the open block in 16
 // bits nothing is ever quantised twice, and a prompt appended at once gives
@@ -62,6 +62,7 @@ struct Kv8AppendArgs {
   int batch, tokens, heads;
   int block_span;                      // blocks a sequence's new tokens can touch
   int64_t kv_ctas;                     // batch * kv_heads * block_span
+  int chunks;                          // query part: as in RopeArgs
   QkNormArgs norm;
 };
 
@@ -114,11 +115,16 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendArgs& a, int b, 
       angles.load(a.norm.rope, fresh ? token : 0, in_head);
       LaneFactors<D, E> f;
       f.set(a.norm.k_weight, angles, a.norm.rope, lane);
-      float y[E], x[E];
+      float y[E];
       norm_rotate<D, E, T>(k_raw[p], y, f, a.norm.k_weight != nullptr, a.norm.eps, angles.turned, a.norm.rope, partner);
-      v_raw[p].values(x);
       k.set(y);
-      v.set(x);
+      if constexpr (sizeof(T) == 2) {
+        v = v_raw[p];
+      } else {
+        float x[E];
+        v_raw[p].values(x);
+        v.set(x);
+      }
     }
     if (fresh && keep) {
       k.store(tail_k + in_block * D);
@@ -135,19 +141,19 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendArgs& a, int b, 
   }
   if (!full) return;
 
-  // The largest magnitude as a bit pattern: the order of non-negative floats,
-  // with infinity and then NaN above every finite value.
-  uint32_t k_max = 0, v_max = 0;
+  // The largest magnitude as a bit pattern, two bf16 at a time: the order of
+  // non-negative floats, with infinity and then NaN above every finite value.
+  uint32_t k_two = 0, v_two = 0;
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
 #pragma unroll
     for (int i = 0; i < E / 2; ++i) {
-      k_max = max(k_max, max((k_bits[p][i] << 16) & 0x7fff0000u, k_bits[p][i] & 0x7fff0000u));
-      v_max = max(v_max, max((v_bits[p][i] << 16) & 0x7fff0000u, v_bits[p][i] & 0x7fff0000u));
+      k_two = __vmaxu2(k_two, k_bits[p][i] & 0x7fff7fffu);
+      v_two = __vmaxu2(v_two, v_bits[p][i] & 0x7fff7fffu);
     }
   }
-  k_max = __reduce_max_sync(0xffffffffu, k_max);
-  v_max = __reduce_max_sync(0xffffffffu, v_max);
+  uint32_t k_max = __reduce_max_sync(0xffffffffu, max(k_two << 16, k_two & 0xffff0000u));
+  uint32_t v_max = __reduce_max_sync(0xffffffffu, max(v_two << 16, v_two & 0xffff0000u));
   __syncthreads();  // a block before this one may still read peak
   if (lane == 0) {
     peak[0][warp] = k_max;
@@ -171,25 +177,35 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendArgs& a, int b, 
   }
   uint8_t* const k_codes = a.cache.codes + at * kKv8Block * D;
   uint8_t* const v_codes = k_codes + static_cast<int64_t>(a.cache.kv_heads) * kKv8Block * D;
-  auto code = [](uint32_t bits, float scale) -> uint32_t {
-    // scale 0: a block of zeros; scale NaN: any code, the scale says it all
-    return scale > 0.f ? static_cast<uint32_t>(__float2int_rn(__uint_as_float(bits) / scale) + 128) : 128u;
+  // scale 0: a block of zeros, codes 128; scale NaN: any code, the scale says it all
+  const float k_inv = k_scale > 0.f ? 1.f / k_scale : 0.f, v_inv = v_scale > 0.f ? 1.f / v_scale : 0.f;
+  // 1.5 2^23 + 128 + x inv, rounded to an integer by the addition: the low byte is the code
+  auto codes = [](uint32_t lo, uint32_t hi, float inv) -> uint32_t {
+    const float shift = 12583040.f;
+    const uint32_t c0 = __float_as_uint(fmaf(__uint_as_float(lo << 16), inv, shift));
+    const uint32_t c1 = __float_as_uint(fmaf(__uint_as_float(lo & 0xffff0000u), inv, shift));
+    const uint32_t c2 = __float_as_uint(fmaf(__uint_as_float(hi << 16), inv, shift));
+    const uint32_t c3 = __float_as_uint(fmaf(__uint_as_float(hi & 0xffff0000u), inv, shift));
+    return __byte_perm(__byte_perm(c0, c1, 0x0040), __byte_perm(c2, c3, 0x0040), 0x5410);
   };
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
     const int in_block = p * PASS + warp * TOKENS + lane / L;
     if (in_block >= kKv8Block) continue;
+    uint32_t kc[E / 4], vc[E / 4];
 #pragma unroll
     for (int i = 0; i < E / 4; ++i) {
-      uint32_t kc = 0, vc = 0;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint32_t kb = k_bits[p][2 * i + j], vb = v_bits[p][2 * i + j];
-        kc |= (code(kb << 16, k_scale) | code(kb & 0xffff0000u, k_scale) << 8) << (16 * j);
-        vc |= (code(vb << 16, v_scale) | code(vb & 0xffff0000u, v_scale) << 8) << (16 * j);
-      }
-      reinterpret_cast<uint32_t*>(k_codes + in_block * D + in_head * E)[i] = kc;
-      reinterpret_cast<uint32_t*>(v_codes + in_block * D + in_head * E)[i] = vc;
+      kc[i] = codes(k_bits[p][2 * i], k_bits[p][2 * i + 1], k_inv);
+      vc[i] = codes(v_bits[p][2 * i], v_bits[p][2 * i + 1], v_inv);
+    }
+    uint8_t* const k_to = k_codes + in_block * D + in_head * E;
+    uint8_t* const v_to = v_codes + in_block * D + in_head * E;
+    if constexpr (E == 8) {
+      *reinterpret_cast<uint2*>(k_to) = make_uint2(kc[0], kc[1]);
+      *reinterpret_cast<uint2*>(v_to) = make_uint2(vc[0], vc[1]);
+    } else {
+      *reinterpret_cast<uint32_t*>(k_to) = kc[0];
+      *reinterpret_cast<uint32_t*>(v_to) = vc[0];
     }
   }
 }
@@ -197,7 +213,7 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendArgs& a, int b, 
 // CTAs below kv_ctas each take one block of one kv head; the rest norm and
 // rotate the queries, a warp for a round of a token's heads as in qk_norm_rope_kernel.
 template <int D, int E, typename T>
-__global__ void __launch_bounds__(kKv8AppendWarps * 32) kv8_append_kernel(Kv8AppendArgs a) {
+__global__ void __launch_bounds__(kKv8AppendWarps * 32, D == 256 ? 1 : 3) kv8_append_kernel(Kv8AppendArgs a) {
   __shared__ uint32_t peak[2][kKv8AppendWarps];
   griddep_wait();
   griddep_launch_dependents();
@@ -229,8 +245,8 @@ __global__ void __launch_bounds__(kKv8AppendWarps * 32) kv8_append_kernel(Kv8App
     }
   }
 
-  constexpr int PER = kRopeUnroll * HeadLanes<D, E>::HEADS;
-  const unsigned rounds = rope_rounds<D, E>(a.heads);
+  const int PER = a.chunks * kRopeUnroll * HeadLanes<D, E>::HEADS;
+  const unsigned rounds = rope_rounds<D, E>(a.heads, a.chunks);
   const unsigned unit = (blockIdx.x - static_cast<unsigned>(a.kv_ctas)) * kKv8AppendWarps + threadIdx.x / 32;
   const unsigned token = unit / rounds;
   if (token >= static_cast<unsigned>(a.batch) * a.tokens) return;
@@ -250,32 +266,45 @@ struct Kv8GatherArgs {
   const int32_t* counts;
   int tokens;        // tokens appended since the lengths were set, where counts is null
   int batch, most;   // tokens given out per sequence
+  int ctas;          // per sequence
   __nv_bfloat16* k;  // [batch, most, kv_heads, D]
   __nv_bfloat16* v;
 };
 
-// Eight values a thread, keys and values: codes in, bf16 out.  Tokens past a
-// sequence's end are zero; a block whose page is not in the table is NaN.
+// Eight codes as bf16 values.
+__device__ __forceinline__ uint4 kv8_values(const uint2& c, float scale) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    // a byte under 2^23 is 2^23 + code
+    const uint32_t two = i < 2 ? c.x : c.y;
+    const float lo = __uint_as_float(__byte_perm(two, 0x4b000000u, i % 2 ? 0x7542 : 0x7540)) - 8388736.f;
+    const float hi = __uint_as_float(__byte_perm(two, 0x4b000000u, i % 2 ? 0x7543 : 0x7541)) - 8388736.f;
+    w[i] = pack_bf16x2(lo * scale, hi * scale);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Eight values a thread, keys and values: codes in, bf16 out (16 bytes, so that a warp's
+// store is whole lines).  Tokens past a sequence's end are zero; a block whose
+// page is not in the table is NaN.
 template <int D>
 __global__ void __launch_bounds__(256) kv8_gather_kernel(Kv8GatherArgs a) {
-  constexpr int PER = D / 8;
+  constexpr unsigned PER = D / 8;
   griddep_wait();
   griddep_launch_dependents();
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t row = at / PER;  // (b, token, head)
-  const int part = static_cast<int>(at % PER) * 8;
-  const int64_t bt = row / a.cache.kv_heads;
-  const int head = static_cast<int>(row % a.cache.kv_heads);
-  const int64_t b = bt / a.most;
-  const int t = static_cast<int>(bt % a.most);
-  if (b >= a.batch) return;
+  const unsigned b = blockIdx.x / a.ctas;
+  const unsigned at = (blockIdx.x - b * a.ctas) * 256 + threadIdx.x;  // (token, head, part)
+  const unsigned row = at / PER, part = at % PER * 8;
+  const unsigned t = row / a.cache.kv_heads, head = row - t * a.cache.kv_heads;
+  if (t >= static_cast<unsigned>(a.most)) return;
   const int slot = a.slot_ids == nullptr ? static_cast<int>(b) : a.slot_ids[b];
   const bool known = slot >= 0 && slot < a.cache.slots;
-  const int total = known ? max(0, a.cache.lengths[slot]) + (a.counts == nullptr ? a.tokens : max(0, a.counts[b])) : 0;
-  uint4 out[2] = {};
-  if (!known) {
-    out[0] = out[1] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
-  } else if (t < total) {
+  const int64_t total =
+      known ? static_cast<int64_t>(max(0, a.cache.lengths[slot])) + (a.counts == nullptr ? a.tokens : max(0, a.counts[b])) : 0;
+  const uint32_t fill = known ? 0u : 0x7fff7fffu;
+  uint4 out[2] = {make_uint4(fill, fill, fill, fill), make_uint4(fill, fill, fill, fill)};
+  if (known && t < total) {
     const int block = t / kKv8Block, in_block = t % kKv8Block;
     if (block == total / kKv8Block) {
 #pragma unroll
@@ -283,26 +312,20 @@ __global__ void __launch_bounds__(256) kv8_gather_kernel(Kv8GatherArgs a) {
         out[kv] = *reinterpret_cast<const uint4*>(kv8_tail(a.cache, slot, block & 1, kv, head, D) + in_block * D + part);
     } else {
       const int page = kv8_page(a.cache, slot, block);
+      const int64_t where = static_cast<int64_t>(max(page, 0)) * 2 * a.cache.kv_heads + head;  // page 0 is always there
+      uint2 c[2];
+      float scale[2];
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
-        float scale = __int_as_float(0x7fffffff);
-        uint2 c = make_uint2(0u, 0u);
-        if (page >= 0) {
-          const int64_t where = (static_cast<int64_t>(page) * 2 + kv) * a.cache.kv_heads + head;
-          scale = a.cache.scales[where];
-          c = *reinterpret_cast<const uint2*>(a.cache.codes + (where * kKv8Block + in_block) * D + part);
-        }
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t two = (i < 2 ? c.x : c.y) >> (16 * (i & 1));
-          w[i] = pack_bf16x2((static_cast<int>(two & 255u) - 128) * scale, (static_cast<int>((two >> 8) & 255u) - 128) * scale);
-        }
-        out[kv] = make_uint4(w[0], w[1], w[2], w[3]);
+        const int64_t w = where + kv * a.cache.kv_heads;
+        scale[kv] = a.cache.scales[w];
+        c[kv] = *reinterpret_cast<const uint2*>(a.cache.codes + (w * kKv8Block + in_block) * D + part);
       }
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) out[kv] = kv8_values(c[kv], page < 0 ? __int_as_float(0x7fffffff) : scale[kv]);
     }
   }
-  const int64_t to = row * D + part;
+  const int64_t to = ((static_cast<int64_t>(b) * a.most + t) * a.cache.kv_heads + head) * D + part;
   *reinterpret_cast<uint4*>(a.k + to) = out[0];
   *reinterpret_cast<uint4*>(a.v + to) = out[1];
 }
