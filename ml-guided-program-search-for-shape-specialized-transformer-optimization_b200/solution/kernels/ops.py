@@ -17,8 +17,13 @@ under meta and fake tensors (tests/solution/test_triton_shape13_attention.py:
 * ``b200tx::linear_residual_layer_norm`` / ``b200tx::mlp_residual_layer_norm``
   -- the fused block boundaries (``sm100_linear_residual_norm`` /
   ``sm100_mlp_residual_norm``), returning ``(residual, normalised)``
+* ``b200tx::qk_norm_rope``         -- ``sm100_qk_norm_rope``
+* ``b200tx::kv8_append``           -- ``sm100_kv8_append`` (writes ``codes``,
+  ``scales`` and ``tail`` of a single-layer cache; returns the queries)
+* ``b200tx::kv8_attention``        -- ``sm100_kv8_attention``
+* ``b200tx::linear_w4``            -- ``sm100_linear_w4``
 
-Each operator is functional: it allocates its outputs and launches on the
+But for ``kv8_append`` each operator is functional: it allocates its outputs and launches on the
 current stream of the inputs' CUDA device.  The kernels are inference-only
 (no autograd formula is registered); an operator runs them with gradient
 recording off whatever the caller's grad mode is.  The fake implementations check
@@ -47,7 +52,10 @@ from .attention import (
     sm100_mma_attention,
     sm100_simt_attention,
 )
+from .kv_cache import KV8_BLOCK, KV8_HEAD_DIMS, Kv8Cache, sm100_kv8_append, sm100_kv8_attention
+from .linear_w4 import W4_GROUPS, W4Weight, sm100_linear_w4
 from .projection import sm100_linear
+from .rotary import ROPE_HEAD_DIMS, RotaryTable, sm100_qk_norm_rope
 
 NAMESPACE = "b200tx"
 OPERATORS = (
@@ -59,6 +67,10 @@ OPERATORS = (
     "layer_norm",
     "linear_residual_layer_norm",
     "mlp_residual_layer_norm",
+    "qk_norm_rope",
+    "kv8_append",
+    "kv8_attention",
+    "linear_w4",
 )
 
 _IO = (torch.float32, torch.bfloat16)
@@ -439,15 +451,228 @@ def _layer_norm_fake(value, weight, bias, eps=1e-5, out_dtype=torch.bfloat16):  
 layer_norm.register_kernel("cpu")(_no_cpu("layer_norm"))
 
 
+# ---------------------------------------------------------------- decoding
+
+
+def _packed_heads(qkv: torch.Tensor, num_heads: int, num_kv_heads: int, head_dims: tuple[int, ...]) -> int:
+    _require(qkv.ndim == 3 and qkv.dtype in _IO, "qkv must be a float32 or bfloat16 [B, T, (H + 2 Hkv) * D] tensor")
+    total = num_heads + 2 * num_kv_heads
+    _require(0 < num_kv_heads <= num_heads and qkv.shape[-1] % total == 0,
+             "the packed width must be (num_heads + 2 * num_kv_heads) * head_dim")
+    head_dim = qkv.shape[-1] // total
+    _require(head_dim in head_dims, f"head_dim {head_dim} is not one of {head_dims}")
+    return head_dim
+
+
+def _rope_check(cos: torch.Tensor | None, sin: torch.Tensor | None, head_dim: int) -> None:
+    _require((cos is None) == (sin is None), "cos and sin come together")
+    if cos is not None:
+        step = 16 if head_dim == 256 else 8
+        _require(cos.ndim == 2 and cos.shape == sin.shape and cos.dtype == sin.dtype == torch.float32
+                 and 0 < 2 * cos.shape[1] <= head_dim and 2 * cos.shape[1] % step == 0,
+                 f"cos and sin must be float32 [positions, rotary / 2], rotary a multiple of {step} up to head_dim")
+
+
+def _rope(cos: torch.Tensor | None, sin: torch.Tensor | None, interleaved: bool) -> RotaryTable | None:
+    return None if cos is None else RotaryTable(cos.contiguous(), sin.contiguous(), interleaved=interleaved)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::qk_norm_rope", mutates_args=(), device_types="cuda")
+def qk_norm_rope(
+    qkv: torch.Tensor,
+    num_heads: int,
+    num_kv_heads: int,
+    q_weight: torch.Tensor | None = None,
+    k_weight: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    cos: torch.Tensor | None = None,
+    sin: torch.Tensor | None = None,
+    interleaved: bool = False,
+    positions: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Query and key heads of the packed projection normed and turned."""
+
+    _rope_check(cos, sin, _packed_heads(qkv, num_heads, num_kv_heads, ROPE_HEAD_DIMS))
+    with torch.no_grad():
+        out, _ = sm100_qk_norm_rope(
+            qkv.contiguous(), num_heads, num_kv_heads, q_weight=q_weight, k_weight=k_weight, eps=eps,
+            rope=_rope(cos, sin, interleaved), positions=positions,
+        )
+    return out
+
+
+@qk_norm_rope.register_fake
+def _qk_norm_rope_fake(qkv, num_heads, num_kv_heads, q_weight=None, k_weight=None, eps=1e-6,  # noqa: ANN001
+                       cos=None, sin=None, interleaved=False, positions=None):  # noqa: ANN001, ANN202, ARG001
+    _rope_check(cos, sin, _packed_heads(qkv, num_heads, num_kv_heads, ROPE_HEAD_DIMS))
+    return qkv.new_empty(qkv.shape)
+
+
+qk_norm_rope.register_kernel("cpu")(_no_cpu("qk_norm_rope"))
+
+
+def _cache_check(
+    codes: torch.Tensor, scales: torch.Tensor, tail: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor
+) -> tuple[int, int]:
+    _require(codes.ndim == 5 and codes.dtype == torch.uint8 and codes.shape[1] == 2 and codes.shape[3] == KV8_BLOCK
+             and codes.shape[4] in KV8_HEAD_DIMS, "codes must be a uint8 [pages, 2, Hkv, 64, D] tensor")
+    pages, _, kv_heads, _, head_dim = codes.shape
+    slots = page_table.shape[0]
+    _require(scales.dtype == torch.float32 and tuple(scales.shape) == (pages, 2, kv_heads),
+             "scales must be a float32 [pages, 2, Hkv] tensor")
+    _require(tail.dtype == torch.bfloat16 and tuple(tail.shape) == (slots, 2, 2, kv_heads, KV8_BLOCK, head_dim),
+             "tail must be a bfloat16 [slots, 2, 2, Hkv, 64, D] tensor")
+    _require(page_table.dtype == torch.int32 and page_table.ndim == 2 and lengths.dtype == torch.int32
+             and tuple(lengths.shape) == (slots,), "page_table must be int32 [slots, max_blocks] and lengths int32 [slots]")
+    return kv_heads, head_dim
+
+
+def _append_shape(qkv: torch.Tensor, num_heads: int, kv_heads: int, head_dim: int) -> tuple[int, int, int, int]:
+    _require(_packed_heads(qkv, num_heads, kv_heads, KV8_HEAD_DIMS) == head_dim,
+             "qkv and the cache disagree on head_dim")
+    return qkv.shape[0], qkv.shape[1], num_heads, head_dim
+
+
+@torch.library.custom_op(f"{NAMESPACE}::kv8_append", mutates_args=("codes", "scales", "tail"), device_types="cuda")
+def kv8_append(
+    codes: torch.Tensor,
+    scales: torch.Tensor,
+    tail: torch.Tensor,
+    page_table: torch.Tensor,
+    lengths: torch.Tensor,
+    qkv: torch.Tensor,
+    num_heads: int,
+    q_weight: torch.Tensor | None = None,
+    k_weight: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    cos: torch.Tensor | None = None,
+    sin: torch.Tensor | None = None,
+    interleaved: bool = False,
+    slots: torch.Tensor | None = None,
+    counts: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """The packed projection's keys and values appended to the cache; returns the queries."""
+
+    kv_heads, head_dim = _cache_check(codes, scales, tail, page_table, lengths)
+    _append_shape(qkv, num_heads, kv_heads, head_dim)
+    _rope_check(cos, sin, head_dim)
+    with torch.no_grad():
+        q, _ = sm100_kv8_append(
+            Kv8Cache(codes, scales, tail, page_table, lengths), qkv.contiguous(), num_heads, q_weight=q_weight,
+            k_weight=k_weight, eps=eps, rope=_rope(cos, sin, interleaved), slots=slots, counts=counts,
+        )
+    return q
+
+
+@kv8_append.register_fake
+def _kv8_append_fake(codes, scales, tail, page_table, lengths, qkv, num_heads, q_weight=None, k_weight=None,  # noqa: ANN001
+                     eps=1e-6, cos=None, sin=None, interleaved=False, slots=None, counts=None):  # noqa: ANN001, ANN202, ARG001
+    kv_heads, head_dim = _cache_check(codes, scales, tail, page_table, lengths)
+    _rope_check(cos, sin, head_dim)
+    return qkv.new_empty(_append_shape(qkv, num_heads, kv_heads, head_dim), dtype=torch.bfloat16)
+
+
+kv8_append.register_kernel("cpu")(_no_cpu("kv8_append"))
+
+
+def _kv8_attention_shape(q: torch.Tensor, kv_heads: int, head_dim: int, scale: float) -> tuple[int, int, int]:
+    _require(q.ndim == 4 and q.dtype == torch.bfloat16 and q.shape[3] == head_dim and q.shape[2] % kv_heads == 0,
+             "q must be a bfloat16 [B, T, H, D] tensor, H a multiple of the cache's heads")
+    _require(scale >= 0.0, "scale must be positive, or 0 for D ** -0.5")
+    return q.shape[0], q.shape[1], q.shape[2] * head_dim
+
+
+@torch.library.custom_op(f"{NAMESPACE}::kv8_attention", mutates_args=(), device_types="cuda")
+def kv8_attention(
+    codes: torch.Tensor,
+    scales: torch.Tensor,
+    tail: torch.Tensor,
+    page_table: torch.Tensor,
+    lengths: torch.Tensor,
+    q: torch.Tensor,
+    scale: float = 0.0,
+    slots: torch.Tensor | None = None,
+    counts: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of the tokens appended last over the cache (``scale`` 0: ``D ** -0.5``)."""
+
+    kv_heads, head_dim = _cache_check(codes, scales, tail, page_table, lengths)
+    _kv8_attention_shape(q, kv_heads, head_dim, scale)
+    with torch.no_grad():
+        out, _ = sm100_kv8_attention(
+            Kv8Cache(codes, scales, tail, page_table, lengths), q.contiguous(), scale=scale or None, slots=slots,
+            counts=counts,
+        )
+    return out
+
+
+@kv8_attention.register_fake
+def _kv8_attention_fake(codes, scales, tail, page_table, lengths, q, scale=0.0,  # noqa: ANN001
+                        slots=None, counts=None):  # noqa: ANN001, ANN202, ARG001
+    kv_heads, head_dim = _cache_check(codes, scales, tail, page_table, lengths)
+    return q.new_empty(_kv8_attention_shape(q, kv_heads, head_dim, scale))
+
+
+kv8_attention.register_kernel("cpu")(_no_cpu("kv8_attention"))
+
+
+def _linear_w4_shape(
+    value: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None, out_dtype: torch.dtype
+) -> tuple[int, ...]:
+    _require(value.dtype == torch.bfloat16 and value.ndim >= 1, "value must be a bfloat16 [..., K] tensor")
+    inner = value.shape[-1]
+    wide = -(-inner // 128) * 128
+    _require(inner > 0 and inner % 8 == 0 and packed.dtype == torch.uint8 and packed.ndim == 2
+             and packed.shape[1] == wide // 2, "packed must be a uint8 [N, Kp / 2] tensor, K a multiple of 8")
+    _require(scales.dtype == torch.bfloat16 and scales.ndim == 2 and scales.shape[1] == packed.shape[0]
+             and scales.shape[0] > 0 and wide % scales.shape[0] == 0 and wide // scales.shape[0] in W4_GROUPS,
+             "scales must be a bfloat16 [Kp / group, N] tensor, group 32, 64 or 128")
+    if bias is not None:
+        _require(bias.dtype == torch.float32 and tuple(bias.shape) == (packed.shape[0],), "bias must be float32 [N]")
+    _require(out_dtype in _IO, "out_dtype must be float32 or bfloat16")
+    return (*value.shape[:-1], packed.shape[0])
+
+
+@torch.library.custom_op(f"{NAMESPACE}::linear_w4", mutates_args=(), device_types="cuda")
+def linear_w4(
+    value: torch.Tensor,
+    packed: torch.Tensor,
+    scales: torch.Tensor,
+    bias: torch.Tensor | None = None,
+    gelu: bool = False,
+    out_dtype: torch.dtype = torch.bfloat16,
+) -> torch.Tensor:
+    """``epilogue(value . W^T + bias)`` with a 4-bit weight (``W4Weight``'s tensors)."""
+
+    _linear_w4_shape(value, packed, scales, bias, out_dtype)
+    with torch.no_grad():
+        out, _ = sm100_linear_w4(
+            value.contiguous(), W4Weight(packed, scales, value.shape[-1]), bias, gelu=gelu, out_dtype=out_dtype
+        )
+    return out
+
+
+@linear_w4.register_fake
+def _linear_w4_fake(value, packed, scales, bias=None, gelu=False, out_dtype=torch.bfloat16):  # noqa: ANN001, ANN202, ARG001
+    return value.new_empty(_linear_w4_shape(value, packed, scales, bias, out_dtype), dtype=out_dtype)
+
+
+linear_w4.register_kernel("cpu")(_no_cpu("linear_w4"))
+
+
 __all__ = [
     "NAMESPACE",
     "OPERATORS",
     "flash_attention",
+    "kv8_append",
+    "kv8_attention",
     "layer_norm",
     "linear",
     "linear_residual_layer_norm",
+    "linear_w4",
     "mlp_residual_layer_norm",
     "mma_attention",
+    "qk_norm_rope",
     "residual_layer_norm",
     "simt_attention",
 ]
