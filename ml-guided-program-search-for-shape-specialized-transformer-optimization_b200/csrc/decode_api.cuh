@@ -187,15 +187,15 @@ template <int TN, int RT, int GROUP>
 cudaError_t launch_w4(b200tx::W4Args& a, DeviceState* dev, int index, cudaStream_t stream) {
   constexpr int kMost = 112 * 1024;  // two CTAs for each SM
   if (!dev->w4_attr[index]) {
-    cudaError_t err =
-        cudaFuncSetAttribute(b200tx::linear_w4_kernel<TN, RT, GROUP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+    cudaError_t err = cudaFuncSetAttribute(b200tx::linear_w4_kernel<TN, RT, GROUP>,
+                                           cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
     if (err != cudaSuccess) return err;
     dev->w4_attr[index] = true;
   }
   // Slices of K: the fewest (they are joined at the end) that give most SMs a second
   // CTA (1 x 8192 -> 8192: 128 CTAs 20.3 us, 256 CTAs 15.9; 8 x 8192 -> 28672:
   // 224 CTAs 38.6 us, 448 CTAs 41.9).
-  const int tiles = (a.outer + 16 * RT - 1) / (16 * RT), all_stages = (a.runs + 1) / 2;
+  const int tiles = (a.outer + 16 * RT - 1) / (16 * RT), all_stages = (a.runs + b200tx::kW4Runs - 1) / b200tx::kW4Runs;
   a.slices = 1;
   while (a.slices < b200tx::kW4Warps && a.slices < all_stages &&
          (tiles * a.slices + b200tx::kW4Warps - 1) / b200tx::kW4Warps < dev->sm_count * 5 / 4 &&
@@ -470,10 +470,12 @@ int b200tx_linear_w4(const void* x, int64_t x_stride, const void* packed, const 
   a.runs = static_cast<int>((K + b200tx::kW4Run - 1) / b200tx::kW4Run);
   a.gelu = epilogue == B200TX_EPI_BIAS_GELU;
   a.out_f32 = out_dtype == B200TX_F32;
-  // rows of x by eights: 1, 2 or 4 MMA columns; past 32 the weights are read again
-  cudaError_t err = M <= 8    ? launch_w4_tiles<1>(group, a, dev, 0, stream)
-                    : M <= 16 ? launch_w4_tiles<2>(group, a, dev, 6, stream)
-                              : launch_w4_tiles<4>(group, a, dev, 12, stream);
+  // Rows of x by eights: 1, 2 or 4 MMA columns.  Four only where the columns of W
+  // fill the SMs; with fewer the rows go 16 at a time, which makes twice the CTAs
+  // and reads the weights again from L2 (29 x 4744 -> 5003: four 23.9 us, twice two WWW).
+  cudaError_t err = M <= 8                                     ? launch_w4_tiles<1>(group, a, dev, 0, stream)
+                    : M <= 16 || a.outer < 80 * dev->sm_count ? launch_w4_tiles<2>(group, a, dev, 6, stream)
+                                                               : launch_w4_tiles<4>(group, a, dev, 12, stream);
   return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "linear_w4");
 }
 

@@ -15,10 +15,10 @@
 //
 // The weights are the A operand (m16: output columns), x the B operand (n8: rows
 // of x), so 8 rows of x cost one MMA.  A CTA is 8 warps: 8 / KS tiles of 16 RT
-// columns x KS slices of K.  A slice goes through K 256 weights at a time, weights
-// and x by cp.async into a ring (8 lanes copy one 128-byte line, chunks permuted by
-// the row so that the fragments are read without bank conflicts); its warps
-// share x.  The sum of a group is multiplied by its scale and added in fp32; the
+// columns x KS slices of K.  A slice goes through K two runs at a time, weights
+// and x by cp.async into a ring (8 lanes copy one 128-byte line of two runs, chunks
+// permuted by the row so that the fragments are read without bank conflicts); its
+// warps share x.  The sum of a group is multiplied by its scale and added in fp32; the
 // slices are joined in shared memory in a fixed order.
 #pragma once
 
@@ -28,8 +28,8 @@
 namespace b200tx {
 
 constexpr int kW4Warps = 8;
-constexpr int kW4Run = 128;    // weights of a row that lie together
-constexpr int kW4Stage = 256;  // weights of a row in a stage
+constexpr int kW4Run = 128;   // weights of a row that lie together
+constexpr int kW4Runs = 2;    // runs of a stage: a whole line
 
 struct W4Args {
   const __nv_bfloat16* x;        // [M, K]
@@ -55,10 +55,19 @@ __device__ __forceinline__ uint32_t nibbles_bf16x2(uint32_t w) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// d = a b
+__device__ __forceinline__ void mma_m16n8k16_bf16_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+      "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};\n"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 // Bytes of a ring stage: 8 warps' weights, then the slices' x.
 template <int TN, int RT>
 constexpr int w4_stage_bytes(int slices) {
-  return kW4Warps * RT * 16 * (kW4Stage / 2) + slices * TN * 8 * kW4Stage * 2;
+  return kW4Warps * RT * 16 * (kW4Runs * kW4Run / 2) + slices * TN * 8 * kW4Runs * kW4Run * 2;
 }
 
 // TN: n8 tiles of x rows; RT: m16 tiles of columns of a warp.
@@ -66,8 +75,13 @@ template <int TN, int RT, int GROUP>
 __global__ void __launch_bounds__(kW4Warps * 32, 2) linear_w4_kernel(W4Args a) {
   constexpr int GROUPS = kW4Run / GROUP;  // groups per run
   constexpr int WORDS = 4 / GROUPS;       // words per group and lane
-  constexpr int W_BYTES = RT * 16 * (kW4Stage / 2);  // of a warp's stage
-  constexpr int X_BYTES = TN * 8 * kW4Stage * 2;     // of a slice's stage
+  constexpr int STAGE = kW4Runs * kW4Run;               // weights of a row in a stage
+  constexpr int ROW = STAGE / 2;                     // their bytes
+  constexpr int W_BYTES = RT * 16 * ROW;             // of a warp's stage
+  constexpr int X_ROW = STAGE * 2;                   // bytes of a row of x
+  constexpr int X_BYTES = TN * 8 * X_ROW;            // of a slice's stage
+  constexpr int CHUNKS = ROW / 16, ROWS_A_COPY = 32 / CHUNKS;
+  constexpr int COPIES = RT * 16 / ROWS_A_COPY;
   extern __shared__ __align__(128) uint8_t w4_smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t4 = lane % 4;
   const int per = kW4Warps / a.slices;  // warps of a slice
@@ -75,49 +89,53 @@ __global__ void __launch_bounds__(kW4Warps * 32, 2) linear_w4_kernel(W4Args a) {
   const int n0 = (blockIdx.x * per + tile) * (16 * RT);
   const int m0 = blockIdx.y * (TN * 8);
   const int stage_bytes = kW4Warps * W_BYTES + a.slices * X_BYTES;
-  const int all_stages = (a.runs + 1) / 2, each = (all_stages + a.slices - 1) / a.slices;
+  const int all_stages = (a.runs + kW4Runs - 1) / kW4Runs, each = (all_stages + a.slices - 1) / a.slices;
   const int begin = min(all_stages, slice * each), count = min(all_stages, begin + each) - begin;
   griddep_wait();
   griddep_launch_dependents();
 
-  // ---- copies: 4 rows x 128 bytes of weights at a time, and this thread's share of the slice's x
+  // ---- copies: 512 bytes of weights (4 or 8 rows) at a time, and this warp's rows of the slice's x
   const int64_t pitch = static_cast<int64_t>(a.runs) * (kW4Run / 2);
   const int first_row = min(n0, a.outer - 1);  // columns past the end read the last one and are not written
-  const uint8_t* const w_src = a.packed + first_row * pitch + lane % 8 * 16;
-  unsigned w_off[RT * 4];
+  const uint8_t* const w_src = a.packed + first_row * pitch + lane % CHUNKS * 16;
+  unsigned w_off[COPIES];
 #pragma unroll
-  for (int i = 0; i < RT * 4; ++i)
-    w_off[i] = static_cast<unsigned>(min(n0 + i * 4 + lane / 8, a.outer - 1) - first_row) * static_cast<unsigned>(pitch);
+  for (int i = 0; i < COPIES; ++i)
+    w_off[i] = static_cast<unsigned>(min(n0 + i * ROWS_A_COPY + lane / CHUNKS, a.outer - 1) - first_row) * static_cast<unsigned>(pitch);
   const uint32_t ring = smem_u32(w4_smem);
   const uint32_t w_put = ring + warp * W_BYTES + kv8_k_place<128>(lane * 16);
+  static_assert(X_ROW == 512, "a copy of 32 lanes is a row of x");
+  const __nv_bfloat16* const x_src = a.x + (m0 + tile) * a.x_stride + lane * 8;
+  const int64_t x_step = per * a.x_stride;
+  const uint32_t x_put = ring + kW4Warps * W_BYTES + slice * X_BYTES + tile * X_ROW;
   auto issue = [&](int s) {
     if (s < count) {
       const int at = begin + s;
       const uint32_t stage = (s % a.stages) * stage_bytes;
-      const bool take = at * 2 + (lane % 8) / 4 < a.runs;
+      const bool take = at * kW4Runs + (lane % CHUNKS) / 4 < a.runs;
 #pragma unroll
-      for (int i = 0; i < RT * 4; ++i)
-        cp_async_or_zero(w_put + stage + i * 512, w_src + w_off[i] + static_cast<int64_t>(at) * 128, take);
-      // x: 32 chunks of 16 bytes a row, a warp copies whole rows
-      for (int row = tile; row < TN * 8; row += per) {
-        const int m = m0 + row, k = at * kW4Stage + lane * 8;
-        const bool in = m < a.rows && k < a.inner;
-        cp_async_or_zero(ring + stage + kW4Warps * W_BYTES + slice * X_BYTES + row * 512 + ((lane * 16) ^ ((row & 1) << 6)),
-                         a.x + (in ? m * a.x_stride + k : 0), in);
-      }
+      for (int i = 0; i < COPIES; ++i)
+        cp_async_or_zero(w_put + stage + i * 512, w_src + w_off[i] + static_cast<int64_t>(at) * ROW, take);
+      // x rows tile, tile + per, ... of the CTA's; a row is a copy
+      const __nv_bfloat16* from = x_src + at * STAGE;
+      uint32_t to = x_put + stage;
+      const int left = at * STAGE + lane * 8 < a.inner ? a.rows - m0 : 0;
+      for (int row = tile; row < TN * 8; row += per, from += x_step, to += per * X_ROW)
+        cp_async_or_zero(to + ((row & 1) << 6 ^ lane * 16), row < left ? from : a.x, row < left);
     }
     cp_async_commit();
   };
   for (int s = 0; s < a.stages - 1; ++s) issue(s);
 
-  // ---- scales: lane = a column of the tile, RT GROUPS registers for a stage's 2 GROUPS groups
-  constexpr int SCALES = RT * GROUPS;
+  // ---- scales: lane = a column of the tile (RT 2), or of one of two groups (RT 1)
+  constexpr int STAGE_GROUPS = kW4Runs * GROUPS;
+  constexpr int SCALES = (STAGE_GROUPS * RT + 1) / 2;
   const int s_col = min(n0 + lane % (16 * RT), a.outer - 1);
   const int all_groups = a.runs * GROUPS;
   auto load_scales = [&](int s, uint16_t (&to)[SCALES]) {
 #pragma unroll
     for (int i = 0; i < SCALES; ++i) {
-      const int q = (begin + s) * 2 * GROUPS + (RT == 2 ? i : 2 * i + lane / 16);
+      const int q = (begin + s) * STAGE_GROUPS + (RT == 2 ? i : 2 * i + lane / 16);
       to[i] = 0;
       if (s < count && q < all_groups)
         to[i] = __ldg(reinterpret_cast<const uint16_t*>(a.scales) + static_cast<int64_t>(q) * a.outer + s_col);
@@ -128,7 +146,7 @@ __global__ void __launch_bounds__(kW4Warps * 32, 2) linear_w4_kernel(W4Args a) {
 
   float sum[RT][TN][4] = {};
   const uint32_t w_get = warp * W_BYTES + kv8_k_place<128>(g * 128 + t4 * 16);
-  const uint32_t x_get = kW4Warps * W_BYTES + slice * X_BYTES + g * 512;
+  const uint32_t x_get = kW4Warps * W_BYTES + slice * X_BYTES + g * X_ROW;
   const uint32_t x_low = (t4 * 16) ^ ((g & 1) << 6);
 #pragma unroll 1
   for (int s = 0; s < count; ++s) {
@@ -140,12 +158,12 @@ __global__ void __launch_bounds__(kW4Warps * 32, 2) linear_w4_kernel(W4Args a) {
     load_scales(s + 1, next_scales);
     const uint8_t* const stage = w4_smem + (s % a.stages) * stage_bytes;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
+    for (int r = 0; r < kW4Runs; ++r) {
       uint32_t w[RT][2][4];
 #pragma unroll
       for (int i = 0; i < RT; ++i) {
-        lds_words<16>(stage + (w_get ^ (r * 64)) + i * 2048, w[i][0]);
-        lds_words<16>(stage + (w_get ^ (r * 64)) + i * 2048 + 1024, w[i][1]);
+        lds_words<16>(stage + (w_get ^ (r * 64)) + i * 16 * ROW, w[i][0]);
+        lds_words<16>(stage + (w_get ^ (r * 64)) + i * 16 * ROW + 8 * ROW, w[i][1]);
       }
 #pragma unroll
       for (int q = 0; q < GROUPS; ++q) {
@@ -155,7 +173,7 @@ __global__ void __launch_bounds__(kW4Warps * 32, 2) linear_w4_kernel(W4Args a) {
           uint32_t xf[TN][4];
 #pragma unroll
           for (int j = 0; j < TN; ++j)
-            lds_words<16>(stage + x_get + (x_low ^ ((c & 1) << 6)) + (c >> 1) * 128 + r * 256 + j * 4096, xf[j]);
+            lds_words<16>(stage + x_get + (x_low ^ ((c & 1) << 6)) + (c >> 1) * 128 + r * 256 + j * 8 * X_ROW, xf[j]);
 #pragma unroll
           for (int i = 0; i < RT; ++i) {
             const uint32_t wa = w[i][0][c], wb = w[i][1][c];
@@ -164,8 +182,11 @@ __global__ void __launch_bounds__(kW4Warps * 32, 2) linear_w4_kernel(W4Args a) {
                                     nibbles_bf16x2(wb >> 12)};
 #pragma unroll
             for (int j = 0; j < TN; ++j) {
-              if (c == q * WORDS) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.f;
-              mma_m16n8k16_bf16(acc[i][j], a0, xf[j][0], xf[j][1]);
+              if (c == q * WORDS) {
+                mma_m16n8k16_bf16_first(acc[i][j], a0, xf[j][0], xf[j][1]);
+              } else {
+                mma_m16n8k16_bf16(acc[i][j], a0, xf[j][0], xf[j][1]);
+              }
               mma_m16n8k16_bf16(acc[i][j], a1, xf[j][2], xf[j][3]);
             }
           }
