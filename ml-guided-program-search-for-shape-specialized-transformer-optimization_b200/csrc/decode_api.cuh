@@ -421,7 +421,7 @@ int b200tx_kv8_attention(const b200tx_kv8_cache* cache, const void* q, void* out
   const int groups = kv8_row_groups(cache->head_dim, tokens * a.group);
   // all steps of the longest sequences that the page table can hold, and the tiles' own cost
   const double units = static_cast<double>(batch) * cache->kv_heads * ((tokens * a.group + 8 * groups - 1) / (8 * groups)) *
-                       (2.0 * cache->max_blocks + 4 + b200tx::kKv8TileCost);
+                       (4.0 * cache->max_blocks + 8 + b200tx::kKv8TileCost);
   if (units >= 4294967296.0)
     return fail(B200TX_ERR_UNSUPPORTED, "kv8_attention: batch x heads x rows x blocks of this call pass 2^32 steps");
   switch (cache->head_dim + groups) {
@@ -472,7 +472,7 @@ int b200tx_linear_w4(const void* x, int64_t x_stride, const void* packed, const 
   a.out_f32 = out_dtype == B200TX_F32;
   // Rows of x by eights: 1, 2 or 4 MMA columns.  Four only where the columns of W
   // fill the SMs; with fewer the rows go 16 at a time, which makes twice the CTAs
-  // and reads the weights again from L2 (29 x 4744 -> 5003: four 23.9 us, twice two 20.7).
+  // and reads the weights again from L2 (29 x 4744 -> 5003: four 23.9 us, twice two 22.4).
   cudaError_t err = M <= 8                                     ? launch_w4_tiles<1>(group, a, dev, 0, stream)
                     : M <= 16 || a.outer < 80 * dev->sm_count ? launch_w4_tiles<2>(group, a, dev, 6, stream)
                                                                : launch_w4_tiles<4>(group, a, dev, 12, stream);

@@ -10,8 +10,8 @@
 // equal share of them whatever the lengths are.
 //
 // Split.  The rows of a (sequence, kv head) are its tokens x the query heads of
-// the group, in tiles of 8 NR.  A tile's keys are cut into steps of 32 or 64 codes
-// (half as many tokens in the open block: as many bytes).  All steps of all tiles, and a
+// the group, in tiles of 8 NR.  A tile's keys are cut into steps of 16 to 64 codes,
+// 8 KB of keys and values (4 KB for head_dim 32), and half as many tokens in the open block.  All steps of all tiles, and a
 // fixed cost for each tile, form one line, cut into equal ranges, one per CTA: a
 // CTA ends within a tile's keys, or does several tiles, and no length of any
 // sequence leaves SMs idle.  A tile that lies in several CTAs is joined by the
@@ -52,6 +52,7 @@ namespace b200tx {
 
 constexpr int kKv8Warps = 4;
 constexpr int kKv8TileCost = 12;  // what beginning and joining a tile costs, in steps (64 ragged sequences: 6 42.3 us, 12 34.5, 24 37.8)
+constexpr float kKv8JoinShare = 0.5f;  // what a part costs to join, against a step: its root
 constexpr float kKv8Headroom = 8.f;  // log2 of how far a score may pass the running maximum
 constexpr float kKv8Unit = 16777216.f;  // 2^24: a code's fp16 number is code / 2^24
 constexpr uint32_t kKv8OffsetF16 = 0x80808080u;   // two fp16 -2^-17 = -128 / 2^24
@@ -60,11 +61,13 @@ constexpr float kKv8SumUnit = -131072.f;          // -2^17
 
 template <int D, int NR>
 struct Kv8Shape {
-  static constexpr int TOK = D <= 64 ? 64 : 32;       // tokens per step in full blocks
+  static constexpr int TOK = D <= 64 ? 64 : D == 128 ? 32 : 16;  // tokens per step in full blocks
   static constexpr int TAIL = TOK / 2;                // and in the open block
   static constexpr int T16 = TOK / 16;
+  static constexpr int TAIL16 = TAIL < 16 ? 1 : TAIL / 16;  // tiles of a step in the open block,
+  static constexpr bool TAIL_HALF = TAIL < 16;              // the only one half empty
   static constexpr int STAGES = D == 32 ? 4 : D == 64 ? 2 : 3;
-  static constexpr int CTAS = D == 256 ? 1 : D == 128 || NR == 4 ? 2 : 3;  // per SM
+  static constexpr int CTAS = D >= 128 || NR == 4 ? 2 : 3;  // per SM
   static constexpr int ROWS = 8 * NR;                 // rows per tile
   static constexpr int KB = D / 4 < 16 ? D / 4 : 16;  // bytes per key copy
   static constexpr int KC = D / 4 / KB;               // key copies per row and lane
@@ -76,6 +79,7 @@ struct Kv8Shape {
   static constexpr int MT = D / 16;                   // m16 tiles of the output
   static constexpr int FRAGS = MT * NR;               // fragments (4 floats a lane) of the output
   static constexpr int SHARE = FRAGS >= kKv8Warps ? FRAGS / kKv8Warps : 1;  // of one warp, when joining
+  static_assert(SHARE <= MT && MT % SHARE == 0, "a warp's share lies in one row group");
   static constexpr int RING = kKv8Warps * STAGES * STAGE;
   static constexpr int JOIN = kKv8Warps * ROWS * D * 4;  // the warps' outputs, over the ring
   static constexpr int MAIN = RING > JOIN ? RING : JOIN;
@@ -266,8 +270,13 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
     all += scan[w];
   }
   const unsigned total = all * tiles;  // the host has checked that it fits
-  // at least a step for each warp, so that short contexts are not cut into crumbs
-  const unsigned ctas = min((total + kKv8Warps - 1) / kKv8Warps, gridDim.x);
+  // Units of a CTA: at least a step for each warp, so that short contexts are not cut
+  // into crumbs; and where few long tiles are left to all CTAs, not so few that joining
+  // a tile's n parts takes longer than reading its units / n (their sum is least at
+  // n ~ sqrt(units); by the mean tile: 32768 tokens of one kv head 31.6 -> 16.4 us).
+  const float mean_units = __fdividef(static_cast<float>(all), static_cast<float>(a.batch));
+  const float least_units = fmaxf(kKv8Warps, kKv8JoinShare * __fsqrt_rn(mean_units));
+  const unsigned ctas = min(static_cast<unsigned>(__fdividef(static_cast<float>(total), least_units)) + (total != 0), gridDim.x);
   if (blockIdx.x >= ctas) return;
   Kv8Ranges ranges;
   ranges.each = total / ctas;
@@ -439,7 +448,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
     }
 
     // Sums s (tokens 16 i + g and + 8, rows 2 t and 2 t + 1) to probabilities 2^(s factor - m).
-    auto softmax = [&](auto& s, float (&factor)[NR][2], int first_token, bool masked) {
+    auto softmax = [&](auto& s, float (&factor)[NR][2], int first_token, bool masked, bool half) {
       constexpr int TILES = sizeof(s) / sizeof(s[0]);
       float top[NR][2];
       bool above = false;
@@ -456,7 +465,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
             for (int i = 0; i < TILES; ++i) {
 #pragma unroll
               for (int h = 0; h < 2; ++h)
-                if (first_token + i * 16 + h * 8 + g > limit[r][e]) s[i][r][2 * h + e] = minus_inf;
+                if (first_token + i * 16 + h * 8 + g > limit[r][e] || (half && h == 1)) s[i][r][2 * h + e] = minus_inf;
             }
           }
 #pragma unroll
@@ -545,7 +554,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
           factor[r][0] = row_scale[r][0] * k_unit;
           factor[r][1] = row_scale[r][1] * k_unit;
         }
-        softmax(s, factor, first_token, masked);
+        softmax(s, factor, first_token, masked, false);
         uint32_t p[S::T16][NR][2];
         float v_start[NR][2], v_scale[NR][2];
 #pragma unroll
@@ -608,14 +617,14 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
           }
         }
       } else {
-        constexpr int TT = S::T16 / 2;  // 16-token groups
+        constexpr int TT = S::TAIL16;  // 16-token groups
         const int first_token = full * kKv8Block + (step - coded_steps) * S::TAIL;
         float s[TT][NR][4];
 #pragma unroll
         for (int c = 0; c < 2 * S::KC; ++c) {
           uint32_t w[2 * TT][S::KB / 4];
 #pragma unroll
-          for (int n = 0; n < 2 * TT; ++n)
+          for (int n = 0; n < S::TAIL / 8; ++n)
             lds_words<S::KB>(stage + (tail_k_at ^ (c % 2 * S::KB)) + c / 2 * 128 + n * 16 * D, w[n]);
 #pragma unroll
           for (int i = 0; i < S::KB / 8; ++i) {
@@ -632,9 +641,11 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
 #pragma unroll
             for (int t = 0; t < TT; ++t) {
               const uint32_t(&wa)[S::KB / 4] = w[2 * t];
-              const uint32_t(&wb)[S::KB / 4] = w[2 * t + 1];
-              const uint32_t kf[4] = {__byte_perm(wa[2 * i], wa[2 * i + 1], 0x5410), __byte_perm(wb[2 * i], wb[2 * i + 1], 0x5410),
-                                      __byte_perm(wa[2 * i], wa[2 * i + 1], 0x7632), __byte_perm(wb[2 * i], wb[2 * i + 1], 0x7632)};
+              const uint32_t(&wb)[S::KB / 4] = w[S::TAIL_HALF ? 0 : 2 * t + 1];
+              const uint32_t kf[4] = {__byte_perm(wa[2 * i], wa[2 * i + 1], 0x5410),
+                                      S::TAIL_HALF ? 0u : __byte_perm(wb[2 * i], wb[2 * i + 1], 0x5410),
+                                      __byte_perm(wa[2 * i], wa[2 * i + 1], 0x7632),
+                                      S::TAIL_HALF ? 0u : __byte_perm(wb[2 * i], wb[2 * i + 1], 0x7632)};
 #pragma unroll
               for (int r = 0; r < NR; ++r) {
                 if (ks == 0) s[t][r][0] = s[t][r][1] = s[t][r][2] = s[t][r][3] = 0.f;
@@ -649,7 +660,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
           factor[r][0] = row_scale[r][0];
           factor[r][1] = row_scale[r][1];
         }
-        softmax(s, factor, first_token, true);
+        softmax(s, factor, first_token, true, S::TAIL_HALF);
         uint32_t high[TT][NR][2], low[TT][NR][2];
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
@@ -692,16 +703,18 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
             for (int h = 0; h < 2; ++h) {
               uint32_t w[4 * TT][S::VB / 4];
 #pragma unroll
-              for (int i = 0; i < 4 * TT; ++i)
+              for (int i = 0; i < S::TAIL / 4; ++i)
                 lds_words<S::VB>(stage + S::HALF + (tail_v_at ^ (h * S::VB)) + c * 256 +
                                      ((i / 4) * 16 + (i & 1) + (i >> 1 & 1) * 8) * 2 * D, w[i]);
 #pragma unroll
               for (int i = 0; i < S::VB / 4; ++i) {
 #pragma unroll
                 for (int t = 0; t < TT; ++t) {
+                  constexpr int C = S::TAIL_HALF ? 0 : 2;
                   const uint32_t vf[4] = {
                       __byte_perm(w[4 * t][i], w[4 * t + 1][i], 0x5410), __byte_perm(w[4 * t][i], w[4 * t + 1][i], 0x7632),
-                      __byte_perm(w[4 * t + 2][i], w[4 * t + 3][i], 0x5410), __byte_perm(w[4 * t + 2][i], w[4 * t + 3][i], 0x7632)};
+                      S::TAIL_HALF ? 0u : __byte_perm(w[4 * t + C][i], w[4 * t + C + 1][i], 0x5410),
+                      S::TAIL_HALF ? 0u : __byte_perm(w[4 * t + C][i], w[4 * t + C + 1][i], 0x7632)};
 #pragma unroll
                   for (int r = 0; r < NR; ++r) {
                     float(&dst)[4] = o[r][c * (S::VB / 2) + h * (S::VB / 4) + i];
@@ -723,7 +736,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
             for (int e = 0; e < 4; ++e) pr[(2 * t4 + (e & 1)) * 16 + g + 8 * (e >> 1)] = s[t][r][e];
             __syncwarp();
 #pragma unroll 1
-            for (int token = 0; token < 16; ++token) {
+            for (int token = 0; token < (S::TAIL_HALF ? 8 : 16); ++token) {
               const int where = first_token + 16 * t + token;
 #pragma unroll
               for (int j = 0; j < S::MT; ++j) {
@@ -777,28 +790,30 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
       }
       return make_float2(top, sum);
     };
+    // a warp's share lies in one row group
+    const int share_rows = frag0 / S::MT;
     float4 acc[S::SHARE];
-    float2 ml_out[S::SHARE][2];
-#pragma unroll
-    for (int i = 0; i < S::SHARE; ++i) {
-      const int r = (frag0 + i) / S::MT;
+    float2 ml_out[2] = {};
+    if (has_share) {
       float weight[2][kKv8Warps];
-      acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (!has_share) continue;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float2 ml[kKv8Warps];
 #pragma unroll
-        for (int w = 0; w < kKv8Warps; ++w) ml[w] = warp_ml[w][r * 8 + 2 * t4 + e];
-        ml_out[i][e] = weigh(ml, weight[e]);
+        for (int w = 0; w < kKv8Warps; ++w) ml[w] = warp_ml[w][share_rows * 8 + 2 * t4 + e];
+        ml_out[e] = weigh(ml, weight[e]);
       }
 #pragma unroll
-      for (int w = 0; w < kKv8Warps; ++w) {
-        const float4 v = join[(w * S::FRAGS + frag0 + i) * 32 + lane];
-        acc[i].x = fmaf(weight[0][w], v.x, acc[i].x);
-        acc[i].y = fmaf(weight[1][w], v.y, acc[i].y);
-        acc[i].z = fmaf(weight[0][w], v.z, acc[i].z);
-        acc[i].w = fmaf(weight[1][w], v.w, acc[i].w);
+      for (int i = 0; i < S::SHARE; ++i) {
+        acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kKv8Warps; ++w) {
+          const float4 v = join[(w * S::FRAGS + frag0 + i) * 32 + lane];
+          acc[i].x = fmaf(weight[0][w], v.x, acc[i].x);
+          acc[i].y = fmaf(weight[1][w], v.y, acc[i].y);
+          acc[i].z = fmaf(weight[0][w], v.z, acc[i].z);
+          acc[i].w = fmaf(weight[1][w], v.w, acc[i].w);
+        }
       }
     }
 
@@ -811,14 +826,10 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
       float* part = a.parts + (static_cast<int64_t>(blockIdx.x) * 2 + which) * S::PART_FLOATS;
       if (has_share) {
 #pragma unroll
-        for (int i = 0; i < S::SHARE; ++i) {
-          __stcg(reinterpret_cast<float4*>(part) + (frag0 + i) * 32 + lane, acc[i]);
-          if ((frag0 + i) % S::MT == 0 && g == 0) {
-            const int row = (frag0 + i) / S::MT * 8 + 2 * t4;
-            __stcg(reinterpret_cast<float4*>(part + S::ROWS * D + 2 * row),
-                   make_float4(ml_out[i][0].x, ml_out[i][0].y, ml_out[i][1].x, ml_out[i][1].y));
-          }
-        }
+        for (int i = 0; i < S::SHARE; ++i) __stcg(reinterpret_cast<float4*>(part) + (frag0 + i) * 32 + lane, acc[i]);
+        if (frag0 % S::MT == 0 && g == 0)
+          __stcg(reinterpret_cast<float4*>(part + S::ROWS * D) + share_rows * 4 + t4,
+                 make_float4(ml_out[0].x, ml_out[0].y, ml_out[1].x, ml_out[1].y));
       }
       __syncthreads();
       if (tid == 0) {
@@ -833,55 +844,49 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
       if (write && has_share) {
         // The parts in the order of the ranges, kAhead at a time with all loads
         // in flight: the latency of L2 is what this costs.
-        constexpr int kAhead = S::SHARE == 1 ? 16 : S::SHARE == 2 ? 8 : 4;
+        constexpr int kAhead = S::SHARE == 1 ? 16 : S::SHARE == 2 ? 12 : 8;
         // in the tile's first CTA it is the second part if the range begins before the tile
         const float* first_part = a.parts + (static_cast<int64_t>(c0) * 2 + (ranges.begin(c0) < tile_begin ? 1 : 0)) * S::PART_FLOATS;
         const float* next_part = a.parts + static_cast<int64_t>(c0) * 2 * S::PART_FLOATS;
-        float top[S::SHARE][2];
+        float top[2] = {minus_inf, minus_inf}, sum[2] = {0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < S::SHARE; ++i) {
-          acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-          ml_out[i][0].y = ml_out[i][1].y = 0.f;
-          top[i][0] = top[i][1] = minus_inf;
-        }
+        for (int i = 0; i < S::SHARE; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
         for (int n0 = 0; n0 < n_parts; n0 += kAhead) {
-          float4 v[kAhead][S::SHARE], ml[kAhead][S::SHARE];  // ml: (max, sum) of rows 2 t and 2 t + 1
+          float4 v[kAhead][S::SHARE], ml[kAhead];  // ml: (max, sum) of rows 2 t and 2 t + 1
 #pragma unroll
           for (int n = 0; n < kAhead; ++n) {
             const float* part_n = n0 + n == 0 ? first_part : next_part + static_cast<int64_t>(n0 + n) * 2 * S::PART_FLOATS;
+            ml[n] = make_float4(minus_inf, 0.f, minus_inf, 0.f);
+            if (n0 + n < n_parts) ml[n] = __ldcg(reinterpret_cast<const float4*>(part_n + S::ROWS * D) + share_rows * 4 + t4);
 #pragma unroll
             for (int i = 0; i < S::SHARE; ++i) {
               v[n][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-              ml[n][i] = make_float4(minus_inf, 0.f, minus_inf, 0.f);
-              if (n0 + n < n_parts) {
-                v[n][i] = __ldcg(reinterpret_cast<const float4*>(part_n) + (frag0 + i) * 32 + lane);
-                ml[n][i] = __ldcg(reinterpret_cast<const float4*>(part_n + S::ROWS * D) + (frag0 + i) / S::MT * 4 + t4);
-              }
+              if (n0 + n < n_parts) v[n][i] = __ldcg(reinterpret_cast<const float4*>(part_n) + (frag0 + i) * 32 + lane);
             }
           }
+          float next[2] = {top[0], top[1]}, from[2], by[2];
 #pragma unroll
-          for (int i = 0; i < S::SHARE; ++i) {
-            float next[2] = {top[i][0], top[i][1]}, from[2];
+          for (int n = 0; n < kAhead; ++n) {
+            next[0] = fmaxf(next[0], ml[n].x);
+            next[1] = fmaxf(next[1], ml[n].z);
+          }
 #pragma unroll
-            for (int n = 0; n < kAhead; ++n) {
-              next[0] = fmaxf(next[0], ml[n][i].x);
-              next[1] = fmaxf(next[1], ml[n][i].z);
-            }
+          for (int e = 0; e < 2; ++e) {
+            from[e] = next[e] == minus_inf ? 0.f : next[e];
+            by[e] = fast_exp2(top[e] - from[e]);
+            top[e] = next[e];
+            sum[e] *= by[e];
+          }
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              from[e] = next[e] == minus_inf ? 0.f : next[e];
-              const float by = fast_exp2(top[i][e] - from[e]);
-              top[i][e] = next[e];
-              ml_out[i][e].y *= by;
-              (e ? acc[i].y : acc[i].x) *= by;
-              (e ? acc[i].w : acc[i].z) *= by;
-            }
+          for (int i = 0; i < S::SHARE; ++i) acc[i] = make_float4(acc[i].x * by[0], acc[i].y * by[1], acc[i].z * by[0], acc[i].w * by[1]);
 #pragma unroll
-            for (int n = 0; n < kAhead; ++n) {
-              const float w0 = fast_exp2(ml[n][i].x - from[0]), w1 = fast_exp2(ml[n][i].z - from[1]);
-              ml_out[i][0].y = fmaf(w0, ml[n][i].y, ml_out[i][0].y);
-              ml_out[i][1].y = fmaf(w1, ml[n][i].w, ml_out[i][1].y);
+          for (int n = 0; n < kAhead; ++n) {
+            const float w0 = fast_exp2(ml[n].x - from[0]), w1 = fast_exp2(ml[n].z - from[1]);
+            sum[0] = fmaf(w0, ml[n].y, sum[0]);
+            sum[1] = fmaf(w1, ml[n].w, sum[1]);
+#pragma unroll
+            for (int i = 0; i < S::SHARE; ++i) {
               acc[i].x = fmaf(w0, v[n][i].x, acc[i].x);
               acc[i].y = fmaf(w1, v[n][i].y, acc[i].y);
               acc[i].z = fmaf(w0, v[n][i].z, acc[i].z);
@@ -889,20 +894,22 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
             }
           }
         }
+        ml_out[0].y = sum[0];
+        ml_out[1].y = sum[1];
       }
     }
     if (write && has_share) {
 #pragma unroll
       for (int i = 0; i < S::SHARE; ++i) {
-        const int r = (frag0 + i) / S::MT, j = (frag0 + i) % S::MT;
+        const int j = (frag0 + i) % S::MT;
         // fragment j has bytes 2 j' and 2 j' + 1 of copy c of lane g
         const int d = j / (S::VB / 2) * 128 + g * S::VB + j % (S::VB / 2) * 2;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int row = row0 + r * 8 + 2 * t4 + e;
+          const int row = row0 + share_rows * 8 + 2 * t4 + e;
           if (row >= a.tokens * a.group) continue;
           const int token = row / a.group;
-          const float sum = ml_out[i][e].y;
+          const float sum = ml_out[e].y;
           const bool real = token < seq.count && sum != 0.f;  // padding rows are zero
           const float by = real ? 1.f / sum : 0.f;
           const uint32_t two = real ? pack_bf16x2((e ? acc[i].y : acc[i].x) * by, (e ? acc[i].w : acc[i].z) * by) : 0u;
