@@ -123,6 +123,56 @@ def test_the_binding_checks_its_arguments() -> None:
         module.kv8_attention(None, None, None, None, None, None, {}, None)
 
 
+def test_c_entry_points_check_before_any_device_work() -> None:
+    """Status -1 (arguments) or -2 (unsupported) and a message, without a GPU."""
+    import ctypes
+
+    lib = _native.load()
+    buf = ctypes.create_string_buffer(64)
+    at = (ctypes.addressof(buf) + 15) // 16 * 16
+    view = _native.Kv8CacheView(at, at, at, at, at, 4, 2, 2, 2, 64)
+    ref = ctypes.byref(view)
+    rope = ctypes.byref(_native.Rope(at, at, 8, 12, 0))
+
+    def rope_call(q: int = at, dtype: int = 1, dim: int = 64, stride: int = 384, table: object = None) -> int:
+        return lib.b200tx_qk_norm_rope(q, at, dtype, 1, 1, 4, 1, dim, stride, stride, stride, stride, None, None, 1e-6,
+                                       table, None, 0, 0, None)
+
+    def append(cache: object = ref, q: int = at, heads: int = 4, batch: int = 1) -> int:
+        return lib.b200tx_kv8_append(cache, q, 1, at, batch, 1, heads, 512, 512, None, None, None, None, 1e-6, None, None)
+
+    def attend(heads: int = 4, scale: float = 1.0, stride: int = 256) -> int:
+        return lib.b200tx_kv8_attention(ref, at, at, 1, 1, heads, stride, stride, None, None, scale, at, 0, None)
+
+    def linear(k: int = 64, group: int = 64, epilogue: int = 0, x: int | None = at) -> int:
+        return lib.b200tx_linear_w4(x, k, at, at, None, at, 1, 1, 8, k, group, epilogue, None)
+
+    for call, status, text in (
+        (lambda: rope_call(q=at + 2), -1, "16-byte aligned"),
+        (lambda: rope_call(dtype=7), -1, "dtype"),
+        (lambda: rope_call(dim=96), -2, "head_dim"),
+        (lambda: rope_call(stride=12), -1, "multiples of 8"),
+        (lambda: rope_call(table=rope), -1, "rotary"),
+        (lambda: append(cache=None), -1, "null cache"),
+        (lambda: append(q=None), -1, "null tensor"),
+        (lambda: append(heads=1), -1, "bad shape"),
+        (lambda: append(batch=3), -1, "slots"),
+        (lambda: attend(heads=5), -1, "evenly"),
+        (lambda: attend(scale=float("inf")), -1, "scale"),
+        (lambda: attend(stride=4), -1, "multiples of 8"),
+        (lambda: lib.b200tx_kv8_gather(ref, at, at, 1, 0, 0, None, None, None), -1, "bad shape"),
+        (lambda: lib.b200tx_kv8_gather(ref, at + 8, at, 1, 1, 0, None, None, None), -1, "aligned"),
+        (lambda: linear(k=60), -1, "bad shape"),
+        (lambda: linear(group=16), -2, "group"),
+        (lambda: linear(epilogue=3), -1, "epilogue"),
+        (lambda: linear(x=None), -1, "null"),
+    ):
+        assert call() == status, text
+        assert text in lib.b200tx_last_error().decode(), (text, lib.b200tx_last_error())
+    view.head_dim = 96
+    assert append() == -2 and "head_dim" in lib.b200tx_last_error().decode()
+
+
 def _meta(*shape: int, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     return torch.empty(*shape, device="meta", dtype=dtype)
 
