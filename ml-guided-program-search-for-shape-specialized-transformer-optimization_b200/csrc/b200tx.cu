@@ -85,6 +85,7 @@ struct DeviceState {
   int rownorm_clusters[4][5] = {};         // their co-resident clusters by CTA pairs per cluster
   bool kv8_attr[9] = {};                   // 8-bit cache attention builds by head_dim and row groups
   bool w4_attr[18] = {};                   // 4-bit linear builds by row tiles, column tiles and group
+  bool w4_line_attr[6] = {};               // the same with x in shared memory, by row tiles and group
   bool seq_forward_attr = false;           // whole-forward kernel's shared-memory size set
   uint8_t* seq_noalloc_images = nullptr;   // device address of g_seq_noalloc_images on this device
 };

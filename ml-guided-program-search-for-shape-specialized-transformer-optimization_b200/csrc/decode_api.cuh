@@ -69,7 +69,8 @@ int kv8_view(const char* what, const b200tx_kv8_cache* c, b200tx::Kv8Cache* out)
 
 // Chunks of heads for a warp: one, for the shortest step, or where there are
 // tokens enough to fill the SMs several, so that angles and factors are made
-// fewer times.
+// fewer times (append of 4 x 4000 tokens: one 114 us, four 103; 2 x 5776 tokens of
+// 48 heads of 64: one 35.8 us, four 31.9).
 int rope_chunks(int64_t tokens) { return tokens >= kRopeManyTokens ? kRopeChunks : 1; }
 
 template <int D, int E, typename T>
@@ -208,6 +209,45 @@ cudaError_t launch_w4(b200tx::W4Args& a, DeviceState* dev, int index, cudaStream
   const dim3 grid(static_cast<unsigned>((tiles + per - 1) / per), static_cast<unsigned>((a.rows + TN * 8 - 1) / (TN * 8)));
   return launch(b200tx::linear_w4_kernel<TN, RT, GROUP>, grid, dim3(b200tx::kW4Warps * 32),
                 static_cast<size_t>(std::max(a.stages * stage, join)), stream, a);
+}
+
+constexpr int kW4LineShared = 227 * 1024;  // of a CTA that has an SM to itself
+constexpr int64_t kW4LineUnits = 48;       // (16 columns, stage) units for each SM
+
+template <int TN, int GROUP>
+cudaError_t launch_w4_line(b200tx::W4Args& a, DeviceState* dev, int index, cudaStream_t stream) {
+  if (!dev->w4_line_attr[index]) {
+    cudaError_t err = cudaFuncSetAttribute(b200tx::linear_w4_line_kernel<TN, GROUP>,
+                                           cudaFuncAttributeMaxDynamicSharedMemorySize, kW4LineShared);
+    if (err != cudaSuccess) return err;
+    dev->w4_line_attr[index] = true;
+  }
+  const int all_stages = (a.runs + b200tx::kW4Runs - 1) / b200tx::kW4Runs;
+  const int x_bytes = a.rows * all_stages * b200tx::kW4Runs * b200tx::kW4Run * 2;
+  const int stage = b200tx::kW4LineWarps * b200tx::kW4LineStage;
+  a.stages = x_bytes + 4 * stage <= kW4LineShared ? 4 : 3;
+  return launch(b200tx::linear_w4_line_kernel<TN, GROUP>, dim3(static_cast<unsigned>(std::min(dev->sm_count, (a.outer + 15) / 16))),
+                dim3(b200tx::kW4LineWarps * 32), static_cast<size_t>(x_bytes + a.stages * stage), stream, a);
+}
+
+template <int TN>
+cudaError_t launch_w4_line_group(int64_t group, b200tx::W4Args& a, DeviceState* dev, int index, cudaStream_t stream) {
+  switch (group) {
+    case 32: return launch_w4_line<TN, 32>(a, dev, index, stream);
+    case 64: return launch_w4_line<TN, 64>(a, dev, index + 1, stream);
+    default: return launch_w4_line<TN, 128>(a, dev, index + 2, stream);
+  }
+}
+
+// The kernel with x in shared memory, where x and three stages for each warp fit and
+// there are units enough for its warps (8 x 8192 -> 28672, 387 units an SM: 32.9 us
+// against 38.2; 16 x 4096 -> 14336, 97: 15.6 against 16.5; 1 x 4096 -> 4096, 28: 5.74 against
+// 5.64; 1 x 1024 -> 4096, 7: 4.8 against 3.3).
+bool w4_in_line(const b200tx::W4Args& a, const DeviceState* dev) {
+  const int64_t all_stages = (a.runs + b200tx::kW4Runs - 1) / b200tx::kW4Runs;
+  return a.rows <= 16 && a.rows * all_stages * b200tx::kW4Runs * b200tx::kW4Run * 2 +
+                                 3 * b200tx::kW4LineWarps * b200tx::kW4LineStage <= kW4LineShared &&
+         (a.outer + 15) / 16 * all_stages >= kW4LineUnits * dev->sm_count;
 }
 
 template <int TN, int RT>
@@ -470,6 +510,10 @@ int b200tx_linear_w4(const void* x, int64_t x_stride, const void* packed, const 
   a.runs = static_cast<int>((K + b200tx::kW4Run - 1) / b200tx::kW4Run);
   a.gelu = epilogue == B200TX_EPI_BIAS_GELU;
   a.out_f32 = out_dtype == B200TX_F32;
+  if (w4_in_line(a, dev)) {
+    cudaError_t err = M <= 8 ? launch_w4_line_group<1>(group, a, dev, 0, stream) : launch_w4_line_group<2>(group, a, dev, 3, stream);
+    return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "linear_w4");
+  }
   // Rows of x by eights: 1, 2 or 4 MMA columns.  Four only where the columns of W
   // fill the SMs; with fewer the rows go 16 at a time, which makes twice the CTAs
   // and reads the weights again from L2 (29 x 4744 -> 5003: four 23.9 us, twice two 22.4).

@@ -10,13 +10,13 @@
 // equal share of them whatever the lengths are.
 //
 // Split.  The rows of a (sequence, kv head) are its tokens x the query heads of
-// the group, in tiles of 8 NR.  A tile's keys are cut into steps of 16 to 64 codes,
-// 8 KB of keys and values (4 KB for head_dim 32), and half as many tokens in the open block.  All steps of all tiles, and a
-// fixed cost for each tile, form one line, cut into equal ranges, one per CTA: a
-// CTA ends within a tile's keys, or does several tiles, and no length of any
-// sequence leaves SMs idle.  A tile that lies in several CTAs is joined by the
-// one that finishes last, in the order of the ranges, so results do not
-// depend on the order of arrival.
+// the group, in tiles of 8 NR.  A tile's keys are cut into steps of 16 to 64
+// codes, 8 KB of keys and values (4 KB for head_dim 32), and half as many tokens in
+// the open block.  All steps of all tiles, and a fixed cost for each tile, form
+// one line, cut into equal ranges, one per CTA: a CTA ends within a tile's keys,
+// or does several tiles, and no length of any sequence leaves SMs idle.  A tile
+// that lies in several CTAs is joined by the one that finishes last, in the order
+// of the ranges, so results do not depend on the order of arrival.
 //
 // Within a CTA the steps of a tile go round the four warps.  Each warp has a ring
 // of steps in shared memory of its own, filled by cp.async: no barrier between
@@ -43,6 +43,12 @@
 // queries are bf16 and each probability is the sum of two bf16 numbers.  The
 // running maximum moves only when a score exceeds it by more than 2^8, which
 // leaves room in fp16 and saves most rescalings and most reductions.
+//
+// Measured: 100000 tokens of 16 heads of 64 in 43 us (4.8 TB/s), 16 x 8192 of 8 heads of
+// 128 in 56 us (4.8 TB/s), 64 ragged sequences up to 8192 in 34 us, 1000 tokens of 16
+// heads of 64 in 7.8 us.  Of a long call some 8 us are launch, ramp and the last join;
+// the rest runs at 6 TB/s.  With 8 to 12 warps an SM the instructions of a step are
+// the next bound.
 #pragma once
 
 #include "attention_mma_kernels.cuh"
@@ -51,7 +57,8 @@
 namespace b200tx {
 
 constexpr int kKv8Warps = 4;
-constexpr int kKv8TileCost = 12;  // what beginning and joining a tile costs, in steps (64 ragged sequences: 6 42.3 us, 12 34.5, 24 37.8)
+// What beginning and joining a tile costs, in steps (64 ragged sequences: 6 steps 42.3 us, 12 34.5, 24 37.8).
+constexpr int kKv8TileCost = 12;
 constexpr float kKv8JoinShare = 0.5f;  // what a part costs to join, against a step: its root
 constexpr float kKv8Headroom = 8.f;  // log2 of how far a score may pass the running maximum
 constexpr float kKv8Unit = 16777216.f;  // 2^24: a code's fp16 number is code / 2^24

@@ -11,9 +11,13 @@
 // the same bits as the same tokens one at a time.  Keys and values are
 // rounded to bf16 when they enter, whichever way they take.
 //
-// The offset of 128 makes a code the low byte of an fp16 number 1024 + code:
-// the attention turns bytes into numbers with one byte permute and one
-// subtraction for two of them.
+// The offset of 128 keeps a code positive: under a zero byte it is an fp16
+// number as it stands, two to an instruction, and the attention takes the
+// offset out of its sums.
+//
+// What bounds them: HBM, each value read and written once.  An append of 4 x 4000 tokens
+// (32 + 2 x 8 heads of 128) and the read-back of its values move 459 MB: 103 us, 4.5 TB/s.
+// The rest are the instructions of norm, rotation and rounding.
 //
 // The tail has two slots, taken by the parity of the block index.  A call of
 // up to 64 tokens touches two blocks at most, and leaves both in their slots;

@@ -16,7 +16,7 @@
 //   y = r (x (w c) + x' (w' s))
 // with w c and w' s computed once for the four groups of heads that a warp takes
 // of a token (a lane holds the same dims of every head); their loads go out
-// together.
+// together.  8 x 2048 tokens of 48 heads of 64 (201 MB) take 38 us, 5.3 TB/s.
 #pragma once
 
 #include "sm100_common.cuh"

@@ -95,7 +95,10 @@ class Kv8Cache:
         self._handles = [(ctypes.addressof(view), codes.get_device()) for view in self._views]
         # The attention's workspace (arrival counters that every launch leaves
         # zero, and the parts of split tiles), one for each stream it runs on.
+        # A spare one is there from the start for a first call inside a graph
+        # capture, where nothing could be zeroed for good.
         self._workspaces: dict[int, torch.Tensor] = {}
+        self._spare = self._new_workspace() if self.device.type == "cuda" else None
 
     @classmethod
     def create(
@@ -136,10 +139,22 @@ class Kv8Cache:
         require(0 <= layer < self.layers, f"layer {layer} of a cache of {self.layers}")
         return ctypes.byref(self._views[layer])
 
+    def _new_workspace(self) -> torch.Tensor:
+        with torch.cuda.device(self.device):
+            return torch.zeros(_native.kv8_workspace_bytes(self.head_dim), dtype=torch.uint8, device=self.device)
+
     def workspace(self, stream: int) -> torch.Tensor:
         found = self._workspaces.get(stream)
         if found is None:
-            found = torch.zeros(_native.kv8_workspace_bytes(self.head_dim), dtype=torch.uint8, device=self.device)
+            if not torch.cuda.is_current_stream_capturing():
+                found = self._new_workspace()
+            elif self._spare is not None:
+                found, self._spare = self._spare, None
+            else:
+                raise RuntimeError(
+                    "the cache's attention is captured on a second stream that it has not run on: "
+                    "call it once on that stream before the capture"
+                )
             self._workspaces[stream] = found
         return found
 

@@ -539,6 +539,30 @@ def test_streams_and_graphs() -> None:
         assert torch.equal(context, want)
 
 
+def test_capture_without_a_call_before() -> None:
+    """The first attention of a cache inside a capture takes the spare
+    workspace; on a second new stream it is refused."""
+    cache, _ = _filled([3000], 2, 64, seed=3)
+    cache.advance(-1)
+    q = _randn(1, 1, 2, 64, seed=3).bfloat16()
+    sm100_kv8_attention(_filled([70], 2, 64, seed=3)[0], q)  # the kernel is set up, the cache is not
+    first, second = torch.cuda.Stream(), torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=first):
+        got, _ = sm100_kv8_attention(cache, q)
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        assert torch.equal(got, sm100_kv8_attention(cache, q)[0])
+    assert first.cuda_stream in cache._workspaces and second.cuda_stream not in cache._workspaces
+    refused = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="before the capture"):
+        with torch.cuda.graph(refused, stream=second):
+            q.clone()
+            sm100_kv8_attention(cache, q)
+    assert torch.equal(got, sm100_kv8_attention(cache, q)[0])
+
+
 # ------------------------------------------------------------------ 4-bit linear
 
 
@@ -575,6 +599,27 @@ def test_linear_w4(rows, inner, outer, group, out_dtype) -> None:  # noqa: ANN00
     got, marker = sm100_linear_w4(x[None], weight, bias, gelu=True, out_dtype=out_dtype)
     assert marker == "sm100_linear_w4_gelu" and got.shape == (1, rows, outer)
     _check_linear(got, x, weight, bias, True)
+
+
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize(
+    ("rows", "inner", "outer"),
+    [(1, 4096, 7117), (8, 4104, 7120), (5, 8192, 4001), (9, 3992, 9001), (16, 4096, 14336), (3, 256, 113900),
+     (16, 264, 57003), (1, 65536, 449), (2, 120, 115001)],
+)
+def test_linear_w4_with_x_in_shared_memory(rows, inner, outer, group, out_dtype) -> None:  # noqa: ANN001
+    """Few rows and many columns: tiles within a warp's range, across two and more of
+    them, and a last tile that ends past the columns."""
+    weight = pack_w4(_randn(outer, inner, seed=outer) * inner**-0.5, group)
+    x = _randn(rows, inner, seed=rows).bfloat16()
+    bias = _randn(outer, seed=3) if rows % 2 else None
+    got, _ = sm100_linear_w4(x, weight, bias, gelu=rows == 8, out_dtype=out_dtype)
+    _check_linear(got, x, weight, bias, rows == 8)
+    assert torch.equal(sm100_linear_w4(x, weight, bias, gelu=rows == 8, out_dtype=out_dtype)[0], got)
+    x[0, inner // 2] = float("nan")
+    got, _ = sm100_linear_w4(x, weight, bias, out_dtype=out_dtype)
+    assert got.isnan().all(-1).tolist() == [True] + [False] * (rows - 1) and not got[1:].isnan().any()
 
 
 def test_linear_w4_codes_past_the_end_and_extremes() -> None:
