@@ -7,6 +7,7 @@ namespace {
 
 constexpr int64_t kRopeManyTokens = 4096;
 constexpr int kRopeChunks = 4;
+constexpr int64_t kKv8ShortSteps = 24;
 
 // Values a lane: eight of bf16, four of fp32 (16 bytes; 25 x 420 tokens of 6 heads of 64
 // in fp32: four 8.0 us, eight 13.7), four of bf16 where the pairs' halves do not lie
@@ -156,8 +157,17 @@ int64_t kv8_part_bytes(int sm_count) {
 
 // Row groups of 8 in a tile, for which a code is expanded once: up to 4 where the
 // outputs of 32 rows fit in the registers (head_dim 32 and 64), 2 for 128, 1 for 256.
-int kv8_row_groups(int64_t head_dim, int64_t rows) {
+// Where tiles of 8 rows are short work even for a full cache, 24 steps a CTA, one:
+// their beginning and join take less (64 rows: 4 x 2 heads of 128 over 3001 tokens, 20
+// steps, one 12.3 us, two 15.3; over 12000, 81 steps, 34.9 and 30.8; 4 x 2 heads of 64 over
+// 3001, 7 steps, one 12.2 us, four 14.7; 8 x 4 of 64 over 3000, 27 steps, 22.8 and 20.7).
+int kv8_row_groups(int64_t head_dim, int64_t rows, int64_t sequence_heads, int64_t max_blocks, int sm_count) {
   if (rows <= 8 || head_dim == 256) return 1;
+  const int64_t steps = sequence_heads * ((rows + 7) / 8) * max_blocks * (head_dim == 128 ? 2 : 1);
+  const int ctas = head_dim == 128   ? kv8_attention_grid<128, 1>(sm_count)
+                   : head_dim == 64 ? kv8_attention_grid<64, 1>(sm_count)
+                                    : kv8_attention_grid<32, 1>(sm_count);
+  if (steps <= kKv8ShortSteps * ctas) return 1;
   if (rows <= 16 || head_dim == 128) return 2;
   return 4;
 }
@@ -458,7 +468,8 @@ int b200tx_kv8_attention(const b200tx_kv8_cache* cache, const void* q, void* out
   a.arrivals = static_cast<unsigned int*>(workspace);
   a.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kKv8ArrivalBytes);
   cudaError_t err;
-  const int groups = kv8_row_groups(cache->head_dim, tokens * a.group);
+  const int groups =
+      kv8_row_groups(cache->head_dim, tokens * a.group, batch * cache->kv_heads, cache->max_blocks, dev->sm_count);
   // all steps of the longest sequences that the page table can hold, and the tiles' own cost
   const double units = static_cast<double>(batch) * cache->kv_heads * ((tokens * a.group + 8 * groups - 1) / (8 * groups)) *
                        (4.0 * cache->max_blocks + 8 + b200tx::kKv8TileCost);

@@ -373,6 +373,47 @@ def test_attention(dim, kv_heads, group, tokens, totals) -> None:  # noqa: ANN00
     assert torch.equal(sm100_kv8_attention(cache, q)[0], got)  # the same bits again
 
 
+def _widened(cache):  # noqa: ANN001, ANN202
+    """The same cache with room for 800000 tokens a slot in the page table, for which
+    the kernels of taller row tiles are taken."""
+    table = torch.full((cache.slots, 12500), -1, dtype=torch.int32, device=DEV)
+    table[:, : cache.max_blocks] = cache.page_table
+    return Kv8Cache(cache.codes, cache.scales, cache.tail, table, cache.lengths)
+
+
+@pytest.mark.parametrize(
+    ("dim", "kv_heads", "group", "tokens", "totals"), [case for case in CASES if case[2] * case[3] > 8 and case[0] < 256]
+)
+def test_attention_tall_row_tiles(dim, kv_heads, group, tokens, totals) -> None:  # noqa: ANN001
+    cache, kv = _filled(totals, kv_heads, dim, seed=dim + tokens)
+    cache.advance(-tokens)
+    wide = _widened(cache)
+    q = _randn(len(totals), tokens, kv_heads * group, dim, seed=7).bfloat16()
+    got, _ = sm100_kv8_attention(wide, q)
+    for b, total in enumerate(totals):
+        want = _attention64(q[b], kv[b], total - tokens, dim**-0.5)
+        _check_attention(got[b].view(tokens, -1, dim), want, kv[b][1].abs().max())
+    assert torch.equal(sm100_kv8_attention(wide, q)[0], got)
+
+
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("tokens", [12, 100])
+def test_attention_tall_row_tiles_poisoned(dim, tokens) -> None:  # noqa: ANN001
+    """Rows that do not see a block do not see its NaN either; a bad page is NaN."""
+    cache, kv = _filled([192, 192], 1, dim, seed=4)
+    cache.advance(-tokens)
+    cache.scales[0, cache.page_table[0, 2].long()] = float("nan")
+    wide = _widened(cache)
+    wide.page_table[1, 1] = 10_000  # not a page
+    q = _randn(2, tokens, 1, dim, seed=1).bfloat16()
+    got = sm100_kv8_attention(wide, q)[0]
+    clear = max(0, 128 - (192 - tokens))  # rows that end before the third block
+    want = _attention64(q[0], [t.nan_to_num() for t in kv[0]], 192 - tokens, dim**-0.5)
+    _check_attention(got[0, :clear].view(clear, 1, dim), want[:clear], kv[0][1].nan_to_num().abs().max())
+    assert bool(got[0, clear:].isnan().all())
+    assert bool(got[1].isnan().all())
+
+
 def test_attention_sharp_and_large_scores() -> None:
     """Scores of hundreds: the running maximum moves often; and tiny queries."""
     cache, kv = _filled([1000, 150], 2, 64, seed=3)
