@@ -250,8 +250,8 @@ cudaError_t launch_w4_line_group(int64_t group, b200tx::W4Args& a, DeviceState* 
 }
 
 // The kernel with x in shared memory, where x and three stages for each warp fit and
-// there are units enough for its warps (8 x 8192 -> 28672, 387 units an SM: 32.9 us
-// against 38.2; 16 x 4096 -> 14336, 97: 15.6 against 16.5; 1 x 4096 -> 4096, 28: 5.74 against
+// there are units enough for its warps (8 x 8192 -> 28672, 387 units an SM: 31.2 us
+// against 38.2; 16 x 4096 -> 14336, 97: 15.4 against 16.2; 1 x 4096 -> 4096, 28: 5.74 against
 // 5.64; 1 x 1024 -> 4096, 7: 4.8 against 3.3).
 bool w4_in_line(const b200tx::W4Args& a, const DeviceState* dev) {
   const int64_t all_stages = (a.runs + b200tx::kW4Runs - 1) / b200tx::kW4Runs;

@@ -24,7 +24,7 @@
 // Measured: 1 x 1024 -> 4096 in 3.3 us, 32 x 4096 -> 14336 in 23 us, 8 x 8192 -> 28672 (122
 // MB) in 38 us.  Masks and shifts run at half rate, and 224 CTAs on 148 SMs leave
 // half of the SMs less to do; for up to 16 rows and many units the kernel at the end
-// of this file keeps x in shared memory and shares evenly: 33 us, 3.7 TB/s.
+// of this file keeps x in shared memory and shares evenly: 31 us, 3.9 TB/s.
 #pragma once
 
 #include "attention_mma_kernels.cuh"
@@ -274,7 +274,8 @@ __global__ void __launch_bounds__(kW4Warps * 32, 2) linear_w4_kernel(W4Args a) {
 // weights only and needs no barrier: each warp has a ring of its own.  A CTA has an
 // equal share of the 16-column tiles; its (tile, stage) units form one line that the
 // warps cut into equal ranges.  Tiles that lie in several ranges are joined in shared
-// memory, in the order of the ranges.  8 x 8192 -> 28672 takes 32.9 us (3.7 TB/s; 38.2 above).
+// memory, in the order of the ranges.  8 x 8192 -> 28672 takes 31.2 us (3.9 TB/s; 38.2
+// above), bound by its instructions: schedulers issue in two of three cycles.
 
 constexpr int kW4LineWarps = 16;
 constexpr int kW4LineStage = 16 * (kW4Runs * kW4Run / 2);  // bytes of a warp's stage
@@ -318,18 +319,28 @@ __global__ void __launch_bounds__(kW4LineWarps * 32, 1) linear_w4_line_kernel(W4
     if (++c.at == all_stages) { c.at = 0; ++c.tile; }
   };
   Cursor copy{begin, first_tile + begin / all_stages, begin % all_stages};
-  int put = 0;
+  uint32_t put = w_put;
+  const uint32_t put_end = w_put + a.stages * kW4LineStage;
+  const uint8_t* from = nullptr;
+  unsigned row_off[COPIES];
+  auto enter_tile = [&]() {  // columns past the end read the last one and are not written
+    const int row = min(copy.tile * 16 + lane / 8, a.outer - 1);
+    from = a.packed + row * pitch + copy.at * ROW + lane % 8 * 16;
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i)
+      row_off[i] = static_cast<unsigned>(min(row + i * 4, a.outer - 1) - row) * static_cast<unsigned>(pitch);
+  };
+  enter_tile();
   auto issue = [&]() {
     if (copy.unit < end) {
       const bool take = copy.at * kW4Runs + lane % 8 / 4 < a.runs;
-      const uint8_t* const from = a.packed + copy.at * ROW + lane % 8 * 16;
 #pragma unroll
-      for (int i = 0; i < COPIES; ++i) {
-        const int n = min(copy.tile * 16 + i * 4 + lane / 8, a.outer - 1);  // past the end: the last, not written
-        cp_async_or_zero(w_put + put * kW4LineStage + i * 512, from + n * pitch, take);
-      }
+      for (int i = 0; i < COPIES; ++i) cp_async_or_zero(put + i * 512, from + row_off[i], take);
       advance(copy);
-      put = put + 1 == a.stages ? 0 : put + 1;
+      from += ROW;
+      if (copy.at == 0) enter_tile();
+      put += kW4LineStage;
+      if (put == put_end) put = w_put;
     }
     cp_async_commit();
   };
@@ -337,22 +348,21 @@ __global__ void __launch_bounds__(kW4LineWarps * 32, 1) linear_w4_line_kernel(W4
 
   // ---- scales, two units ahead: lane = a column of one of two groups
   const int all_groups = a.runs * GROUPS;
-  auto load_scales = [&](const Cursor& c, uint16_t (&to)[SCALES]) {
-    const int col = min(c.tile * 16 + lane % 16, a.outer - 1);
+  Cursor now{begin, first_tile + begin / all_stages, begin % all_stages}, ahead = now;
+  auto load_scales = [&](uint16_t (&to)[SCALES]) {
+    const int col = min(ahead.tile * 16 + lane % 16, a.outer - 1);
 #pragma unroll
     for (int i = 0; i < SCALES; ++i) {
-      const int q = c.at * STAGE_GROUPS + 2 * i + lane / 16;
+      const int q = ahead.at * STAGE_GROUPS + 2 * i + lane / 16;
       to[i] = 0;
-      if (c.unit < end && q < all_groups)
+      if (ahead.unit < end && q < all_groups)
         to[i] = __ldg(reinterpret_cast<const uint16_t*>(a.scales) + static_cast<int64_t>(q) * a.outer + col);
     }
+    advance(ahead);
   };
-  Cursor now{begin, first_tile + begin / all_stages, begin % all_stages}, ahead = now;
   uint16_t scales[3][SCALES];
-  load_scales(ahead, scales[0]);
-  advance(ahead);
-  load_scales(ahead, scales[1]);
-  advance(ahead);
+  load_scales(scales[0]);
+  load_scales(scales[1]);
 
   if (a.stages == 3) cp_async_wait<2>();
   else cp_async_wait<3>();
@@ -391,8 +401,7 @@ __global__ void __launch_bounds__(kW4LineWarps * 32, 1) linear_w4_line_kernel(W4
     else cp_async_wait<2>();
     __syncwarp();
     issue();
-    load_scales(ahead, scales[2]);
-    advance(ahead);
+    load_scales(scales[2]);
     const uint8_t* const stage = w4_smem + get * kW4LineStage;
     const uint8_t* const x_stage = w4_smem + now.at * (STAGE * 2);
 #pragma unroll
