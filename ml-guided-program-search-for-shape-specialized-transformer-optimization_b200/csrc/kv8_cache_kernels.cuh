@@ -71,6 +71,8 @@ struct Kv8AppendArgs {
 };
 
 constexpr int kKv8AppendWarps = 8;
+constexpr float kKv8Tiny = 5.421010862427522e-20f;    // 2^-64
+constexpr float kKv8Raise = 7.922816251426434e+28f;  // 2^96
 
 // One block of one kv head: its new tokens normed, rotated and stored, and the
 // block quantised if it is full now.
@@ -181,8 +183,22 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendArgs& a, int b, 
   }
   uint8_t* const k_codes = a.cache.codes + at * kKv8Block * D;
   uint8_t* const v_codes = k_codes + static_cast<int64_t>(a.cache.kv_heads) * kKv8Block * D;
+  // Below 2^-64 a block is taken up by 2^96, values and scale alike and exactly, so that the
+  // scale is a normal number and its reciprocal a finite one whatever the block's peak is.
+  auto raise = [](uint32_t (&bits)[PASSES][E / 2], float scale) {
+    if (scale >= kKv8Tiny) return scale;  // NaN is no matter, as below
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+#pragma unroll
+      for (int i = 0; i < E / 2; ++i)
+        bits[p][i] = pack_bf16x2(__uint_as_float(bits[p][i] << 16) * kKv8Raise,
+                                 __uint_as_float(bits[p][i] & 0xffff0000u) * kKv8Raise);
+    }
+    return scale * kKv8Raise;
+  };
+  const float k_unit = raise(k_bits, k_scale), v_unit = raise(v_bits, v_scale);
   // scale 0: a block of zeros, codes 128; scale NaN: any code, the scale says it all
-  const float k_inv = k_scale > 0.f ? 1.f / k_scale : 0.f, v_inv = v_scale > 0.f ? 1.f / v_scale : 0.f;
+  const float k_inv = k_unit > 0.f ? 1.f / k_unit : 0.f, v_inv = v_unit > 0.f ? 1.f / v_unit : 0.f;
   // 1.5 2^23 + 128 + x inv, rounded to an integer by the addition: the low byte is the code
   auto codes = [](uint32_t lo, uint32_t hi, float inv) -> uint32_t {
     const float shift = 12583040.f;

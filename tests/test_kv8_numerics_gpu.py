@@ -1,0 +1,61 @@
+"""The 8-bit cache at the ends of the number range."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from solution.kernels import KV8_BLOCK, Kv8Cache, sm100_kv8_append, sm100_kv8_gather
+
+pytestmark = pytest.mark.gpu
+
+DEV = torch.device("cuda", 0)
+
+
+@pytest.fixture(autouse=True)
+def _inference():
+    with torch.inference_mode():
+        yield
+    torch.cuda.synchronize()
+
+
+def _coded(x: torch.Tensor) -> Kv8Cache:
+    """A cache of one kv head that holds x, bf16 [tokens, 2, D] (keys, values), appended at once."""
+    tokens, _, dim = x.shape
+    cache = Kv8Cache.create(slots=1, max_tokens=tokens, num_kv_heads=1, head_dim=dim, device=DEV)
+    qkv = torch.cat((torch.zeros_like(x[:, :1]), x), 1).reshape(1, tokens, 3 * dim)
+    sm100_kv8_append(cache, qkv.contiguous(), 1)
+    cache.advance(tokens)
+    return cache
+
+
+def _definition(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Scales and codes of x in 32 bits, on the CPU: max / 127, rint(x / scale) + 128."""
+    blocks = x.float().cpu().unflatten(0, (-1, KV8_BLOCK)).transpose(1, 2)  # block, kv, token, dim
+    scale = blocks.abs().amax((-2, -1)) / 127
+    code = torch.where(scale[..., None, None] > 0, blocks / scale[..., None, None], torch.zeros_like(blocks))
+    return scale, code.round() + 128
+
+
+@pytest.mark.parametrize("dim", [32, 64, 128, 256])
+def test_blocks_of_tiny_values_keep_their_values(dim: int) -> None:
+    """Peaks of 2^-60 down to the smallest bf16 number, where the scale and its
+    reciprocal leave the normal numbers: every value within half a step."""
+    peaks = [-60, -64, -90, -100, -119, -120, -121, -122, -124, -126, -130, -133]
+    g = torch.Generator().manual_seed(dim)
+    x = (2 * torch.rand(len(peaks), KV8_BLOCK, 2, dim, generator=g) - 1).double()
+    x[:, 0, :, 0], x[:, 1, :, 1], x[:, 2, :, 2] = 1.0, -1.0, 0.0
+    x = (x * 2.0 ** torch.tensor(peaks, dtype=torch.float64)[:, None, None, None]).flatten(0, 1).to(torch.bfloat16)
+    cache = _coded(x.to(DEV))
+    scale, code = _definition(x)
+    assert torch.equal(cache.scales[0, :, :, 0].cpu(), scale)
+    # the definition's quotient is rounded once, the kernel's at most by 2^-22 more: half a step and 2^-15
+    want = x.double().unflatten(0, (-1, KV8_BLOCK)).transpose(1, 2) / scale.double()[..., None, None] + 128
+    off = (cache.codes[0, :, :, 0].cpu().double() - want).abs()
+    assert float(off.max()) <= 0.5 + 2.0**-15, off.amax((1, 2, 3)).tolist()
+    k, v, _ = sm100_kv8_gather(cache, len(x))
+    got = torch.stack((k, v), 2)[0, :, :, 0].cpu().double()  # token, kv, dim
+    step = scale.double().repeat_interleave(KV8_BLOCK, 0)[..., None]
+    # half a step and the rounding to bf16 (2^-8, or half the smallest subnormal 2^-133)
+    bound = step * (0.5 + 2.0**-15) + 2.0**-8 * x.double().abs() + 2.0**-134
+    assert bool(((got - x.double()).abs() <= bound).all())
