@@ -4,7 +4,7 @@
 // A sequence's tokens lie in blocks of 64.  A block that is full is held as
 // 8-bit codes with one fp32 scale per kv head, for keys and for values:
 //     scale = max |x| / 127 over the block's 64 x D values of the head
-//     code  = rint(x (1 / scale)) + 128,       x ~ (code - 128) * scale
+//     code  = rint(x / scale) + 128,           x ~ (code - 128) * scale
 // The block that is still open is held in bf16 in the sequence's tail.  Its
 // scale is only known when its last token arrives; with the open block in 16
 // bits nothing is ever quantised twice, and a prompt appended at once gives
@@ -199,14 +199,22 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendArgs& a, int b, 
   const float k_unit = raise(k_bits, k_scale), v_unit = raise(v_bits, v_scale);
   // scale 0: a block of zeros, codes 128; scale NaN: any code, the scale says it all
   const float k_inv = k_unit > 0.f ? 1.f / k_unit : 0.f, v_inv = v_unit > 0.f ? 1.f / v_unit : 0.f;
-  // 1.5 2^23 + 128 + x inv, rounded to an integer by the addition: the low byte is the code
-  auto codes = [](uint32_t lo, uint32_t hi, float inv) -> uint32_t {
-    const float shift = 12583040.f;
-    const uint32_t c0 = __float_as_uint(fmaf(__uint_as_float(lo << 16), inv, shift));
-    const uint32_t c1 = __float_as_uint(fmaf(__uint_as_float(lo & 0xffff0000u), inv, shift));
-    const uint32_t c2 = __float_as_uint(fmaf(__uint_as_float(hi << 16), inv, shift));
-    const uint32_t c3 = __float_as_uint(fmaf(__uint_as_float(hi & 0xffff0000u), inv, shift));
-    return __byte_perm(__byte_perm(c0, c1, 0x0040), __byte_perm(c2, c3, 0x0040), 0x5410);
+  // The quotient x / scale in 32 bits, correctly rounded, by Markstein's method ("Computation
+  // of elementary functions on the IBM RISC System/6000 processor", 1990): a first
+  // quotient by the rounded reciprocal, and its exact remainder times the reciprocal.
+  // A product with the reciprocal alone takes values halfway between two codes, such as
+  // half the block's peak, to either side.  Then 1.5 2^23 + 128 + quotient, rounded to an
+  // integer by the addition: the low byte is the code.  Two values at a time.
+  auto codes = [](uint32_t lo, uint32_t hi, float unit, float inv) -> uint32_t {
+    const uint64_t by = f32x2(inv, inv), unit2 = f32x2(-unit, -unit), shift = f32x2(12583040.f, 12583040.f);
+    auto two = [&](uint32_t w) {
+      const uint64_t x = f32x2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+      const uint64_t near = mul_f32x2(x, by);
+      return unpack_f32x2(add_f32x2(fma_f32x2(fma_f32x2(near, unit2, x), by, near), shift));
+    };
+    const float2 c01 = two(lo), c23 = two(hi);
+    return __byte_perm(__byte_perm(__float_as_uint(c01.x), __float_as_uint(c01.y), 0x0040),
+                       __byte_perm(__float_as_uint(c23.x), __float_as_uint(c23.y), 0x0040), 0x5410);
   };
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
@@ -215,8 +223,8 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendArgs& a, int b, 
     uint32_t kc[E / 4], vc[E / 4];
 #pragma unroll
     for (int i = 0; i < E / 4; ++i) {
-      kc[i] = codes(k_bits[p][2 * i], k_bits[p][2 * i + 1], k_inv);
-      vc[i] = codes(v_bits[p][2 * i], v_bits[p][2 * i + 1], v_inv);
+      kc[i] = codes(k_bits[p][2 * i], k_bits[p][2 * i + 1], k_unit, k_inv);
+      vc[i] = codes(v_bits[p][2 * i], v_bits[p][2 * i + 1], v_unit, v_inv);
     }
     uint8_t* const k_to = k_codes + in_block * D + in_head * E;
     uint8_t* const v_to = v_codes + in_block * D + in_head * E;

@@ -1,4 +1,4 @@
-"""The 8-bit cache at the ends of the number range."""
+"""The 8-bit cache at the ends of the number range, and values halfway between two codes."""
 
 from __future__ import annotations
 
@@ -59,3 +59,25 @@ def test_blocks_of_tiny_values_keep_their_values(dim: int) -> None:
     # half a step and the rounding to bf16 (2^-8, or half the smallest subnormal 2^-133)
     bound = step * (0.5 + 2.0**-15) + 2.0**-8 * x.double().abs() + 2.0**-134
     assert bool(((got - x.double()).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("dim", [32, 64, 128, 256])
+def test_codes_are_the_rounded_quotients(dim: int) -> None:
+    """code = rint(x / scale) + 128 with the quotient rounded to 32 bits, bit for bit, halfway
+    values (half the block's peak, and other ties) among them."""
+    g = torch.Generator().manual_seed(dim)
+    blocks = 48
+    x = torch.randn(blocks, KV8_BLOCK, 2, dim, generator=g)
+    peak = torch.tensor([1 + i / 128 for i in range(blocks)])[:, None, None, None] * 8  # 8 bits: exact in bf16
+    x = x.clamp(-7, 7)
+    x[:, 0] = peak[:, 0]
+    x[:, 1:9] = peak / 2
+    x[:, 9:17] = -peak / 2
+    x[:, 17:25] = peak * torch.randint(-127, 128, (blocks, 8, 2, dim), generator=g) / 254
+    x[1::3] *= 2.0**-30
+    x[2::3] *= 2.0**60
+    x = x.flatten(0, 1).to(torch.bfloat16)
+    cache = _coded(x.to(DEV))
+    scale, code = _definition(x)
+    assert torch.equal(cache.scales[0, :, :, 0].cpu(), scale)
+    assert torch.equal(cache.codes[0, :, :, 0].cpu().float(), code)
