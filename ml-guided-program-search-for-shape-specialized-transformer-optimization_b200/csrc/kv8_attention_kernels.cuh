@@ -39,10 +39,12 @@
 // denominator).  The queries are scaled by a power of two per row into fp16
 // (exact but for what is 2^-24 of the row's largest value), products accumulate
 // in fp32, the block's scale multiplies the sum.  Probabilities are rounded to
-// fp16 (2^-11, finer than the bf16 output's 2^-8).  In the open block keys and
-// queries are bf16 and each probability is the sum of two bf16 numbers.  The
-// running maximum moves only when a score exceeds it by more than 2^8, which
-// leaves room in fp16 and saves most rescalings and most reductions.
+// fp16: to 2^-11 of themselves (finer than the bf16 output's 2^-8) down to 2^-21 of
+// the row's largest so far, below that to 2^-32 of it, which takes a million tokens a
+// warp to reach 2^-12.  For that a row's exponents are taken from a base 2^7 under its
+// running maximum; the base moves only when a score exceeds it by more than 2^15,
+// fp16's room, which saves most rescalings and most reductions.  In the open block keys
+// and queries are bf16 and each probability is the sum of two bf16 numbers.
 //
 // Measured: 100000 tokens of 16 heads of 64 in 43 us (4.8 TB/s), 16 x 8192 of 8 heads of
 // 128 in 56 us (4.8 TB/s), 64 ragged sequences up to 8192 in 34 us, 1000 tokens of 16
@@ -60,7 +62,8 @@ constexpr int kKv8Warps = 4;
 // What beginning and joining a tile costs, in steps (64 ragged sequences: 6 steps 42.3 us, 12 34.5, 24 37.8).
 constexpr int kKv8TileCost = 12;
 constexpr float kKv8JoinShare = 0.5f;  // what a part costs to join, against a step: its root
-constexpr float kKv8Headroom = 8.f;  // log2 of how far a score may pass the running maximum
+constexpr float kKv8Under = 7.f;      // log2 of how far a row's base lies under its maximum when it moves
+constexpr float kKv8Headroom = 15.f;  // and of how far a score may pass the base: fp16 ends at 2^16
 constexpr float kKv8Unit = 16777216.f;  // 2^24: a code's fp16 number is code / 2^24
 constexpr uint32_t kKv8OffsetF16 = 0x80808080u;   // two fp16 -2^-17 = -128 / 2^24
 constexpr uint32_t kKv8OffsetBf16 = 0xb700b700u;  // two bf16 -2^-17
@@ -445,7 +448,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
     least = __reduce_min_sync(0xffffffffu, least);
 
     float o[NR][S::MT][4];
-    float m[NR][2], l[NR][2];
+    float m[NR][2], l[NR][2];  // the rows' bases and sums
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
 #pragma unroll
@@ -488,7 +491,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
           for (int e = 0; e < 2; ++e) {
             float next = fmaxf(top[r][e], __shfl_xor_sync(0xffffffffu, top[r][e], 4));
             next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, 8));
-            next = max3(next, __shfl_xor_sync(0xffffffffu, next, 16), m[r][e]);
+            next = fmaxf(fmaxf(next, __shfl_xor_sync(0xffffffffu, next, 16)) - kKv8Under, m[r][e]);
             const float by = m[r][e] == minus_inf ? 0.f : fast_exp2(m[r][e] - next);
             m[r][e] = next;
             l[r][e] *= by;

@@ -1,11 +1,14 @@
-"""The 8-bit cache at the ends of the number range, and values halfway between two codes."""
+"""The 8-bit cache at the ends of the number range, values halfway between two
+codes, and long tails of small probabilities."""
 
 from __future__ import annotations
+
+import math
 
 import pytest
 import torch
 
-from solution.kernels import KV8_BLOCK, Kv8Cache, sm100_kv8_append, sm100_kv8_gather
+from solution.kernels import KV8_BLOCK, Kv8Cache, sm100_kv8_append, sm100_kv8_attention, sm100_kv8_gather
 
 pytestmark = pytest.mark.gpu
 
@@ -81,3 +84,40 @@ def test_codes_are_the_rounded_quotients(dim: int) -> None:
     scale, code = _definition(x)
     assert torch.equal(cache.scales[0, :, :, 0].cpu(), scale)
     assert torch.equal(cache.codes[0, :, :, 0].cpu().float(), code)
+
+
+def _shared_pages(batch: int, kv_heads: int, dim: int, blocks: int, sinks: int) -> Kv8Cache:
+    """Sequences of full blocks that lie in two pages: the first `sinks` blocks in page 0
+    (its first key is zero and its value too), all others in page 1."""
+    cache = Kv8Cache(
+        torch.full((2, 2, kv_heads, KV8_BLOCK, dim), 128, dtype=torch.uint8, device=DEV),
+        torch.full((2, 2, kv_heads), 1.0 / 127, device=DEV),
+        torch.zeros(batch, 2, 2, kv_heads, KV8_BLOCK, dim, dtype=torch.bfloat16, device=DEV),
+        torch.ones(batch, blocks, dtype=torch.int32, device=DEV),
+        torch.full((batch,), blocks * KV8_BLOCK - 1, dtype=torch.int32, device=DEV),
+    )
+    cache.page_table[:, :sinks] = 0
+    return cache
+
+
+def test_a_long_tail_of_small_probabilities_counts() -> None:
+    """A token that takes nearly all of the weight before 262144 tokens of 2^-25.05 each. Taken
+    together they weigh 2^-7; what probabilities of 16 bits may cost is 2^-11 of the
+    largest value.  A warp has some 38000 of the tokens."""
+    batch, kv_heads, dim, blocks = 16, 16, 32, 4096
+    cache = _shared_pages(batch, kv_heads, dim, blocks, 4)
+    codes = cache.codes[0]
+    codes[:, 0, :, :, 0] = 128 - 127  # keys (-1, 0, ...): far below the sink's 0
+    codes[0, 0, :, 0, 0] = 128  # the first key of page 0
+    codes[:, 1] = 255  # values 1, the sink's 0
+    codes[0, 1, :, 0] = 128
+    low = 25.05 * math.log(2.0)
+    q = torch.zeros(batch, 1, kv_heads, dim, device=DEV, dtype=torch.bfloat16)
+    q[..., 0] = 1.0
+    got, _ = sm100_kv8_attention(cache, q, scale=low)
+    tokens = blocks * KV8_BLOCK
+    tail = (tokens - 4) * 2.0**-25.05
+    want = tail / (4 + tail)
+    # scores carry 2^-22 of themselves, 2^-17 in a weight
+    bound = 2.0**-8 * want + 2.0**-11 + 2.0**-17 * want
+    assert abs(float(got.float().mean()) - want) <= bound and float((got.double() - want).abs().max()) <= bound
