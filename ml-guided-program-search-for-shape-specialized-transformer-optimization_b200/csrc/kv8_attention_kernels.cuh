@@ -920,7 +920,9 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
           if (row >= a.tokens * a.group) continue;
           const int token = row / a.group;
           const float sum = ml_out[e].y;
-          const bool real = token < seq.count && sum != 0.f;  // padding rows are zero
+          // Padding rows are zero.  A row sees its own key at least, so that its sum is zero only
+          // where all its scores are -infinity: 0 / 0, as softmax has it.
+          const bool real = token < seq.count;
           const float by = real ? 1.f / sum : 0.f;
           const uint32_t two = real ? pack_bf16x2((e ? acc[i].y : acc[i].x) * by, (e ? acc[i].w : acc[i].z) * by) : 0u;
           *reinterpret_cast<uint32_t*>(a.out + ((static_cast<int64_t>(b) * a.tokens + token) * a.heads + head * a.group +

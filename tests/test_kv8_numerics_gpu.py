@@ -1,5 +1,6 @@
-"""The 8-bit cache at the ends of the number range, values halfway between two
-codes, and long tails of small probabilities."""
+"""The 8-bit cache at the ends of the number range: blocks of tiny values, values
+that lie halfway between two codes, long tails of small probabilities, and
+rows whose scores are all minus infinity."""
 
 from __future__ import annotations
 
@@ -121,3 +122,15 @@ def test_a_long_tail_of_small_probabilities_counts() -> None:
     # scores carry 2^-22 of themselves, 2^-17 in a weight
     bound = 2.0**-8 * want + 2.0**-11 + 2.0**-17 * want
     assert abs(float(got.float().mean()) - want) <= bound and float((got.double() - want).abs().max()) <= bound
+
+
+@pytest.mark.parametrize("dim", [32, 64, 128, 256])
+def test_scores_that_are_all_minus_infinity_give_nan(dim: int) -> None:
+    """As softmax does: no weight is defined.  Rows with one finite score are not concerned."""
+    cache = Kv8Cache.create(slots=1, max_tokens=64, num_kv_heads=1, head_dim=dim, device=DEV)
+    qkv = torch.ones(1, 9, 3 * dim, dtype=torch.bfloat16, device=DEV)
+    qkv[0, :3, dim] = float("-inf")  # the first three tokens' keys
+    q, _ = sm100_kv8_append(cache, qkv, 1)
+    got = sm100_kv8_attention(cache, q)[0][0]
+    assert got.isnan().all(-1).tolist() == [True] * 3 + [False] * 6
+    assert bool((got[3:] == 1).all())  # all values are 1
