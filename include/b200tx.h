@@ -484,7 +484,9 @@ int b200tx_kv8_append(const b200tx_kv8_cache* cache, const void* qkv, int dtype,
 int b200tx_kv8_gather(const b200tx_kv8_cache* cache, void* k_out, void* v_out, int64_t batch, int64_t most,
                       int64_t tokens, const int32_t* slot_ids, const int32_t* counts, cudaStream_t stream);
 
-/* Bytes of workspace that b200tx_kv8_attention needs on the current device. */
+/* Bytes of workspace that b200tx_kv8_attention needs on the current device; the
+ * first B200TX_KV8_COUNTER_BYTES of them are its counters. */
+#define B200TX_KV8_COUNTER_BYTES 8192
 int b200tx_kv8_workspace_bytes(int64_t head_dim, int64_t* bytes_out);
 
 /*
@@ -492,8 +494,9 @@ int b200tx_kv8_workspace_bytes(int64_t head_dim, int64_t* bytes_out);
  * lengths[slot] + t sees the keys up to there) over the cache: softmax(scale q k) v per
  * head, heads / kv_heads query heads to a kv head.  q BF16 [batch, tokens, heads,
  * head_dim] (heads dense, strides in elements), out BF16 dense.  Rows past
- * counts[b] are zero.  workspace: 16-byte aligned, zeroed once before its first
- * use, for one stream at a time; the kernel leaves its counters zero.
+ * counts[b] are zero.  workspace: 16-byte aligned, its counters zeroed once before
+ * its first use, for launches that follow one another only: not for two streams, nor for
+ * a graph and calls beside it; the kernel leaves its counters zero.
  */
 int b200tx_kv8_attention(const b200tx_kv8_cache* cache, const void* q, void* out, int64_t batch, int64_t tokens,
                          int64_t heads, int64_t q_batch_stride, int64_t q_token_stride, const int32_t* slot_ids,

@@ -143,7 +143,7 @@ cudaError_t launch_kv8_gather(b200tx::Kv8GatherArgs& a, cudaStream_t stream) {
 
 // The workspace of the attention: arrival counters, then the parts of tiles
 // that lie in two or more CTAs.
-constexpr int64_t kKv8ArrivalBytes = 8192;
+constexpr int64_t kKv8ArrivalBytes = B200TX_KV8_COUNTER_BYTES;
 
 template <int D, int NR>
 int kv8_attention_grid(int sm_count) {

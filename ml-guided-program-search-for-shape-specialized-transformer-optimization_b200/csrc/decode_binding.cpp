@@ -17,6 +17,7 @@
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <cuda_runtime_api.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -306,8 +307,28 @@ PyObject* kv8_attention_ok(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded(n, 2, [&]() -> PyObject* { return PyBool_FromLong(attention_fits(layer_of(args[0]), tensor(args[1]))); });
 }
 
+// The id of the capture that the stream is in, 0 where it is in none.
+unsigned long long capture_of(cudaStream_t stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  const cudaError_t err = cudaStreamGetCaptureInfo_v2(stream, &status, &id, nullptr, nullptr, nullptr);
+  if (err != cudaSuccess) ineligible("the stream's capture status cannot be read (an earlier CUDA error?)");
+  return status == cudaStreamCaptureStatusNone ? 0 : id;
+}
+
+// A reference that is given up when it goes.
+struct Owned {
+  PyObject* o;
+  explicit Owned(PyObject* p) : o(p) {
+    if (o == nullptr) throw python_error();
+  }
+  Owned(const Owned&) = delete;
+  ~Owned() { Py_DECREF(o); }
+};
+
 // kv8_attention(layer, q, scale or None, slots, counts, out, workspaces, make) -> context
-// workspaces: {stream: uint8 tensor}; make(stream) adds one.
+// workspaces: {stream: uint8 tensor} of the calls outside of captures; make(stream) adds one
+// and gives it, make(stream, capture) gives the one of the capture with that id.
 PyObject* kv8_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded(n, 8, [&]() -> PyObject* {
     const Layer c = layer_of(args[0]);
@@ -322,16 +343,22 @@ PyObject* kv8_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     at::Tensor out = result(args[5], {batch, tokens, heads * dim}, at::kBFloat16, q,
                             "out must be a contiguous, 16-byte aligned bf16 [B, T, H * D] tensor");
     cudaStream_t stream = stream_of(q);
-    PyObject* key = PyLong_FromVoidPtr(stream);
-    PyObject* held = PyDict_GetItemWithError(args[6], key);  // borrowed
-    if (held == nullptr && !PyErr_Occurred()) {
-      PyObject* made = PyObject_CallOneArg(args[7], key);
-      Py_XDECREF(made);  // the dict holds it
-      if (made != nullptr) held = PyDict_GetItemWithError(args[6], key);
+    const Owned key(PyLong_FromVoidPtr(stream));
+    const unsigned long long capture = capture_of(stream);
+    PyObject* held = capture == 0 ? PyDict_GetItemWithError(args[6], key.o) : nullptr;  // borrowed
+    if (held == nullptr && PyErr_Occurred()) throw python_error();
+    if (held != nullptr) {
+      Py_INCREF(held);
+    } else if (capture == 0) {
+      held = PyObject_CallOneArg(args[7], key.o);
+    } else {
+      const Owned id(PyLong_FromUnsignedLongLong(capture));
+      held = PyObject_CallFunctionObjArgs(args[7], key.o, id.o, nullptr);
     }
-    Py_DECREF(key);
-    if (held == nullptr) throw python_error();
-    const at::Tensor& work = THPVariable_Unpack(held);
+    const Owned mine(held);
+    const at::Tensor* given = tensor(mine.o);
+    require(given != nullptr, "the workspace is not a tensor");
+    const at::Tensor& work = *given;
     launched(entry.kv8_attention(c.view, q.const_data_ptr(), out.data_ptr(), batch, tokens, heads, q.stride(0), q.stride(1),
                                  slots, counts, static_cast<float>(scale), work.data_ptr(), work.numel(), stream),
              "b200tx_kv8_attention");

@@ -1008,6 +1008,7 @@ class Kv8CacheView(ctypes.Structure):
 
 
 KV8_BLOCK = 64  # B200TX_KV8_BLOCK
+KV8_COUNTER_BYTES = 8192  # B200TX_KV8_COUNTER_BYTES
 
 
 def _pointer(tensor: torch.Tensor | None) -> int | None:
@@ -1135,6 +1136,7 @@ def linear_w4(
 
 __all__ = [
     "KV8_BLOCK",
+    "KV8_COUNTER_BYTES",
     "Kv8CacheView",
     "Rope",
     "kv8_append",

@@ -94,10 +94,12 @@ class Kv8Cache:
         # what the binding takes for a layer: the struct's address and the device
         self._handles = [(ctypes.addressof(view), codes.get_device()) for view in self._views]
         # The attention's workspace (arrival counters that every launch leaves
-        # zero, and the parts of split tiles), one for each stream it runs on.
-        # A spare one is there from the start for a first call inside a graph
-        # capture, where nothing could be zeroed for good.
+        # zero, and the parts of split tiles): one for each stream it runs on,
+        # and one for each capture, whose graph may be replayed on any stream
+        # beside calls on the one that it was captured on.  A spare is there
+        # from the start for a first call inside a capture.
         self._workspaces: dict[int, torch.Tensor] = {}
+        self._captured: dict[int, tuple[int, torch.Tensor]] = {}  # stream: capture, workspace; of the last capture
         self._spare = self._new_workspace() if self.device.type == "cuda" else None
 
     @classmethod
@@ -141,22 +143,30 @@ class Kv8Cache:
 
     def _new_workspace(self) -> torch.Tensor:
         with torch.cuda.device(self.device):
-            return torch.zeros(_native.kv8_workspace_bytes(self.head_dim), dtype=torch.uint8, device=self.device)
+            made = torch.empty(_native.kv8_workspace_bytes(self.head_dim), dtype=torch.uint8, device=self.device)
+            made[: _native.KV8_COUNTER_BYTES].zero_()
+        return made
 
-    def workspace(self, stream: int) -> torch.Tensor:
-        found = self._workspaces.get(stream)
-        if found is None:
-            if not torch.cuda.is_current_stream_capturing():
-                found = self._new_workspace()
-            elif self._spare is not None:
-                found, self._spare = self._spare, None
-            else:
+    def workspace(self, stream: int, capture: int | None = None) -> torch.Tensor:
+        """What the calls on ``stream`` share, or those of the capture with the
+        id ``capture`` on it.  The latter lies in the graph's own memory, and
+        its counters are cleared by every replay."""
+
+        if capture is None:
+            if stream not in self._workspaces:
+                self._workspaces[stream] = self._new_workspace()
+            return self._workspaces[stream]
+        if stream not in self._workspaces:
+            if self._spare is None:
                 raise RuntimeError(
                     "the cache's attention is captured on a second stream that it has not run on: "
                     "call it once on that stream before the capture"
                 )
-            self._workspaces[stream] = found
-        return found
+            self._workspaces[stream], self._spare = self._spare, None
+        if stream not in self._captured or self._captured[stream][0] != capture:
+            self._captured = {s: held for s, held in self._captured.items() if held[0] == capture}
+            self._captured[stream] = (capture, self._new_workspace())
+        return self._captured[stream][1]
 
     def advance(self, tokens: int | torch.Tensor, slots: torch.Tensor | None = None) -> None:
         """Count the appended tokens as held (all slots, or ``slots``)."""

@@ -1,0 +1,71 @@
+"""Whose workspace an attention call over the 8-bit cache uses: calls on one
+stream share one, a captured graph has its own."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from solution.kernels import Kv8Cache, sm100_kv8_append, sm100_kv8_attention
+
+DEV = "cuda:0"
+
+
+def _randn(*shape: int, seed: int) -> torch.Tensor:
+    return torch.randn(*shape, generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV)
+
+
+def _filled(tokens: int) -> Kv8Cache:
+    cache = Kv8Cache.create(slots=1, max_tokens=tokens, num_kv_heads=2, head_dim=64, device=DEV)
+    sm100_kv8_append(cache, _randn(1, tokens, 6 * 64, seed=3).bfloat16(), 2)
+    cache.advance(tokens - 1)
+    return cache
+
+
+def test_a_capture_has_a_workspace_of_its_own(monkeypatch: pytest.MonkeyPatch) -> None:
+    """By stream outside of captures, by stream and capture inside; no GPU needed."""
+    monkeypatch.setattr(Kv8Cache, "_new_workspace", lambda self: torch.zeros(16))
+    cache = Kv8Cache.create(slots=1, max_tokens=64, num_kv_heads=1, head_dim=64, device="cpu")
+    five, six = cache.workspace(5), cache.workspace(6)
+    assert five is not six and cache.workspace(5) is five
+    first = cache.workspace(5, 101)
+    assert first is not five and cache.workspace(5, 101) is first
+    fork = cache.workspace(6, 101)
+    assert fork is not six and fork is not first and cache.workspace(5, 101) is first
+    second = cache.workspace(5, 102)
+    assert second is not first and second is not five and cache.workspace(5, 102) is second
+    assert cache.workspace(5) is five and cache.workspace(6) is six
+
+
+@pytest.mark.gpu
+def test_a_replay_beside_calls_on_its_capture_stream() -> None:
+    """A graph on one stream, calls on the stream that it was captured on, and another
+    graph captured there on a third, all at once: each gives the bits that it gives alone."""
+    with torch.inference_mode():
+        cache = _filled(30000)  # one sequence over every SM: all tiles are split
+        queries = [_randn(1, 1, 2, 64, seed=s).bfloat16() for s in range(3)]
+        want = [sm100_kv8_attention(cache, q)[0].clone() for q in queries]
+        capture, one, two = (torch.cuda.Stream() for _ in range(3))
+        capture.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(capture):
+            sm100_kv8_attention(cache, queries[0])
+        torch.cuda.synchronize()
+        graphs, outs = [], []
+        for q in queries[:2]:
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=capture):
+                # two calls of a capture share its workspace, as a model's layers do
+                sm100_kv8_attention(cache, queries[2])
+                outs.append(sm100_kv8_attention(cache, q)[0])
+        for stream in (one, two, capture):
+            stream.wait_stream(torch.cuda.current_stream())
+        held = []
+        for _ in range(50):
+            for graph, stream in zip(graphs, (one, two)):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+            with torch.cuda.stream(capture):
+                held.append(sm100_kv8_attention(cache, queries[2])[0])
+        torch.cuda.synchronize()
+        assert all(torch.equal(got, want[2]) for got in held)
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
