@@ -327,7 +327,7 @@ struct Owned {
 };
 
 // kv8_attention(layer, q, scale or None, slots, counts, out, workspaces, make) -> context
-// workspaces: {stream: uint8 tensor} of the calls outside of captures; make(stream) adds one
+// workspaces: {stream: uint8 tensor or None} of the calls outside of captures; make(stream) adds one
 // and gives it, make(stream, capture) gives the one of the capture with that id.
 PyObject* kv8_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded(n, 8, [&]() -> PyObject* {
@@ -347,7 +347,7 @@ PyObject* kv8_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const unsigned long long capture = capture_of(stream);
     PyObject* held = capture == 0 ? PyDict_GetItemWithError(args[6], key.o) : nullptr;  // borrowed
     if (held == nullptr && PyErr_Occurred()) throw python_error();
-    if (held != nullptr) {
+    if (held != nullptr && held != Py_None) {
       Py_INCREF(held);
     } else if (capture == 0) {
       held = PyObject_CallOneArg(args[7], key.o);

@@ -96,11 +96,10 @@ class Kv8Cache:
         # The attention's workspace (arrival counters that every launch leaves
         # zero, and the parts of split tiles): one for each stream it runs on,
         # and one for each capture, whose graph may be replayed on any stream
-        # beside calls on the one that it was captured on.  A spare is there
-        # from the start for a first call inside a capture.
-        self._workspaces: dict[int, torch.Tensor] = {}
+        # beside calls on the one that it was captured on.  All are made when
+        # they are first asked for; None: the stream has been captured on only.
+        self._workspaces: dict[int, torch.Tensor | None] = {}
         self._captured: dict[int, tuple[int, torch.Tensor]] = {}  # stream: capture, workspace; of the last capture
-        self._spare = self._new_workspace() if self.device.type == "cuda" else None
 
     @classmethod
     def create(
@@ -153,16 +152,18 @@ class Kv8Cache:
         its counters are cleared by every replay."""
 
         if capture is None:
-            if stream not in self._workspaces:
-                self._workspaces[stream] = self._new_workspace()
-            return self._workspaces[stream]
+            found = self._workspaces.get(stream)
+            if found is None:
+                found = self._workspaces[stream] = self._new_workspace()
+            return found
         if stream not in self._workspaces:
-            if self._spare is None:
+            # a call on the stream comes before its captures; one stream may do without
+            if any(held is None for held in self._workspaces.values()):
                 raise RuntimeError(
                     "the cache's attention is captured on a second stream that it has not run on: "
                     "call it once on that stream before the capture"
                 )
-            self._workspaces[stream], self._spare = self._spare, None
+            self._workspaces[stream] = None
         if stream not in self._captured or self._captured[stream][0] != capture:
             self._captured = {s: held for s, held in self._captured.items() if held[0] == capture}
             self._captured[stream] = (capture, self._new_workspace())

@@ -69,3 +69,25 @@ def test_a_replay_beside_calls_on_its_capture_stream() -> None:
         torch.cuda.synchronize()
         assert all(torch.equal(got, want[2]) for got in held)
         assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+
+
+@pytest.mark.gpu
+def test_registered_operators_make_what_they_use(monkeypatch: pytest.MonkeyPatch) -> None:
+    """Their handles live for one call: the append makes no workspace, the attention one,
+    of which only the counters are cleared."""
+    made = []
+    make = Kv8Cache._new_workspace
+
+    def counted(self: Kv8Cache) -> torch.Tensor:
+        made.append(make(self))
+        return made[-1]
+
+    monkeypatch.setattr(Kv8Cache, "_new_workspace", counted)
+    with torch.inference_mode():
+        cache = _filled(300)
+        parts = (cache.codes[0], cache.scales[0], cache.tail[0], cache.page_table, cache.lengths)
+        made.clear()
+        q = torch.ops.b200tx.kv8_append(*parts, _randn(1, 1, 6 * 64, seed=2).bfloat16(), 2)
+        assert q.shape == (1, 1, 2, 64) and not made
+        got = torch.ops.b200tx.kv8_attention(*parts, q)
+        assert len(made) == 1 and torch.equal(got, sm100_kv8_attention(cache, q)[0])
