@@ -25,6 +25,7 @@ SM100_KV8_GATHER_BACKEND = "sm100_kv8_gather"
 SM100_KV8_ATTENTION_BACKEND = "sm100_kv8_attention"
 KV8_BLOCK = _native.KV8_BLOCK
 KV8_HEAD_DIMS = (32, 64, 128, 256)
+_MOST_STREAMS = 8  # that a cache holds a workspace for; each is 2 to 5 MB
 
 
 class Kv8Cache:
@@ -154,6 +155,10 @@ class Kv8Cache:
         if capture is None:
             found = self._workspaces.get(stream)
             if found is None:
+                # The oldest goes: it was allocated on the stream that it served, so that
+                # the allocator gives its memory out after that stream's launches.
+                while len(self._workspaces) >= _MOST_STREAMS:
+                    del self._workspaces[next(iter(self._workspaces))]
                 found = self._workspaces[stream] = self._new_workspace()
             return found
         if stream not in self._workspaces:

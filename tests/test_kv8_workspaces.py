@@ -37,6 +37,20 @@ def test_a_capture_has_a_workspace_of_its_own(monkeypatch: pytest.MonkeyPatch) -
     assert cache.workspace(5) is five and cache.workspace(6) is six
 
 
+def test_workspaces_of_many_streams_are_given_up(monkeypatch: pytest.MonkeyPatch) -> None:
+    """The oldest ones; a stream that comes back gets a new one; captures hold the last one's."""
+    monkeypatch.setattr(Kv8Cache, "_new_workspace", lambda self: torch.zeros(16))
+    cache = Kv8Cache.create(slots=1, max_tokens=64, num_kv_heads=1, head_dim=64, device="cpu")
+    first = cache.workspace(1)
+    for stream in range(2, 100):
+        latest = cache.workspace(stream)
+        assert cache.workspace(stream) is latest
+        for capture in (2 * stream, 2 * stream + 1):
+            cache.workspace(stream, capture)
+        assert len(cache._workspaces) <= 8 and len(cache._captured) == 1
+    assert cache.workspace(1) is not first
+
+
 @pytest.mark.gpu
 def test_a_replay_beside_calls_on_its_capture_stream() -> None:
     """A graph on one stream, calls on the stream that it was captured on, and another
@@ -91,3 +105,22 @@ def test_registered_operators_make_what_they_use(monkeypatch: pytest.MonkeyPatch
         assert q.shape == (1, 1, 2, 64) and not made
         got = torch.ops.b200tx.kv8_attention(*parts, q)
         assert len(made) == 1 and torch.equal(got, sm100_kv8_attention(cache, q)[0])
+
+
+@pytest.mark.gpu
+def test_more_streams_than_workspaces() -> None:
+    with torch.inference_mode():
+        cache = _filled(30000)
+        q = _randn(1, 1, 2, 64, seed=1).bfloat16()
+        want = sm100_kv8_attention(cache, q)[0].clone()
+        streams = [torch.cuda.Stream() for _ in range(12)]
+        outs = []
+        for stream in streams:
+            stream.wait_stream(torch.cuda.current_stream())
+        for _ in range(5):
+            for stream in streams:
+                with torch.cuda.stream(stream):
+                    outs.append(sm100_kv8_attention(cache, q)[0])
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want) for out in outs)
+        assert len(cache._workspaces) <= 8
