@@ -429,7 +429,7 @@ typedef struct b200tx_rope {
  * RMS norm of each query and key head (x / sqrt(mean(x^2) + eps) * weight; a NULL
  * weight: none) and the rotation (rope NULL: none), over the packed projection
  * [batch, tokens, (heads + 2 kv_heads) * head_dim]: query, key, value heads.
- * Value heads are copied; out may be qkv (in place).  dtype F32 or BF16 for both; pointers
+ * Value heads are copied; out may be qkv (in place), else they share no memory.  dtype F32 or BF16 for both; pointers
  * 16-byte aligned, strides in elements, multiples of 8; head_dim 8..256, a power
  * of two.  positions: int32 (or int64 with positions_64), element
  * [b * position_batch_stride + t], or NULL = t.
@@ -467,7 +467,7 @@ typedef struct b200tx_kv8_cache {
  * of `batch` sequences (slot slot_ids[b], or b): keys normed and rotated at
  * their position lengths[slot] + t as b200tx_qk_norm_rope does, keys and values
  * rounded to BF16 and stored; blocks that fill are quantised.  q_out BF16
- * [batch, tokens, heads, head_dim]: the queries, normed and rotated.  qkv
+ * [batch, tokens, heads, head_dim]: the queries, normed and rotated (no memory of qkv's).  qkv
  * [batch, tokens, (heads + 2 kv_heads) * head_dim] in dtype, strides in
  * elements.  lengths is not changed: the caller advances it when every layer
  * has run, by any number up to `tokens` when that is at most 64 (tokens past it
@@ -493,7 +493,8 @@ int b200tx_kv8_workspace_bytes(int64_t head_dim, int64_t* bytes_out);
  * Attention of the `tokens` tokens appended last (query t at position
  * lengths[slot] + t sees the keys up to there) over the cache: softmax(scale q k) v per
  * head, heads / kv_heads query heads to a kv head.  q BF16 [batch, tokens, heads,
- * head_dim] (heads dense, strides in elements), out BF16 dense.  Rows past
+ * head_dim] (heads dense, strides in elements), out BF16 dense: other memory than q's, or q
+ * itself where q is dense.  Rows past
  * counts[b] are zero.  workspace: 16-byte aligned, its counters zeroed once before
  * its first use, for launches that follow one another only: not for two streams, nor for
  * a graph and calls beside it; the kernel leaves its counters zero.
@@ -509,6 +510,7 @@ int b200tx_kv8_attention(const b200tx_kv8_cache* cache, const void* q, void* out
  * for each 32).  x BF16, rows x_stride elements apart (a multiple of 8); scales
  * BF16 [Kp / group, N], Kp = K rounded up to 128; bias F32 or NULL; out F32 or
  * BF16; group 32, 64 or 128; K a multiple of 8; epilogue B200TX_EPI_*.
+ * out shares no memory with x.
  * packed [N, Kp / 2] uint8, 16-byte aligned, codes past K any, x counts as 0 there: the
  * 128 codes of a run are 16 little-endian 32-bit words of 8 consecutive weights, nibble i of a
  * word (from the lowest) holding weight {0,2,4,6,1,3,5,7}[i]; word 4 a + b is

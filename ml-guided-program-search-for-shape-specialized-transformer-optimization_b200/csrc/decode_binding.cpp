@@ -98,12 +98,65 @@ void launched(int status, const char* what) {
   throw python_error();
 }
 
-// `out` if the caller gave one (checked), else a new tensor.
-at::Tensor result(PyObject* out, at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like, const char* text) {
+struct Span {
+  uintptr_t begin, end;
+};
+
+// The addresses that a tensor lies within.
+Span span(const at::Tensor& t) {
+  int64_t last = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+  return {begin, begin + static_cast<uintptr_t>(last + 1) * t.element_size()};
+}
+
+bool apart(const at::Tensor& a, const at::Tensor& b) {
+  const Span x = span(a), y = span(b);
+  return x.end <= y.begin || y.end <= x.begin;
+}
+
+// The rows of a packed tensor [B, T, W] in memory: `inner` rows at the smaller distance `near`,
+// groups of them `far` apart.
+struct Rows {
+  int64_t inner, near, outer, far;
+};
+
+Rows rows(const at::Tensor& t) {
+  const int64_t batch = t.size(0), tokens = t.size(1), b = t.stride(0), k = t.stride(1);
+  return tokens > 1 && (batch == 1 || k <= b) ? Rows{tokens, k, batch, b} : Rows{batch, b, tokens, k};
+}
+
+// Whether no two rows share memory.
+bool rows_once(const at::Tensor& t) {
+  const Rows r = rows(t);
+  const int64_t width = t.size(2), group = (r.inner > 1 ? (r.inner - 1) * r.near : 0) + width;
+  return (r.inner == 1 || r.near >= width) && (r.outer == 1 || r.far >= group);
+}
+
+// Whether two packed tensors of one shape and type share no memory: they lie apart, or are columns
+// of the same longer rows.
+bool rows_apart(const at::Tensor& a, const at::Tensor& b) {
+  if (apart(a, b)) return true;
+  const Rows r = rows(a), other = rows(b);
+  if (r.inner == 1 || r.inner != other.inner || r.near != other.near || r.near <= 0 ||
+      (r.outer > 1 && (r.far != other.far || r.far % r.near != 0)))
+    return false;
+  const int64_t bytes = static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.const_data_ptr()) -
+                                             reinterpret_cast<uintptr_t>(b.const_data_ptr()));
+  const int64_t row = r.near * a.element_size(), width = a.size(2) * a.element_size();
+  const int64_t off = (bytes % row + row) % row;
+  return off >= width && row - off >= width;
+}
+
+// `out` if the caller gave one (checked: it shares no memory with `like`, the input), else a new tensor.
+at::Tensor result(PyObject* out, at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like, const char* text,
+                  bool in_place = false) {
   if (out == Py_None) return at::empty(sizes, at::TensorOptions().dtype(type).device(like.device()));
   const at::Tensor* t = tensor(out);
   require(t != nullptr && t->sizes() == sizes && t->scalar_type() == type && t->device() == like.device() &&
               t->is_contiguous() && aligned(*t), text);
+  require(apart(*t, like) || (in_place && t->const_data_ptr() == like.const_data_ptr() && like.is_contiguous()),
+          "out shares memory with the input");
   return *t;
 }
 
@@ -215,6 +268,9 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
                   (given->const_data_ptr() != qkv.const_data_ptr() || given->strides() == qkv.strides()),
               "out must have qkv's shape, dtype and device, 16-byte aligned heads, and qkv's strides when it is qkv");
       out = *given;
+      // in place every value is read and written by the same lane
+      require(rows_once(out) && (out.const_data_ptr() == qkv.const_data_ptr() || rows_apart(out, qkv)),
+              "out shares memory with qkv or with itself");
     }
     launched(entry.qk_norm_rope(qkv.const_data_ptr(), out.data_ptr(), dtype(qkv), qkv.size(0), qkv.size(1), heads, kv_heads,
                                 dim, qkv.stride(0), qkv.stride(1), out.stride(0), out.stride(1), qw, kw,
@@ -341,7 +397,7 @@ PyObject* kv8_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int32_t* counts = per_sequence(args[4], batch, q, kCounts);
     require(slots != nullptr || batch <= c.view->slots, kBatch);
     at::Tensor out = result(args[5], {batch, tokens, heads * dim}, at::kBFloat16, q,
-                            "out must be a contiguous, 16-byte aligned bf16 [B, T, H * D] tensor");
+                            "out must be a contiguous, 16-byte aligned bf16 [B, T, H * D] tensor", true);
     cudaStream_t stream = stream_of(q);
     const Owned key(PyLong_FromVoidPtr(stream));
     const unsigned long long capture = capture_of(stream);

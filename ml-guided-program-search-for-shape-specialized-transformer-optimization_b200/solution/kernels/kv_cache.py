@@ -265,7 +265,8 @@ def sm100_kv8_attention(
     """``softmax(scale q k^T) v`` of the ``T`` tokens appended last over their
     sequences' keys, causal: ``q`` bf16 ``[B, T, H, D]`` at positions ``lengths + t``.
     Returns the context, bf16 ``[B, T, H * D]``; rows past ``counts[b]`` are zero.
-    ``H / Hkv`` query heads share a kv head; ``scale`` defaults to ``D ** -0.5``."""
+    ``H / Hkv`` query heads share a kv head; ``scale`` defaults to ``D ** -0.5``.
+    ``out`` may be a dense ``q``'s own memory."""
 
     result = binding().kv8_attention(
         cache.handle(layer), q, scale, slots, counts, out, cache._workspaces, cache.workspace
