@@ -175,14 +175,14 @@ class Kv8Cache:
         return self._captured[stream][1]
 
     def advance(self, tokens: int | torch.Tensor, slots: torch.Tensor | None = None) -> None:
-        """Count the appended tokens as held (all slots, or ``slots``)."""
+        """Count the appended tokens as held (all slots, or ``slots``; as in the
+        kernels, a row whose slot is none counts nowhere)."""
 
         if slots is None:
             self.lengths.add_(tokens)
-        elif isinstance(tokens, torch.Tensor):
-            self.lengths.index_add_(0, slots, tokens.to(torch.int32))
-        else:
-            self.lengths.index_add_(0, slots, torch.full_like(slots, tokens, dtype=torch.int32))
+            return
+        inside = slots.clamp(0, self.slots - 1)
+        self.lengths.index_add_(0, inside, (inside == slots).to(torch.int32).mul_(tokens))
 
 
 def can_use_sm100_kv8_append(cache: Kv8Cache, qkv: torch.Tensor, num_heads: int) -> bool:
