@@ -39,6 +39,17 @@ def require(condition: bool, message: str) -> None:
         raise ValueError(message)
 
 
+class TensorHandle:
+    """Base of handles whose tensors are checked, and their addresses taken, when the
+    handle is made: they are changed in place, and not exchanged for others."""
+
+    def __setattr__(self, name: str, value: object) -> None:
+        held = self.__dict__.get(name)
+        if isinstance(held, torch.Tensor) and held is not value:
+            raise AttributeError(f"{type(self).__name__}.{name} cannot be exchanged: change it in place, or make a new handle")
+        super().__setattr__(name, value)
+
+
 def launch(fn, *args) -> None:  # noqa: ANN001 - thin forwarding helper
     """Run a launch on the tensors' device, translating failures to RuntimeError."""
 

@@ -17,7 +17,7 @@ import ctypes
 import torch
 
 from .. import _native
-from ._common import binding, is_sm100_cuda, library_ready, require
+from ._common import TensorHandle, binding, is_sm100_cuda, library_ready, require
 from .rotary import RotaryTable
 
 SM100_KV8_APPEND_BACKEND = "sm100_kv8_append"
@@ -28,7 +28,7 @@ KV8_HEAD_DIMS = (32, 64, 128, 256)
 _MOST_STREAMS = 8  # that a cache holds a workspace for; each is 2 to 5 MB
 
 
-class Kv8Cache:
+class Kv8Cache(TensorHandle):
     """The tensors of a cache, shared by the layers of a model.
 
     * ``codes`` uint8 ``[layers, pages, 2, Hkv, 64, D]`` (keys, values): a full
@@ -40,7 +40,7 @@ class Kv8Cache:
 
     ``codes``, ``scales`` and ``tail`` may leave out the layers.  The caller
     fills ``page_table`` (``create`` gives each slot pages of its own) and may
-    change it and ``lengths`` between steps; the kernels check both, store
+    change it and ``lengths`` in place between steps; the kernels check both, store
     nothing out of range and read NaN from there.
     """
 

@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import torch
 
-from ._common import binding, is_sm100_cuda, library_ready, require
+from ._common import TensorHandle, binding, is_sm100_cuda, library_ready, require
 
 SM100_LINEAR_W4_BACKEND = "sm100_linear_w4"
 SM100_LINEAR_W4_GELU_BACKEND = "sm100_linear_w4_gelu"
@@ -21,7 +21,7 @@ _ORDER = (0, 2, 4, 6, 1, 3, 5, 7)  # nibble i of a word holds weight _ORDER[i] o
 _OUT = (torch.float32, torch.bfloat16)
 
 
-class W4Weight:
+class W4Weight(TensorHandle):
     """A packed ``[N, K]`` weight.
 
     * ``packed`` uint8 ``[N, Kp / 2]``, ``Kp`` = K rounded up to 128.  128 weights of a

@@ -16,13 +16,13 @@ import ctypes
 import torch
 
 from .. import _native
-from ._common import binding, is_sm100_cuda, library_ready, require
+from ._common import TensorHandle, binding, is_sm100_cuda, library_ready, require
 
 SM100_QK_NORM_ROPE_BACKEND = "sm100_qk_norm_rope"
 ROPE_HEAD_DIMS = (8, 16, 32, 64, 128, 256)
 
 
-class RotaryTable:
+class RotaryTable(TensorHandle):
     """cos and sin of the angles, fp32 ``[positions, rotary / 2]``.
 
     The first ``rotary`` dims of a head are turned: pairs ``(i, i + rotary/2)``,
