@@ -183,7 +183,6 @@ int64_t kv8_workspace(int sm_count) {
 template <int D, int NR>
 cudaError_t launch_kv8_attention(b200tx::Kv8AttnArgs& a, DeviceState* dev, int index, cudaStream_t stream) {
   using S = b200tx::Kv8Shape<D, NR>;
-  a.row_tiles = (a.tokens * a.group + S::ROWS - 1) / S::ROWS;
   if (!dev->kv8_attr[index]) {
     cudaError_t err =
         cudaFuncSetAttribute(b200tx::kv8_attention_kernel<D, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::MAIN);

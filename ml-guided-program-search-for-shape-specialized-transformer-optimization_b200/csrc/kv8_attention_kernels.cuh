@@ -104,7 +104,7 @@ struct Kv8AttnArgs {
   __nv_bfloat16* out;                   // [batch, tokens, heads, D]
   const int32_t* slot_ids;
   const int32_t* counts;
-  int batch, tokens, heads, group, row_tiles;
+  int batch, tokens, heads, group;
   float scale_log2;                     // scale * log2(e)
   float* parts;                         // [grid, 2, PART_FLOATS]
   unsigned int* arrivals;               // [grid], zero between launches
@@ -201,13 +201,15 @@ __host__ __device__ constexpr uint32_t kv8_tail_v_place(uint32_t at) {
   return D >= 64 ? at ^ (((pair & 1u) << 4) | ((pair & 2u) << 5)) : at;
 }
 
-// What one sequence asks for: its tokens in all, and the steps over them.
+// What one sequence asks for: its tokens in all, the steps over them, and the units of the
+// line: a tile's steps and its fixed cost, for the tiles that its own new tokens fill.
 struct Kv8Sequence {
   int slot, total, count, steps;
-  bool bad;  // no such slot, or longer than its page table: outputs are NaN
+  unsigned tiles, cost, units;  // cost: of one tile; units: of all
+  bool bad;                     // no such slot, or longer than its page table: outputs are NaN
 };
 
-template <int TOK>
+template <int TOK, int ROWS>
 __device__ __forceinline__ Kv8Sequence kv8_sequence(const Kv8AttnArgs& a, int b) {
   Kv8Sequence s;
   s.slot = a.slot_ids == nullptr ? b : a.slot_ids[b];
@@ -220,6 +222,9 @@ __device__ __forceinline__ Kv8Sequence kv8_sequence(const Kv8AttnArgs& a, int b)
   s.steps = s.bad || s.count == 0
                 ? 0
                 : s.total / kKv8Block * (kKv8Block / TOK) + (open + TOK / 2 - 1) / (TOK / 2);
+  s.cost = s.steps == 0 ? 0u : static_cast<unsigned>(s.steps + kKv8TileCost);
+  s.tiles = s.steps == 0 ? 0u : a.cache.kv_heads * ((static_cast<unsigned>(s.count) * a.group + ROWS - 1) / ROWS);
+  s.units = s.cost * s.tiles;
   return s;
 }
 
@@ -237,31 +242,27 @@ template <int D, int NR>
 __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_attention_kernel(Kv8AttnArgs a) {
   using S = Kv8Shape<D, NR>;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ unsigned scan[kKv8Warps];
+  __shared__ unsigned scan[kKv8Warps], scan_tiles[kKv8Warps];
   __shared__ unsigned found_offset;
   __shared__ int found_b;
   __shared__ float2 warp_ml[kKv8Warps][S::ROWS];
   __shared__ int is_last;
 
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t4 = lane % 4;
-  const unsigned tiles = a.cache.kv_heads * a.row_tiles;  // of a sequence
+  auto sequence = [&](int b) { return kv8_sequence<S::TOK, S::ROWS>(a, b); };
   const float minus_inf = __int_as_float(0xff800000), nan = __int_as_float(0x7fffffff);
   griddep_wait();
   griddep_launch_dependents();
 
   // ---- where this CTA's range begins
-  auto cost_of = [&](int steps) { return steps == 0 ? 0u : static_cast<unsigned>(steps + kKv8TileCost); };
   const int chunk = (a.batch + kKv8Warps * 32 - 1) / (kKv8Warps * 32);
-  unsigned mine = 0;
+  unsigned mine = 0, mine_tiles = 0;
+  bool gaps = false;
   for (int b = tid * chunk; b < min(a.batch, (tid + 1) * chunk); ++b) {
-    const Kv8Sequence s = kv8_sequence<S::TOK>(a, b);
-    mine += cost_of(s.steps);
-    if (s.steps == 0 && b % gridDim.x == blockIdx.x) {
-      // nothing to attend to: zeros (NaN if the sequence is not one)
-      const uint32_t fill = s.bad ? 0x7fff7fffu : 0u;
-      uint4* o = reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(b) * a.tokens * a.heads * D);
-      for (int64_t i = 0; i < static_cast<int64_t>(a.tokens) * a.heads * D / 8; ++i) o[i] = make_uint4(fill, fill, fill, fill);
-    }
+    const Kv8Sequence s = sequence(b);
+    mine += s.units;
+    mine_tiles += s.tiles;
+    gaps = gaps || s.bad || s.count < a.tokens;
   }
   // inclusive sums over the warp, then exclusive over the CTA
   unsigned before = mine;
@@ -270,21 +271,39 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
     const unsigned n = __shfl_up_sync(0xffffffffu, before, d);
     if (lane >= d) before += n;
   }
-  if (lane == 31) scan[warp] = before;
-  __syncthreads();
+  mine_tiles = __reduce_add_sync(0xffffffffu, mine_tiles);
+  if (lane == 31) {
+    scan[warp] = before;
+    scan_tiles[warp] = mine_tiles;
+  }
+  gaps = __syncthreads_or(gaps);
   before -= mine;
-  unsigned all = 0;
+  unsigned total = 0, tiles = 0;  // the host has checked that they fit
 #pragma unroll
   for (int w = 0; w < kKv8Warps; ++w) {
     if (w < warp) before += scan[w];
-    all += scan[w];
+    total += scan[w];
+    tiles += scan_tiles[w];
   }
-  const unsigned total = all * tiles;  // the host has checked that it fits
+  if (gaps) {
+    // Rows past the counts are zero, all rows of what is no sequence NaN: no tile has them.  A
+    // sequence's rows for each CTA, or a part of them where the sequences are fewer.
+    const unsigned parts = max(1u, gridDim.x / a.batch);
+    for (unsigned item = blockIdx.x; item < parts * a.batch; item += gridDim.x) {
+      const unsigned b = item % a.batch, part = item / a.batch;
+      const Kv8Sequence s = sequence(b);
+      const int first = s.bad ? 0 : s.count;
+      const uint32_t fill = s.bad ? 0x7fff7fffu : 0u;
+      const int64_t values = static_cast<int64_t>(a.heads) * D / 8, n = (a.tokens - first) * values;
+      uint4* const o = reinterpret_cast<uint4*>(a.out) + (static_cast<int64_t>(b) * a.tokens + first) * values;
+      for (int64_t i = part * (kKv8Warps * 32) + tid; i < n; i += parts * (kKv8Warps * 32)) o[i] = make_uint4(fill, fill, fill, fill);
+    }
+  }
   // Units of a CTA: at least a step for each warp, so that short contexts are not cut
   // into crumbs; and where few long tiles are left to all CTAs, not so few that joining
   // a tile's n parts takes longer than reading its units / n (their sum is least at
   // n ~ sqrt(units); by the mean tile: 32768 tokens of one kv head 31.6 -> 16.4 us).
-  const float mean_units = __fdividef(static_cast<float>(all), static_cast<float>(a.batch));
+  const float mean_units = __fdividef(static_cast<float>(total), fmaxf(1.f, static_cast<float>(tiles)));
   const float least_units = fmaxf(kKv8Warps, kKv8JoinShare * __fsqrt_rn(mean_units));
   const unsigned ctas = min(static_cast<unsigned>(__fdividef(static_cast<float>(total), least_units)) + (total != 0), gridDim.x);
   if (blockIdx.x >= ctas) return;
@@ -292,11 +311,11 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
   ranges.each = total / ctas;
   ranges.more = total - ranges.each * ctas;
   const unsigned lo = ranges.begin(blockIdx.x), hi = ranges.begin(blockIdx.x + 1);
-  if (lo >= before * tiles && lo < (before + mine) * tiles) {
-    unsigned offset = before * tiles;
+  if (lo >= before && lo < before + mine) {
+    unsigned offset = before;
     int b = tid * chunk;
     for (;; ++b) {
-      const unsigned n = cost_of(kv8_sequence<S::TOK>(a, b).steps) * tiles;
+      const unsigned n = sequence(b).units;
       if (lo < offset + n) break;
       offset += n;
     }
@@ -307,16 +326,16 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
 
   int b = found_b;
   unsigned offset = found_offset;  // of sequence b in the line
-  Kv8Sequence seq = kv8_sequence<S::TOK>(a, b);
+  Kv8Sequence seq = sequence(b);
   uint8_t* const ring = smem + warp * S::STAGES * S::STAGE;
   unsigned cur = lo;
   bool first_piece = true;
   while (cur < hi) {
-    while (cur >= offset + cost_of(seq.steps) * tiles) {
-      offset += cost_of(seq.steps) * tiles;
-      seq = kv8_sequence<S::TOK>(a, ++b);
+    while (cur >= offset + seq.units) {
+      offset += seq.units;
+      seq = sequence(++b);
     }
-    const unsigned cost = cost_of(seq.steps);
+    const unsigned cost = seq.cost;
     const int tile = static_cast<int>((cur - offset) / cost);
     const unsigned tile_begin = offset + tile * cost;
     // a tile's units are its fixed cost, then its steps
@@ -346,7 +365,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
     for (int r = 0; r < NR; ++r) {
       const int row = row0 + r * 8 + g;
       const int token = a.tokens == 1 ? row >= a.group : row / a.group;
-      const bool real = row < a.tokens * a.group && token < seq.count;
+      const bool real = token < seq.count;
       my_limit[r] = real ? start + token : -1;
       if (real) least = min(least, my_limit[r]);
       const __nv_bfloat16* src = a.q + static_cast<int64_t>(b) * a.q_batch_stride + token * a.q_token_stride +
@@ -917,14 +936,12 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int row = row0 + share_rows * 8 + 2 * t4 + e;
-          if (row >= a.tokens * a.group) continue;
           const int token = row / a.group;
-          const float sum = ml_out[e].y;
-          // Padding rows are zero.  A row sees its own key at least, so that its sum is zero only
-          // where all its scores are -infinity: 0 / 0, as softmax has it.
-          const bool real = token < seq.count;
-          const float by = real ? 1.f / sum : 0.f;
-          const uint32_t two = real ? pack_bf16x2((e ? acc[i].y : acc[i].x) * by, (e ? acc[i].w : acc[i].z) * by) : 0u;
+          if (token >= seq.count) continue;
+          // A row sees its own key at least, so that its sum is zero only where all its scores
+          // are -infinity: 0 / 0, as softmax has it.
+          const float by = 1.f / ml_out[e].y;
+          const uint32_t two = pack_bf16x2((e ? acc[i].y : acc[i].x) * by, (e ? acc[i].w : acc[i].z) * by);
           *reinterpret_cast<uint32_t*>(a.out + ((static_cast<int64_t>(b) * a.tokens + token) * a.heads + head * a.group +
                                                 row % a.group) * D + d) = two;
         }
