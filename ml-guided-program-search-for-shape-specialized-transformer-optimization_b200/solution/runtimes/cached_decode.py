@@ -54,7 +54,8 @@ class CachedDecoder:
       of ``group``), ``"bf16"`` runs them with the model's own
     * ``rope``: a ``RotaryTable``; ``qk_norms``: per layer ``(q_weight, k_weight)``,
       fp32 ``[head_dim]`` each
-    * ``graph``: replay a step from a CUDA graph, one for each input buffer
+    * ``graph``: replay a step of up to 64 tokens from a CUDA graph, captured once for
+      each shape and dtype; ``x`` is copied into the buffer that the graph reads
       (``solution.runtimes.CudaGraphReplay``)
 
     The model's weights are read when the decoder is made: make a new one
@@ -110,7 +111,7 @@ class CachedDecoder:
                     {name: pack_w4(linear.weight, group) for name, linear in self._linears(layer)}
                     for layer in model.layers
                 ]
-        self._replays: dict[tuple[object, ...], CudaGraphReplay] = {}
+        self._replays: dict[tuple[object, ...], tuple[torch.Tensor, CudaGraphReplay]] = {}
 
     @staticmethod
     def _linears(layer: Any) -> tuple[tuple[str, Any], ...]:
@@ -255,8 +256,9 @@ class CachedDecoder:
             if self.graph and x.shape[1] <= _REPEATABLE:
                 key = (tuple(x.shape), x.dtype)
                 if key not in self._replays:
-                    self._replays[key] = CudaGraphReplay()
-                y = self._replays[key].run(self._program, x, None)
+                    self._replays[key] = (torch.empty_like(x), CudaGraphReplay())
+                buffer, replay = self._replays[key]
+                y = replay.run(self._program, buffer.copy_(x), None)
             else:
                 y = self._program(x)
         if advance:
