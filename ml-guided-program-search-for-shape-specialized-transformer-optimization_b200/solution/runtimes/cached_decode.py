@@ -95,6 +95,7 @@ class CachedDecoder:
         self.slots = slots
         self.max_tokens = max_tokens
         self.held = 0  # tokens of each slot, as far as this decoder has counted them
+        self.pending = 0  # of those appended last, the ones that may still be counted
         self.rope = rope
         self.qk_norms = qk_norms or [(None, None)] * config.num_layers
         self.qk_norm_eps = float(qk_norm_eps)
@@ -224,14 +225,21 @@ class CachedDecoder:
 
         with torch.inference_mode():
             self.cache.lengths.zero_()
-        self.held = 0
+        self.held = self.pending = 0
 
     def advance(self, tokens: int) -> None:
-        """Count ``tokens`` of those appended last as held, in every slot."""
+        """Count ``tokens`` of those that the last step appended as held, in every
+        slot: any number of them up to 64, else all (a block that a longer call
+        fills is only kept as codes, and cannot be open again)."""
 
+        if not 0 <= tokens <= self.pending:
+            raise ValueError(f"{tokens} tokens cannot be counted: {self.pending} are not counted yet")
+        if tokens != self.pending > _REPEATABLE:
+            raise ValueError(f"a step of {self.pending} tokens, more than {_REPEATABLE}, is counted whole")
         with torch.inference_mode():
             self.cache.advance(tokens)
         self.held += tokens
+        self.pending -= tokens
 
     def prompt(self, x: torch.Tensor) -> torch.Tensor:
         """The forward of ``x`` ``[slots, T, D]`` from empty sequences, which it leaves
@@ -241,15 +249,19 @@ class CachedDecoder:
         self.reset()
         with torch.inference_mode():
             y = self._program(x, prompt=True)
+        self.pending = x.shape[1]
         self.advance(x.shape[1])
         return y
 
     def step(self, x: torch.Tensor, *, advance: bool = True) -> torch.Tensor:
         """The forward of the next tokens ``x`` ``[slots, T, D]``.  With
         ``advance=False`` the caller says afterwards how many of them count
-        (``decoder.advance(n)``; for up to 64 tokens any number of them)."""
+        (``decoder.advance(n)``; for up to 64 tokens any number of them, none
+        where the next step comes first)."""
 
         self._check(x, self.held)
+        if self.pending > _REPEATABLE:
+            raise ValueError(f"the last step's {self.pending} tokens cannot be taken back: advance({self.pending}) first")
         with torch.inference_mode():
             # A capture runs the step once before it records it, so that the
             # first call appends the same tokens twice.
@@ -261,6 +273,7 @@ class CachedDecoder:
                 y = replay.run(self._program, buffer.copy_(x), None)
             else:
                 y = self._program(x)
+        self.pending = x.shape[1]
         if advance:
             self.advance(x.shape[1])
         return y

@@ -1,4 +1,4 @@
-"""Steps of ``CachedDecoder``: how often they are captured."""
+"""Steps of ``CachedDecoder``: how often they are captured, and which of their tokens count."""
 
 from __future__ import annotations
 
@@ -59,3 +59,57 @@ def test_fresh_inputs_replay_one_graph(monkeypatch: pytest.MonkeyPatch) -> None:
         _near(decoder.step(x[:, t : t + 4].contiguous()), want[:, t : t + 4])
     _near(decoder.step(x[:, 90:91].contiguous().bfloat16()), want[:, 90:91])
     assert len(captures) == 3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("graph", [False, True])
+def test_advance_counts_what_can_be_counted(graph: bool) -> None:
+    config = WorkloadConfig(2, 400, 128, 2, 256, 2)
+    model = _model(config)
+    x = _randn(2, 400, 128)
+    with torch.inference_mode():
+        want = model(x)
+    decoder = CachedDecoder(model, slots=2, max_tokens=400, weights="bf16", graph=graph)
+
+    def lengths() -> list[int]:
+        return [decoder.held, *decoder.cache.lengths.tolist()]
+
+    with pytest.raises(ValueError, match="counted"):
+        decoder.advance(1)  # nothing has been appended
+    decoder.prompt(x[:, :60].contiguous())
+    for n in (-1, 1):
+        with pytest.raises(ValueError, match="counted"):
+            decoder.advance(n)
+    decoder.advance(0)
+    # a draft over a block's end: three of nine, then two more, then none of the rest
+    _near(decoder.step(x[:, 60:69].contiguous(), advance=False), want[:, 60:69])
+    for n in (-1, 10):
+        with pytest.raises(ValueError, match="counted"):
+            decoder.advance(n)
+    decoder.advance(3)
+    with pytest.raises(ValueError, match="counted"):
+        decoder.advance(7)
+    decoder.advance(2)
+    assert lengths() == [65, 65, 65]
+    _near(decoder.step(x[:, 65:66].contiguous()), want[:, 65:66])
+    with pytest.raises(ValueError, match="counted"):
+        decoder.advance(1)
+    # more than 64 tokens: all or nothing else
+    _near(decoder.step(x[:, 66:166].contiguous(), advance=False), want[:, 66:166])
+    for n in (0, 50, 99, 101, -1):
+        with pytest.raises(ValueError, match="counted"):
+            decoder.advance(n)
+    with pytest.raises(ValueError, match="taken back"):
+        decoder.step(x[:, 66:67].contiguous())
+    assert lengths() == [66, 66, 66]
+    decoder.advance(100)
+    assert lengths() == [166, 166, 166]
+    _near(decoder.step(x[:, 166:167].contiguous()), want[:, 166:167])
+    # forgetting everything is always possible
+    decoder.step(x[:, 167:267].contiguous(), advance=False)
+    decoder.reset()
+    assert lengths() == [0, 0, 0]
+    _near(decoder.step(x[:, :70].contiguous()), want[:, :70])
+    decoder.step(x[:, 70:270].contiguous(), advance=False)
+    _near(decoder.prompt(x[:, :30].contiguous()), want[:, :30])
+    _near(decoder.step(x[:, 30:31].contiguous()), want[:, 30:31])
