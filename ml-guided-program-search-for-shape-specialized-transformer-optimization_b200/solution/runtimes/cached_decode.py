@@ -42,7 +42,11 @@ from ..kernels import (
 from ..kernels.kv_cache import KV8_HEAD_DIMS
 from .cuda_graph import CudaGraphReplay
 
-_W4_ROWS = 32  # rows of a step up to which the 4-bit kernel reads the weights once
+# Rows of a step up to which its projections go through the 4-bit kernel, which reads the weights
+# again for each 16 or 32 rows; above, through the bf16 GEMM with the values that the packed
+# weights stand for.  The four layers of 1024 (FFN 4096) at 64 rows: 24 us against 37, at 128 38 against 47, at 256
+# 70 against 48; 4096 -> 14336 at 32 rows 28 against 29, at 64 48 against 28.
+_W4_ROWS = 64
 _REPEATABLE = 64  # tokens that can be appended twice over and leave what once leaves
 
 
@@ -51,7 +55,9 @@ class CachedDecoder:
     sequences of up to ``max_tokens`` tokens.
 
     * ``weights``: ``"w4"`` packs the projections to 4 bits for the steps (groups
-      of ``group``), ``"bf16"`` runs them with the model's own
+      of ``group``; a step of more than 64 rows takes the same values rounded to
+      bf16, which the first such step lays out), ``"bf16"`` runs the steps with the
+      model's own, as the prompt always does
     * ``rope``: a ``RotaryTable``; ``qk_norms``: per layer ``(q_weight, k_weight)``,
       fp32 ``[head_dim]`` each
     * ``graph``: replay a step of up to 64 tokens from a CUDA graph, captured once for
@@ -112,6 +118,7 @@ class CachedDecoder:
                     {name: pack_w4(linear.weight, group) for name, linear in self._linears(layer)}
                     for layer in model.layers
                 ]
+        self._wide_weights: list[dict[str, torch.Tensor]] | None = None  # the packed ones' values in bf16
         self._replays: dict[tuple[object, ...], tuple[torch.Tensor, CudaGraphReplay]] = {}
 
     @staticmethod
@@ -141,12 +148,14 @@ class CachedDecoder:
         batch, tokens, d_model = value.shape
         rows = batch * tokens
         flat = value.reshape(rows, d_model)
-        packed = None if prompt or rows > _W4_ROWS else self.step_weights
+        packed = None if prompt else self.step_weights
 
         def linear(index: int, name: str, module: Any, x: torch.Tensor, *, gelu: bool = False) -> torch.Tensor:
             weight, bias = module.shadow_parameters()
-            if packed is not None:
+            if packed is not None and rows <= _W4_ROWS:
                 return sm100_linear_w4(x, packed[index][name], bias, gelu=gelu)[0]
+            if packed is not None:
+                weight = self._wide_weights[index][name]
             return sm100_linear(x, weight, bias, gelu=gelu)[0]
 
         normalized, _ = sm100_initial_layer_norm(flat, (layers[0].norm1 if len(layers) else final).kernel_norm())
@@ -263,6 +272,11 @@ class CachedDecoder:
         if self.pending > _REPEATABLE:
             raise ValueError(f"the last step's {self.pending} tokens cannot be taken back: advance({self.pending}) first")
         with torch.inference_mode():
+            if self.step_weights is not None and self._wide_weights is None and self.slots * x.shape[1] > _W4_ROWS:
+                self._wide_weights = [
+                    {name: packed.dequantize(torch.bfloat16).contiguous() for name, packed in layer.items()}
+                    for layer in self.step_weights
+                ]
             # A capture runs the step once before it records it, so that the
             # first call appends the same tokens twice.
             if self.graph and x.shape[1] <= _REPEATABLE:

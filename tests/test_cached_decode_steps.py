@@ -1,4 +1,5 @@
-"""Steps of ``CachedDecoder``: how often they are captured, and which of their tokens count."""
+"""Steps of ``CachedDecoder``: how often they are captured, which of their tokens
+count, and which weights they run with."""
 
 from __future__ import annotations
 
@@ -8,6 +9,7 @@ import pytest
 import torch
 from conftest import MAX_ABS_TOL, REL_L2_TOL
 
+from solution.kernels import pack_w4
 from solution.runtimes import CachedDecoder, cuda_graph
 from solution.transformer import UserOptimizedTransformer, copy_model_weights
 from workloads import WorkloadConfig, seeded_state_dict
@@ -113,3 +115,29 @@ def test_advance_counts_what_can_be_counted(graph: bool) -> None:
     decoder.step(x[:, 70:270].contiguous(), advance=False)
     _near(decoder.prompt(x[:, :30].contiguous()), want[:, :30])
     _near(decoder.step(x[:, 30:31].contiguous()), want[:, 30:31])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize(("slots", "tokens"), [(1, 1), (33, 1), (64, 1), (65, 1), (130, 1), (4, 16), (4, 17), (2, 100)])
+def test_steps_of_any_size_run_with_the_packed_weights(slots: int, tokens: int) -> None:
+    """Within the gate of the model that has the packed weights' values, and outside it for
+    the one that has its own: weights of unlike size in one group make the two differ."""
+    config = WorkloadConfig(slots, 40 + 2 * tokens, 128, 2, 256, 2)
+    linears = lambda model: [  # noqa: E731
+        linear for layer in model.layers
+        for linear in (layer.attention.qkv_proj, layer.attention.out_proj, layer.ffn_in, layer.ffn_out)
+    ]
+    model, same = _model(config), _model(config)
+    with torch.no_grad():
+        for linear, other in zip(linears(model), linears(same)):
+            linear.weight[:, ::2] *= 0.06  # beside full weights these round to none or one step
+            other.weight.copy_(pack_w4(linear.weight).dequantize())
+    x = _randn(slots, config.seq_len, 128)
+    with torch.inference_mode():
+        want, plain = same(x), model(x)
+    decoder = CachedDecoder(model, slots=slots, max_tokens=config.seq_len)
+    for t in range(0, config.seq_len - tokens + 1, tokens):
+        got = decoder.step(x[:, t : t + tokens].contiguous())
+        _near(got, want[:, t : t + tokens])
+    with pytest.raises(AssertionError):
+        _near(got, plain[:, t : t + tokens])
