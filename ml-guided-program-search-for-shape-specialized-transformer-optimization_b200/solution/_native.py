@@ -1015,74 +1015,6 @@ def _pointer(tensor: torch.Tensor | None) -> int | None:
     return None if tensor is None else tensor.data_ptr()
 
 
-def qk_norm_rope(
-    qkv: torch.Tensor,
-    out: torch.Tensor,
-    heads: int,
-    kv_heads: int,
-    head_dim: int,
-    q_weight: torch.Tensor | None,
-    k_weight: torch.Tensor | None,
-    eps: float,
-    rope: object | None,
-    positions: torch.Tensor | None,
-) -> None:
-    """Launch b200tx_qk_norm_rope over qkv [B, T, W]; `rope` is a ctypes
-    reference to a Rope, `positions` [B, T] or [T]."""
-
-    batch, tokens, _ = qkv.shape
-    status = load().b200tx_qk_norm_rope(
-        qkv.data_ptr(), out.data_ptr(), dtype_code(qkv.dtype), batch, tokens, heads, kv_heads, head_dim,
-        qkv.stride(0), qkv.stride(1), out.stride(0), out.stride(1), _pointer(q_weight), _pointer(k_weight), eps, rope,
-        _pointer(positions), int(positions is not None and positions.dtype == torch.int64),
-        positions.stride(0) if positions is not None and positions.ndim == 2 else 0, _stream(qkv.device),
-    )
-    if status:
-        _check(status, "b200tx_qk_norm_rope")
-
-
-def kv8_append(
-    cache: object,
-    qkv: torch.Tensor,
-    q_out: torch.Tensor,
-    heads: int,
-    slot_ids: torch.Tensor | None,
-    counts: torch.Tensor | None,
-    q_weight: torch.Tensor | None,
-    k_weight: torch.Tensor | None,
-    eps: float,
-    rope: object | None,
-) -> None:
-    """Launch b200tx_kv8_append; `cache` is a ctypes reference to a Kv8CacheView."""
-
-    batch, tokens, _ = qkv.shape
-    status = load().b200tx_kv8_append(
-        cache, qkv.data_ptr(), dtype_code(qkv.dtype), q_out.data_ptr(), batch, tokens, heads, qkv.stride(0),
-        qkv.stride(1), _pointer(slot_ids), _pointer(counts), _pointer(q_weight), _pointer(k_weight), eps, rope,
-        _stream(qkv.device),
-    )
-    if status:
-        _check(status, "b200tx_kv8_append")
-
-
-def kv8_gather(
-    cache: object,
-    k_out: torch.Tensor,
-    v_out: torch.Tensor,
-    tokens: int,
-    slot_ids: torch.Tensor | None,
-    counts: torch.Tensor | None,
-) -> None:
-    """Launch b200tx_kv8_gather into k_out and v_out [B, most, Hkv, D]."""
-
-    status = load().b200tx_kv8_gather(
-        cache, k_out.data_ptr(), v_out.data_ptr(), k_out.shape[0], k_out.shape[1], tokens, _pointer(slot_ids),
-        _pointer(counts), _stream(k_out.device),
-    )
-    if status:
-        _check(status, "b200tx_kv8_gather")
-
-
 def kv8_workspace_bytes(head_dim: int) -> int:
     """The attention's workspace on the current device."""
 
@@ -1139,12 +1071,9 @@ __all__ = [
     "KV8_COUNTER_BYTES",
     "Kv8CacheView",
     "Rope",
-    "kv8_append",
     "kv8_attention",
-    "kv8_gather",
     "kv8_workspace_bytes",
     "linear_w4",
-    "qk_norm_rope",
     "IPC_HANDLE_BYTES",
     "peer_alloc",
     "peer_close",
