@@ -416,7 +416,7 @@ int b200tx_peer_wait(const uint32_t* flags, int count, int self, uint32_t epoch,
 /* Rotation tables: cos and sin F32 [positions, rotary / 2]; the first `rotary`
  * dims of a head are turned, pairs (i, i + rotary / 2), or (2i, 2i + 1) when
  * interleaved.  rotary: a multiple of 8 (16 for head_dim 256) up to head_dim.
- * A position outside the table gives NaN heads. */
+ * At a position outside the table the turned dims are NaN. */
 typedef struct b200tx_rope {
   const float* cos;
   const float* sin;
@@ -464,7 +464,7 @@ typedef struct b200tx_kv8_cache {
 
 /*
  * Appends `tokens` new tokens (counts[b] of them where counts is given) of each
- * of `batch` sequences (slot slot_ids[b], or b): keys normed and rotated at
+ * of `batch` sequences (slot slot_ids[b], or b; a slot once at most): keys normed and rotated at
  * their position lengths[slot] + t as b200tx_qk_norm_rope does, keys and values
  * rounded to BF16 and stored; blocks that fill are quantised.  q_out BF16
  * [batch, tokens, heads, head_dim]: the queries, normed and rotated (no memory of qkv's).  qkv
@@ -506,8 +506,8 @@ int b200tx_kv8_attention(const b200tx_kv8_cache* cache, const void* q, void* out
 
 /*
  * out[M, N] = epilogue(x[M, K] . W^T + bias), W[n, k] = scales[k / group, n] *
- * (code[n, k] - 8) with 4-bit codes, for a few rows (the weights are read once
- * for each 32).  x BF16, rows x_stride elements apart (a multiple of 8); scales
+ * (code[n, k] - 8) with 4-bit codes, for a few rows: the weights are read once for
+ * each 16, or for each 32 where N >= 80 for each SM.  x BF16, rows x_stride elements apart (a multiple of 8); scales
  * BF16 [Kp / group, N], Kp = K rounded up to 128; bias F32 or NULL; out F32 or
  * BF16; group 32, 64 or 128; K a multiple of 8; epilogue B200TX_EPI_*.
  * out shares no memory with x.

@@ -22,8 +22,8 @@
 // of steps in shared memory of its own, filled by cp.async: no barrier between
 // warps, deep enough to cover the HBM latency.  A copy of 8 lanes is one
 // 128-byte line; with the lanes in the fragments' order instead (rows 2 t for
-// values) the same loads took 67 us where these take 52 (16 sequences x 8192
-// tokens, 8 heads of 128).  Within a line the 16-byte chunks are permuted by
+// values) the call took 1.29 times as long (16 sequences x 8192 tokens, 8 heads of
+// 128).  Within a line the 16-byte chunks are permuted by
 // the row, so that the fragments are read without bank conflicts.
 //
 // Products.  Keys and values are the A operand (16 tokens, or 16 dims), queries
@@ -47,8 +47,8 @@
 // and queries are bf16 and each probability is the sum of two bf16 numbers.
 //
 // Measured: 100000 tokens of 16 heads of 64 in 43 us (4.8 TB/s), 16 x 8192 of 8 heads of
-// 128 in 56 us (4.8 TB/s), 64 ragged sequences up to 8192 in 34 us, 1000 tokens of 16
-// heads of 64 in 7.8 us.  Of a long call some 8 us are launch, ramp and the last join;
+// 128 in 56 us (4.8 TB/s), 64 ragged sequences up to 8192 in 33 us, 1000 tokens of 16
+// heads of 64 in 8.6 us.  Of a long call some 8 us are launch, ramp and the last join;
 // the rest runs at 6 TB/s.  With 8 to 12 warps an SM the instructions of a step are
 // the next bound.
 #pragma once
@@ -59,7 +59,10 @@
 namespace b200tx {
 
 constexpr int kKv8Warps = 4;
-// What beginning and joining a tile costs, in steps (64 ragged sequences: 6 steps 42.3 us, 12 34.5, 24 37.8).
+// What beginning and joining a tile costs, in steps, one number for all head_dims.  64 ragged sequences up
+// to 8192, with 6 / 12 / 24 steps: head_dim 128 40.5 / 33.9 / 38.5 us, 256 50.1 / 37.6 / 36.0, 32 28.1 / 26.3 /
+// 30.4, 64 22.3 / 22.9 / 27.2; 16 x 8 tokens over up to 4000: 128 35.7 / 28.8 / 32.0, 256 27.2 / 22.9 / 23.7,
+// 64 21.1 / 21.4 / 24.5; 128 sequences up to 500: 128 20.4 / 21.7 / 23.5, 64 15.0 / 15.8 / 16.3.
 constexpr int kKv8TileCost = 12;
 constexpr float kKv8JoinShare = 0.5f;  // what a part costs to join, against a step: its root
 constexpr float kKv8Under = 7.f;      // log2 of how far a row's base lies under its maximum when it moves

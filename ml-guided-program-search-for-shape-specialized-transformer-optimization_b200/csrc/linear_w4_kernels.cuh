@@ -2,9 +2,9 @@
 // held in 4 bits and a bf16 scale for each group of weights along K:
 //   W[n, k] = scale[k / group, n] * (code[n, k] - 8),   code in 0..15
 //
-// What bounds it: with up to 32 rows the weights' bytes over HBM, N K / 2 (and
-// 2 N K / group of scales); next to it the instructions that turn codes into
-// numbers, 11 for a word of 8.
+// What bounds it: with few rows the weights' bytes over HBM, N K / 2 (and 2 N K / group
+// of scales); next to it the instructions, of which turning codes into numbers is 11
+// for a word of 8; with 17 rows and more x, which every CTA copies for its own columns.
 //
 // Layout.  A word is 8 consecutive weights of a row, ordered so that one mask
 // takes two neighbours (nibble i holds weight {0,2,4,6,1,3,5,7}[i]): the
@@ -21,7 +21,7 @@
 // warps share x.  The sum of a group is multiplied by its scale and added in fp32; the
 // slices are joined in shared memory in a fixed order.
 //
-// Measured: 1 x 1024 -> 4096 in 3.3 us, 32 x 4096 -> 14336 in 23 us, 8 x 8192 -> 28672 (122
+// Measured: 1 x 1024 -> 4096 in 3.0 us, 32 x 4096 -> 14336 in 25 us, 8 x 8192 -> 28672 (122
 // MB) in 38 us.  Masks and shifts run at half rate, and 224 CTAs on 148 SMs leave
 // half of the SMs less to do; for up to 16 rows and many units the kernel at the end
 // of this file keeps x in shared memory and shares evenly: 31 us, 3.9 TB/s.
@@ -49,7 +49,8 @@ struct W4Args {
   int stages;                    // of the ring
 };
 
-// The lowest nibbles of both halves as bf16 numbers code - 8.  The mask and the
+// The lowest nibbles of both halves as bf16 numbers code - 8, the usual way to expand
+// 4-bit codes.  The mask and the
 // exponent are one three-input operation: these and the shifts run at half
 // rate and are what the kernel issues most.
 __device__ __forceinline__ uint32_t nibbles_bf16x2(uint32_t w) {
@@ -274,8 +275,9 @@ __global__ void __launch_bounds__(kW4Warps * 32, 2) linear_w4_kernel(W4Args a) {
 // weights only and needs no barrier: each warp has a ring of its own.  A CTA has an
 // equal share of the 16-column tiles; its (tile, stage) units form one line that the
 // warps cut into equal ranges.  Tiles that lie in several ranges are joined in shared
-// memory, in the order of the ranges.  8 x 8192 -> 28672 takes 31.2 us (3.9 TB/s; 38.2
-// above), bound by its instructions: schedulers issue in two of three cycles.
+// memory, in the order of the ranges.  8 x 8192 -> 28672 takes 30.9 us (3.9 TB/s; 38.2
+// above), bound by its instructions, 363 for 16 columns x 256 weights: schedulers issue in
+// two of three cycles.
 
 constexpr int kW4LineWarps = 16;
 constexpr int kW4LineStage = 16 * (kW4Runs * kW4Run / 2);  // bytes of a warp's stage

@@ -213,8 +213,8 @@ def sm100_kv8_append(
     the way as ``sm100_qk_norm_rope`` does with position ``lengths + t``; returns
     the queries, normed and rotated, bf16 ``[B, T, H, D]``.
 
-    Row b is slot ``slots[b]`` (default b) and has ``counts[b]`` tokens (default
-    T).  ``lengths`` stays as it is until ``cache.advance``: by all the tokens,
+    Row b is slot ``slots[b]`` (default b; a slot once at most) and has ``counts[b]``
+    tokens (default T).  ``lengths`` stays as it is until ``cache.advance``: by all the tokens,
     or, for ``T <= 64``, by any number of them (the rest is forgotten)."""
 
     result = binding().kv8_append(

@@ -106,8 +106,9 @@ def sm100_linear_w4(
     out: torch.Tensor | None = None,
 ) -> tuple[torch.Tensor, str]:
     """``[..., K] x [N, K]^T -> [..., N]`` with a packed weight: bf16 ``value``,
-    fp32 accumulation, fp32 bias and erf GELU before the cast.  Made for up to 32
-    rows; more are taken 32 at a time, each time reading the weight again."""
+    fp32 accumulation, fp32 bias and erf GELU before the cast.  Made for few rows:
+    beyond 16 they are taken 16 at a time, or 32 where N is at least 80 for each SM,
+    each time reading the weight again.  ``out`` shares no memory with ``value``."""
 
     require(out_dtype in _OUT, "out_dtype must be float32 or bfloat16")
     result = binding().linear_w4(

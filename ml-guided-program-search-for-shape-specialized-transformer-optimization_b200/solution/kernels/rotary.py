@@ -27,7 +27,7 @@ class RotaryTable(TensorHandle):
 
     The first ``rotary`` dims of a head are turned: pairs ``(i, i + rotary/2)``,
     or ``(2i, 2i + 1)`` with ``interleaved``.  ``rotary`` is a multiple of 8 (of
-    16 for head_dim 256).  A position outside the table gives NaN heads.
+    16 for head_dim 256).  At a position outside the table the turned dims are NaN.
     """
 
     def __init__(self, cos: torch.Tensor, sin: torch.Tensor, *, interleaved: bool = False) -> None:
