@@ -220,6 +220,7 @@ cudaError_t launch_w4(b200tx::W4Args& a, DeviceState* dev, int index, cudaStream
                 static_cast<size_t>(std::max(a.stages * stage, join)), stream, a);
 }
 
+constexpr int64_t kW4GridRows = 65535;     // of x tiles: the grid's second dimension
 constexpr int kW4LineShared = 227 * 1024;  // of a CTA that has an SM to itself
 constexpr int64_t kW4LineUnits = 48;       // (16 columns, stage) units for each SM
 
@@ -527,9 +528,10 @@ int b200tx_linear_w4(const void* x, int64_t x_stride, const void* packed, const 
   // Rows of x by eights: 1, 2 or 4 MMA columns.  Four only where the columns of W
   // fill the SMs; with fewer the rows go 16 at a time, which makes twice the CTAs
   // and reads the weights again from L2 (29 x 4744 -> 5003: four 23.9 us, twice two 22.4).
-  cudaError_t err = M <= 8                                     ? launch_w4_tiles<1>(group, a, dev, 0, stream)
-                    : M <= 16 || a.outer < 80 * dev->sm_count ? launch_w4_tiles<2>(group, a, dev, 6, stream)
-                                                               : launch_w4_tiles<4>(group, a, dev, 12, stream);
+  const bool by_16 = M <= 16 || (a.outer < 80 * dev->sm_count && M <= 16 * kW4GridRows);
+  cudaError_t err = M <= 8   ? launch_w4_tiles<1>(group, a, dev, 0, stream)
+                    : by_16 ? launch_w4_tiles<2>(group, a, dev, 6, stream)
+                             : launch_w4_tiles<4>(group, a, dev, 12, stream);
   return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "linear_w4");
 }
 

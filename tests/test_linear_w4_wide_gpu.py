@@ -48,3 +48,14 @@ def test_linear_w4_many_columns(rows: int, inner: int, outer: int, group: int, o
         x[rows - 1, inner // 2] = float("nan")  # stays in its own row
         got, _ = sm100_linear_w4(x, weight, bias, out_dtype=out_dtype)
         assert got.isnan().all(-1).tolist() == [False] * (rows - 1) + [True] and not got[:-1].isnan().any()
+
+
+@pytest.mark.parametrize("rows", [65535 * 16, 65535 * 16 + 1, 1 << 20])
+def test_linear_w4_as_many_rows_as_there_may_be(rows: int) -> None:
+    with torch.inference_mode():
+        weight = pack_w4(_randn(3, 16, seed=1), 32)
+        x = _randn(rows, 16, seed=2).bfloat16()
+        got, _ = sm100_linear_w4(x, weight, out_dtype=torch.float32)
+        want = x.double() @ weight.dequantize(torch.float64).t()
+        bound = 18 * 2.0**-23 * (x.double().abs() @ weight.dequantize(torch.float64).abs().t())
+        assert bool(((got.double() - want).abs() <= bound).all())
