@@ -47,8 +47,8 @@
 // and queries are bf16 and each probability is the sum of two bf16 numbers.
 //
 // Measured: 100000 tokens of 16 heads of 64 in 43 us (4.8 TB/s), 16 x 8192 of 8 heads of
-// 128 in 56 us (4.8 TB/s), 64 ragged sequences up to 8192 in 33 us, 1000 tokens of 16
-// heads of 64 in 8.6 us.  Of a long call some 8 us are launch, ramp and the last join;
+// 128 in 55 us (4.9 TB/s), 64 ragged sequences up to 8192 in 33 us, 1000 tokens of 16
+// heads of 64 in 7.9 us.  Of a long call some 8 us are launch, ramp and the last join;
 // the rest runs at 6 TB/s.  With 8 to 12 warps an SM the instructions of a step are
 // the next bound.
 #pragma once
@@ -245,7 +245,7 @@ template <int D, int NR>
 __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_attention_kernel(Kv8AttnArgs a) {
   using S = Kv8Shape<D, NR>;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ unsigned scan[kKv8Warps], scan_tiles[kKv8Warps];
+  __shared__ unsigned scan[kKv8Warps], scan_tiles[kKv8Warps], scan_gaps[kKv8Warps];
   __shared__ unsigned found_offset;
   __shared__ int found_b;
   __shared__ float2 warp_ml[kKv8Warps][S::ROWS];
@@ -275,20 +275,23 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
     if (lane >= d) before += n;
   }
   mine_tiles = __reduce_add_sync(0xffffffffu, mine_tiles);
+  const unsigned warp_gaps = __any_sync(0xffffffffu, gaps);
   if (lane == 31) {
     scan[warp] = before;
     scan_tiles[warp] = mine_tiles;
+    scan_gaps[warp] = warp_gaps;
   }
-  gaps = __syncthreads_or(gaps);
+  __syncthreads();  // a barrier that joins the flags costs 0.6 us of 1000 tokens of 16 heads of 64
   before -= mine;
-  unsigned total = 0, tiles = 0;  // the host has checked that they fit
+  unsigned total = 0, tiles = 0, all_gaps = 0;  // the host has checked that they fit
 #pragma unroll
   for (int w = 0; w < kKv8Warps; ++w) {
     if (w < warp) before += scan[w];
     total += scan[w];
     tiles += scan_tiles[w];
+    all_gaps |= scan_gaps[w];
   }
-  if (gaps) {
+  if (all_gaps != 0) {
     // Rows past the counts are zero, all rows of what is no sequence NaN: no tile has them.  A
     // sequence's rows for each CTA, or a part of them where the sequences are fewer.
     const unsigned parts = max(1u, gridDim.x / a.batch);
