@@ -368,7 +368,10 @@ unsigned long long capture_of(cudaStream_t stream) {
   cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
   unsigned long long id = 0;
   const cudaError_t err = cudaStreamGetCaptureInfo_v2(stream, &status, &id, nullptr, nullptr, nullptr);
-  if (err != cudaSuccess) ineligible("the stream's capture status cannot be read (an earlier CUDA error?)");
+  if (err != cudaSuccess) {
+    cudaGetLastError();  // it is told here; whoever asks next does not find it again
+    ineligible("the stream's capture status cannot be read (another stream's capture, or an earlier CUDA error)");
+  }
   return status == cudaStreamCaptureStatusNone ? 0 : id;
 }
 
