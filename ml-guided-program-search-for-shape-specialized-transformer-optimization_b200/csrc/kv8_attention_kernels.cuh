@@ -360,7 +360,6 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
     const int open = seq.total - full * kKv8Block;
     const int start = seq.total - seq.count;
     const int mine_steps = max(0, (step1 - step0 - warp + kKv8Warps - 1) / kKv8Warps);
-    bool poisoned = false;
 
     // ---- queries: lane (g, t) has dims of row g of each row group, as B fragments.
     // Their loads go out first, to wait together with the page numbers'.
@@ -397,7 +396,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
         const uint32_t stage = smem_u32(ring + (k % S::STAGES) * S::STAGE);
         constexpr int COPIES = S::HALF / 512;  // of 16 bytes a lane
         if (step < coded_steps) {
-          poisoned = poisoned || page < 0;
+          const bool known = page >= 0;
           page = max(page, 0);  // page 0 is always there
           const int64_t at = static_cast<int64_t>(page) * 2 * a.cache.kv_heads + head;
           const uint8_t* kp = a.cache.codes + at * kKv8Block * D + step % (kKv8Block / S::TOK) * S::HALF + lane * 16;
@@ -407,7 +406,14 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
 #pragma unroll
           for (int x = 0; x < COPIES; ++x)
             cp_async<16>(stage + S::HALF + (kv8_v_place<D>(lane * 16) ^ (kv8_v_place<D>(x * 512) & 511u)) + x * 512, vp + x * 512);
-          if (lane < 2) cp_async<4>(stage + 2 * S::HALF + 4 * lane, a.cache.scales + at + lane * a.cache.kv_heads);
+          if (lane < 2) {
+            // a block whose page is not in the table counts as one whose scales are NaN
+            if (known) {
+              cp_async<4>(stage + 2 * S::HALF + 4 * lane, a.cache.scales + at + lane * a.cache.kv_heads);
+            } else {
+              *reinterpret_cast<float*>(ring + (k % S::STAGES) * S::STAGE + 2 * S::HALF + 4 * lane) = nan;
+            }
+          }
         } else {
           const int first = (step - coded_steps) * S::TAIL;
           const __nv_bfloat16* kp = kv8_tail(a.cache, seq.slot, full & 1, 0, head, D) + first * D + lane * 8;
@@ -798,7 +804,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, Kv8Shape<D, NR>::CTAS) kv8_att
       for (int r = 0; r < NR; ++r) {
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          warp_ml[warp][r * 8 + 2 * t4 + e] = make_float2(m[r][e], poisoned ? nan : l[r][e] * kKv8SumUnit);
+          warp_ml[warp][r * 8 + 2 * t4 + e] = make_float2(m[r][e], l[r][e] * kKv8SumUnit);
       }
     }
     __syncthreads();  // everyone is done with the ring

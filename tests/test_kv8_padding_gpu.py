@@ -1,5 +1,6 @@
 """Attention over the 8-bit cache for batches whose sequences have different numbers of
-new tokens: rows past a sequence's count are zero and cost next to nothing.
+new tokens: rows past a sequence's count are zero and cost next to nothing; and rows
+that end before a block whose page is not in the table.
 
 Tolerance as for the attention elsewhere: a bf16 result (2^-8 of its size) of
 probabilities rounded to 11 bits (2^-11 of the largest value)."""
@@ -102,6 +103,30 @@ def test_more_sequences_than_ctas() -> None:
     slots[5], slots[600] = -1, batch
     _check(cache, _randn(batch, tokens, heads, dim, seed=2).bfloat16(), counts, slots,
            [None if not 0 <= s < batch else t for s, t in zip(slots, totals)])
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("dim", [32, 64, 128, 256])
+def test_rows_before_a_block_without_a_page(dim: int, wide: bool) -> None:
+    """New tokens over a block's end: the rows that do not see the block are what they are, the
+    others NaN."""
+    cache = _filled([192, 200], 2, dim, 256)
+    cache.lengths.sub_(100)  # rows at 92..191 and 100..199; block 2 is tokens 128..191
+    want = [None, None]
+    q = _randn(2, 100, 4, dim, seed=3).bfloat16()
+    for b, (total, seen) in enumerate(((192, 36), (200, 28))):
+        want[b] = _want(cache, b, q[b], total)[:seen]
+    if wide:
+        table = torch.full((cache.slots, 12500), -1, dtype=torch.int32, device=DEV)
+        table[:, : cache.max_blocks] = cache.page_table
+        cache = Kv8Cache(cache.codes, cache.scales, cache.tail, table, cache.lengths)
+    cache.page_table[0, 2], cache.page_table[1, 2] = -1, cache.pages
+    got = sm100_kv8_attention(cache, q)[0].view(2, 100, 4, dim)
+    for b, rows in enumerate(want):
+        n = len(rows)
+        off = (got[b, :n].double() - rows).abs()
+        assert bool((off <= 2.0**-8 * rows.abs() + 2.0**-11 * 6).all())
+        assert bool(got[b, n:].isnan().all())
 
 
 def _time(call) -> float:  # noqa: ANN001
