@@ -52,7 +52,8 @@ _REPEATABLE = 64  # tokens that can be appended twice over and leave what once l
 
 class CachedDecoder:
     """Prompt and steps of a ``UserOptimizedTransformer`` over a cache of ``slots``
-    sequences of up to ``max_tokens`` tokens.
+    sequences of up to ``max_tokens`` tokens.  The slots go together: all hold
+    the same number of tokens.
 
     * ``weights``: ``"w4"`` packs the projections to 4 bits for the steps (groups
       of ``group``; a step of more than 64 rows takes the same values rounded to
@@ -266,7 +267,8 @@ class CachedDecoder:
         """The forward of the next tokens ``x`` ``[slots, T, D]``.  With
         ``advance=False`` the caller says afterwards how many of them count
         (``decoder.advance(n)``; for up to 64 tokens any number of them, none
-        where the next step comes first)."""
+        where the next step comes first).  A step of more than 64 tokens that
+        fails on its way forgets every sequence."""
 
         self._check(x, self.held)
         if self.pending > _REPEATABLE:
@@ -286,7 +288,13 @@ class CachedDecoder:
                 buffer, replay = self._replays[key]
                 y = replay.run(self._program, buffer.copy_(x), None)
             else:
-                y = self._program(x)
+                try:
+                    y = self._program(x)
+                except BaseException:
+                    # the layers that it came to may hold some of it in place of older tokens
+                    if x.shape[1] > _REPEATABLE:
+                        self.reset()
+                    raise
         self.pending = x.shape[1]
         if advance:
             self.advance(x.shape[1])

@@ -10,7 +10,7 @@ import torch
 from conftest import MAX_ABS_TOL, REL_L2_TOL
 
 from solution.kernels import pack_w4
-from solution.runtimes import CachedDecoder, cuda_graph
+from solution.runtimes import CachedDecoder, cached_decode, cuda_graph
 from solution.transformer import UserOptimizedTransformer, copy_model_weights
 from workloads import WorkloadConfig, seeded_state_dict
 
@@ -141,3 +141,36 @@ def test_steps_of_any_size_run_with_the_packed_weights(slots: int, tokens: int) 
         _near(got, want[:, t : t + tokens])
     with pytest.raises(AssertionError):
         _near(got, plain[:, t : t + tokens])
+
+
+@pytest.mark.gpu
+def test_a_step_that_fails_on_its_way(monkeypatch: pytest.MonkeyPatch) -> None:
+    """Up to 64 tokens nothing is lost; more may have taken the place of older ones in the
+    layers that came first, so that the sequences are forgotten."""
+    config = WorkloadConfig(2, 300, 128, 2, 256, 2)
+    model = _model(config)
+    x = _randn(2, 300, 128)
+    with torch.inference_mode():
+        want = model(x)
+    decoder = CachedDecoder(model, slots=2, max_tokens=300, weights="bf16", graph=False)
+    decoder.prompt(x[:, :60].contiguous())
+    attend, calls = cached_decode.sm100_kv8_attention, []
+
+    def failing(*args, **kwargs):  # noqa: ANN002, ANN003, ANN202
+        calls.append(args)
+        if len(calls) == 2:
+            raise RuntimeError("second layer")
+        return attend(*args, **kwargs)
+
+    for tokens in (40, 140):
+        calls.clear()
+        monkeypatch.setattr(cached_decode, "sm100_kv8_attention", failing)
+        with pytest.raises(RuntimeError, match="second layer"):
+            decoder.step(x[:, 60 : 60 + tokens].contiguous())
+        monkeypatch.setattr(cached_decode, "sm100_kv8_attention", attend)
+        if tokens == 40:
+            assert decoder.held == 60
+            _near(decoder.step(x[:, 60:61].contiguous(), advance=False), want[:, 60:61])
+    assert [decoder.held, decoder.pending, *decoder.cache.lengths.tolist()] == [0, 0, 0, 0]
+    _near(decoder.prompt(x[:, :30].contiguous()), want[:, :30])
+    _near(decoder.step(x[:, 30:31].contiguous()), want[:, 30:31])
