@@ -3,6 +3,8 @@ stream share one, a captured graph has its own."""
 
 from __future__ import annotations
 
+import threading
+
 import pytest
 import torch
 
@@ -124,3 +126,31 @@ def test_more_streams_than_workspaces() -> None:
         torch.cuda.synchronize()
         assert all(torch.equal(out, want) for out in outs)
         assert len(cache._workspaces) <= 8
+
+
+@pytest.mark.gpu
+def test_two_host_threads_on_one_cache() -> None:
+    """Each on a stream of its own."""
+    with torch.inference_mode():
+        cache = _filled(30000)
+        queries = [_randn(1, 1, 2, 64, seed=s).bfloat16() for s in range(2)]
+        want = [sm100_kv8_attention(cache, q)[0].clone() for q in queries]
+        torch.cuda.synchronize()
+    wrong: list[object] = []
+
+    def work(which: int) -> None:
+        try:
+            with torch.inference_mode(), torch.cuda.stream(torch.cuda.Stream()):
+                outs = [sm100_kv8_attention(cache, queries[which])[0] for _ in range(100)]
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(out, want[which]) for out in outs):
+                    wrong.append(which)
+        except Exception as exc:  # noqa: BLE001 - told by the assertion below
+            wrong.append(exc)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not wrong
