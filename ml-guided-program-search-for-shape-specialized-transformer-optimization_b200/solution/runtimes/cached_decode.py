@@ -119,6 +119,8 @@ class CachedDecoder:
                     {name: pack_w4(linear.weight, group) for name, linear in self._linears(layer)}
                     for layer in model.layers
                 ]
+        # what all graphs share, as steps follow one another: memory, and the stream of their captures
+        self._capture: tuple[object, torch.cuda.Stream] | None = None
         self._wide_weights: list[dict[str, torch.Tensor]] | None = None  # the packed ones' values in bf16
         self._replays: dict[tuple[object, ...], tuple[torch.Tensor, CudaGraphReplay]] = {}
 
@@ -284,7 +286,10 @@ class CachedDecoder:
             if self.graph and x.shape[1] <= _REPEATABLE:
                 key = (tuple(x.shape), x.dtype)
                 if key not in self._replays:
-                    self._replays[key] = (torch.empty_like(x), CudaGraphReplay())
+                    if self._capture is None:
+                        self._capture = (torch.cuda.graph_pool_handle(), torch.cuda.Stream(self.cache.device))
+                    pool, stream = self._capture
+                    self._replays[key] = (torch.empty_like(x), CudaGraphReplay(pool=pool, stream=stream))
                 buffer, replay = self._replays[key]
                 y = replay.run(self._program, buffer.copy_(x), None)
             else:

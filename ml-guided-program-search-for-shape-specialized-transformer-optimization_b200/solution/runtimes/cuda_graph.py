@@ -62,17 +62,22 @@ class _Binding:
 
 
 def capture_program(
-    program: Program, value: torch.Tensor, mask: torch.Tensor | None, pool: object
+    program: Program,
+    value: torch.Tensor,
+    mask: torch.Tensor | None,
+    pool: object,
+    stream: torch.cuda.Stream | None = None,
 ) -> tuple[torch.cuda.CUDAGraph, Callable[[torch.Tensor], torch.Tensor]]:
     """Capture ``program`` on ``value``/``mask`` in place; return the graph and
-    the deferred final launch.  One eager run on the capture stream first
+    the deferred final launch.  ``stream``: the one to capture on (a graph
+    reuses the pool's memory that was allocated on its stream).  One eager run on the capture stream first
     completes every lazy set-up of the launches (weight shadows, kernel
     attributes, the tensor-map encoder), none of which may happen inside a
     capture."""
 
     device = value.device
     current = torch.cuda.current_stream(device)
-    side = torch.cuda.Stream(device=device)
+    side = torch.cuda.Stream(device=device) if stream is None else stream
     side.wait_stream(current)
     with torch.cuda.stream(side), torch.inference_mode():
         program(value, mask)
@@ -86,7 +91,14 @@ def capture_program(
 class CudaGraphReplay:
     """Graph replays of one input signature, one capture per bound buffer."""
 
-    def __init__(self, *, reuse_unchanged_input: bool = False, max_bindings: int = 4) -> None:
+    def __init__(
+        self,
+        *,
+        reuse_unchanged_input: bool = False,
+        max_bindings: int = 4,
+        pool: object | None = None,
+        stream: torch.cuda.Stream | None = None,
+    ) -> None:
         # ``reuse_unchanged_input`` is the schedule knob of the reference's
         # staging copy; with the input bound in place no call copies it, so
         # the knob has nothing left to skip and is accepted as is.
@@ -96,7 +108,10 @@ class CudaGraphReplay:
         self.max_bindings = max_bindings
         self._bindings: OrderedDict[tuple[object, ...], _Binding] = OrderedDict()
         self._layout: tuple[object, ...] | None = None
-        self._pool: object | None = None
+        # ``pool`` and ``stream``: graphs of several objects that share memory, captured on one
+        # stream; their replays follow one another on one stream, too.
+        self._given_pool = self._pool = pool
+        self._stream = stream
 
     @property
     def captured(self) -> bool:
@@ -121,7 +136,7 @@ class CudaGraphReplay:
         if binding is None:
             if self._pool is None:
                 self._pool = torch.cuda.graph_pool_handle()
-            graph, finish = capture_program(program, value, mask, self._pool)
+            graph, finish = capture_program(program, value, mask, self._pool, self._stream)
             if len(self._bindings) >= self.max_bindings:
                 self._bindings.popitem(last=False)
             binding = _Binding(graph, finish, (value, mask))
@@ -137,7 +152,7 @@ class CudaGraphReplay:
 
         self._bindings.clear()
         self._layout = None
-        self._pool = None
+        self._pool = self._given_pool
 
 
 __all__ = ["CudaGraphReplay", "Program", "capture_program"]

@@ -174,3 +174,31 @@ def test_a_step_that_fails_on_its_way(monkeypatch: pytest.MonkeyPatch) -> None:
     assert [decoder.held, decoder.pending, *decoder.cache.lengths.tolist()] == [0, 0, 0, 0]
     _near(decoder.prompt(x[:, :30].contiguous()), want[:, :30])
     _near(decoder.step(x[:, 30:31].contiguous()), want[:, 30:31])
+
+
+@pytest.mark.gpu
+def test_graphs_of_many_shapes_share_their_memory() -> None:
+    """Steps of changing sizes in turn give what the whole forward gives, and another shape costs
+    no memory pool of its own (at least 20 MB, the allocator's segment)."""
+    config = WorkloadConfig(2, 300, 128, 2, 256, 2)
+    model = _model(config)
+    x = _randn(2, 300, 128)
+    with torch.inference_mode():
+        want = model(x)
+    decoder = CachedDecoder(model, slots=2, max_tokens=300, weights="bf16")
+    at = 0
+    for sizes in ((1, 2, 3), range(4, 16), (3, 15, 1, 2, 9, 1, 14, 4)):
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        before = torch.cuda.memory_reserved()
+        for tokens in sizes:
+            draft = x[:, at : at + tokens].contiguous()
+            _near(decoder.step(draft, advance=False), want[:, at : at + tokens])
+            keep = (tokens + 1) // 2
+            decoder.advance(keep)
+            at += keep
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        if len(sizes) == 12:
+            assert torch.cuda.memory_reserved() - before <= 60 << 20
+    assert len(decoder._replays) == 15
