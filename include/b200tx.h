@@ -520,6 +520,75 @@ int b200tx_linear_w4(const void* x, int64_t x_stride, const void* packed, const 
                      void* out, int out_dtype, int64_t M, int64_t N, int64_t K, int64_t group, int epilogue,
                      cudaStream_t stream);
 
+/*
+ * Low-rank adapters of many requests beside a shared projection:
+ * out[r] = epilogue(base[r] + scales[a] * (x[r] . down[a]^T) . up[a]^T), a = indices[r / (M / index_count)]
+ * the row's adapter; a < 0: none; a >= adapters: the row becomes NaN.  x BF16 [M, K]; base and
+ * out F32 or BF16 [M, N], out other memory than x's and base's, or base itself in one dtype;
+ * down BF16 [adapters, rank, K], up BF16 [adapters, N, rank], scales F32 [adapters];
+ * rank a multiple of 8 up to 128, K a multiple of 8; index_count divides M; all 16-byte aligned but
+ * scales and indices.  fp32 accumulation; epilogue B200TX_EPI_* (no bias: base holds it).
+ */
+int b200tx_low_rank_add(const void* x, const void* base, int base_dtype, void* out, int out_dtype, const void* down,
+                        const void* up, const float* scales, const int32_t* indices, int64_t index_count, int64_t M,
+                        int64_t N, int64_t K, int64_t rank, int64_t adapters, int epilogue, cudaStream_t stream);
+
+/* The pages of an 8-bit cache, all layers: layer 0's view (the layers of codes, scales and tail follow
+ * one another without gaps; page_table and lengths are written here), refs[page] = the entries of the page
+ * table that hold the page (0: it is free), and scratch, b200tx_kv8_pool_scratch ints, zeroed once.
+ * One call at a time works on a pool: calls, and replays of graphs that hold them, follow one
+ * another. */
+typedef struct b200tx_kv8_pool {
+  b200tx_kv8_cache cache;
+  int64_t layers;
+  int32_t* refs;    /* [pages] */
+  int32_t* scratch;
+} b200tx_kv8_pool;
+
+int b200tx_kv8_pool_scratch(int64_t pages, int64_t* ints_out);
+
+/*
+ * Slot target[i] becomes what slot source[i] was before the call, for all pairs (2048 at most) at once: it
+ * holds the same pages for the full blocks, a copy of the open block in its tail, and the length; its own
+ * pages are given up.  A source below 0, or source NULL: the slot becomes empty.  A pair with source ==
+ * target, with a target that is no slot or a source past the slots does nothing; of pairs
+ * with one target the last counts.
+ */
+int b200tx_kv8_fork(const b200tx_kv8_pool* pool, const int32_t* source, const int32_t* target, int64_t pairs,
+                    cudaStream_t stream);
+
+/*
+ * Pages for the blocks that the next tokens of each sequence may fill: counts[b] of them (tokens where counts
+ * is NULL, and at most) behind lengths[slot] for slot slot_ids[b] (b where NULL).  An entry without a page, or with one
+ * that another entry holds as well, takes the lowest free page, in the order of rows and blocks; without free pages it
+ * becomes -1 and counts in missing[b], as does a block past the table.  Of rows with one slot
+ * the first counts.  At most 2048 rows.
+ */
+int b200tx_kv8_reserve(const b200tx_kv8_pool* pool, const int32_t* slot_ids, const int32_t* counts, int64_t tokens,
+                       int64_t rows, int32_t* missing, cudaStream_t stream);
+
+/*
+ * Brings the pages in use to the front: with n of them, the k-th one from page n on moves to the k-th free page below n,
+ * codes and scales of all layers; the page table and refs follow (an entry whose page nothing counts becomes -1).
+ * used[0] = n.  What a page held that moved away stays behind in it.
+ */
+int b200tx_kv8_compact(const b200tx_kv8_pool* pool, int32_t* used, cudaStream_t stream);
+
+/*
+ * Verification of drafted tokens.  target [batch, tokens + 1, vocab] and draft [batch, tokens, vocab] (NULL: probability
+ * 1 at the drafted token) are probabilities in dtype, F32 or BF16, the vocabulary dense, strides in
+ * elements; drafted [batch, tokens] int32 or int64, uniform [batch, tokens + 1] in [0, 1), counts[b] (tokens where
+ * NULL) tokens of each sequence drafted.  Token t counts while uniform[t] * draft[t][d] < target[t][d]; accepted[b] = how
+ * many do, n.  out [batch, tokens + 1] in drafted's type: these n tokens, then one from max(target[n] - draft[n],
+ * 0), or from target[n] where all count or nothing is left: the first index whose running sum passes uniform[tokens]
+ * times the whole (the last index with mass where none does, -1 where there is no mass); then -1.  Sums in 64 bits;
+ * a mass that is NaN counts as none.  At most 1024 drafted tokens each.
+ */
+int b200tx_verify_draft(const void* target, int64_t target_batch_stride, int64_t target_token_stride, const void* draft,
+                        int64_t draft_batch_stride, int64_t draft_token_stride, int dtype, const void* drafted,
+                        int drafted_64, const float* uniform, const int32_t* counts, int64_t batch, int64_t tokens,
+                        int64_t vocab, void* out, int32_t* accepted, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -35,6 +35,8 @@ NVCC_FLAGS = (
     "-Xcompiler",
     "-fPIC",
     "-shared",
+    "--split-compile",
+    "0",  # the kernels by as many threads as there are
 )
 
 

@@ -29,11 +29,14 @@
 #include "gemm_warp_kernels.cuh"
 #include "kv8_attention_kernels.cuh"
 #include "kv8_cache_kernels.cuh"
+#include "kv8_pages_kernels.cuh"
 #include "linear_w4_kernels.cuh"
+#include "low_rank_kernels.cuh"
 #include "norm_kernels.cuh"
 #include "rope_kernels.cuh"
 #include "seq_forward_kernels.cuh"
 #include "sm100_common.cuh"
+#include "verify_kernels.cuh"
 
 // Weight images of b200tx_sequence_forward_noalloc, the library's only fixed
 // scratch array: B200TX_SEQ_NOALLOC_MAX_LAYERS layers x 6 images x 32 KB =
@@ -86,6 +89,8 @@ struct DeviceState {
   bool kv8_attr[9] = {};                   // 8-bit cache attention builds by head_dim and row groups
   bool w4_attr[18] = {};                   // 4-bit linear builds by row tiles, column tiles and group
   bool w4_line_attr[6] = {};               // the same with x in shared memory, by row tiles and group
+  bool low_rank_attr[16] = {};             // low-rank adapter builds by rank, rows and base dtype
+  bool fork_attr = false, reserve_attr = false;
   bool seq_forward_attr = false;           // whole-forward kernel's shared-memory size set
   uint8_t* seq_noalloc_images = nullptr;   // device address of g_seq_noalloc_images on this device
 };
@@ -1471,3 +1476,4 @@ int b200tx_attention(const void* qkv, void* out, int64_t batch, int64_t seq, int
 }  // extern "C"
 
 #include "decode_api.cuh"
+#include "request_api.cuh"

@@ -35,6 +35,11 @@ struct Entry {
   decltype(&b200tx_kv8_gather) kv8_gather;
   decltype(&b200tx_kv8_attention) kv8_attention;
   decltype(&b200tx_linear_w4) linear_w4;
+  decltype(&b200tx_low_rank_add) low_rank_add;
+  decltype(&b200tx_kv8_fork) kv8_fork;
+  decltype(&b200tx_kv8_reserve) kv8_reserve;
+  decltype(&b200tx_kv8_compact) kv8_compact;
+  decltype(&b200tx_verify_draft) verify_draft;
 } entry = {};
 
 struct Refusal {
@@ -222,6 +227,11 @@ PyObject* init(PyObject*, PyObject* const* args, Py_ssize_t n) {
     take("b200tx_kv8_gather", entry.kv8_gather);
     take("b200tx_kv8_attention", entry.kv8_attention);
     take("b200tx_linear_w4", entry.linear_w4);
+    take("b200tx_low_rank_add", entry.low_rank_add);
+    take("b200tx_kv8_fork", entry.kv8_fork);
+    take("b200tx_kv8_reserve", entry.kv8_reserve);
+    take("b200tx_kv8_compact", entry.kv8_compact);
+    take("b200tx_verify_draft", entry.verify_draft);
     Py_RETURN_NONE;
   });
 }
@@ -465,6 +475,166 @@ PyObject* linear_w4(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
+bool low_rank_fits(const at::Tensor* x, const at::Tensor* base, const at::Tensor* down, const at::Tensor* up) {
+  if (!ready(x) || base == nullptr || down == nullptr || up == nullptr || x->scalar_type() != at::kBFloat16 || x->dim() < 1 ||
+      x->numel() == 0 || !x->is_contiguous() || !aligned(*x) || base->dim() != x->dim() || down->device() != x->device() ||
+      base->device() != x->device() || !base->is_contiguous() || !aligned(*base) ||
+      (base->scalar_type() != at::kBFloat16 && base->scalar_type() != at::kFloat))
+    return false;
+  const int64_t last = x->dim() - 1;
+  return x->sizes().slice(0, last) == base->sizes().slice(0, last) && x->size(last) == down->size(2) &&
+         base->size(last) == up->size(1);
+}
+
+PyObject* low_rank_add_ok(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded(n, 4, [&]() -> PyObject* {
+    return PyBool_FromLong(low_rank_fits(tensor(args[0]), tensor(args[1]), tensor(args[2]), tensor(args[3])));
+  });
+}
+
+// low_rank_add(x, base, down, up, scales, indices, gelu, out_f32 or None, out) -> out
+PyObject* low_rank_add(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded(n, 9, [&]() -> PyObject* {
+    const at::Tensor *x = tensor(args[0]), *base = tensor(args[1]), *down = tensor(args[2]), *up = tensor(args[3]);
+    if (!low_rank_fits(x, base, down, up)) ineligible("sm100 low-rank adapters are ineligible for the requested operands");
+    const at::Tensor* scales = tensor(args[4]);
+    require(scales != nullptr, "adapters must be a LowRankAdapters");
+    const at::Tensor* indices = tensor(args[5]);
+    const int64_t rows = x->numel() / x->size(-1);
+    require(indices != nullptr && indices->scalar_type() == at::kInt && indices->is_contiguous() &&
+                indices->device() == x->device() && indices->numel() > 0 && rows % indices->numel() == 0,
+            "indices must be a contiguous int32 tensor on the input's device whose size divides the rows");
+    const bool f32 = args[7] == Py_None ? base->scalar_type() == at::kFloat : integer(args[7]) != 0;
+    const at::ScalarType type = f32 ? at::kFloat : at::kBFloat16;
+    at::Tensor out = result(args[8], base->sizes(), type, *x, "out has the wrong shape, dtype, device or layout");
+    require(args[8] == Py_None || apart(out, *base) || (out.const_data_ptr() == base->const_data_ptr() && type == base->scalar_type()),
+            "out shares memory with base without being it");
+    launched(entry.low_rank_add(x->const_data_ptr(), base->const_data_ptr(), dtype(*base), out.data_ptr(),
+                                f32 ? B200TX_F32 : B200TX_BF16, down->const_data_ptr(), up->const_data_ptr(),
+                                scales->const_data_ptr<float>(), indices->const_data_ptr<int32_t>(), indices->numel(), rows,
+                                base->size(-1), x->size(-1), down->size(1), down->size(0),
+                                integer(args[6]) != 0 ? B200TX_EPI_BIAS_GELU : B200TX_EPI_BIAS, stream_of(*x)),
+             "b200tx_low_rank_add");
+    return THPVariable_Wrap(out);
+  });
+}
+
+// A pool of pages: (address of b200tx_kv8_pool, its refs).
+struct Pool {
+  const b200tx_kv8_pool* view;
+  const at::Tensor* refs;
+};
+
+Pool pool_of(PyObject* o) {
+  require(PyTuple_Check(o) && PyTuple_GET_SIZE(o) == 2, "pages must be a Kv8Pages");
+  const Pool pool = {address<const b200tx_kv8_pool>(PyTuple_GET_ITEM(o, 0)), tensor(PyTuple_GET_ITEM(o, 1))};
+  require(pool.refs != nullptr, "pages must be a Kv8Pages");
+  if (!pool.refs->is_cuda()) ineligible("the pages of a cache are moved on an sm_100 CUDA device; there is no CPU fallback");
+  return pool;
+}
+
+const int32_t* slot_list(PyObject* o, const at::Tensor& like, int64_t* size, const char* text) {
+  const at::Tensor* t = tensor(o);
+  require(t != nullptr && t->scalar_type() == at::kInt && t->dim() == 1 && t->is_contiguous() && t->device() == like.device(), text);
+  *size = t->size(0);
+  return t->const_data_ptr<int32_t>();
+}
+
+// kv8_fork(pool, source or None, target)
+PyObject* kv8_fork(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded(n, 3, [&]() -> PyObject* {
+    const Pool pool = pool_of(args[0]);
+    int64_t pairs = 0, sources = 0;
+    const int32_t* target = slot_list(args[2], *pool.refs, &pairs, "target must be a contiguous int32 [n] tensor on the cache's device");
+    const int32_t* source = nullptr;
+    if (args[1] != Py_None) {
+      source = slot_list(args[1], *pool.refs, &sources, "source must be a contiguous int32 [n] tensor on the cache's device");
+      require(sources == pairs, "source and target differ in size");
+    }
+    require(pairs <= 2048, "at most 2048 sequences at once");
+    launched(entry.kv8_fork(pool.view, source, target, pairs, stream_of(*pool.refs)), "b200tx_kv8_fork");
+    Py_RETURN_NONE;
+  });
+}
+
+// kv8_reserve(pool, tokens, slots, counts) -> missing
+PyObject* kv8_reserve(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded(n, 4, [&]() -> PyObject* {
+    const Pool pool = pool_of(args[0]);
+    const int64_t tokens = integer(args[1]);
+    require(tokens >= 0, "tokens must not be negative");
+    int64_t rows = pool.view->cache.slots;
+    const int32_t* slots = nullptr;
+    if (args[2] != Py_None) {
+      slots = slot_list(args[2], *pool.refs, &rows, kSlots);
+    } else if (args[3] != Py_None) {
+      slot_list(args[3], *pool.refs, &rows, kCounts);
+      require(rows <= pool.view->cache.slots, kBatch);
+    }
+    const int32_t* counts = per_sequence(args[3], rows, *pool.refs, kCounts);
+    require(rows > 0 && rows <= 2048, "1 to 2048 sequences at once");
+    at::Tensor missing = at::empty({rows}, at::TensorOptions().dtype(at::kInt).device(pool.refs->device()));
+    launched(entry.kv8_reserve(pool.view, slots, counts, tokens, rows, missing.data_ptr<int32_t>(), stream_of(*pool.refs)),
+             "b200tx_kv8_reserve");
+    return THPVariable_Wrap(missing);
+  });
+}
+
+// kv8_compact(pool) -> used
+PyObject* kv8_compact(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded(n, 1, [&]() -> PyObject* {
+    const Pool pool = pool_of(args[0]);
+    at::Tensor used = at::empty({1}, at::TensorOptions().dtype(at::kInt).device(pool.refs->device()));
+    launched(entry.kv8_compact(pool.view, used.data_ptr<int32_t>(), stream_of(*pool.refs)), "b200tx_kv8_compact");
+    return THPVariable_Wrap(used);
+  });
+}
+
+bool probabilities_fit(const at::Tensor* t, int64_t batch, int64_t tokens) {
+  return t != nullptr && t->dim() == 3 && t->size(0) == batch && t->size(1) == tokens && t->size(2) > 0 &&
+         (t->stride(2) == 1 || t->size(2) == 1) && (t->scalar_type() == at::kFloat || t->scalar_type() == at::kBFloat16);
+}
+
+bool verify_fits(const at::Tensor* target, const at::Tensor* drafted) {
+  return target != nullptr && drafted != nullptr && target->is_cuda() && drafted->device() == target->device() &&
+         drafted->dim() == 2 && drafted->size(0) > 0 && drafted->is_contiguous() &&
+         (drafted->scalar_type() == at::kInt || drafted->scalar_type() == at::kLong) &&
+         probabilities_fit(target, drafted->size(0), drafted->size(1) + 1);
+}
+
+PyObject* verify_draft_ok(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded(n, 2, [&]() -> PyObject* { return PyBool_FromLong(verify_fits(tensor(args[0]), tensor(args[1]))); });
+}
+
+// verify_draft(target, drafted, uniform, draft, counts) -> (tokens, accepted)
+PyObject* verify_draft(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded(n, 5, [&]() -> PyObject* {
+    const at::Tensor *target = tensor(args[0]), *drafted = tensor(args[1]), *uniform = tensor(args[2]);
+    if (!verify_fits(target, drafted)) ineligible("sm100 draft verification is ineligible for the requested inputs");
+    const int64_t batch = drafted->size(0), tokens = drafted->size(1);
+    require(uniform != nullptr && uniform->scalar_type() == at::kFloat && uniform->is_contiguous() && uniform->dim() == 2 &&
+                uniform->size(0) == batch && uniform->size(1) == tokens + 1 && uniform->device() == target->device(),
+            "uniform must be a contiguous float32 [B, T + 1] tensor on the input's device");
+    static const char* text = "draft must be a [B, T, V] tensor of the target's dtype, device and vocabulary";
+    const at::Tensor* draft = optional(args[3], text);
+    require(draft == nullptr || (probabilities_fit(draft, batch, tokens) && draft->size(2) == target->size(2) &&
+                                 draft->scalar_type() == target->scalar_type() && draft->device() == target->device()), text);
+    const int32_t* counts =
+        per_sequence(args[4], batch, *target, "counts must be a contiguous int32 [B] tensor on the input's device");
+    at::Tensor out = at::empty({batch, tokens + 1}, drafted->options());
+    at::Tensor accepted = at::empty({batch}, at::TensorOptions().dtype(at::kInt).device(target->device()));
+    const bool given = draft != nullptr && tokens > 0;
+    launched(entry.verify_draft(target->const_data_ptr(), target->stride(0), target->stride(1),
+                                given ? draft->const_data_ptr() : nullptr, given ? draft->stride(0) : 0,
+                                given ? draft->stride(1) : 0, dtype(*target), drafted->const_data_ptr(),
+                                drafted->scalar_type() == at::kLong, uniform->const_data_ptr<float>(), counts, batch, tokens,
+                                target->size(2), out.data_ptr(), accepted.data_ptr<int32_t>(), stream_of(*target)),
+             "b200tx_verify_draft");
+    const Owned first(THPVariable_Wrap(out)), second(THPVariable_Wrap(accepted));
+    return PyTuple_Pack(2, first.o, second.o);
+  });
+}
+
 #define B200TX_METHOD(name) \
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 
@@ -479,6 +649,13 @@ PyMethodDef methods[] = {
     B200TX_METHOD(kv8_attention),
     B200TX_METHOD(linear_w4_ok),
     B200TX_METHOD(linear_w4),
+    B200TX_METHOD(low_rank_add_ok),
+    B200TX_METHOD(low_rank_add),
+    B200TX_METHOD(kv8_fork),
+    B200TX_METHOD(kv8_reserve),
+    B200TX_METHOD(kv8_compact),
+    B200TX_METHOD(verify_draft_ok),
+    B200TX_METHOD(verify_draft),
     {nullptr, nullptr, 0, nullptr},
 };
 

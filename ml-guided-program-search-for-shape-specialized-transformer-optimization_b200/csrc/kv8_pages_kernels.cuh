@@ -1,0 +1,518 @@
+// kv8_pages_kernels.cuh -- moving sequences and pages of the 8-bit cache about:
+// sequences that share pages (fork, free), pages for the tokens to come
+// (reserve), and pages in use brought together (compact).
+//
+// refs[page] counts the page table's entries that hold the page; a page with none is
+// free.  A full block is never written again, so sequences with a common
+// beginning hold the same pages for it, and a fork copies no codes: only the open block's
+// rows, which lie in the sequence's own tail.
+//
+// All is decided on the device, from lengths and tables as they are there: nothing is read
+// back, and the calls go into a captured graph.  Every result is a function of the state
+// before the call: pages are given out lowest first, in the order of rows and blocks, and
+// counts are integers, so the order in which CTAs run changes nothing.  One call at a time
+// works on a cache's pages.
+#pragma once
+
+#include "kv8_cache_kernels.cuh"
+
+namespace b200tx {
+
+struct Kv8Pool {
+  uint8_t* codes;       // [layers, pages, 2, kv_heads, 64, D]
+  float* scales;        // [layers, pages, 2, kv_heads]
+  uint4* tail;          // [layers, slots, 2 (block parity), 2, kv_heads, 64, D] bf16
+  int32_t* page_table;  // [slots, max_blocks]
+  int32_t* lengths;     // [slots]
+  int32_t* refs;        // [pages]
+  int32_t* scratch;     // counters (kPoolCounters), then two lists of pages
+  int64_t pages;
+  int slots, max_blocks, kv_heads, dim, layers;
+};
+
+constexpr int kPoolCounters = 64;  // [0] arrivals of a fork's CTAs, [1] moves, [2] pages in use
+constexpr int kPoolRows = 2048;    // sequences of a call
+
+// ------------------------------------------------------------------ which rows count
+// Of rows that name the same slot one counts: the last (fork) or the first (reserve).  A table of
+// twice as many places, in shared memory: the slot, and the row that counts.
+struct SlotOwners {
+  int* slots;
+  int* rows;
+  int mask;
+
+  __device__ __forceinline__ int place(int slot) const {
+    int at = static_cast<int>((static_cast<uint32_t>(slot) * 2654435761u) >> 8) & mask;
+    while (true) {
+      const int found = atomicCAS(slots + at, -1, slot);
+      if (found == -1 || found == slot) return at;
+      at = (at + 1) & mask;
+    }
+  }
+};
+
+// ------------------------------------------------------------------ fork and free
+constexpr int kForkThreads = 256;
+constexpr int kForkHeld = 8;                                 // 16-byte pieces a thread holds
+constexpr int kForkPieces = kForkThreads * kForkHeld;        // of all pairs of an item
+static_assert(kForkPieces >= kPoolRows, "an item holds a piece of every pair");
+
+struct Kv8ForkArgs {
+  Kv8Pool pool;
+  const int32_t* source;  // [pairs], or null: from nothing
+  const int32_t* target;  // [pairs]
+  int pairs;
+  int owners;             // places of the table of slots, a power of two
+  int piece_shift;        // log2 of the pieces of a pair in a tail item
+  int column_shift;       // log2 of the columns in a table item
+  int tail_items, table_items;
+};
+
+struct ForkPair {
+  int source, target;  // target -1: the pair does nothing; source -1: from nothing
+  int full;            // full blocks of the source
+  int open;            // rows of its open block, or'ed with 64 times the block's parity
+};
+
+// All pairs at once: every target becomes what its source was before the call.  An item is
+// a place in the tails (or some columns of the table) for all pairs: its values
+// are read for every pair before any is written, so a slot may be the source of one pair and the
+// target of another (beams that are put in a new order).
+__global__ void __launch_bounds__(kForkThreads, 3) kv8_fork_kernel(const __grid_constant__ Kv8ForkArgs a) {
+  extern __shared__ __align__(16) uint8_t fork_smem[];
+  __shared__ int s_last;
+  ForkPair* const pair = reinterpret_cast<ForkPair*>(fork_smem);
+  SlotOwners owners;
+  owners.slots = reinterpret_cast<int*>(pair + a.pairs);
+  owners.rows = owners.slots + a.owners;
+  owners.mask = a.owners - 1;
+  const Kv8Pool& p = a.pool;
+  const int tid = threadIdx.x;
+  griddep_wait();
+  griddep_launch_dependents();
+
+  for (int i = tid; i < a.owners; i += kForkThreads) owners.slots[i] = owners.rows[i] = -1;
+  __syncthreads();
+  for (int i = tid; i < a.pairs; i += kForkThreads) {
+    const int target = a.target[i];
+    if (target >= 0 && target < p.slots) atomicMax(owners.rows + owners.place(target), i);
+  }
+  __syncthreads();
+  for (int i = tid; i < a.pairs; i += kForkThreads) {
+    ForkPair f;
+    f.source = a.source == nullptr ? -1 : a.source[i];
+    f.target = a.target[i];
+    f.full = f.open = 0;
+    const bool known = f.target >= 0 && f.target < p.slots && f.source < p.slots;
+    // a sequence that becomes itself stays as it is, with the pages that are reserved for it
+    if (!known || f.source == f.target || owners.rows[owners.place(f.target)] != i) {
+      f.target = -1;
+    } else if (f.source >= 0) {
+      const int held = max(0, p.lengths[f.source]), block = held / kKv8Block;
+      f.full = min(block, p.max_blocks);
+      f.open = held % kKv8Block | (block & 1) * kKv8Block;
+    } else {
+      f.source = -1;
+    }
+    pair[i] = f;
+  }
+  __syncthreads();
+
+  const int row = p.dim / 8;                 // 16-byte pieces of a token's head
+  const int region = kKv8Block * row;        // of a head's block
+  const int each = 1 << a.piece_shift, pieces = region >> a.piece_shift;
+  for (int item = blockIdx.x; item < a.tail_items + a.table_items; item += gridDim.x) {
+    if (item < a.tail_items) {
+      const int part = item % pieces, rest = item / pieces;
+      const int heads = 2 * p.kv_heads, head = rest % heads, layer = rest / heads;
+      uint4 v[kForkHeld];
+      uint4* to[kForkHeld];
+#pragma unroll
+      for (int j = 0; j < kForkHeld; ++j) {
+        const int e = j * kForkThreads + tid, i = e >> a.piece_shift, at = part * each + (e & (each - 1));
+        to[j] = nullptr;
+        if (i >= a.pairs) continue;
+        const ForkPair f = pair[i];
+        if (f.target < 0 || at >= (f.open & (kKv8Block - 1)) * row) continue;
+        const int64_t inside = (static_cast<int64_t>(f.open / kKv8Block) * heads + head) * region + at;
+        const int64_t slot = static_cast<int64_t>(2) * heads * region, first = static_cast<int64_t>(layer) * p.slots;
+        v[j] = p.tail[(first + f.source) * slot + inside];
+        to[j] = p.tail + (first + f.target) * slot + inside;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kForkHeld; ++j)
+        if (to[j] != nullptr) *to[j] = v[j];
+    } else {
+      const int columns = 1 << a.column_shift, from = (item - a.tail_items) << a.column_shift;
+      int page[kForkHeld];
+#pragma unroll
+      for (int j = 0; j < kForkHeld; ++j) {
+        const int e = j * kForkThreads + tid, i = e >> a.column_shift, block = from + (e & (columns - 1));
+        page[j] = -1;
+        if (i >= a.pairs || block >= p.max_blocks) continue;
+        const ForkPair f = pair[i];
+        if (f.target < 0 || f.source < 0 || block >= f.full) continue;
+        const int found = p.page_table[static_cast<int64_t>(f.source) * p.max_blocks + block];
+        if (found >= 0 && found < p.pages) page[j] = found;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kForkHeld; ++j) {
+        const int e = j * kForkThreads + tid, i = e >> a.column_shift, block = from + (e & (columns - 1));
+        if (i >= a.pairs || block >= p.max_blocks || pair[i].target < 0) continue;
+        int32_t* const entry = p.page_table + static_cast<int64_t>(pair[i].target) * p.max_blocks + block;
+        const int before = *entry;
+        if (before == page[j]) continue;
+        if (before >= 0 && before < p.pages) atomicSub(p.refs + before, 1);
+        if (page[j] >= 0) atomicAdd(p.refs + page[j], 1);
+        *entry = page[j];
+      }
+    }
+  }
+
+  // The lengths change when every CTA has read them: the last to arrive writes them.
+  __syncthreads();
+  if (tid == 0) {
+    __threadfence();
+    s_last = atomicInc(reinterpret_cast<unsigned int*>(p.scratch), gridDim.x - 1) == gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  for (int i = tid; i < a.pairs; i += kForkThreads) owners.rows[i] = pair[i].target >= 0 && pair[i].source >= 0 ? max(0, p.lengths[pair[i].source]) : 0;
+  __syncthreads();
+  for (int i = tid; i < a.pairs; i += kForkThreads)
+    if (pair[i].target >= 0) p.lengths[pair[i].target] = owners.rows[i];
+}
+
+// ------------------------------------------------------------------ order over a cluster
+// One cluster of CTAs does what needs an order over all pages or entries: each
+// CTA takes a stretch, and the stretches' counts go round through distributed shared memory.
+constexpr int kPoolCtas = 8;
+constexpr int kPoolThreads = 1024;
+constexpr int kPoolWarps = kPoolThreads / 32;
+constexpr int kPoolAllWarps = kPoolCtas * kPoolWarps;
+
+struct PoolShared {
+  int warp[kPoolWarps];
+  int cta[2][2][kPoolCtas];  // [exchange's parity][which count][CTA]
+};
+
+// The counts of two kinds that the warps before this one hold, and of all, over the cluster.  All
+// threads call it; the counts are a warp's (the same in its lanes).
+__device__ __forceinline__ void pool_order(PoolShared& s, int& turn, const int (&count)[2], int (&before)[2], int (&all)[2]) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, me = static_cast<int>(cluster_ctarank());
+  const int parity = turn++ & 1;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    __syncthreads();
+    if (lane == 0) s.warp[warp] = count[k];
+    __syncthreads();
+    int mine = s.warp[lane];
+    int sum = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int o = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += o;
+    }
+    before[k] = __shfl_sync(0xffffffffu, sum - mine, warp);
+    const int total = __shfl_sync(0xffffffffu, sum, 31);
+    if (warp == 0 && lane < kPoolCtas)
+      asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(peer_smem_addr(&s.cta[parity][k][me], lane)), "r"(total) : "memory");
+  }
+  cluster_sync();
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    all[k] = 0;
+#pragma unroll
+    for (int i = 0; i < kPoolCtas; ++i) {
+      if (i < me) before[k] += s.cta[parity][k][i];
+      all[k] += s.cta[parity][k][i];
+    }
+  }
+}
+
+// Calls f(page, refs) for this warp's stretch of the pages, 32 neighbouring pages at a time (all lanes
+// call; past the end refs is -1).
+template <typename F>
+__device__ __forceinline__ void pool_pages(const Kv8Pool& p, F f) {
+  const int64_t each = ((p.pages + 31) / 32 + kPoolAllWarps - 1) / kPoolAllWarps * 32;
+  const int64_t from = each * (cluster_ctarank() * kPoolWarps + threadIdx.x / 32);
+  constexpr int U = 8;
+  for (int64_t at = from; at < min(from + each, p.pages); at += U * 32) {
+    int refs[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t page = at + u * 32 + threadIdx.x % 32;
+      refs[u] = page < p.pages && at + u * 32 < from + each ? max(0, __ldcg(p.refs + page)) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (at + u * 32 < min(from + each, p.pages)) f(static_cast<int>(at + u * 32 + threadIdx.x % 32), refs[u]);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ reserve
+struct Kv8ReserveArgs {
+  Kv8Pool pool;
+  const int32_t* slot_ids;  // [rows] or null = identity
+  const int32_t* counts;    // [rows] tokens, or null = tokens
+  int32_t* missing;         // [rows]
+  int tokens, rows;
+  int owners;
+};
+
+// The blocks that the next tokens may fill get pages of their own: an entry without a page, or with one
+// that another entry holds too, takes the lowest free page.  Entries are in the order
+// of rows and blocks; the pages that all entries give back are free for all.
+__global__ void __launch_bounds__(kPoolThreads, 1) kv8_reserve_kernel(const __grid_constant__ Kv8ReserveArgs a) {
+  extern __shared__ __align__(16) uint8_t reserve_smem[];
+  __shared__ PoolShared s;
+  int* const slot_of = reinterpret_cast<int*>(reserve_smem);  // [rows]
+  int* const begin = slot_of + a.rows;                        // [rows] first block
+  int* const upto = begin + a.rows;                           // [rows] entries of the rows up to this one
+  SlotOwners owners;
+  owners.slots = upto + a.rows;
+  owners.rows = owners.slots + a.owners;
+  owners.mask = a.owners - 1;
+  const Kv8Pool& p = a.pool;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, me = static_cast<int>(cluster_ctarank());
+  int turn = 0;
+  cluster_sync();
+  griddep_wait();
+  griddep_launch_dependents();
+
+  for (int i = tid; i < a.owners; i += kPoolThreads) {
+    owners.slots[i] = -1;
+    owners.rows[i] = kPoolRows;
+  }
+  __syncthreads();
+  for (int b = tid; b < a.rows; b += kPoolThreads) {
+    const int slot = a.slot_ids == nullptr ? b : a.slot_ids[b];
+    slot_of[b] = slot;
+    if (slot >= 0 && slot < p.slots) atomicMin(owners.rows + owners.place(slot), b);
+  }
+  __syncthreads();
+  int running = 0;
+  for (int base = 0; base < a.rows; base += kPoolThreads) {
+    const int b = base + tid;
+    int entries = 0;
+    if (b < a.rows) {
+      const int slot = slot_of[b];
+      int past = 0;
+      if (slot >= 0 && slot < p.slots && owners.rows[owners.place(slot)] == b) {
+        const int64_t held = max(0, p.lengths[slot]), n = a.counts == nullptr ? a.tokens : min(max(a.counts[b], 0), a.tokens);
+        const int64_t from = held / kKv8Block, to = (held + n) / kKv8Block;
+        begin[b] = static_cast<int>(from);
+        entries = static_cast<int>(max(static_cast<int64_t>(0), min(to, static_cast<int64_t>(p.max_blocks)) - from));
+        past = static_cast<int>(to - from) - entries;
+      }
+      if (me == 0) a.missing[b] = past;  // blocks that the table has no place for
+    }
+    // entries up to and with this row
+    int sum = entries;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int o = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += o;
+    }
+    __syncthreads();
+    if (lane == 31) s.warp[warp] = sum;
+    __syncthreads();
+    int total = s.warp[lane];
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int o = __shfl_up_sync(0xffffffffu, total, d);
+      if (lane >= d) total += o;
+    }
+    const int warps_before = warp == 0 ? 0 : __shfl_sync(0xffffffffu, total, max(warp - 1, 0));
+    if (b < a.rows) upto[b] = running + warps_before + sum;
+    running += __shfl_sync(0xffffffffu, total, 31);
+  }
+  __syncthreads();
+  const int all_entries = running;
+
+  // this warp's stretch of the entries, 32 neighbours at a time
+  const int each = ((all_entries + 31) / 32 + kPoolAllWarps - 1) / kPoolAllWarps * 32;
+  const int first = each * (me * kPoolWarps + warp), last = min(first + each, all_entries);
+  auto row_of = [&](int entry) {
+    int lo = 0, hi = a.rows - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (upto[mid] > entry) hi = mid;
+      else lo = mid + 1;
+    }
+    return lo;
+  };
+  auto entry_of = [&](int entry, int row) {
+    const int in_row = entry - (row == 0 ? 0 : upto[row - 1]);
+    return p.page_table + static_cast<int64_t>(slot_of[row]) * p.max_blocks + begin[row] + in_row;
+  };
+  // A page that another entry holds too: the entry is marked with it, and given back when all are marked.
+  int wanted = 0;
+  for (int at = first; at < last; at += 32) {
+    const int e = at + lane;
+    bool want = false;
+    if (e < last) {
+      int32_t* const entry = entry_of(e, row_of(e));
+      const int page = *entry;
+      if (page < 0 || page >= p.pages) {
+        want = true;
+        *entry = -1;
+      } else if (p.refs[page] > 1) {
+        want = true;
+        *entry = -2 - page;
+      }
+    }
+    wanted += __popc(__ballot_sync(0xffffffffu, want));
+  }
+  int before[2], all[2];
+  pool_order(s, turn, {wanted, 0}, before, all);
+  if (all[0] == 0) return;
+  for (int at = first; at < last; at += 32) {
+    const int e = at + lane;
+    if (e < last) {
+      const int page = *entry_of(e, row_of(e));
+      if (page <= -2) atomicSub(p.refs + (-2 - page), 1);
+    }
+  }
+  cluster_sync();
+
+  int free_pages = 0;
+  pool_pages(p, [&](int, int refs) { free_pages += __popc(__ballot_sync(0xffffffffu, refs == 0)); });
+  int free_before[2], free_all[2];
+  pool_order(s, turn, {free_pages, 0}, free_before, free_all);
+  int32_t* const list = p.scratch + kPoolCounters;
+  int at_free = free_before[0];
+  pool_pages(p, [&](int page, int refs) {
+    const uint32_t bits = __ballot_sync(0xffffffffu, refs == 0);
+    const int k = at_free + __popc(bits & ((1u << lane) - 1));
+    if (refs == 0 && k < all[0]) list[k] = page;
+    at_free += __popc(bits);
+  });
+  cluster_sync();
+  int at_want = before[0];
+  for (int at = first; at < last; at += 32) {
+    const int e = at + lane;
+    int row = 0;
+    int32_t* entry = nullptr;
+    if (e < last) {
+      row = row_of(e);
+      entry = entry_of(e, row);
+      if (*entry >= 0) entry = nullptr;
+    }
+    const uint32_t bits = __ballot_sync(0xffffffffu, entry != nullptr);
+    if (entry != nullptr) {
+      const int k = at_want + __popc(bits & ((1u << lane) - 1));
+      if (k < free_all[0]) {
+        const int page = __ldcg(list + k);
+        *entry = page;
+        p.refs[page] = 1;
+      } else {
+        *entry = -1;
+        atomicAdd(a.missing + row, 1);
+      }
+    }
+    at_want += __popc(bits);
+  }
+}
+
+// ------------------------------------------------------------------ compact
+struct Kv8CompactArgs {
+  Kv8Pool pool;
+  int32_t* used;  // [1]
+  int64_t page_bytes;
+  int piece;      // bytes of a page that a CTA copies at a time
+  int pieces;     // of a page
+};
+
+// With n pages in use: the k-th page in use from n on goes to the k-th free one below n.
+// scratch: the number of moves and of pages in use; where[page], -1 for a free page; the pages that move.
+__global__ void __launch_bounds__(kPoolThreads, 1) kv8_compact_plan_kernel(const __grid_constant__ Kv8CompactArgs a) {
+  __shared__ PoolShared s;
+  const Kv8Pool& p = a.pool;
+  const int lane = threadIdx.x % 32;
+  const uint32_t below = (1u << lane) - 1;
+  int32_t* const where = p.scratch + kPoolCounters;
+  int32_t* const list = where + p.pages;  // holes from the front, movers from the back: not more than the pages
+  int turn = 0;
+  cluster_sync();
+  griddep_wait();
+  griddep_launch_dependents();
+  int held = 0;
+  pool_pages(p, [&](int, int refs) { held += __popc(__ballot_sync(0xffffffffu, refs > 0)); });
+  int before[2], all[2];
+  pool_order(s, turn, {held, 0}, before, all);
+  const int used = all[0];
+  int holes = 0, movers = 0;
+  pool_pages(p, [&](int page, int refs) {
+    holes += __popc(__ballot_sync(0xffffffffu, refs == 0 && page < used));
+    movers += __popc(__ballot_sync(0xffffffffu, refs > 0 && page >= used));
+  });
+  pool_order(s, turn, {holes, movers}, before, all);
+  int hole = before[0], mover = before[1];
+  pool_pages(p, [&](int page, int refs) {
+    const uint32_t to = __ballot_sync(0xffffffffu, refs == 0 && page < used);
+    const uint32_t of = __ballot_sync(0xffffffffu, refs > 0 && page >= used);
+    if (refs == 0 && page < used) list[hole + __popc(to & below)] = page;
+    if (refs > 0 && page >= used) list[p.pages - 1 - (mover + __popc(of & below))] = page;
+    if (refs >= 0) where[page] = refs > 0 && page < used ? page : -1;
+    hole += __popc(to);
+    mover += __popc(of);
+  });
+  cluster_sync();
+  const int moves = all[1];
+  for (int k = static_cast<int>(cluster_ctarank()) * kPoolThreads + threadIdx.x; k < moves; k += kPoolCtas * kPoolThreads) {
+    const int to = __ldcg(list + k), of = __ldcg(list + p.pages - 1 - k);
+    where[of] = to;
+    p.refs[to] = __ldcg(p.refs + of);
+    p.refs[of] = 0;
+  }
+  if (cluster_ctarank() == 0 && threadIdx.x == 0) {
+    p.scratch[1] = moves;
+    *a.used = used;
+  }
+}
+
+constexpr int kCompactThreads = 256;
+constexpr int kCompactHeld = 8;
+
+__global__ void __launch_bounds__(kCompactThreads) kv8_compact_move_kernel(const __grid_constant__ Kv8CompactArgs a) {
+  const Kv8Pool& p = a.pool;
+  const int tid = threadIdx.x;
+  griddep_wait();
+  griddep_launch_dependents();
+  const int32_t* const where = p.scratch + kPoolCounters;
+  const int32_t* const list = where + p.pages;
+  const int64_t moves = p.scratch[1], items = moves * p.layers * a.pieces;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int piece = static_cast<int>(item % a.pieces);
+    const int64_t rest = item / a.pieces;
+    const int layer = static_cast<int>(rest % p.layers);
+    const int64_t k = rest / p.layers;
+    const int64_t first = layer * p.pages, to = first + list[k], of = first + list[p.pages - 1 - k];
+    const uint4* const src = reinterpret_cast<const uint4*>(p.codes + of * a.page_bytes);
+    uint4* const dst = reinterpret_cast<uint4*>(p.codes + to * a.page_bytes);
+    const int begin = piece * (a.piece / 16), end = min(begin + a.piece / 16, static_cast<int>(a.page_bytes / 16));
+    for (int at = begin + tid; at < end; at += kCompactThreads * kCompactHeld) {
+      uint4 v[kCompactHeld];
+#pragma unroll
+      for (int j = 0; j < kCompactHeld; ++j)
+        if (at + j * kCompactThreads < end) v[j] = __ldcs(src + at + j * kCompactThreads);
+#pragma unroll
+      for (int j = 0; j < kCompactHeld; ++j)
+        if (at + j * kCompactThreads < end) __stcs(dst + at + j * kCompactThreads, v[j]);
+    }
+    if (piece == 0)
+      for (int i = tid; i < 2 * p.kv_heads; i += kCompactThreads) p.scales[to * 2 * p.kv_heads + i] = p.scales[of * 2 * p.kv_heads + i];
+  }
+  const int64_t entries = static_cast<int64_t>(p.slots) * p.max_blocks;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kCompactThreads + tid; i < entries; i += static_cast<int64_t>(gridDim.x) * kCompactThreads) {
+    const int page = p.page_table[i];
+    const int now = page >= 0 && page < p.pages ? where[page] : -1;
+    if (now != page) p.page_table[i] = now;
+  }
+}
+
+}  // namespace b200tx

@@ -1,0 +1,277 @@
+// request_api.cuh -- argument checks and launches of the operators for batches of
+// many requests: low-rank adapters beside a shared projection, pages of the 8-bit cache,
+// verification of drafted tokens.  Part of b200tx.cu's translation unit.
+#pragma once
+
+namespace {
+
+constexpr int kLrShared = 212 * 1024;  // most that a build asks for
+constexpr int kLrTwo = 110 * 1024;     // with which two CTAs share an SM
+
+template <int RT, int NT, bool F32>
+cudaError_t launch_low_rank(b200tx::LowRankArgs& a, DeviceState* dev, int index, cudaStream_t stream) {
+  using S = b200tx::LrShape<RT, NT>;
+  static_assert(S::bytes(8) <= kLrShared, "the sums of eight CTAs do not fit");
+  if (!dev->low_rank_attr[index]) {
+    cudaError_t err = cudaFuncSetAttribute(b200tx::low_rank_kernel<RT, NT, F32>,
+                                           cudaFuncAttributeMaxDynamicSharedMemorySize, kLrShared);
+    if (err != cudaSuccess) return err;
+    dev->low_rank_attr[index] = true;
+  }
+  const int64_t windows = (a.rows + b200tx::kLrWindow - 1) / b200tx::kLrWindow;
+  const int64_t rows = std::min<int64_t>(a.rows, b200tx::kLrWindow);
+  const int64_t least = (rows + S::G - 1) / S::G;  // groups of a window, where its rows share an adapter
+  // Groups that can be: one more for each further index that occurs.
+  const int64_t most = std::min<int64_t>(rows, least + a.count + 1);
+  // CTAs of a group: as many as leave every SM two CTAs at most.
+  int ctas = 8;
+  while (ctas > 1 && windows * least * ctas > 2 * dev->sm_count) ctas /= 2;
+  const int resident = dev->sm_count * (S::bytes(ctas) <= kLrTwo ? 2 : 1);
+  const int64_t tiles = (a.outer + b200tx::kLrTile - 1) / b200tx::kLrTile;
+  a.parts = static_cast<int>((tiles + ctas * b200tx::kLrWarps - 1) / (ctas * b200tx::kLrWarps));
+  a.clusters = static_cast<int>(std::min(std::max(least, resident / (ctas * windows)), most * a.parts));
+  return launch_clustered(b200tx::low_rank_kernel<RT, NT, F32>, dim3(static_cast<unsigned>(windows * a.clusters * ctas)),
+                          dim3(b200tx::kLrThreads), static_cast<size_t>(S::bytes(ctas)), static_cast<unsigned>(ctas), stream, a);
+}
+
+template <int RT, int NT>
+cudaError_t launch_low_rank_base(b200tx::LowRankArgs& a, bool f32, DeviceState* dev, int index, cudaStream_t stream) {
+  return f32 ? launch_low_rank<RT, NT, true>(a, dev, index, stream) : launch_low_rank<RT, NT, false>(a, dev, index + 1, stream);
+}
+
+int kv8_pool(const char* what, const b200tx_kv8_pool* c, b200tx::Kv8Pool* out) {
+  if (c == nullptr) return fail(B200TX_ERR_INVALID_ARGUMENT, "%s: null pool", what);
+  b200tx::Kv8Cache view;
+  int rc = kv8_view(what, &c->cache, &view);
+  if (rc != B200TX_OK) return rc;
+  if (c->refs == nullptr || c->scratch == nullptr)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "%s: null pool pointer", what);
+  if (c->layers <= 0 || c->layers > (1 << 16)) return fail(B200TX_ERR_INVALID_ARGUMENT, "%s: %lld layers", what, (long long)c->layers);
+  if (c->cache.pages > (1 << 30)) return fail(B200TX_ERR_INVALID_ARGUMENT, "%s: %lld pages", what, (long long)c->cache.pages);
+  out->codes = view.codes;
+  out->scales = view.scales;
+  out->tail = reinterpret_cast<uint4*>(view.tail);
+  out->page_table = const_cast<int32_t*>(view.page_table);
+  out->lengths = const_cast<int32_t*>(view.lengths);
+  out->refs = c->refs;
+  out->scratch = c->scratch;
+  out->pages = view.pages;
+  out->slots = view.slots;
+  out->max_blocks = view.max_blocks;
+  out->kv_heads = view.kv_heads;
+  out->dim = static_cast<int>(c->cache.head_dim);
+  out->layers = static_cast<int>(c->layers);
+  return B200TX_OK;
+}
+
+// Places of the table of slots: a power of two, at least twice the rows.
+int slot_places(int64_t rows) {
+  int places = 2;
+  while (places < 2 * rows) places *= 2;
+  return places;
+}
+
+int low_log2(int64_t v) {
+  int shift = 0;
+  while ((int64_t{2} << shift) <= v) ++shift;
+  return shift;
+}
+
+constexpr int kPoolShared = 64 * 1024;  // of 2048 rows' records and places
+
+template <typename Kernel>
+cudaError_t pool_attribute(Kernel kernel, bool* done) {
+  if (*done) return cudaSuccess;
+  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPoolShared);
+  if (err == cudaSuccess) *done = true;
+  return err;
+}
+
+}  // namespace
+
+extern "C" {
+
+int b200tx_low_rank_add(const void* x, const void* base, int base_dtype, void* out, int out_dtype, const void* down,
+                        const void* up, const float* scales, const int32_t* indices, int64_t index_count, int64_t M,
+                        int64_t N, int64_t K, int64_t rank, int64_t adapters, int epilogue, cudaStream_t stream) {
+  if (x == nullptr || base == nullptr || out == nullptr || down == nullptr || up == nullptr || scales == nullptr ||
+      indices == nullptr)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "low_rank_add: null tensor pointer");
+  if (M <= 0 || N <= 0 || K <= 0 || M > (1 << 26) || N > (1 << 24) || K > (1 << 24) || K % 8 != 0)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "low_rank_add: bad shape M %lld N %lld K %lld (K a multiple of 8)",
+                (long long)M, (long long)N, (long long)K);
+  if (rank <= 0 || rank > 128 || rank % 8 != 0)
+    return fail(B200TX_ERR_UNSUPPORTED, "low_rank_add: rank %lld (multiples of 8 up to 128 are built)", (long long)rank);
+  if (adapters <= 0 || adapters > (1 << 20))
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "low_rank_add: %lld adapters", (long long)adapters);
+  if (index_count <= 0 || M % index_count != 0)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "low_rank_add: %lld indices for %lld rows", (long long)index_count, (long long)M);
+  if ((base_dtype != B200TX_F32 && base_dtype != B200TX_BF16) || (out_dtype != B200TX_F32 && out_dtype != B200TX_BF16))
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "low_rank_add: dtypes %d and %d", base_dtype, out_dtype);
+  if (epilogue != B200TX_EPI_BIAS && epilogue != B200TX_EPI_BIAS_GELU)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "low_rank_add: epilogue %d", epilogue);
+  if (!aligned16(x) || !aligned16(base) || !aligned16(out) || !aligned16(down) || !aligned16(up))
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "low_rank_add: x, base, out, down and up must be 16-byte aligned");
+  if (base == out && base_dtype != out_dtype)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "low_rank_add: out is base in another type");
+  DeviceState* dev = nullptr;
+  int rc = current_device(&dev);
+  if (rc != B200TX_OK) return rc;
+  b200tx::LowRankArgs a{};
+  a.x = static_cast<const __nv_bfloat16*>(x);
+  a.base = base;
+  a.out = out;
+  a.down = static_cast<const __nv_bfloat16*>(down);
+  a.up = static_cast<const __nv_bfloat16*>(up);
+  a.scales = scales;
+  a.indices = indices;
+  a.rows = M;
+  a.per_index = static_cast<int>(M / index_count);
+  a.inner = static_cast<int>(K);
+  a.outer = static_cast<int>(N);
+  a.rank = static_cast<int>(rank);
+  a.count = static_cast<int>(adapters);
+  a.out_f32 = out_dtype == B200TX_F32;
+  a.gelu = epilogue == B200TX_EPI_BIAS_GELU;
+  a.skip_bare = base == out && !a.gelu;
+  const bool f32 = base_dtype == B200TX_F32, few = M <= 8;
+  cudaError_t err = rank <= 16   ? few ? launch_low_rank_base<1, 1>(a, f32, dev, 0, stream) : launch_low_rank_base<1, 4>(a, f32, dev, 2, stream)
+                    : rank <= 32 ? few ? launch_low_rank_base<2, 1>(a, f32, dev, 4, stream) : launch_low_rank_base<2, 4>(a, f32, dev, 6, stream)
+                    : rank <= 64 ? few ? launch_low_rank_base<4, 1>(a, f32, dev, 8, stream) : launch_low_rank_base<4, 4>(a, f32, dev, 10, stream)
+                    : few        ? launch_low_rank_base<8, 1>(a, f32, dev, 12, stream)
+                                 : launch_low_rank_base<8, 2>(a, f32, dev, 14, stream);
+  return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "low_rank_add");
+}
+
+int b200tx_kv8_pool_scratch(int64_t pages, int64_t* ints_out) {
+  if (ints_out == nullptr || pages <= 0 || pages > (1 << 30))
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_pool_scratch: %lld pages", (long long)pages);
+  *ints_out = b200tx::kPoolCounters + 2 * pages;
+  return B200TX_OK;
+}
+
+int b200tx_kv8_fork(const b200tx_kv8_pool* pool, const int32_t* source, const int32_t* target, int64_t pairs,
+                    cudaStream_t stream) {
+  b200tx::Kv8ForkArgs a{};
+  int rc = kv8_pool("kv8_fork", pool, &a.pool);
+  if (rc != B200TX_OK) return rc;
+  if (pairs < 0 || pairs > b200tx::kPoolRows)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_fork: %lld sequences (%d at most)", (long long)pairs, b200tx::kPoolRows);
+  if (pairs == 0) return B200TX_OK;
+  if (target == nullptr) return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_fork: null target");
+  DeviceState* dev = nullptr;
+  rc = current_device(&dev);
+  if (rc != B200TX_OK) return rc;
+  a.source = source;
+  a.target = target;
+  a.pairs = static_cast<int>(pairs);
+  a.owners = slot_places(pairs);
+  const int region = b200tx::kKv8Block * a.pool.dim / 8;
+  a.piece_shift = std::min(low_log2(b200tx::kForkPieces / pairs), low_log2(region));
+  a.column_shift = low_log2(b200tx::kForkPieces / pairs);
+  const int64_t tail_items =
+      source == nullptr ? 0 : static_cast<int64_t>(a.pool.layers) * 2 * a.pool.kv_heads * (region >> a.piece_shift);
+  const int64_t table_items = ((a.pool.max_blocks - 1) >> a.column_shift) + 1;
+  if (tail_items + table_items > 0x7fffffffLL)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_fork: too many layers and heads");
+  a.tail_items = static_cast<int>(tail_items);
+  a.table_items = static_cast<int>(table_items);
+  cudaError_t err = pool_attribute(b200tx::kv8_fork_kernel, &dev->fork_attr);
+  const int64_t grid = std::min<int64_t>(tail_items + table_items, 4 * dev->sm_count);
+  if (err == cudaSuccess)
+    err = launch(b200tx::kv8_fork_kernel, dim3(static_cast<unsigned>(grid)), dim3(b200tx::kForkThreads),
+                 pairs * sizeof(b200tx::ForkPair) + 8 * a.owners, stream, a);
+  return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "kv8_fork");
+}
+
+int b200tx_kv8_reserve(const b200tx_kv8_pool* pool, const int32_t* slot_ids, const int32_t* counts, int64_t tokens,
+                       int64_t rows, int32_t* missing, cudaStream_t stream) {
+  b200tx::Kv8ReserveArgs a{};
+  int rc = kv8_pool("kv8_reserve", pool, &a.pool);
+  if (rc != B200TX_OK) return rc;
+  if (rows <= 0 || rows > b200tx::kPoolRows || tokens < 0 || tokens > (1 << 26))
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_reserve: %lld tokens of %lld sequences (%d at most)", (long long)tokens,
+                (long long)rows, b200tx::kPoolRows);
+  if (missing == nullptr) return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_reserve: null result");
+  if (slot_ids == nullptr && rows > a.pool.slots)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_reserve: %lld sequences in a cache of %d slots", (long long)rows, a.pool.slots);
+  if (rows * std::min<int64_t>(a.pool.max_blocks, tokens / b200tx::kKv8Block + 1) > (1 << 30))
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_reserve: too many blocks");
+  DeviceState* dev = nullptr;
+  rc = current_device(&dev);
+  if (rc != B200TX_OK) return rc;
+  a.slot_ids = slot_ids;
+  a.counts = counts;
+  a.missing = missing;
+  a.tokens = static_cast<int>(tokens);
+  a.rows = static_cast<int>(rows);
+  a.owners = slot_places(rows);
+  cudaError_t err = pool_attribute(b200tx::kv8_reserve_kernel, &dev->reserve_attr);
+  if (err == cudaSuccess)
+    err = launch_clustered(b200tx::kv8_reserve_kernel, dim3(b200tx::kPoolCtas), dim3(b200tx::kPoolThreads),
+                           static_cast<size_t>(12 * rows + 8 * a.owners), b200tx::kPoolCtas, stream, a);
+  return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "kv8_reserve");
+}
+
+int b200tx_kv8_compact(const b200tx_kv8_pool* pool, int32_t* used, cudaStream_t stream) {
+  b200tx::Kv8CompactArgs a{};
+  int rc = kv8_pool("kv8_compact", pool, &a.pool);
+  if (rc != B200TX_OK) return rc;
+  if (used == nullptr) return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_compact: null result");
+  DeviceState* dev = nullptr;
+  rc = current_device(&dev);
+  if (rc != B200TX_OK) return rc;
+  a.used = used;
+  a.page_bytes = static_cast<int64_t>(2) * a.pool.kv_heads * b200tx::kKv8Block * a.pool.dim;
+  constexpr int64_t kPiece = b200tx::kCompactThreads * b200tx::kCompactHeld * 16;
+  a.piece = static_cast<int>(std::min(a.page_bytes, kPiece));
+  a.pieces = static_cast<int>((a.page_bytes + a.piece - 1) / a.piece);
+  cudaError_t err = launch_clustered(b200tx::kv8_compact_plan_kernel, dim3(b200tx::kPoolCtas), dim3(b200tx::kPoolThreads), 0,
+                                     b200tx::kPoolCtas, stream, a);
+  if (err == cudaSuccess)
+    err = launch(b200tx::kv8_compact_move_kernel, dim3(static_cast<unsigned>(4 * dev->sm_count)), dim3(b200tx::kCompactThreads),
+                 0, stream, a);
+  return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "kv8_compact");
+}
+
+int b200tx_verify_draft(const void* target, int64_t target_batch_stride, int64_t target_token_stride, const void* draft,
+                        int64_t draft_batch_stride, int64_t draft_token_stride, int dtype, const void* drafted,
+                        int drafted_64, const float* uniform, const int32_t* counts, int64_t batch, int64_t tokens,
+                        int64_t vocab, void* out, int32_t* accepted, cudaStream_t stream) {
+  if (target == nullptr || (drafted == nullptr && tokens > 0) || uniform == nullptr || out == nullptr || accepted == nullptr)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "verify_draft: null tensor pointer");
+  if (batch <= 0 || batch > (1 << 20) || tokens < 0 || tokens > b200tx::kVerifyTokens || vocab <= 0 || vocab > (1 << 28))
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "verify_draft: bad shape batch %lld tokens %lld (%d at most) vocab %lld",
+                (long long)batch, (long long)tokens, b200tx::kVerifyTokens, (long long)vocab);
+  if (dtype != B200TX_F32 && dtype != B200TX_BF16)
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "verify_draft: dtype %d", dtype);
+  DeviceState* dev = nullptr;
+  int rc = current_device(&dev);
+  if (rc != B200TX_OK) return rc;
+  b200tx::VerifyArgs a{};
+  a.target = target;
+  a.draft = draft;
+  a.drafted = drafted;
+  a.uniform = uniform;
+  a.counts = counts;
+  a.out = out;
+  a.accepted = accepted;
+  a.target_batch_stride = target_batch_stride;
+  a.target_token_stride = target_token_stride;
+  a.draft_batch_stride = draft_batch_stride;
+  a.draft_token_stride = draft_token_stride;
+  a.tokens = static_cast<int>(tokens);
+  a.vocab = static_cast<int>(vocab);
+  a.wide = drafted_64 != 0;
+  a.vec = aligned16(target) && (draft == nullptr || aligned16(draft)) &&
+          (target_batch_stride | target_token_stride | draft_batch_stride | draft_token_stride) % 4 == 0;
+  constexpr unsigned kCtas = 8;
+  const dim3 grid(static_cast<unsigned>(batch) * kCtas);
+  cudaError_t err = dtype == B200TX_F32
+                        ? launch_clustered(b200tx::verify_draft_kernel<float>, grid, dim3(b200tx::kVerifyThreads), 0, kCtas, stream, a)
+                        : launch_clustered(b200tx::verify_draft_kernel<__nv_bfloat16>, grid, dim3(b200tx::kVerifyThreads), 0,
+                                           kCtas, stream, a);
+  return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "verify_draft");
+}
+
+}  // extern "C"

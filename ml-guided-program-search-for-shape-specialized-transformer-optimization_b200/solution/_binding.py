@@ -25,6 +25,11 @@ _ENTRY_POINTS = (
     "b200tx_kv8_gather",
     "b200tx_kv8_attention",
     "b200tx_linear_w4",
+    "b200tx_low_rank_add",
+    "b200tx_kv8_fork",
+    "b200tx_kv8_reserve",
+    "b200tx_kv8_compact",
+    "b200tx_verify_draft",
 )
 
 _lock = threading.Lock()

@@ -387,6 +387,73 @@ def _declare(lib: ctypes.CDLL) -> None:
         _c_void_p,  # stream
     ]
 
+    lib.b200tx_low_rank_add.restype = ctypes.c_int
+    lib.b200tx_low_rank_add.argtypes = [
+        _c_void_p,  # x
+        _c_void_p,  # base
+        ctypes.c_int,  # base_dtype
+        _c_void_p,  # out
+        ctypes.c_int,  # out_dtype
+        _c_void_p,  # down
+        _c_void_p,  # up
+        _c_void_p,  # scales
+        _c_void_p,  # indices
+        _c_int64,  # index_count
+        _c_int64,  # M
+        _c_int64,  # N
+        _c_int64,  # K
+        _c_int64,  # rank
+        _c_int64,  # adapters
+        ctypes.c_int,  # epilogue
+        _c_void_p,  # stream
+    ]
+    lib.b200tx_kv8_pool_scratch.restype = ctypes.c_int
+    lib.b200tx_kv8_pool_scratch.argtypes = [_c_int64, ctypes.POINTER(_c_int64)]
+    lib.b200tx_kv8_fork.restype = ctypes.c_int
+    lib.b200tx_kv8_fork.argtypes = [
+        _c_void_p,  # pool (b200tx_kv8_pool*)
+        _c_void_p,  # source
+        _c_void_p,  # target
+        _c_int64,  # pairs
+        _c_void_p,  # stream
+    ]
+    lib.b200tx_kv8_reserve.restype = ctypes.c_int
+    lib.b200tx_kv8_reserve.argtypes = [
+        _c_void_p,  # pool
+        _c_void_p,  # slot_ids
+        _c_void_p,  # counts
+        _c_int64,  # tokens
+        _c_int64,  # rows
+        _c_void_p,  # missing
+        _c_void_p,  # stream
+    ]
+    lib.b200tx_kv8_compact.restype = ctypes.c_int
+    lib.b200tx_kv8_compact.argtypes = [
+        _c_void_p,  # pool
+        _c_void_p,  # used
+        _c_void_p,  # stream
+    ]
+    lib.b200tx_verify_draft.restype = ctypes.c_int
+    lib.b200tx_verify_draft.argtypes = [
+        _c_void_p,  # target
+        _c_int64,  # target_batch_stride
+        _c_int64,  # target_token_stride
+        _c_void_p,  # draft
+        _c_int64,  # draft_batch_stride
+        _c_int64,  # draft_token_stride
+        ctypes.c_int,  # dtype
+        _c_void_p,  # drafted
+        ctypes.c_int,  # drafted_64
+        _c_void_p,  # uniform
+        _c_void_p,  # counts
+        _c_int64,  # batch
+        _c_int64,  # tokens
+        _c_int64,  # vocab
+        _c_void_p,  # out
+        _c_void_p,  # accepted
+        _c_void_p,  # stream
+    ]
+
 
 def library_path() -> Path:
     return LIB_PATH
@@ -1007,6 +1074,17 @@ class Kv8CacheView(ctypes.Structure):
     ]
 
 
+class Kv8PoolView(ctypes.Structure):
+    """b200tx_kv8_pool: the pages of an 8-bit cache, all layers."""
+
+    _fields_ = [
+        ("cache", Kv8CacheView),
+        ("layers", ctypes.c_int64),
+        ("refs", ctypes.c_void_p),
+        ("scratch", ctypes.c_void_p),
+    ]
+
+
 KV8_BLOCK = 64  # B200TX_KV8_BLOCK
 KV8_COUNTER_BYTES = 8192  # B200TX_KV8_COUNTER_BYTES
 
@@ -1020,6 +1098,14 @@ def kv8_workspace_bytes(head_dim: int) -> int:
 
     size = ctypes.c_int64(0)
     _check(load().b200tx_kv8_workspace_bytes(head_dim, ctypes.byref(size)), "b200tx_kv8_workspace_bytes")
+    return int(size.value)
+
+
+def kv8_pool_scratch(pages: int) -> int:
+    """The ints of scratch that a pool of this many pages needs."""
+
+    size = ctypes.c_int64(0)
+    _check(load().b200tx_kv8_pool_scratch(pages, ctypes.byref(size)), "b200tx_kv8_pool_scratch")
     return int(size.value)
 
 
@@ -1070,8 +1156,10 @@ __all__ = [
     "KV8_BLOCK",
     "KV8_COUNTER_BYTES",
     "Kv8CacheView",
+    "Kv8PoolView",
     "Rope",
     "kv8_attention",
+    "kv8_pool_scratch",
     "kv8_workspace_bytes",
     "linear_w4",
     "IPC_HANDLE_BYTES",

@@ -42,6 +42,17 @@ from .kv_cache import (
     sm100_kv8_attention,
     sm100_kv8_gather,
 )
+from .kv_pages import (
+    KV8_POOL_ROWS,
+    SM100_KV8_COMPACT_BACKEND,
+    SM100_KV8_FORK_BACKEND,
+    SM100_KV8_RESERVE_BACKEND,
+    Kv8Pages,
+    sm100_kv8_compact,
+    sm100_kv8_fork,
+    sm100_kv8_free,
+    sm100_kv8_reserve,
+)
 from .linear_w4 import (
     SM100_LINEAR_W4_BACKEND,
     SM100_LINEAR_W4_GELU_BACKEND,
@@ -49,6 +60,13 @@ from .linear_w4 import (
     can_use_sm100_linear_w4,
     pack_w4,
     sm100_linear_w4,
+)
+from .low_rank import (
+    SM100_LOW_RANK_ADD_BACKEND,
+    SM100_LOW_RANK_ADD_GELU_BACKEND,
+    LowRankAdapters,
+    can_use_sm100_low_rank_add,
+    sm100_low_rank_add,
 )
 from .norm import (
     MASK_DROP_UPDATE,
@@ -74,9 +92,31 @@ from .rotary import (
     can_use_sm100_qk_norm_rope,
     sm100_qk_norm_rope,
 )
+from .verify import (
+    SM100_VERIFY_DRAFT_BACKEND,
+    can_use_sm100_verify_draft,
+    sm100_verify_draft,
+)
 from . import ops  # noqa: E402 - registers the torch.ops.b200tx.* operators
 
 __all__ = [
+    "KV8_POOL_ROWS",
+    "Kv8Pages",
+    "LowRankAdapters",
+    "SM100_KV8_COMPACT_BACKEND",
+    "SM100_KV8_FORK_BACKEND",
+    "SM100_KV8_RESERVE_BACKEND",
+    "SM100_LOW_RANK_ADD_BACKEND",
+    "SM100_LOW_RANK_ADD_GELU_BACKEND",
+    "SM100_VERIFY_DRAFT_BACKEND",
+    "can_use_sm100_low_rank_add",
+    "can_use_sm100_verify_draft",
+    "sm100_kv8_compact",
+    "sm100_kv8_fork",
+    "sm100_kv8_free",
+    "sm100_kv8_reserve",
+    "sm100_low_rank_add",
+    "sm100_verify_draft",
     "KV8_BLOCK",
     "Kv8Cache",
     "RotaryTable",

@@ -111,17 +111,23 @@ class Kv8Cache(TensorHandle):
         num_kv_heads: int,
         head_dim: int,
         layers: int = 1,
+        pages: int | None = None,
         device: torch.device | str = "cuda",
     ) -> Kv8Cache:
-        """An empty cache of ``slots`` sequences of up to ``max_tokens`` tokens."""
+        """An empty cache of ``slots`` sequences of up to ``max_tokens`` tokens: each slot with
+        pages of its own, or, with ``pages``, that many pages that no slot holds yet (``Kv8Pages``)."""
 
         blocks = -(-max_tokens // KV8_BLOCK)
-        pages = slots * blocks
+        own = pages is None
+        if own:
+            pages = slots * blocks
         return cls(
             torch.zeros((layers, pages, 2, num_kv_heads, KV8_BLOCK, head_dim), dtype=torch.uint8, device=device),
             torch.zeros((layers, pages, 2, num_kv_heads), dtype=torch.float32, device=device),
             torch.zeros((layers, slots, 2, 2, num_kv_heads, KV8_BLOCK, head_dim), dtype=torch.bfloat16, device=device),
-            torch.arange(pages, dtype=torch.int32, device=device).reshape(slots, blocks),
+            torch.arange(pages, dtype=torch.int32, device=device).reshape(slots, blocks)
+            if own
+            else torch.full((slots, blocks), -1, dtype=torch.int32, device=device),
             torch.zeros(slots, dtype=torch.int32, device=device),
         )
 
