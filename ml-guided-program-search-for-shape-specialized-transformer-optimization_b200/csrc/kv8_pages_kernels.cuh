@@ -71,7 +71,7 @@ struct Kv8ForkArgs {
 struct ForkPair {
   int source, target;  // target -1: the pair does nothing; source -1: from nothing
   int full;            // full blocks of the source
-  int open;            // rows of its open block, or'ed with 64 times the block's parity
+  int held;            // tokens of the source
 };
 
 // All pairs at once: every target becomes what its source was before the call.  An item is
@@ -102,15 +102,14 @@ __global__ void __launch_bounds__(kForkThreads, 3) kv8_fork_kernel(const __grid_
     ForkPair f;
     f.source = a.source == nullptr ? -1 : a.source[i];
     f.target = a.target[i];
-    f.full = f.open = 0;
+    f.full = f.held = 0;
     const bool known = f.target >= 0 && f.target < p.slots && f.source < p.slots;
     // a sequence that becomes itself stays as it is, with the pages that are reserved for it
     if (!known || f.source == f.target || owners.rows[owners.place(f.target)] != i) {
       f.target = -1;
     } else if (f.source >= 0) {
-      const int held = max(0, p.lengths[f.source]), block = held / kKv8Block;
-      f.full = min(block, p.max_blocks);
-      f.open = held % kKv8Block | (block & 1) * kKv8Block;
+      f.held = max(0, p.lengths[f.source]);
+      f.full = min(f.held / kKv8Block, p.max_blocks);
     } else {
       f.source = -1;
     }
@@ -120,29 +119,32 @@ __global__ void __launch_bounds__(kForkThreads, 3) kv8_fork_kernel(const __grid_
 
   const int row = p.dim / 8;                 // 16-byte pieces of a token's head
   const int region = kKv8Block * row;        // of a head's block
-  const int each = 1 << a.piece_shift, pieces = region >> a.piece_shift;
+  const int each = 1 << a.piece_shift, pieces = region >> a.piece_shift, heads = 2 * p.kv_heads;
+  const uint32_t parity_pieces = static_cast<uint32_t>(heads) * region;  // of a slot's blocks of one parity
   for (int item = blockIdx.x; item < a.tail_items + a.table_items; item += gridDim.x) {
     if (item < a.tail_items) {
       const int part = item % pieces, rest = item / pieces;
-      const int heads = 2 * p.kv_heads, head = rest % heads, layer = rest / heads;
+      const int head = rest % heads, layer = rest / heads;
+      uint4* const base = p.tail + static_cast<int64_t>(layer) * p.slots * 2 * parity_pieces + static_cast<int64_t>(head) * region;
+      // a piece's place in a slot, the same for all of a thread's pairs where an item has up to 256 pieces of each
+      auto place = [&](int j) { return part * each + ((j * kForkThreads + tid) & (each - 1)); };
+      auto open = [&](const ForkPair& f, int at) { return f.target >= 0 && at < f.held % kKv8Block * row; };
       uint4 v[kForkHeld];
-      uint4* to[kForkHeld];
 #pragma unroll
       for (int j = 0; j < kForkHeld; ++j) {
-        const int e = j * kForkThreads + tid, i = e >> a.piece_shift, at = part * each + (e & (each - 1));
-        to[j] = nullptr;
+        const int i = (j * kForkThreads + tid) >> a.piece_shift, at = place(j);
         if (i >= a.pairs) continue;
         const ForkPair f = pair[i];
-        if (f.target < 0 || at >= (f.open & (kKv8Block - 1)) * row) continue;
-        const int64_t inside = (static_cast<int64_t>(f.open / kKv8Block) * heads + head) * region + at;
-        const int64_t slot = static_cast<int64_t>(2) * heads * region, first = static_cast<int64_t>(layer) * p.slots;
-        v[j] = p.tail[(first + f.source) * slot + inside];
-        to[j] = p.tail + (first + f.target) * slot + inside;
+        if (open(f, at)) v[j] = base[static_cast<uint64_t>(2 * f.source + (f.held / kKv8Block & 1)) * parity_pieces + at];
       }
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < kForkHeld; ++j)
-        if (to[j] != nullptr) *to[j] = v[j];
+      for (int j = 0; j < kForkHeld; ++j) {
+        const int i = (j * kForkThreads + tid) >> a.piece_shift, at = place(j);
+        if (i >= a.pairs) continue;
+        const ForkPair f = pair[i];
+        if (open(f, at)) base[static_cast<uint64_t>(2 * f.target + (f.held / kKv8Block & 1)) * parity_pieces + at] = v[j];
+      }
     } else {
       const int columns = 1 << a.column_shift, from = (item - a.tail_items) << a.column_shift;
       int page[kForkHeld];
@@ -179,53 +181,58 @@ __global__ void __launch_bounds__(kForkThreads, 3) kv8_fork_kernel(const __grid_
   }
   __syncthreads();
   if (!s_last) return;
-  for (int i = tid; i < a.pairs; i += kForkThreads) owners.rows[i] = pair[i].target >= 0 && pair[i].source >= 0 ? max(0, p.lengths[pair[i].source]) : 0;
-  __syncthreads();
   for (int i = tid; i < a.pairs; i += kForkThreads)
-    if (pair[i].target >= 0) p.lengths[pair[i].target] = owners.rows[i];
+    if (pair[i].target >= 0) p.lengths[pair[i].target] = pair[i].held;
 }
 
 // ------------------------------------------------------------------ order over a cluster
-// One cluster of CTAs does what needs an order over all pages or entries: each
-// CTA takes a stretch, and the stretches' counts go round through distributed shared memory.
+// One CTA, or a cluster of them for many pages or entries, does what needs an order over all: each
+// takes a stretch, and the stretches' counts go round through (distributed) shared memory.
 constexpr int kPoolCtas = 8;
 constexpr int kPoolThreads = 1024;
 constexpr int kPoolWarps = kPoolThreads / 32;
-constexpr int kPoolAllWarps = kPoolCtas * kPoolWarps;
+
+__device__ __forceinline__ int pool_ctas() {
+  uint32_t n;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+  return static_cast<int>(n);
+}
+
+__device__ __forceinline__ void pool_sync(int ctas) {
+  if (ctas > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+}
 
 struct PoolShared {
-  int warp[kPoolWarps];
+  int warp[2][kPoolWarps];
   int cta[2][2][kPoolCtas];  // [exchange's parity][which count][CTA]
 };
 
-// The counts of two kinds that the warps before this one hold, and of all, over the cluster.  All
+// N counts that the warps before this one hold, and of all, over the cluster.  All
 // threads call it; the counts are a warp's (the same in its lanes).
-__device__ __forceinline__ void pool_order(PoolShared& s, int& turn, const int (&count)[2], int (&before)[2], int (&all)[2]) {
+template <int N>
+__device__ __forceinline__ void pool_order(PoolShared& s, int ctas, int& turn, const int (&count)[N], int (&before)[N], int (&all)[N]) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, me = static_cast<int>(cluster_ctarank());
   const int parity = turn++ & 1;
+  __syncthreads();
+  if (lane < N) s.warp[lane][warp] = lane == 0 ? count[0] : count[N - 1];
+  __syncthreads();
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    __syncthreads();
-    if (lane == 0) s.warp[warp] = count[k];
-    __syncthreads();
-    int mine = s.warp[lane];
-    int sum = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-      const int o = __shfl_up_sync(0xffffffffu, sum, d);
-      if (lane >= d) sum += o;
-    }
-    before[k] = __shfl_sync(0xffffffffu, sum - mine, warp);
-    const int total = __shfl_sync(0xffffffffu, sum, 31);
-    if (warp == 0 && lane < kPoolCtas)
-      asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(peer_smem_addr(&s.cta[parity][k][me], lane)), "r"(total) : "memory");
+  for (int k = 0; k < N; ++k) {
+    const int mine = s.warp[k][lane];
+    all[k] = __reduce_add_sync(0xffffffffu, mine);
+    before[k] = __reduce_add_sync(0xffffffffu, lane < warp ? mine : 0);
+    if (ctas > 1 && warp == 0 && lane < ctas)
+      asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(peer_smem_addr(&s.cta[parity][k][me], lane)), "r"(all[k]) : "memory");
   }
+  if (ctas == 1) return;
   cluster_sync();
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
+  for (int k = 0; k < N; ++k) {
     all[k] = 0;
-#pragma unroll
-    for (int i = 0; i < kPoolCtas; ++i) {
+    for (int i = 0; i < ctas; ++i) {
       if (i < me) before[k] += s.cta[parity][k][i];
       all[k] += s.cta[parity][k][i];
     }
@@ -235,8 +242,9 @@ __device__ __forceinline__ void pool_order(PoolShared& s, int& turn, const int (
 // Calls f(page, refs) for this warp's stretch of the pages, 32 neighbouring pages at a time (all lanes
 // call; past the end refs is -1).
 template <typename F>
-__device__ __forceinline__ void pool_pages(const Kv8Pool& p, F f) {
-  const int64_t each = ((p.pages + 31) / 32 + kPoolAllWarps - 1) / kPoolAllWarps * 32;
+__device__ __forceinline__ void pool_pages(const Kv8Pool& p, int ctas, F f) {
+  const int warps = ctas * kPoolWarps;
+  const int64_t each = ((p.pages + 31) / 32 + warps - 1) / warps * 32;
   const int64_t from = each * (cluster_ctarank() * kPoolWarps + threadIdx.x / 32);
   constexpr int U = 8;
   for (int64_t at = from; at < min(from + each, p.pages); at += U * 32) {
@@ -279,21 +287,26 @@ __global__ void __launch_bounds__(kPoolThreads, 1) kv8_reserve_kernel(const __gr
   const Kv8Pool& p = a.pool;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, me = static_cast<int>(cluster_ctarank());
   int turn = 0;
-  cluster_sync();
+  const int ctas = pool_ctas();
+  if (ctas > 1) cluster_sync();
   griddep_wait();
   griddep_launch_dependents();
 
-  for (int i = tid; i < a.owners; i += kPoolThreads) {
-    owners.slots[i] = -1;
-    owners.rows[i] = kPoolRows;
+  if (a.slot_ids != nullptr) {
+    for (int i = tid; i < a.owners; i += kPoolThreads) {
+      owners.slots[i] = -1;
+      owners.rows[i] = kPoolRows;
+    }
+    __syncthreads();
+    for (int b = tid; b < a.rows; b += kPoolThreads) {
+      const int slot = a.slot_ids[b];
+      slot_of[b] = slot;
+      if (slot >= 0 && slot < p.slots) atomicMin(owners.rows + owners.place(slot), b);
+    }
+    __syncthreads();
+  } else {
+    for (int b = tid; b < a.rows; b += kPoolThreads) slot_of[b] = b;
   }
-  __syncthreads();
-  for (int b = tid; b < a.rows; b += kPoolThreads) {
-    const int slot = a.slot_ids == nullptr ? b : a.slot_ids[b];
-    slot_of[b] = slot;
-    if (slot >= 0 && slot < p.slots) atomicMin(owners.rows + owners.place(slot), b);
-  }
-  __syncthreads();
   int running = 0;
   for (int base = 0; base < a.rows; base += kPoolThreads) {
     const int b = base + tid;
@@ -301,7 +314,7 @@ __global__ void __launch_bounds__(kPoolThreads, 1) kv8_reserve_kernel(const __gr
     if (b < a.rows) {
       const int slot = slot_of[b];
       int past = 0;
-      if (slot >= 0 && slot < p.slots && owners.rows[owners.place(slot)] == b) {
+      if (slot >= 0 && slot < p.slots && (a.slot_ids == nullptr || owners.rows[owners.place(slot)] == b)) {
         const int64_t held = max(0, p.lengths[slot]), n = a.counts == nullptr ? a.tokens : min(max(a.counts[b], 0), a.tokens);
         const int64_t from = held / kKv8Block, to = (held + n) / kKv8Block;
         begin[b] = static_cast<int>(from);
@@ -318,104 +331,114 @@ __global__ void __launch_bounds__(kPoolThreads, 1) kv8_reserve_kernel(const __gr
       if (lane >= d) sum += o;
     }
     __syncthreads();
-    if (lane == 31) s.warp[warp] = sum;
+    if (lane == 31) s.warp[0][warp] = sum;
     __syncthreads();
-    int total = s.warp[lane];
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-      const int o = __shfl_up_sync(0xffffffffu, total, d);
-      if (lane >= d) total += o;
-    }
-    const int warps_before = warp == 0 ? 0 : __shfl_sync(0xffffffffu, total, max(warp - 1, 0));
+    const int of_warp = s.warp[0][lane];
+    const int warps_before = __reduce_add_sync(0xffffffffu, lane < warp ? of_warp : 0);
     if (b < a.rows) upto[b] = running + warps_before + sum;
-    running += __shfl_sync(0xffffffffu, total, 31);
+    running += __reduce_add_sync(0xffffffffu, of_warp);
   }
   __syncthreads();
   const int all_entries = running;
 
-  // this warp's stretch of the entries, 32 neighbours at a time
-  const int each = ((all_entries + 31) / 32 + kPoolAllWarps - 1) / kPoolAllWarps * 32;
+  // this warp's stretch of the entries, 32 neighbours at a time, several of these with their loads in flight
+  const int warps = ctas * kPoolWarps;
+  const int each = ((all_entries + 31) / 32 + warps - 1) / warps * 32;
   const int first = each * (me * kPoolWarps + warp), last = min(first + each, all_entries);
-  auto row_of = [&](int entry) {
-    int lo = 0, hi = a.rows - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (upto[mid] > entry) hi = mid;
-      else lo = mid + 1;
+  constexpr int U = 4;
+  // f(page, entry, row, whether there is one) for each entry with its page, all lanes
+  auto entries = [&](auto f) {
+    for (int at = first; at < last; at += 32 * U) {
+      int row[U], page[U];
+      int32_t* entry[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int e = at + u * 32 + lane;
+        entry[u] = nullptr;
+        row[u] = page[u] = 0;
+        if (e >= last) continue;
+        int lo = 0, hi = a.rows - 1;
+        while (lo < hi) {
+          const int mid = (lo + hi) / 2;
+          if (upto[mid] > e)
+            hi = mid;
+          else
+            lo = mid + 1;
+        }
+        row[u] = lo;
+        entry[u] = p.page_table + static_cast<int64_t>(slot_of[lo]) * p.max_blocks + begin[lo] + (e - (lo == 0 ? 0 : upto[lo - 1]));
+        page[u] = *entry[u];
+      }
+      f(page, entry, row);
     }
-    return lo;
-  };
-  auto entry_of = [&](int entry, int row) {
-    const int in_row = entry - (row == 0 ? 0 : upto[row - 1]);
-    return p.page_table + static_cast<int64_t>(slot_of[row]) * p.max_blocks + begin[row] + in_row;
   };
   // A page that another entry holds too: the entry is marked with it, and given back when all are marked.
-  int wanted = 0;
-  for (int at = first; at < last; at += 32) {
-    const int e = at + lane;
-    bool want = false;
-    if (e < last) {
-      int32_t* const entry = entry_of(e, row_of(e));
-      const int page = *entry;
-      if (page < 0 || page >= p.pages) {
-        want = true;
-        *entry = -1;
-      } else if (p.refs[page] > 1) {
-        want = true;
-        *entry = -2 - page;
-      }
+  int wanted = 0, shared = 0;
+  entries([&](int (&page)[U], int32_t* (&entry)[U], int (&)[U]) {
+    int refs[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool known = entry[u] != nullptr && page[u] >= 0 && page[u] < p.pages;
+      refs[u] = known ? p.refs[page[u]] : 0;
+      if (!known) page[u] = -1;
     }
-    wanted += __popc(__ballot_sync(0xffffffffu, want));
-  }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool twice = refs[u] > 1, want = entry[u] != nullptr && (page[u] < 0 || twice);
+      if (want) *entry[u] = twice ? -2 - page[u] : -1;
+      wanted += __popc(__ballot_sync(0xffffffffu, want));
+      shared += __popc(__ballot_sync(0xffffffffu, twice));
+    }
+  });
   int before[2], all[2];
-  pool_order(s, turn, {wanted, 0}, before, all);
+  pool_order(s, ctas, turn, {wanted, shared}, before, all);
   if (all[0] == 0) return;
-  for (int at = first; at < last; at += 32) {
-    const int e = at + lane;
-    if (e < last) {
-      const int page = *entry_of(e, row_of(e));
-      if (page <= -2) atomicSub(p.refs + (-2 - page), 1);
-    }
+  if (all[1] != 0) {
+    entries([&](int (&page)[U], int32_t* (&)[U], int (&)[U]) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (page[u] <= -2) atomicSub(p.refs + (-2 - page[u]), 1);
+    });
+    pool_sync(ctas);
   }
-  cluster_sync();
 
   int free_pages = 0;
-  pool_pages(p, [&](int, int refs) { free_pages += __popc(__ballot_sync(0xffffffffu, refs == 0)); });
-  int free_before[2], free_all[2];
-  pool_order(s, turn, {free_pages, 0}, free_before, free_all);
+  pool_pages(p, ctas, [&](int, int refs) { free_pages += __popc(__ballot_sync(0xffffffffu, refs == 0)); });
+  int free_before[1], free_all[1];
+  pool_order(s, ctas, turn, {free_pages}, free_before, free_all);
   int32_t* const list = p.scratch + kPoolCounters;
   int at_free = free_before[0];
-  pool_pages(p, [&](int page, int refs) {
-    const uint32_t bits = __ballot_sync(0xffffffffu, refs == 0);
-    const int k = at_free + __popc(bits & ((1u << lane) - 1));
-    if (refs == 0 && k < all[0]) list[k] = page;
-    at_free += __popc(bits);
-  });
-  cluster_sync();
-  int at_want = before[0];
-  for (int at = first; at < last; at += 32) {
-    const int e = at + lane;
-    int row = 0;
-    int32_t* entry = nullptr;
-    if (e < last) {
-      row = row_of(e);
-      entry = entry_of(e, row);
-      if (*entry >= 0) entry = nullptr;
-    }
-    const uint32_t bits = __ballot_sync(0xffffffffu, entry != nullptr);
-    if (entry != nullptr) {
-      const int k = at_want + __popc(bits & ((1u << lane) - 1));
-      if (k < free_all[0]) {
-        const int page = __ldcg(list + k);
-        *entry = page;
-        p.refs[page] = 1;
-      } else {
-        *entry = -1;
-        atomicAdd(a.missing + row, 1);
-      }
-    }
-    at_want += __popc(bits);
+  if (at_free < all[0]) {
+    pool_pages(p, ctas, [&](int page, int refs) {
+      const uint32_t bits = __ballot_sync(0xffffffffu, refs == 0);
+      const int k = at_free + __popc(bits & ((1u << lane) - 1));
+      if (refs == 0 && k < all[0]) list[k] = page;
+      at_free += __popc(bits);
+    });
   }
+  pool_sync(ctas);
+  int at_want = before[0];
+  entries([&](int (&page)[U], int32_t* (&entry)[U], int (&row)[U]) {
+    int given[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool want = entry[u] != nullptr && page[u] < 0;
+      const uint32_t bits = __ballot_sync(0xffffffffu, want);
+      const int k = at_want + __popc(bits & ((1u << lane) - 1));
+      if (!want) entry[u] = nullptr;
+      given[u] = want && k < free_all[0] ? __ldcg(list + k) : -1;
+      at_want += __popc(bits);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (entry[u] == nullptr) continue;
+      *entry[u] = given[u];
+      if (given[u] >= 0)
+        p.refs[given[u]] = 1;
+      else
+        atomicAdd(a.missing + row[u], 1);
+    }
+  });
 }
 
 // ------------------------------------------------------------------ compact
@@ -437,22 +460,23 @@ __global__ void __launch_bounds__(kPoolThreads, 1) kv8_compact_plan_kernel(const
   int32_t* const where = p.scratch + kPoolCounters;
   int32_t* const list = where + p.pages;  // holes from the front, movers from the back: not more than the pages
   int turn = 0;
-  cluster_sync();
+  const int ctas = pool_ctas();
+  if (ctas > 1) cluster_sync();
   griddep_wait();
   griddep_launch_dependents();
   int held = 0;
-  pool_pages(p, [&](int, int refs) { held += __popc(__ballot_sync(0xffffffffu, refs > 0)); });
-  int before[2], all[2];
-  pool_order(s, turn, {held, 0}, before, all);
-  const int used = all[0];
+  pool_pages(p, ctas, [&](int, int refs) { held += __popc(__ballot_sync(0xffffffffu, refs > 0)); });
+  int before[2], all[2], none[1], in_use[1];
+  pool_order(s, ctas, turn, {held}, none, in_use);
+  const int used = in_use[0];
   int holes = 0, movers = 0;
-  pool_pages(p, [&](int page, int refs) {
+  pool_pages(p, ctas, [&](int page, int refs) {
     holes += __popc(__ballot_sync(0xffffffffu, refs == 0 && page < used));
     movers += __popc(__ballot_sync(0xffffffffu, refs > 0 && page >= used));
   });
-  pool_order(s, turn, {holes, movers}, before, all);
+  pool_order(s, ctas, turn, {holes, movers}, before, all);
   int hole = before[0], mover = before[1];
-  pool_pages(p, [&](int page, int refs) {
+  pool_pages(p, ctas, [&](int page, int refs) {
     const uint32_t to = __ballot_sync(0xffffffffu, refs == 0 && page < used);
     const uint32_t of = __ballot_sync(0xffffffffu, refs > 0 && page >= used);
     if (refs == 0 && page < used) list[hole + __popc(to & below)] = page;
@@ -461,9 +485,9 @@ __global__ void __launch_bounds__(kPoolThreads, 1) kv8_compact_plan_kernel(const
     hole += __popc(to);
     mover += __popc(of);
   });
-  cluster_sync();
+  pool_sync(ctas);
   const int moves = all[1];
-  for (int k = static_cast<int>(cluster_ctarank()) * kPoolThreads + threadIdx.x; k < moves; k += kPoolCtas * kPoolThreads) {
+  for (int k = static_cast<int>(cluster_ctarank()) * kPoolThreads + threadIdx.x; k < moves; k += ctas * kPoolThreads) {
     const int to = __ldcg(list + k), of = __ldcg(list + p.pages - 1 - k);
     where[of] = to;
     p.refs[to] = __ldcg(p.refs + of);

@@ -5,13 +5,13 @@
 
 namespace {
 
-constexpr int kLrShared = 212 * 1024;  // most that a build asks for
+constexpr int kLrShared = 220 * 1024;  // most that a build asks for
 constexpr int kLrTwo = 110 * 1024;     // with which two CTAs share an SM
 
 template <int RT, int NT, bool F32>
 cudaError_t launch_low_rank(b200tx::LowRankArgs& a, DeviceState* dev, int index, cudaStream_t stream) {
   using S = b200tx::LrShape<RT, NT>;
-  static_assert(S::bytes(8) <= kLrShared, "the sums of eight CTAs do not fit");
+  static_assert(S::bytes(8, 3) <= kLrShared, "the sums of eight CTAs do not fit");
   if (!dev->low_rank_attr[index]) {
     cudaError_t err = cudaFuncSetAttribute(b200tx::low_rank_kernel<RT, NT, F32>,
                                            cudaFuncAttributeMaxDynamicSharedMemorySize, kLrShared);
@@ -26,12 +26,13 @@ cudaError_t launch_low_rank(b200tx::LowRankArgs& a, DeviceState* dev, int index,
   // CTAs of a group: as many as leave every SM two CTAs at most.
   int ctas = 8;
   while (ctas > 1 && windows * least * ctas > 2 * dev->sm_count) ctas /= 2;
-  const int resident = dev->sm_count * (S::bytes(ctas) <= kLrTwo ? 2 : 1);
+  const int bytes = S::bytes(ctas, a.out_f32 ? 3 : 2);
+  const int resident = dev->sm_count * (bytes <= kLrTwo ? 2 : 1);
   const int64_t tiles = (a.outer + b200tx::kLrTile - 1) / b200tx::kLrTile;
   a.parts = static_cast<int>((tiles + ctas * b200tx::kLrWarps - 1) / (ctas * b200tx::kLrWarps));
   a.clusters = static_cast<int>(std::min(std::max(least, resident / (ctas * windows)), most * a.parts));
   return launch_clustered(b200tx::low_rank_kernel<RT, NT, F32>, dim3(static_cast<unsigned>(windows * a.clusters * ctas)),
-                          dim3(b200tx::kLrThreads), static_cast<size_t>(S::bytes(ctas)), static_cast<unsigned>(ctas), stream, a);
+                          dim3(b200tx::kLrThreads), static_cast<size_t>(bytes), static_cast<unsigned>(ctas), stream, a);
 }
 
 template <int RT, int NT>
@@ -79,12 +80,23 @@ int low_log2(int64_t v) {
 
 constexpr int kPoolShared = 64 * 1024;  // of 2048 rows' records and places
 
+// CTAs for an order over so many pages and entries: one, without exchanges, while its
+// threads take few of them each.
+constexpr int64_t kPoolFew = 8192;
+unsigned pool_cluster(int64_t pages, int64_t entries) { return std::max(pages, entries) <= kPoolFew ? 1 : b200tx::kPoolCtas; }
+
 template <typename Kernel>
 cudaError_t pool_attribute(Kernel kernel, bool* done) {
   if (*done) return cudaSuccess;
   cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPoolShared);
   if (err == cudaSuccess) *done = true;
   return err;
+}
+
+template <typename T, bool VEC>
+cudaError_t launch_verify(b200tx::VerifyArgs& a, int64_t batch, cudaStream_t stream) {
+  return launch_clustered(b200tx::verify_draft_kernel<T, VEC>, dim3(static_cast<unsigned>(batch) * b200tx::kVerifyMostCtas),
+                          dim3(b200tx::kVerifyThreads), 0, b200tx::kVerifyMostCtas, stream, a);
 }
 
 }  // namespace
@@ -195,7 +207,8 @@ int b200tx_kv8_reserve(const b200tx_kv8_pool* pool, const int32_t* slot_ids, con
   if (missing == nullptr) return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_reserve: null result");
   if (slot_ids == nullptr && rows > a.pool.slots)
     return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_reserve: %lld sequences in a cache of %d slots", (long long)rows, a.pool.slots);
-  if (rows * std::min<int64_t>(a.pool.max_blocks, tokens / b200tx::kKv8Block + 1) > (1 << 30))
+  const int64_t entries = rows * std::min<int64_t>(a.pool.max_blocks, tokens / b200tx::kKv8Block + 1);
+  if (entries > (1 << 30))
     return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_reserve: too many blocks");
   DeviceState* dev = nullptr;
   rc = current_device(&dev);
@@ -207,9 +220,10 @@ int b200tx_kv8_reserve(const b200tx_kv8_pool* pool, const int32_t* slot_ids, con
   a.rows = static_cast<int>(rows);
   a.owners = slot_places(rows);
   cudaError_t err = pool_attribute(b200tx::kv8_reserve_kernel, &dev->reserve_attr);
+  const unsigned ctas = pool_cluster(a.pool.pages, entries);
   if (err == cudaSuccess)
-    err = launch_clustered(b200tx::kv8_reserve_kernel, dim3(b200tx::kPoolCtas), dim3(b200tx::kPoolThreads),
-                           static_cast<size_t>(12 * rows + 8 * a.owners), b200tx::kPoolCtas, stream, a);
+    err = launch_clustered(b200tx::kv8_reserve_kernel, dim3(ctas), dim3(b200tx::kPoolThreads),
+                           static_cast<size_t>(12 * rows + 8 * a.owners), ctas, stream, a);
   return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "kv8_reserve");
 }
 
@@ -226,8 +240,9 @@ int b200tx_kv8_compact(const b200tx_kv8_pool* pool, int32_t* used, cudaStream_t 
   constexpr int64_t kPiece = b200tx::kCompactThreads * b200tx::kCompactHeld * 16;
   a.piece = static_cast<int>(std::min(a.page_bytes, kPiece));
   a.pieces = static_cast<int>((a.page_bytes + a.piece - 1) / a.piece);
-  cudaError_t err = launch_clustered(b200tx::kv8_compact_plan_kernel, dim3(b200tx::kPoolCtas), dim3(b200tx::kPoolThreads), 0,
-                                     b200tx::kPoolCtas, stream, a);
+  const unsigned ctas = pool_cluster(a.pool.pages, 0);
+  cudaError_t err =
+      launch_clustered(b200tx::kv8_compact_plan_kernel, dim3(ctas), dim3(b200tx::kPoolThreads), 0, ctas, stream, a);
   if (err == cudaSuccess)
     err = launch(b200tx::kv8_compact_move_kernel, dim3(static_cast<unsigned>(4 * dev->sm_count)), dim3(b200tx::kCompactThreads),
                  0, stream, a);
@@ -263,14 +278,12 @@ int b200tx_verify_draft(const void* target, int64_t target_batch_stride, int64_t
   a.tokens = static_cast<int>(tokens);
   a.vocab = static_cast<int>(vocab);
   a.wide = drafted_64 != 0;
-  a.vec = aligned16(target) && (draft == nullptr || aligned16(draft)) &&
-          (target_batch_stride | target_token_stride | draft_batch_stride | draft_token_stride) % 4 == 0;
-  constexpr unsigned kCtas = 8;
-  const dim3 grid(static_cast<unsigned>(batch) * kCtas);
-  cudaError_t err = dtype == B200TX_F32
-                        ? launch_clustered(b200tx::verify_draft_kernel<float>, grid, dim3(b200tx::kVerifyThreads), 0, kCtas, stream, a)
-                        : launch_clustered(b200tx::verify_draft_kernel<__nv_bfloat16>, grid, dim3(b200tx::kVerifyThreads), 0,
-                                           kCtas, stream, a);
+  const int per = dtype == B200TX_F32 ? 4 : 8;  // values in 16 bytes
+  const bool vec = aligned16(target) && (draft == nullptr || aligned16(draft)) &&
+                   (target_batch_stride | target_token_stride | (draft == nullptr ? 0 : draft_batch_stride | draft_token_stride)) % per == 0;
+  cudaError_t err = dtype == B200TX_F32 ? vec ? launch_verify<float, true>(a, batch, stream) : launch_verify<float, false>(a, batch, stream)
+                    : vec               ? launch_verify<__nv_bfloat16, true>(a, batch, stream)
+                                        : launch_verify<__nv_bfloat16, false>(a, batch, stream);
   return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "verify_draft");
 }
 

@@ -10,7 +10,7 @@
 // which decides borders as the definition does.  The work is one row of p and of q a
 // sequence (not T + 1 of them): the row is known after one trip to memory for the drafts' tokens and one for
 // their probabilities.  A cluster takes a sequence: its CTAs sum stretches of the row,
-// exchange the sums, and the one CTA where the sum is passed looks through one stretch again.
+// exchange the sums, and the one CTA where the sum is passed looks through one warp's stretch again.
 #pragma once
 
 #include "sm100_common.cuh"
@@ -19,8 +19,9 @@ namespace b200tx {
 
 constexpr int kVerifyThreads = 256;
 constexpr int kVerifyWarps = kVerifyThreads / 32;
-constexpr int kVerifyParts = 64;     // stretches of a CTA's part of the row
+constexpr int kVerifyMostCtas = 8;
 constexpr int kVerifyTokens = 1024;  // drafted tokens of a sequence
+constexpr int kVerifyLook = 256;     // values that a warp looks through one by one
 
 struct VerifyArgs {
   const void* target;  // [batch, tokens + 1, vocab]
@@ -31,48 +32,117 @@ struct VerifyArgs {
   void* out;              // [batch, tokens + 1], drafted's type
   int32_t* accepted;      // [batch]
   int64_t target_batch_stride, target_token_stride, draft_batch_stride, draft_token_stride;
-  int tokens, vocab, bf16, wide, vec;
+  int tokens, vocab, wide;
 };
 
 template <typename T>
-__device__ __forceinline__ double verify_value(const T* p) {
+__device__ __forceinline__ float verify_value(const T* p) {
   if constexpr (sizeof(T) == 2)
-    return __uint_as_float(static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p)) << 16);
+    return __uint_as_float(static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(p))) << 16);
   else
-    return *p;
+    return __ldg(p);
 }
 
-// Four neighbouring values.
-template <typename T>
-__device__ __forceinline__ void verify_four(const T* p, bool vec, int valid, float (&v)[4]) {
-  if (vec && valid == 4) {
-    if constexpr (sizeof(T) == 2) {
-      const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
-      v[0] = __uint_as_float(w.x << 16), v[1] = __uint_as_float(w.x & 0xffff0000u);
-      v[2] = __uint_as_float(w.y << 16), v[3] = __uint_as_float(w.y & 0xffff0000u);
-    } else {
-      const float4 w = __ldg(reinterpret_cast<const float4*>(p));
-      v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
-    }
-    return;
+// A row's masses: what is left of p where the draft is refused.  A mass that is NaN counts as nothing.
+template <typename T, bool VEC>
+struct VerifyRow {
+  const T* p;
+  const T* q;    // or null
+  int excluded;  // a token whose mass is taken away whole, or -1
+
+  __device__ __forceinline__ double mass(float a, float b, int at) const {
+    const double d = static_cast<double>(a) - static_cast<double>(b);
+    return d > 0.0 && at != excluded ? d : 0.0;
   }
+
+  __device__ __forceinline__ double one(int at) const { return mass(verify_value(p + at), q == nullptr ? 0.f : verify_value(q + at), at); }
+
+  // Values that a lane reads at once, 16 bytes, or one where rows start anywhere.
+  static constexpr int PER = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
+
+  template <bool TWO>
+  __device__ __forceinline__ double sum_of(int from, int to) const {
+    constexpr int U = VEC ? 4 : 16, STEP = 32 * PER;
+    const int lane = threadIdx.x % 32;
+    double sum = 0.0, other = 0.0;  // two sums, for the latency of an addition
+    int at = from + lane * PER;
+    if constexpr (VEC) {
+      // whole steps, their loads together
+      for (; at + (U - 1) * STEP + PER <= to; at += U * STEP) {
+        uint4 v[U], w[U];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = i < valid ? static_cast<float>(verify_value<T>(p + i)) : 0.f;
+        for (int u = 0; u < U; ++u) {
+          v[u] = __ldg(reinterpret_cast<const uint4*>(p + at + u * STEP));
+          if (TWO) w[u] = __ldg(reinterpret_cast<const uint4*>(q + at + u * STEP));
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const uint32_t x[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+          const uint32_t y[4] = {TWO ? w[u].x : 0u, TWO ? w[u].y : 0u, TWO ? w[u].z : 0u, TWO ? w[u].w : 0u};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int where = at + u * STEP;
+            if constexpr (sizeof(T) == 2) {
+              sum += mass(__uint_as_float(x[i] << 16), __uint_as_float(y[i] << 16), where + 2 * i);
+              other += mass(__uint_as_float(x[i] & 0xffff0000u), __uint_as_float(y[i] & 0xffff0000u), where + 2 * i + 1);
+            } else if (i % 2) {
+              other += mass(__uint_as_float(x[i]), __uint_as_float(y[i]), where + i);
+            } else {
+              sum += mass(__uint_as_float(x[i]), __uint_as_float(y[i]), where + i);
+            }
+          }
+        }
+      }
+    } else {
+      for (; at + (U - 1) * STEP < to; at += U * STEP) {
+        float v[U], w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          v[u] = verify_value(p + at + u * STEP);
+          w[u] = TWO ? verify_value(q + at + u * STEP) : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) (u % 2 ? other : sum) += mass(v[u], w[u], at + u * STEP);
+      }
+    }
+    for (; at < to; at += STEP) {
+      for (int i = 0; i < PER && at + i < to; ++i) sum += one(at + i);
+    }
+    sum += other;
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    return sum;
+  }
+
+  // The masses from..to - 1 summed by a warp; the same in all lanes.
+  __device__ __forceinline__ double sum(int from, int to) const {
+    return q != nullptr ? sum_of<true>(from, to) : sum_of<false>(from, to);
+  }
+};
+
+// Of n sums in order the one in which the running sum passes `wanted`; where rounding, or a wish past the whole, leaves
+// none, the last with mass, and from then on.
+__device__ __forceinline__ int verify_pick(const double* sums, int n, double& running, double& wanted) {
+  int last = 0;
+  double before = running;
+  for (int i = 0; i < n; ++i) {
+    if (running + sums[i] > wanted) return i;
+    if (sums[i] > 0.0) {
+      last = i;
+      before = running;
+    }
+    running += sums[i];
+  }
+  running = before;
+  wanted = __longlong_as_double(0x7ff0000000000000ll);
+  return last;
 }
 
-// The mass of token i of four: what is left of p where the draft is refused.  NaN counts as nothing.
-__device__ __forceinline__ double verify_mass(float p, float q) {
-  const double d = static_cast<double>(p) - static_cast<double>(q);
-  return d > 0.0 ? d : 0.0;
-}
-
-template <typename T>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(kVerifyThreads) verify_draft_kernel(const __grid_constant__ VerifyArgs a) {
-  __shared__ int s_first, s_token;
-  __shared__ double s_part[kVerifyParts];
-  __shared__ double s_cta[2][8];
-  __shared__ int s_last[2][8];  // the last index of a CTA's part with mass, -1: none
-  __shared__ int s_warp_last[kVerifyWarps];
+  __shared__ int s_first;
+  __shared__ double s_part[2][kVerifyWarps];
+  __shared__ double s_cta[2][kVerifyMostCtas];
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   uint32_t ctas;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
@@ -85,6 +155,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_draft_kernel(const __gr
   const T* const target = static_cast<const T*>(a.target) + b * a.target_batch_stride;
   const T* const draft = a.draft == nullptr ? nullptr : static_cast<const T*>(a.draft) + b * a.draft_batch_stride;
   const float* const uniform = a.uniform + b * (a.tokens + 1);
+  const double u = fmax(static_cast<double>(uniform[a.tokens]), 0.0);
   const int n = a.counts == nullptr ? a.tokens : min(max(a.counts[b], 0), a.tokens);
   auto drafted = [&](int t) -> int64_t {
     const int64_t at = b * a.tokens + t;
@@ -93,143 +164,105 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_draft_kernel(const __gr
   if (tid == 0) s_first = n;
   __syncthreads();
   for (int t = tid; t < n; t += kVerifyThreads) {
+    const float mine = uniform[t];
     const int64_t token = drafted(t);
     bool good = false;  // a token outside of the vocabulary is refused
     if (token >= 0 && token < a.vocab) {
       const double p = verify_value<T>(target + t * a.target_token_stride + token);
-      const double q = draft == nullptr ? 1.0 : verify_value<T>(draft + t * a.draft_token_stride + token);
-      good = static_cast<double>(uniform[t]) * q < p;
+      const double q = draft == nullptr ? 1.0 : static_cast<double>(verify_value<T>(draft + t * a.draft_token_stride + token));
+      good = static_cast<double>(mine) * q < p;
     }
     if (!good) atomicMin(&s_first, t);
   }
   __syncthreads();
   const int first = s_first;
   const bool refused = first < n;
-  const int64_t token = refused ? drafted(first) : -1;
-  const T* const p_row = target + first * a.target_token_stride;
-  const T* const q_row = refused && draft != nullptr ? draft + first * a.draft_token_stride : nullptr;
-  const double u = fmax(static_cast<double>(uniform[a.tokens]), 0.0);
+  VerifyRow<T, VEC> row;
+  row.p = target + first * a.target_token_stride;
+  row.q = nullptr;
+  row.excluded = -1;
+  if (refused && draft != nullptr) row.q = draft + first * a.draft_token_stride;
+  if (refused && draft == nullptr) {
+    const int64_t token = drafted(first);
+    row.excluded = token >= 0 && token < a.vocab ? static_cast<int>(token) : -1;
+  }
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 
-  // stretches: parts of the row for CTAs, of these for warps, whole fours for 32 lanes
-  const int stretch = static_cast<int>((static_cast<int64_t>(a.vocab) + C * kVerifyParts * 128 - 1) / (C * kVerifyParts * 128)) * 128;
-  const int begin = min(static_cast<int64_t>(a.vocab), static_cast<int64_t>(c) * kVerifyParts * stretch);
+  // a part of the row for each warp of the cluster, in order
+  const int64_t parts = C * kVerifyWarps;
+  int length = static_cast<int>((a.vocab + parts * 256 - 1) / (parts * 256) * 256);
+  auto end = [&](int64_t from, int64_t many) { return static_cast<int>(min(static_cast<int64_t>(a.vocab), from + many)); };
+  double all = 0.0;
+  int turn = 0;
   // what is left of p; where nothing is, p itself
-  for (int whole = refused ? 0 : 1; whole < 2; ++whole) {
-    auto mass_of = [&](int at, float (&v)[4], double (&mass)[4]) {
-      const int valid = min(max(a.vocab - at, 0), 4);
-      float q[4] = {};
-      verify_four<T>(p_row + at, a.vec, valid, v);
-      if (whole == 0 && q_row != nullptr) verify_four<T>(q_row + at, a.vec, valid, q);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        mass[i] = whole == 0 && q_row == nullptr && at + i == token ? 0.0 : verify_mass(v[i], q[i]);
-    };
-    int last = -1;
-    for (int part = warp; part < kVerifyParts; part += kVerifyWarps) {
-      double sum = 0.0;
-      const int64_t from = begin + static_cast<int64_t>(part) * stretch, to = min(static_cast<int64_t>(a.vocab), from + stretch);
-#pragma unroll 4
-      for (int64_t at = from + lane * 4; at < to; at += 128) {
-        float v[4];
-        double mass[4];
-        mass_of(static_cast<int>(at), v, mass);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          sum += mass[i];
-          if (mass[i] > 0.0) last = static_cast<int>(at) + i;
-        }
-      }
-#pragma unroll
-      for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      if (lane == 0) s_part[part] = sum;
-    }
-    last = __reduce_max_sync(0xffffffffu, last);
-    if (lane == 0) s_warp_last[warp] = last;
+  for (;; ++turn) {
+    const int64_t from = static_cast<int64_t>(c * kVerifyWarps + warp) * length;
+    const double sum = from < a.vocab ? row.sum(static_cast<int>(from), end(from, length)) : 0.0;
+    if (lane == 0) s_part[0][warp] = sum;
     __syncthreads();
-    if (warp == 0) {
-      double sum = 0.0;
-      for (int i = 0; i < kVerifyParts; ++i) sum += s_part[i];
-      int most = -1;
-      for (int i = 0; i < kVerifyWarps; ++i) most = max(most, s_warp_last[i]);
-      if (lane < C) {
-        asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(peer_smem_addr(&s_cta[whole][c], lane)), "d"(sum) : "memory");
-        asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(peer_smem_addr(&s_last[whole][c], lane)), "r"(most) : "memory");
-      }
+    if (warp == 0 && lane < C) {
+      double mine = 0.0;
+      for (int i = 0; i < kVerifyWarps; ++i) mine += s_part[0][i];
+      asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(peer_smem_addr(&s_cta[turn][c], lane)), "d"(mine) : "memory");
     }
     cluster_sync();
-    double all = 0.0;
-    int end = -1;
-    for (int i = 0; i < C; ++i) {
-      all += s_cta[whole][i];
-      end = max(end, s_last[whole][i]);
-    }
-    if (end < 0 && whole == 0) continue;  // the same in every CTA
-    const double wanted = u * all;
-    // the first CTA in which the running sum passes what is wanted; if none, the last index with mass
-    double running = 0.0;
-    int owner = -1;
-    for (int i = 0; i < C; ++i) {
-      if (running + s_cta[whole][i] > wanted) {
-        owner = i;
-        break;
-      }
-      running += s_cta[whole][i];
-    }
-    if (owner < 0) {
-      if (c == 0 && tid == 0) s_token = end;
-      owner = 0;
-    } else if (owner == c && warp == 0) {
-      int part = 0;
-      for (; part < kVerifyParts - 1; ++part) {
-        if (running + s_part[part] > wanted) break;
-        running += s_part[part];
-      }
-      // 128 values at a time, in order
-      int found = -1, latest = -1;
-      const int64_t from = begin + static_cast<int64_t>(part) * stretch, to = min(static_cast<int64_t>(a.vocab), from + stretch);
-      for (int64_t base = from; base < to && found < 0; base += 128) {
-        float v[4];
-        double mass[4];
-        const int at = static_cast<int>(base) + lane * 4;
-        mass_of(at, v, mass);
-        const double mine = mass[0] + mass[1] + mass[2] + mass[3];
-        double sum = mine;
-#pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
-          const double o = __shfl_up_sync(0xffffffffu, sum, d);
-          if (lane >= d) sum += o;
-        }
-        double at_sum = running + (sum - mine);
-        int here = -1, held = -1;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          at_sum += mass[i];
-          if (mass[i] > 0.0) held = at + i;
-          if (here < 0 && mass[i] > 0.0 && at_sum > wanted) here = at + i;
-        }
-        const uint32_t bits = __ballot_sync(0xffffffffu, here >= 0);
-        if (bits != 0) found = __shfl_sync(0xffffffffu, here, __ffs(bits) - 1);
-        latest = max(latest, __reduce_max_sync(0xffffffffu, held));
-        running += __shfl_sync(0xffffffffu, sum, 31);
-      }
-      // rounding may leave the sum of one's parts short of their total: then the last with mass is it
-      if (lane == 0) s_token = found >= 0 ? found : latest >= 0 ? latest : s_last[whole][c];
-    }
-    __syncthreads();
-    if (owner == c) {
-      for (int t = tid; t <= a.tokens; t += kVerifyThreads) {
-        const int64_t value = t < first ? drafted(t) : t == first ? s_token : -1;
-        const int64_t at = b * (a.tokens + 1) + t;
-        if (a.wide)
-          static_cast<int64_t*>(a.out)[at] = value;
-        else
-          static_cast<int32_t*>(a.out)[at] = static_cast<int32_t>(value);
-      }
-      if (tid == 0) a.accepted[b] = first;
-    }
-    return;
+    all = 0.0;
+    for (int i = 0; i < C; ++i) all += s_cta[turn][i];
+    if (turn == 1 || (row.q == nullptr && row.excluded < 0) || all > 0.0) break;  // the same in every CTA
+    row.q = nullptr;
+    row.excluded = -1;
   }
+  double wanted = u * all, running = 0.0;
+  if (verify_pick(s_cta[turn], C, running, wanted) != c) return;
+
+  int64_t token = -1;
+  if (all > 0.0) {
+    // a part, the eighth of it, and so on, until a warp looks through what is left
+    int pick = verify_pick(s_part[0], kVerifyWarps, running, wanted);
+    int64_t from = static_cast<int64_t>(c * kVerifyWarps + pick) * length;
+    int limit = end(from, length);
+    for (int level = 1; length > kVerifyLook; ++level) {
+      length = (length + kVerifyWarps * 256 - 1) / (kVerifyWarps * 256) * 256;
+      const int64_t mine = from + static_cast<int64_t>(warp) * length;
+      const double sum = mine < limit ? row.sum(static_cast<int>(mine), min(limit, end(mine, length))) : 0.0;
+      if (lane == 0) s_part[level & 1][warp] = sum;
+      __syncthreads();
+      pick = verify_pick(s_part[level & 1], kVerifyWarps, running, wanted);
+      from += static_cast<int64_t>(pick) * length;
+      limit = min(limit, end(from, length));
+    }
+    double mass[kVerifyLook / 32];
+    int latest = -1, found = -1;
+#pragma unroll
+    for (int i = 0; i < kVerifyLook / 32; ++i) {
+      const int64_t at = from + i * 32 + lane;
+      mass[i] = at < limit ? row.one(static_cast<int>(at)) : 0.0;
+    }
+#pragma unroll
+    for (int i = 0; i < kVerifyLook / 32; ++i) {
+      double sum = mass[i];
+#pragma unroll
+      for (int d = 1; d < 32; d *= 2) {
+        const double o = __shfl_up_sync(0xffffffffu, sum, d);
+        if (lane >= d) sum += o;
+      }
+      const uint32_t passed = __ballot_sync(0xffffffffu, mass[i] > 0.0 && running + sum > wanted);
+      const uint32_t held = __ballot_sync(0xffffffffu, mass[i] > 0.0);
+      if (found < 0 && passed != 0) found = i * 32 + __ffs(passed) - 1;
+      if (held != 0) latest = i * 32 + 31 - __clz(held);
+      running += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    token = from + (found >= 0 ? found : latest);
+  }
+  for (int t = tid; t <= a.tokens; t += kVerifyThreads) {
+    const int64_t value = t < first ? drafted(t) : t == first ? token : -1;
+    const int64_t at = b * (a.tokens + 1) + t;
+    if (a.wide)
+      static_cast<int64_t*>(a.out)[at] = value;
+    else
+      static_cast<int32_t*>(a.out)[at] = static_cast<int32_t>(value);
+  }
+  if (tid == 0) a.accepted[b] = first;
 }
 
 }  // namespace b200tx
