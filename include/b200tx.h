@@ -535,7 +535,7 @@ int b200tx_low_rank_add(const void* x, const void* base, int base_dtype, void* o
 
 /* The pages of an 8-bit cache, all layers: layer 0's view (the layers of codes, scales and tail follow
  * one another without gaps; page_table and lengths are written here), refs[page] = the entries of the page
- * table that hold the page (0: it is free), and scratch, b200tx_kv8_pool_scratch ints, zeroed once.
+ * table that hold the page (0: it is free), and scratch, b200tx_kv8_pool_scratch ints, zeroed once; both 16-byte aligned.
  * One call at a time works on a pool: calls, and replays of graphs that hold them, follow one
  * another. */
 typedef struct b200tx_kv8_pool {

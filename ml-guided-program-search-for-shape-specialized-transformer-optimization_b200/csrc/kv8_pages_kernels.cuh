@@ -63,15 +63,20 @@ struct Kv8ForkArgs {
   const int32_t* target;  // [pairs]
   int pairs;
   int owners;             // places of the table of slots, a power of two
+  int region_log2;        // log2 of the pieces of a head's block
   int piece_shift;        // log2 of the pieces of a pair in a tail item
   int column_shift;       // log2 of the columns in a table item
   int tail_items, table_items;
 };
 
-struct ForkPair {
-  int source, target;  // target -1: the pair does nothing; source -1: from nothing
-  int full;            // full blocks of the source
-  int held;            // tokens of the source
+struct __align__(16) ForkPair {
+  uint32_t from, to;  // the block's place in the source's and in the target's tail: 16-byte pieces from the layer's first slot
+  int pieces;         // of the open block in a head, 0: there is nothing to copy
+  int target;         // -1: the pair does nothing
+  int source;         // -1: from nothing
+  int full;           // full blocks of the source
+  int held;           // tokens of the source
+  int unused;
 };
 
 // All pairs at once: every target becomes what its source was before the call.  An item is
@@ -80,7 +85,7 @@ struct ForkPair {
 // target of another (beams that are put in a new order).
 __global__ void __launch_bounds__(kForkThreads, 3) kv8_fork_kernel(const __grid_constant__ Kv8ForkArgs a) {
   extern __shared__ __align__(16) uint8_t fork_smem[];
-  __shared__ int s_last;
+  __shared__ int s_last, s_most;
   ForkPair* const pair = reinterpret_cast<ForkPair*>(fork_smem);
   SlotOwners owners;
   owners.slots = reinterpret_cast<int*>(pair + a.pairs);
@@ -98,11 +103,15 @@ __global__ void __launch_bounds__(kForkThreads, 3) kv8_fork_kernel(const __grid_
     if (target >= 0 && target < p.slots) atomicMax(owners.rows + owners.place(target), i);
   }
   __syncthreads();
+  const int row = p.dim / 8;           // 16-byte pieces of a token's head
+  const int region = kKv8Block * row;  // of a head's block
+  const int heads = 2 * p.kv_heads;
+  const uint32_t of_parity = static_cast<uint32_t>(heads) * region;  // of a slot's blocks of one parity
+  int most = 0;  // pieces of the longest open block
   for (int i = tid; i < a.pairs; i += kForkThreads) {
-    ForkPair f;
+    ForkPair f = {};
     f.source = a.source == nullptr ? -1 : a.source[i];
     f.target = a.target[i];
-    f.full = f.held = 0;
     const bool known = f.target >= 0 && f.target < p.slots && f.source < p.slots;
     // a sequence that becomes itself stays as it is, with the pages that are reserved for it
     if (!known || f.source == f.target || owners.rows[owners.place(f.target)] != i) {
@@ -110,65 +119,69 @@ __global__ void __launch_bounds__(kForkThreads, 3) kv8_fork_kernel(const __grid_
     } else if (f.source >= 0) {
       f.held = max(0, p.lengths[f.source]);
       f.full = min(f.held / kKv8Block, p.max_blocks);
+      const uint32_t parity = f.held / kKv8Block & 1;
+      f.from = (2u * f.source + parity) * of_parity;
+      f.to = (2u * f.target + parity) * of_parity;
+      f.pieces = f.held % kKv8Block * row;
     } else {
       f.source = -1;
     }
     pair[i] = f;
+    most = max(most, f.pieces);
   }
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (tid == 0) s_most = 0;
   __syncthreads();
+  if (tid % 32 == 0) atomicMax(&s_most, most);
+  __syncthreads();
+  most = s_most;
 
-  const int row = p.dim / 8;                 // 16-byte pieces of a token's head
-  const int region = kKv8Block * row;        // of a head's block
-  const int each = 1 << a.piece_shift, pieces = region >> a.piece_shift, heads = 2 * p.kv_heads;
-  const uint32_t parity_pieces = static_cast<uint32_t>(heads) * region;  // of a slot's blocks of one parity
+  const int each = 1 << a.piece_shift, pieces_log2 = a.region_log2 - a.piece_shift;
   for (int item = blockIdx.x; item < a.tail_items + a.table_items; item += gridDim.x) {
     if (item < a.tail_items) {
-      const int part = item % pieces, rest = item / pieces;
-      const int head = rest % heads, layer = rest / heads;
-      uint4* const base = p.tail + static_cast<int64_t>(layer) * p.slots * 2 * parity_pieces + static_cast<int64_t>(head) * region;
-      // a piece's place in a slot, the same for all of a thread's pairs where an item has up to 256 pieces of each
-      auto place = [&](int j) { return part * each + ((j * kForkThreads + tid) & (each - 1)); };
-      auto open = [&](const ForkPair& f, int at) { return f.target >= 0 && at < f.held % kKv8Block * row; };
+      const int part = (item & ((1 << pieces_log2) - 1)) << a.piece_shift;
+      if (part >= most) continue;  // past every open block
+      const int rest = item >> pieces_log2, layer = rest / heads, head = rest - layer * heads;
+      uint4* const base = p.tail + static_cast<int64_t>(layer) * p.slots * 2 * of_parity + static_cast<int64_t>(head) * region;
       uint4 v[kForkHeld];
+      uint32_t to[kForkHeld];
 #pragma unroll
       for (int j = 0; j < kForkHeld; ++j) {
-        const int i = (j * kForkThreads + tid) >> a.piece_shift, at = place(j);
+        const int e = j * kForkThreads + tid, i = e >> a.piece_shift, at = part + (e & (each - 1));
+        to[j] = 0xffffffffu;
         if (i >= a.pairs) continue;
-        const ForkPair f = pair[i];
-        if (open(f, at)) v[j] = base[static_cast<uint64_t>(2 * f.source + (f.held / kKv8Block & 1)) * parity_pieces + at];
+        const int4 f = *reinterpret_cast<const int4*>(pair + i);
+        if (at >= f.z) continue;
+        v[j] = base[static_cast<uint32_t>(f.x) + at];
+        to[j] = static_cast<uint32_t>(f.y) + at;
       }
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < kForkHeld; ++j) {
-        const int i = (j * kForkThreads + tid) >> a.piece_shift, at = place(j);
-        if (i >= a.pairs) continue;
-        const ForkPair f = pair[i];
-        if (open(f, at)) base[static_cast<uint64_t>(2 * f.target + (f.held / kKv8Block & 1)) * parity_pieces + at] = v[j];
-      }
+      for (int j = 0; j < kForkHeld; ++j)
+        if (to[j] != 0xffffffffu) base[to[j]] = v[j];
     } else {
       const int columns = 1 << a.column_shift, from = (item - a.tail_items) << a.column_shift;
-      int page[kForkHeld];
+      int now[kForkHeld], before[kForkHeld];
+      int32_t* entry[kForkHeld];
 #pragma unroll
       for (int j = 0; j < kForkHeld; ++j) {
         const int e = j * kForkThreads + tid, i = e >> a.column_shift, block = from + (e & (columns - 1));
-        page[j] = -1;
-        if (i >= a.pairs || block >= p.max_blocks) continue;
-        const ForkPair f = pair[i];
-        if (f.target < 0 || f.source < 0 || block >= f.full) continue;
-        const int found = p.page_table[static_cast<int64_t>(f.source) * p.max_blocks + block];
-        if (found >= 0 && found < p.pages) page[j] = found;
+        now[j] = before[j] = -1;
+        entry[j] = nullptr;
+        if (i >= a.pairs || block >= p.max_blocks || pair[i].target < 0) continue;
+        entry[j] = p.page_table + static_cast<int64_t>(pair[i].target) * p.max_blocks + block;
+        before[j] = __ldcg(entry[j]);
+        if (block < pair[i].full) now[j] = __ldcg(p.page_table + static_cast<int64_t>(pair[i].source) * p.max_blocks + block);
       }
       __syncthreads();
 #pragma unroll
       for (int j = 0; j < kForkHeld; ++j) {
-        const int e = j * kForkThreads + tid, i = e >> a.column_shift, block = from + (e & (columns - 1));
-        if (i >= a.pairs || block >= p.max_blocks || pair[i].target < 0) continue;
-        int32_t* const entry = p.page_table + static_cast<int64_t>(pair[i].target) * p.max_blocks + block;
-        const int before = *entry;
-        if (before == page[j]) continue;
-        if (before >= 0 && before < p.pages) atomicSub(p.refs + before, 1);
-        if (page[j] >= 0) atomicAdd(p.refs + page[j], 1);
-        *entry = page[j];
+        if (entry[j] == nullptr) continue;
+        if (now[j] < 0 || now[j] >= p.pages) now[j] = -1;
+        if (before[j] == now[j]) continue;
+        if (before[j] >= 0 && before[j] < p.pages) atomicSub(p.refs + before[j], 1);
+        if (now[j] >= 0) atomicAdd(p.refs + now[j], 1);
+        *entry[j] = now[j];
       }
     }
   }
@@ -239,26 +252,52 @@ __device__ __forceinline__ void pool_order(PoolShared& s, int ctas, int& turn, c
   }
 }
 
-// Calls f(page, refs) for this warp's stretch of the pages, 32 neighbouring pages at a time (all lanes
-// call; past the end refs is -1).
+// Calls f(page, refs[4]) for this warp's stretch of the pages: four neighbours a lane, 128 a warp, all lanes
+// together; refs past the end is -1.
 template <typename F>
 __device__ __forceinline__ void pool_pages(const Kv8Pool& p, int ctas, F f) {
-  const int warps = ctas * kPoolWarps;
-  const int64_t each = ((p.pages + 31) / 32 + warps - 1) / warps * 32;
-  const int64_t from = each * (cluster_ctarank() * kPoolWarps + threadIdx.x / 32);
-  constexpr int U = 8;
-  for (int64_t at = from; at < min(from + each, p.pages); at += U * 32) {
-    int refs[U];
+  const int pages = static_cast<int>(p.pages), warps = ctas * kPoolWarps;
+  const int each = ((pages + 127) / 128 + warps - 1) / warps * 128;
+  const int from = static_cast<int>(min(static_cast<int64_t>(pages), static_cast<int64_t>(each) * (cluster_ctarank() * kPoolWarps + threadIdx.x / 32)));
+  const int to = min(pages, from + each);
+  constexpr int U = 4;
+  for (int at = from; at < to; at += U * 128) {
+    int4 refs[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t page = at + u * 32 + threadIdx.x % 32;
-      refs[u] = page < p.pages && at + u * 32 < from + each ? max(0, __ldcg(p.refs + page)) : -1;
+      const int page = at + u * 128 + threadIdx.x % 32 * 4;
+      refs[u] = make_int4(-1, -1, -1, -1);
+      if (page + 4 <= to) {
+        refs[u] = __ldcg(reinterpret_cast<const int4*>(p.refs + page));
+      } else {
+        if (page < to) refs[u].x = __ldcg(p.refs + page);
+        if (page + 1 < to) refs[u].y = __ldcg(p.refs + page + 1);
+        if (page + 2 < to) refs[u].z = __ldcg(p.refs + page + 2);
+      }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (at + u * 32 < min(from + each, p.pages)) f(static_cast<int>(at + u * 32 + threadIdx.x % 32), refs[u]);
+      if (at + u * 128 >= to) break;
+      const int page = at + u * 128 + threadIdx.x % 32 * 4;
+      int four[4] = {refs[u].x, refs[u].y, refs[u].z, refs[u].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) four[i] = page + i < to ? max(0, four[i]) : -1;
+      f(page, four);
     }
   }
+}
+
+// The sum of the lanes' counts before this one; `total` of all.
+__device__ __forceinline__ int lanes_before(int count, int& total) {
+  const int lane = threadIdx.x % 32;
+  int sum = count;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int o = __shfl_up_sync(0xffffffffu, sum, d);
+    if (lane >= d) sum += o;
+  }
+  total = __shfl_sync(0xffffffffu, sum, 31);
+  return sum - count;
 }
 
 // ------------------------------------------------------------------ reserve
@@ -347,7 +386,21 @@ __global__ void __launch_bounds__(kPoolThreads, 1) kv8_reserve_kernel(const __gr
   const int first = each * (me * kPoolWarps + warp), last = min(first + each, all_entries);
   constexpr int U = 4;
   // f(page, entry, row, whether there is one) for each entry with its page, all lanes
+  auto row_of = [&](int entry, int lo, int hi) {
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (upto[mid] > entry)
+        hi = mid;
+      else
+        lo = mid + 1;
+    }
+    return lo;
+  };
+  // the rows of this warp's first and last entry: mostly one, or two
+  const int row0 = first < last ? row_of(first, 0, a.rows - 1) : 0;
+  const int row1 = first < last ? row_of(last - 1, row0, a.rows - 1) : 0;
   auto entries = [&](auto f) {
+    int near = row0;
     for (int at = first; at < last; at += 32 * U) {
       int row[U], page[U];
       int32_t* entry[U];
@@ -357,16 +410,9 @@ __global__ void __launch_bounds__(kPoolThreads, 1) kv8_reserve_kernel(const __gr
         entry[u] = nullptr;
         row[u] = page[u] = 0;
         if (e >= last) continue;
-        int lo = 0, hi = a.rows - 1;
-        while (lo < hi) {
-          const int mid = (lo + hi) / 2;
-          if (upto[mid] > e)
-            hi = mid;
-          else
-            lo = mid + 1;
-        }
-        row[u] = lo;
-        entry[u] = p.page_table + static_cast<int64_t>(slot_of[lo]) * p.max_blocks + begin[lo] + (e - (lo == 0 ? 0 : upto[lo - 1]));
+        near = row_of(e, near, row1);
+        row[u] = near;
+        entry[u] = p.page_table + static_cast<int64_t>(slot_of[near]) * p.max_blocks + begin[near] + (e - (near == 0 ? 0 : upto[near - 1]));
         page[u] = *entry[u];
       }
       f(page, entry, row);
@@ -403,17 +449,25 @@ __global__ void __launch_bounds__(kPoolThreads, 1) kv8_reserve_kernel(const __gr
   }
 
   int free_pages = 0;
-  pool_pages(p, ctas, [&](int, int refs) { free_pages += __popc(__ballot_sync(0xffffffffu, refs == 0)); });
+  pool_pages(p, ctas, [&](int, int (&refs)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) free_pages += refs[i] == 0;
+  });
+  free_pages = __reduce_add_sync(0xffffffffu, free_pages);
   int free_before[1], free_all[1];
   pool_order(s, ctas, turn, {free_pages}, free_before, free_all);
   int32_t* const list = p.scratch + kPoolCounters;
   int at_free = free_before[0];
   if (at_free < all[0]) {
-    pool_pages(p, ctas, [&](int page, int refs) {
-      const uint32_t bits = __ballot_sync(0xffffffffu, refs == 0);
-      const int k = at_free + __popc(bits & ((1u << lane) - 1));
-      if (refs == 0 && k < all[0]) list[k] = page;
-      at_free += __popc(bits);
+    pool_pages(p, ctas, [&](int page, int (&refs)[4]) {
+      int total, k = at_free + lanes_before((refs[0] == 0) + (refs[1] == 0) + (refs[2] == 0) + (refs[3] == 0), total);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (refs[i] != 0) continue;
+        if (k < all[0]) list[k] = page + i;
+        ++k;
+      }
+      at_free += total;
     });
   }
   pool_sync(ctas);
@@ -455,8 +509,6 @@ struct Kv8CompactArgs {
 __global__ void __launch_bounds__(kPoolThreads, 1) kv8_compact_plan_kernel(const __grid_constant__ Kv8CompactArgs a) {
   __shared__ PoolShared s;
   const Kv8Pool& p = a.pool;
-  const int lane = threadIdx.x % 32;
-  const uint32_t below = (1u << lane) - 1;
   int32_t* const where = p.scratch + kPoolCounters;
   int32_t* const list = where + p.pages;  // holes from the front, movers from the back: not more than the pages
   int turn = 0;
@@ -465,25 +517,44 @@ __global__ void __launch_bounds__(kPoolThreads, 1) kv8_compact_plan_kernel(const
   griddep_wait();
   griddep_launch_dependents();
   int held = 0;
-  pool_pages(p, ctas, [&](int, int refs) { held += __popc(__ballot_sync(0xffffffffu, refs > 0)); });
+  pool_pages(p, ctas, [&](int, int (&refs)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) held += refs[i] > 0;
+  });
+  held = __reduce_add_sync(0xffffffffu, held);
   int before[2], all[2], none[1], in_use[1];
   pool_order(s, ctas, turn, {held}, none, in_use);
   const int used = in_use[0];
+  auto hole_at = [&](int page, int refs) { return refs == 0 && page < used; };
+  auto mover_at = [&](int page, int refs) { return refs > 0 && page >= used; };
   int holes = 0, movers = 0;
-  pool_pages(p, ctas, [&](int page, int refs) {
-    holes += __popc(__ballot_sync(0xffffffffu, refs == 0 && page < used));
-    movers += __popc(__ballot_sync(0xffffffffu, refs > 0 && page >= used));
+  pool_pages(p, ctas, [&](int page, int (&refs)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      holes += hole_at(page + i, refs[i]);
+      movers += mover_at(page + i, refs[i]);
+    }
   });
-  pool_order(s, ctas, turn, {holes, movers}, before, all);
+  pool_order(s, ctas, turn, {__reduce_add_sync(0xffffffffu, holes), __reduce_add_sync(0xffffffffu, movers)}, before, all);
   int hole = before[0], mover = before[1];
-  pool_pages(p, ctas, [&](int page, int refs) {
-    const uint32_t to = __ballot_sync(0xffffffffu, refs == 0 && page < used);
-    const uint32_t of = __ballot_sync(0xffffffffu, refs > 0 && page >= used);
-    if (refs == 0 && page < used) list[hole + __popc(to & below)] = page;
-    if (refs > 0 && page >= used) list[p.pages - 1 - (mover + __popc(of & below))] = page;
-    if (refs >= 0) where[page] = refs > 0 && page < used ? page : -1;
-    hole += __popc(to);
-    mover += __popc(of);
+  pool_pages(p, ctas, [&](int page, int (&refs)[4]) {
+    int to = 0, of = 0, all_to, all_of;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      to += hole_at(page + i, refs[i]);
+      of += mover_at(page + i, refs[i]);
+    }
+    to = hole + lanes_before(to, all_to);
+    of = mover + lanes_before(of, all_of);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (refs[i] < 0) continue;
+      if (hole_at(page + i, refs[i])) list[to++] = page + i;
+      if (mover_at(page + i, refs[i])) list[p.pages - 1 - of++] = page + i;
+      where[page + i] = refs[i] > 0 && page + i < used ? page + i : -1;
+    }
+    hole += all_to;
+    mover += all_of;
   });
   pool_sync(ctas);
   const int moves = all[1];

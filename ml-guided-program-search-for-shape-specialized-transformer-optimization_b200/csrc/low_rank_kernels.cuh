@@ -51,6 +51,7 @@ struct LowRankArgs {
   int64_t rows;
   int per_index, inner, outer, rank, count;
   int out_f32, gelu;
+  int group;        // most rows of a group
   int clusters;     // for each window
   int parts;        // most that the columns are cut into between clusters
   int skip_bare;    // out is base and has nothing done to it where there is no adapter
@@ -83,7 +84,7 @@ struct LrGroups {
     }
     const uint32_t same = __match_any_sync(0xffffffffu, mine);
     before += __popc(same & ((1u << lane) - 1));
-    const bool leads = tid < n && before % G == 0;
+    const bool leads = tid < n && before % a.group == 0;
     const uint32_t leaders = __ballot_sync(0xffffffffu, leads);
     rank[tid] = before;
     if (lane == 0) warp_leads[warp] = __popc(leaders);
@@ -100,9 +101,9 @@ struct LrGroups {
   }
 
   // Fills `rows` with the group's; all threads, which are done with the one before.  Returns how many.
-  __device__ __forceinline__ int take(int group, int n) {
+  __device__ __forceinline__ int take(int group, int n, int most) {
     const int tid = threadIdx.x, leader = lead[group], adapter = key[leader], from = rank[leader];
-    const bool in = tid < n && key[tid] == adapter && rank[tid] >= from && rank[tid] < from + G;
+    const bool in = tid < n && key[tid] == adapter && rank[tid] >= from && rank[tid] < from + most;
     if (tid < G) rows[tid] = -1;
     const int many = __syncthreads_count(in);
     if (in) rows[rank[tid] - from] = tid;
@@ -111,12 +112,14 @@ struct LrGroups {
   }
 };
 
-// Floats of a group's sums, as the MMA leaves them: RT tiles of 16 ranks, NT of 8 rows.
-template <int RT, int NT>
+// A build for RT tiles of 16 ranks: groups of up to NT eights of rows.
+template <int RT>
 struct LrShape {
+  static constexpr int NT = RT <= 4 ? 4 : 2;
   static constexpr int G = NT * 8;
-  static constexpr int SUMS = RT * NT * 128;
-  static constexpr int H_ROW = RT * 16 + 8;  // padded: a lane's 16 bytes of 8 rows fall into different banks
+  static constexpr bool TWO = RT <= 2;               // the registers leave room for two CTAs on an SM
+  static constexpr int SUMS = RT * NT * 128;         // floats of a group's sums, as the MMA leaves them
+  static constexpr int H_ROW = RT * 16 + 8;          // padded: a lane's 16 bytes of 8 rows fall into different banks
   static constexpr int TERM = G * H_ROW;             // of one of the terms
   static constexpr int STAGE = 8 * kLrStageRow;      // floats in which a warp turns its results
   static constexpr int JOIN = kLrWarps * (SUMS > STAGE ? SUMS : STAGE) * 4;
@@ -129,12 +132,14 @@ __device__ __forceinline__ void st_cluster_v4(uint32_t addr, const float4& v) {
                : "memory");
 }
 
+__device__ __noinline__ float lr_gelu_32(float x) { return 0.5f * x * (1.f + erff(x * 0.70710678118654752f)); }
+
 // GELU of two values: with the library's erf where the result has 32 bits, by the approximation of the
 // projections' epilogue (1.5e-7 of the value) where it has 16.  There infinity is no number in the product of its factors.
 __device__ __forceinline__ void lr_gelu(float& x, float& y, bool f32) {
   if (f32) {
-    x = 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
-    y = 0.5f * y * (1.f + erff(y * 0.70710678118654752f));
+    x = lr_gelu_32(x);
+    y = lr_gelu_32(y);
     return;
   }
   const float inf = __int_as_float(0x7f800000), x0 = x, y0 = y;
@@ -214,155 +219,60 @@ __device__ __forceinline__ void lr_terms(float h, int parts, __nv_bfloat16* to, 
   }
 }
 
-// What the column part of a group works on.
-struct LrColumns {
-  int64_t first;                // the window's first row
-  const int* rows;              // of the group, in the window
-  const __nv_bfloat16* up;      // the adapter's, or null: nothing is added
-  const __nv_bfloat16* terms;   // [parts][G][H_ROW]
-  float* stage;                 // the warp's
-  int parts;                    // terms that the sums are split into
-  bool bad;                     // an index past the set: NaN
+// A warp's 64 columns of up, as the MMA takes them: 4 ranks a lane of its 8 columns, or 8 of each 32.
+template <int RT>
+struct LrUp {
+  static constexpr int CHUNKS = RT == 1 ? 1 : RT / 2;
+  static constexpr int KEPT = CHUNKS <= 2 ? CHUNKS : 1;  // more than the registers hold are read for each eight of rows
+  uint32_t w[KEPT][8][RT == 1 ? 2 : 4];
+
+  // p: the adapter's up at the lane's first column and rank
+  __device__ __forceinline__ void load(const LowRankArgs& a, const __nv_bfloat16* p, int to, int chunk, int columns) {
+    const int rank = (RT == 1 ? 4 : 8) * (threadIdx.x % 4) + chunk * 32;
+#pragma unroll
+    for (int m = 0; m < 8; ++m) {
+      const __nv_bfloat16* const at = p + m * a.rank + chunk * 32;
+      const bool in = m < columns && rank < a.rank;
+      if constexpr (RT == 1) {
+        const uint2 v = in ? __ldg(reinterpret_cast<const uint2*>(at)) : make_uint2(0, 0);
+        w[to][m][0] = v.x, w[to][m][1] = v.y;
+      } else {
+        const uint4 v = in ? __ldg(reinterpret_cast<const uint4*>(at)) : make_uint4(0, 0, 0, 0);
+        w[to][m][0] = v.x, w[to][m][1] = v.y, w[to][m][2] = v.z, w[to][m][3] = v.w;
+      }
+    }
+  }
+
+  // Adds the product with the rows' terms at p (16 or 32 ranks).
+  __device__ __forceinline__ void add(int from, const __nv_bfloat16* p, float (&acc)[4][4]) const {
+    if constexpr (RT == 1) {
+      const uint2 b = *reinterpret_cast<const uint2*>(p);
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        const uint32_t f[4] = {w[from][2 * m][0], w[from][2 * m + 1][0], w[from][2 * m][1], w[from][2 * m + 1][1]};
+        mma_m16n8k16_bf16(acc[m], f, b.x, b.y);
+      }
+    } else {
+      const uint4 b = *reinterpret_cast<const uint4*>(p);
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        const uint32_t f[4] = {w[from][2 * m][0], w[from][2 * m + 1][0], w[from][2 * m][1], w[from][2 * m + 1][1]};
+        const uint32_t h[4] = {w[from][2 * m][2], w[from][2 * m + 1][2], w[from][2 * m][3], w[from][2 * m + 1][3]};
+        mma_m16n8k16_bf16(acc[m], f, b.x, b.y);
+        mma_m16n8k16_bf16(acc[m], h, b.z, b.w);
+      }
+    }
+  }
 };
 
-// TILES tiles of 64 columns, `stride` apart, for the first NTU * 8 rows of the group.
-template <int RT, int NT, int NTU, int TILES, bool F32>
-__device__ __forceinline__ void lr_columns(const LowRankArgs& a, const LrColumns& o, int tile0, int stride, int tiles) {
-  using S = LrShape<RT, NT>;
-  const int lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-  const bool whole = a.outer % 8 == 0;
-  // base goes out first: no load of it waits behind a store that might be to the same place
-  LrEight<F32> base[TILES][NTU][2];
-  if (whole) {
-#pragma unroll
-    for (int q = 0; q < TILES; ++q) {
-      const int col = (tile0 + q * stride) * kLrTile + 8 * g;
-#pragma unroll
-      for (int i = 0; i < NTU; ++i) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int row = o.rows[i * 8 + 2 * t + e];
-          if (row >= 0 && tile0 + q * stride < tiles && col < a.outer) base[q][i][e].load(a, (o.first + row) * a.outer + col);
-        }
-      }
-    }
-  }
-  float acc[TILES][4][NTU][4] = {};
-  if (o.up != nullptr) {
-    constexpr int CHUNKS = RT == 1 ? 1 : RT / 2;  // of 16 or 32 ranks
-#pragma unroll(TILES * CHUNKS <= 2 ? CHUNKS : 1)
-    for (int r = 0; r < CHUNKS; ++r) {
-      // 4 ranks a lane, or 8
-      uint4 w[TILES][4][2];
-#pragma unroll
-      for (int q = 0; q < TILES; ++q) {
-        const int col = (tile0 + q * stride) * kLrTile + 8 * g;
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int at = col + 2 * m + h, rank = RT == 1 ? 4 * t : r * 32 + 8 * t;
-            const __nv_bfloat16* const p = o.up + static_cast<int64_t>(at) * a.rank + rank;
-            const bool in = tile0 + q * stride < tiles && at < a.outer && rank < a.rank;
-            w[q][m][h] = make_uint4(0, 0, 0, 0);
-            if constexpr (RT == 1) {
-              if (in) {
-                const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-                w[q][m][h].x = v.x, w[q][m][h].y = v.y;
-              }
-            } else {
-              if (in) w[q][m][h] = __ldg(reinterpret_cast<const uint4*>(p));
-            }
-          }
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < NTU; ++i) {
-        for (int part = 0; part < o.parts; ++part) {
-          const __nv_bfloat16* const p = o.terms + part * S::TERM + (i * 8 + g) * S::H_ROW + (RT == 1 ? 4 * t : r * 32 + 8 * t);
-          uint4 b = make_uint4(0, 0, 0, 0);
-          if constexpr (RT == 1) {
-            const uint2 v = *reinterpret_cast<const uint2*>(p);
-            b.x = v.x, b.y = v.y;
-          } else {
-            b = *reinterpret_cast<const uint4*>(p);
-          }
-#pragma unroll
-          for (int q = 0; q < TILES; ++q) {
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-              const uint32_t one[4] = {w[q][m][0].x, w[q][m][1].x, w[q][m][0].y, w[q][m][1].y};
-              mma_m16n8k16_bf16(acc[q][m][i], one, b.x, b.y);
-              if constexpr (RT > 1) {
-                const uint32_t two[4] = {w[q][m][0].z, w[q][m][1].z, w[q][m][0].w, w[q][m][1].w};
-                mma_m16n8k16_bf16(acc[q][m][i], two, b.z, b.w);
-              }
-            }
-          }
-        }
-      }
-    }
-  }
-  const float nan = __int_as_float(0x7fffffff);
-#pragma unroll
-  for (int q = 0; q < TILES; ++q) {
-    const int tile = tile0 + q * stride, col = tile * kLrTile + 8 * g;
-    if (tile >= tiles) break;
-#pragma unroll
-    for (int i = 0; i < NTU; ++i) {
-      if (whole) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int row = o.rows[i * 8 + 2 * t + e];
-          if (row < 0 || col >= a.outer) continue;
-          float y[8];
-          base[q][i][e].values(y);
-#pragma unroll
-          for (int m = 0; m < 4; ++m) {
-            y[2 * m] = o.bad ? nan : y[2 * m] + acc[q][m][i][e];
-            y[2 * m + 1] = o.bad ? nan : y[2 * m + 1] + acc[q][m][i][2 + e];
-          }
-          lr_store_eight(a, (o.first + row) * a.outer + col, y);
-        }
-        continue;
-      }
-      // Rows that start anywhere: turned in shared memory, so that a warp reads and writes 32 neighbouring values.
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float4* const to = reinterpret_cast<float4*>(o.stage + (2 * t + e) * kLrStageRow + 8 * g);
-        to[0] = make_float4(acc[q][0][i][e], acc[q][0][i][2 + e], acc[q][1][i][e], acc[q][1][i][2 + e]);
-        to[1] = make_float4(acc[q][2][i][e], acc[q][2][i][2 + e], acc[q][3][i][e], acc[q][3][i][2 + e]);
-      }
-      __syncwarp();
-      float y[8][2];
-#pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        const int row = o.rows[i * 8 + r];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int at = tile * kLrTile + h * 32 + lane;
-          y[r][h] = row >= 0 && at < a.outer ? lr_load_one<F32>(a, (o.first + row) * a.outer + at) : 0.f;
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        const int row = o.rows[i * 8 + r];
-        if (row < 0) break;
-        float lo = y[r][0] + o.stage[r * kLrStageRow + lane], hi = y[r][1] + o.stage[r * kLrStageRow + 32 + lane];
-        if (a.gelu) lr_gelu(lo, hi, a.out_f32);
-        const int at = tile * kLrTile + lane;
-        const int64_t where = (o.first + row) * a.outer + at;
-        if (at < a.outer) lr_store_one(a, where, o.bad ? nan : lo);
-        if (at + 32 < a.outer) lr_store_one(a, where + 32, o.bad ? nan : hi);
-      }
-      __syncwarp();
-    }
-  }
-}
-
-template <int RT, int NT, bool F32>
-__global__ void __launch_bounds__(kLrThreads, RT * NT <= (F32 ? 4 : 8) ? 2 : 1) low_rank_kernel(const __grid_constant__ LowRankArgs a) {
-  using S = LrShape<RT, NT>;
+// F32: base has 32 bits.  WHOLE: the rows of base and out are multiples of 16 bytes.
+// The code is kept short (few copies of the inner parts): a call lasts so few microseconds
+// that instructions which are run once cost what fetching them takes.
+template <int RT, bool F32, bool WHOLE>
+__global__ void __launch_bounds__(kLrThreads, LrShape<RT>::TWO ? 2 : 1) low_rank_kernel(const __grid_constant__ LowRankArgs a) {
+  using S = LrShape<RT>;
+  constexpr int NT = S::NT;
+  constexpr bool EARLY = RT <= 2;  // up's first columns are loaded before the sums are taken
   extern __shared__ __align__(16) uint8_t lr_smem[];
   __shared__ LrGroups<S::G> s;
 
@@ -373,6 +283,7 @@ __global__ void __launch_bounds__(kLrThreads, RT * NT <= (F32 ? 4 : 8) ? 2 : 1) 
   float* const join = reinterpret_cast<float*>(lr_smem);
   float* const sums = join + S::JOIN / 4;  // [2][C][SUMS], where C > 1
   __nv_bfloat16* const terms = reinterpret_cast<__nv_bfloat16*>(sums + (C > 1 ? 2 * C * S::SUMS : 0));
+  float* const stage = join + warp * S::STAGE;
 
   // the CTAs of the cluster all run before any writes into another's shared memory
   if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -381,16 +292,13 @@ __global__ void __launch_bounds__(kLrThreads, RT * NT <= (F32 ? 4 : 8) ? 2 : 1) 
 
   const int cluster = static_cast<int>(blockIdx.x) / C;
   const int mine = cluster % a.clusters;
-  LrColumns o;
-  o.first = static_cast<int64_t>(cluster / a.clusters) * kLrWindow;
-  o.rows = s.rows;
-  o.terms = terms;
-  o.stage = join + warp * S::STAGE;
-  o.parts = a.out_f32 ? 3 : 2;
-  const int n = static_cast<int>(min(static_cast<int64_t>(kLrWindow), a.rows - o.first));
-  const int groups = s.form(a, o.first, n);
+  const int64_t first = static_cast<int64_t>(cluster / a.clusters) * kLrWindow;
+  const int n = static_cast<int>(min(static_cast<int64_t>(kLrWindow), a.rows - first));
+  const int groups = s.form(a, first, n);
   if (C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 
+  const int parts = a.out_f32 ? 3 : 2;  // terms that the sums are split into
+  const float nan = __int_as_float(0x7fffffff);
   // fewer groups than clusters: several share a group and split its columns
   const int split = max(1, min(a.clusters / groups, a.parts));
   const int part = split == 1 ? 0 : mine / groups;
@@ -402,60 +310,108 @@ __global__ void __launch_bounds__(kLrThreads, RT * NT <= (F32 ? 4 : 8) ? 2 : 1) 
     const int adapter = s.key[s.lead[group]];
     if (adapter < 0 && a.skip_bare) continue;
     __syncthreads();  // the rows, terms and stages of the group before are read
-    const int many = s.take(group, n);
-    o.bad = adapter >= a.count;
-    o.up = adapter < 0 || o.bad ? nullptr : a.up + static_cast<int64_t>(adapter) * a.outer * a.rank;
+    const int many = s.take(group, n, a.group);
+    const bool bad = adapter >= a.count, bare = adapter < 0 || bad;
 
-    if (o.up != nullptr) {
-      // the warp's first columns of up are on their way while the sums are taken
-      for (int tile = tile0, k = 0; tile < tiles && k < 4; tile += stride, ++k) {
-        const char* const p = reinterpret_cast<const char*>(o.up + static_cast<int64_t>(tile) * kLrTile * a.rank);
-        const int bytes = min(kLrTile, a.outer - tile * kLrTile) * a.rank * 2;
-        for (int at = lane * 128; at < bytes; at += 32 * 128) prefetch_l2(p + at);
+    // the warp's columns, from its first tile on
+    LrUp<RT> next;
+    LrEight<F32> next_base[2];
+    const __nv_bfloat16* const up = a.up + (static_cast<int64_t>(bare ? 0 : adapter) * a.outer + 8 * g) * a.rank + (RT == 1 ? 4 : 8) * t;
+    auto load_up = [&](int tile, int to, int chunk) {
+      const int col = tile * kLrTile;
+      next.load(a, up + static_cast<int64_t>(col) * a.rank, to, chunk, a.outer - col - 8 * g);
+    };
+    auto load_base = [&](int tile, int i) {
+      const int col = tile * kLrTile + 8 * g;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = s.rows[i * 8 + 2 * t + e];
+        if (row >= 0 && col < a.outer) next_base[e].load(a, (first + row) * a.outer + col);
       }
+    };
+    // where rows start anywhere: 64 neighbouring values of each of 8 rows by a warp
+    float next_y[8][2] = {};
+    auto load_ragged = [&](int tile, int i) {
+      const int at = tile * kLrTile + lane, here = many - i * 8;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        if (r >= here) break;
+        const int64_t where = (first + s.rows[i * 8 + r]) * a.outer + at;
+        if (at < a.outer) next_y[r][0] = lr_load_one<F32>(a, where);
+        if (at + 32 < a.outer) next_y[r][1] = lr_load_one<F32>(a, where + 32);
+      }
+    };
+    auto load_rows = [&](int tile, int i) {
+      if constexpr (WHOLE)
+        load_base(tile, i);
+      else
+        load_ragged(tile, i);
+    };
+    if (bare && tile0 < tiles) load_rows(tile0, 0);
+
+    if (!bare) {
       // ---- sums over K: [ranks] x [rows of the group]
       float acc[RT][NT][4] = {};
-      const __nv_bfloat16* xp[NT];
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        const int row = s.rows[i * 8 + g];
-        xp[i] = row < 0 ? nullptr : a.x + (o.first + row) * a.inner + 8 * t;
-      }
-      const __nv_bfloat16* const dp = a.down + (static_cast<int64_t>(adapter) * a.rank + g) * a.inner + 8 * t;
       const int steps = (a.inner + 31) / 32, units = C * kLrWarps, unit = c * kLrWarps + warp;
       const int from = static_cast<int>(static_cast<int64_t>(steps) * unit / units);
       const int to = static_cast<int>(static_cast<int64_t>(steps) * (unit + 1) / units);
+      const __nv_bfloat16* xp[NT];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) xp[i] = a.x + (first + max(s.rows[i * 8 + g], 0)) * a.inner + from * 32 + 8 * t;
+      const __nv_bfloat16* dp = a.down + (static_cast<int64_t>(adapter) * a.rank + g) * a.inner + from * 32 + 8 * t;
       const uint4 zero = make_uint4(0, 0, 0, 0);
-      constexpr int U = RT * 2 + NT <= 6 ? 4 : RT * 2 + NT <= 12 ? 2 : 1;  // steps whose loads go out together
+      // What the columns need is asked for behind the first values of K, and arrives while the sums are taken.
+      auto columns_ahead = [&]() {
+        if (tile0 < tiles) {
+          load_rows(tile0, 0);
+          if (EARLY) {
+#pragma unroll
+            for (int r = 0; r < LrUp<RT>::KEPT; ++r) load_up(tile0, r, r);
+          }
+        }
+        for (int tile = EARLY ? tile0 + stride : tile0, k = 0; tile < tiles && k < 4; tile += stride, ++k) {
+          const char* const p = reinterpret_cast<const char*>(a.up + (static_cast<int64_t>(adapter) * a.outer + tile * kLrTile) * a.rank);
+          const int bytes = min(kLrTile, a.outer - tile * kLrTile) * a.rank * 2;
+          for (int at = lane * 128; at < bytes; at += 32 * 128) prefetch_l2(p + at);
+        }
+      };
+      if (from == to) columns_ahead();
+      constexpr int U = RT == 1 ? 2 : 1;  // steps whose loads go out together
+#pragma unroll 1
       for (int at = from; at < to; at += U) {
         uint4 w[U][RT][2], v[U][NT];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int k = (at + u) * 32;
-          const bool in = at + u < to && k + 8 * t < a.inner;
+          const bool in = at + u < to && (at + u) * 32 + 8 * t < a.inner;
 #pragma unroll
           for (int r = 0; r < RT; ++r) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const int row = r * 16 + h * 8;
               w[u][r][h] = in && row + g < a.rank
-                               ? __ldg(reinterpret_cast<const uint4*>(dp + static_cast<int64_t>(row) * a.inner + k))
+                               ? __ldg(reinterpret_cast<const uint4*>(dp + static_cast<int64_t>(row) * a.inner + u * 32))
                                : zero;
             }
           }
 #pragma unroll
-          for (int i = 0; i < NT; ++i)
-            v[u][i] = in && xp[i] != nullptr ? __ldg(reinterpret_cast<const uint4*>(xp[i] + k)) : zero;
+          for (int i = 0; i < NT; ++i) {
+            if (i * 8 >= many) break;
+            v[u][i] = in && i * 8 + g < many ? __ldg(reinterpret_cast<const uint4*>(xp[i] + u * 32)) : zero;
+          }
         }
+        if (at == from) columns_ahead();
+        dp += U * 32;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) xp[i] += U * 32;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
 #pragma unroll
-          for (int r = 0; r < RT; ++r) {
-            const uint4 lo = w[u][r][0], hi = w[u][r][1];
-            const uint32_t one[4] = {lo.x, hi.x, lo.y, hi.y}, two[4] = {lo.z, hi.z, lo.w, hi.w};
+          for (int i = 0; i < NT; ++i) {
+            if (i * 8 >= many) break;
 #pragma unroll
-            for (int i = 0; i < NT; ++i) {
-              if (i * 8 >= many) break;
+            for (int r = 0; r < RT; ++r) {
+              const uint4 lo = w[u][r][0], hi = w[u][r][1];
+              const uint32_t one[4] = {lo.x, hi.x, lo.y, hi.y}, two[4] = {lo.z, hi.z, lo.w, hi.w};
               mma_m16n8k16_bf16(acc[r][i], one, v[u][i].x, v[u][i].y);
               mma_m16n8k16_bf16(acc[r][i], two, v[u][i].z, v[u][i].w);
             }
@@ -464,53 +420,126 @@ __global__ void __launch_bounds__(kLrThreads, RT * NT <= (F32 ? 4 : 8) ? 2 : 1) 
       }
       // ---- joined: warps, then CTAs, each in order
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
+      for (int i = 0; i < NT; ++i) {
+        if (i * 8 >= many) break;
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
-          *reinterpret_cast<float4*>(join + warp * S::SUMS + ((r * NT + i) * 32 + lane) * 4) =
+        for (int r = 0; r < RT; ++r)
+          *reinterpret_cast<float4*>(join + warp * S::SUMS + ((i * RT + r) * 32 + lane) * 4) =
               make_float4(acc[r][i][0], acc[r][i][1], acc[r][i][2], acc[r][i][3]);
       }
       __syncthreads();
+      const int held = (many + 7) / 8 * RT * 32;  // float4s of the rows that there are
       float* const shared_sums = sums + (round++ & 1) * C * S::SUMS;
       if (C > 1) {
-        for (int i = tid; i < S::SUMS / 4; i += kLrThreads) {
+        // a warp for each CTA that the sums go to, in turn
+        for (int i = lane; i < held; i += 32) {
           float4 v = *reinterpret_cast<const float4*>(join + i * 4);
 #pragma unroll
           for (int w = 1; w < kLrWarps; ++w) {
             const float4 u = *reinterpret_cast<const float4*>(join + w * S::SUMS + i * 4);
             v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
           }
-          for (int peer = 0; peer < C; ++peer) st_cluster_v4(peer_smem_addr(shared_sums + c * S::SUMS + i * 4, peer), v);
+          for (int peer = warp; peer < C; peer += kLrWarps) st_cluster_v4(peer_smem_addr(shared_sums + c * S::SUMS + i * 4, peer), v);
         }
         cluster_sync();
       }
       const float scale = __ldg(a.scales + adapter);
       const float* const from_all = C > 1 ? shared_sums : join;
       const int pieces = C > 1 ? C : kLrWarps;
-      for (int i = tid; i < S::SUMS / 4; i += kLrThreads) {
-        float4 v = *reinterpret_cast<const float4*>(from_all + i * 4);
-        for (int w = 1; w < pieces; ++w) {
-          const float4 u = *reinterpret_cast<const float4*>(from_all + w * S::SUMS + i * 4);
-          v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
-        }
-        const int l = i % 32, tile = i / 32, r = tile / NT, q = tile % NT;
-        const float y[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int at_rank = r * 16 + l / 4 + (e / 2) * 8, at_row = q * 8 + 2 * (l % 4) + e % 2;
-          // no rank there: 0, also where x is infinite
-          lr_terms(at_rank < a.rank ? y[e] * scale : 0.f, o.parts, terms + at_row * S::H_ROW + at_rank, S::TERM);
-        }
+      for (int i = tid; i < held * 4; i += kLrThreads) {
+        float v = from_all[i];
+        for (int w = 1; w < pieces; ++w) v += from_all[w * S::SUMS + i];
+        const int e = i % 4, l = i / 4 % 32, tile = i / 128, q = tile / RT, r = tile % RT;
+        const int at_rank = r * 16 + l / 4 + (e / 2) * 8, at_row = q * 8 + 2 * (l % 4) + e % 2;
+        // no rank there: 0, also where x is infinite
+        lr_terms(at_rank < a.rank ? v * scale : 0.f, parts, terms + at_row * S::H_ROW + at_rank, S::TERM);
       }
       __syncthreads();
     }
 
     // ---- columns
-    if (many <= 8) {
-      constexpr int TILES = RT * (F32 ? 2 : 1) <= 4 ? 2 : 1;
-      for (int tile = tile0; tile < tiles; tile += TILES * stride) lr_columns<RT, NT, 1, TILES, F32>(a, o, tile, stride, tiles);
-    } else if constexpr (NT > 1) {
-      for (int tile = tile0; tile < tiles; tile += stride) lr_columns<RT, NT, NT, 1, F32>(a, o, tile, stride, tiles);
+#pragma unroll 1
+    for (int tile = tile0; tile < tiles; tile += stride) {
+      if (!EARLY && !bare) {
+#pragma unroll
+        for (int r = 0; r < LrUp<RT>::KEPT; ++r)
+          if (LrUp<RT>::CHUNKS == LrUp<RT>::KEPT) load_up(tile, r, r);
+      }
+      const LrUp<RT> now = next;
+      if (EARLY && !bare && tile + stride < tiles) {
+#pragma unroll
+        for (int r = 0; r < LrUp<RT>::KEPT; ++r) load_up(tile + stride, r, r);
+      }
+      const int col = tile * kLrTile + 8 * g;
+#pragma unroll 1
+      for (int i = 0; i * 8 < many; ++i) {
+        const LrEight<F32> base[2] = {next_base[0], next_base[1]};
+        float y8[8][2];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) y8[r][0] = next_y[r][0], y8[r][1] = next_y[r][1];
+        // the next eight rows' values, or the next columns', before a store that might be to the same place
+        if ((i + 1) * 8 < many)
+          load_rows(tile, i + 1);
+        else if (tile + stride < tiles)
+          load_rows(tile + stride, 0);
+        float acc[4][4] = {};
+        if (!bare) {
+          const __nv_bfloat16* const p = terms + (i * 8 + g) * S::H_ROW + (RT == 1 ? 4 : 8) * t;
+          if constexpr (LrUp<RT>::CHUNKS == LrUp<RT>::KEPT) {
+#pragma unroll
+            for (int r = 0; r < LrUp<RT>::KEPT; ++r) {
+#pragma unroll 1
+              for (int k = 0; k < parts; ++k) now.add(r, p + k * S::TERM + r * 32, acc);
+            }
+          } else {
+#pragma unroll 1
+            for (int r = 0; r < LrUp<RT>::CHUNKS; ++r) {
+              load_up(tile, 0, r);
+#pragma unroll 1
+              for (int k = 0; k < parts; ++k) next.add(0, p + k * S::TERM + r * 32, acc);
+            }
+          }
+        }
+        if constexpr (WHOLE) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int row = s.rows[i * 8 + 2 * t + e];
+            if (row < 0 || col >= a.outer) continue;
+            float y[8];
+            base[e].values(y);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+              y[2 * m] += acc[m][e];
+              y[2 * m + 1] += acc[m][2 + e];
+            }
+            if (bad) {
+#pragma unroll
+              for (int m = 0; m < 8; ++m) y[m] = nan;
+            }
+            lr_store_eight(a, (first + row) * a.outer + col, y);
+          }
+        } else {
+          // Rows that start anywhere: turned in shared memory, so that a warp reads and writes 32 neighbouring values.
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float4* const to = reinterpret_cast<float4*>(stage + (2 * t + e) * kLrStageRow + 8 * g);
+            to[0] = make_float4(acc[0][e], acc[0][2 + e], acc[1][e], acc[1][2 + e]);
+            to[1] = make_float4(acc[2][e], acc[2][2 + e], acc[3][e], acc[3][2 + e]);
+          }
+          __syncwarp();
+          const int at = tile * kLrTile + lane, here = min(many - i * 8, 8);
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            if (r >= here) break;
+            float lo = y8[r][0] + stage[r * kLrStageRow + lane], hi = y8[r][1] + stage[r * kLrStageRow + 32 + lane];
+            if (a.gelu) lr_gelu(lo, hi, a.out_f32);
+            const int64_t where = (first + s.rows[i * 8 + r]) * a.outer + at;
+            if (at < a.outer) lr_store_one(a, where, bad ? nan : lo);
+            if (at + 32 < a.outer) lr_store_one(a, where + 32, bad ? nan : hi);
+          }
+          __syncwarp();
+        }
+      }
     }
   }
 }

@@ -8,37 +8,83 @@ namespace {
 constexpr int kLrShared = 220 * 1024;  // most that a build asks for
 constexpr int kLrTwo = 110 * 1024;     // with which two CTAs share an SM
 
-template <int RT, int NT, bool F32>
+constexpr int kLrSteps = 2;  // of 32 values of K, for a warp
+
+template <int RT, bool F32, bool WHOLE>
 cudaError_t launch_low_rank(b200tx::LowRankArgs& a, DeviceState* dev, int index, cudaStream_t stream) {
-  using S = b200tx::LrShape<RT, NT>;
+  using S = b200tx::LrShape<RT>;
   static_assert(S::bytes(8, 3) <= kLrShared, "the sums of eight CTAs do not fit");
   if (!dev->low_rank_attr[index]) {
-    cudaError_t err = cudaFuncSetAttribute(b200tx::low_rank_kernel<RT, NT, F32>,
+    cudaError_t err = cudaFuncSetAttribute(b200tx::low_rank_kernel<RT, F32, WHOLE>,
                                            cudaFuncAttributeMaxDynamicSharedMemorySize, kLrShared);
     if (err != cudaSuccess) return err;
     dev->low_rank_attr[index] = true;
   }
   const int64_t windows = (a.rows + b200tx::kLrWindow - 1) / b200tx::kLrWindow;
   const int64_t rows = std::min<int64_t>(a.rows, b200tx::kLrWindow);
-  const int64_t least = (rows + S::G - 1) / S::G;  // groups of a window, where its rows share an adapter
+  const int terms = a.out_f32 ? 3 : 2;
+  // CTAs of a cluster: as many as leave each warp a few steps of K, while that leaves every SM two CTAs at most.
+  const int64_t warps = (a.inner + 32 * kLrSteps - 1) / (32 * kLrSteps);
+  int ctas = 8;
+  while (ctas > 1 && (ctas / 2 * b200tx::kLrWarps >= warps || windows * ((rows + S::G - 1) / S::G) * ctas > 2 * dev->sm_count))
+    ctas /= 2;
+  const int bytes = S::bytes(ctas, terms);
+  const int64_t resident = std::max(1, dev->sm_count * (S::TWO && bytes <= kLrTwo ? 2 : 1) / ctas);  // clusters
+  // Rows of a group: fewer, while the groups then all run at once.
+  a.group = S::G;
+  while (a.group > 8 && windows * ((rows + a.group / 2 - 1) / (a.group / 2)) <= resident) a.group /= 2;
+  const int64_t least = (rows + a.group - 1) / a.group;  // groups of a window, where its rows share an adapter
   // Groups that can be: one more for each further index that occurs.
   const int64_t most = std::min<int64_t>(rows, least + a.count + 1);
-  // CTAs of a group: as many as leave every SM two CTAs at most.
-  int ctas = 8;
-  while (ctas > 1 && windows * least * ctas > 2 * dev->sm_count) ctas /= 2;
-  const int bytes = S::bytes(ctas, a.out_f32 ? 3 : 2);
-  const int resident = dev->sm_count * (bytes <= kLrTwo ? 2 : 1);
   const int64_t tiles = (a.outer + b200tx::kLrTile - 1) / b200tx::kLrTile;
   a.parts = static_cast<int>((tiles + ctas * b200tx::kLrWarps - 1) / (ctas * b200tx::kLrWarps));
-  a.clusters = static_cast<int>(std::min(std::max(least, resident / (ctas * windows)), most * a.parts));
-  return launch_clustered(b200tx::low_rank_kernel<RT, NT, F32>, dim3(static_cast<unsigned>(windows * a.clusters * ctas)),
+  a.clusters = static_cast<int>(std::min(std::max(least, resident / windows), most * a.parts));
+  return launch_clustered(b200tx::low_rank_kernel<RT, F32, WHOLE>, dim3(static_cast<unsigned>(windows * a.clusters * ctas)),
                           dim3(b200tx::kLrThreads), static_cast<size_t>(bytes), static_cast<unsigned>(ctas), stream, a);
 }
 
-template <int RT, int NT>
-cudaError_t launch_low_rank_base(b200tx::LowRankArgs& a, bool f32, DeviceState* dev, int index, cudaStream_t stream) {
-  return f32 ? launch_low_rank<RT, NT, true>(a, dev, index, stream) : launch_low_rank<RT, NT, false>(a, dev, index + 1, stream);
+template <int RT>
+cudaError_t launch_low_rank_io(b200tx::LowRankArgs& a, bool f32, DeviceState* dev, int index, cudaStream_t stream) {
+  if (a.outer % 8 == 0)
+    return f32 ? launch_low_rank<RT, true, true>(a, dev, index, stream) : launch_low_rank<RT, false, true>(a, dev, index + 1, stream);
+  return f32 ? launch_low_rank<RT, true, false>(a, dev, index + 2, stream) : launch_low_rank<RT, false, false>(a, dev, index + 3, stream);
 }
+
+template <int RA, bool F32, bool WHOLE>
+cudaError_t launch_low_rank_tile(b200tx::LowRankArgs& a, DeviceState* dev, int index, cudaStream_t stream) {
+  using S = b200tx::LtShape<RA>;
+  constexpr int kMost = 215 * 1024;
+  static_assert(S::bytes(RA * 64, 3) <= kMost, "the terms do not fit");
+  if (!dev->low_rank_tile_attr[index]) {
+    cudaError_t err = cudaFuncSetAttribute(b200tx::low_rank_tile_kernel<RA, F32, WHOLE>,
+                                           cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+    if (err != cudaSuccess) return err;
+    dev->low_rank_tile_attr[index] = true;
+  }
+  const int rank16 = (a.rank + 15) / 16 * 16;
+  const int bytes = static_cast<int>(S::bytes(rank16, a.out_f32 ? 3 : 2));
+  const int64_t windows = (a.rows + b200tx::kLrWindow - 1) / b200tx::kLrWindow;
+  const int64_t rows = std::min<int64_t>(a.rows, b200tx::kLrWindow);
+  a.group = b200tx::kLtRows;
+  const int64_t least = (rows + a.group - 1) / a.group;
+  // The columns are cut into parts, for each of which the sums are taken anew, while all CTAs then run at once.
+  const int64_t resident = dev->sm_count * (RA == 1 && bytes <= kLrTwo ? 2 : 1);
+  const int64_t rounds = (a.outer + b200tx::kLtColumns - 1) / b200tx::kLtColumns;
+  a.parts = static_cast<int>(std::min(rounds, std::max<int64_t>(1, resident / (windows * least))));
+  a.clusters = static_cast<int>(least * a.parts);
+  return launch(b200tx::low_rank_tile_kernel<RA, F32, WHOLE>, dim3(static_cast<unsigned>(windows * a.clusters)),
+                dim3(b200tx::kLrThreads), static_cast<size_t>(bytes), stream, a);
+}
+
+template <int RA>
+cudaError_t launch_low_rank_tile_io(b200tx::LowRankArgs& a, bool f32, DeviceState* dev, int index, cudaStream_t stream) {
+  if (a.outer % 4 == 0)
+    return f32 ? launch_low_rank_tile<RA, true, true>(a, dev, index, stream) : launch_low_rank_tile<RA, false, true>(a, dev, index + 1, stream);
+  return f32 ? launch_low_rank_tile<RA, true, false>(a, dev, index + 2, stream) : launch_low_rank_tile<RA, false, false>(a, dev, index + 3, stream);
+}
+
+// Many rows with runs of one adapter go by 128 on tcgen05.
+constexpr int64_t kLtLeastRows = 1024, kLtLeastRun = 64;
 
 int kv8_pool(const char* what, const b200tx_kv8_pool* c, b200tx::Kv8Pool* out) {
   if (c == nullptr) return fail(B200TX_ERR_INVALID_ARGUMENT, "%s: null pool", what);
@@ -47,6 +93,8 @@ int kv8_pool(const char* what, const b200tx_kv8_pool* c, b200tx::Kv8Pool* out) {
   if (rc != B200TX_OK) return rc;
   if (c->refs == nullptr || c->scratch == nullptr)
     return fail(B200TX_ERR_INVALID_ARGUMENT, "%s: null pool pointer", what);
+  if (!aligned16(c->refs) || !aligned16(c->scratch))
+    return fail(B200TX_ERR_INVALID_ARGUMENT, "%s: refs and scratch must be 16-byte aligned", what);
   if (c->layers <= 0 || c->layers > (1 << 16)) return fail(B200TX_ERR_INVALID_ARGUMENT, "%s: %lld layers", what, (long long)c->layers);
   if (c->cache.pages > (1 << 30)) return fail(B200TX_ERR_INVALID_ARGUMENT, "%s: %lld pages", what, (long long)c->cache.pages);
   out->codes = view.codes;
@@ -78,7 +126,7 @@ int low_log2(int64_t v) {
   return shift;
 }
 
-constexpr int kPoolShared = 64 * 1024;  // of 2048 rows' records and places
+constexpr int kPoolShared = 96 * 1024;  // of 2048 rows' records and places
 
 // CTAs for an order over so many pages and entries: one, without exchanges, while its
 // threads take few of them each.
@@ -146,12 +194,15 @@ int b200tx_low_rank_add(const void* x, const void* base, int base_dtype, void* o
   a.out_f32 = out_dtype == B200TX_F32;
   a.gelu = epilogue == B200TX_EPI_BIAS_GELU;
   a.skip_bare = base == out && !a.gelu;
-  const bool f32 = base_dtype == B200TX_F32, few = M <= 8;
-  cudaError_t err = rank <= 16   ? few ? launch_low_rank_base<1, 1>(a, f32, dev, 0, stream) : launch_low_rank_base<1, 4>(a, f32, dev, 2, stream)
-                    : rank <= 32 ? few ? launch_low_rank_base<2, 1>(a, f32, dev, 4, stream) : launch_low_rank_base<2, 4>(a, f32, dev, 6, stream)
-                    : rank <= 64 ? few ? launch_low_rank_base<4, 1>(a, f32, dev, 8, stream) : launch_low_rank_base<4, 4>(a, f32, dev, 10, stream)
-                    : few        ? launch_low_rank_base<8, 1>(a, f32, dev, 12, stream)
-                                 : launch_low_rank_base<8, 2>(a, f32, dev, 14, stream);
+  const bool f32 = base_dtype == B200TX_F32;
+  if (M >= kLtLeastRows && a.per_index >= kLtLeastRun) {
+    cudaError_t err = rank <= 64 ? launch_low_rank_tile_io<1>(a, f32, dev, 0, stream) : launch_low_rank_tile_io<2>(a, f32, dev, 4, stream);
+    return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "low_rank_add");
+  }
+  cudaError_t err = rank <= 16   ? launch_low_rank_io<1>(a, f32, dev, 0, stream)
+                    : rank <= 32 ? launch_low_rank_io<2>(a, f32, dev, 4, stream)
+                    : rank <= 64 ? launch_low_rank_io<4>(a, f32, dev, 8, stream)
+                                 : launch_low_rank_io<8>(a, f32, dev, 12, stream);
   return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "low_rank_add");
 }
 
@@ -179,7 +230,10 @@ int b200tx_kv8_fork(const b200tx_kv8_pool* pool, const int32_t* source, const in
   a.pairs = static_cast<int>(pairs);
   a.owners = slot_places(pairs);
   const int region = b200tx::kKv8Block * a.pool.dim / 8;
-  a.piece_shift = std::min(low_log2(b200tx::kForkPieces / pairs), low_log2(region));
+  a.region_log2 = low_log2(region);
+  a.piece_shift = std::min(low_log2(b200tx::kForkPieces / pairs), a.region_log2);
+  if (static_cast<double>(a.pool.slots) * 4 * a.pool.kv_heads * region >= 4294967295.0)
+    return fail(B200TX_ERR_UNSUPPORTED, "kv8_fork: a layer's tails pass 64 GB");
   a.column_shift = low_log2(b200tx::kForkPieces / pairs);
   const int64_t tail_items =
       source == nullptr ? 0 : static_cast<int64_t>(a.pool.layers) * 2 * a.pool.kv_heads * (region >> a.piece_shift);
@@ -244,8 +298,9 @@ int b200tx_kv8_compact(const b200tx_kv8_pool* pool, int32_t* used, cudaStream_t 
   cudaError_t err =
       launch_clustered(b200tx::kv8_compact_plan_kernel, dim3(ctas), dim3(b200tx::kPoolThreads), 0, ctas, stream, a);
   if (err == cudaSuccess)
-    err = launch(b200tx::kv8_compact_move_kernel, dim3(static_cast<unsigned>(4 * dev->sm_count)), dim3(b200tx::kCompactThreads),
-                 0, stream, a);
+    err = launch(b200tx::kv8_compact_move_kernel,
+                 dim3(static_cast<unsigned>(std::min<int64_t>(4 * dev->sm_count, (a.pool.pages + 1) / 2 * a.pool.layers * a.pieces))),
+                 dim3(b200tx::kCompactThreads), 0, stream, a);
   return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "kv8_compact");
 }
 

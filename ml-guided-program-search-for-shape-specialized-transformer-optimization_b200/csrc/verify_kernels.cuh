@@ -21,7 +21,7 @@ constexpr int kVerifyThreads = 256;
 constexpr int kVerifyWarps = kVerifyThreads / 32;
 constexpr int kVerifyMostCtas = 8;
 constexpr int kVerifyTokens = 1024;  // drafted tokens of a sequence
-constexpr int kVerifyLook = 256;     // values that a warp looks through one by one
+constexpr int kVerifyLook = 256;     // values that a warp looks through one by one, the CTA's warps at the same time
 
 struct VerifyArgs {
   const void* target;  // [batch, tokens + 1, vocab]
@@ -217,11 +217,11 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_draft_kernel(const __gr
 
   int64_t token = -1;
   if (all > 0.0) {
-    // a part, the eighth of it, and so on, until a warp looks through what is left
+    // a part, the eighth of it, and so on, until the warps look through what is left
     int pick = verify_pick(s_part[0], kVerifyWarps, running, wanted);
     int64_t from = static_cast<int64_t>(c * kVerifyWarps + pick) * length;
-    int limit = end(from, length);
-    for (int level = 1; length > kVerifyLook; ++level) {
+    int limit = end(from, length), level = 1;
+    for (; length > kVerifyWarps * kVerifyLook; ++level) {
       length = (length + kVerifyWarps * 256 - 1) / (kVerifyWarps * 256) * 256;
       const int64_t mine = from + static_cast<int64_t>(warp) * length;
       const double sum = mine < limit ? row.sum(static_cast<int>(mine), min(limit, end(mine, length))) : 0.0;
@@ -231,30 +231,40 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_draft_kernel(const __gr
       from += static_cast<int64_t>(pick) * length;
       limit = min(limit, end(from, length));
     }
-    double mass[kVerifyLook / 32];
-    int latest = -1, found = -1;
+    from += warp * kVerifyLook;
+    double mass[kVerifyLook / 32], sum = 0.0;
 #pragma unroll
     for (int i = 0; i < kVerifyLook / 32; ++i) {
       const int64_t at = from + i * 32 + lane;
       mass[i] = at < limit ? row.one(static_cast<int>(at)) : 0.0;
+      sum += mass[i];
     }
 #pragma unroll
+    for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (lane == 0) s_part[level & 1][warp] = sum;
+    __syncthreads();
+    if (verify_pick(s_part[level & 1], kVerifyWarps, running, wanted) != warp) return;
+    int latest = -1, found = -1;
+#pragma unroll
     for (int i = 0; i < kVerifyLook / 32; ++i) {
-      double sum = mass[i];
+      double before = mass[i];
 #pragma unroll
       for (int d = 1; d < 32; d *= 2) {
-        const double o = __shfl_up_sync(0xffffffffu, sum, d);
-        if (lane >= d) sum += o;
+        const double o = __shfl_up_sync(0xffffffffu, before, d);
+        if (lane >= d) before += o;
       }
-      const uint32_t passed = __ballot_sync(0xffffffffu, mass[i] > 0.0 && running + sum > wanted);
+      const uint32_t passed = __ballot_sync(0xffffffffu, mass[i] > 0.0 && running + before > wanted);
       const uint32_t held = __ballot_sync(0xffffffffu, mass[i] > 0.0);
       if (found < 0 && passed != 0) found = i * 32 + __ffs(passed) - 1;
       if (held != 0) latest = i * 32 + 31 - __clz(held);
-      running += __shfl_sync(0xffffffffu, sum, 31);
+      running += __shfl_sync(0xffffffffu, before, 31);
     }
     token = from + (found >= 0 ? found : latest);
+  } else if (warp != 0) {
+    return;
   }
-  for (int t = tid; t <= a.tokens; t += kVerifyThreads) {
+  // one warp of one CTA is left
+  for (int t = lane; t <= a.tokens; t += 32) {
     const int64_t value = t < first ? drafted(t) : t == first ? token : -1;
     const int64_t at = b * (a.tokens + 1) + t;
     if (a.wide)
@@ -262,7 +272,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_draft_kernel(const __gr
     else
       static_cast<int32_t*>(a.out)[at] = static_cast<int32_t>(value);
   }
-  if (tid == 0) a.accepted[b] = first;
+  if (lane == 0) a.accepted[b] = first;
 }
 
 }  // namespace b200tx

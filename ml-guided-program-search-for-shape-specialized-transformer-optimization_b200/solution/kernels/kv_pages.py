@@ -51,8 +51,8 @@ class Kv8Pages(TensorHandle):
             refs = torch.zeros(cache.pages, dtype=torch.int32, device=cache.device)
         require(
             refs.dtype == torch.int32 and tuple(refs.shape) == (cache.pages,) and refs.is_contiguous()
-            and refs.device == cache.device,
-            "refs must be a contiguous int32 [pages] tensor on the cache's device",
+            and refs.device == cache.device and refs.data_ptr() % 16 == 0,
+            "refs must be a contiguous, 16-byte aligned int32 [pages] tensor on the cache's device",
         )
         self.cache = cache
         self.refs = refs

@@ -410,7 +410,8 @@ def test_pool_without_a_gpu() -> None:
     assert Kv8Pages(cache, torch.ones(5, dtype=torch.int32)).refs.tolist() == [1] * 5
     whole = Kv8Cache.create(slots=2, max_tokens=200, num_kv_heads=1, head_dim=32, device="cpu")
     assert Kv8Pages(whole).free == 0
-    for refs in (torch.zeros(4, dtype=torch.int32), torch.zeros(5), torch.zeros(10, dtype=torch.int32)[::2]):
+    for refs in (torch.zeros(4, dtype=torch.int32), torch.zeros(5), torch.zeros(10, dtype=torch.int32)[::2],
+                 torch.zeros(6, dtype=torch.int32)[1:]):
         with pytest.raises(ValueError):
             Kv8Pages(cache, refs)
     with pytest.raises(AttributeError):
@@ -474,7 +475,7 @@ def test_c_entry_refusals() -> None:
     for call in calls:
         assert call(None) < 0
         for bad in ({"codes": None}, {"codes": 8}, {"tail": None}, {"tail": 24}, {"scales": None}, {"page_table": None},
-                    {"lengths": None}, {"refs": None}, {"scratch": None}, {"layers": 0}, {"pages": 0}, {"slots": 0},
+                    {"lengths": None}, {"refs": None}, {"refs": 20}, {"scratch": None}, {"scratch": 8}, {"layers": 0}, {"pages": 0}, {"slots": 0},
                     {"head_dim": 48}, {"max_blocks": 0}, {"kv_heads": 0}):
             assert call(ctypes.byref(view(**bad))) < 0, bad
     good = ctypes.byref(view())

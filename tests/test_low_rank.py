@@ -105,6 +105,46 @@ def test_low_rank_add(rows, inner, outer, rank, count, base_dtype) -> None:  # n
 
 
 @gpu
+@pytest.mark.parametrize(
+    ("batch", "tokens", "inner", "outer", "rank", "count"),
+    [
+        (4, 300, 264, 1032, 16, 3),
+        (2, 700, 1000, 515, 72, 2),
+        (16, 64, 72, 200, 8, 5),
+        (5, 257, 2056, 384, 128, 3),
+        (1, 1024, 8, 130, 64, 1),
+        (20, 100, 512, 4096, 40, 4),
+    ],
+)
+@pytest.mark.parametrize("base_dtype", [torch.bfloat16, torch.float32])
+def test_prompts(batch, tokens, inner, outer, rank, count, base_dtype) -> None:  # noqa: ANN001
+    """Long runs of rows with one adapter each."""
+    g = torch.Generator(device="cuda").manual_seed(batch + outer)
+    adapters = _adapters(count, rank, inner, outer, g)
+    x = torch.randn(batch, tokens, inner, generator=g, device="cuda").bfloat16()
+    base = torch.randn(batch, tokens, outer, generator=g, device="cuda").to(base_dtype)
+    indices = torch.randint(-1, count + 1, (batch,), generator=g, device="cuda", dtype=torch.int32)
+    x[0, 3, 5], x[0, tokens - 1, 0], base[-1, 1, 7] = torch.inf, torch.nan, torch.nan
+    keep = torch.ones(batch, tokens, dtype=torch.bool, device="cuda")
+    keep[0, 3] = keep[0, -1] = keep[-1, 1] = False
+    want = {}
+    for gelu in (False, True):
+        for out_dtype in (torch.bfloat16, torch.float32):
+            value, off = _expected(x, base, adapters, indices, gelu, out_dtype)
+            got, _ = sm100_low_rank_add(x, base, adapters, indices, gelu=gelu, out_dtype=out_dtype)
+            rows = keep.flatten()
+            got = got.double().flatten(0, 1)[rows]
+            bad = value[rows].isnan()
+            assert torch.equal(got.isnan(), bad)
+            assert float(torch.where(bad, 0, (got - value[rows]).abs() - off[rows]).max()) <= 0
+            want[gelu, out_dtype] = got
+    for gelu in (False, True):  # in place, and the same again
+        there = base.clone()
+        sm100_low_rank_add(x, there, adapters, indices, gelu=gelu, out=there)
+        assert torch.equal(there.double().flatten(0, 1)[keep.flatten()].nan_to_num(5.0), want[gelu, base_dtype].nan_to_num(5.0))
+
+
+@gpu
 @pytest.mark.parametrize("rows", [7, 300, 2500])
 def test_indices_of_runs_and_every_mix(rows) -> None:  # noqa: ANN001
     """One index for each sequence; all rows alike; every row another; none at all; indices past the set."""
