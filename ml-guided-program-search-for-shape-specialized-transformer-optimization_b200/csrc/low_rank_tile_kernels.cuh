@@ -8,8 +8,10 @@
 //      layout that the UMMA reads, which leaves the rows free and any multiple of 8 for K;
 //   2. the sums, scaled, become bf16 terms in shared memory (each the rounded rest of the ones before);
 //   3. for each 128 columns: terms . up^T into one of two TMEM buffers, while the warps bring
-//      the buffer before to the result: a warp turns 32 rows x 32 columns in shared memory, so
-//      that base is read and the result written in whole 64-byte pieces of rows.
+//      the buffer before to the result.  The columns stand in the buffer in an order in which a lane that
+//      reads two neighbouring ones of each eight (tcgen05.ld of 16 lanes x 256 bits) has 16 neighbouring columns of the result, of two
+//      rows: it reads base and writes the result 16 bytes at a time, four lanes a whole line, and
+//      nothing is turned in shared memory.
 //
 // Bound by the bytes of base and the result, which are 9 of 10 of a feed-forward layer's: the weights of
 // an adapter are read (from L2) once for 128 rows, and two CTAs on an SM cover each other's waits.
@@ -26,9 +28,7 @@ namespace b200tx {
 constexpr int kLtRows = 128;
 constexpr int kLtColumns = 128;          // of the result, for one round
 constexpr int kLtStages = 4;             // of 64 values of K
-constexpr int kLtTurnRow = 36;           // floats: 32, padded so that 8 rows fall into different banks
 constexpr uint32_t kLtXBytes = kLtRows * 128;
-constexpr uint32_t kLtTurnBytes = kLrWarps * 32 * kLtTurnRow * 4;
 constexpr int kErrLowRankWait = 0x501;
 
 // RA atoms of 64 ranks.
@@ -37,18 +37,34 @@ struct LtShape {
   static constexpr uint32_t UP = RA * kLtColumns * 128;  // a round's columns of up
   static constexpr uint32_t TERM = RA * kLtRows * 128;
   __host__ __device__ static constexpr uint32_t stage(int rank16) { return kLtXBytes + rank16 * 128; }
-  // the stages of the sums, and later the terms, two rounds' columns and the turned results, in the same place
+  // the stages of the sums, and later the terms and two rounds' columns, in the same place
   __host__ __device__ static constexpr uint32_t bytes(int rank16, int terms) {
-    return (kLtStages * stage(rank16) > terms * TERM + 2 * UP + kLtTurnBytes ? kLtStages * stage(rank16)
-                                                                            : terms * TERM + 2 * UP + kLtTurnBytes) + 1024;
+    return (kLtStages * stage(rank16) > terms * TERM + 2 * UP ? kLtStages * stage(rank16) : terms * TERM + 2 * UP) + 1024;
   }
 };
+
+// A lane of 32 reads two neighbouring columns of each eight, of 64, of rows lane / 4 (r[4 j], r[4 j + 1]) and lane / 4 + 8.
+__device__ __forceinline__ void tmem_ld_16x64(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32"
+      " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15,"
+      " %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31},"
+      " [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+
+// Where column c of a round stands in its buffer: column 16 t + 2 j + b of 64 is lane t's j-th, at 8 j + 2 t + b.
+__device__ __forceinline__ int lt_column(int c) { return (c & 64) | (c >> 1 & 7) * 8 | (c >> 4 & 3) * 2 | (c & 1); }
 
 // Where 16 bytes of a 128-byte row stand under the 128-byte swizzle.
 __device__ __forceinline__ uint32_t lt_place(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
 
-template <int RA, bool F32, bool WHOLE>
-__global__ void __launch_bounds__(kLrThreads, RA == 1 ? 2 : 1) low_rank_tile_kernel(const __grid_constant__ LowRankArgs a) {
+template <int RA, bool F32>
+__global__ void __launch_bounds__(kLrThreads, RA == 1 && !F32 ? 2 : 1) low_rank_tile_kernel(const __grid_constant__ LowRankArgs a) {
   using S = LtShape<RA>;
   extern __shared__ uint8_t lt_smem[];
   __shared__ LrGroups<kLtRows> s;
@@ -61,8 +77,6 @@ __global__ void __launch_bounds__(kLrThreads, RA == 1 ? 2 : 1) low_rank_tile_ker
   const uint32_t smem0 = smem_u32(smem);
   const int rank16 = (a.rank + 15) / 16 * 16, parts = a.out_f32 ? 3 : 2;
   const uint32_t up0 = smem0 + parts * S::TERM;
-  float* const turn = reinterpret_cast<float*>(smem + parts * S::TERM + 2 * S::UP) + warp * 32 * kLtTurnRow;
-
   if (tid == 0) {
     for (int i = 0; i < kLtStages; ++i) mbar_init(&stage_bar[i], 1);
     for (int i = 0; i < 2; ++i) mbar_init(&round_bar[i], 1);
@@ -105,13 +119,12 @@ __global__ void __launch_bounds__(kLrThreads, RA == 1 ? 2 : 1) low_rank_tile_ker
 
     // 128 columns of up, K-major; ranks past the adapter's up to a multiple of 16, and columns past the last, are zero
     auto load_up = [&](int round) {
-      const int chunks = rank16 / 8;
+      const int col = tid / 2, at = (round0 + round) * kLtColumns + col;  // two threads a column
       const uint32_t to = up0 + (round & 1) * S::UP;
-      for (int i = tid; i < kLtColumns * chunks; i += kLrThreads) {
-        const int col = i / chunks, chunk = i - col * chunks, at = (round0 + round) * kLtColumns + col;
+      const __nv_bfloat16* const from = up + (at < a.outer ? static_cast<int64_t>(at) * a.rank : 0);
+      for (int chunk = tid % 2; chunk < rank16 / 8; chunk += 2) {
         const bool in = at < a.outer && chunk * 8 < a.rank;
-        cp_async_or_zero(to + chunk / 8 * (kLtColumns * 128) + lt_place(col, chunk % 8),
-                         up + (in ? static_cast<int64_t>(at) * a.rank + chunk * 8 : 0), in);
+        cp_async_or_zero(to + chunk / 8 * (kLtColumns * 128) + lt_place(lt_column(col), chunk % 8), from + (in ? chunk * 8 : 0), in);
       }
       cp_async_commit();
     };
@@ -211,26 +224,30 @@ __global__ void __launch_bounds__(kLrThreads, RA == 1 ? 2 : 1) low_rank_tile_ker
     // ---- columns: round j's UMMAs run while round j - 1 is brought to the result
     const uint32_t idesc = umma_idesc_bf16(kLtRows, kLtColumns, false, false);
     const int quarter = warp % 4 * 32, half = warp / 4 * 64;
-    // base's values of this lane, 4 neighbouring columns of every 4th row, on their way before they are wanted
-    float4 next[8];
-    auto load_base = [&](int round, int sub) {
-      const int column = (round0 + round) * kLtColumns + half + sub + lane % 8 * 4;
+    // This lane's values: 16 neighbouring columns of four rows.  Places in the window have 32 bits (256 rows of 2^24 columns).
+    uint32_t place[4];
+    uint32_t live = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int row = s.rows[quarter + i * 4 + lane / 8];
-        if (row < 0 || column >= a.outer) continue;
-        const int64_t at = (first + row) * a.outer + column;
-        if constexpr (WHOLE && F32) {
-          next[i] = *reinterpret_cast<const float4*>(static_cast<const float*>(a.base) + at);
-        } else if constexpr (WHOLE) {
-          const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(a.base) + at);
-          next[i].x = __uint_as_float(v.x), next[i].y = __uint_as_float(v.y);  // taken apart where it is used
-        } else {
-          next[i].x = lr_load_one<F32>(a, at);
-          if (column + 1 < a.outer) next[i].y = lr_load_one<F32>(a, at + 1);
-          if (column + 2 < a.outer) next[i].z = lr_load_one<F32>(a, at + 2);
-          if (column + 3 < a.outer) next[i].w = lr_load_one<F32>(a, at + 3);
-        }
+    for (int i = 0; i < 4; ++i) {
+      const int row = s.rows[quarter + i * 8 + lane / 4];
+      live |= static_cast<uint32_t>(row >= 0) << i;
+      place[i] = static_cast<uint32_t>(max(row, 0)) * a.outer + half + lane % 4 * 16;
+    }
+    constexpr int IN = F32 ? 4 : 2;  // 16-byte pieces of base in 16 columns
+    const uint8_t* const base0 = static_cast<const uint8_t*>(a.base) + first * a.outer * (F32 ? 4 : 2);
+    uint8_t* const out0 = static_cast<uint8_t*>(a.out) + first * a.outer * (a.out_f32 ? 4 : 2);
+    // base's values are on their way before they are wanted: rows 2 i and 2 i + 1 of the four
+    uint4 next[2][IN];
+    auto load_base = [&](int round, int i) {
+      const uint32_t column = (round0 + round) * kLtColumns;
+      const int left = a.outer - static_cast<int>(column) - half - lane % 4 * 16;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if (!(live >> (2 * i + e) & 1)) continue;
+        const uint4* const p = reinterpret_cast<const uint4*>(base0 + static_cast<uint64_t>(place[2 * i + e] + column) * (F32 ? 4 : 2));
+#pragma unroll
+        for (int k = 0; k < IN; ++k)
+          if (left > k * (16 / IN)) next[e][k] = p[k];
       }
     };
     load_base(0, 0);
@@ -264,57 +281,67 @@ __global__ void __launch_bounds__(kLrThreads, RA == 1 ? 2 : 1) low_rank_tile_ker
         if (j + 1 < rounds) load_up(j + 1);
       }
       if (j == 0) continue;
-      const int column0 = (round0 + j - 1) * kLtColumns + half;
-#pragma unroll 1
-      for (int sub = 0; sub < 64; sub += 32) {
-        const int column = column0 + sub + lane % 8 * 4;
-        float4 base[8];
+      const uint32_t column = (round0 + j - 1) * kLtColumns;
+      const int left = a.outer - static_cast<int>(column) - half - lane % 4 * 16;  // columns from this lane's first one on
 #pragma unroll
-        for (int i = 0; i < 8; ++i) base[i] = next[i];
-        if (sub == 0)
-          load_base(j - 1, 32);
+      for (int i = 0; i < 2; ++i) {
+        uint4 base[2][IN];
+#pragma unroll
+        for (int k = 0; k < 2 * IN; ++k) base[k / IN][k % IN] = next[k / IN][k % IN];
+        if (i == 0)
+          load_base(j - 1, 1);
         else if (j < rounds)
           load_base(j, 0);
+        uint32_t r[32];
         if (!bare) {
-          uint32_t r[32];
-          tmem_ld_32cols(tmem + ((j - 1) & 1) * 128 + (static_cast<uint32_t>(quarter) << 16) + half + sub, r);
+          tmem_ld_16x64(tmem + ((j - 1) & 1) * 128 + (static_cast<uint32_t>(quarter + i * 16) << 16) + half, r);
           tmem_wait_ld();
-          __syncwarp();
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<uint4*>(turn + lane * kLtTurnRow + i * 4) = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
-          __syncwarp();
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int row = s.rows[quarter + i * 4 + lane / 8];
-          if (row < 0 || column >= a.outer) continue;
-          float4 y = base[i];
-          if constexpr (WHOLE && !F32) {
-            const uint32_t lo = __float_as_uint(y.x), hi = __float_as_uint(y.y);
-            y = make_float4(__uint_as_float(lo << 16), __uint_as_float(lo & 0xffff0000u), __uint_as_float(hi << 16),
-                            __uint_as_float(hi & 0xffff0000u));
+        for (int e = 0; e < 2; ++e) {
+          if (!(live >> (2 * i + e) & 1)) continue;
+          float y[16];
+#pragma unroll
+          for (int k = 0; k < IN; ++k) {
+            const uint32_t w[4] = {base[e][k].x, base[e][k].y, base[e][k].z, base[e][k].w};
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+              if constexpr (F32) {
+                y[4 * k + m] = __uint_as_float(w[m]);
+              } else {
+                y[8 * k + 2 * m] = __uint_as_float(w[m] << 16);
+                y[8 * k + 2 * m + 1] = __uint_as_float(w[m] & 0xffff0000u);
+              }
+            }
           }
           if (!bare) {
-            const float4 v = *reinterpret_cast<const float4*>(turn + (i * 4 + lane / 8) * kLtTurnRow + lane % 8 * 4);
-            y.x += v.x, y.y += v.y, y.z += v.z, y.w += v.w;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) y[k] += __uint_as_float(r[k / 2 * 4 + 2 * e + k % 2]);
           }
-          if (bad) y = make_float4(nan, nan, nan, nan);
-          if (a.gelu) {
-            lr_gelu(y.x, y.y, a.out_f32);
-            lr_gelu(y.z, y.w, a.out_f32);
+          if (bad) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) y[k] = nan;
           }
-          const int64_t at = (first + row) * a.outer + column;
-          if constexpr (WHOLE) {
-            if (a.out_f32)
-              *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = y;
-            else
-              *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + at) = make_uint2(pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
+          if (a.out_f32) {
+            float4* const to = reinterpret_cast<float4*>(out0 + static_cast<uint64_t>(place[2 * i + e] + column) * 4);
+            if (a.gelu) {
+#pragma unroll
+              for (int k = 0; k < 16; ++k) y[k] = lr_gelu_32(y[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (left > 4 * k) to[k] = make_float4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
           } else {
-            lr_store_one(a, at, y.x);
-            if (column + 1 < a.outer) lr_store_one(a, at + 1, y.y);
-            if (column + 2 < a.outer) lr_store_one(a, at + 2, y.z);
-            if (column + 3 < a.outer) lr_store_one(a, at + 3, y.w);
+            uint4* const to = reinterpret_cast<uint4*>(out0 + static_cast<uint64_t>(place[2 * i + e] + column) * 2);
+            if (a.gelu) {
+#pragma unroll
+              for (int k = 0; k < 16; ++k) y[k] = lr_gelu_16(y[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              if (left > 8 * k)
+                to[k] = make_uint4(pack_bf16x2(y[8 * k], y[8 * k + 1]), pack_bf16x2(y[8 * k + 2], y[8 * k + 3]),
+                                   pack_bf16x2(y[8 * k + 4], y[8 * k + 5]), pack_bf16x2(y[8 * k + 6], y[8 * k + 7]));
           }
         }
       }

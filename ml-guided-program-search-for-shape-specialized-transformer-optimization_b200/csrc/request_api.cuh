@@ -50,13 +50,13 @@ cudaError_t launch_low_rank_io(b200tx::LowRankArgs& a, bool f32, DeviceState* de
   return f32 ? launch_low_rank<RT, true, false>(a, dev, index + 2, stream) : launch_low_rank<RT, false, false>(a, dev, index + 3, stream);
 }
 
-template <int RA, bool F32, bool WHOLE>
+template <int RA, bool F32>
 cudaError_t launch_low_rank_tile(b200tx::LowRankArgs& a, DeviceState* dev, int index, cudaStream_t stream) {
   using S = b200tx::LtShape<RA>;
   constexpr int kMost = 215 * 1024;
   static_assert(S::bytes(RA * 64, 3) <= kMost, "the terms do not fit");
   if (!dev->low_rank_tile_attr[index]) {
-    cudaError_t err = cudaFuncSetAttribute(b200tx::low_rank_tile_kernel<RA, F32, WHOLE>,
+    cudaError_t err = cudaFuncSetAttribute(b200tx::low_rank_tile_kernel<RA, F32>,
                                            cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
     if (err != cudaSuccess) return err;
     dev->low_rank_tile_attr[index] = true;
@@ -68,22 +68,15 @@ cudaError_t launch_low_rank_tile(b200tx::LowRankArgs& a, DeviceState* dev, int i
   a.group = b200tx::kLtRows;
   const int64_t least = (rows + a.group - 1) / a.group;
   // The columns are cut into parts, for each of which the sums are taken anew, while all CTAs then run at once.
-  const int64_t resident = dev->sm_count * (RA == 1 && bytes <= kLrTwo ? 2 : 1);
+  const int64_t resident = dev->sm_count * (RA == 1 && !F32 && bytes <= kLrTwo ? 2 : 1);
   const int64_t rounds = (a.outer + b200tx::kLtColumns - 1) / b200tx::kLtColumns;
   a.parts = static_cast<int>(std::min(rounds, std::max<int64_t>(1, resident / (windows * least))));
   a.clusters = static_cast<int>(least * a.parts);
-  return launch(b200tx::low_rank_tile_kernel<RA, F32, WHOLE>, dim3(static_cast<unsigned>(windows * a.clusters)),
+  return launch(b200tx::low_rank_tile_kernel<RA, F32>, dim3(static_cast<unsigned>(windows * a.clusters)),
                 dim3(b200tx::kLrThreads), static_cast<size_t>(bytes), stream, a);
 }
 
-template <int RA>
-cudaError_t launch_low_rank_tile_io(b200tx::LowRankArgs& a, bool f32, DeviceState* dev, int index, cudaStream_t stream) {
-  if (a.outer % 4 == 0)
-    return f32 ? launch_low_rank_tile<RA, true, true>(a, dev, index, stream) : launch_low_rank_tile<RA, false, true>(a, dev, index + 1, stream);
-  return f32 ? launch_low_rank_tile<RA, true, false>(a, dev, index + 2, stream) : launch_low_rank_tile<RA, false, false>(a, dev, index + 3, stream);
-}
-
-// Many rows with runs of one adapter go by 128 on tcgen05.
+// Many rows with runs of one adapter go by 128 on tcgen05, where rows of base and the result are multiples of 16 bytes.
 constexpr int64_t kLtLeastRows = 1024, kLtLeastRun = 64;
 
 int kv8_pool(const char* what, const b200tx_kv8_pool* c, b200tx::Kv8Pool* out) {
@@ -195,8 +188,10 @@ int b200tx_low_rank_add(const void* x, const void* base, int base_dtype, void* o
   a.gelu = epilogue == B200TX_EPI_BIAS_GELU;
   a.skip_bare = base == out && !a.gelu;
   const bool f32 = base_dtype == B200TX_F32;
-  if (M >= kLtLeastRows && a.per_index >= kLtLeastRun) {
-    cudaError_t err = rank <= 64 ? launch_low_rank_tile_io<1>(a, f32, dev, 0, stream) : launch_low_rank_tile_io<2>(a, f32, dev, 4, stream);
+  if (M >= kLtLeastRows && a.per_index >= kLtLeastRun && N % 8 == 0) {
+    cudaError_t err = rank <= 64 ? f32 ? launch_low_rank_tile<1, true>(a, dev, 0, stream) : launch_low_rank_tile<1, false>(a, dev, 1, stream)
+                      : f32      ? launch_low_rank_tile<2, true>(a, dev, 2, stream)
+                                 : launch_low_rank_tile<2, false>(a, dev, 3, stream);
     return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "low_rank_add");
   }
   cudaError_t err = rank <= 16   ? launch_low_rank_io<1>(a, f32, dev, 0, stream)
