@@ -138,8 +138,9 @@ __device__ __noinline__ float lr_gelu_32(float x) { return 0.5f * x * (1.f + erf
 // 1.1e-7 (and 2.4e-4 of itself, a tenth of the result's rounding).  12 instructions; one value at a time, as pairs of
 // values in one instruction want their constants in registers, and moves for them.
 __device__ __forceinline__ float lr_gelu_16(float x) {
-  float a;  // past 16 the tail is 0; NaN stays
-  asm("min.NaN.f32 %0, %1, 0f41800000;" : "=f"(a) : "f"(fabsf(x)));
+  float positive;  // with NaN kept
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(positive) : "f"(x));
+  const float a = fminf(fabsf(x), 16.f);  // past 16 the tail is 0
   float p = fmaf(-7.928164222903433e-07f, a, 4.487410114961676e-05f);
   p = fmaf(p, a, -0.0008306637755595148f);
   p = fmaf(p, a, 0.008231189101934433f);
@@ -147,7 +148,7 @@ __device__ __forceinline__ float lr_gelu_16(float x) {
   p = fmaf(p, a, -0.45865529775619507f);
   p = fmaf(p, a, -1.151233434677124f);
   p = fmaf(p, a, -0.9999903440475464f);
-  return fmaf(-a, fast_exp2(p), fmaxf(x, 0.f));
+  return fmaf(-a, fast_exp2(p), positive);
 }
 
 // GELU of two values, by the library's erf where the result has 32 bits.
@@ -168,10 +169,9 @@ template <bool F32>
 struct LrEight {
   uint4 w[F32 ? 2 : 1];
 
-  __device__ __forceinline__ void load(const LowRankArgs& a, int64_t at) {
-    const uint4* const p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.base) + at * (F32 ? 4 : 2));
+  __device__ __forceinline__ void load(const uint8_t* p) {
 #pragma unroll
-    for (int i = 0; i < (F32 ? 2 : 1); ++i) w[i] = p[i];
+    for (int i = 0; i < (F32 ? 2 : 1); ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
   }
 
   __device__ __forceinline__ void values(float (&y)[8]) const {
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(kLrThreads, LrShape<RT>::TWO ? 2 : 1) low_rank
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int row = s.rows[i * 8 + 2 * t + e];
-        if (row >= 0 && col < a.outer) next_base[e].load(a, (first + row) * a.outer + col);
+        if (row >= 0 && col < a.outer) next_base[e].load(static_cast<const uint8_t*>(a.base) + ((first + row) * a.outer + col) * (F32 ? 4 : 2));
       }
     };
     // where rows start anywhere: 64 neighbouring values of each of 8 rows by a warp

@@ -9,8 +9,8 @@
 //   2. the sums, scaled, become bf16 terms in shared memory (each the rounded rest of the ones before);
 //   3. for each 128 columns: terms . up^T into one of two TMEM buffers, while the warps bring
 //      the buffer before to the result.  The columns stand in the buffer in an order in which a lane that
-//      reads two neighbouring ones of each eight (tcgen05.ld of 16 lanes x 256 bits) has 16 neighbouring columns of the result, of two
-//      rows: it reads base and writes the result 16 bytes at a time, four lanes a whole line, and
+//      reads two neighbouring ones of each eight (tcgen05.ld of 16 lanes x 256 bits) has twice 8 neighbouring columns of the result,
+//      of two rows: it reads base and writes the result 16 bytes at a time, four lanes 64 that lie together, and
 //      nothing is turned in shared memory.
 //
 // Bound by the bytes of base and the result, which are 9 of 10 of a feed-forward layer's: the weights of
@@ -57,8 +57,11 @@ __device__ __forceinline__ void tmem_ld_16x64(uint32_t taddr, uint32_t (&r)[32])
       : "r"(taddr));
 }
 
-// Where column c of a round stands in its buffer: column 16 t + 2 j + b of 64 is lane t's j-th, at 8 j + 2 t + b.
-__device__ __forceinline__ int lt_column(int c) { return (c & 64) | (c >> 1 & 7) * 8 | (c >> 4 & 3) * 2 | (c & 1); }
+// Where column c of a round stands in its buffer: of 64, a lane t of four has columns 8 t to 8 t + 7 of each 32, column
+// 32 k + 8 t + 2 i + b at 8 (4 k + i) + 2 t + b.
+__device__ __forceinline__ int lt_column(int c) {
+  return (c & 64) | ((c >> 5 & 1) * 4 + (c >> 1 & 3)) * 8 | (c >> 3 & 3) * 2 | (c & 1);
+}
 
 // Where 16 bytes of a 128-byte row stand under the 128-byte swizzle.
 __device__ __forceinline__ uint32_t lt_place(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
@@ -224,33 +227,49 @@ __global__ void __launch_bounds__(kLrThreads, RA == 1 && !F32 ? 2 : 1) low_rank_
     // ---- columns: round j's UMMAs run while round j - 1 is brought to the result
     const uint32_t idesc = umma_idesc_bf16(kLtRows, kLtColumns, false, false);
     const int quarter = warp % 4 * 32, half = warp / 4 * 64;
-    // This lane's values: 16 neighbouring columns of four rows.  Places in the window have 32 bits (256 rows of 2^24 columns).
+    // This lane's values: twice 8 neighbouring columns of four rows.  Places in the window have 32 bits (256 rows of 2^24 columns).
     uint32_t place[4];
     uint32_t live = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = s.rows[quarter + i * 8 + lane / 4];
       live |= static_cast<uint32_t>(row >= 0) << i;
-      place[i] = static_cast<uint32_t>(max(row, 0)) * a.outer + half + lane % 4 * 16;
+      place[i] = static_cast<uint32_t>(max(row, 0)) * a.outer + half + lane % 4 * 8;
     }
-    constexpr int IN = F32 ? 4 : 2;  // 16-byte pieces of base in 16 columns
     const uint8_t* const base0 = static_cast<const uint8_t*>(a.base) + first * a.outer * (F32 ? 4 : 2);
     uint8_t* const out0 = static_cast<uint8_t*>(a.out) + first * a.outer * (a.out_f32 ? 4 : 2);
-    // base's values are on their way before they are wanted: rows 2 i and 2 i + 1 of the four
+    // A warp with all its rows takes whole rounds without a check between the values; base's are on their way then before
+    // they are wanted, rows 2 i and 2 i + 1 of the four.
+    const bool plain = __all_sync(0xffffffffu, live == 0xf) && !bare;
+    auto whole = [&](int round) { return plain && (round0 + round + 1) * kLtColumns <= a.outer; };
+    constexpr int IN = F32 ? 4 : 2;  // 16-byte pieces of base in 16 columns
     uint4 next[2][IN];
     auto load_base = [&](int round, int i) {
-      const uint32_t column = (round0 + round) * kLtColumns;
-      const int left = a.outer - static_cast<int>(column) - half - lane % 4 * 16;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        if (!(live >> (2 * i + e) & 1)) continue;
-        const uint4* const p = reinterpret_cast<const uint4*>(base0 + static_cast<uint64_t>(place[2 * i + e] + column) * (F32 ? 4 : 2));
+        const uint8_t* const p = base0 + static_cast<uint64_t>(place[2 * i + e] + (round0 + round) * kLtColumns) * (F32 ? 4 : 2);
 #pragma unroll
-        for (int k = 0; k < IN; ++k)
-          if (left > k * (16 / IN)) next[e][k] = p[k];
+        for (int k = 0; k < IN; ++k) next[e][k] = *reinterpret_cast<const uint4*>(p + (F32 ? k / 2 * 128 + k % 2 * 16 : k * 64));
       }
     };
-    load_base(0, 0);
+    auto store = [&](uint8_t* to, float (&y)[8]) {
+      if (a.out_f32) {
+        if (a.gelu) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) y[k] = lr_gelu_32(y[k]);
+        }
+        reinterpret_cast<float4*>(to)[0] = make_float4(y[0], y[1], y[2], y[3]);
+        reinterpret_cast<float4*>(to)[1] = make_float4(y[4], y[5], y[6], y[7]);
+      } else {
+        if (a.gelu) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) y[k] = lr_gelu_16(y[k]);
+        }
+        *reinterpret_cast<uint4*>(to) =
+            make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
+      }
+    };
+    if (whole(0)) load_base(0, 0);
     for (int j = 0; j <= rounds; ++j) {
       if (!bare) {
         cp_async_wait<0>();
@@ -282,66 +301,70 @@ __global__ void __launch_bounds__(kLrThreads, RA == 1 && !F32 ? 2 : 1) low_rank_
       }
       if (j == 0) continue;
       const uint32_t column = (round0 + j - 1) * kLtColumns;
-      const int left = a.outer - static_cast<int>(column) - half - lane % 4 * 16;  // columns from this lane's first one on
+      const int size = a.out_f32 ? 4 : 2;
+      const uint32_t d = tmem + ((j - 1) & 1) * 128 + (static_cast<uint32_t>(quarter) << 16) + half;
+      if (whole(j - 1)) {
 #pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint4 base[2][IN];
+#pragma unroll
+          for (int k = 0; k < 2 * IN; ++k) base[k / IN][k % IN] = next[k / IN][k % IN];
+          if (i == 0)
+            load_base(j - 1, 1);
+          else if (j < rounds && whole(j))
+            load_base(j, 0);
+          uint32_t r[32];
+          tmem_ld_16x64(d + (static_cast<uint32_t>(i * 16) << 16), r);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            uint8_t* const to = out0 + static_cast<uint64_t>(place[2 * i + e] + column) * size;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              float y[8];
+#pragma unroll
+              for (int m = 0; m < 4; ++m) {
+                if constexpr (F32) {
+                  const uint4 &lo = base[e][2 * k], &hi = base[e][2 * k + 1];
+                  const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+                  y[2 * m] = __uint_as_float(w[2 * m]);
+                  y[2 * m + 1] = __uint_as_float(w[2 * m + 1]);
+                } else {
+                  const uint32_t w[4] = {base[e][k].x, base[e][k].y, base[e][k].z, base[e][k].w};
+                  y[2 * m] = __uint_as_float(w[m] << 16);
+                  y[2 * m + 1] = __uint_as_float(w[m] & 0xffff0000u);
+                }
+                y[2 * m] += __uint_as_float(r[(4 * k + m) * 4 + 2 * e]);
+                y[2 * m + 1] += __uint_as_float(r[(4 * k + m) * 4 + 2 * e + 1]);
+              }
+              store(to + k * 32 * size, y);
+            }
+          }
+        }
+        continue;
+      }
+      // rows or columns are missing, or there is nothing to add
+#pragma unroll 1
       for (int i = 0; i < 2; ++i) {
-        uint4 base[2][IN];
-#pragma unroll
-        for (int k = 0; k < 2 * IN; ++k) base[k / IN][k % IN] = next[k / IN][k % IN];
-        if (i == 0)
-          load_base(j - 1, 1);
-        else if (j < rounds)
-          load_base(j, 0);
-        uint32_t r[32];
+        uint32_t r[32] = {};
         if (!bare) {
-          tmem_ld_16x64(tmem + ((j - 1) & 1) * 128 + (static_cast<uint32_t>(quarter + i * 16) << 16) + half, r);
+          tmem_ld_16x64(d + (static_cast<uint32_t>(i * 16) << 16), r);
           tmem_wait_ld();
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          if (!(live >> (2 * i + e) & 1)) continue;
-          float y[16];
+          const uint32_t from = (i == 0 ? place[e] : place[2 + e]) + column;
 #pragma unroll
-          for (int k = 0; k < IN; ++k) {
-            const uint32_t w[4] = {base[e][k].x, base[e][k].y, base[e][k].z, base[e][k].w};
+          for (int k = 0; k < 2; ++k) {
+            if (!(live >> (2 * i + e) & 1) || column + half + lane % 4 * 8 + k * 32 >= static_cast<uint32_t>(a.outer)) continue;
+            const uint64_t at = static_cast<uint64_t>(from) + k * 32;
+            LrEight<F32> base;
+            base.load(base0 + at * (F32 ? 4 : 2));
+            float y[8];
+            base.values(y);
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
-              if constexpr (F32) {
-                y[4 * k + m] = __uint_as_float(w[m]);
-              } else {
-                y[8 * k + 2 * m] = __uint_as_float(w[m] << 16);
-                y[8 * k + 2 * m + 1] = __uint_as_float(w[m] & 0xffff0000u);
-              }
-            }
-          }
-          if (!bare) {
-#pragma unroll
-            for (int k = 0; k < 16; ++k) y[k] += __uint_as_float(r[k / 2 * 4 + 2 * e + k % 2]);
-          }
-          if (bad) {
-#pragma unroll
-            for (int k = 0; k < 16; ++k) y[k] = nan;
-          }
-          if (a.out_f32) {
-            float4* const to = reinterpret_cast<float4*>(out0 + static_cast<uint64_t>(place[2 * i + e] + column) * 4);
-            if (a.gelu) {
-#pragma unroll
-              for (int k = 0; k < 16; ++k) y[k] = lr_gelu_32(y[k]);
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (left > 4 * k) to[k] = make_float4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
-          } else {
-            uint4* const to = reinterpret_cast<uint4*>(out0 + static_cast<uint64_t>(place[2 * i + e] + column) * 2);
-            if (a.gelu) {
-#pragma unroll
-              for (int k = 0; k < 16; ++k) y[k] = lr_gelu_16(y[k]);
-            }
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-              if (left > 8 * k)
-                to[k] = make_uint4(pack_bf16x2(y[8 * k], y[8 * k + 1]), pack_bf16x2(y[8 * k + 2], y[8 * k + 3]),
-                                   pack_bf16x2(y[8 * k + 4], y[8 * k + 5]), pack_bf16x2(y[8 * k + 6], y[8 * k + 7]));
+            for (int m = 0; m < 8; ++m) y[m] = bad ? nan : y[m] + __uint_as_float(r[(4 * k + m / 2) * 4 + 2 * e + m % 2]);
+            store(out0 + at * size, y);
           }
         }
       }
