@@ -65,7 +65,7 @@ struct LrGroups {
   int warp_leads[kLrWarps];
   int rows[G];                       // of the group at hand, -1 past its end
 
-  // Ranks the window's n rows; returns the number of groups.
+  // Ranks the window's n rows; returns the number of groups.  All threads of the CTA, kLrThreads or more.
   __device__ __forceinline__ int form(const LowRankArgs& a, int64_t first, int n) {
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     int mine = -2;
@@ -85,8 +85,8 @@ struct LrGroups {
     before += __popc(same & ((1u << lane) - 1));
     const bool leads = tid < n && before % a.group == 0;
     const uint32_t leaders = __ballot_sync(0xffffffffu, leads);
-    rank[tid] = before;
-    if (lane == 0) warp_leads[warp] = __popc(leaders);
+    if (tid < kLrWindow) rank[tid] = before;
+    if (lane == 0 && warp < kLrWarps) warp_leads[warp] = __popc(leaders);
     __syncthreads();
     int groups = 0, at = 0;
 #pragma unroll

@@ -17,7 +17,8 @@
 // an adapter are read (from L2) once for 128 rows, and two CTAs on an SM cover each other's waits.
 // The warp MMA form of this reads them for every 32 rows and keeps the tensor pipe busy for as long as the bytes take.
 //
-// All threads do all of it in step; one of them issues the UMMAs.  Waits are bounded as everywhere.
+// The sums are taken in step by all of eight warps; then two more bring the columns of up and issue the UMMAs, and the eight
+// bring the results out, each for itself: they meet at the buffers' barriers only.  Waits are bounded as everywhere.
 #pragma once
 
 #include "kv8_attention_kernels.cuh"
@@ -30,6 +31,8 @@ constexpr int kLtColumns = 128;          // of the result, for one round
 constexpr int kLtStages = 4;             // of 64 values of K
 constexpr uint32_t kLtXBytes = kLtRows * 128;
 constexpr int kErrLowRankWait = 0x501;
+constexpr int kLtFeeders = 64;           // threads that bring up and issue the UMMAs of the columns
+constexpr int kLtThreads = kLrThreads + kLtFeeders;
 
 // RA atoms of 64 ranks.
 template <int RA>
@@ -43,17 +46,13 @@ struct LtShape {
   }
 };
 
-// A lane of 32 reads two neighbouring columns of each eight, of 64, of rows lane / 4 (r[4 j], r[4 j + 1]) and lane / 4 + 8.
-__device__ __forceinline__ void tmem_ld_16x64(uint32_t taddr, uint32_t (&r)[32]) {
+// A lane of 32 reads two neighbouring columns of each eight, of 32, of rows lane / 4 (r[4 j], r[4 j + 1]) and lane / 4 + 8.
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x8.b32"
-      " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15,"
-      " %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31},"
-      " [%32];"
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32"
+      " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
 }
 
@@ -67,11 +66,11 @@ __device__ __forceinline__ int lt_column(int c) {
 __device__ __forceinline__ uint32_t lt_place(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
 
 template <int RA, bool F32>
-__global__ void __launch_bounds__(kLrThreads, RA == 1 && !F32 ? 2 : 1) low_rank_tile_kernel(const __grid_constant__ LowRankArgs a) {
+__global__ void __launch_bounds__(kLtThreads, RA == 1 && !F32 ? 2 : 1) low_rank_tile_kernel(const __grid_constant__ LowRankArgs a) {
   using S = LtShape<RA>;
   extern __shared__ uint8_t lt_smem[];
   __shared__ LrGroups<kLtRows> s;
-  __shared__ uint64_t stage_bar[kLtStages], round_bar[2];
+  __shared__ uint64_t stage_bar[kLtStages], full_bar[2], empty_bar[2];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
 
@@ -82,7 +81,10 @@ __global__ void __launch_bounds__(kLrThreads, RA == 1 && !F32 ? 2 : 1) low_rank_
   const uint32_t up0 = smem0 + parts * S::TERM;
   if (tid == 0) {
     for (int i = 0; i < kLtStages; ++i) mbar_init(&stage_bar[i], 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&round_bar[i], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&full_bar[i], 1);
+      mbar_init(&empty_bar[i], kLrWarps);
+    }
     fence_barrier_init();
     abort_flag = 0;
   }
@@ -108,28 +110,29 @@ __global__ void __launch_bounds__(kLrThreads, RA == 1 && !F32 ? 2 : 1) low_rank_
   const float nan = __int_as_float(0x7fffffff);
   const uint32_t sums_tmem = tmem + 128;  // the second round's columns: free until then
   uint32_t steps_done = 0, rounds_done = 0;
-  bool ok = true;
 
-  for (int group = split == 1 ? mine : part < split ? mine % groups : groups; group < groups && ok;
+  for (int group = split == 1 ? mine : part < split ? mine % groups : groups; group < groups;
        group += split == 1 ? a.clusters : groups) {
     const int adapter = s.key[s.lead[group]];
     if (adapter < 0 && a.skip_bare) continue;
     tc_fence_before();
-    __syncthreads();
+    if (__syncthreads_or(abort_flag)) break;
     const int many = s.take(group, n, a.group);
     const bool bad = adapter >= a.count, bare = adapter < 0 || bad;
     const __nv_bfloat16* const up = a.up + static_cast<int64_t>(bare ? 0 : adapter) * a.outer * a.rank;
 
-    // 128 columns of up, K-major; ranks past the adapter's up to a multiple of 16, and columns past the last, are zero
+    // 128 columns of up, K-major, by the feeders; ranks past the adapter's up to a multiple of 16, and columns past the last, are zero
     auto load_up = [&](int round) {
-      const int col = tid / 2, at = (round0 + round) * kLtColumns + col;  // two threads a column
       const uint32_t to = up0 + (round & 1) * S::UP;
-      const __nv_bfloat16* const from = up + (at < a.outer ? static_cast<int64_t>(at) * a.rank : 0);
-      for (int chunk = tid % 2; chunk < rank16 / 8; chunk += 2) {
-        const bool in = at < a.outer && chunk * 8 < a.rank;
-        cp_async_or_zero(to + chunk / 8 * (kLtColumns * 128) + lt_place(lt_column(col), chunk % 8), from + (in ? chunk * 8 : 0), in);
+      const int part2 = tid % 2;  // two threads a column
+      for (int col = (tid - kLrThreads) / 2; col < kLtColumns; col += kLtFeeders / 2) {
+        const int at = (round0 + round) * kLtColumns + col, row = lt_column(col);
+        const __nv_bfloat16* const from = up + (at < a.outer ? static_cast<int64_t>(at) * a.rank : 0);
+        for (int chunk = part2; chunk < rank16 / 8; chunk += 2) {
+          const bool in = at < a.outer && chunk * 8 < a.rank;
+          cp_async_or_zero(to + chunk / 8 * (kLtColumns * 128) + lt_place(row, chunk % 8), from + (in ? chunk * 8 : 0), in);
+        }
       }
-      cp_async_commit();
     };
 
     if (!bare) {
@@ -139,9 +142,10 @@ __global__ void __launch_bounds__(kLrThreads, RA == 1 && !F32 ? 2 : 1) low_rank_
       const __nv_bfloat16* const down = a.down + static_cast<int64_t>(adapter) * a.rank * a.inner;
       // a thread's pieces: 16 bytes at the same place of every 32nd row
       const int chunk = tid % 8, row0 = tid / 8;
+      const bool loads = tid < kLrThreads;
       const __nv_bfloat16* xp[kLtRows / 32];
 #pragma unroll
-      for (int i = 0; i < kLtRows / 32; ++i) xp[i] = a.x + (first + max(s.rows[row0 + 32 * i], 0)) * a.inner + chunk * 8;
+      for (int i = 0; i < kLtRows / 32; ++i) xp[i] = a.x + (first + (loads ? max(s.rows[row0 + 32 * i], 0) : 0)) * a.inner + chunk * 8;
       auto load_stage = [&](int step) {
         const uint32_t to = smem0 + (steps_done + step) % kLtStages * stage_bytes;
         const bool in = step * 64 + chunk * 8 < a.inner;
@@ -157,7 +161,7 @@ __global__ void __launch_bounds__(kLrThreads, RA == 1 && !F32 ? 2 : 1) low_rank_
         }
       };
       for (int i = 0; i < kLtStages - 1; ++i) {
-        if (i < steps) load_stage(i);
+        if (i < steps && loads) load_stage(i);
         cp_async_commit();
       }
       const uint32_t idesc = umma_idesc_bf16(kLtRows, rank16, false, false);
@@ -178,7 +182,7 @@ __global__ void __launch_bounds__(kLrThreads, RA == 1 && !F32 ? 2 : 1) low_rank_
           const uint32_t at = steps_done + step - 1;
           mbar_wait(&stage_bar[at % kLtStages], at / kLtStages & 1, kErrLowRankWait, &abort_flag);
         }
-        if (step + kLtStages - 1 < steps) load_stage(step + kLtStages - 1);
+        if (step + kLtStages - 1 < steps && loads) load_stage(step + kLtStages - 1);
         cp_async_commit();
       }
       if (abort_flag == 0) {
@@ -187,16 +191,14 @@ __global__ void __launch_bounds__(kLrThreads, RA == 1 && !F32 ? 2 : 1) low_rank_
       }
       cp_async_wait<0>();
       if (__syncthreads_or(abort_flag)) {  // else every stage is read: its place is free
-        ok = false;
         break;
       }
       steps_done += steps;
       tc_fence_after();
-      load_up(0);
       // ---- terms
       const float scale = __ldg(a.scales + adapter);
       const int row = warp % 4 * 32 + lane;
-      for (int col = warp / 4 * 32; col < rank16; col += 64) {
+      for (int col = warp / 4 * 32; loads && col < rank16; col += 64) {
         uint32_t r[32];
         tmem_ld_32cols(sums_tmem + (static_cast<uint32_t>(warp % 4 * 32) << 16) + col, r);
         tmem_wait_ld();
@@ -222,10 +224,43 @@ __global__ void __launch_bounds__(kLrThreads, RA == 1 && !F32 ? 2 : 1) low_rank_
         }
       }
       tc_fence_before();
+      fence_proxy_async_smem();
+      __syncthreads();  // the terms are there, and the sums' place is free
     }
 
-    // ---- columns: round j's UMMAs run while round j - 1 is brought to the result
-    const uint32_t idesc = umma_idesc_bf16(kLtRows, kLtColumns, false, false);
+    // ---- columns
+    if (tid >= kLrThreads) {
+      // feeders
+      const uint32_t idesc = umma_idesc_bf16(kLtRows, kLtColumns, false, false);
+      if (!bare) load_up(0);
+      for (int j = 0; j < rounds && !bare; ++j) {
+        cp_async_commit();
+        cp_async_wait<0>();
+        fence_proxy_async_smem();
+        asm volatile("bar.sync 1, %0;" ::"n"(kLtFeeders) : "memory");
+        const uint32_t at = rounds_done + j, buffer = at & 1;
+        if (tid == kLrThreads && mbar_wait(&empty_bar[buffer], (at >> 1 & 1) ^ 1, kErrLowRankWait, &abort_flag)) {
+          tc_fence_after();
+          const uint32_t w = up0 + (j & 1) * S::UP;
+          uint32_t more = 0;
+          for (int k = 0; k < parts; ++k) {
+            for (int r = 0; r < rank16 / 16; ++r) {
+              const uint32_t in = r / 4 * (kLtRows * 128) + r % 4 * 32;
+              umma_bf16_ss(tmem + buffer * 128, sw128_desc(smem0 + k * S::TERM + in, 16, 1024), sw128_desc(w + in, 16, 1024), idesc, more);
+              more = 1;
+            }
+          }
+          umma_commit(&full_bar[buffer]);
+        }
+        if (j + 1 < rounds) {
+          // the other columns' place is free when the round before is done
+          if (j > 0) mbar_wait(&full_bar[(at - 1) & 1], (at - 1) >> 1 & 1, kErrLowRankWait, &abort_flag);
+          load_up(j + 1);
+        }
+      }
+      if (!bare) rounds_done += rounds;
+      continue;
+    }
     const int quarter = warp % 4 * 32, half = warp / 4 * 64;
     // This lane's values: twice 8 neighbouring columns of four rows.  Places in the window have 32 bits (256 rows of 2^24 columns).
     uint32_t place[4];
@@ -238,19 +273,15 @@ __global__ void __launch_bounds__(kLrThreads, RA == 1 && !F32 ? 2 : 1) low_rank_
     }
     const uint8_t* const base0 = static_cast<const uint8_t*>(a.base) + first * a.outer * (F32 ? 4 : 2);
     uint8_t* const out0 = static_cast<uint8_t*>(a.out) + first * a.outer * (a.out_f32 ? 4 : 2);
-    // A warp with all its rows takes whole rounds without a check between the values; base's are on their way then before
-    // they are wanted, rows 2 i and 2 i + 1 of the four.
+    // A warp with all its rows takes whole rounds without a check between the values; base's are on their way then a
+    // round before they are wanted: rows 2 i and 2 i + 1 of the four, columns 32 k and on.
     const bool plain = __all_sync(0xffffffffu, live == 0xf) && !bare;
     auto whole = [&](int round) { return plain && (round0 + round + 1) * kLtColumns <= a.outer; };
-    constexpr int IN = F32 ? 4 : 2;  // 16-byte pieces of base in 16 columns
-    uint4 next[2][IN];
-    auto load_base = [&](int round, int i) {
+    LrEight<F32> ahead[2][2][2];
+    auto load_base = [&](int round, int i, int k) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint8_t* const p = base0 + static_cast<uint64_t>(place[2 * i + e] + (round0 + round) * kLtColumns) * (F32 ? 4 : 2);
-#pragma unroll
-        for (int k = 0; k < IN; ++k) next[e][k] = *reinterpret_cast<const uint4*>(p + (F32 ? k / 2 * 128 + k % 2 * 16 : k * 64));
-      }
+      for (int e = 0; e < 2; ++e)
+        ahead[i][k][e].load(base0 + static_cast<uint64_t>(place[2 * i + e] + ((round0 + round) * kLtColumns + k * 32)) * (F32 ? 4 : 2));
     };
     auto store = [&](uint8_t* to, float (&y)[8]) {
       if (a.out_f32) {
@@ -269,75 +300,42 @@ __global__ void __launch_bounds__(kLrThreads, RA == 1 && !F32 ? 2 : 1) low_rank_
             make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
       }
     };
-    if (whole(0)) load_base(0, 0);
-    for (int j = 0; j <= rounds; ++j) {
-      if (!bare) {
-        cp_async_wait<0>();
-        fence_proxy_async_smem();
-        tc_fence_before();
-        if (__syncthreads_or(abort_flag)) {  // else the round's columns (and the terms) are there, and its TMEM buffer is read
-          ok = false;
-          break;
-        }
-        if (j < rounds && tid == 0) {
-          tc_fence_after();
-          const uint32_t d = tmem + (j & 1) * 128, w = up0 + (j & 1) * S::UP;
-          uint32_t more = 0;
-          for (int k = 0; k < parts; ++k) {
-            for (int r = 0; r < rank16 / 16; ++r) {
-              const uint32_t at = r / 4 * (kLtRows * 128) + r % 4 * 32;
-              umma_bf16_ss(d, sw128_desc(smem0 + k * S::TERM + at, 16, 1024), sw128_desc(w + at, 16, 1024), idesc, more);
-              more = 1;
-            }
-          }
-          umma_commit(&round_bar[(rounds_done + j) & 1]);
-        }
-        if (j > 0) {
-          const uint32_t at = rounds_done + j - 1;
-          mbar_wait(&round_bar[at & 1], at >> 1 & 1, kErrLowRankWait, &abort_flag);  // if it runs out, all see it at the next barrier
-          tc_fence_after();
-        }
-        if (j + 1 < rounds) load_up(j + 1);
-      }
-      if (j == 0) continue;
-      const uint32_t column = (round0 + j - 1) * kLtColumns;
+    if (whole(0)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) load_base(0, i / 2, i % 2);
+    }
+    for (int j = 0; j < rounds; ++j) {
+      const uint32_t at = rounds_done + j;
+      // the warp goes on, or stops, together
+      if (!__all_sync(0xffffffffu, bare || mbar_wait(&full_bar[at & 1], at >> 1 & 1, kErrLowRankWait, &abort_flag))) break;
+      tc_fence_after();
+      const uint32_t column = (round0 + j) * kLtColumns;
       const int size = a.out_f32 ? 4 : 2;
-      const uint32_t d = tmem + ((j - 1) & 1) * 128 + (static_cast<uint32_t>(quarter) << 16) + half;
-      if (whole(j - 1)) {
+      const uint32_t d = tmem + (at & 1) * 128 + (static_cast<uint32_t>(quarter) << 16) + half;
+      auto done = [&]() {  // the buffer is read
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty_bar[at & 1]);
+      };
+      if (whole(j)) {
+        const bool more = j + 1 < rounds && whole(j + 1);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          uint4 base[2][IN];
 #pragma unroll
-          for (int k = 0; k < 2 * IN; ++k) base[k / IN][k % IN] = next[k / IN][k % IN];
-          if (i == 0)
-            load_base(j - 1, 1);
-          else if (j < rounds && whole(j))
-            load_base(j, 0);
-          uint32_t r[32];
-          tmem_ld_16x64(d + (static_cast<uint32_t>(i * 16) << 16), r);
-          tmem_wait_ld();
+          for (int k = 0; k < 2; ++k) {
+            uint32_t r[16];
+            tmem_ld_16x32(d + (static_cast<uint32_t>(i * 16) << 16) + k * 32, r);
+            float y[2][8];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            uint8_t* const to = out0 + static_cast<uint64_t>(place[2 * i + e] + column) * size;
+            for (int e = 0; e < 2; ++e) ahead[i][k][e].values(y[e]);
+            if (more) load_base(j + 1, i, k);
+            tmem_wait_ld();
+            if (i == 1 && k == 1) done();
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              float y[8];
+            for (int e = 0; e < 2; ++e) {
 #pragma unroll
-              for (int m = 0; m < 4; ++m) {
-                if constexpr (F32) {
-                  const uint4 &lo = base[e][2 * k], &hi = base[e][2 * k + 1];
-                  const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-                  y[2 * m] = __uint_as_float(w[2 * m]);
-                  y[2 * m + 1] = __uint_as_float(w[2 * m + 1]);
-                } else {
-                  const uint32_t w[4] = {base[e][k].x, base[e][k].y, base[e][k].z, base[e][k].w};
-                  y[2 * m] = __uint_as_float(w[m] << 16);
-                  y[2 * m + 1] = __uint_as_float(w[m] & 0xffff0000u);
-                }
-                y[2 * m] += __uint_as_float(r[(4 * k + m) * 4 + 2 * e]);
-                y[2 * m + 1] += __uint_as_float(r[(4 * k + m) * 4 + 2 * e + 1]);
-              }
-              store(to + k * 32 * size, y);
+              for (int m = 0; m < 8; ++m) y[e][m] += __uint_as_float(r[m / 2 * 4 + 2 * e + m % 2]);
+              store(out0 + static_cast<uint64_t>(place[2 * i + e] + (column + k * 32)) * size, y[e]);
             }
           }
         }
@@ -345,29 +343,28 @@ __global__ void __launch_bounds__(kLrThreads, RA == 1 && !F32 ? 2 : 1) low_rank_
       }
       // rows or columns are missing, or there is nothing to add
 #pragma unroll 1
-      for (int i = 0; i < 2; ++i) {
-        uint32_t r[32] = {};
+      for (int i = 0; i < 4; ++i) {
+        uint32_t r[16] = {};
         if (!bare) {
-          tmem_ld_16x64(d + (static_cast<uint32_t>(i * 16) << 16), r);
+          tmem_ld_16x32(d + (static_cast<uint32_t>(i / 2 * 16) << 16) + i % 2 * 32, r);
           tmem_wait_ld();
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const uint32_t from = (i == 0 ? place[e] : place[2 + e]) + column;
+          const uint32_t here = column + half + lane % 4 * 8 + i % 2 * 32;
+          const int row = s.rows[quarter + i / 2 * 16 + e * 8 + lane / 4];
+          if (row < 0 || here >= static_cast<uint32_t>(a.outer)) continue;
+          const uint64_t from = static_cast<uint64_t>(static_cast<uint32_t>(row) * a.outer + here);
+          LrEight<F32> base;
+          base.load(base0 + from * (F32 ? 4 : 2));
+          float y[8];
+          base.values(y);
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            if (!(live >> (2 * i + e) & 1) || column + half + lane % 4 * 8 + k * 32 >= static_cast<uint32_t>(a.outer)) continue;
-            const uint64_t at = static_cast<uint64_t>(from) + k * 32;
-            LrEight<F32> base;
-            base.load(base0 + at * (F32 ? 4 : 2));
-            float y[8];
-            base.values(y);
-#pragma unroll
-            for (int m = 0; m < 8; ++m) y[m] = bad ? nan : y[m] + __uint_as_float(r[(4 * k + m / 2) * 4 + 2 * e + m % 2]);
-            store(out0 + at * size, y);
-          }
+          for (int m = 0; m < 8; ++m) y[m] = bad ? nan : y[m] + __uint_as_float(r[m / 2 * 4 + 2 * e + m % 2]);
+          store(out0 + from * size, y);
         }
       }
+      if (!bare) done();
     }
     if (!bare) rounds_done += rounds;
   }

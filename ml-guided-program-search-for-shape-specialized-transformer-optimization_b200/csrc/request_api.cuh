@@ -73,7 +73,7 @@ cudaError_t launch_low_rank_tile(b200tx::LowRankArgs& a, DeviceState* dev, int i
   a.parts = static_cast<int>(std::min(rounds, std::max<int64_t>(1, resident / (windows * least))));
   a.clusters = static_cast<int>(least * a.parts);
   return launch(b200tx::low_rank_tile_kernel<RA, F32>, dim3(static_cast<unsigned>(windows * a.clusters)),
-                dim3(b200tx::kLrThreads), static_cast<size_t>(bytes), stream, a);
+                dim3(b200tx::kLtThreads), static_cast<size_t>(bytes), stream, a);
 }
 
 // Many rows with runs of one adapter go by 128 on tcgen05, where rows of base and the result are multiples of 16 bytes.
