@@ -3,22 +3,22 @@
 // 128 rows of an adapter at a time on tcgen05.
 //
 // A CTA takes a group of up to 128 rows (found as there) and a part of the columns:
-//   1. sums = x . down^T over K, 128 x R, accumulated in TMEM; x (rows gathered from
-//      anywhere) and down come in 64-column stages by cp.async into the 128-byte swizzled
-//      layout that the UMMA reads, which leaves the rows free and any multiple of 8 for K;
+//   1. sums = x . down^T over K, 128 x R, accumulated in TMEM from stages of 64 values of K.  Rows that
+//      follow one another (a prompt's) come by TMA, others by cp.async from where they are,
+//      into the same 128-byte swizzled layout;
 //   2. the sums, scaled, become bf16 terms in shared memory (each the rounded rest of the ones before);
 //   3. for each 128 columns: terms . up^T into one of two TMEM buffers, while the warps bring
-//      the buffer before to the result.  The columns stand in the buffer in an order in which a lane that
-//      reads two neighbouring ones of each eight (tcgen05.ld of 16 lanes x 256 bits) has twice 8 neighbouring columns of the result,
-//      of two rows: it reads base and writes the result 16 bytes at a time, four lanes 64 that lie together, and
-//      nothing is turned in shared memory.
+//      the buffer before to the result.  up comes by TMA, two neighbouring columns of
+//      each eight at a time, so that a lane that reads two neighbouring ones of each eight of the buffer (tcgen05.ld of
+//      16 lanes x 256 bits) has 8 neighbouring columns of the result, of two rows: it reads base and writes the
+//      result 16 bytes at a time, four lanes 64 that lie together, and nothing is turned in shared memory.
 //
-// Bound by the bytes of base and the result, which are 9 of 10 of a feed-forward layer's: the weights of
-// an adapter are read (from L2) once for 128 rows, and two CTAs on an SM cover each other's waits.
-// The warp MMA form of this reads them for every 32 rows and keeps the tensor pipe busy for as long as the bytes take.
+// The bytes are base's and the result's, 9 of 10 of a feed-forward layer's: the weights of
+// an adapter are read (from L2) once for 128 rows.  The warp MMA form of this reads them for every 32 rows
+// and keeps the tensor pipe busy for as long as the bytes take.
 //
-// The sums are taken in step by all of eight warps; then two more bring the columns of up and issue the UMMAs, and the eight
-// bring the results out, each for itself: they meet at the buffers' barriers only.  Waits are bounded as everywhere.
+// One thread brings the stages and up's columns and issues the UMMAs; 16 warps make the terms and bring the results
+// out, each for itself: they meet the thread at the buffers' barriers only.  Waits are bounded as everywhere.
 #pragma once
 
 #include "kv8_attention_kernels.cuh"
@@ -28,49 +28,47 @@ namespace b200tx {
 
 constexpr int kLtRows = 128;
 constexpr int kLtColumns = 128;          // of the result, for one round
-constexpr int kLtStages = 4;             // of 64 values of K
+constexpr int kLtStages = 6;             // of 64 values of K
 constexpr uint32_t kLtXBytes = kLtRows * 128;
 constexpr int kErrLowRankWait = 0x501;
-constexpr int kLtFeeders = 64;           // threads that bring up and issue the UMMAs of the columns
-constexpr int kLtThreads = kLrThreads + kLtFeeders;
+constexpr int kLtWorkers = 512;          // threads that make the terms and bring the results out
+constexpr int kLtThreads = kLtWorkers + 32;
+constexpr int kLtAhead = kLtStages - 2;  // stages that are asked for before one is used
 
 // RA atoms of 64 ranks.
 template <int RA>
 struct LtShape {
   static constexpr uint32_t UP = RA * kLtColumns * 128;  // a round's columns of up
+  static constexpr int UPS = RA == 1 ? 4 : 3;            // rounds whose columns are there or on their way
   static constexpr uint32_t TERM = RA * kLtRows * 128;
   __host__ __device__ static constexpr uint32_t stage(int rank16) { return kLtXBytes + rank16 * 128; }
-  // the stages of the sums, and later the terms and two rounds' columns, in the same place
+  // the stages of the sums, and later the terms and the rounds' columns, in the same place
   __host__ __device__ static constexpr uint32_t bytes(int rank16, int terms) {
-    return (kLtStages * stage(rank16) > terms * TERM + 2 * UP ? kLtStages * stage(rank16) : terms * TERM + 2 * UP) + 1024;
+    return (kLtStages * stage(rank16) > terms * TERM + UPS * UP ? kLtStages * stage(rank16) : terms * TERM + UPS * UP) + 1024;
   }
 };
 
-// A lane of 32 reads two neighbouring columns of each eight, of 32, of rows lane / 4 (r[4 j], r[4 j + 1]) and lane / 4 + 8.
+// Column 32 g + 8 t + 2 i + b of a round stands in its buffer at 32 i + 8 g + 2 t + b.  Of 16 rows, a lane reads columns
+// 2 t and 2 t + 1 (t = lane % 4) of the eight at 32 i + 8 g for each i: r[4 i + b] of row lane / 4, r[4 i + 2 + b] of row lane / 4 + 8.
 __device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x4.b32"
-      " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-}
-
-// Where column c of a round stands in its buffer: of 64, a lane t of four has columns 8 t to 8 t + 7 of each 32, column
-// 32 k + 8 t + 2 i + b at 8 (4 k + i) + 2 t + b.
-__device__ __forceinline__ int lt_column(int c) {
-  return (c & 64) | ((c >> 5 & 1) * 4 + (c >> 1 & 3)) * 8 | (c >> 3 & 3) * 2 | (c & 1);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[4 * i]), "=r"(r[4 * i + 1]), "=r"(r[4 * i + 2]), "=r"(r[4 * i + 3])
+                 : "r"(taddr + 32 * i));
 }
 
 // Where 16 bytes of a 128-byte row stand under the 128-byte swizzle.
 __device__ __forceinline__ uint32_t lt_place(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
 
 template <int RA, bool F32>
-__global__ void __launch_bounds__(kLtThreads, RA == 1 && !F32 ? 2 : 1) low_rank_tile_kernel(const __grid_constant__ LowRankArgs a) {
+__global__ void __launch_bounds__(kLtThreads, 1) low_rank_tile_kernel(const __grid_constant__ LowRankArgs a, const __grid_constant__ CUtensorMap x_map,
+                         const __grid_constant__ CUtensorMap down_map, const __grid_constant__ CUtensorMap up_map) {
   using S = LtShape<RA>;
   extern __shared__ uint8_t lt_smem[];
   __shared__ LrGroups<kLtRows> s;
-  __shared__ uint64_t stage_bar[kLtStages], full_bar[2], empty_bar[2];
+  __shared__ uint64_t copied_bar[kLtStages], free_bar[kLtStages], stage_bar[kLtStages];
+  __shared__ uint64_t up_bar[S::UPS], full_bar[2], empty_bar[2];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
 
@@ -78,12 +76,16 @@ __global__ void __launch_bounds__(kLtThreads, RA == 1 && !F32 ? 2 : 1) low_rank_
   uint8_t* const smem = align_1024(lt_smem);
   const uint32_t smem0 = smem_u32(smem);
   const int rank16 = (a.rank + 15) / 16 * 16, parts = a.out_f32 ? 3 : 2;
-  const uint32_t up0 = smem0 + parts * S::TERM;
   if (tid == 0) {
-    for (int i = 0; i < kLtStages; ++i) mbar_init(&stage_bar[i], 1);
+    for (int i = 0; i < kLtStages; ++i) {
+      mbar_init(&copied_bar[i], 1);
+      mbar_init(&free_bar[i], 1);
+      mbar_init(&stage_bar[i], 1);
+    }
+    for (int i = 0; i < S::UPS; ++i) mbar_init(&up_bar[i], 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&full_bar[i], 1);
-      mbar_init(&empty_bar[i], kLrWarps);
+      mbar_init(&empty_bar[i], kLtWorkers / 32);
     }
     fence_barrier_init();
     abort_flag = 0;
@@ -109,96 +111,112 @@ __global__ void __launch_bounds__(kLtThreads, RA == 1 && !F32 ? 2 : 1) low_rank_
   const int round0 = all_rounds * part / split, rounds = all_rounds * (part + 1) / split - round0;
   const float nan = __int_as_float(0x7fffffff);
   const uint32_t sums_tmem = tmem + 128;  // the second round's columns: free until then
-  uint32_t steps_done = 0, rounds_done = 0;
+  const bool feeds = tid == kLtWorkers;  // the thread that copies and issues
+  uint32_t steps_done = 0, copied_done = 0, rounds_done = 0;
 
   for (int group = split == 1 ? mine : part < split ? mine % groups : groups; group < groups;
        group += split == 1 ? a.clusters : groups) {
     const int adapter = s.key[s.lead[group]];
     if (adapter < 0 && a.skip_bare) continue;
     tc_fence_before();
+    fence_proxy_async_smem();
     if (__syncthreads_or(abort_flag)) break;
     const int many = s.take(group, n, a.group);
     const bool bad = adapter >= a.count, bare = adapter < 0 || bad;
     const __nv_bfloat16* const up = a.up + static_cast<int64_t>(bare ? 0 : adapter) * a.outer * a.rank;
 
-    // 128 columns of up, K-major, by the feeders; ranks past the adapter's up to a multiple of 16, and columns past the last, are zero
-    auto load_up = [&](int round) {
-      const uint32_t to = up0 + (round & 1) * S::UP;
-      const int part2 = tid % 2;  // two threads a column
-      for (int col = (tid - kLrThreads) / 2; col < kLtColumns; col += kLtFeeders / 2) {
-        const int at = (round0 + round) * kLtColumns + col, row = lt_column(col);
-        const __nv_bfloat16* const from = up + (at < a.outer ? static_cast<int64_t>(at) * a.rank : 0);
-        for (int chunk = part2; chunk < rank16 / 8; chunk += 2) {
-          const bool in = at < a.outer && chunk * 8 < a.rank;
-          cp_async_or_zero(to + chunk / 8 * (kLtColumns * 128) + lt_place(row, chunk % 8), from + (in ? chunk * 8 : 0), in);
-        }
-      }
-    };
-
     if (!bare) {
       // ---- sums over K
       const int steps = (a.inner + 63) / 64;
       const uint32_t stage_bytes = S::stage(rank16);
-      const __nv_bfloat16* const down = a.down + static_cast<int64_t>(adapter) * a.rank * a.inner;
-      // a thread's pieces: 16 bytes at the same place of every 32nd row
-      const int chunk = tid % 8, row0 = tid / 8;
-      const bool loads = tid < kLrThreads;
-      const __nv_bfloat16* xp[kLtRows / 32];
-#pragma unroll
-      for (int i = 0; i < kLtRows / 32; ++i) xp[i] = a.x + (first + (loads ? max(s.rows[row0 + 32 * i], 0) : 0)) * a.inner + chunk * 8;
-      auto load_stage = [&](int step) {
-        const uint32_t to = smem0 + (steps_done + step) % kLtStages * stage_bytes;
-        const bool in = step * 64 + chunk * 8 < a.inner;
-#pragma unroll
-        for (int i = 0; i < kLtRows / 32; ++i) {
-          const bool take = in && row0 + 32 * i < many;
-          cp_async_or_zero(to + lt_place(row0 + 32 * i, chunk), take ? xp[i] + step * 64 : a.x, take);
-        }
-        for (int row = row0; row < rank16; row += 32) {
-          const bool take = in && row < a.rank;
-          cp_async_or_zero(to + kLtXBytes + lt_place(row, chunk),
-                           down + (take ? static_cast<int64_t>(row) * a.inner + step * 64 + chunk * 8 : 0), take);
-        }
-      };
-      for (int i = 0; i < kLtStages - 1; ++i) {
-        if (i < steps && loads) load_stage(i);
-        cp_async_commit();
-      }
       const uint32_t idesc = umma_idesc_bf16(kLtRows, rank16, false, false);
-      for (int step = 0; step < steps; ++step) {
-        cp_async_wait<kLtStages - 2>();
-        fence_proxy_async_smem();
-        if (__syncthreads_or(abort_flag)) break;
-        const uint32_t slot = (steps_done + step) % kLtStages;
-        if (tid == 0) {
-          tc_fence_after();
-          const uint32_t x = smem0 + slot * stage_bytes, w = x + kLtXBytes;
-          for (int k = 0; k < 4; ++k)
-            umma_bf16_ss(sums_tmem, sw128_desc(x + k * 32, 16, 1024), sw128_desc(w + k * 32, 16, 1024), idesc, step + k > 0);
-          umma_commit(&stage_bar[slot]);
+      auto add_step = [&](uint32_t slot, bool more, uint64_t* bar) {
+        tc_fence_after();
+        const uint32_t x = smem0 + slot * stage_bytes, w = x + kLtXBytes;
+        for (int k = 0; k < 4; ++k)
+          umma_bf16_ss(sums_tmem, sw128_desc(x + k * 32, 16, 1024), sw128_desc(w + k * 32, 16, 1024), idesc, more || k > 0);
+        umma_commit(bar);
+      };
+      if (s.rows[many - 1] - s.rows[0] == many - 1) {
+        // rows in a row; those behind the group's come along, and what becomes of them is not written
+        if (feeds) {
+          const int row = static_cast<int>(first) + s.rows[0];
+          int asked = 0, used = 0;
+          for (; used < steps; ) {
+            bool ok = true;
+            if (asked < steps && asked <= used + kLtAhead) {
+              const uint32_t at = copied_done + asked, slot = at % kLtStages;
+              if (asked >= kLtStages) ok = mbar_wait(&free_bar[slot], at / kLtStages & 1 ^ 1, kErrLowRankWait, &abort_flag);
+              if (!ok) break;
+              mbar_arrive_expect_tx(&copied_bar[slot], stage_bytes);
+              tma_load_2d(smem + slot * stage_bytes, &x_map, &copied_bar[slot], asked * 64, row);
+              tma_load_2d(smem + slot * stage_bytes + kLtXBytes, &down_map, &copied_bar[slot], asked * 64, adapter * a.rank);
+              ++asked;
+              continue;
+            }
+            const uint32_t at = copied_done + used, slot = at % kLtStages;
+            if (!mbar_wait(&copied_bar[slot], at / kLtStages & 1, kErrLowRankWait, &abort_flag)) break;
+            add_step(slot, used > 0, &free_bar[slot]);
+            ++used;
+          }
+          for (; used < asked; ++used) {  // given up: no copy is left on its way
+            const uint32_t at = copied_done + used;
+            mbar_drain_wait(&copied_bar[at % kLtStages], at / kLtStages & 1);
+          }
         }
-        // the stage before is free when its UMMAs are done
-        if (step > 0) {
-          const uint32_t at = steps_done + step - 1;
-          mbar_wait(&stage_bar[at % kLtStages], at / kLtStages & 1, kErrLowRankWait, &abort_flag);
+        const uint32_t at = copied_done + steps - 1;
+        mbar_wait(&free_bar[at % kLtStages], at / kLtStages & 1, kErrLowRankWait, &abort_flag);
+        copied_done += steps;
+      } else {
+        const __nv_bfloat16* const down = a.down + static_cast<int64_t>(adapter) * a.rank * a.inner;
+        // a thread's pieces: 16 bytes at the same place of every 64th row
+        constexpr int APART = kLtWorkers / 8;
+        const int chunk = tid % 8, row0 = tid / 8;
+        const bool loads = tid < kLtWorkers;
+        const __nv_bfloat16* xp[kLtRows / APART];
+#pragma unroll
+        for (int i = 0; i < kLtRows / APART; ++i)
+          xp[i] = a.x + (first + (loads ? max(s.rows[row0 + APART * i], 0) : 0)) * a.inner + chunk * 8;
+        auto load_stage = [&](int step) {
+          const uint32_t to = smem0 + (steps_done + step) % kLtStages * stage_bytes;
+          const bool in = step * 64 + chunk * 8 < a.inner;
+#pragma unroll
+          for (int i = 0; i < kLtRows / APART; ++i) {
+            const bool take = in && row0 + APART * i < many;
+            cp_async_or_zero(to + lt_place(row0 + APART * i, chunk), take ? xp[i] + step * 64 : a.x, take);
+          }
+          for (int row = row0; row < rank16; row += APART) {
+            const bool take = in && row < a.rank;
+            cp_async_or_zero(to + kLtXBytes + lt_place(row, chunk),
+                             down + (take ? static_cast<int64_t>(row) * a.inner + step * 64 + chunk * 8 : 0), take);
+          }
+        };
+        for (int i = 0; i < kLtStages - 1; ++i) {
+          if (i < steps && loads) load_stage(i);
+          cp_async_commit();
         }
-        if (step + kLtStages - 1 < steps && loads) load_stage(step + kLtStages - 1);
-        cp_async_commit();
-      }
-      if (abort_flag == 0) {
+        for (int step = 0; step < steps; ++step) {
+          cp_async_wait<kLtStages - 2>();
+          fence_proxy_async_smem();
+          if (__syncthreads_or(abort_flag)) break;
+          const uint32_t at = steps_done + step;
+          if (feeds) add_step(at % kLtStages, step > 0, &stage_bar[at % kLtStages]);
+          // the stage before is free when its UMMAs are done
+          if (step > 0) mbar_wait(&stage_bar[(at - 1) % kLtStages], (at - 1) / kLtStages & 1, kErrLowRankWait, &abort_flag);
+          if (step + kLtStages - 1 < steps && loads) load_stage(step + kLtStages - 1);
+          cp_async_commit();
+        }
         const uint32_t at = steps_done + steps - 1;
-        mbar_wait(&stage_bar[at % kLtStages], at / kLtStages & 1, kErrLowRankWait, &abort_flag);
+        if (abort_flag == 0) mbar_wait(&stage_bar[at % kLtStages], at / kLtStages & 1, kErrLowRankWait, &abort_flag);
+        cp_async_wait<0>();
+        steps_done += steps;
       }
-      cp_async_wait<0>();
-      if (__syncthreads_or(abort_flag)) {  // else every stage is read: its place is free
-        break;
-      }
-      steps_done += steps;
+      if (__syncthreads_or(abort_flag)) break;  // else every stage is read: its place is free
       tc_fence_after();
       // ---- terms
       const float scale = __ldg(a.scales + adapter);
       const int row = warp % 4 * 32 + lane;
-      for (int col = warp / 4 * 32; loads && col < rank16; col += 64) {
+      if (const int col = warp / 4 * 32; warp < kLtWorkers / 32 && col < rank16) {
         uint32_t r[32];
         tmem_ld_32cols(sums_tmem + (static_cast<uint32_t>(warp % 4 * 32) << 16) + col, r);
         tmem_wait_ld();
@@ -229,19 +247,28 @@ __global__ void __launch_bounds__(kLtThreads, RA == 1 && !F32 ? 2 : 1) low_rank_
     }
 
     // ---- columns
-    if (tid >= kLrThreads) {
-      // feeders
-      const uint32_t idesc = umma_idesc_bf16(kLtRows, kLtColumns, false, false);
-      if (!bare) load_up(0);
-      for (int j = 0; j < rounds && !bare; ++j) {
-        cp_async_commit();
-        cp_async_wait<0>();
-        fence_proxy_async_smem();
-        asm volatile("bar.sync 1, %0;" ::"n"(kLtFeeders) : "memory");
-        const uint32_t at = rounds_done + j, buffer = at & 1;
-        if (tid == kLrThreads && mbar_wait(&empty_bar[buffer], (at >> 1 & 1) ^ 1, kErrLowRankWait, &abort_flag)) {
+    if (tid >= kLtWorkers) {
+      if (feeds && !bare) {
+        const uint32_t idesc = umma_idesc_bf16(kLtRows, kLtColumns, false, false);
+        const uint8_t* const up_smem = smem + parts * S::TERM;
+        // 8 columns of up are one of the map's outermost dimension; those past the adapter's last come along
+        const int eight0 = static_cast<int>((static_cast<int64_t>(adapter) * a.outer + round0 * kLtColumns) / 8);
+        auto ask = [&](int round) {
+          const uint32_t slot = (rounds_done + round) % S::UPS;
+          uint8_t* const to = const_cast<uint8_t*>(up_smem) + slot * S::UP;
+          mbar_arrive_expect_tx(&up_bar[slot], S::UP);
+#pragma unroll
+          for (int r = 0; r < 4 * RA; ++r)
+            tma_load_3d(to + r * 32 * 128, &up_map, &up_bar[slot], r / 4 * 64, r % 4 * 2, eight0 + round * (kLtColumns / 8));
+        };
+        int asked = 0, used = 0;
+        for (; asked < S::UPS - 1 && asked < rounds; ++asked) ask(asked);
+        for (; used < rounds; ++used) {
+          const uint32_t at = rounds_done + used, buffer = at & 1, slot = at % S::UPS;
+          if (!mbar_wait(&up_bar[slot], at / S::UPS & 1, kErrLowRankWait, &abort_flag)) break;
+          if (!mbar_wait(&empty_bar[buffer], (at >> 1 & 1) ^ 1, kErrLowRankWait, &abort_flag)) break;
           tc_fence_after();
-          const uint32_t w = up0 + (j & 1) * S::UP;
+          const uint32_t w = smem_u32(up_smem) + slot * S::UP;
           uint32_t more = 0;
           for (int k = 0; k < parts; ++k) {
             for (int r = 0; r < rank16 / 16; ++r) {
@@ -251,37 +278,44 @@ __global__ void __launch_bounds__(kLtThreads, RA == 1 && !F32 ? 2 : 1) low_rank_
             }
           }
           umma_commit(&full_bar[buffer]);
+          if (asked < rounds) {
+            // into the place of the round before, when that is done
+            if (used > 0 && !mbar_wait(&full_bar[(at - 1) & 1], (at - 1) >> 1 & 1, kErrLowRankWait, &abort_flag)) {
+              ++used;
+              break;
+            }
+            ask(asked++);
+          }
         }
-        if (j + 1 < rounds) {
-          // the other columns' place is free when the round before is done
-          if (j > 0) mbar_wait(&full_bar[(at - 1) & 1], (at - 1) >> 1 & 1, kErrLowRankWait, &abort_flag);
-          load_up(j + 1);
+        for (; used < asked; ++used) {  // given up: no copy is left on its way
+          const uint32_t at = rounds_done + used;
+          mbar_drain_wait(&up_bar[at % S::UPS], at / S::UPS & 1);
         }
       }
       if (!bare) rounds_done += rounds;
       continue;
     }
-    const int quarter = warp % 4 * 32, half = warp / 4 * 64;
-    // This lane's values: twice 8 neighbouring columns of four rows.  Places in the window have 32 bits (256 rows of 2^24 columns).
+    const int quarter = warp % 4 * 32, columns = warp / 4 * 32;  // this warp's rows and columns of a round
+    // This lane's values: 8 neighbouring columns of four rows.  Places in the window have 32 bits (256 rows of 2^24 columns).
     uint32_t place[4];
     uint32_t live = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = s.rows[quarter + i * 8 + lane / 4];
       live |= static_cast<uint32_t>(row >= 0) << i;
-      place[i] = static_cast<uint32_t>(max(row, 0)) * a.outer + half + lane % 4 * 8;
+      place[i] = static_cast<uint32_t>(max(row, 0)) * a.outer + columns + lane % 4 * 8;
     }
     const uint8_t* const base0 = static_cast<const uint8_t*>(a.base) + first * a.outer * (F32 ? 4 : 2);
     uint8_t* const out0 = static_cast<uint8_t*>(a.out) + first * a.outer * (a.out_f32 ? 4 : 2);
     // A warp with all its rows takes whole rounds without a check between the values; base's are on their way then a
-    // round before they are wanted: rows 2 i and 2 i + 1 of the four, columns 32 k and on.
+    // round before they are wanted: rows 2 i and 2 i + 1 of the four.
     const bool plain = __all_sync(0xffffffffu, live == 0xf) && !bare;
     auto whole = [&](int round) { return plain && (round0 + round + 1) * kLtColumns <= a.outer; };
-    LrEight<F32> ahead[2][2][2];
-    auto load_base = [&](int round, int i, int k) {
+    LrEight<F32> ahead[2][2];
+    auto load_base = [&](int round, int i) {
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        ahead[i][k][e].load(base0 + static_cast<uint64_t>(place[2 * i + e] + ((round0 + round) * kLtColumns + k * 32)) * (F32 ? 4 : 2));
+        ahead[i][e].load(base0 + static_cast<uint64_t>(place[2 * i + e] + (round0 + round) * kLtColumns) * (F32 ? 4 : 2));
     };
     auto store = [&](uint8_t* to, float (&y)[8]) {
       if (a.out_f32) {
@@ -302,7 +336,7 @@ __global__ void __launch_bounds__(kLtThreads, RA == 1 && !F32 ? 2 : 1) low_rank_
     };
     if (whole(0)) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) load_base(0, i / 2, i % 2);
+      for (int i = 0; i < 2; ++i) load_base(0, i);
     }
     for (int j = 0; j < rounds; ++j) {
       const uint32_t at = rounds_done + j;
@@ -311,7 +345,7 @@ __global__ void __launch_bounds__(kLtThreads, RA == 1 && !F32 ? 2 : 1) low_rank_
       tc_fence_after();
       const uint32_t column = (round0 + j) * kLtColumns;
       const int size = a.out_f32 ? 4 : 2;
-      const uint32_t d = tmem + (at & 1) * 128 + (static_cast<uint32_t>(quarter) << 16) + half;
+      const uint32_t d = tmem + (at & 1) * 128 + (static_cast<uint32_t>(quarter) << 16) + columns / 4;
       auto done = [&]() {  // the buffer is read
         tc_fence_before();
         __syncwarp();
@@ -321,38 +355,35 @@ __global__ void __launch_bounds__(kLtThreads, RA == 1 && !F32 ? 2 : 1) low_rank_
         const bool more = j + 1 < rounds && whole(j + 1);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
+          uint32_t r[16];
+          tmem_ld_16x32(d + (static_cast<uint32_t>(i * 16) << 16), r);
+          float y[2][8];
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            uint32_t r[16];
-            tmem_ld_16x32(d + (static_cast<uint32_t>(i * 16) << 16) + k * 32, r);
-            float y[2][8];
+          for (int e = 0; e < 2; ++e) ahead[i][e].values(y[e]);
+          if (more) load_base(j + 1, i);
+          tmem_wait_ld();
+          if (i == 1) done();
 #pragma unroll
-            for (int e = 0; e < 2; ++e) ahead[i][k][e].values(y[e]);
-            if (more) load_base(j + 1, i, k);
-            tmem_wait_ld();
-            if (i == 1 && k == 1) done();
+          for (int e = 0; e < 2; ++e) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-#pragma unroll
-              for (int m = 0; m < 8; ++m) y[e][m] += __uint_as_float(r[m / 2 * 4 + 2 * e + m % 2]);
-              store(out0 + static_cast<uint64_t>(place[2 * i + e] + (column + k * 32)) * size, y[e]);
-            }
+            for (int m = 0; m < 8; ++m) y[e][m] += __uint_as_float(r[m / 2 * 4 + 2 * e + m % 2]);
+            store(out0 + static_cast<uint64_t>(place[2 * i + e] + column) * size, y[e]);
           }
         }
         continue;
       }
       // rows or columns are missing, or there is nothing to add
 #pragma unroll 1
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 2; ++i) {
         uint32_t r[16] = {};
         if (!bare) {
-          tmem_ld_16x32(d + (static_cast<uint32_t>(i / 2 * 16) << 16) + i % 2 * 32, r);
+          tmem_ld_16x32(d + (static_cast<uint32_t>(i * 16) << 16), r);
           tmem_wait_ld();
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const uint32_t here = column + half + lane % 4 * 8 + i % 2 * 32;
-          const int row = s.rows[quarter + i / 2 * 16 + e * 8 + lane / 4];
+          const uint32_t here = column + columns + lane % 4 * 8;
+          const int row = s.rows[quarter + i * 16 + e * 8 + lane / 4];
           if (row < 0 || here >= static_cast<uint32_t>(a.outer)) continue;
           const uint64_t from = static_cast<uint64_t>(static_cast<uint32_t>(row) * a.outer + here);
           LrEight<F32> base;

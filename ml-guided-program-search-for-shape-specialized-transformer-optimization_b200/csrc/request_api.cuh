@@ -51,14 +51,14 @@ cudaError_t launch_low_rank_io(b200tx::LowRankArgs& a, bool f32, DeviceState* de
 }
 
 template <int RA, bool F32>
-cudaError_t launch_low_rank_tile(b200tx::LowRankArgs& a, DeviceState* dev, int index, cudaStream_t stream) {
+int launch_low_rank_tile(b200tx::LowRankArgs& a, DeviceState* dev, int index, cudaStream_t stream) {
   using S = b200tx::LtShape<RA>;
   constexpr int kMost = 215 * 1024;
   static_assert(S::bytes(RA * 64, 3) <= kMost, "the terms do not fit");
   if (!dev->low_rank_tile_attr[index]) {
     cudaError_t err = cudaFuncSetAttribute(b200tx::low_rank_tile_kernel<RA, F32>,
                                            cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
-    if (err != cudaSuccess) return err;
+    if (err != cudaSuccess) return cuda_fail(err, "low_rank_add");
     dev->low_rank_tile_attr[index] = true;
   }
   const int rank16 = (a.rank + 15) / 16 * 16;
@@ -68,12 +68,24 @@ cudaError_t launch_low_rank_tile(b200tx::LowRankArgs& a, DeviceState* dev, int i
   a.group = b200tx::kLtRows;
   const int64_t least = (rows + a.group - 1) / a.group;
   // The columns are cut into parts, for each of which the sums are taken anew, while all CTAs then run at once.
-  const int64_t resident = dev->sm_count * (RA == 1 && !F32 && bytes <= kLrTwo ? 2 : 1);
+  const int64_t resident = dev->sm_count;
   const int64_t rounds = (a.outer + b200tx::kLtColumns - 1) / b200tx::kLtColumns;
   a.parts = static_cast<int>(std::min(rounds, std::max<int64_t>(1, resident / (windows * least))));
   a.clusters = static_cast<int>(least * a.parts);
-  return launch(b200tx::low_rank_tile_kernel<RA, F32>, dim3(static_cast<unsigned>(windows * a.clusters)),
-                dim3(b200tx::kLtThreads), static_cast<size_t>(bytes), stream, a);
+  using u64 = uint64_t;
+  CUtensorMap x_map, down_map, up_map;
+  const u64 inner = a.inner, rank = a.rank, count = a.count;
+  const u64 x_dims[2] = {inner, static_cast<u64>(a.rows)}, down_dims[2] = {inner, count * rank}, k_stride[1] = {inner * 2};
+  const uint32_t x_box[2] = {64, b200tx::kLtRows}, down_box[2] = {64, static_cast<uint32_t>(rank16)};
+  const u64 up_dims[3] = {rank, 8, count * a.outer / 8}, up_strides[2] = {rank * 2, rank * 16};
+  const uint32_t up_box[3] = {64, 2, b200tx::kLtColumns / 8};
+  int rc = encode_bf16_map(&x_map, a.x, 2, x_dims, k_stride, x_box);
+  if (rc == B200TX_OK) rc = encode_bf16_map(&down_map, a.down, 2, down_dims, k_stride, down_box);
+  if (rc == B200TX_OK) rc = encode_bf16_map(&up_map, a.up, 3, up_dims, up_strides, up_box);
+  if (rc != B200TX_OK) return rc;
+  cudaError_t err = launch(b200tx::low_rank_tile_kernel<RA, F32>, dim3(static_cast<unsigned>(windows * a.clusters)),
+                           dim3(b200tx::kLtThreads), static_cast<size_t>(bytes), stream, a, x_map, down_map, up_map);
+  return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "low_rank_add");
 }
 
 // Many rows with runs of one adapter go by 128 on tcgen05, where rows of base and the result are multiples of 16 bytes.
@@ -188,11 +200,10 @@ int b200tx_low_rank_add(const void* x, const void* base, int base_dtype, void* o
   a.gelu = epilogue == B200TX_EPI_BIAS_GELU;
   a.skip_bare = base == out && !a.gelu;
   const bool f32 = base_dtype == B200TX_F32;
-  if (M >= kLtLeastRows && a.per_index >= kLtLeastRun && N % 8 == 0) {
-    cudaError_t err = rank <= 64 ? f32 ? launch_low_rank_tile<1, true>(a, dev, 0, stream) : launch_low_rank_tile<1, false>(a, dev, 1, stream)
-                      : f32      ? launch_low_rank_tile<2, true>(a, dev, 2, stream)
-                                 : launch_low_rank_tile<2, false>(a, dev, 3, stream);
-    return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "low_rank_add");
+  if (M >= kLtLeastRows && a.per_index >= kLtLeastRun && N % 8 == 0 && adapters * N < (int64_t{1} << 34)) {
+    return rank <= 64 ? f32 ? launch_low_rank_tile<1, true>(a, dev, 0, stream) : launch_low_rank_tile<1, false>(a, dev, 1, stream)
+           : f32      ? launch_low_rank_tile<2, true>(a, dev, 2, stream)
+                      : launch_low_rank_tile<2, false>(a, dev, 3, stream);
   }
   cudaError_t err = rank <= 16   ? launch_low_rank_io<1>(a, f32, dev, 0, stream)
                     : rank <= 32 ? launch_low_rank_io<2>(a, f32, dev, 4, stream)
