@@ -17,8 +17,9 @@
 // an adapter are read (from L2) once for 128 rows.  The warp MMA form of this reads them for every 32 rows
 // and keeps the tensor pipe busy for as long as the bytes take.
 //
-// One thread brings the stages and up's columns and issues the UMMAs; 16 warps make the terms and bring the results
-// out, each for itself: they meet the thread at the buffers' barriers only.  Waits are bounded as everywhere.
+// One thread brings the stages and up's columns, one of another warp issues the UMMAs (in one thread the two take 0.57 us
+// for a stage); 16 warps make the terms and bring the results out, each for itself: they all meet at the
+// buffers' barriers only.  Waits are bounded as everywhere.
 #pragma once
 
 #include "kv8_attention_kernels.cuh"
@@ -32,8 +33,7 @@ constexpr int kLtStages = 6;             // of 64 values of K
 constexpr uint32_t kLtXBytes = kLtRows * 128;
 constexpr int kErrLowRankWait = 0x501;
 constexpr int kLtWorkers = 512;          // threads that make the terms and bring the results out
-constexpr int kLtThreads = kLtWorkers + 32;
-constexpr int kLtAhead = kLtStages - 2;  // stages that are asked for before one is used
+constexpr int kLtThreads = kLtWorkers + 64;
 
 // RA atoms of 64 ranks.
 template <int RA>
@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(kLtThreads, 1) low_rank_tile_kernel(const __gr
   extern __shared__ uint8_t lt_smem[];
   __shared__ LrGroups<kLtRows> s;
   __shared__ uint64_t copied_bar[kLtStages], free_bar[kLtStages], stage_bar[kLtStages];
-  __shared__ uint64_t up_bar[S::UPS], full_bar[2], empty_bar[2];
+  __shared__ uint64_t up_bar[S::UPS], up_free_bar[S::UPS], full_bar[2], empty_bar[2];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
 
@@ -82,7 +82,10 @@ __global__ void __launch_bounds__(kLtThreads, 1) low_rank_tile_kernel(const __gr
       mbar_init(&free_bar[i], 1);
       mbar_init(&stage_bar[i], 1);
     }
-    for (int i = 0; i < S::UPS; ++i) mbar_init(&up_bar[i], 1);
+    for (int i = 0; i < S::UPS; ++i) {
+      mbar_init(&up_bar[i], 1);
+      mbar_init(&up_free_bar[i], 1);
+    }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&full_bar[i], 1);
       mbar_init(&empty_bar[i], kLtWorkers / 32);
@@ -111,8 +114,10 @@ __global__ void __launch_bounds__(kLtThreads, 1) low_rank_tile_kernel(const __gr
   const int round0 = all_rounds * part / split, rounds = all_rounds * (part + 1) / split - round0;
   const float nan = __int_as_float(0x7fffffff);
   const uint32_t sums_tmem = tmem + 128;  // the second round's columns: free until then
-  const bool feeds = tid == kLtWorkers;  // the thread that copies and issues
+  const uint64_t smem_desc = sw128_desc(smem0, 16, 1024);  // an operand's place is its 16-byte units more
+  const bool copies = tid == kLtWorkers, issues = tid == kLtWorkers + 32;
   uint32_t steps_done = 0, copied_done = 0, rounds_done = 0;
+  uint32_t asked = 0, asked_up = 0;  // copies that the copying thread has asked for, of stages and of up's columns
 
   for (int group = split == 1 ? mine : part < split ? mine % groups : groups; group < groups;
        group += split == 1 ? a.clusters : groups) {
@@ -132,40 +137,35 @@ __global__ void __launch_bounds__(kLtThreads, 1) low_rank_tile_kernel(const __gr
       const uint32_t idesc = umma_idesc_bf16(kLtRows, rank16, false, false);
       auto add_step = [&](uint32_t slot, bool more, uint64_t* bar) {
         tc_fence_after();
-        const uint32_t x = smem0 + slot * stage_bytes, w = x + kLtXBytes;
-        for (int k = 0; k < 4; ++k)
-          umma_bf16_ss(sums_tmem, sw128_desc(x + k * 32, 16, 1024), sw128_desc(w + k * 32, 16, 1024), idesc, more || k > 0);
+        const uint64_t x = smem_desc + (slot * stage_bytes >> 4), w = x + (kLtXBytes >> 4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) umma_bf16_ss(sums_tmem, x + 2 * k, w + 2 * k, idesc, more || k > 0);
         umma_commit(bar);
       };
       if (s.rows[many - 1] - s.rows[0] == many - 1) {
         // rows in a row; those behind the group's come along, and what becomes of them is not written
-        if (feeds) {
+        if (copies) {
           const int row = static_cast<int>(first) + s.rows[0];
-          int asked = 0, used = 0;
-          for (; used < steps; ) {
-            bool ok = true;
-            if (asked < steps && asked <= used + kLtAhead) {
-              const uint32_t at = copied_done + asked, slot = at % kLtStages;
-              if (asked >= kLtStages) ok = mbar_wait(&free_bar[slot], at / kLtStages & 1 ^ 1, kErrLowRankWait, &abort_flag);
-              if (!ok) break;
-              mbar_arrive_expect_tx(&copied_bar[slot], stage_bytes);
-              tma_load_2d(smem + slot * stage_bytes, &x_map, &copied_bar[slot], asked * 64, row);
-              tma_load_2d(smem + slot * stage_bytes + kLtXBytes, &down_map, &copied_bar[slot], asked * 64, adapter * a.rank);
-              ++asked;
-              continue;
-            }
-            const uint32_t at = copied_done + used, slot = at % kLtStages;
-            if (!mbar_wait(&copied_bar[slot], at / kLtStages & 1, kErrLowRankWait, &abort_flag)) break;
-            add_step(slot, used > 0, &free_bar[slot]);
-            ++used;
+          uint32_t slot = copied_done % kLtStages, phase = copied_done / kLtStages & 1;
+          for (int step = 0; step < steps; ++step) {
+            if (!mbar_wait(&free_bar[slot], phase ^ 1, kErrLowRankWait, &abort_flag)) break;
+            mbar_arrive_expect_tx(&copied_bar[slot], stage_bytes);
+            tma_load_2d(smem + slot * stage_bytes, &x_map, &copied_bar[slot], step * 64, row);
+            tma_load_2d(smem + slot * stage_bytes + kLtXBytes, &down_map, &copied_bar[slot], step * 64, adapter * a.rank);
+            if (++slot == kLtStages) slot = 0, phase ^= 1;
+            ++asked;
           }
-          for (; used < asked; ++used) {  // given up: no copy is left on its way
-            const uint32_t at = copied_done + used;
-            mbar_drain_wait(&copied_bar[at % kLtStages], at / kLtStages & 1);
+        } else if (issues) {
+          uint32_t slot = copied_done % kLtStages, phase = copied_done / kLtStages & 1;
+          for (int step = 0; step < steps; ++step) {
+            if (!mbar_wait(&copied_bar[slot], phase, kErrLowRankWait, &abort_flag)) break;
+            add_step(slot, step > 0, &free_bar[slot]);
+            if (++slot == kLtStages) slot = 0, phase ^= 1;
           }
+          // the others wait at the barrier below, which costs no instructions that this thread would wait behind
+          const uint32_t at = copied_done + steps - 1;
+          mbar_wait(&free_bar[at % kLtStages], at / kLtStages & 1, kErrLowRankWait, &abort_flag);
         }
-        const uint32_t at = copied_done + steps - 1;
-        mbar_wait(&free_bar[at % kLtStages], at / kLtStages & 1, kErrLowRankWait, &abort_flag);
         copied_done += steps;
       } else {
         const __nv_bfloat16* const down = a.down + static_cast<int64_t>(adapter) * a.rank * a.inner;
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(kLtThreads, 1) low_rank_tile_kernel(const __gr
           fence_proxy_async_smem();
           if (__syncthreads_or(abort_flag)) break;
           const uint32_t at = steps_done + step;
-          if (feeds) add_step(at % kLtStages, step > 0, &stage_bar[at % kLtStages]);
+          if (issues) add_step(at % kLtStages, step > 0, &stage_bar[at % kLtStages]);
           // the stage before is free when its UMMAs are done
           if (step > 0) mbar_wait(&stage_bar[(at - 1) % kLtStages], (at - 1) / kLtStages & 1, kErrLowRankWait, &abort_flag);
           if (step + kLtStages - 1 < steps && loads) load_stage(step + kLtStages - 1);
@@ -248,48 +248,40 @@ __global__ void __launch_bounds__(kLtThreads, 1) low_rank_tile_kernel(const __gr
 
     // ---- columns
     if (tid >= kLtWorkers) {
-      if (feeds && !bare) {
-        const uint32_t idesc = umma_idesc_bf16(kLtRows, kLtColumns, false, false);
-        const uint8_t* const up_smem = smem + parts * S::TERM;
+      if (copies && !bare) {
         // 8 columns of up are one of the map's outermost dimension; those past the adapter's last come along
         const int eight0 = static_cast<int>((static_cast<int64_t>(adapter) * a.outer + round0 * kLtColumns) / 8);
-        auto ask = [&](int round) {
-          const uint32_t slot = (rounds_done + round) % S::UPS;
-          uint8_t* const to = const_cast<uint8_t*>(up_smem) + slot * S::UP;
+        uint32_t slot = rounds_done % S::UPS, phase = rounds_done / S::UPS & 1;
+        for (int j = 0; j < rounds; ++j) {
+          if (!mbar_wait(&up_free_bar[slot], phase ^ 1, kErrLowRankWait, &abort_flag)) break;
+          uint8_t* const to = smem + parts * S::TERM + slot * S::UP;
           mbar_arrive_expect_tx(&up_bar[slot], S::UP);
 #pragma unroll
           for (int r = 0; r < 4 * RA; ++r)
-            tma_load_3d(to + r * 32 * 128, &up_map, &up_bar[slot], r / 4 * 64, r % 4 * 2, eight0 + round * (kLtColumns / 8));
-        };
-        int asked = 0, used = 0;
-        for (; asked < S::UPS - 1 && asked < rounds; ++asked) ask(asked);
-        for (; used < rounds; ++used) {
-          const uint32_t at = rounds_done + used, buffer = at & 1, slot = at % S::UPS;
-          if (!mbar_wait(&up_bar[slot], at / S::UPS & 1, kErrLowRankWait, &abort_flag)) break;
+            tma_load_3d(to + r * 32 * 128, &up_map, &up_bar[slot], r / 4 * 64, r % 4 * 2, eight0 + j * (kLtColumns / 8));
+          if (++slot == S::UPS) slot = 0, phase ^= 1;
+          ++asked_up;
+        }
+      } else if (issues && !bare) {
+        const uint32_t idesc = umma_idesc_bf16(kLtRows, kLtColumns, false, false);
+        uint32_t slot = rounds_done % S::UPS, phase = rounds_done / S::UPS & 1;
+        for (int j = 0; j < rounds; ++j) {
+          const uint32_t at = rounds_done + j, buffer = at & 1;
+          if (!mbar_wait(&up_bar[slot], phase, kErrLowRankWait, &abort_flag)) break;
           if (!mbar_wait(&empty_bar[buffer], (at >> 1 & 1) ^ 1, kErrLowRankWait, &abort_flag)) break;
           tc_fence_after();
-          const uint32_t w = smem_u32(up_smem) + slot * S::UP;
-          uint32_t more = 0;
+          const uint64_t w = smem_desc + (parts * S::TERM + slot * S::UP >> 4);
           for (int k = 0; k < parts; ++k) {
-            for (int r = 0; r < rank16 / 16; ++r) {
-              const uint32_t in = r / 4 * (kLtRows * 128) + r % 4 * 32;
-              umma_bf16_ss(tmem + buffer * 128, sw128_desc(smem0 + k * S::TERM + in, 16, 1024), sw128_desc(w + in, 16, 1024), idesc, more);
-              more = 1;
+#pragma unroll
+            for (int r = 0; r < 4 * RA; ++r) {
+              const uint32_t in = (r / 4 * (kLtRows * 128) + r % 4 * 32) >> 4;
+              if (r * 16 < rank16)
+                umma_bf16_ss(tmem + buffer * 128, smem_desc + (k * S::TERM >> 4) + in, w + in, idesc, k + r > 0);
             }
           }
+          umma_commit(&up_free_bar[slot]);
           umma_commit(&full_bar[buffer]);
-          if (asked < rounds) {
-            // into the place of the round before, when that is done
-            if (used > 0 && !mbar_wait(&full_bar[(at - 1) & 1], (at - 1) >> 1 & 1, kErrLowRankWait, &abort_flag)) {
-              ++used;
-              break;
-            }
-            ask(asked++);
-          }
-        }
-        for (; used < asked; ++used) {  // given up: no copy is left on its way
-          const uint32_t at = rounds_done + used;
-          mbar_drain_wait(&up_bar[at % S::UPS], at / S::UPS & 1);
+          if (++slot == S::UPS) slot = 0, phase ^= 1;
         }
       }
       if (!bare) rounds_done += rounds;
@@ -401,6 +393,12 @@ __global__ void __launch_bounds__(kLtThreads, 1) low_rank_tile_kernel(const __gr
   }
 
   cp_async_wait<0>();
+  if (copies) {  // no copy is left on its way, also where a wait has run out
+    for (uint32_t i = asked > kLtStages ? asked - kLtStages : 0; i < asked; ++i)
+      mbar_drain_wait(&copied_bar[i % kLtStages], i / kLtStages & 1);
+    for (uint32_t i = asked_up > S::UPS ? asked_up - S::UPS : 0; i < asked_up; ++i)
+      mbar_drain_wait(&up_bar[i % S::UPS], i / S::UPS & 1);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

@@ -88,8 +88,11 @@ int launch_low_rank_tile(b200tx::LowRankArgs& a, DeviceState* dev, int index, cu
   return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "low_rank_add");
 }
 
-// Many rows with runs of one adapter go by 128 on tcgen05, where rows of base and the result are multiples of 16 bytes.
-constexpr int64_t kLtLeastRows = 1024, kLtLeastRun = 64;
+// Rows go by 128 on tcgen05 where there are many, in runs of one adapter, and rows of base and the result are multiples of 16
+// bytes.  The warp MMAs' time grows with rows x ranks, the UMMAs' hardly with either, but these begin with a
+// longer chain (1024 rows of 1024 -> 4096: rank 16 12.7 us by warps, 14.8 so; rank 64 19.5 and 15.9; 4096 rows: rank 16 29.4 and 26.7,
+// rank 64 60 and 27.9; 4096 -> 4096 of rank 16 34 and 42, 4096 -> 14336 83 and 76).
+constexpr int64_t kLtLeastRows = 1024, kLtLeastRun = 64, kLtLeastWork = 65536;
 
 int kv8_pool(const char* what, const b200tx_kv8_pool* c, b200tx::Kv8Pool* out) {
   if (c == nullptr) return fail(B200TX_ERR_INVALID_ARGUMENT, "%s: null pool", what);
@@ -200,7 +203,7 @@ int b200tx_low_rank_add(const void* x, const void* base, int base_dtype, void* o
   a.gelu = epilogue == B200TX_EPI_BIAS_GELU;
   a.skip_bare = base == out && !a.gelu;
   const bool f32 = base_dtype == B200TX_F32;
-  if (M >= kLtLeastRows && a.per_index >= kLtLeastRun && N % 8 == 0 && adapters * N < (int64_t{1} << 34)) {
+  if (M >= kLtLeastRows && M * rank >= kLtLeastWork && a.per_index >= kLtLeastRun && N % 8 == 0 && adapters * N < (int64_t{1} << 34)) {
     return rank <= 64 ? f32 ? launch_low_rank_tile<1, true>(a, dev, 0, stream) : launch_low_rank_tile<1, false>(a, dev, 1, stream)
            : f32      ? launch_low_rank_tile<2, true>(a, dev, 2, stream)
                       : launch_low_rank_tile<2, false>(a, dev, 3, stream);

@@ -22,8 +22,12 @@ under meta and fake tensors (tests/solution/test_triton_shape13_attention.py:
   ``scales`` and ``tail`` of a single-layer cache; returns the queries)
 * ``b200tx::kv8_attention``        -- ``sm100_kv8_attention``
 * ``b200tx::linear_w4``            -- ``sm100_linear_w4``
+* ``b200tx::low_rank_add``         -- ``sm100_low_rank_add``
+* ``b200tx::kv8_fork`` / ``b200tx::kv8_reserve`` / ``b200tx::kv8_compact`` -- ``sm100_kv8_fork``,
+  ``sm100_kv8_reserve`` and ``sm100_kv8_compact`` (they write the tables, ``refs`` and what moves)
+* ``b200tx::verify_draft``         -- ``sm100_verify_draft``
 
-But for ``kv8_append`` each operator is functional: it allocates its outputs and launches on the
+But for ``kv8_append`` and those of the pages each operator is functional: it allocates its outputs and launches on the
 current stream of the inputs' CUDA device.  The kernels are inference-only
 (no autograd formula is registered); an operator runs them with gradient
 recording off whatever the caller's grad mode is.  The fake implementations check
@@ -53,9 +57,12 @@ from .attention import (
     sm100_simt_attention,
 )
 from .kv_cache import KV8_BLOCK, KV8_HEAD_DIMS, Kv8Cache, sm100_kv8_append, sm100_kv8_attention
+from .kv_pages import Kv8Pages, sm100_kv8_compact, sm100_kv8_fork, sm100_kv8_reserve
 from .linear_w4 import W4_GROUPS, W4Weight, sm100_linear_w4
+from .low_rank import LOW_RANK_MOST, LowRankAdapters, sm100_low_rank_add
 from .projection import sm100_linear
 from .rotary import ROPE_HEAD_DIMS, RotaryTable, sm100_qk_norm_rope
+from .verify import sm100_verify_draft
 
 NAMESPACE = "b200tx"
 OPERATORS = (
@@ -71,6 +78,11 @@ OPERATORS = (
     "kv8_append",
     "kv8_attention",
     "linear_w4",
+    "low_rank_add",
+    "kv8_fork",
+    "kv8_reserve",
+    "kv8_compact",
+    "verify_draft",
 )
 
 _IO = (torch.float32, torch.bfloat16)
@@ -660,19 +672,214 @@ def _linear_w4_fake(value, packed, scales, bias=None, gelu=False, out_dtype=torc
 linear_w4.register_kernel("cpu")(_no_cpu("linear_w4"))
 
 
+# ---------------------------------------------------------------- batches of many requests
+
+
+def _low_rank_check(
+    value: torch.Tensor,
+    base: torch.Tensor,
+    down: torch.Tensor,
+    up: torch.Tensor,
+    scales: torch.Tensor,
+    indices: torch.Tensor,
+    out_dtype: torch.dtype,
+) -> None:
+    _require(value.dtype == torch.bfloat16 and value.ndim >= 1 and base.dtype in _IO and out_dtype in _IO,
+             "value must be a bfloat16 [..., K] tensor, base and out_dtype float32 or bfloat16")
+    _require(down.dtype == up.dtype == torch.bfloat16 and down.ndim == up.ndim == 3 and down.shape[0] == up.shape[0]
+             and down.shape[1] == up.shape[2], "down must be bfloat16 [count, R, K] and up bfloat16 [count, N, R]")
+    _require(down.shape[1] % 8 == 0 and 0 < down.shape[1] <= LOW_RANK_MOST and down.shape[2] % 8 == 0,
+             f"R must be a multiple of 8 up to {LOW_RANK_MOST}, K a multiple of 8")
+    _require(value.shape[:-1] == base.shape[:-1] and value.shape[-1] == down.shape[2] and base.shape[-1] == up.shape[1],
+             "value, base and the adapters disagree")
+    _require(scales.dtype == torch.float32 and tuple(scales.shape) == (down.shape[0],), "scales must be float32 [count]")
+    _require(indices.dtype == torch.int32 and indices.numel() > 0
+             and (value.numel() // value.shape[-1]) % indices.numel() == 0,
+             "indices must be int32, and divide the rows")
+
+
+@torch.library.custom_op(f"{NAMESPACE}::low_rank_add", mutates_args=(), device_types="cuda")
+def low_rank_add(
+    value: torch.Tensor,
+    base: torch.Tensor,
+    down: torch.Tensor,
+    up: torch.Tensor,
+    scales: torch.Tensor,
+    indices: torch.Tensor,
+    gelu: bool = False,
+    out_dtype: torch.dtype = torch.bfloat16,
+) -> torch.Tensor:
+    """``epilogue(base + scale * (value . down^T) . up^T)`` with each row's adapter (``LowRankAdapters``' tensors)."""
+
+    _low_rank_check(value, base, down, up, scales, indices, out_dtype)
+    with torch.no_grad():
+        out, _ = sm100_low_rank_add(
+            value.contiguous(), base.contiguous(), LowRankAdapters(down, up, scales), indices.contiguous(), gelu=gelu,
+            out_dtype=out_dtype,
+        )
+    return out
+
+
+@low_rank_add.register_fake
+def _low_rank_add_fake(value, base, down, up, scales, indices, gelu=False, out_dtype=torch.bfloat16):  # noqa: ANN001, ANN202, ARG001
+    _low_rank_check(value, base, down, up, scales, indices, out_dtype)
+    return base.new_empty(base.shape, dtype=out_dtype)
+
+
+low_rank_add.register_kernel("cpu")(_no_cpu("low_rank_add"))
+
+
+def _pool_check(
+    codes: torch.Tensor, scales: torch.Tensor, tail: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+    refs: torch.Tensor, *lists: torch.Tensor | None,
+) -> None:
+    _require(codes.ndim == 6, "codes must be a uint8 [layers, pages, 2, Hkv, 64, D] tensor")
+    _cache_check(codes[0], scales[0], tail[0], page_table, lengths)
+    _require(refs.dtype == torch.int32 and tuple(refs.shape) == (codes.shape[1],), "refs must be int32 [pages]")
+    for slots in lists:
+        _require(slots is None or (slots.dtype == torch.int32 and slots.ndim == 1), "slots and counts must be int32 [n]")
+
+
+@torch.library.custom_op(
+    f"{NAMESPACE}::kv8_fork", mutates_args=("tail", "page_table", "lengths", "refs"), device_types="cuda"
+)
+def kv8_fork(
+    codes: torch.Tensor,
+    scales: torch.Tensor,
+    tail: torch.Tensor,
+    page_table: torch.Tensor,
+    lengths: torch.Tensor,
+    refs: torch.Tensor,
+    source: torch.Tensor | None,
+    target: torch.Tensor,
+) -> None:
+    """Slots ``target`` become what slots ``source`` (None: nothing) were; all layers' tensors."""
+
+    _pool_check(codes, scales, tail, page_table, lengths, refs, source, target)
+    pages = Kv8Pages(Kv8Cache(codes, scales, tail, page_table, lengths), refs)
+    sm100_kv8_fork(pages, torch.full_like(target, -1) if source is None else source, target)
+
+
+@kv8_fork.register_fake
+def _kv8_fork_fake(codes, scales, tail, page_table, lengths, refs, source, target):  # noqa: ANN001, ANN202
+    _pool_check(codes, scales, tail, page_table, lengths, refs, source, target)
+    _require(source is None or source.shape == target.shape, "source and target differ in size")
+
+
+kv8_fork.register_kernel("cpu")(_no_cpu("kv8_fork"))
+
+
+@torch.library.custom_op(f"{NAMESPACE}::kv8_reserve", mutates_args=("page_table", "refs"), device_types="cuda")
+def kv8_reserve(
+    codes: torch.Tensor,
+    scales: torch.Tensor,
+    tail: torch.Tensor,
+    page_table: torch.Tensor,
+    lengths: torch.Tensor,
+    refs: torch.Tensor,
+    tokens: int,
+    slots: torch.Tensor | None = None,
+    counts: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Pages for the blocks that the next tokens may fill; returns how many each row lacks."""
+
+    _pool_check(codes, scales, tail, page_table, lengths, refs, slots, counts)
+    pages = Kv8Pages(Kv8Cache(codes, scales, tail, page_table, lengths), refs)
+    return sm100_kv8_reserve(pages, tokens, slots=slots, counts=counts)[0]
+
+
+@kv8_reserve.register_fake
+def _kv8_reserve_fake(codes, scales, tail, page_table, lengths, refs, tokens, slots=None, counts=None):  # noqa: ANN001, ANN202, ARG001
+    _pool_check(codes, scales, tail, page_table, lengths, refs, slots, counts)
+    rows = slots.shape[0] if slots is not None else counts.shape[0] if counts is not None else lengths.shape[0]
+    return lengths.new_empty((rows,))
+
+
+kv8_reserve.register_kernel("cpu")(_no_cpu("kv8_reserve"))
+
+
+@torch.library.custom_op(
+    f"{NAMESPACE}::kv8_compact", mutates_args=("codes", "scales", "page_table", "refs"), device_types="cuda"
+)
+def kv8_compact(
+    codes: torch.Tensor,
+    scales: torch.Tensor,
+    tail: torch.Tensor,
+    page_table: torch.Tensor,
+    lengths: torch.Tensor,
+    refs: torch.Tensor,
+) -> torch.Tensor:
+    """Brings the pages in use to the front; returns how many they are."""
+
+    _pool_check(codes, scales, tail, page_table, lengths, refs)
+    return sm100_kv8_compact(Kv8Pages(Kv8Cache(codes, scales, tail, page_table, lengths), refs))[0]
+
+
+@kv8_compact.register_fake
+def _kv8_compact_fake(codes, scales, tail, page_table, lengths, refs):  # noqa: ANN001, ANN202
+    _pool_check(codes, scales, tail, page_table, lengths, refs)
+    return refs.new_empty((1,))
+
+
+kv8_compact.register_kernel("cpu")(_no_cpu("kv8_compact"))
+
+
+def _verify_check(
+    target: torch.Tensor, drafted: torch.Tensor, uniform: torch.Tensor, draft: torch.Tensor | None,
+    counts: torch.Tensor | None,
+) -> None:
+    _require(target.ndim == 3 and target.dtype in _IO and drafted.ndim == 2 and drafted.dtype in (torch.int32, torch.int64)
+             and target.shape[:2] == (drafted.shape[0], drafted.shape[1] + 1),
+             "target must be a float32 or bfloat16 [B, T + 1, V] tensor, drafted an int32 or int64 [B, T] one")
+    _require(uniform.dtype == torch.float32 and uniform.shape == target.shape[:2], "uniform must be float32 [B, T + 1]")
+    _require(draft is None or (draft.dtype == target.dtype and tuple(draft.shape) == (*drafted.shape, target.shape[2])),
+             "draft must be a [B, T, V] tensor of the target's dtype")
+    _require(counts is None or (counts.dtype == torch.int32 and tuple(counts.shape) == (drafted.shape[0],)),
+             "counts must be int32 [B]")
+
+
+@torch.library.custom_op(f"{NAMESPACE}::verify_draft", mutates_args=(), device_types="cuda")
+def verify_draft(
+    target: torch.Tensor,
+    drafted: torch.Tensor,
+    uniform: torch.Tensor,
+    draft: torch.Tensor | None = None,
+    counts: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """The drafted tokens that count, the one after them, and how many count."""
+
+    _verify_check(target, drafted, uniform, draft, counts)
+    tokens, accepted, _ = sm100_verify_draft(target, drafted.contiguous(), uniform.contiguous(), draft=draft, counts=counts)
+    return tokens, accepted
+
+
+@verify_draft.register_fake
+def _verify_draft_fake(target, drafted, uniform, draft=None, counts=None):  # noqa: ANN001, ANN202
+    _verify_check(target, drafted, uniform, draft, counts)
+    return drafted.new_empty(target.shape[:2]), drafted.new_empty((drafted.shape[0],), dtype=torch.int32)
+
+
+verify_draft.register_kernel("cpu")(_no_cpu("verify_draft"))
+
+
 __all__ = [
     "NAMESPACE",
     "OPERATORS",
     "flash_attention",
     "kv8_append",
     "kv8_attention",
+    "kv8_compact",
+    "kv8_fork",
+    "kv8_reserve",
     "layer_norm",
     "linear",
     "linear_residual_layer_norm",
     "linear_w4",
+    "low_rank_add",
     "mlp_residual_layer_norm",
     "mma_attention",
     "qk_norm_rope",
     "residual_layer_norm",
     "simt_attention",
+    "verify_draft",
 ]

@@ -15,16 +15,26 @@ cache 8-bit codes; the prompt runs the bf16 kernels.
 The model has neither a position rotation nor norms of queries and keys (its
 positions come with its inputs); ``rope`` and ``qk_norms`` put them in for
 models that do.
+
+The slots may be many requests': each has a low-rank adapter of its own
+(``adapters``, ``set_adapters``), takes over another's sequence (``fork``: samples, beams), and keeps as
+many of its drafted tokens as are verified (``accept``):
+
+    y = decoder.step(drafts, advance=False)       # [8, 1 + n, D]: the last token and n drafted ones
+    tokens, accepted = decoder.accept(probabilities(y), drafted, uniform)
 """
 
 from __future__ import annotations
 
+from collections.abc import Sequence
 from typing import Any
 
 import torch
 
 from ..kernels import (
     Kv8Cache,
+    Kv8Pages,
+    LowRankAdapters,
     RotaryTable,
     W4Weight,
     pack_w4,
@@ -32,14 +42,19 @@ from ..kernels import (
     sm100_initial_layer_norm,
     sm100_kv8_append,
     sm100_kv8_attention,
+    sm100_kv8_fork,
+    sm100_kv8_reserve,
     sm100_linear,
     sm100_linear_w4,
+    sm100_low_rank_add,
     sm100_mma_attention,
     sm100_qk_norm_rope,
     sm100_residual_layer_norm,
     sm100_simt_attention,
+    sm100_verify_draft,
 )
 from ..kernels.kv_cache import KV8_HEAD_DIMS
+from ..kernels.kv_pages import KV8_POOL_ROWS
 from .cuda_graph import CudaGraphReplay
 
 # Rows of a step up to which its projections go through the 4-bit kernel, which reads the weights
@@ -53,7 +68,8 @@ _REPEATABLE = 64  # tokens that can be appended twice over and leave what once l
 class CachedDecoder:
     """Prompt and steps of a ``UserOptimizedTransformer`` over a cache of ``slots``
     sequences of up to ``max_tokens`` tokens.  The slots go together: all hold
-    the same number of tokens.
+    the same number of tokens, unless a step's are counted for each slot
+    (``accept``, ``advance`` with a tensor).
 
     * ``weights``: ``"w4"`` packs the projections to 4 bits for the steps (groups
       of ``group``; a step of more than 64 rows takes the same values rounded to
@@ -61,6 +77,8 @@ class CachedDecoder:
       model's own, as the prompt always does
     * ``rope``: a ``RotaryTable``; ``qk_norms``: per layer ``(q_weight, k_weight)``,
       fp32 ``[head_dim]`` each
+    * ``adapters``: per layer, low-rank adapters of its projections by name (``"qkv"``,
+      ``"out"``, ``"ffn_in"``, ``"ffn_out"``; any of them), which ``set_adapters`` gives to the slots
     * ``graph``: replay a step of up to 64 tokens from a CUDA graph, captured once for
       each shape and dtype; ``x`` is copied into the buffer that the graph reads
       (``solution.runtimes.CudaGraphReplay``)
@@ -80,6 +98,7 @@ class CachedDecoder:
         rope: RotaryTable | None = None,
         qk_norms: list[tuple[torch.Tensor, torch.Tensor]] | None = None,
         qk_norm_eps: float = 1e-6,
+        adapters: Sequence[dict[str, LowRankAdapters]] | None = None,
         graph: bool = True,
     ) -> None:
         config = model.config
@@ -94,6 +113,17 @@ class CachedDecoder:
             raise ValueError("qk_norms must hold one pair of weights per layer")
         if slots < 1 or max_tokens < 1:
             raise ValueError("slots and max_tokens must be positive")
+        if adapters is not None:
+            if len(adapters) != config.num_layers:
+                raise ValueError("adapters must hold one dict per layer")
+            for given, layer in zip(adapters, model.layers):
+                linears = dict(self._linears(layer))
+                for name, adapter in given.items():
+                    if name not in linears:
+                        raise ValueError(f"adapters are of {tuple(linears)}, not of {name!r}")
+                    weight = linears[name].weight
+                    if (adapter.out_features, adapter.in_features) != tuple(weight.shape) or adapter.device != weight.device:
+                        raise ValueError(f"the adapters of {name!r} do not fit its weight {tuple(weight.shape)} on {weight.device}")
         device = next(model.parameters()).device
         if device.type != "cuda":
             raise RuntimeError("CachedDecoder needs a model on an sm_100 CUDA device; there is no CPU fallback")
@@ -101,13 +131,17 @@ class CachedDecoder:
         self.heads = config.num_heads
         self.slots = slots
         self.max_tokens = max_tokens
-        self.held = 0  # tokens of each slot, as far as this decoder has counted them
+        self.held = 0  # tokens of each slot, as far as this decoder has counted them; where slots differ, no less than the most
         self.pending = 0  # of those appended last, the ones that may still be counted
         self.rope = rope
         self.qk_norms = qk_norms or [(None, None)] * config.num_layers
         self.qk_norm_eps = float(qk_norm_eps)
         self.graph = bool(graph)
+        self.adapters = None if adapters is None else [dict(given) for given in adapters]
+        self._differ = False  # whether the slots' tokens have been counted apart
+        self._pages: Kv8Pages | None = None  # made by the first fork: slots share pages from then on
         with torch.inference_mode():
+            self.adapter_indices = torch.full((slots,), -1, dtype=torch.int32, device=device)
             model._materialize_shadow_weights()
             self.cache = Kv8Cache.create(
                 slots=slots, max_tokens=max_tokens, num_kv_heads=self.heads, head_dim=self.head_dim,
@@ -155,11 +189,18 @@ class CachedDecoder:
 
         def linear(index: int, name: str, module: Any, x: torch.Tensor, *, gelu: bool = False) -> torch.Tensor:
             weight, bias = module.shadow_parameters()
+            own = None if self.adapters is None else self.adapters[index].get(name)
+            # with adapters the projection stays in 32 bits until theirs are added, and the GELU comes after that
+            form = {"gelu": gelu} if own is None else {"out_dtype": torch.float32}
             if packed is not None and rows <= _W4_ROWS:
-                return sm100_linear_w4(x, packed[index][name], bias, gelu=gelu)[0]
-            if packed is not None:
-                weight = self._wide_weights[index][name]
-            return sm100_linear(x, weight, bias, gelu=gelu)[0]
+                y = sm100_linear_w4(x, packed[index][name], bias, **form)[0]
+            else:
+                if packed is not None:
+                    weight = self._wide_weights[index][name]
+                y = sm100_linear(x, weight, bias, **form)[0]
+            if own is None:
+                return y
+            return sm100_low_rank_add(x, y, own, self.adapter_indices, gelu=gelu, out_dtype=torch.bfloat16)[0]
 
         normalized, _ = sm100_initial_layer_norm(flat, (layers[0].norm1 if len(layers) else final).kernel_norm())
         residual = torch.empty((rows, d_model), dtype=torch.float32, device=value.device)
@@ -228,6 +269,8 @@ class CachedDecoder:
             raise ValueError("x must be a contiguous tensor on the decoder's device")
         if x.dtype not in (torch.float32, torch.bfloat16):
             raise ValueError("x must be float32 or bfloat16")
+        if held and held + x.shape[1] > self.max_tokens and self._differ:
+            self.held = held = int(self.cache.lengths.max())  # what the slots really hold: read from the device
         if held + x.shape[1] > self.max_tokens:
             raise ValueError(f"{held} tokens held and {x.shape[1]} more pass the cache's {self.max_tokens}")
 
@@ -238,12 +281,26 @@ class CachedDecoder:
         with torch.inference_mode():
             self.cache.lengths.zero_()
         self.held = self.pending = 0
+        self._differ = False
 
-    def advance(self, tokens: int) -> None:
+    def advance(self, tokens: int | torch.Tensor) -> None:
         """Count ``tokens`` of those that the last step appended as held, in every
         slot: any number of them up to 64, else all (a block that a longer call
-        fills is only kept as codes, and cannot be open again)."""
+        fills is only kept as codes, and cannot be open again).  An int32 tensor
+        ``[slots]`` counts for each slot its own (of a step of up to 64 tokens; numbers outside
+        are taken as none or all); the rest is forgotten."""
 
+        if isinstance(tokens, torch.Tensor):
+            if tokens.dtype != torch.int32 or tuple(tokens.shape) != (self.slots,) or tokens.device != self.cache.device:
+                raise ValueError(f"tokens must be a number or an int32 [{self.slots}] tensor on the decoder's device")
+            if self.pending > _REPEATABLE:
+                raise ValueError(f"a step of {self.pending} tokens, more than {_REPEATABLE}, is counted whole")
+            with torch.inference_mode():
+                self.cache.advance(tokens.clamp(0, self.pending))
+            self.held += self.pending
+            self.pending = 0
+            self._differ = True
+            return
         if not 0 <= tokens <= self.pending:
             raise ValueError(f"{tokens} tokens cannot be counted: {self.pending} are not counted yet")
         if tokens != self.pending > _REPEATABLE:
@@ -253,6 +310,71 @@ class CachedDecoder:
         self.held += tokens
         self.pending -= tokens
 
+    def accept(
+        self,
+        target: torch.Tensor,
+        drafted: torch.Tensor,
+        uniform: torch.Tensor,
+        *,
+        draft: torch.Tensor | None = None,
+        counts: torch.Tensor | None = None,
+    ) -> tuple[torch.Tensor, torch.Tensor]:
+        """Verifies the ``T`` drafted tokens of the last step, ``step(x, advance=False)`` of each slot's last token
+        and its drafted ones, and counts those that stand: ``target`` ``[slots, T + 1, V]`` are the probabilities that follow
+        from the step's outputs, the rest as in ``solution.kernels.sm100_verify_draft``.  Returns its tokens
+        and ``accepted``; each slot holds ``accepted + 1`` tokens more."""
+
+        if drafted.ndim != 2 or drafted.shape[0] != self.slots or drafted.shape[1] + 1 != self.pending or self.pending > _REPEATABLE:
+            raise ValueError(
+                f"drafted must be [{self.slots}, T] where the last step had T + 1 tokens that are not counted yet, "
+                f"{_REPEATABLE} at most; {self.pending} are not"
+            )
+        with torch.inference_mode():
+            tokens, accepted, _ = sm100_verify_draft(target, drafted, uniform, draft=draft, counts=counts)
+            self.advance(accepted + 1)
+        return tokens, accepted
+
+    def set_adapters(self, indices: Sequence[int] | torch.Tensor) -> None:
+        """The adapter of each slot from now on, -1: none (for graphs that are captured already, too)."""
+
+        if self.adapters is None:
+            raise ValueError("the decoder was made without adapters")
+        given = torch.as_tensor(indices)
+        if tuple(given.shape) != (self.slots,) or given.is_floating_point() or given.dtype == torch.bool:
+            raise ValueError(f"indices must be {self.slots} whole numbers")
+        with torch.inference_mode():
+            self.adapter_indices.copy_(given)
+
+    def fork(self, parents: Sequence[int] | torch.Tensor) -> None:
+        """Slot i goes on from slot ``parents[i]``'s sequence, for all slots at once, with its adapter: samples
+        of one prompt, or beams in a new order.  Full blocks are shared and not copied.  A number
+        below 0 empties the slot, one past the slots leaves it as it is.  Tokens that are not
+        counted yet are forgotten."""
+
+        given = torch.as_tensor(parents)
+        if tuple(given.shape) != (self.slots,) or given.is_floating_point() or given.dtype == torch.bool:
+            raise ValueError(f"parents must be {self.slots} whole numbers")
+        if self.slots > KV8_POOL_ROWS:
+            raise ValueError(f"at most {KV8_POOL_ROWS} slots can be forked")
+        if self.pending > _REPEATABLE:
+            raise ValueError(f"the last step's {self.pending} tokens cannot be taken back: advance({self.pending}) first")
+        with torch.inference_mode():
+            if self._pages is None:
+                self._pages = Kv8Pages(self.cache)
+            source = given.to(device=self.cache.device, dtype=torch.int32).contiguous()
+            each = torch.arange(self.slots, dtype=torch.int32, device=self.cache.device)
+            sm100_kv8_fork(self._pages, source, each)
+            inside = (source >= 0) & (source < self.slots)
+            of = torch.where(inside, source, each).long()
+            self.adapter_indices.copy_(torch.where(source < 0, -1, self.adapter_indices[of]))
+        self.pending = 0
+        self._differ = True
+
+    def _reserve(self, tokens: int) -> None:
+        # There are as many pages as entries of the table, so that none is ever missing.
+        if self._pages is not None:
+            sm100_kv8_reserve(self._pages, tokens)
+
     def prompt(self, x: torch.Tensor) -> torch.Tensor:
         """The forward of ``x`` ``[slots, T, D]`` from empty sequences, which it leaves
         in the cache (what the slots held before is forgotten)."""
@@ -260,6 +382,7 @@ class CachedDecoder:
         self._check(x, 0)
         self.reset()
         with torch.inference_mode():
+            self._reserve(x.shape[1])
             y = self._program(x, prompt=True)
         self.pending = x.shape[1]
         self.advance(x.shape[1])
@@ -281,6 +404,7 @@ class CachedDecoder:
                     {name: packed.dequantize(torch.bfloat16).contiguous() for name, packed in layer.items()}
                     for layer in self.step_weights
                 ]
+            self._reserve(x.shape[1])
             # A capture runs the step once before it records it, so that the
             # first call appends the same tokens twice.
             if self.graph and x.shape[1] <= _REPEATABLE:

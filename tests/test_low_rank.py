@@ -114,6 +114,12 @@ def test_low_rank_add(rows, inner, outer, rank, count, base_dtype) -> None:  # n
         (5, 257, 2056, 384, 128, 3),
         (1, 1024, 8, 130, 64, 1),
         (20, 100, 512, 4096, 40, 4),
+        (4, 1100, 264, 1032, 16, 3),
+        (32, 64, 136, 200, 64, 3),  # sequences of one adapter with others between them
+        (70, 65, 72, 328, 24, 3),  # groups that end anywhere
+        (3, 1000, 1000, 8, 72, 2),
+        (2, 4096, 8, 136, 8, 2),
+        (24, 128, 520, 1160, 112, 30),
     ],
 )
 @pytest.mark.parametrize("base_dtype", [torch.bfloat16, torch.float32])
