@@ -92,7 +92,7 @@ struct DeviceState {
   bool w4_line_attr[6] = {};               // the same with x in shared memory, by row tiles and group
   bool low_rank_attr[16] = {};             // low-rank adapter builds by rank, rows and base dtype
   bool low_rank_tile_attr[4] = {};         // their builds for many rows
-  bool fork_attr = false, reserve_attr = false;
+  bool fork_attr = false, reserve_attr = false, compact_attr = false;  // pages: shared memory and cluster sizes set
   bool seq_forward_attr = false;           // whole-forward kernel's shared-memory size set
   uint8_t* seq_noalloc_images = nullptr;   // device address of g_seq_noalloc_images on this device
 };

@@ -53,6 +53,7 @@ struct SlotOwners {
 
 // ------------------------------------------------------------------ fork and free
 constexpr int kForkThreads = 256;
+constexpr int kForkCtas = 3;                                 // of an SM
 constexpr int kForkHeld = 8;                                 // 16-byte pieces a thread holds
 constexpr int kForkPieces = kForkThreads * kForkHeld;        // of all pairs of an item
 static_assert(kForkPieces >= kPoolRows, "an item holds a piece of every pair");
@@ -83,7 +84,7 @@ struct __align__(16) ForkPair {
 // a place in the tails (or some columns of the table) for all pairs: its values
 // are read for every pair before any is written, so a slot may be the source of one pair and the
 // target of another (beams that are put in a new order).
-__global__ void __launch_bounds__(kForkThreads, 3) kv8_fork_kernel(const __grid_constant__ Kv8ForkArgs a) {
+__global__ void __launch_bounds__(kForkThreads, kForkCtas) kv8_fork_kernel(const __grid_constant__ Kv8ForkArgs a) {
   extern __shared__ __align__(16) uint8_t fork_smem[];
   __shared__ int s_last, s_most;
   ForkPair* const pair = reinterpret_cast<ForkPair*>(fork_smem);
@@ -201,7 +202,7 @@ __global__ void __launch_bounds__(kForkThreads, 3) kv8_fork_kernel(const __grid_
 // ------------------------------------------------------------------ order over a cluster
 // One CTA, or a cluster of them for many pages or entries, does what needs an order over all: each
 // takes a stretch, and the stretches' counts go round through (distributed) shared memory.
-constexpr int kPoolCtas = 8;
+constexpr int kPoolCtas = 16;  // (more than 8: the most that this GPU allows)
 constexpr int kPoolThreads = 1024;
 constexpr int kPoolWarps = kPoolThreads / 32;
 

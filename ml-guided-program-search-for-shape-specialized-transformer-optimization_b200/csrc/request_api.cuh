@@ -145,6 +145,7 @@ template <typename Kernel>
 cudaError_t pool_attribute(Kernel kernel, bool* done) {
   if (*done) return cudaSuccess;
   cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPoolShared);
+  if (err == cudaSuccess) err = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (err == cudaSuccess) *done = true;
   return err;
 }
@@ -252,7 +253,7 @@ int b200tx_kv8_fork(const b200tx_kv8_pool* pool, const int32_t* source, const in
   a.tail_items = static_cast<int>(tail_items);
   a.table_items = static_cast<int>(table_items);
   cudaError_t err = pool_attribute(b200tx::kv8_fork_kernel, &dev->fork_attr);
-  const int64_t grid = std::min<int64_t>(tail_items + table_items, 4 * dev->sm_count);
+  const int64_t grid = std::min<int64_t>(tail_items + table_items, b200tx::kForkCtas * dev->sm_count);
   if (err == cudaSuccess)
     err = launch(b200tx::kv8_fork_kernel, dim3(static_cast<unsigned>(grid)), dim3(b200tx::kForkThreads),
                  pairs * sizeof(b200tx::ForkPair) + 8 * a.owners, stream, a);
@@ -304,8 +305,9 @@ int b200tx_kv8_compact(const b200tx_kv8_pool* pool, int32_t* used, cudaStream_t 
   a.piece = static_cast<int>(std::min(a.page_bytes, kPiece));
   a.pieces = static_cast<int>((a.page_bytes + a.piece - 1) / a.piece);
   const unsigned ctas = pool_cluster(a.pool.pages, 0);
-  cudaError_t err =
-      launch_clustered(b200tx::kv8_compact_plan_kernel, dim3(ctas), dim3(b200tx::kPoolThreads), 0, ctas, stream, a);
+  cudaError_t err = pool_attribute(b200tx::kv8_compact_plan_kernel, &dev->compact_attr);
+  if (err == cudaSuccess)
+    err = launch_clustered(b200tx::kv8_compact_plan_kernel, dim3(ctas), dim3(b200tx::kPoolThreads), 0, ctas, stream, a);
   if (err == cudaSuccess)
     err = launch(b200tx::kv8_compact_move_kernel,
                  dim3(static_cast<unsigned>(std::min<int64_t>(4 * dev->sm_count, (a.pool.pages + 1) / 2 * a.pool.layers * a.pieces))),

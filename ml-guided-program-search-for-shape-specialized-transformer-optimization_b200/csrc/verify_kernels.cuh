@@ -231,35 +231,35 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_draft_kernel(const __gr
       from += static_cast<int64_t>(pick) * length;
       limit = min(limit, end(from, length));
     }
-    from += warp * kVerifyLook;
-    double mass[kVerifyLook / 32], sum = 0.0;
+    // eight neighbouring values a lane
+    from += warp * kVerifyLook + lane * kVerifyLook / 32;
+    double mass[kVerifyLook / 32], mine = 0.0;
 #pragma unroll
-    for (int i = 0; i < kVerifyLook / 32; ++i) {
-      const int64_t at = from + i * 32 + lane;
-      mass[i] = at < limit ? row.one(static_cast<int>(at)) : 0.0;
-      sum += mass[i];
+    for (int i = 0; i < kVerifyLook / 32; ++i) mass[i] = from + i < limit ? row.one(static_cast<int>(from + i)) : 0.0;
+#pragma unroll
+    for (int i = 0; i < kVerifyLook / 32; ++i) mine += mass[i];
+    double upto = mine;  // with the lanes before
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const double o = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += o;
     }
-#pragma unroll
-    for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (lane == 0) s_part[level & 1][warp] = sum;
+    if (lane == 31) s_part[level & 1][warp] = upto;
     __syncthreads();
     if (verify_pick(s_part[level & 1], kVerifyWarps, running, wanted) != warp) return;
+    running += upto - mine;
     int latest = -1, found = -1;
 #pragma unroll
     for (int i = 0; i < kVerifyLook / 32; ++i) {
-      double before = mass[i];
-#pragma unroll
-      for (int d = 1; d < 32; d *= 2) {
-        const double o = __shfl_up_sync(0xffffffffu, before, d);
-        if (lane >= d) before += o;
+      running += mass[i];
+      if (mass[i] > 0.0) {
+        latest = i;
+        if (found < 0 && running > wanted) found = i;
       }
-      const uint32_t passed = __ballot_sync(0xffffffffu, mass[i] > 0.0 && running + before > wanted);
-      const uint32_t held = __ballot_sync(0xffffffffu, mass[i] > 0.0);
-      if (found < 0 && passed != 0) found = i * 32 + __ffs(passed) - 1;
-      if (held != 0) latest = i * 32 + 31 - __clz(held);
-      running += __shfl_sync(0xffffffffu, before, 31);
     }
-    token = from + (found >= 0 ? found : latest);
+    const uint32_t passed = __ballot_sync(0xffffffffu, found >= 0), held = __ballot_sync(0xffffffffu, latest >= 0);
+    const int64_t at = from + (passed != 0 ? found : latest);
+    token = __shfl_sync(0xffffffffu, at, passed != 0 ? __ffs(passed) - 1 : 31 - __clz(held));
   } else if (warp != 0) {
     return;
   }
