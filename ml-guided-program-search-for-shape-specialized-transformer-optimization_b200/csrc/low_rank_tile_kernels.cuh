@@ -31,7 +31,6 @@ constexpr int kLtRows = 128;
 constexpr int kLtColumns = 128;          // of the result, for one round
 constexpr int kLtStages = 6;             // of 64 values of K
 constexpr uint32_t kLtXBytes = kLtRows * 128;
-constexpr int kErrLowRankWait = 0x501;
 constexpr int kLtWorkers = 512;          // threads that make the terms and bring the results out
 constexpr int kLtThreads = kLtWorkers + 64;
 

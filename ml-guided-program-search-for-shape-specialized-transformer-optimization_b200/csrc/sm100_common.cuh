@@ -31,6 +31,7 @@ enum DeviceErrorCode : unsigned int {
   kErrAttnSoftmaxWait = 0x203,
   kErrPeerWait = 0x301,  // a tensor-parallel peer did not publish its partial in time
   kErrSeqWait = 0x401,   // the whole-forward kernel's copy or UMMA did not complete in time
+  kErrLowRankWait = 0x501,  // the same of the low-rank adapters' kernel for many rows
 };
 
 // A single wait gives up after this many nanoseconds.  Every event waited on

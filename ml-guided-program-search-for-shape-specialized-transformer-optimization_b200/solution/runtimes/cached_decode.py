@@ -335,13 +335,19 @@ class CachedDecoder:
         return tokens, accepted
 
     def set_adapters(self, indices: Sequence[int] | torch.Tensor) -> None:
-        """The adapter of each slot from now on, -1: none (for graphs that are captured already, too)."""
+        """The adapter of each slot from now on, -1: none (for graphs that are captured already, too).
+        Numbers on the host are checked; one on the device past a projection's set makes its
+        slot's outputs NaN."""
 
         if self.adapters is None:
             raise ValueError("the decoder was made without adapters")
         given = torch.as_tensor(indices)
         if tuple(given.shape) != (self.slots,) or given.is_floating_point() or given.dtype == torch.bool:
             raise ValueError(f"indices must be {self.slots} whole numbers")
+        sizes = [own.count for layer in self.adapters for own in layer.values()]
+        if given.device.type == "cpu" and sizes and int(given.max()) >= min(sizes):
+            raise ValueError(f"adapter {int(given.max())} of {min(sizes)}")
+        given = given.clamp(-1, 2**31 - 1)
         with torch.inference_mode():
             self.adapter_indices.copy_(given)
 
@@ -361,7 +367,7 @@ class CachedDecoder:
         with torch.inference_mode():
             if self._pages is None:
                 self._pages = Kv8Pages(self.cache)
-            source = given.to(device=self.cache.device, dtype=torch.int32).contiguous()
+            source = given.clamp(-1, self.slots).to(device=self.cache.device, dtype=torch.int32).contiguous()
             each = torch.arange(self.slots, dtype=torch.int32, device=self.cache.device)
             sm100_kv8_fork(self._pages, source, each)
             inside = (source >= 0) & (source < self.slots)

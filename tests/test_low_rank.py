@@ -354,6 +354,8 @@ def test_refusals() -> None:
     with pytest.raises(ValueError):  # base's memory in another type
         sm100_low_rank_add(x, base, adapters, indices, out_dtype=torch.bfloat16,
                            out=base.view(torch.bfloat16).view(-1)[: 6 * 48].view(6, 48))
+    with pytest.raises(ValueError):  # the adapters' memory
+        sm100_low_rank_add(x, base, adapters, indices, out_dtype=torch.bfloat16, out=adapters.up.view(-1)[: 6 * 48].view(6, 48))
     with pytest.raises(ValueError):  # x's memory
         sm100_low_rank_add(x, base, adapters, indices, out_dtype=torch.bfloat16, out=x.view(-1)[: 6 * 48].view(6, 48))
     with torch.inference_mode(False), torch.enable_grad(), pytest.raises(RuntimeError):

@@ -235,12 +235,17 @@ def test_counts_of_each_slot_and_refusals() -> None:
             call()
     decoder.advance(70)
     for call in (lambda: decoder.fork([0]), lambda: decoder.fork([0.0, 1.0]), lambda: decoder.set_adapters([0]),
-                 lambda: decoder.set_adapters([0.5, 1.0])):
+                 lambda: decoder.set_adapters([0.5, 1.0]), lambda: decoder.set_adapters([0, 2])):
         with pytest.raises(ValueError):
             call()
     decoder.set_adapters([1, 0])
+    decoder.fork([1 << 33, 1 << 32])  # past the slots: nothing
+    assert decoder.adapter_indices.tolist() == [1, 0] and decoder.cache.lengths.tolist() == [72, 75]
     decoder.fork([1, 1])
     assert decoder.adapter_indices.tolist() == [0, 0] and decoder.cache.lengths.tolist() == [75, 75]
+    decoder.set_adapters(torch.tensor([0, 5], device=DEV))
+    y = decoder.step(_randn(2, 1, 128))
+    assert bool(y[0].isfinite().all()) and bool(y[1].isnan().all())
     with pytest.raises(ValueError, match="without adapters"):
         CachedDecoder(model, slots=2, max_tokens=64).set_adapters([0, 0])
     for sets in ([], [{"middle": None}], [{"qkv": _adapters(model, 1, 8, ("out",))[0]["out"]}],
