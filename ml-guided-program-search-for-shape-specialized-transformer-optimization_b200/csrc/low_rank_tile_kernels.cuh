@@ -111,6 +111,10 @@ __global__ void __launch_bounds__(kLtThreads, 1) low_rank_tile_kernel(const __gr
   const int part = split == 1 ? 0 : mine / groups;
   const int all_rounds = (a.outer + kLtColumns - 1) / kLtColumns;
   const int round0 = all_rounds * part / split, rounds = all_rounds * (part + 1) / split - round0;
+  // Every CTA begins with another of its rounds: rows lie a power of two apart as often as not, and in step all CTAs
+  // would go to the same memory channels.
+  const int turn = static_cast<int>(blockIdx.x * 5u % static_cast<unsigned>(rounds));
+  auto column_of = [&](int j) { return static_cast<uint32_t>(round0 + (j + turn >= rounds ? j + turn - rounds : j + turn)) * kLtColumns; };
   const float nan = __int_as_float(0x7fffffff);
   const uint32_t sums_tmem = tmem + 128;  // the second round's columns: free until then
   const uint64_t smem_desc = sw128_desc(smem0, 16, 1024);  // an operand's place is its 16-byte units more
@@ -249,7 +253,7 @@ __global__ void __launch_bounds__(kLtThreads, 1) low_rank_tile_kernel(const __gr
     if (tid >= kLtWorkers) {
       if (copies && !bare) {
         // 8 columns of up are one of the map's outermost dimension; those past the adapter's last come along
-        const int eight0 = static_cast<int>((static_cast<int64_t>(adapter) * a.outer + round0 * kLtColumns) / 8);
+        const int eight0 = static_cast<int>(static_cast<int64_t>(adapter) * a.outer / 8);
         uint32_t slot = rounds_done % S::UPS, phase = rounds_done / S::UPS & 1;
         for (int j = 0; j < rounds; ++j) {
           if (!mbar_wait(&up_free_bar[slot], phase ^ 1, kErrLowRankWait, &abort_flag)) break;
@@ -257,7 +261,7 @@ __global__ void __launch_bounds__(kLtThreads, 1) low_rank_tile_kernel(const __gr
           mbar_arrive_expect_tx(&up_bar[slot], S::UP);
 #pragma unroll
           for (int r = 0; r < 4 * RA; ++r)
-            tma_load_3d(to + r * 32 * 128, &up_map, &up_bar[slot], r / 4 * 64, r % 4 * 2, eight0 + j * (kLtColumns / 8));
+            tma_load_3d(to + r * 32 * 128, &up_map, &up_bar[slot], r / 4 * 64, r % 4 * 2, eight0 + static_cast<int>(column_of(j) / 8));
           if (++slot == S::UPS) slot = 0, phase ^= 1;
           ++asked_up;
         }
@@ -300,13 +304,13 @@ __global__ void __launch_bounds__(kLtThreads, 1) low_rank_tile_kernel(const __gr
     uint8_t* const out0 = static_cast<uint8_t*>(a.out) + first * a.outer * (a.out_f32 ? 4 : 2);
     // A warp with all its rows takes whole rounds without a check between the values; base's are on their way then a
     // round before they are wanted: rows 2 i and 2 i + 1 of the four.
-    const bool plain = __all_sync(0xffffffffu, live == 0xf) && !bare;
-    auto whole = [&](int round) { return plain && (round0 + round + 1) * kLtColumns <= a.outer; };
+    const bool plain = __all_sync(0xffffffffu, live == 0xf) && !bad;
+    auto whole = [&](int j) { return plain && column_of(j) + kLtColumns <= static_cast<uint32_t>(a.outer); };
     LrEight<F32> ahead[2][2];
-    auto load_base = [&](int round, int i) {
+    auto load_base = [&](int j, int i) {
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        ahead[i][e].load(base0 + static_cast<uint64_t>(place[2 * i + e] + (round0 + round) * kLtColumns) * (F32 ? 4 : 2));
+        ahead[i][e].load(base0 + static_cast<uint64_t>(place[2 * i + e] + column_of(j)) * (F32 ? 4 : 2));
     };
     auto store = [&](uint8_t* to, float (&y)[8]) {
       if (a.out_f32) {
@@ -334,7 +338,7 @@ __global__ void __launch_bounds__(kLtThreads, 1) low_rank_tile_kernel(const __gr
       // the warp goes on, or stops, together
       if (!__all_sync(0xffffffffu, bare || mbar_wait(&full_bar[at & 1], at >> 1 & 1, kErrLowRankWait, &abort_flag))) break;
       tc_fence_after();
-      const uint32_t column = (round0 + j) * kLtColumns;
+      const uint32_t column = column_of(j);
       const int size = a.out_f32 ? 4 : 2;
       const uint32_t d = tmem + (at & 1) * 128 + (static_cast<uint32_t>(quarter) << 16) + columns / 4;
       auto done = [&]() {  // the buffer is read
@@ -346,14 +350,16 @@ __global__ void __launch_bounds__(kLtThreads, 1) low_rank_tile_kernel(const __gr
         const bool more = j + 1 < rounds && whole(j + 1);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          uint32_t r[16];
-          tmem_ld_16x32(d + (static_cast<uint32_t>(i * 16) << 16), r);
+          uint32_t r[16] = {};
+          if (!bare) tmem_ld_16x32(d + (static_cast<uint32_t>(i * 16) << 16), r);
           float y[2][8];
 #pragma unroll
           for (int e = 0; e < 2; ++e) ahead[i][e].values(y[e]);
           if (more) load_base(j + 1, i);
-          tmem_wait_ld();
-          if (i == 1) done();
+          if (!bare) {
+            tmem_wait_ld();
+            if (i == 1) done();
+          }
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
 #pragma unroll
@@ -363,7 +369,7 @@ __global__ void __launch_bounds__(kLtThreads, 1) low_rank_tile_kernel(const __gr
         }
         continue;
       }
-      // rows or columns are missing, or there is nothing to add
+      // rows or columns are missing, or all is NaN
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
         uint32_t r[16] = {};
@@ -387,6 +393,10 @@ __global__ void __launch_bounds__(kLtThreads, 1) low_rank_tile_kernel(const __gr
         }
       }
       if (!bare) done();
+      if (j + 1 < rounds && whole(j + 1)) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) load_base(j + 1, i);
+      }
     }
     if (!bare) rounds_done += rounds;
   }
