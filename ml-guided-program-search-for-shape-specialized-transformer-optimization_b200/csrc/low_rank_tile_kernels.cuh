@@ -111,10 +111,7 @@ __global__ void __launch_bounds__(kLtThreads, 1) low_rank_tile_kernel(const __gr
   const int part = split == 1 ? 0 : mine / groups;
   const int all_rounds = (a.outer + kLtColumns - 1) / kLtColumns;
   const int round0 = all_rounds * part / split, rounds = all_rounds * (part + 1) / split - round0;
-  // Every CTA begins with another of its rounds: rows lie a power of two apart as often as not, and in step all CTAs
-  // would go to the same memory channels.
-  const int turn = static_cast<int>(blockIdx.x * 5u % static_cast<unsigned>(rounds));
-  auto column_of = [&](int j) { return static_cast<uint32_t>(round0 + (j + turn >= rounds ? j + turn - rounds : j + turn)) * kLtColumns; };
+  auto column_of = [&](int j) { return static_cast<uint32_t>(round0 + j) * kLtColumns; };
   const float nan = __int_as_float(0x7fffffff);
   const uint32_t sums_tmem = tmem + 128;  // the second round's columns: free until then
   const uint64_t smem_desc = sw128_desc(smem0, 16, 1024);  // an operand's place is its 16-byte units more
@@ -393,10 +390,6 @@ __global__ void __launch_bounds__(kLtThreads, 1) low_rank_tile_kernel(const __gr
         }
       }
       if (!bare) done();
-      if (j + 1 < rounds && whole(j + 1)) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) load_base(j + 1, i);
-      }
     }
     if (!bare) rounds_done += rounds;
   }

@@ -8,7 +8,9 @@ namespace {
 constexpr int kLrShared = 220 * 1024;  // most that a build asks for
 constexpr int kLrTwo = 110 * 1024;     // with which two CTAs share an SM
 
-constexpr int kLrSteps = 2;  // of 32 values of K, for a warp
+// Steps of 32 values of K for a warp, where a group has CTAs enough (64 rows of 32 adapters, 4096 -> 14336: 2 steps and eight CTAs
+// 11.2 us, 4 and four 11.8, 16 and one 13.7).
+constexpr int kLrSteps = 2;
 
 template <int RT, bool F32, bool WHOLE>
 cudaError_t launch_low_rank(b200tx::LowRankArgs& a, DeviceState* dev, int index, cudaStream_t stream) {
@@ -30,7 +32,7 @@ cudaError_t launch_low_rank(b200tx::LowRankArgs& a, DeviceState* dev, int index,
     ctas /= 2;
   const int bytes = S::bytes(ctas, terms);
   const int64_t resident = std::max(1, dev->sm_count * (S::TWO && bytes <= kLrTwo ? 2 : 1) / ctas);  // clusters
-  // Rows of a group: fewer, while the groups then all run at once.
+  // Rows of a group: fewer, while the groups then all run at once (203 rows of 4744 -> 5003: 8 rows 17.4 us, 32 rows 24.2).
   a.group = S::G;
   while (a.group > 8 && windows * ((rows + a.group / 2 - 1) / (a.group / 2)) <= resident) a.group /= 2;
   const int64_t least = (rows + a.group - 1) / a.group;  // groups of a window, where its rows share an adapter
@@ -136,9 +138,10 @@ int low_log2(int64_t v) {
 
 constexpr int kPoolShared = 96 * 1024;  // of 2048 rows' records and places
 
-// CTAs for an order over so many pages and entries: one, without exchanges, while its
-// threads take few of them each.
-constexpr int64_t kPoolFew = 8192;
+// CTAs for an order over so many pages and entries: one, without exchanges, while its threads take few of them
+// each (free and reserve with 1320 pages: one 10.9 us, a cluster 13.2; 10320: 15.8 and 17.3; 20640: 20.2 and 18.8; 82080: 53
+// and 22; compaction of 3572 pages 12.6 and 15.5, of 14286 27.7 and 23.9).
+constexpr int64_t kPoolFew = 12288;
 unsigned pool_cluster(int64_t pages, int64_t entries) { return std::max(pages, entries) <= kPoolFew ? 1 : b200tx::kPoolCtas; }
 
 template <typename Kernel>
