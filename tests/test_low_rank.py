@@ -120,6 +120,7 @@ def test_low_rank_add(rows, inner, outer, rank, count, base_dtype) -> None:  # n
         (3, 1000, 1000, 8, 72, 2),
         (2, 4096, 8, 136, 8, 2),
         (24, 128, 520, 1160, 112, 30),
+        (64, 64, 200, 64, 40, 3),  # several groups for a CTA, in a row and not
     ],
 )
 @pytest.mark.parametrize("base_dtype", [torch.bfloat16, torch.float32])

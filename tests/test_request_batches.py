@@ -218,6 +218,42 @@ def test_drafted_tokens_that_are_verified() -> None:
 
 
 @pytest.mark.gpu
+def test_all_of_it_together() -> None:
+    """Adapters, forks and verified drafts over packed weights, as a server runs them: bit for bit what slots give that share
+    nothing."""
+    config = WorkloadConfig(4, 128, 256, 4, 512, 2)
+    model = _model(config)
+    sets = _adapters(model, 3, 24)
+    vocab = 50
+    g = torch.Generator().manual_seed(6)
+    head = torch.randn(256, vocab, generator=g).to(DEV)
+    prompt = _randn(4, 70, 256)
+    shared = CachedDecoder(model, slots=4, max_tokens=160, adapters=sets)
+    apart = CachedDecoder(model, slots=4, max_tokens=160, adapters=sets)
+    shared.set_adapters([2, 0, 1, -1])
+    shared.prompt(prompt)
+    parents, mixed = [0, 0, 2, 3], [2, 2, 1, -1]
+    shared.fork(parents)
+    apart.set_adapters(mixed)
+    apart.prompt(prompt[parents].contiguous())
+    assert shared.adapter_indices.tolist() == mixed
+    for turn in range(12):
+        x = _randn(4, 5, 256, seed=20 + turn)
+        drafted = torch.randint(0, vocab, (4, 4), generator=g).to(DEV)
+        uniform = torch.rand(4, 5, generator=g).to(DEV) * 0.2  # so that some are accepted
+        draft = torch.softmax(torch.randn(4, 4, vocab, generator=g), -1).to(DEV)
+        results = []
+        for decoder in (shared, apart):
+            y = decoder.step(x, advance=False)
+            target = torch.softmax(y @ head, -1)
+            results.append((y, *decoder.accept(target, drafted, uniform, draft=draft)))
+        for a, b in zip(*results):
+            assert torch.equal(a, b)
+        assert torch.equal(shared.cache.lengths, apart.cache.lengths)
+    assert int(shared.cache.lengths.min()) < int(shared.cache.lengths.max())
+
+
+@pytest.mark.gpu
 def test_counts_of_each_slot_and_refusals() -> None:
     config = WorkloadConfig(2, 80, 128, 2, 128, 1)
     model = _model(config)
