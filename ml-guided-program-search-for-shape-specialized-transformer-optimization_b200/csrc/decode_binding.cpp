@@ -509,7 +509,8 @@ PyObject* low_rank_add(PyObject*, PyObject* const* args, Py_ssize_t n) {
     at::Tensor out = result(args[8], base->sizes(), type, *x, "out has the wrong shape, dtype, device or layout");
     require(args[8] == Py_None || apart(out, *base) || (out.const_data_ptr() == base->const_data_ptr() && type == base->scalar_type()),
             "out shares memory with base without being it");
-    require(args[8] == Py_None || (apart(out, *down) && apart(out, *up)), "out shares memory with the adapters");
+    require(args[8] == Py_None || (apart(out, *down) && apart(out, *up) && apart(out, *scales) && apart(out, *indices)),
+            "out shares memory with the adapters or indices");
     launched(entry.low_rank_add(x->const_data_ptr(), base->const_data_ptr(), dtype(*base), out.data_ptr(),
                                 f32 ? B200TX_F32 : B200TX_BF16, down->const_data_ptr(), up->const_data_ptr(),
                                 scales->const_data_ptr<float>(), indices->const_data_ptr<int32_t>(), indices->numel(), rows,

@@ -245,13 +245,13 @@ int b200tx_kv8_fork(const b200tx_kv8_pool* pool, const int32_t* source, const in
   const int region = b200tx::kKv8Block * a.pool.dim / 8;
   a.region_log2 = low_log2(region);
   a.piece_shift = std::min(low_log2(b200tx::kForkPieces / pairs), a.region_log2);
-  if (static_cast<double>(a.pool.slots) * 4 * a.pool.kv_heads * region >= 4294967295.0)
+  if (source != nullptr && static_cast<double>(a.pool.slots) * 4 * a.pool.kv_heads * region >= 4294967295.0)
     return fail(B200TX_ERR_UNSUPPORTED, "kv8_fork: a layer's tails pass 64 GB");
   a.column_shift = low_log2(b200tx::kForkPieces / pairs);
   const int64_t tail_items =
       source == nullptr ? 0 : static_cast<int64_t>(a.pool.layers) * 2 * a.pool.kv_heads * (region >> a.piece_shift);
   const int64_t table_items = ((a.pool.max_blocks - 1) >> a.column_shift) + 1;
-  if (tail_items + table_items > 0x7fffffffLL)
+  if (tail_items + table_items > (1 << 30))
     return fail(B200TX_ERR_INVALID_ARGUMENT, "kv8_fork: too many layers and heads");
   a.tail_items = static_cast<int>(tail_items);
   a.table_items = static_cast<int>(table_items);

@@ -347,7 +347,7 @@ class CachedDecoder:
         sizes = [own.count for layer in self.adapters for own in layer.values()]
         if given.device.type == "cpu" and sizes and int(given.max()) >= min(sizes):
             raise ValueError(f"adapter {int(given.max())} of {min(sizes)}")
-        given = given.clamp(-1, 2**31 - 1)
+        given = given.long().clamp(-1, 2**31 - 1)
         with torch.inference_mode():
             self.adapter_indices.copy_(given)
 
@@ -367,7 +367,7 @@ class CachedDecoder:
         with torch.inference_mode():
             if self._pages is None:
                 self._pages = Kv8Pages(self.cache)
-            source = given.clamp(-1, self.slots).to(device=self.cache.device, dtype=torch.int32).contiguous()
+            source = given.long().clamp(-1, self.slots).to(device=self.cache.device, dtype=torch.int32).contiguous()
             each = torch.arange(self.slots, dtype=torch.int32, device=self.cache.device)
             sm100_kv8_fork(self._pages, source, each)
             inside = (source >= 0) & (source < self.slots)

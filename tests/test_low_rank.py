@@ -314,6 +314,18 @@ def test_handle_refusals() -> None:
 
 
 @gpu
+def test_results_over_what_the_call_reads_are_refused() -> None:
+    adapters = _adapters(8, 8, 8, 8, torch.Generator(device="cuda").manual_seed(5))
+    x = torch.zeros(1, 8, dtype=torch.bfloat16, device="cuda")
+    base = torch.zeros(1, 8, device="cuda")
+    indices = torch.zeros(1, dtype=torch.int32, device="cuda")
+    over_indices = torch.zeros(8, device="cuda")
+    for its, out in ((indices, adapters.scales.view(1, 8)), (over_indices.view(torch.int32)[5:6], over_indices.view(1, 8))):
+        with pytest.raises(ValueError, match="shares memory"):
+            sm100_low_rank_add(x, base, adapters, its, out=out)
+
+
+@gpu
 def test_refusals() -> None:
     g = torch.Generator(device="cuda").manual_seed(2)
     adapters = _adapters(2, 16, 64, 48, g)

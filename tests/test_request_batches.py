@@ -290,6 +290,20 @@ def test_counts_of_each_slot_and_refusals() -> None:
             CachedDecoder(model, slots=2, max_tokens=64, adapters=sets)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64])
+def test_slots_in_any_whole_type(dtype) -> None:  # noqa: ANN001
+    config = WorkloadConfig(3, 40, 128, 2, 128, 1)
+    model = _model(config)
+    decoder = CachedDecoder(model, slots=3, max_tokens=100, adapters=_adapters(model, 2, 8, ("qkv",)))
+    decoder.prompt(_randn(3, 10, 128))
+    for device in ("cpu", DEV):
+        decoder.set_adapters(torch.tensor([0, 1, 0], dtype=dtype, device=device))
+        assert decoder.adapter_indices.tolist() == [0, 1, 0]
+        decoder.fork(torch.tensor([1, 0, 100], dtype=dtype, device=device))
+        assert decoder.adapter_indices.tolist() == [1, 0, 0] and decoder.cache.lengths.tolist() == [10, 10, 10]
+
+
 def _meta(*shape, dtype=torch.bfloat16):  # noqa: ANN001, ANN002, ANN202
     return torch.empty(*shape, device="meta", dtype=dtype)
 
