@@ -35,8 +35,6 @@ NVCC_FLAGS = (
     "-Xcompiler",
     "-fPIC",
     "-shared",
-    "--split-compile",
-    "0",  # the kernels by as many threads as there are
 )
 
 
