@@ -91,6 +91,7 @@ struct DeviceState {
   bool w4_attr[18] = {};                   // 4-bit linear builds by row tiles, column tiles and group
   bool w4_line_attr[6] = {};               // the same with x in shared memory, by row tiles and group
   bool low_rank_attr[16] = {};             // low-rank adapter builds by rank, rows and base dtype
+  int low_rank_resident[16][2][4] = {};    // of these, by terms and CTAs of a cluster: clusters that run at once, 0: not asked yet
   bool low_rank_tile_attr[4] = {};         // their builds for many rows
   bool fork_attr = false, reserve_attr = false, compact_attr = false;  // pages: shared memory and cluster sizes set
   bool seq_forward_attr = false;           // whole-forward kernel's shared-memory size set

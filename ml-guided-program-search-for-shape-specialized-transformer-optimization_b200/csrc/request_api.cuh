@@ -6,11 +6,27 @@
 namespace {
 
 constexpr int kLrShared = 220 * 1024;  // most that a build asks for
-constexpr int kLrTwo = 110 * 1024;     // with which two CTAs share an SM
 
-// Steps of 32 values of K for a warp, where a group has CTAs enough (64 rows of 32 adapters, 4096 -> 14336: 2 steps and eight CTAs
-// 11.2 us, 4 and four 11.8, 16 and one 13.7).
-constexpr int kLrSteps = 2;
+// Clusters of 1 << shift CTAs that run at once: those of 4 and 8 do not fill each part of the GPU (33 of eight CTAs with two on an
+// SM, 15 with one, where 148 SMs would have room for 37 and 18).
+template <typename Kernel>
+cudaError_t low_rank_resident(Kernel kernel, int bytes, int shift, int* clusters) {
+  if (*clusters > 0) return cudaSuccess;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(1u << shift);
+  config.blockDim = dim3(b200tx::kLrThreads);
+  config.dynamicSmemBytes = bytes;
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = 1u << shift;
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  int found = 0;
+  cudaError_t err = cudaOccupancyMaxActiveClusters(&found, kernel, &config);
+  if (err == cudaSuccess) *clusters = std::max(1, found);
+  return err;
+}
 
 template <int RT, bool F32, bool WHOLE>
 cudaError_t launch_low_rank(b200tx::LowRankArgs& a, DeviceState* dev, int index, cudaStream_t stream) {
@@ -25,22 +41,45 @@ cudaError_t launch_low_rank(b200tx::LowRankArgs& a, DeviceState* dev, int index,
   const int64_t windows = (a.rows + b200tx::kLrWindow - 1) / b200tx::kLrWindow;
   const int64_t rows = std::min<int64_t>(a.rows, b200tx::kLrWindow);
   const int terms = a.out_f32 ? 3 : 2;
-  // CTAs of a cluster: as many as leave each warp a few steps of K, while that leaves every SM two CTAs at most.
-  const int64_t warps = (a.inner + 32 * kLrSteps - 1) / (32 * kLrSteps);
-  int ctas = 8;
-  while (ctas > 1 && (ctas / 2 * b200tx::kLrWarps >= warps || windows * ((rows + S::G - 1) / S::G) * ctas > 2 * dev->sm_count))
-    ctas /= 2;
-  const int bytes = S::bytes(ctas, terms);
-  const int64_t resident = std::max(1, dev->sm_count * (S::TWO && bytes <= kLrTwo ? 2 : 1) / ctas);  // clusters
-  // Rows of a group: fewer, while the groups then all run at once (203 rows of 4744 -> 5003: 8 rows 17.4 us, 32 rows 24.2).
-  a.group = S::G;
-  while (a.group > 8 && windows * ((rows + a.group / 2 - 1) / (a.group / 2)) <= resident) a.group /= 2;
-  const int64_t least = (rows + a.group - 1) / a.group;  // groups of a window, where its rows share an adapter
+  // Groups of a window as far as can be told here: where its rows share an adapter, and half a group more for each
+  // adapter that they may differ in.
+  const int64_t differ = std::min<int64_t>(a.count, (rows + a.per_index - 1) / a.per_index);
+  auto groups_of = [&](int64_t size) { return windows * std::min(rows, (rows + size - 1) / size + differ / 2); };
+  const int64_t tiles = (a.outer + b200tx::kLrTile - 1) / b200tx::kLrTile, steps = (a.inner + 31) / 32;
+  int64_t resident[4];  // clusters of 1, 2, 4 and 8 CTAs that run at once
+  for (int i = 0; i < 4; ++i) {
+    cudaError_t err = low_rank_resident(b200tx::low_rank_kernel<RT, F32, WHOLE>, S::bytes(1 << i, terms), i,
+                                        &dev->low_rank_resident[index][terms - 2][i]);
+    if (err != cudaSuccess) return err;
+    resident[i] = dev->low_rank_resident[index][terms - 2][i];
+  }
+  // Groups of as few rows as let all run at once, in clusters of the size for which a warp has least to do: steps of K, and
+  // rounds of columns, which take eight times as long.  A second wave costs more than all else (256 rows of 8 adapters,
+  // 4096 -> 4096, rank 32: 8 rows by four CTAs 11.6 us, by eight 16.5; rank 128 by two 20.3, by eight 37.0; 203 rows of
+  // 4744 -> 5003: by two CTAs, with one round, 15.1, by eight, with two, 17.5, and 32 rows by eight 27).
+  int shift = -1;
+  int64_t least = 0;
+  for (a.group = 8;; a.group *= 2) {
+    const int64_t groups = groups_of(a.group);
+    for (int i = 0; i < 4; ++i) {
+      if (groups > resident[i] || (i == 0 && steps > 8 * b200tx::kLrWarps)) continue;  // one CTA only where K is short
+      const int64_t units = b200tx::kLrWarps << i;
+      const int64_t split = std::min(resident[i] / groups, (tiles + units - 1) / units);
+      const int64_t cost = 2 * ((steps + units - 1) / units) + 16 * ((tiles + units * split - 1) / (units * split)) + (i > 0) * 2 + (i == 3);
+      if (shift >= 0 && cost >= least) continue;
+      least = cost;
+      shift = i;
+    }
+    if (shift >= 0 || a.group == S::G) break;
+  }
+  // Too many for that: several waves of small clusters (1024 rows of 32 adapters, 4096 -> 4096: rank 32 by one CTA 34.4 us, two
+  // 27.1, four 39; rank 64 37.7, 46.5 and 58).
+  if (shift < 0) shift = S::TWO ? 1 : 0;
+  const int ctas = 1 << shift, bytes = S::bytes(ctas, terms);
   // Groups that can be: one more for each further index that occurs.
-  const int64_t most = std::min<int64_t>(rows, least + a.count + 1);
-  const int64_t tiles = (a.outer + b200tx::kLrTile - 1) / b200tx::kLrTile;
+  const int64_t most = std::min<int64_t>(rows, (rows + a.group - 1) / a.group + a.count + 1);
   a.parts = static_cast<int>((tiles + ctas * b200tx::kLrWarps - 1) / (ctas * b200tx::kLrWarps));
-  a.clusters = static_cast<int>(std::min(std::max(least, resident / windows), most * a.parts));
+  a.clusters = static_cast<int>(std::min(std::max(groups_of(a.group), resident[shift]) / windows, most * a.parts));
   return launch_clustered(b200tx::low_rank_kernel<RT, F32, WHOLE>, dim3(static_cast<unsigned>(windows * a.clusters * ctas)),
                           dim3(b200tx::kLrThreads), static_cast<size_t>(bytes), static_cast<unsigned>(ctas), stream, a);
 }
