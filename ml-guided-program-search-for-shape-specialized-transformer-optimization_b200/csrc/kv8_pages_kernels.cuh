@@ -13,10 +13,10 @@
 // counts are integers, so the order in which CTAs run changes nothing.  One call at a time
 // works on a cache's pages.
 //
-// What bounds them, in a graph: the small calls are chains of trips to memory (fork of 4 of 8 slots 4.7 us; free and reserve
-// for 2 of 32 slots 10.4, two launches).  Fork of 8 prompts to 128 samples (4 layers of 8 heads of 128): 66 MB written in 22.7 us, 2.9
+// What bounds them, in a graph: the small calls are chains of trips to memory (fork of 4 of 8 slots 4.5 us; free and reserve
+// for 2 of 32 slots 9.8, two launches).  Fork of 8 prompts to 128 samples (4 layers of 8 heads of 128): 66 MB written in 22.6 us, 2.9
 // TB/s, the sources out of L2; issue 43 %, barriers between an item's reads and writes.  Free and reserve for 64 of 128 long
-// sequences (62000 entries, 200000 pages): 26 us, 16 SMs in step, barriers.  Compaction that moves 336 MB: 123 us, 5.5 TB/s of the measured 6.55.
+// sequences (62000 entries, 200000 pages): 25 us, 16 SMs in step, barriers.  Compaction that moves 336 MB: 123 us, 5.5 TB/s of the measured 6.55.
 #pragma once
 
 #include "kv8_cache_kernels.cuh"

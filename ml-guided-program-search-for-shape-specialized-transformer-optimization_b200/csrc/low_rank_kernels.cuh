@@ -27,9 +27,9 @@
 //
 // What bounds it: the chain launch -> indices -> ranks -> sums over K -> exchange in the cluster -> columns, each about
 // a microsecond, most of it trips to memory and barriers; and beyond a few groups the instructions of a tile (issue
-// 32 % with two CTAs on an SM).  One row of 1024 -> 4096, rank 16: 5.3 us in a graph (0.6 indices, 0.5 ranks, 1.2 sums, 0.7 exchange,
-// 0.35 terms, 0.8 columns).  64 rows of 32 adapters, 4096 -> 14336: 11 to 12 us for 19.9 MB (3.0 us at the copy rate; cold 16).  203 rows
-// in no order, 4744 -> 5003, rank 24, 32 bits: 18 us for 12.4 MB.
+// 32 % with two CTAs on an SM).  One row of 1024 -> 4096, rank 16: 5.0 us in a graph (0.6 indices, 0.5 ranks, 1.2 sums, 0.7 exchange,
+// 0.35 terms, 0.8 columns).  64 rows of 32 adapters, 4096 -> 14336: 12 us for 19.9 MB (3.0 us at the copy rate; cold 16).  203 rows
+// in no order, 4744 -> 5003, rank 24, 32 bits: 15 us for 12.4 MB.
 //
 // The R sums of a row are fp32.  The second product takes them as bf16 terms, each the rounded rest of the
 // ones before: two (2^-17 of the sum is left) where the result has 16 bits, three (2^-25) where it has 32.
@@ -118,7 +118,7 @@ struct LrGroups {
 };
 
 // A build for RT tiles of 16 ranks: groups of up to NT eights of rows.  With more ranks two eights are enough for the
-// registers (512 rows of 4096 -> 1024, rank 64: two 28.0 us, four 31.8; 16 rows 7.9 and 8.8).
+// registers (rank 64, 4096 -> 1024: 16 rows 7.9 us, with four 8.1; 256 rows 17.2 and 17.9).
 template <int RT>
 struct LrShape {
   static constexpr int NT = RT <= 2 ? 4 : 2;

@@ -130,10 +130,10 @@ int launch_low_rank_tile(b200tx::LowRankArgs& a, DeviceState* dev, int index, cu
 }
 
 // Rows go by 128 on tcgen05 where there are many, in runs of one adapter, and rows of base and the result are multiples of 16
-// bytes.  The warp MMAs' time grows with rows x ranks, the UMMAs' hardly with either, but these begin with a
-// longer chain (1024 rows of 1024 -> 4096: rank 16 12.7 us by warps, 14.8 so; rank 64 19.5 and 15.9; 4096 rows: rank 16 29.4 and 26.7,
-// rank 64 60 and 27.9; 4096 -> 4096 of rank 16 34 and 42, 4096 -> 14336 83 and 76).
-constexpr int64_t kLtLeastRows = 1024, kLtLeastRun = 64, kLtLeastWork = 65536;
+// bytes.  The warp MMAs' time grows with rows x ranks, the UMMAs' with K: a group's sums are one CTA's (1024 -> 4096: 1024 rows of rank
+// 16 13.1 us by warps, 14.2 so; rank 32 16.1 and 14.7, rank 64 20.3 and 15.0; 4096 rows of rank 64 57 and 27.  4096 -> 4096:
+// 1024 rows of rank 64 23.6 and 31.0, 2048 38.5 and 34.1, 4096 76 and 41.5; 4096 rows of rank 16 33.9 and 41, 8192 66.6 and 52.8).
+constexpr int64_t kLtLeastRows = 1024, kLtLeastRun = 64, kLtLeastRanks = 32, kLtLeastInner = 1024;
 
 int kv8_pool(const char* what, const b200tx_kv8_pool* c, b200tx::Kv8Pool* out) {
   if (c == nullptr) return fail(B200TX_ERR_INVALID_ARGUMENT, "%s: null pool", what);
@@ -178,8 +178,8 @@ int low_log2(int64_t v) {
 constexpr int kPoolShared = 96 * 1024;  // of 2048 rows' records and places
 
 // CTAs for an order over so many pages and entries: one, without exchanges, while its threads take few of them
-// each (free and reserve with 1320 pages: one 10.9 us, a cluster 13.2; 10320: 15.8 and 17.3; 20640: 20.2 and 18.8; 82080: 53
-// and 22; compaction of 3572 pages 12.6 and 15.5, of 14286 27.7 and 23.9).
+// each (free and reserve with 1320 pages: one 10.3 us, a cluster 12.4; 10320: 14.9 and 16.4; 20640: 19.3 and 17.9; 82080: 51
+// and 21; compaction of 3572 pages 11.6 and 14.7, of 14286 23.5 and 19.8).
 constexpr int64_t kPoolFew = 12288;
 unsigned pool_cluster(int64_t pages, int64_t entries) { return std::max(pages, entries) <= kPoolFew ? 1 : b200tx::kPoolCtas; }
 
@@ -246,7 +246,7 @@ int b200tx_low_rank_add(const void* x, const void* base, int base_dtype, void* o
   a.gelu = epilogue == B200TX_EPI_BIAS_GELU;
   a.skip_bare = base == out && !a.gelu;
   const bool f32 = base_dtype == B200TX_F32;
-  if (M >= kLtLeastRows && M * rank >= kLtLeastWork && a.per_index >= kLtLeastRun && N % 8 == 0 && adapters * N < (int64_t{1} << 34)) {
+  if (M >= kLtLeastRows && M * rank >= kLtLeastRanks * std::max(K, kLtLeastInner) && a.per_index >= kLtLeastRun && N % 8 == 0 && adapters * N < (int64_t{1} << 34)) {
     return rank <= 64 ? f32 ? launch_low_rank_tile<1, true>(a, dev, 0, stream) : launch_low_rank_tile<1, false>(a, dev, 1, stream)
            : f32      ? launch_low_rank_tile<2, true>(a, dev, 2, stream)
                       : launch_low_rank_tile<2, false>(a, dev, 3, stream);

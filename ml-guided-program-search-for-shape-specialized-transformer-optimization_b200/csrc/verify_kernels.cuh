@@ -12,8 +12,8 @@
 // their probabilities.  A cluster takes a sequence: its CTAs sum stretches of the row,
 // exchange the sums, and the one CTA where the sum is passed looks through one warp's stretch again.
 //
-// What bounds it: 64 sequences x 128000, both rows fp32: 16.8 us for 52 MB (8.0 at the copy rate): 1.2 to 2.5 until the row is known, the
-// rows at the copy rate, then exchange, choice and the second look 2 to 4 more.  One sequence x 32000: 5.3 us, five trips to memory.
+// What bounds it: 64 sequences x 128000, both rows fp32: 15.5 us for 52 MB (8.0 at the copy rate): 1.2 to 2.5 until the row is known, the
+// rows at the copy rate, then exchange, choice and the second look 2 to 4 more.  One sequence x 32000: 5.1 us, five trips to memory.
 #pragma once
 
 #include "sm100_common.cuh"
