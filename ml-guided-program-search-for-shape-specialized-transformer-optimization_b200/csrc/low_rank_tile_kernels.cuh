@@ -19,7 +19,7 @@
 //
 // What bounds it: 8 x 2048 rows of 1024 -> 4096, rank 64, GELU: 79.5 us, 3.85 TB/s of the measured 6.55 (46.7 us; the warp MMAs
 // take 300).  Of these 3 are launch and ranks, 8.7 the sums (0.33 us a stage: the issuing thread), 1 the terms, and 32 rounds of 2.0 us: 21
-// instructions a value, 12 of them GELU, issued in 61 % of cycles on 128 of 148 SMs (a group to an SM; cutting a
+// instructions a value, 12 of them GELU, issued in 65 % of cycles on 128 of 148 SMs (a group to an SM; cutting a
 // group's columns would take its sums twice).
 //
 // One thread brings the stages and up's columns, one of another warp issues the UMMAs (in one thread the two take 0.57 us
