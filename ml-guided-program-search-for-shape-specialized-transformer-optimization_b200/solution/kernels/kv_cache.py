@@ -101,6 +101,8 @@ class Kv8Cache(TensorHandle):
         # they are first asked for; None: the stream has been captured on only.
         self._workspaces: dict[int, torch.Tensor | None] = {}
         self._captured: dict[int, tuple[int, torch.Tensor]] = {}  # stream: capture, workspace; of the last capture
+        # Counts and scratch of the pool that the pages are (Kv8Pages); None: nothing but the table says whose they are.
+        self._pool: tuple[torch.Tensor, torch.Tensor] | None = None
 
     @classmethod
     def create(

@@ -43,11 +43,17 @@ class Kv8Pages(TensorHandle):
     ``refs`` int32 ``[pages]`` counts the entries of the cache's ``page_table`` that hold a page; a
     page with none is free.  Counted from the table where it is not given; who
     changes the table by other means calls ``recount``.
+
+    A cache has one pool: a further handle of it shares the counts.  One that is made with other
+    ``refs`` takes their place, and calls on the handles before it are refused.
     """
 
     def __init__(self, cache: Kv8Cache, refs: torch.Tensor | None = None) -> None:
         counted = refs is None
-        if counted:
+        scratch = None
+        if cache._pool is not None and (counted or refs is cache._pool[0]):
+            refs, scratch = cache._pool
+        elif counted:
             refs = torch.zeros(cache.pages, dtype=torch.int32, device=cache.device)
         require(
             refs.dtype == torch.int32 and tuple(refs.shape) == (cache.pages,) and refs.is_contiguous()
@@ -56,21 +62,34 @@ class Kv8Pages(TensorHandle):
         )
         self.cache = cache
         self.refs = refs
-        self._scratch = torch.zeros(_native.kv8_pool_scratch(cache.pages), dtype=torch.int32, device=cache.device)
+        if scratch is None:
+            scratch = torch.zeros(_native.kv8_pool_scratch(cache.pages), dtype=torch.int32, device=cache.device)
+        self._scratch = scratch
         self._struct = _native.Kv8PoolView(
             cache._views[0], cache.layers, refs.data_ptr(), self._scratch.data_ptr()
         )
         # what the binding takes: the struct's address and a tensor on the pool's device
-        self.handle = (ctypes.addressof(self._struct), refs)
+        self._handle = (ctypes.addressof(self._struct), refs)
+        cache._pool = (refs, scratch)
         if counted:
             self.recount()
+
+    @property
+    def handle(self) -> tuple[int, torch.Tensor]:
+        """For the binding; RuntimeError where the cache's pages go by other counts since this was made."""
+
+        if self.cache._pool[0] is not self.refs:
+            raise RuntimeError("the cache's pages go by other counts: a Kv8Pages was made with refs of its own after this one")
+        return self._handle
 
     def recount(self) -> None:
         """Count the table's entries anew."""
 
-        flat = self.cache.page_table.reshape(-1).long()
-        held = (flat >= 0) & (flat < self.cache.pages)
-        self.refs.zero_().index_add_(0, torch.where(held, flat, 0), held.to(torch.int32))
+        self.handle  # noqa: B018 - refuses
+        with torch.inference_mode():  # where the counts were made in that mode too
+            flat = self.cache.page_table.reshape(-1).long()
+            held = (flat >= 0) & (flat < self.cache.pages)
+            self.refs.zero_().index_add_(0, torch.where(held, flat, 0), held.to(torch.int32))
 
     @property
     def free(self) -> int:

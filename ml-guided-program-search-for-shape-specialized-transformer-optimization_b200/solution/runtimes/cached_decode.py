@@ -139,7 +139,7 @@ class CachedDecoder:
         self.graph = bool(graph)
         self.adapters = None if adapters is None else [dict(given) for given in adapters]
         self._differ = False  # whether the slots' tokens have been counted apart
-        self._pages: Kv8Pages | None = None  # made by the first fork: slots share pages from then on
+        self._pages: Kv8Pages | None = None  # made by the first fork, or once the cache's pages are a pool by other means
         with torch.inference_mode():
             self.adapter_indices = torch.full((slots,), -1, dtype=torch.int32, device=device)
             model._materialize_shadow_weights()
@@ -269,7 +269,7 @@ class CachedDecoder:
             raise ValueError("x must be a contiguous tensor on the decoder's device")
         if x.dtype not in (torch.float32, torch.bfloat16):
             raise ValueError("x must be float32 or bfloat16")
-        if held and held + x.shape[1] > self.max_tokens and self._differ:
+        if held and held + x.shape[1] > self.max_tokens and (self._differ or self.cache._pool is not None):
             self.held = held = int(self.cache.lengths.max())  # what the slots really hold: read from the device
         if held + x.shape[1] > self.max_tokens:
             raise ValueError(f"{held} tokens held and {x.shape[1]} more pass the cache's {self.max_tokens}")
@@ -365,21 +365,36 @@ class CachedDecoder:
         if self.pending > _REPEATABLE:
             raise ValueError(f"the last step's {self.pending} tokens cannot be taken back: advance({self.pending}) first")
         with torch.inference_mode():
-            if self._pages is None:
-                self._pages = Kv8Pages(self.cache)
+            pages = self.pages
             source = given.long().clamp(-1, self.slots).to(device=self.cache.device, dtype=torch.int32).contiguous()
             each = torch.arange(self.slots, dtype=torch.int32, device=self.cache.device)
-            sm100_kv8_fork(self._pages, source, each)
+            sm100_kv8_fork(pages, source, each)
             inside = (source >= 0) & (source < self.slots)
             of = torch.where(inside, source, each).long()
             self.adapter_indices.copy_(torch.where(source < 0, -1, self.adapter_indices[of]))
         self.pending = 0
         self._differ = True
 
+    @property
+    def pages(self) -> Kv8Pages:
+        """The cache's pages as one pool, to free, fork or compact by hand between steps (any other ``Kv8Pages`` of the
+        cache does as well).  From then on the steps reserve the pages that they fill."""
+
+        held = self.cache._pool
+        if self._pages is None or held is None or self._pages.refs is not held[0]:
+            with torch.inference_mode():
+                self._pages = Kv8Pages(self.cache, None if held is None else held[0])
+        return self._pages
+
     def _reserve(self, tokens: int) -> None:
         # There are as many pages as entries of the table, so that none is ever missing.
-        if self._pages is not None:
-            sm100_kv8_reserve(self._pages, tokens)
+        if self.cache._pool is None:
+            return
+        if self.slots <= KV8_POOL_ROWS:
+            sm100_kv8_reserve(self.pages, tokens)
+            return
+        for some in torch.arange(self.slots, dtype=torch.int32, device=self.cache.device).split(KV8_POOL_ROWS):
+            sm100_kv8_reserve(self.pages, tokens, slots=some)
 
     def prompt(self, x: torch.Tensor) -> torch.Tensor:
         """The forward of ``x`` ``[slots, T, D]`` from empty sequences, which it leaves
