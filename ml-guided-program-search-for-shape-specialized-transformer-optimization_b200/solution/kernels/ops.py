@@ -57,7 +57,7 @@ from .attention import (
     sm100_simt_attention,
 )
 from .kv_cache import KV8_BLOCK, KV8_HEAD_DIMS, Kv8Cache, sm100_kv8_append, sm100_kv8_attention
-from .kv_pages import Kv8Pages, sm100_kv8_compact, sm100_kv8_fork, sm100_kv8_reserve
+from .kv_pages import Kv8Pages, sm100_kv8_compact, sm100_kv8_fork, sm100_kv8_free, sm100_kv8_reserve
 from .linear_w4 import W4_GROUPS, W4Weight, sm100_linear_w4
 from .low_rank import LOW_RANK_MOST, LowRankAdapters, sm100_low_rank_add
 from .projection import sm100_linear
@@ -757,7 +757,10 @@ def kv8_fork(
 
     _pool_check(codes, scales, tail, page_table, lengths, refs, source, target)
     pages = Kv8Pages(Kv8Cache(codes, scales, tail, page_table, lengths), refs)
-    sm100_kv8_fork(pages, torch.full_like(target, -1) if source is None else source, target)
+    if source is None:
+        sm100_kv8_free(pages, target)
+    else:
+        sm100_kv8_fork(pages, source, target)
 
 
 @kv8_fork.register_fake
