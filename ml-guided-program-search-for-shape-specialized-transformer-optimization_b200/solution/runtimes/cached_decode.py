@@ -334,6 +334,20 @@ class CachedDecoder:
             self.advance(accepted + 1)
         return tokens, accepted
 
+    def _whole(self, given: Sequence[int] | torch.Tensor, what: str) -> torch.Tensor:
+        """A number of each slot, in 64 bits (those that only an unsigned type holds as the largest)."""
+
+        numbers = torch.as_tensor(given)
+        if (
+            tuple(numbers.shape) != (self.slots,) or numbers.is_floating_point() or numbers.is_complex()
+            or numbers.dtype == torch.bool
+        ):
+            raise ValueError(f"{what} must be {self.slots} whole numbers")
+        wide = numbers.long()
+        if numbers.dtype == torch.uint64:
+            wide = torch.where(wide < 0, torch.iinfo(torch.int64).max, wide)
+        return wide
+
     def set_adapters(self, indices: Sequence[int] | torch.Tensor) -> None:
         """The adapter of each slot from now on, -1: none (for graphs that are captured already, too).
         Numbers on the host are checked; one on the device past a projection's set makes its
@@ -341,13 +355,11 @@ class CachedDecoder:
 
         if self.adapters is None:
             raise ValueError("the decoder was made without adapters")
-        given = torch.as_tensor(indices)
-        if tuple(given.shape) != (self.slots,) or given.is_floating_point() or given.dtype == torch.bool:
-            raise ValueError(f"indices must be {self.slots} whole numbers")
+        given = self._whole(indices, "indices")
         sizes = [own.count for layer in self.adapters for own in layer.values()]
         if given.device.type == "cpu" and sizes and int(given.max()) >= min(sizes):
             raise ValueError(f"adapter {int(given.max())} of {min(sizes)}")
-        given = given.long().clamp(-1, 2**31 - 1)
+        given = given.clamp(-1, 2**31 - 1)
         with torch.inference_mode():
             self.adapter_indices.copy_(given)
 
@@ -357,16 +369,14 @@ class CachedDecoder:
         below 0 empties the slot, one past the slots leaves it as it is.  Tokens that are not
         counted yet are forgotten."""
 
-        given = torch.as_tensor(parents)
-        if tuple(given.shape) != (self.slots,) or given.is_floating_point() or given.dtype == torch.bool:
-            raise ValueError(f"parents must be {self.slots} whole numbers")
+        given = self._whole(parents, "parents")
         if self.slots > KV8_POOL_ROWS:
             raise ValueError(f"at most {KV8_POOL_ROWS} slots can be forked")
         if self.pending > _REPEATABLE:
             raise ValueError(f"the last step's {self.pending} tokens cannot be taken back: advance({self.pending}) first")
         with torch.inference_mode():
             pages = self.pages
-            source = given.long().clamp(-1, self.slots).to(device=self.cache.device, dtype=torch.int32).contiguous()
+            source = given.clamp(-1, self.slots).to(device=self.cache.device, dtype=torch.int32).contiguous()
             each = torch.arange(self.slots, dtype=torch.int32, device=self.cache.device)
             sm100_kv8_fork(pages, source, each)
             inside = (source >= 0) & (source < self.slots)
