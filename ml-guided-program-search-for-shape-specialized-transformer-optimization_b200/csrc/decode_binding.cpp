@@ -599,7 +599,7 @@ bool probabilities_fit(const at::Tensor* t, int64_t batch, int64_t tokens) {
 
 bool verify_fits(const at::Tensor* target, const at::Tensor* drafted) {
   return target != nullptr && drafted != nullptr && target->is_cuda() && drafted->device() == target->device() &&
-         drafted->dim() == 2 && drafted->size(0) > 0 && drafted->is_contiguous() &&
+         drafted->dim() == 2 && drafted->size(0) > 0 && drafted->size(1) <= 1024 && drafted->is_contiguous() &&
          (drafted->scalar_type() == at::kInt || drafted->scalar_type() == at::kLong) &&
          probabilities_fit(target, drafted->size(0), drafted->size(1) + 1);
 }

@@ -57,12 +57,19 @@ from .attention import (
     sm100_simt_attention,
 )
 from .kv_cache import KV8_BLOCK, KV8_HEAD_DIMS, Kv8Cache, sm100_kv8_append, sm100_kv8_attention
-from .kv_pages import Kv8Pages, sm100_kv8_compact, sm100_kv8_fork, sm100_kv8_free, sm100_kv8_reserve
+from .kv_pages import (
+    KV8_POOL_ROWS,
+    Kv8Pages,
+    sm100_kv8_compact,
+    sm100_kv8_fork,
+    sm100_kv8_free,
+    sm100_kv8_reserve,
+)
 from .linear_w4 import W4_GROUPS, W4Weight, sm100_linear_w4
 from .low_rank import LOW_RANK_MOST, LowRankAdapters, sm100_low_rank_add
 from .projection import sm100_linear
 from .rotary import ROPE_HEAD_DIMS, RotaryTable, sm100_qk_norm_rope
-from .verify import sm100_verify_draft
+from .verify import VERIFY_MOST, sm100_verify_draft
 
 NAMESPACE = "b200tx"
 OPERATORS = (
@@ -692,6 +699,7 @@ def _low_rank_check(
              f"R must be a multiple of 8 up to {LOW_RANK_MOST}, K a multiple of 8")
     _require(value.shape[:-1] == base.shape[:-1] and value.shape[-1] == down.shape[2] and base.shape[-1] == up.shape[1],
              "value, base and the adapters disagree")
+    _require(value.numel() > 0 and base.numel() > 0, "value and base must not be empty")
     _require(scales.dtype == torch.float32 and tuple(scales.shape) == (down.shape[0],), "scales must be float32 [count]")
     _require(indices.dtype == torch.int32 and indices.numel() > 0
              and (value.numel() // value.shape[-1]) % indices.numel() == 0,
@@ -737,7 +745,8 @@ def _pool_check(
     _cache_check(codes[0], scales[0], tail[0], page_table, lengths)
     _require(refs.dtype == torch.int32 and tuple(refs.shape) == (codes.shape[1],), "refs must be int32 [pages]")
     for slots in lists:
-        _require(slots is None or (slots.dtype == torch.int32 and slots.ndim == 1), "slots and counts must be int32 [n]")
+        _require(slots is None or (slots.dtype == torch.int32 and slots.ndim == 1 and slots.shape[0] <= KV8_POOL_ROWS),
+                 f"slots and counts must be int32 [n], n up to {KV8_POOL_ROWS}")
 
 
 @torch.library.custom_op(
@@ -795,6 +804,9 @@ def kv8_reserve(
 def _kv8_reserve_fake(codes, scales, tail, page_table, lengths, refs, tokens, slots=None, counts=None):  # noqa: ANN001, ANN202, ARG001
     _pool_check(codes, scales, tail, page_table, lengths, refs, slots, counts)
     rows = slots.shape[0] if slots is not None else counts.shape[0] if counts is not None else lengths.shape[0]
+    _require(tokens >= 0 and 0 < rows <= KV8_POOL_ROWS, f"tokens must not be negative, and the sequences 1 to {KV8_POOL_ROWS}")
+    _require(counts is None or counts.shape[0] == rows, "counts must be int32 [B]")
+    _require(slots is not None or rows <= lengths.shape[0], "the batch is larger than the cache's slots")
     return lengths.new_empty((rows,))
 
 
@@ -834,6 +846,8 @@ def _verify_check(
     _require(target.ndim == 3 and target.dtype in _IO and drafted.ndim == 2 and drafted.dtype in (torch.int32, torch.int64)
              and target.shape[:2] == (drafted.shape[0], drafted.shape[1] + 1),
              "target must be a float32 or bfloat16 [B, T + 1, V] tensor, drafted an int32 or int64 [B, T] one")
+    _require(target.numel() > 0 and drafted.shape[1] <= VERIFY_MOST,
+             f"target must not be empty, and the drafted tokens of a sequence at most {VERIFY_MOST}")
     _require(uniform.dtype == torch.float32 and uniform.shape == target.shape[:2], "uniform must be float32 [B, T + 1]")
     _require(draft is None or (draft.dtype == target.dtype and tuple(draft.shape) == (*drafted.shape, target.shape[2])),
              "draft must be a [B, T, V] tensor of the target's dtype")

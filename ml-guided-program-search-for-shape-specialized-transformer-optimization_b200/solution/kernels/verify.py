@@ -14,6 +14,7 @@ import torch
 from ._common import binding, is_sm100_cuda, library_ready
 
 SM100_VERIFY_DRAFT_BACKEND = "sm100_verify_draft"
+VERIFY_MOST = 1024  # drafted tokens of a sequence
 
 
 def can_use_sm100_verify_draft(target: torch.Tensor, drafted: torch.Tensor) -> bool:
@@ -52,6 +53,7 @@ def sm100_verify_draft(
 
 __all__ = [
     "SM100_VERIFY_DRAFT_BACKEND",
+    "VERIFY_MOST",
     "can_use_sm100_verify_draft",
     "sm100_verify_draft",
 ]
