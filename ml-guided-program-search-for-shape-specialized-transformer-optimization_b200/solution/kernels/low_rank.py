@@ -65,18 +65,18 @@ class LowRankAdapters(TensorHandle):
         each rounded to bf16 and filled up with zeros to the largest rank."""
 
         require(len(adapters) > 0, "there must be an adapter at least")
+        require(all(down.ndim == 2 and up.ndim == 2 for down, up, _ in adapters), "an adapter is (down [r, K], up [N, r], scale)")
         first_down, first_up, _ = adapters[0]
-        require(first_down.ndim == 2 and first_up.ndim == 2, "an adapter is (down [r, K], up [N, r], scale)")
         inner, outer = first_down.shape[1], first_up.shape[0]
         rank = 8 * max(1, max(-(-down.shape[0] // 8) for down, _, _ in adapters))
+        require(rank <= LOW_RANK_MOST, f"an adapter's rank is at most {LOW_RANK_MOST}")
         device = first_down.device if device is None else device
         down_all = torch.zeros(len(adapters), rank, inner, dtype=torch.bfloat16, device=device)
         up_all = torch.zeros(len(adapters), outer, rank, dtype=torch.bfloat16, device=device)
         scales = torch.empty(len(adapters), dtype=torch.float32)
         for i, (down, up, scale) in enumerate(adapters):
             require(
-                down.ndim == 2 and up.ndim == 2 and down.shape[1] == inner and up.shape[0] == outer
-                and down.shape[0] == up.shape[1],
+                down.shape[1] == inner and up.shape[0] == outer and down.shape[0] == up.shape[1],
                 "the adapters of a set must fit one projection",
             )
             down_all[i, : down.shape[0]] = down.detach()

@@ -1,11 +1,11 @@
-"""What the operators for many requests cannot run on is refused as such, at trace time too."""
+"""What the operators for many requests cannot run on is refused as such: at trace time too, and by the adapters' stack."""
 
 from __future__ import annotations
 
 import pytest
 import torch
 
-from solution.kernels import Kv8Cache, ops  # noqa: F401 - registers the operators
+from solution.kernels import Kv8Cache, LowRankAdapters, ops  # noqa: F401 - registers the operators
 
 B200 = torch.ops.b200tx
 I32, F32 = torch.int32, torch.float32
@@ -51,6 +51,15 @@ def test_pages_at_trace_time() -> None:
 def test_drafts_at_trace_time(batch, tokens, vocab) -> None:  # noqa: ANN001
     with pytest.raises(ValueError):
         B200.verify_draft(_meta(batch, tokens + 1, vocab), _meta(batch, tokens, dtype=I32), _meta(batch, tokens + 1, dtype=F32))
+
+
+def test_a_stack_of_what_is_no_adapter() -> None:
+    good = (torch.zeros(4, 16), torch.zeros(10, 4), 1.0)
+    for bad in ((torch.tensor(1.0), good[1], 1.0), (good[0], torch.zeros(10), 1.0), (torch.zeros(2, 4, 16), good[1], 1.0),
+                (torch.zeros(200, 16), torch.zeros(10, 4), 1.0)):
+        for order in ([good, bad], [bad, good]):
+            with pytest.raises(ValueError):
+                LowRankAdapters.stack(order)
 
 
 @pytest.mark.gpu
