@@ -22,6 +22,13 @@ many of its drafted tokens as are verified (``accept``):
 
     y = decoder.step(drafts, advance=False)       # [8, 1 + n, D]: the last token and n drafted ones
     tokens, accepted = decoder.accept(probabilities(y), drafted, uniform)
+
+They begin together, with ``prompt``, which takes all slots.  A slot whose request has ended takes another one
+in steps of up to 64 tokens that count for it alone (the other slots' rows are anything, and need room to be appended):
+
+    decoder.fork([0, -1, 2, ...])                 # slot 1 is empty
+    y = decoder.step(x, advance=False)            # [8, 64, D], its tokens in x[1]
+    decoder.advance(counts)                       # int32 [8]: 64 for slot 1, 0 for the others
 """
 
 from __future__ import annotations
