@@ -527,7 +527,8 @@ int b200tx_linear_w4(const void* x, int64_t x_stride, const void* packed, const 
  * out F32 or BF16 [M, N], out other memory than x's and base's, or base itself in one dtype;
  * down BF16 [adapters, rank, K], up BF16 [adapters, N, rank], scales F32 [adapters];
  * rank a multiple of 8 up to 128, K a multiple of 8; index_count divides M; all 16-byte aligned but
- * scales and indices.  fp32 accumulation; epilogue B200TX_EPI_* (no bias: base holds it).
+ * scales and indices.  fp32 accumulation; epilogue B200TX_EPI_* (no bias: base holds it).  The adapters' values
+ * are finite (with an infinite one of up, NaN may stand where the formula has an infinity).
  */
 int b200tx_low_rank_add(const void* x, const void* base, int base_dtype, void* out, int out_dtype, const void* down,
                         const void* up, const float* scales, const int32_t* indices, int64_t index_count, int64_t M,

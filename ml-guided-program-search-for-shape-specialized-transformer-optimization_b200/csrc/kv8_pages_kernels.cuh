@@ -14,9 +14,10 @@
 // works on a cache's pages.
 //
 // What bounds them, in a graph: the small calls are chains of trips to memory (fork of 4 of 8 slots 4.5 us; free and reserve
-// for 2 of 32 slots 9.8, two launches).  Fork of 8 prompts to 128 samples (4 layers of 8 heads of 128): 66 MB written in 22.6 us, 2.9
-// TB/s, the sources out of L2; issue 43 %, barriers between an item's reads and writes.  Free and reserve for 64 of 128 long
-// sequences (62000 entries, 200000 pages): 25 us, 16 SMs in step, barriers.  Compaction that moves 336 MB: 123 us, 5.5 TB/s of the measured 6.55.
+// for 2 of 32 slots 9.8, two launches).  Fork of 8 prompts to 128 samples (4 layers of 8 heads of 128): 66 MB written in
+// 22.6 us, 2.9 TB/s, the sources out of L2 (written once, with 3 MB read, 10.6 us at the copy rate); issue 43 %, barriers
+// between an item's reads and writes.  Free and reserve for 64 of 128 long sequences (62000 entries, 200000 pages): 25 us,
+// 16 SMs in step, barriers.  Compaction that moves 336 MB: 123 us, 5.5 TB/s of the measured 6.55.
 #pragma once
 
 #include "kv8_cache_kernels.cuh"
@@ -35,7 +36,7 @@ struct Kv8Pool {
   int slots, max_blocks, kv_heads, dim, layers;
 };
 
-constexpr int kPoolCounters = 64;  // [0] arrivals of a fork's CTAs, [1] moves, [2] pages in use
+constexpr int kPoolCounters = 64;  // [0] arrivals of a fork's CTAs, [1] moves of a compaction
 constexpr int kPoolRows = 2048;    // sequences of a call
 
 // ------------------------------------------------------------------ which rows count
@@ -264,7 +265,8 @@ template <typename F>
 __device__ __forceinline__ void pool_pages(const Kv8Pool& p, int ctas, F f) {
   const int pages = static_cast<int>(p.pages), warps = ctas * kPoolWarps;
   const int each = ((pages + 127) / 128 + warps - 1) / warps * 128;
-  const int from = static_cast<int>(min(static_cast<int64_t>(pages), static_cast<int64_t>(each) * (cluster_ctarank() * kPoolWarps + threadIdx.x / 32)));
+  const int64_t warp = cluster_ctarank() * kPoolWarps + threadIdx.x / 32;
+  const int from = static_cast<int>(min(static_cast<int64_t>(pages), each * warp));
   const int to = min(pages, from + each);
   constexpr int U = 4;
   for (int at = from; at < to; at += U * 128) {
@@ -511,7 +513,7 @@ struct Kv8CompactArgs {
 };
 
 // With n pages in use: the k-th page in use from n on goes to the k-th free one below n.
-// scratch: the number of moves and of pages in use; where[page], -1 for a free page; the pages that move.
+// scratch: the number of moves; where[page], -1 for a free page; the pages that move.
 __global__ void __launch_bounds__(kPoolThreads, 1) kv8_compact_plan_kernel(const __grid_constant__ Kv8CompactArgs a) {
   __shared__ PoolShared s;
   const Kv8Pool& p = a.pool;
@@ -609,7 +611,8 @@ __global__ void __launch_bounds__(kCompactThreads) kv8_compact_move_kernel(const
       for (int i = tid; i < 2 * p.kv_heads; i += kCompactThreads) p.scales[to * 2 * p.kv_heads + i] = p.scales[of * 2 * p.kv_heads + i];
   }
   const int64_t entries = static_cast<int64_t>(p.slots) * p.max_blocks;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kCompactThreads + tid; i < entries; i += static_cast<int64_t>(gridDim.x) * kCompactThreads) {
+  const int64_t threads = static_cast<int64_t>(gridDim.x) * kCompactThreads;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kCompactThreads + tid; i < entries; i += threads) {
     const int page = p.page_table[i];
     const int now = page >= 0 && page < p.pages ? where[page] : -1;
     if (now != page) p.page_table[i] = now;

@@ -32,7 +32,8 @@
 // in no order, 4744 -> 5003, rank 24, 32 bits: 15 us for 12.4 MB.
 //
 // The R sums of a row are fp32.  The second product takes them as bf16 terms, each the rounded rest of the
-// ones before: two (2^-17 of the sum is left) where the result has 16 bits, three (2^-25) where it has 32.
+// ones before: two (2^-17 of the sum is left) where the result has 16 bits, three (2^-25) where it has 32.  An infinity
+// among up's values meets terms of either sign and zeros, so that NaN may stand where the formula has an infinity.
 #pragma once
 
 #include "attention_mma_kernels.cuh"
@@ -142,10 +143,10 @@ __device__ __noinline__ float lr_gelu_32(float x) { return 0.5f * x * (1.f + erf
 
 // GELU for a result of 16 bits.  With a = |x|, GELU(x) = max(x, 0) - a Q(a), Q the normal distribution's tail,
 // and -log2 Q is smooth: a polynomial of degree 7, fitted on [0, 6] for the least error of a Q(a).  The bound is an absolute
-// one: with the polynomial in fp32 (1.05e-7) and the exponential (4.1e-8) a value is off by less than 1.5e-7.  That is 4e-4 of the
-// value itself down to x = -6, at most a fifth of the rounding of the result; below, where a value is smaller than 6e-9, 1.3 % at -7 and the
-// size only past -10.  13 instructions; one value at a time, as pairs of values in one instruction want their constants in registers,
-// and moves for them.
+// one: with the polynomial in fp32 (1.05e-7) and the exponential (4.1e-8) a value is off by less than 1.5e-7.  That is 4e-4
+// of the value itself down to x = -6, at most a fifth of the rounding of the result; below, where a value is smaller than
+// 6e-9, 1.3 % at -7, and past -10 the size is wrong.  13 instructions; one value at a time, as pairs of values in one
+// instruction want their constants in registers, and moves for them.
 __device__ __forceinline__ float lr_gelu_16(float x) {
   float positive;  // with NaN kept
   asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(positive) : "f"(x));
@@ -349,7 +350,8 @@ __global__ void __launch_bounds__(kLrThreads, LrShape<RT>::TWO ? 2 : 1) low_rank
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int row = s.rows[i * 8 + 2 * t + e];
-        if (row >= 0 && col < a.outer) next_base[e].load(static_cast<const uint8_t*>(a.base) + ((first + row) * a.outer + col) * (F32 ? 4 : 2));
+        if (row >= 0 && col < a.outer)
+          next_base[e].load(static_cast<const uint8_t*>(a.base) + ((first + row) * a.outer + col) * (F32 ? 4 : 2));
       }
     };
     // where rows start anywhere: 64 neighbouring values of each of 8 rows by a warp

@@ -17,10 +17,10 @@
 // an adapter are read (from L2) once for 128 rows.  The warp MMA form of this reads them for every 32 rows
 // and keeps the tensor pipe busy for as long as the bytes take.
 //
-// What bounds it: 8 x 2048 rows of 1024 -> 4096, rank 64, GELU: 79.5 us, 3.85 TB/s of the measured 6.55 (46.7 us; the warp MMAs
-// take 300).  Of these 3 are launch and ranks, 8.7 the sums (0.33 us a stage: the issuing thread), 1 the terms, and 32 rounds of 2.0 us: 21
-// instructions a value, 12 of them GELU, issued in 65 % of cycles on 128 of 148 SMs (a group to an SM; cutting a
-// group's columns would take its sums twice).
+// What bounds it: 8 x 2048 rows of 1024 -> 4096, rank 64, GELU: 79.8 us, 3.85 TB/s of the measured 6.55 (46.7 us; the warp MMAs
+// take 238).  Of these 3 are launch and ranks, 8.7 the sums (0.33 us a stage: the issuing thread), 1 the terms, and 32 rounds
+// of 2.0 us: 22 instructions a value, 13 of them GELU, issued in 65 % of cycles on 128 of 148 SMs (a group to an SM; cutting a
+// group's columns would take its sums twice).  With base in 32 bits, 436 MB: 124 us, 3.5 TB/s.
 //
 // One thread brings the stages and up's columns, one of another warp issues the UMMAs (in one thread the two take 0.57 us
 // for a stage); 16 warps make the terms and bring the results out, each for itself: they all meet at the
@@ -66,7 +66,8 @@ __device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t (&r)[16])
 __device__ __forceinline__ uint32_t lt_place(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
 
 template <int RA, bool F32>
-__global__ void __launch_bounds__(kLtThreads, 1) low_rank_tile_kernel(const __grid_constant__ LowRankArgs a, const __grid_constant__ CUtensorMap x_map,
+__global__ void __launch_bounds__(kLtThreads, 1)
+    low_rank_tile_kernel(const __grid_constant__ LowRankArgs a, const __grid_constant__ CUtensorMap x_map,
                          const __grid_constant__ CUtensorMap down_map, const __grid_constant__ CUtensorMap up_map) {
   using S = LtShape<RA>;
   extern __shared__ uint8_t lt_smem[];

@@ -65,7 +65,8 @@ cudaError_t launch_low_rank(b200tx::LowRankArgs& a, DeviceState* dev, int index,
       if (groups > resident[i] || (i == 0 && steps > 8 * b200tx::kLrWarps)) continue;  // one CTA only where K is short
       const int64_t units = b200tx::kLrWarps << i;
       const int64_t split = std::min(resident[i] / groups, (tiles + units - 1) / units);
-      const int64_t cost = 2 * ((steps + units - 1) / units) + 16 * ((tiles + units * split - 1) / (units * split)) + (i > 0) * 2 + (i == 3);
+      const int64_t cost = 2 * ((steps + units - 1) / units) + 16 * ((tiles + units * split - 1) / (units * split)) +
+                           (i > 0) * 2 + (i == 3);
       if (shift >= 0 && cost >= least) continue;
       least = cost;
       shift = i;
@@ -133,6 +134,8 @@ int launch_low_rank_tile(b200tx::LowRankArgs& a, DeviceState* dev, int index, cu
 // bytes.  The warp MMAs' time grows with rows x ranks, the UMMAs' with K: a group's sums are one CTA's (1024 -> 4096: 1024 rows of rank
 // 16 13.1 us by warps, 14.2 so; rank 32 16.1 and 14.7, rank 64 20.3 and 15.0; 4096 rows of rank 64 57 and 27.  4096 -> 4096:
 // 1024 rows of rank 64 23.6 and 31.0, 2048 38.5 and 34.1, 4096 76 and 41.5; 4096 rows of rank 16 33.9 and 41, 8192 66.6 and 52.8).
+// Runs are told by how many rows an index stands for, which is known here; with an index for each row the warp MMAs take
+// all (8 x 2048 rows of rank 64, 1024 -> 4096, GELU: 238 us in runs and 275 in no order, where 8 indices take 79.8).
 constexpr int64_t kLtLeastRows = 1024, kLtLeastRun = 64, kLtLeastRanks = 32, kLtLeastInner = 1024;
 
 int kv8_pool(const char* what, const b200tx_kv8_pool* c, b200tx::Kv8Pool* out) {
@@ -246,7 +249,8 @@ int b200tx_low_rank_add(const void* x, const void* base, int base_dtype, void* o
   a.gelu = epilogue == B200TX_EPI_BIAS_GELU;
   a.skip_bare = base == out && !a.gelu;
   const bool f32 = base_dtype == B200TX_F32;
-  if (M >= kLtLeastRows && M * rank >= kLtLeastRanks * std::max(K, kLtLeastInner) && a.per_index >= kLtLeastRun && N % 8 == 0 && adapters * N < (int64_t{1} << 34)) {
+  if (M >= kLtLeastRows && M * rank >= kLtLeastRanks * std::max(K, kLtLeastInner) && a.per_index >= kLtLeastRun &&
+      N % 8 == 0 && adapters * N < (int64_t{1} << 34)) {
     return rank <= 64 ? f32 ? launch_low_rank_tile<1, true>(a, dev, 0, stream) : launch_low_rank_tile<1, false>(a, dev, 1, stream)
            : f32      ? launch_low_rank_tile<2, true>(a, dev, 2, stream)
                       : launch_low_rank_tile<2, false>(a, dev, 3, stream);
@@ -387,11 +391,13 @@ int b200tx_verify_draft(const void* target, int64_t target_batch_stride, int64_t
   a.vocab = static_cast<int>(vocab);
   a.wide = drafted_64 != 0;
   const int per = dtype == B200TX_F32 ? 4 : 8;  // values in 16 bytes
-  const bool vec = aligned16(target) && (draft == nullptr || aligned16(draft)) &&
-                   (target_batch_stride | target_token_stride | (draft == nullptr ? 0 : draft_batch_stride | draft_token_stride)) % per == 0;
-  cudaError_t err = dtype == B200TX_F32 ? vec ? launch_verify<float, true>(a, batch, stream) : launch_verify<float, false>(a, batch, stream)
-                    : vec               ? launch_verify<__nv_bfloat16, true>(a, batch, stream)
-                                        : launch_verify<__nv_bfloat16, false>(a, batch, stream);
+  const int64_t strides = target_batch_stride | target_token_stride | (draft == nullptr ? 0 : draft_batch_stride | draft_token_stride);
+  const bool vec = aligned16(target) && (draft == nullptr || aligned16(draft)) && strides % per == 0;
+  cudaError_t err;
+  if (dtype == B200TX_F32)
+    err = vec ? launch_verify<float, true>(a, batch, stream) : launch_verify<float, false>(a, batch, stream);
+  else
+    err = vec ? launch_verify<__nv_bfloat16, true>(a, batch, stream) : launch_verify<__nv_bfloat16, false>(a, batch, stream);
   return err == cudaSuccess ? B200TX_OK : cuda_fail(err, "verify_draft");
 }
 

@@ -32,7 +32,8 @@ class LowRankAdapters(TensorHandle):
     * ``up`` bf16 ``[count, N, R]``
     * ``scales`` float32 ``[count]``
 
-    Their values may be changed in place between calls (an adapter loaded over another).
+    Their values may be changed in place between calls (an adapter loaded over another).  They are
+    finite numbers: with an infinite one of ``up``, NaN may stand where the formula has an infinity.
     """
 
     def __init__(self, down: torch.Tensor, up: torch.Tensor, scales: torch.Tensor) -> None:
@@ -111,11 +112,15 @@ def sm100_low_rank_add(
     """``base + scale * (value . down^T) . up^T`` with each row's adapter: bf16 ``value``
     ``[..., K]``, ``base`` ``[..., N]`` (float32 or bf16) the projection's output, erf GELU
     after the sum with ``gelu``.  fp32 inside, one rounding to ``out_dtype``
-    (default: ``base``'s).
+    (default: ``base``'s).  For a bf16 result the row's R sums keep 2^-17 of themselves, and the GELU is
+    within 1.5e-7 (4e-4 of the value down to -6) before the rounding.
 
     ``indices`` int32 holds one adapter for each of the equal runs of rows that it divides
     them into: ``[B]`` for ``[B, T, K]``, or one for each row.  A negative one: no adapter;
-    one past the set: the row becomes NaN.  ``out`` may be ``base`` itself, in its dtype."""
+    one past the set: the row becomes NaN.  ``out`` may be ``base`` itself, in its dtype.
+
+    Many rows are fastest where an index stands for 64 of them or more and N is a multiple of 8: they
+    go by 128 then (8 prompts of 2048 rows, 1024 -> 4096, rank 64: 80 us with 8 indices, 238 with one for each row)."""
 
     require(out_dtype is None or out_dtype in _OUT, "out_dtype must be float32 or bfloat16")
     result = binding().low_rank_add(

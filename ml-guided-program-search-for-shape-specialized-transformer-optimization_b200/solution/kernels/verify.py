@@ -40,7 +40,7 @@ def sm100_verify_draft(
     Token t counts while ``uniform[t] * draft[t, d] < target[t, d]``; ``draft`` ``[B, T, V]`` are the
     probabilities that the tokens were drawn with (None: 1, as for tokens that were looked up).  The
     token after the last that counts is drawn from ``max(target - draft, 0)`` at the
-    first refusal, else from the target's last row: the first index whose running sum passes
+    first refusal (from the target's row where that leaves nothing), else from the target's last row: the first index whose running sum passes
     ``uniform[T]`` times the whole.  Sequence b has ``counts[b]`` drafted tokens (default T).
 
     Returns ``tokens`` ``[B, T + 1]`` in ``drafted``'s dtype (those that count, the one after
