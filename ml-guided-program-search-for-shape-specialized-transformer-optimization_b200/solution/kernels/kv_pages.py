@@ -50,27 +50,24 @@ class Kv8Pages(TensorHandle):
 
     def __init__(self, cache: Kv8Cache, refs: torch.Tensor | None = None) -> None:
         counted = refs is None
-        scratch = None
-        if cache._pool is not None and (counted or refs is cache._pool[0]):
-            refs, scratch = cache._pool
-        elif counted:
-            refs = torch.zeros(cache.pages, dtype=torch.int32, device=cache.device)
+        if counted:
+            refs = torch.zeros(cache.pages, dtype=torch.int32, device=cache.device) if cache._pool is None else cache._pool[0]
         require(
             refs.dtype == torch.int32 and tuple(refs.shape) == (cache.pages,) and refs.is_contiguous()
             and refs.device == cache.device and refs.data_ptr() % 16 == 0,
             "refs must be a contiguous, 16-byte aligned int32 [pages] tensor on the cache's device",
         )
+        if cache._pool is None or cache._pool[0].data_ptr() != refs.data_ptr():
+            cache._pool = (refs, torch.zeros(_native.kv8_pool_scratch(cache.pages), dtype=torch.int32, device=cache.device))
+        refs, scratch = cache._pool
         self.cache = cache
         self.refs = refs
-        if scratch is None:
-            scratch = torch.zeros(_native.kv8_pool_scratch(cache.pages), dtype=torch.int32, device=cache.device)
         self._scratch = scratch
         self._struct = _native.Kv8PoolView(
             cache._views[0], cache.layers, refs.data_ptr(), self._scratch.data_ptr()
         )
         # what the binding takes: the struct's address and a tensor on the pool's device
         self._handle = (ctypes.addressof(self._struct), refs)
-        cache._pool = (refs, scratch)
         if counted:
             self.recount()
 

@@ -127,3 +127,15 @@ def test_a_pool_of_more_slots_than_a_call_takes() -> None:
         x = _randn(2100, n, 64, seed=seed)
         assert torch.equal(shared.step(x), apart.step(x))
     assert pool.free == 2100 and int(pool.refs.max()) == 1
+
+
+def test_the_same_counts_by_another_name() -> None:
+    cache = _cache()
+    first = Kv8Pages(cache)
+    second = Kv8Pages(cache, first.refs.view(5, 1).view(5))
+    assert second.refs is first.refs
+    first.recount()
+    second.recount()
+    with pytest.raises(ValueError):
+        Kv8Pages(cache, first.refs[:4])
+    first.recount()
